@@ -474,7 +474,7 @@ def run(s):
         return {"q": q, "k": k, "dq": dq, "dk": dk}
     if case["op"] == "append":
         q = ktt.paged_append(s["k"], s["v"], s["k_pages"], s["v_pages"], s["table"], s["lengths"], cos=s["cos"], sin=s["sin"], q=s["q"],
-                             interleaved=case["interleaved"], cu_seq=s["cu"], max_new=s["max_q"], lengths_out=s["next"])
+                             interleaved=case["interleaved"], cu_seq=s["cu"], lengths_out=s["next"])
         if case["bits"] == 16:
             return {"q": q, "lengths": s["next"], "k": s["k_pages"], "v": s["v_pages"]}
         k, v = ktt.paged_read(s["k_pages"], s["v_pages"], s["table"], s["next"])
