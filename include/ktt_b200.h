@@ -328,6 +328,112 @@ KTT_B200_API int ktt_b200_merge_partials(
     void* out, float* lse, const void* out2, const float* lse2,
     int64_t rows, int32_t dv, int32_t out_is_f32, void* stream);
 
+/* ---- rotary positions and a paged cache ------------------------------------------------
+ *
+ * The reference rotates with ktt.rotary (csrc/aten/nn/aten_fused.cpp:30-43: half layout, the whole head) and keeps its
+ * keys and values in a static cache; what follows serves models that turn part of a head or pairs of neighbours, contexts
+ * stretched past what a model was trained on, training through the rotation, and caches in pages. */
+
+/* cos / sin [positions][pairs] fp32, rows dense: scale * cos(p f_i), scale * sin(p f_i) for positions p = 0, 1, ... and the
+ * `pairs` (at most 256) frequencies f_i, which are read from host memory during the call. Angles are taken in 64 bits. */
+KTT_B200_API int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, int32_t pairs, const double* frequencies, double scale, void* stream);
+
+/* Rotation of queries and keys (or of queries alone: kv_heads 0): [B, H, S, D] with (batch, head, row) element strides and
+ * unit head-dim strides (packed [T, H, D]: batch 1). The first 2 * pairs columns turn, the others are copied: pairs
+ * (i, i + pairs), or (2 i, 2 i + 1) where `interleaved`; y1 = x1 c - x2 s, y2 = x2 c + x1 s, products and sums rounded one
+ * by one in fp32, the result once to dtype. inverse: -s for s, which is the gradient's rotation. Row r of entry b has
+ * position positions[b, r], clamped to [0, table_rows), or r where positions is NULL. Inputs and outputs may not overlap. */
+typedef struct ktt_b200_rotary_args {
+    int32_t batch, rows, heads, kv_heads, d;
+    int32_t pairs, interleaved, inverse;
+    int32_t dtype;                 /* KTT_B200_MASK_BF16, _F16 or _F32 */
+    int32_t positions_are_64;      /* int64 positions, else int32 */
+    const void* q;
+    void* q_out;
+    const void* k;
+    void* k_out;
+    int64_t q_strides[3], q_out_strides[3], k_strides[3], k_out_strides[3];
+    const float* cos;
+    const float* sin;
+    int64_t table_stride, table_rows;
+    const void* positions;
+    int64_t position_strides[2];   /* (batch, row) */
+} ktt_b200_rotary_args;
+KTT_B200_API int ktt_b200_rotary(const ktt_b200_rotary_args* args, void* stream);
+
+/* A cache in pages: key j of sequence b is row j % page_size of page block_table[b][j / page_size]. An entry outside
+ * [0, pages) names no page: rows appended there go nowhere, keys read there are not there. page_size is a multiple of 16.
+ * bits 16: bf16 rows of D values, (page, head, row) strides in elements, multiples of 8. bits 4: bytes, of which each 16
+ * tokens of a head are one block of 9 D: 8 D bytes of codes, then D / 64 words of 32 bits per token that hold (step, least
+ * value) of 64 channels as bf16 from the low half up; a code c is worth least + step * c. Eight channels share a 32-bit
+ * word of codes, channel e of them at nibble (e >> 1) + 4 (e & 1). Keys: the word of token r, channels 32 i + 8 t .. is word
+ * r D / 8 + t D / 32 + i. Values: the word of token r = 2 p + o, channels 64 w + 8 g .. is word
+ * ((8 p + place) 2 + o) D / 64 + w with place = g ^ (2 (p & 3)) for D 128 and g ^ (4 ((p >> 1) & 1)) for D 64. Page and head
+ * strides in bytes, multiples of 16; a head's blocks are dense. */
+typedef struct ktt_b200_pages {
+    void* k;
+    void* v;
+    int32_t bits, page_size, kv_heads, table_width;
+    int64_t pages;
+    int64_t k_strides[3], v_strides[3];
+    const int32_t* block_table;    /* int32 [batch][table_width] on the device */
+    int64_t table_stride;
+    const int32_t* lengths;        /* int32 [batch] on the device: keys in the cache, clamped to [0, capacity] */
+    int32_t max_keys;              /* capacity of a sequence where it is less than table_width * page_size; 0: that */
+} ktt_b200_pages;
+
+/* Appends rows lengths[b] .. of sequence b: k rotated (as above, at the position it is cached at; cos NULL: as it is) and
+ * rounded to bf16, v as it is; 4-bit pages hold step = bf16((most - least) / 15), code = (x - least) / step to the nearest
+ * (0 where step is 0) of each 64 channels, a group with a NaN only NaN. Rows past a sequence's capacity go nowhere.
+ * q (optional, heads 0 without) is rotated alongside into q_out. Dense: [B, H, rows, D]; packed (cu_seqlens int32
+ * [batch + 1] on the device): [rows, H, D] with batch strides 0, rows that no sequence covers are neither read nor
+ * written. lengths_out (optional, another buffer than lengths) receives the new lengths. No two sequences may append to one
+ * page in one call. */
+typedef struct ktt_b200_append_args {
+    ktt_b200_pages cache;
+    int32_t batch, rows, heads, d;  /* packed: rows = all rows of q, k and v */
+    int32_t pairs, interleaved;
+    const void* q;
+    void* q_out;
+    const void* k;
+    const void* v;
+    int64_t q_strides[3], q_out_strides[3], k_strides[3], v_strides[3];
+    const float* cos;
+    const float* sin;
+    int64_t table_stride, table_rows;
+    const int32_t* cu_seqlens;
+    int32_t* lengths_out;
+} ktt_b200_append_args;
+KTT_B200_API int ktt_b200_paged_append(const ktt_b200_append_args* args, void* stream);
+
+/* The cache as dense bf16 k_out / v_out [batch, kv heads, rows, D] with (batch, head, row) strides: rows past a sequence's
+ * length, and those that have no page, are zero. */
+typedef struct ktt_b200_read_args {
+    ktt_b200_pages cache;
+    int32_t batch, rows, d;
+    void* k_out;
+    void* v_out;
+    int64_t k_strides[3], v_strides[3];
+} ktt_b200_read_args;
+KTT_B200_API int ktt_b200_paged_read(const ktt_b200_read_args* args, void* stream);
+
+/* Attention over the cache: q dense [B, H, sq, D] or packed [total_q, H, D] (cu_seqlens_q int32 [batch + 1] on the device, sq
+ * = the longest, batch stride 0), D 64 or 128. `lengths` count the keys with those of the call's own tokens. causal (1):
+ * query i of n sees keys j <= length - n + i; a row that sees none gets zeros. Packed rows that no sequence covers are
+ * left as they were. */
+typedef struct ktt_b200_paged_sdpa_args {
+    ktt_b200_pages cache;
+    int32_t batch, heads, sq, d;
+    int64_t total_q;
+    int32_t causal;
+    float scale;
+    const void* q;
+    void* out;
+    int64_t q_strides[3], out_strides[3];
+    const int32_t* cu_seqlens_q;
+} ktt_b200_paged_sdpa_args;
+KTT_B200_API int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,9 @@
     y = ktt.sdpa(q, k, v, key_lengths=lengths)
     y = ktt.sdpa_varlen(q, k, v, cu_seqlens)
     with ktt.sdpa_kernel("flash"): ...
+    cos, sin = ktt.rotary_table(positions, dim); q, k = ktt.rotary(q, k, cos, sin)
+    q = ktt.paged_append(k, v, k_pages, v_pages, table, lengths, cos, sin, q=q, lengths_out=n)
+    y = ktt.sdpa_paged(q, k_pages, v_pages, table, n)
 
 Everything runs on hand-written sm_100a CUDA in lib/libktt_b200.so (C ABI in
 include/ktt_b200.h); there is no CPU or PyTorch-math fallback.
@@ -16,6 +19,8 @@ from ._lib import build_shim as _build_shim
 from .aten import fused_sdp_choice, install, installed, installed_for, uninstall
 from .attention import decode_step, sdpa, sdpa_varlen
 from .numerics import KERNELS, sdpa_kernel
+from .paged import paged_append, paged_cache, paged_read, sdpa_paged
+from .rotary import rotary, rotary_table
 from .stats import diff_stats, format_stats, rel_rms
 from .trace import debug_flash_dump
 
@@ -47,6 +52,12 @@ __all__ = [
     "sdpa",
     "sdpa_kernel",
     "debug_flash_dump",
+    "paged_append",
+    "paged_cache",
+    "paged_read",
+    "rotary",
+    "rotary_table",
+    "sdpa_paged",
     "sdpa_varlen",
     "uninstall",
 ]

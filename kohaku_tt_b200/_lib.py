@@ -60,6 +60,11 @@ EXPORTS = (
     "ktt_b200_decode_static",
     "ktt_b200_decode_append",
     "ktt_b200_merge_partials",
+    "ktt_b200_rotary_table",
+    "ktt_b200_rotary",
+    "ktt_b200_paged_append",
+    "ktt_b200_paged_read",
+    "ktt_b200_paged_sdpa",
 )
 
 _i32, _i64, _f32, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -152,6 +157,120 @@ class DecodeAppendArgs(ctypes.Structure):
         ("rope_row_stride", _i64),
         ("rope_by_position", _i32),
         ("lengths_out", _ptr),
+    ]
+
+
+class RotaryArgs(ctypes.Structure):
+    """struct ktt_b200_rotary_args."""
+
+    _fields_ = [
+        ("batch", _i32),
+        ("rows", _i32),
+        ("heads", _i32),
+        ("kv_heads", _i32),
+        ("d", _i32),
+        ("pairs", _i32),
+        ("interleaved", _i32),
+        ("inverse", _i32),
+        ("dtype", _i32),
+        ("positions_are_64", _i32),
+        ("q", _ptr),
+        ("q_out", _ptr),
+        ("k", _ptr),
+        ("k_out", _ptr),
+        ("q_strides", _i64 * 3),
+        ("q_out_strides", _i64 * 3),
+        ("k_strides", _i64 * 3),
+        ("k_out_strides", _i64 * 3),
+        ("cos", _ptr),
+        ("sin", _ptr),
+        ("table_stride", _i64),
+        ("table_rows", _i64),
+        ("positions", _ptr),
+        ("position_strides", _i64 * 2),
+    ]
+
+
+class Pages(ctypes.Structure):
+    """struct ktt_b200_pages."""
+
+    _fields_ = [
+        ("k", _ptr),
+        ("v", _ptr),
+        ("bits", _i32),
+        ("page_size", _i32),
+        ("kv_heads", _i32),
+        ("table_width", _i32),
+        ("pages", _i64),
+        ("k_strides", _i64 * 3),
+        ("v_strides", _i64 * 3),
+        ("block_table", _ptr),
+        ("table_stride", _i64),
+        ("lengths", _ptr),
+        ("max_keys", _i32),
+    ]
+
+
+class AppendArgs(ctypes.Structure):
+    """struct ktt_b200_append_args."""
+
+    _fields_ = [
+        ("cache", Pages),
+        ("batch", _i32),
+        ("rows", _i32),
+        ("heads", _i32),
+        ("d", _i32),
+        ("pairs", _i32),
+        ("interleaved", _i32),
+        ("q", _ptr),
+        ("q_out", _ptr),
+        ("k", _ptr),
+        ("v", _ptr),
+        ("q_strides", _i64 * 3),
+        ("q_out_strides", _i64 * 3),
+        ("k_strides", _i64 * 3),
+        ("v_strides", _i64 * 3),
+        ("cos", _ptr),
+        ("sin", _ptr),
+        ("table_stride", _i64),
+        ("table_rows", _i64),
+        ("cu_seqlens", _ptr),
+        ("lengths_out", _ptr),
+    ]
+
+
+class ReadArgs(ctypes.Structure):
+    """struct ktt_b200_read_args."""
+
+    _fields_ = [
+        ("cache", Pages),
+        ("batch", _i32),
+        ("rows", _i32),
+        ("d", _i32),
+        ("k_out", _ptr),
+        ("v_out", _ptr),
+        ("k_strides", _i64 * 3),
+        ("v_strides", _i64 * 3),
+    ]
+
+
+class PagedSdpaArgs(ctypes.Structure):
+    """struct ktt_b200_paged_sdpa_args."""
+
+    _fields_ = [
+        ("cache", Pages),
+        ("batch", _i32),
+        ("heads", _i32),
+        ("sq", _i32),
+        ("d", _i32),
+        ("total_q", _i64),
+        ("causal", _i32),
+        ("scale", _f32),
+        ("q", _ptr),
+        ("out", _ptr),
+        ("q_strides", _i64 * 3),
+        ("out_strides", _i64 * 3),
+        ("cu_seqlens_q", _ptr),
     ]
 
 
@@ -306,6 +425,11 @@ def lib():
     handle.ktt_b200_selftest_wait_timeout.argtypes = [_ptr]
     handle.ktt_b200_probe_read.argtypes = [_ptr, ctypes.c_int64, _ptr, _ptr]
     handle.ktt_b200_merge_partials.argtypes = [_ptr, _ptr, _ptr, _ptr, _i64, _i32, _i32, _ptr]
+    handle.ktt_b200_rotary_table.argtypes = [_ptr, _ptr, _i64, _i32, ctypes.POINTER(ctypes.c_double), ctypes.c_double, _ptr]
+    handle.ktt_b200_rotary.argtypes = [ctypes.POINTER(RotaryArgs), _ptr]
+    handle.ktt_b200_paged_append.argtypes = [ctypes.POINTER(AppendArgs), _ptr]
+    handle.ktt_b200_paged_read.argtypes = [ctypes.POINTER(ReadArgs), _ptr]
+    handle.ktt_b200_paged_sdpa.argtypes = [ctypes.POINTER(PagedSdpaArgs), _ptr]
     if handle.ktt_b200_abi_version() != 1:
         raise RuntimeError("kohaku_tt_b200: libktt_b200.so has another ABI version")
     _LIB = handle

@@ -1,0 +1,427 @@
+// The paged cache: appending rows (with the rotation of the keys and of the step's queries) and reading it back.
+#include "paged.cuh"
+
+#include "rotary.cuh"
+
+namespace ktt {
+
+const char* pages_of(Pages& c, const ktt_b200_pages& a, int d) {
+    if (a.bits != 16 && a.bits != 4) return "pages hold 16 or 4 bits per value";
+    if (d != 64 && d != 128) return "head dim 64 or 128";
+    if (a.page_size < 16 || a.page_size % 16) return "the page size must be a multiple of 16";
+    if (a.kv_heads < 1 || a.table_width < 1 || a.pages < 1) return "sizes must be positive";
+    if (a.kv_heads > 4096) return "at most 4096 K / V heads";
+    const int64_t all = static_cast<int64_t>(a.table_width) * a.page_size;
+    if (all > (1 << 30)) return "at most 2^30 keys per sequence";
+    const int size = a.bits == 16 ? 2 : 1;
+    for (int i = 0; i < 3; ++i) {
+        c.ks[i] = a.k_strides[i] * size;
+        c.vs[i] = a.v_strides[i] * size;
+        if (i < 2 || a.bits == 16) {
+            if ((c.ks[i] | c.vs[i]) & 15) return "page strides must be multiples of 16 bytes";
+        }
+    }
+    if ((reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v)) & 15) return "pages must be 16-byte aligned";
+    c.k = static_cast<unsigned char*>(a.k);
+    c.v = static_cast<unsigned char*>(a.v);
+    c.table = a.block_table;
+    c.table_stride = a.table_stride;
+    c.lengths = a.lengths;
+    c.pages = a.pages;
+    c.page_size = a.page_size;
+    c.cap = static_cast<int>(a.max_keys > 0 && a.max_keys < all ? a.max_keys : all);
+    return nullptr;
+}
+
+namespace {
+
+struct AppendParams {
+    Pages c;
+    Turn turn;
+    int batch, rows, heads, kv_heads;
+    int groups;            // blocks of the grid's y that rotate queries; the keys' and the values' follow
+    int64_t tokens;        // rows of all sequences
+    const __nv_bfloat16* q;
+    __nv_bfloat16* q_out;
+    const __nv_bfloat16* k;
+    const __nv_bfloat16* v;
+    int64_t qs[3], qos[3], ks[3], vs[3];
+    const int32_t* cu;
+    int32_t* lengths_out;
+    int vec;
+};
+
+// The sequence of packed row n, or -1: offsets do not decrease, sequences may be empty.
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int64_t n) {
+    if (n < cu[0] || n >= cu[batch]) return -1;
+    int lo = 0, hi = batch - 1;   // the last b with cu[b] <= n
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cu[mid] <= n) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Eight columns of one token in the cache's 4 bits. The 8 threads of a group of 64 columns are neighbours in a warp and
+// all arrive here; `there`: the row has a place. Sums and quotients round as fp32's own do: the codes are the
+// definition's to the bit.
+template <int D, bool kValue>
+__device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, unsigned char* block, int token, int chunk, bool there) {
+    float v[8], least = INFINITY, most = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] = to_f32(x.get(e));
+        nan |= v[e] != v[e];
+        least = fminf(least, v[e]);
+        most = fmaxf(most, v[e]);
+    }
+#pragma unroll
+    for (int off = 1; off < 8; off <<= 1) {
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, off));
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+        nan |= __shfl_xor_sync(0xffffffffu, static_cast<int>(nan), off) != 0;
+    }
+    const __nv_bfloat16 step = __float2bfloat16_rn(nan ? NAN : __fmul_rn(__fsub_rn(most, least), 1.f / 15.f));
+    const float s = __bfloat162float(step);
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float c = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[e], least), s)), 0.f), 15.f) : 0.f;
+        word |= static_cast<uint32_t>(c) << (4 * ((e >> 1) + 4 * (e & 1)));
+    }
+    if (!there) return;
+    uint32_t* to = reinterpret_cast<uint32_t*>(block);
+    to[kValue ? value_word<D>(token, chunk) : key_word<D>(token, chunk)] = word;
+    if (chunk % 8 == 0) {
+        const __nv_bfloat16 low = nan ? __float2bfloat16_rn(NAN) : __float2bfloat16_rn(least);
+        to[step_word<D>(token, chunk / 8)] = static_cast<uint32_t>(__bfloat16_as_ushort(step)) | static_cast<uint32_t>(__bfloat16_as_ushort(low)) << 16;
+    }
+}
+
+// A thread has eight columns of one token and head: of a query, a key or a value. No thread leaves before the
+// group's shuffles.
+template <int D, int kBits, bool kFast>
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int chunk = threadIdx.x, col = chunk * 8, y = blockIdx.y;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (p.lengths_out && blockIdx.x == 0 && y == 0) {
+        for (int b = threadIdx.y * blockDim.x + threadIdx.x; b < p.batch; b += blockDim.x * blockDim.y) {
+            const int64_t more = p.cu ? max(p.cu[b + 1] - p.cu[b], 0) : p.rows, all = cached_keys(p.c, b) + more;
+            p.lengths_out[b] = static_cast<int32_t>(all < p.c.cap ? all : p.c.cap);
+        }
+    }
+    int b = -1;
+    int64_t r = 0, in = 0;   // row of the operands, and of the sequence's new ones
+    if (n < p.tokens) {
+        if (p.cu) {
+            b = sequence_of(p.cu, p.batch, n);
+            r = n;
+            in = b >= 0 ? n - p.cu[b] : 0;
+        } else {
+            b = static_cast<int>(n / p.rows);
+            r = in = n - static_cast<int64_t>(b) * p.rows;
+        }
+    }
+    const bool row = b >= 0;
+    const int64_t pos = row ? cached_keys(p.c, b) + in : 0;
+    const int64_t batch = p.cu || !row ? 0 : b;
+    Eight<__nv_bfloat16> x, other;
+    if (y < p.groups) {
+        if (!row) return;
+        Turned<kFast> turned;
+        turned.load(p.turn, pos, col);
+        const __nv_bfloat16* from = p.q + batch * p.qs[0] + y * p.qs[1] + r * p.qs[2];
+        if (p.vec) x.load(from + col); else x.load_some(from + col, 8);
+        if (kFast && turned.partner >= 0) {
+            if (p.vec) other.load(from + turned.partner); else other.load_some(from + turned.partner, 8);
+        }
+        turned.apply(p.turn, x, other, from, col);
+        __nv_bfloat16* to = p.q_out + batch * p.qos[0] + y * p.qos[1] + r * p.qos[2] + col;
+        if (p.vec) x.store(to); else x.store_some(to, 8);
+        return;
+    }
+    const bool value = y >= p.groups + p.kv_heads;
+    const int head = y - p.groups - (value ? p.kv_heads : 0);
+    int64_t page = -1;
+    if (row && pos < p.c.cap) page = page_of(p.c, b, static_cast<int>(pos));
+    const bool there = page >= 0;
+    if (there) {
+        const __nv_bfloat16* from = value ? p.v + batch * p.vs[0] + head * p.vs[1] + r * p.vs[2] : p.k + batch * p.ks[0] + head * p.ks[1] + r * p.ks[2];
+        if (p.vec) x.load(from + col); else x.load_some(from + col, 8);
+        if (!value) {
+            Turned<kFast> turned;
+            turned.load(p.turn, pos, col);
+            if (kFast && turned.partner >= 0) {
+                if (p.vec) other.load(from + turned.partner); else other.load_some(from + turned.partner, 8);
+            }
+            turned.apply(p.turn, x, other, from, col);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.set(e, __float2bfloat16_rn(0.f));
+    }
+    const int at = static_cast<int>(pos % p.c.page_size);
+    unsigned char* base = there ? (value ? p.c.v + page * p.c.vs[0] + head * p.c.vs[1] : p.c.k + page * p.c.ks[0] + head * p.c.ks[1]) : nullptr;
+    if constexpr (kBits == 16) {
+        if (there) x.store(reinterpret_cast<__nv_bfloat16*>(base + at * (value ? p.c.vs[2] : p.c.ks[2])) + col);
+    } else {
+        unsigned char* block = base + (there ? (at >> 4) * (9 * D) : 0);
+        if (value) put_four_bits<D, true>(x, block, at & 15, chunk, there);
+        else put_four_bits<D, false>(x, block, at & 15, chunk, there);
+    }
+}
+
+struct ReadParams {
+    Pages c;
+    int rows;
+    __nv_bfloat16* k;
+    __nv_bfloat16* v;
+    int64_t ks[3], vs[3];
+};
+
+template <int D, bool kValue>
+__device__ __forceinline__ Eight<__nv_bfloat16> get_four_bits(const unsigned char* block, int token, int chunk) {
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(block);
+    const uint32_t word = from[kValue ? value_word<D>(token, chunk) : key_word<D>(token, chunk)], pair = from[step_word<D>(token, chunk / 8)];
+    Eight<__nv_bfloat16> x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        // (step * code is exact in fp32: one rounding to fp32, one to bf16.)
+        x.set(e, __float2bfloat16_rn(fmaf(step_of(pair), static_cast<float>(nibble_of(word, e)), least_of(pair))));
+    }
+    return x;
+}
+
+// A thread brings eight columns of one key and its value.
+template <int D, int kBits>
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams p) {
+    const int j = blockIdx.x * blockDim.y + threadIdx.y, head = blockIdx.y, b = blockIdx.z;
+    const int chunk = threadIdx.x, col = chunk * 8;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (j >= p.rows) return;
+    Eight<__nv_bfloat16> k, v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        k.set(e, __float2bfloat16_rn(0.f));
+        v.set(e, __float2bfloat16_rn(0.f));
+    }
+    const int64_t page = j < cached_keys(p.c, b) ? page_of(p.c, b, j) : -1;
+    if (page >= 0) {
+        const unsigned char* kp = p.c.k + page * p.c.ks[0] + head * p.c.ks[1];
+        const unsigned char* vp = p.c.v + page * p.c.vs[0] + head * p.c.vs[1];
+        const int at = j % p.c.page_size;
+        if constexpr (kBits == 16) {
+            k.load(reinterpret_cast<const __nv_bfloat16*>(kp + at * p.c.ks[2]) + col);
+            v.load(reinterpret_cast<const __nv_bfloat16*>(vp + at * p.c.vs[2]) + col);
+        } else {
+            k = get_four_bits<D, false>(kp + (at >> 4) * (9 * D), at & 15, chunk);
+            v = get_four_bits<D, true>(vp + (at >> 4) * (9 * D), at & 15, chunk);
+        }
+    }
+    k.store(p.k + b * p.ks[0] + head * p.ks[1] + j * p.ks[2] + col);
+    v.store(p.v + b * p.vs[0] + head * p.vs[1] + j * p.vs[2] + col);
+}
+
+template <typename Params>
+int launch_dependent(void (*kernel)(Params), const Params& p, dim3 grid, dim3 block, cudaStream_t stream, const char* what) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), what);
+}
+
+template <int D, int kBits>
+int launch_append(const AppendParams& p, cudaStream_t stream) {
+    const dim3 block(D / 8, 256 / (D / 8));
+    const int64_t blocks = (p.tokens + block.y - 1) / block.y;   // one at least: it writes the new lengths
+    const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), static_cast<unsigned>(p.groups + 2 * p.kv_heads));
+    if (turn_is_fast(p.turn)) return launch_dependent(append_kernel<D, kBits, true>, p, grid, block, stream, "paged_append launch");
+    return launch_dependent(append_kernel<D, kBits, false>, p, grid, block, stream, "paged_append launch");
+}
+
+template <int D, int kBits>
+int launch_read(const ReadParams& p, int batch, int kv_heads, cudaStream_t stream) {
+    const dim3 block(D / 8, 256 / (D / 8));
+    const dim3 grid(static_cast<unsigned>((p.rows + block.y - 1) / block.y), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
+    return launch_dependent(read_kernel<D, kBits>, p, grid, block, stream, "paged_read launch");
+}
+
+// ---- attention, the plain way: a warp per query row and head, one key after another -----------
+
+struct PlainParams {
+    Pages c;
+    int batch, heads, kv_heads, sq, causal;
+    float scale_log2;
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    int64_t qs[3], os[3];
+    const int32_t* cu;
+    int64_t total_q;
+};
+
+template <int D, int kBits>
+__global__ void __launch_bounds__(128) paged_plain_kernel(const __grid_constant__ PlainParams p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int i = blockIdx.x * 4 + warp, h = blockIdx.y, b = blockIdx.z;
+    const int n = p.cu ? p.cu[b + 1] - p.cu[b] : p.sq;
+    if (i >= n) return;
+    const int64_t row = p.cu ? p.cu[b] + i : i, batch = p.cu ? 0 : b;
+    if (p.cu && (row < 0 || row >= p.total_q)) return;
+    const int len = cached_keys(p.c, b), hk = h / (p.heads / p.kv_heads);
+    const int seen = p.causal ? len - n + i + 1 : len;
+    constexpr int E = D / 32;
+    float q[E], o[E], m = -INFINITY, l = 0.f;
+    const __nv_bfloat16* from = p.q + batch * p.qs[0] + h * p.qs[1] + row * p.qs[2];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        q[e] = to_f32(from[lane * E + e]) * p.scale_log2;
+        o[e] = 0.f;
+    }
+    for (int j = 0; j < seen; ++j) {
+        const int64_t page = page_of(p.c, b, j);
+        if (page < 0) continue;
+        const unsigned char* kp = p.c.k + page * p.c.ks[0] + hk * p.c.ks[1];
+        const unsigned char* vp = p.c.v + page * p.c.vs[0] + hk * p.c.vs[1];
+        const int at = j % p.c.page_size;
+        float k[E], v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int c = lane * E + e;
+            if constexpr (kBits == 16) {
+                k[e] = to_f32(reinterpret_cast<const __nv_bfloat16*>(kp + at * p.c.ks[2])[c]);
+                v[e] = to_f32(reinterpret_cast<const __nv_bfloat16*>(vp + at * p.c.vs[2])[c]);
+            } else {
+                const uint32_t* kw = reinterpret_cast<const uint32_t*>(kp + (at >> 4) * (9 * D));
+                const uint32_t* vw = reinterpret_cast<const uint32_t*>(vp + (at >> 4) * (9 * D));
+                const uint32_t ks = kw[step_word<D>(at & 15, c / 64)], vs = vw[step_word<D>(at & 15, c / 64)];
+                k[e] = fmaf(step_of(ks), static_cast<float>(nibble_of(kw[key_word<D>(at & 15, c / 8)], c & 7)), least_of(ks));
+                v[e] = fmaf(step_of(vs), static_cast<float>(nibble_of(vw[value_word<D>(at & 15, c / 8)], c & 7)), least_of(vs));
+            }
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = fmaf(q[e], k[e], s);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), w = exp2f(s - base);
+        m = top;
+        l = l * f + w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[e], o[e] * f);
+    }
+    __nv_bfloat16* to = p.out + batch * p.os[0] + h * p.os[1] + row * p.os[2];
+#pragma unroll
+    for (int e = 0; e < E; ++e) to[lane * E + e] = __float2bfloat16_rn(l > 0.f || l != l ? o[e] / l : 0.f);
+}
+
+}  // namespace
+}  // namespace ktt
+
+using namespace ktt;
+
+extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream) {
+    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: null arguments");
+    AppendParams p = {};
+    if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: %s", why);
+    if (a->batch < 1 || a->rows < 0 || a->heads < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: sizes must be positive");
+    if (a->heads > 32768) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: at most 32768 heads");
+    if (a->cos && (!a->sin || a->pairs < 1 || 2 * a->pairs > a->d || a->table_rows < 1)) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: 1 to D / 2 pairs of columns turn, by two tables");
+    }
+    if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || (a->heads && a->rows && (!a->q || !a->q_out)) || (a->rows && (!a->k || !a->v))) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: null pointer");
+    }
+    if (a->lengths_out && a->lengths_out == a->cache.lengths) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: lengths_out must not be the lengths themselves");
+    p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, 0};
+    p.batch = a->batch;
+    p.rows = a->rows;
+    p.heads = p.groups = a->heads;
+    p.kv_heads = a->cache.kv_heads;
+    p.tokens = a->cu_seqlens ? a->rows : static_cast<int64_t>(a->batch) * a->rows;
+    if (p.tokens > (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: at most 2^31 rows");
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.q_out = static_cast<__nv_bfloat16*>(a->q_out);
+    p.k = static_cast<const __nv_bfloat16*>(a->k);
+    p.v = static_cast<const __nv_bfloat16*>(a->v);
+    uintptr_t low = reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->v);
+    if (a->heads) low |= reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_out);
+    bool vec = (low & 15) == 0;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a->q_strides[i]; p.qos[i] = a->q_out_strides[i];
+        p.ks[i] = a->k_strides[i]; p.vs[i] = a->v_strides[i];
+        vec = vec && p.ks[i] % 8 == 0 && p.vs[i] % 8 == 0 && (!a->heads || (p.qs[i] % 8 == 0 && p.qos[i] % 8 == 0));
+    }
+    p.vec = vec;
+    p.cu = a->cu_seqlens;
+    p.lengths_out = a->lengths_out;
+    if (p.tokens == 0 && !p.lengths_out) return 0;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->cache.bits == 16) return a->d == 64 ? launch_append<64, 16>(p, st) : launch_append<128, 16>(p, st);
+    return a->d == 64 ? launch_append<64, 4>(p, st) : launch_append<128, 4>(p, st);
+}
+
+extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {
+    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_read: null arguments");
+    ReadParams p = {};
+    if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_read: %s", why);
+    if (a->batch < 1 || a->rows < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_read: sizes must be positive");
+    if (a->batch > 65535) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_read: at most 65535 sequences");
+    if (a->rows == 0) return 0;
+    if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || !a->k_out || !a->v_out) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_read: null pointer");
+    }
+    uintptr_t low = reinterpret_cast<uintptr_t>(a->k_out) | reinterpret_cast<uintptr_t>(a->v_out);
+    p.rows = a->rows;
+    p.k = static_cast<__nv_bfloat16*>(a->k_out);
+    p.v = static_cast<__nv_bfloat16*>(a->v_out);
+    for (int i = 0; i < 3; ++i) {
+        p.ks[i] = a->k_strides[i]; p.vs[i] = a->v_strides[i];
+        low |= static_cast<uintptr_t>((p.ks[i] | p.vs[i]) * 2);
+    }
+    if (low & 15) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_read: outputs must be 16-byte aligned in every row");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int hk = a->cache.kv_heads;
+    if (a->cache.bits == 16) return a->d == 64 ? launch_read<64, 16>(p, a->batch, hk, st) : launch_read<128, 16>(p, a->batch, hk, st);
+    return a->d == 64 ? launch_read<64, 4>(p, a->batch, hk, st) : launch_read<128, 4>(p, a->batch, hk, st);
+}
+
+extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stream) {
+    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null arguments");
+    PlainParams p = {};
+    if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: %s", why);
+    if (a->batch < 1 || a->heads < 1 || a->sq < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: sizes must be positive");
+    if (a->heads % a->cache.kv_heads) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: K / V heads must divide Q heads");
+    if (!(a->scale > 0.f)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: the softmax scale must be positive");
+    if (a->sq == 0) return 0;
+    if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || !a->q || !a->out) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null pointer");
+    }
+    p.batch = a->batch; p.heads = a->heads; p.kv_heads = a->cache.kv_heads; p.sq = a->sq; p.causal = a->causal;
+    p.scale_log2 = a->scale * kLog2e;
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a->q_strides[i];
+        p.os[i] = a->out_strides[i];
+    }
+    p.cu = a->cu_seqlens_q;
+    p.total_q = a->total_q;
+    const dim3 grid((a->sq + 3) / 4, a->heads, a->batch);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto go = [&](auto kernel) {
+        kernel<<<grid, 128, 0, st>>>(p);
+        return check_cuda(cudaGetLastError(), "paged_sdpa launch");
+    };
+    if (a->cache.bits == 16) return a->d == 64 ? go(paged_plain_kernel<64, 16>) : go(paged_plain_kernel<128, 16>);
+    return a->d == 64 ? go(paged_plain_kernel<64, 4>) : go(paged_plain_kernel<128, 4>);
+}

@@ -1,0 +1,180 @@
+// Rotary positions: the tables of cosines and sines, and the rotation of queries and keys (its gradient too).
+#include "rotary.cuh"
+
+namespace ktt {
+namespace {
+
+// ---- tables ----------------------------------------------------------------------------------
+//
+// cos, sin[p][i] = scale * (cos, sin)(p f_i). What a position of 10^5 at f = 1 turns by is no 32-bit matter: the
+// turns p f / 2 pi are taken in 64 bits, their whole part goes, and what is left, at most half a turn, is split
+// into an fp32 value and its fp32 rest; then sin(pi (h + r)) = sin(pi h) + pi r cos(pi h), and the cosine likewise.
+// That is 4 operations in 64 bits per pair, where a 64-bit sine takes some dozens. Bound: the writing of the tables.
+constexpr int kMaxPairs = 256;
+struct TableParams {
+    float* cos;
+    float* sin;
+    int64_t positions;
+    int pairs;
+    float scale;
+    double turns[kMaxPairs];   // f_i / 2 pi
+};
+
+__global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
+    const int64_t n = p.positions * p.pairs, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+    for (int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; at < n; at += step) {
+        const int64_t pos = at / p.pairs;
+        const int i = static_cast<int>(at - pos * p.pairs);
+        double turn = static_cast<double>(pos) * p.turns[i];
+        turn = 2.0 * (turn - rint(turn));
+        const float h = static_cast<float>(turn);
+        const float r = static_cast<float>(turn - static_cast<double>(h)) * 3.14159265358979f;
+        float s, c;
+        sincospif(h, &s, &c);
+        p.cos[at] = p.scale * fmaf(-r, s, c);
+        p.sin[at] = p.scale * fmaf(r, c, s);
+    }
+}
+
+// ---- rotation --------------------------------------------------------------------------------
+
+struct RotaryParams {
+    Turn turn;
+    const void* x[2];        // queries, keys
+    void* y[2];
+    int64_t xs[2][3], ys[2][3];   // (batch, head, row) strides
+    int heads[2], groups[2];      // heads, and how many blocks of kHeads that is
+    int64_t tokens;          // of all batch entries
+    int rows;                // of one
+    int d;
+    const void* positions;   // null: the row
+    int wide_positions;      // int64, else int32
+    int64_t ps[2];           // (batch, row) strides
+    int vec;                 // rows may be read and written in 16-byte pieces
+};
+
+// A thread turns eight columns of kHeads heads of one token: the table is read once for all of them. A thread reads
+// its partner columns too (its neighbour in the block brings the same line, so they come from L1).
+template <typename T, bool kFast, int kHeads>
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int col = threadIdx.x * 8;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (n >= p.tokens) return;
+    const int which = static_cast<int>(blockIdx.y) >= p.groups[0];
+    const int h0 = (static_cast<int>(blockIdx.y) - (which ? p.groups[0] : 0)) * kHeads;
+    const int64_t b = n / p.rows, r = n - b * p.rows;
+    int64_t pos = r;
+    if (p.positions) {
+        const int64_t at = b * p.ps[0] + r * p.ps[1];
+        pos = p.wide_positions ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
+    }
+    Turned<kFast> turned;
+    turned.load(p.turn, pos, col);
+    const T* x = static_cast<const T*>(p.x[which]) + b * p.xs[which][0] + r * p.xs[which][2];
+    T* y = static_cast<T*>(p.y[which]) + b * p.ys[which][0] + r * p.ys[which][2];
+    const int left = p.d - col;
+    Eight<T> v[kHeads], o[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        const T* row = x + static_cast<int64_t>(min(h0 + i, p.heads[which] - 1)) * p.xs[which][1];
+        if (kFast || p.vec) v[i].load(row + col);
+        else v[i].load_some(row + col, left);
+        if (kFast && turned.partner >= 0) o[i].load(row + turned.partner);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        const int h = h0 + i;
+        if (h >= p.heads[which]) break;
+        turned.apply(p.turn, v[i], o[i], x + h * p.xs[which][1], col);
+        T* to = y + h * p.ys[which][1] + col;
+        if (kFast || p.vec) v[i].store(to);
+        else v[i].store_some(to, left);
+    }
+}
+
+template <typename T>
+int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
+    RotaryParams p = given;
+    const int chunks = (p.d + 7) / 8;
+    const int tokens_per_block = 256 / chunks > 0 ? 256 / chunks : 1;
+    const int64_t blocks = (p.tokens + tokens_per_block - 1) / tokens_per_block;
+    const bool fast = p.vec && turn_is_fast(p.turn);
+    auto go = [&](auto kernel, int per) {
+        for (int i = 0; i < 2; ++i) p.groups[i] = (p.heads[i] + per - 1) / per;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.groups[0] + p.groups[1]));
+        cfg.blockDim = dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(tokens_per_block));
+        cfg.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "rotary launch");
+    };
+    if (fast) return go(rotary_kernel<T, true, 1>, 1);
+    return go(rotary_kernel<T, false, 1>, 1);
+}
+
+}  // namespace
+}  // namespace ktt
+
+using namespace ktt;
+
+extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, int32_t pairs, const double* frequencies, double scale, void* stream) {
+    if (!cos || !sin || !frequencies) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: null pointer");
+    if (positions < 1 || pairs < 1 || pairs > kMaxPairs) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: 1 or more positions and 1 to %d pairs", kMaxPairs);
+    if (positions > (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary_table: at most 2^31 positions");
+    TableParams p = {};
+    p.cos = cos;
+    p.sin = sin;
+    p.positions = positions;
+    p.pairs = pairs;
+    p.scale = static_cast<float>(scale);
+    for (int i = 0; i < pairs; ++i) p.turns[i] = frequencies[i] * 0.15915494309189533577;   // 1 / 2 pi
+    const int64_t blocks = (positions * pairs + 255) / 256;
+    rotary_table_kernel<<<static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    return check_cuda(cudaGetLastError(), "rotary_table launch");
+}
+
+extern "C" int ktt_b200_rotary(const ktt_b200_rotary_args* a, void* stream) {
+    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: null arguments");
+    if (a->batch < 0 || a->rows < 0 || a->heads < 1 || a->kv_heads < 0 || a->d < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: sizes must be positive");
+    if (a->d > 1024) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary: head dims above 1024 are not taken");
+    if (a->pairs < 1 || 2 * a->pairs > a->d) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: 1 to D / 2 pairs of columns turn");
+    if (a->dtype < KTT_B200_MASK_BF16 || a->dtype > KTT_B200_MASK_F16) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary: bf16, fp16 or fp32 operands");
+    if (a->heads > 65535 - a->kv_heads) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary: at most 65535 heads");
+    const int64_t tokens = static_cast<int64_t>(a->batch) * a->rows;
+    if (tokens == 0) return 0;
+    if (tokens > (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary: at most 2^31 tokens");
+    if (!a->q || !a->q_out || !a->cos || !a->sin || (a->kv_heads && (!a->k || !a->k_out))) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: null pointer");
+    if (a->table_rows < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: the tables have no rows");
+    RotaryParams p = {};
+    p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, a->inverse};
+    p.x[0] = a->q; p.x[1] = a->k;
+    p.y[0] = a->q_out; p.y[1] = a->k_out;
+    p.heads[0] = a->heads; p.heads[1] = a->kv_heads;
+    const int size = a->dtype == KTT_B200_MASK_F32 ? 4 : 2, wide = 16 / size;
+    uintptr_t low = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->q_out);
+    if (a->kv_heads) low |= reinterpret_cast<uintptr_t>(a->k) | reinterpret_cast<uintptr_t>(a->k_out);
+    bool vec = (low & 15) == 0 && a->d % 8 == 0;
+    for (int i = 0; i < 3; ++i) {
+        p.xs[0][i] = a->q_strides[i]; p.ys[0][i] = a->q_out_strides[i];
+        p.xs[1][i] = a->k_strides[i]; p.ys[1][i] = a->k_out_strides[i];
+        vec = vec && a->q_strides[i] % wide == 0 && a->q_out_strides[i] % wide == 0;
+        if (a->kv_heads) vec = vec && a->k_strides[i] % wide == 0 && a->k_out_strides[i] % wide == 0;
+    }
+    p.tokens = tokens;
+    p.rows = a->rows;
+    p.d = a->d;
+    p.positions = a->positions;
+    p.wide_positions = a->positions_are_64;
+    p.ps[0] = a->position_strides[0]; p.ps[1] = a->position_strides[1];
+    p.vec = vec;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->dtype == KTT_B200_MASK_F32) return launch_rotary<float>(p, st);
+    if (a->dtype == KTT_B200_MASK_F16) return launch_rotary<__half>(p, st);
+    return launch_rotary<__nv_bfloat16>(p, st);
+}
