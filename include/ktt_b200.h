@@ -45,6 +45,8 @@ enum {
     KTT_B200_CAUSAL_NONE = 0,
     KTT_B200_CAUSAL_TOP_LEFT = 1,
     KTT_B200_CAUSAL_BOTTOM_RIGHT = 2,
+    KTT_B200_CAUSAL_KEY_END = 3, /* forward with key_lengths: query i of a sequence's Lq sees keys
+                                    j <= key_lengths[b] - Lq + i */
 };
 
 /* Kernel choice of ktt_b200_attn_args.kernel. */
@@ -100,7 +102,8 @@ typedef struct ktt_b200_attn_args {
     int64_t mask_strides[4];
 
     /* Optional per-batch key counts, int32 [B] on the device, clamped to [1, sk] by
-     * the kernel (ktt_flash/reader.cpp:111-160); never read on the host. */
+     * the kernel (ktt_flash/reader.cpp:111-160); never read on the host. Packed forward: of the
+     * rows that cu_seqlens_k gives a sequence so many are keys; causal is then KEY_END. */
     const int32_t* key_lengths;
 
     /* Packed calls: int32 [batch + 1] on the device; NULL for dense calls. */
@@ -362,8 +365,8 @@ typedef struct ktt_b200_rotary_args {
 KTT_B200_API int ktt_b200_rotary(const ktt_b200_rotary_args* args, void* stream);
 
 /* A cache in pages: key j of sequence b is row j % page_size of page block_table[b][j / page_size]. An entry outside
- * [0, pages) names no page: rows appended there go nowhere, keys read there are not there. page_size is a multiple of 16.
- * bits 16: bf16 rows of D values, (page, head, row) strides in elements, multiples of 8. bits 4: bytes, of which each 16
+ * [0, pages) names no page: rows appended there go nowhere, keys and values read there are zeros. page_size is a multiple of
+ * 16. bits 16: bf16 rows of D values, (page, head, row) strides in elements, multiples of 8. bits 4: bytes, of which each 16
  * tokens of a head are one block of 9 D: 8 D bytes of codes, then D / 64 words of 32 bits per token that hold (step, least
  * value) of 64 channels as bf16 from the low half up; a code c is worth least + step * c. Eight channels share a 32-bit
  * word of codes, channel e of them at nibble (e >> 1) + 4 (e & 1). Keys: the word of token r, channels 32 i + 8 t .. is word
@@ -431,7 +434,14 @@ typedef struct ktt_b200_paged_sdpa_args {
     void* out;
     int64_t q_strides[3], out_strides[3];
     const int32_t* cu_seqlens_q;
+    void* counters;                /* 4096 bytes, 16-byte aligned, zero-filled once before their first use (the kernels
+                                      leave them zero); calls that share them must not overlap on the GPU */
+    void* workspace;               /* ktt_b200_paged_sdpa_workspace() bytes, 16-byte aligned, of any content */
+    int64_t workspace_bytes;
 } ktt_b200_paged_sdpa_args;
+/* Bytes of workspace of a call of these sizes (pointers of q and out included where they are set); -1: refused. Chunks of
+ * prompts take dense rows of some sequences' keys there, 1 GB or one sequence's at most. */
+KTT_B200_API int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args* args);
 KTT_B200_API int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* args, void* stream);
 
 #ifdef __cplusplus

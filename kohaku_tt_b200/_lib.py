@@ -35,7 +35,7 @@ ERR_LAUNCH = -3
 ERR_DEVICE_WAIT = -4
 
 MASK_NONE, MASK_BOOL, MASK_BF16, MASK_F32, MASK_F16 = range(5)
-CAUSAL_NONE, CAUSAL_TOP_LEFT, CAUSAL_BOTTOM_RIGHT = range(3)
+CAUSAL_NONE, CAUSAL_TOP_LEFT, CAUSAL_BOTTOM_RIGHT, CAUSAL_KEY_END = range(4)
 KERNEL_AUTO, KERNEL_MMA, KERNEL_TC5, KERNEL_TC5_WIDE, KERNEL_PAIR = range(5)
 
 EXPORTS = (
@@ -65,6 +65,7 @@ EXPORTS = (
     "ktt_b200_paged_append",
     "ktt_b200_paged_read",
     "ktt_b200_paged_sdpa",
+    "ktt_b200_paged_sdpa_workspace",
 )
 
 _i32, _i64, _f32, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -271,6 +272,9 @@ class PagedSdpaArgs(ctypes.Structure):
         ("q_strides", _i64 * 3),
         ("out_strides", _i64 * 3),
         ("cu_seqlens_q", _ptr),
+        ("counters", _ptr),
+        ("workspace", _ptr),
+        ("workspace_bytes", _i64),
     ]
 
 
@@ -429,6 +433,8 @@ def lib():
     handle.ktt_b200_rotary.argtypes = [ctypes.POINTER(RotaryArgs), _ptr]
     handle.ktt_b200_paged_append.argtypes = [ctypes.POINTER(AppendArgs), _ptr]
     handle.ktt_b200_paged_read.argtypes = [ctypes.POINTER(ReadArgs), _ptr]
+    handle.ktt_b200_paged_sdpa_workspace.argtypes = [ctypes.POINTER(PagedSdpaArgs)]
+    handle.ktt_b200_paged_sdpa_workspace.restype = _i64
     handle.ktt_b200_paged_sdpa.argtypes = [ctypes.POINTER(PagedSdpaArgs), _ptr]
     if handle.ktt_b200_abi_version() != 1:
         raise RuntimeError("kohaku_tt_b200: libktt_b200.so has another ABI version")

@@ -60,19 +60,22 @@ const char* forward_refusal(const ktt_b200_attn_args* a) {
     if (a->heads % a->kv_heads) return "q, k and v shapes do not match (K / V heads must divide Q heads)";
     if (a->d > 256 || a->dv > 256) return "head dims above 256 are not taken";
     if (a->batch > 65535 || a->heads > 65535) return "batch and heads must not exceed 65535";
-    if (a->causal < 0 || a->causal > 2) return "unknown causal mode";
+    if (a->causal < 0 || a->causal > KTT_B200_CAUSAL_KEY_END) return "unknown causal mode";
+    if (a->causal == KTT_B200_CAUSAL_KEY_END && !a->key_lengths) return "a diagonal at the key lengths' end needs key lengths";
     if (a->causal && a->mask_dtype != KTT_B200_MASK_NONE && !a->cu_seqlens_q) return "causal takes no mask";
     if (a->mask_dtype < 0 || a->mask_dtype > KTT_B200_MASK_F16) return "unknown mask dtype";
     if ((a->mask_dtype != KTT_B200_MASK_NONE) != (a->mask != nullptr)) return "mask pointer and mask dtype disagree";
     if ((a->cu_seqlens_q == nullptr) != (a->cu_seqlens_k == nullptr)) return "packed calls need both offset arrays";
     if (a->cu_seqlens_q && a->causal == KTT_B200_CAUSAL_TOP_LEFT) return "packed causal attention is bottom-right aligned";
-    if (a->cu_seqlens_q && a->key_lengths) return "packed calls take no key lengths";
+    if (a->cu_seqlens_q && a->key_lengths && a->causal == KTT_B200_CAUSAL_BOTTOM_RIGHT) return "packed calls with key lengths have their diagonal at the lengths' end";
     if (!(a->scale == a->scale) || a->scale <= 0.f) return "the softmax scale must be positive";
     return nullptr;
 }
 
 const char* backward_refusal(const ktt_b200_attn_args* a) {
     if (const char* why = forward_refusal(a)) return why;
+    if (a->causal == KTT_B200_CAUSAL_KEY_END) return "a diagonal at the key lengths' end is a matter of the forward";
+    if (a->cu_seqlens_q && a->key_lengths) return "the backward of packed calls takes no key lengths";
     return nullptr;
 }
 

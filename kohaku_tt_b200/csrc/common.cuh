@@ -80,7 +80,7 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int b) {
         l = l < 1 ? 1 : l;
         s.klen = l > s.lk ? s.lk : l;
     }
-    s.shift = p.causal == KTT_B200_CAUSAL_BOTTOM_RIGHT ? s.lk - s.lq : 0;
+    s.shift = p.causal == KTT_B200_CAUSAL_BOTTOM_RIGHT ? s.lk - s.lq : p.causal == KTT_B200_CAUSAL_KEY_END ? s.klen - s.lq : 0;
     return s;
 }
 

@@ -37,6 +37,7 @@
 
 #include "common.cuh"
 #include "kept.h"
+#include "split.cuh"
 
 namespace ktt {
 
@@ -121,126 +122,11 @@ __device__ __forceinline__ uint32_t rope_pair(const __nv_bfloat16* x, const __nv
                      __fadd_rn(__fmul_rn(a.y, co.y), __fmul_rn(r1, si.y)));
 }
 
-// prefix[b] = sum_{b' < b} (ceil(len_b' / 64) + kPairCost) for b in [0, batch], by one CTA of
-// 128 threads: the units of one kv head's pass over batch entries [0, b).
-template <bool kAppend>
-__device__ __forceinline__ void scan_lengths(const DecodeParams& p, int* prefix, int* lens, int* warp_sums) {
-    constexpr int kPer = kMaxBatch / kThreads;  // consecutive entries per thread
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int tiles[kPer], mine = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int b = threadIdx.x * kPer + i;
-        const int len = b < p.batch ? clamp_len<kAppend>(p, b) : 0;
-        if (b < p.batch) lens[b] = len;
-        tiles[i] = b < p.batch ? (len + kTile - 1) / kTile + kPairCost : 0;
-        mine += tiles[i];
-    }
-    int x = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += y;
-    }
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    int before = x - mine;
-    for (int w = 0; w < warp; ++w) before += warp_sums[w];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int b = threadIdx.x * kPer + i;
-        if (b <= p.batch) prefix[b] = before;
-        before += tiles[i];
-    }
-    if (threadIdx.x == kThreads - 1 && p.batch == kMaxBatch) prefix[kMaxBatch] = before;
-    __syncthreads();
-}
-
-// Position inside the end-to-end sequence of (batch, kv head) pairs.
-struct Cursor {
-    int b, hk, tile, ntiles, len;
-};
-
-// Largest b with kv_heads * prefix[b] <= unit.
-__device__ __forceinline__ int entry_of(const DecodeParams& p, const int* prefix, int unit) {
-    int lo = 0, hi = p.batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.kv_heads * prefix[mid] <= unit) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-}
-
-// Tiles whose unit lies before `unit` (a pair's units: its tiles, then kPairCost units that
-// belong to its last tile).
-__device__ __forceinline__ int tiles_before(const DecodeParams& p, const int* prefix, int unit) {
-    const int b = entry_of(p, prefix, unit);
-    const int span = prefix[b + 1] - prefix[b], ntiles = span - kPairCost;
-    const int rem = unit - p.kv_heads * prefix[b];
-    const int hk = rem / span, pos = rem % span;
-    return p.kv_heads * (prefix[b] - kPairCost * b) + hk * ntiles + min(pos, ntiles);
-}
-
-// The first tile at or after `unit`.
-__device__ __forceinline__ void cursor_seek(const DecodeParams& p, const int* prefix, const int* lens, Cursor& c, int unit) {
-    const int b = entry_of(p, prefix, unit);
-    const int span = prefix[b + 1] - prefix[b];
-    c.b = b;
-    c.ntiles = span - kPairCost;
-    c.len = lens[b];
-    const int rem = unit - p.kv_heads * prefix[b];
-    c.hk = rem / span;
-    c.tile = rem % span;
-    if (c.tile >= c.ntiles) {   // inside a pair's closing units: the next pair's first tile
-        c.tile = 0;
-        if (++c.hk == p.kv_heads) {
-            c.hk = 0;
-            if (++c.b < p.batch) {
-                c.len = lens[c.b];
-                c.ntiles = prefix[c.b + 1] - prefix[c.b] - kPairCost;
-            }
-        }
-    }
-}
-
-__device__ __forceinline__ void cursor_next(const DecodeParams& p, const int* prefix, const int* lens, Cursor& c) {
-    if (++c.tile < c.ntiles) return;
-    c.tile = 0;
-    if (++c.hk < p.kv_heads) return;
-    c.hk = 0;
-    if (++c.b < p.batch) {
-        c.len = lens[c.b];
-        c.ntiles = prefix[c.b + 1] - prefix[c.b] - kPairCost;
-    }
-}
-
 // Byte offset of element (row, col) in a [rows][D] bf16 tile whose 16-byte chunks are
 // XOR-swizzled by the row, which keeps fragment loads and ldmatrix conflict-free.
 template <int D>
 __device__ __forceinline__ int swz(int row, int col) {
     return (row * D + ((((col >> 3) ^ (row & 7))) << 3) + (col & 7)) * 2;
-}
-
-// The CTAs of a cluster meet; what each wrote to its shared memory before is visible to the others after.
-__device__ __forceinline__ void cluster_meet() {
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// The address of `addr` (shared memory of this CTA) in CTA `rank` of the cluster, and loads from there.
-__device__ __forceinline__ uint32_t in_rank(uint32_t addr, int rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
 }
 
 // kCluster: a cluster of p.ranks CTAs per (batch, kv head) pair (decode_ranks), rank r of which takes tiles r,
@@ -305,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const DecodeParams 
         if (kAppend && p.lengths_out && rank == 0 && cons.hk == 0 && threadIdx.x == 0) p.lengths_out[cons.b] = cons.len;
         stamp(2);
     } else {
-        scan_lengths<kAppend>(p, prefix_s, lens_s, misc);
+        scan_lengths<kThreads, kMaxBatch, kTile, kPairCost>(p.batch, [&](int b) { return clamp_len<kAppend>(p, b); }, prefix_s, lens_s, misc);
         stamp(2);
         if (kAppend && blockIdx.x == 0 && p.lengths_out) {
             for (int b = threadIdx.x; b < p.batch; b += kThreads) p.lengths_out[b] = lens_s[b];
@@ -314,14 +200,14 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const DecodeParams 
         const int total = p.kv_heads * prefix_s[p.batch];
         upc = max(static_cast<int>((total + gridDim.x - 1) / gridDim.x), kMinUnits);
         const int first_unit = min(static_cast<int>(blockIdx.x) * upc, total), end_unit = min(first_unit + upc, total);
-        u1 = tiles_before(p, prefix_s, end_unit) - tiles_before(p, prefix_s, first_unit);
+        u1 = tiles_before<kPairCost>(p, prefix_s, end_unit) - tiles_before<kPairCost>(p, prefix_s, first_unit);
         if (u1 <= 0) return;
-        cursor_seek(p, prefix_s, lens_s, cons, first_unit);
+        cursor_seek<kPairCost>(p, prefix_s, lens_s, cons, first_unit);
     }
     prod = cons;
     auto next = [&](Cursor& c) {
         if constexpr (kCluster) c.tile += p.ranks;
-        else cursor_next(p, prefix_s, lens_s, c);
+        else cursor_next<kPairCost>(p, prefix_s, lens_s, c);
     };
 
     // One normalised output row chunk (4 columns) of (batch b, kv head hk, tile row r).

@@ -177,6 +177,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 struct ReadParams {
     Pages c;
     int rows;
+    int32_t* cu_k;   // optional: gets 0, rows, 2 rows, ...
     __nv_bfloat16* k;
     __nv_bfloat16* v;
     int64_t ks[3], vs[3];
@@ -202,6 +203,11 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
     const int chunk = threadIdx.x, col = chunk * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int len = cached_keys(p.c, b);
+    if (p.cu_k && blockIdx.x == 0 && head == 0 && threadIdx.x == 0 && threadIdx.y == 0) {
+        p.cu_k[b] = b * p.rows;
+        if (b == static_cast<int>(gridDim.z) - 1) p.cu_k[b + 1] = (b + 1) * p.rows;
+    }
     if (j >= p.rows) return;
     Eight<__nv_bfloat16> k, v;
 #pragma unroll
@@ -209,7 +215,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
         k.set(e, __float2bfloat16_rn(0.f));
         v.set(e, __float2bfloat16_rn(0.f));
     }
-    const int64_t page = j < cached_keys(p.c, b) ? page_of(p.c, b, j) : -1;
+    const int64_t page = j < len ? page_of(p.c, b, j) : -1;
     if (page >= 0) {
         const unsigned char* kp = p.c.k + page * p.c.ks[0] + head * p.c.ks[1];
         const unsigned char* vp = p.c.v + page * p.c.vs[0] + head * p.c.vs[1];
@@ -256,75 +262,24 @@ int launch_read(const ReadParams& p, int batch, int kv_heads, cudaStream_t strea
     return launch_dependent(read_kernel<D, kBits>, p, grid, block, stream, "paged_read launch");
 }
 
-// ---- attention, the plain way: a warp per query row and head, one key after another -----------
-
-struct PlainParams {
-    Pages c;
-    int batch, heads, kv_heads, sq, causal;
-    float scale_log2;
-    const __nv_bfloat16* q;
-    __nv_bfloat16* out;
-    int64_t qs[3], os[3];
-    const int32_t* cu;
-    int64_t total_q;
-};
-
-template <int D, int kBits>
-__global__ void __launch_bounds__(128) paged_plain_kernel(const __grid_constant__ PlainParams p) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int i = blockIdx.x * 4 + warp, h = blockIdx.y, b = blockIdx.z;
-    const int n = p.cu ? p.cu[b + 1] - p.cu[b] : p.sq;
-    if (i >= n) return;
-    const int64_t row = p.cu ? p.cu[b] + i : i, batch = p.cu ? 0 : b;
-    if (p.cu && (row < 0 || row >= p.total_q)) return;
-    const int len = cached_keys(p.c, b), hk = h / (p.heads / p.kv_heads);
-    const int seen = p.causal ? len - n + i + 1 : len;
-    constexpr int E = D / 32;
-    float q[E], o[E], m = -INFINITY, l = 0.f;
-    const __nv_bfloat16* from = p.q + batch * p.qs[0] + h * p.qs[1] + row * p.qs[2];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = to_f32(from[lane * E + e]) * p.scale_log2;
-        o[e] = 0.f;
-    }
-    for (int j = 0; j < seen; ++j) {
-        const int64_t page = page_of(p.c, b, j);
-        if (page < 0) continue;
-        const unsigned char* kp = p.c.k + page * p.c.ks[0] + hk * p.c.ks[1];
-        const unsigned char* vp = p.c.v + page * p.c.vs[0] + hk * p.c.vs[1];
-        const int at = j % p.c.page_size;
-        float k[E], v[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int c = lane * E + e;
-            if constexpr (kBits == 16) {
-                k[e] = to_f32(reinterpret_cast<const __nv_bfloat16*>(kp + at * p.c.ks[2])[c]);
-                v[e] = to_f32(reinterpret_cast<const __nv_bfloat16*>(vp + at * p.c.vs[2])[c]);
-            } else {
-                const uint32_t* kw = reinterpret_cast<const uint32_t*>(kp + (at >> 4) * (9 * D));
-                const uint32_t* vw = reinterpret_cast<const uint32_t*>(vp + (at >> 4) * (9 * D));
-                const uint32_t ks = kw[step_word<D>(at & 15, c / 64)], vs = vw[step_word<D>(at & 15, c / 64)];
-                k[e] = fmaf(step_of(ks), static_cast<float>(nibble_of(kw[key_word<D>(at & 15, c / 8)], c & 7)), least_of(ks));
-                v[e] = fmaf(step_of(vs), static_cast<float>(nibble_of(vw[value_word<D>(at & 15, c / 8)], c & 7)), least_of(vs));
-            }
-        }
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s = fmaf(q[e], k[e], s);
-#pragma unroll
-        for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-        const float top = fmaxf(m, s), base = top == -INFINITY ? 0.f : top, f = exp2f(m - base), w = exp2f(s - base);
-        m = top;
-        l = l * f + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = fmaf(w, v[e], o[e] * f);
-    }
-    __nv_bfloat16* to = p.out + batch * p.os[0] + h * p.os[1] + row * p.os[2];
-#pragma unroll
-    for (int e = 0; e < E; ++e) to[lane * E + e] = __float2bfloat16_rn(l > 0.f || l != l ? o[e] / l : 0.f);
+int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, cudaStream_t stream) {
+    if (bits == 16) return d == 64 ? launch_read<64, 16>(p, batch, kv_heads, stream) : launch_read<128, 16>(p, batch, kv_heads, stream);
+    return d == 64 ? launch_read<64, 4>(p, batch, kv_heads, stream) : launch_read<128, 4>(p, batch, kv_heads, stream);
 }
 
 }  // namespace
+
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* cu_k, cudaStream_t stream) {
+    ReadParams p = {};
+    p.c = c;
+    p.rows = rows;
+    p.cu_k = cu_k;
+    p.k = static_cast<__nv_bfloat16*>(k);
+    p.v = static_cast<__nv_bfloat16*>(v);
+    for (int i = 0; i < 3; ++i) p.ks[i] = p.vs[i] = strides[i];
+    return launch_read(p, bits, d, batch, kv_heads, stream);
+}
+
 }  // namespace ktt
 
 using namespace ktt;
@@ -389,39 +344,5 @@ extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {
         low |= static_cast<uintptr_t>((p.ks[i] | p.vs[i]) * 2);
     }
     if (low & 15) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_read: outputs must be 16-byte aligned in every row");
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int hk = a->cache.kv_heads;
-    if (a->cache.bits == 16) return a->d == 64 ? launch_read<64, 16>(p, a->batch, hk, st) : launch_read<128, 16>(p, a->batch, hk, st);
-    return a->d == 64 ? launch_read<64, 4>(p, a->batch, hk, st) : launch_read<128, 4>(p, a->batch, hk, st);
-}
-
-extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stream) {
-    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null arguments");
-    PlainParams p = {};
-    if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: %s", why);
-    if (a->batch < 1 || a->heads < 1 || a->sq < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: sizes must be positive");
-    if (a->heads % a->cache.kv_heads) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: K / V heads must divide Q heads");
-    if (!(a->scale > 0.f)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: the softmax scale must be positive");
-    if (a->sq == 0) return 0;
-    if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || !a->q || !a->out) {
-        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null pointer");
-    }
-    p.batch = a->batch; p.heads = a->heads; p.kv_heads = a->cache.kv_heads; p.sq = a->sq; p.causal = a->causal;
-    p.scale_log2 = a->scale * kLog2e;
-    p.q = static_cast<const __nv_bfloat16*>(a->q);
-    p.out = static_cast<__nv_bfloat16*>(a->out);
-    for (int i = 0; i < 3; ++i) {
-        p.qs[i] = a->q_strides[i];
-        p.os[i] = a->out_strides[i];
-    }
-    p.cu = a->cu_seqlens_q;
-    p.total_q = a->total_q;
-    const dim3 grid((a->sq + 3) / 4, a->heads, a->batch);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    auto go = [&](auto kernel) {
-        kernel<<<grid, 128, 0, st>>>(p);
-        return check_cuda(cudaGetLastError(), "paged_sdpa launch");
-    };
-    if (a->cache.bits == 16) return a->d == 64 ? go(paged_plain_kernel<64, 16>) : go(paged_plain_kernel<128, 16>);
-    return a->d == 64 ? go(paged_plain_kernel<64, 4>) : go(paged_plain_kernel<128, 4>);
+    return launch_read(p, a->cache.bits, a->d, a->batch, a->cache.kv_heads, static_cast<cudaStream_t>(stream));
 }

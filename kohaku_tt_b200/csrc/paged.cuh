@@ -38,7 +38,7 @@ __device__ __forceinline__ float step_of(uint32_t pair) { return __uint_as_float
 __device__ __forceinline__ float least_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 
 // A paged cache: byte strides; pages outside [0, pages) are no pages (append: the rows go nowhere; read and
-// attention: the keys are not there).
+// attention: zeros).
 struct Pages {
     unsigned char* k;
     unsigned char* v;

@@ -1,0 +1,1023 @@
+// Attention over a paged cache, bf16 or 4 bits: one launch for a few query rows per K / V head, split over the keys.
+//
+//   out_r = sum_j p_rj v_j,  p_r = softmax over the keys j that row r sees of q_r k_j scale.
+//
+// Bound: the reading of the pages, 4 D bytes per key and head in bf16, 9 / 8 D in 4 bits. So all query rows of a K / V head
+// (its group's heads x tokens, in tiles of 8 or 16 rows) share one pass over the keys, and the keys of all (sequence,
+// K / V head) pairs are laid end to end and cut into equal shares (split.cuh), as in decode.cu; where the pairs are few, a
+// cluster of CTAs has a pair to itself. Partial results of a pair meet behind a ticket in L2, or in the cluster's shared
+// memory, and are added in a fixed order.
+//
+// A warp has 16 keys of a tile and a ring of stages of its own: one page, of which it needs one block. Both products have the
+// keys or channels as the rows of their matrix instruction (m16n8k16) and the queries as its 8 columns, so that a
+// group of 8 heads or fewer leaves nothing idle: S^T = K Q^T, then O^T += V^T P^T. P^T comes out of S^T's registers by
+// an 8 x 8 transpose (movmatrix). The reference of the exponentials moves when a score exceeds it by 2^8.
+//
+// 4 bits: a code c is worth least + step c per 64 channels. Codes become bf16 128 + c by one logic operation for two (the
+// pages' layout is made for it, paged.cuh) and never anything else:
+//   s_j   = sum_g step_jg (q_g . (128 + c_jg)) + (least_jg - 128 step_jg) sum(q_g): one product per group of channels g
+//   o_g  += (p_j step_jg) (c_jg - 8), and p_j (least_jg + 8 step_jg) once for all channels of the group: with codes about
+//           their middle, neither sum is large beside the result.
+// p_j step_jg is rounded to bf16 for the product, as p_j is over bf16 pages; all else is fp32.
+#include <atomic>
+
+#include "kept.h"
+#include "paged.cuh"
+#include "split.cuh"
+
+namespace ktt {
+
+// paged.cu: dense rows of the cache for a chunk of a prompt; cu_k (optional) gets the offsets 0, rows, 2 rows, ...
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* cu_k, cudaStream_t stream);
+
+namespace {
+
+struct PagedParams {
+    Pages c;
+    int batch, heads;
+    int kv_heads;            // of the pairs: K / V heads x row tiles
+    int row_tiles, group, sq, causal;
+    int page_blocks;         // blocks of 16 keys in a page
+    float scale_log2;
+    const __nv_bfloat16* q;
+    __nv_bfloat16* out;
+    int64_t qs[3], os[3];
+    const int32_t* cu;       // packed queries
+    int64_t total_q;
+    int32_t* counters;       // [kMaxCtas] tickets, zero between calls
+    float* part_m;           // [slots][16]
+    float* part_l;
+    float* part_o;           // [slots][16][D]
+    int ranks;               // CTAs of a cluster
+};
+
+constexpr int kMaxBatch = 512;    // lengths and their prefix sums live in shared memory
+constexpr int kMaxPending = 8;
+constexpr int kMaxCtas = 1024;
+constexpr int kPairCost = 4;      // what ending a pair costs a CTA, in tiles
+constexpr int kMinUnits = 2;
+
+// What a variant has: D, bits of the pages, NT column tiles of 8 query rows.
+template <int D, int kBits, int NT>
+struct Shape {
+    static constexpr int W = kBits == 4 && NT == 1 ? 8 : 4;       // warps
+    static constexpr int kThreads = 32 * W, kTile = 16 * W;       // keys of a tile
+    static constexpr int kStage = kBits == 4 ? 18 * D : 64 * D;   // bytes: 16 keys, then their values
+    static constexpr int NS = kBits == 4 ? (D == 64 ? 6 : 4) : (D == 64 ? 6 : 3);
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kCtas = kBits == 4 && NT == 2 ? 3 : 2;   // per SM
+    static constexpr int kRing = W * NS * kStage;
+    static constexpr int kSlab = kBits == 4 ? W * kRows * D * 4 : 0;   // bf16: in the stage just consumed
+    static constexpr int kStats = (3 * W + 2) * kRows * 4;
+    static constexpr int smem(bool cluster) {
+        return kRing + kSlab + kStats + (cluster ? kRows * D * 4 : (2 * kMaxBatch + 1 + 8 + 6 * kMaxPending + 3) * 4);
+    }
+};
+
+// Chunk of 16 bytes of a row of the slab where its values lie: rows 2 t and 2 t + 1 of the threads that write at
+// once in different banks.
+__device__ __forceinline__ int slab_chunk(int row, int chunk) {
+    const int t = (row >> 1) & 3;
+    return chunk ^ ((t & 1) | ((t & 2) << 1));
+}
+
+// Byte offset of (row, col) in 16 rows of D bf16 values whose 16-byte chunks are XOR-ed with the row: no two rows of an
+// 8 x 8 matrix in one bank.
+template <int D>
+__device__ __forceinline__ int swizzled(int row, int col) {
+    return (row * D + (((col >> 3) ^ (row & 7)) << 3) + (col & 7)) * 2;
+}
+
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// Two codes of a word as the bf16 values 128 + c.
+__device__ __forceinline__ uint32_t code_pair(uint32_t word) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(y) : "r"(word));   // (word & mask) | 128
+    return y;
+}
+// ... less 136: codes about their middle, exactly.
+__device__ __forceinline__ uint32_t about_middle(uint32_t pair) {
+    const __nv_bfloat162 x = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&pair), __floats2bfloat162_rn(136.f, 136.f));
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Rows of a sequence's queries: how many tokens, and where they start.
+__device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& first) {
+    if (!p.cu) {
+        first = 0;
+        return p.sq;
+    }
+    int64_t lo = p.cu[b], hi = p.cu[b + 1];
+    lo = lo < 0 ? 0 : (lo > p.total_q ? p.total_q : lo);
+    hi = hi < lo ? lo : (hi > p.total_q ? p.total_q : hi);
+    first = lo;
+    return static_cast<int>(hi - lo);
+}
+
+template <int D, int kBits, int NT, bool kCluster>
+__global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBits, NT>::kCtas)) paged_kernel(const __grid_constant__ PagedParams p) {
+    using S = Shape<D, kBits, NT>;
+    constexpr int W = S::W, NS = S::NS, kRows = S::kRows, kTile = S::kTile, kThreads = S::kThreads;
+    constexpr int G = D / 64, MT = D / 16;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    unsigned char* ring = smem + warp * NS * S::kStage;     // this warp's
+    float* sm_m = reinterpret_cast<float*>(smem + S::kRing + S::kSlab);   // [W][kRows]
+    float* sm_l = sm_m + W * kRows;
+    float* sm_f = sm_l + W * kRows;    // a warp's weight in its CTA's sum
+    float* fin_m = sm_f + W * kRows;   // [kRows]
+    float* fin_l = fin_m + kRows;
+    int* prefix_s = reinterpret_cast<int*>(fin_l + kRows);       // [kMaxBatch + 1]
+    int* lens_s = prefix_s + kMaxBatch + 1;
+    int* misc = lens_s + kMaxBatch;
+    float* part_s = fin_l + kRows;     // kCluster: [kRows][D] this CTA's partial
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    Cursor prod, cons;
+    int u1, upc = 0, rank = 0;
+    const int step = kCluster ? p.ranks : 1;
+    if constexpr (kCluster) {
+        const int pair = static_cast<int>(blockIdx.x) / p.ranks;
+        rank = static_cast<int>(blockIdx.x) - pair * p.ranks;
+        cons.b = pair / p.kv_heads;
+        cons.hk = pair - cons.b * p.kv_heads;
+        cons.tile = rank;
+        cons.len = cached_keys(p.c, cons.b);
+        cons.ntiles = max((cons.len + kTile - 1) / kTile, 1);
+        u1 = cons.ntiles > rank ? (cons.ntiles - rank + p.ranks - 1) / p.ranks : 0;
+    } else {
+        scan_lengths<kThreads, kMaxBatch, kTile, kPairCost>(p.batch, [&](int b) { return cached_keys(p.c, b); }, prefix_s, lens_s, misc);
+        const int total = p.kv_heads * prefix_s[p.batch];
+        upc = max(static_cast<int>((total + gridDim.x - 1) / gridDim.x), kMinUnits);
+        const int64_t from = static_cast<int64_t>(blockIdx.x) * upc;
+        const int first_unit = static_cast<int>(from < total ? from : total), end_unit = min(first_unit + upc, total);
+        u1 = tiles_before<kPairCost>(p, prefix_s, end_unit) - tiles_before<kPairCost>(p, prefix_s, first_unit);
+        if (u1 <= 0) return;
+        cursor_seek<kPairCost>(p, prefix_s, lens_s, cons, first_unit);
+    }
+    prod = cons;
+    auto next = [&](Cursor& c) {
+        if constexpr (kCluster) c.tile += p.ranks;
+        else cursor_next<kPairCost>(p, prefix_s, lens_s, c);
+    };
+
+    // One normalised chunk of 4 columns of (pair, row of its tile).
+    auto write_row = [&](int b, int vh, int r, int c4, float4 sum, float ll) {
+        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // (a NaN stays one)
+        const int hk = vh / p.row_tiles, row = (vh - hk * p.row_tiles) * kRows + r;
+        int64_t first;
+        const int n = tokens_of(p, b, first);
+        const int gi = row / n, tq = row - gi * n;
+        __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + (hk * p.group + gi) * p.os[1] + (first + tq) * p.os[2] + c4 * 4;
+        uint2 packed;
+        packed.x = pack_bf16(sum.x * inv, sum.y * inv);
+        packed.y = pack_bf16(sum.z * inv, sum.w * inv);
+        *reinterpret_cast<uint2*>(to) = packed;
+    };
+    // Rows that a pair has in its tile.
+    auto rows_of = [&](int b, int vh) {
+        int64_t first;
+        const int all = p.group * tokens_of(p, b, first);
+        return max(min(all - (vh % p.row_tiles) * kRows, kRows), 0);
+    };
+
+    int* pend = misc + 8;            // [kMaxPending][5]: pair, first CTA, last CTA, batch, head of the pair
+    int* npend_s = pend + 5 * kMaxPending;
+    int* last_s = npend_s + 1;
+    if (!kCluster && threadIdx.x == 0) npend_s[0] = 0;
+
+    // Draws a ticket for each pending pair; the last holder adds the pair's partials up, in the order of the CTAs, and
+    // puts the counter back to zero. (The same as in decode.cu, which has the measurements.)
+    auto draw_tickets = [&]() {
+        __syncthreads();
+        const int n = npend_s[0];
+        if (static_cast<int>(threadIdx.x) < n) {
+            const int* e = pend + 5 * threadIdx.x;
+            const int parts = e[2] - e[1] + 1;
+            int ticket;
+            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + e[1]) : "memory");
+            last_s[threadIdx.x] = ticket == parts - 1;
+            if (ticket == parts - 1) p.counters[e[1]] = 0;
+        }
+        __syncthreads();
+        constexpr int per_pair = kRows * (D / 4), kHolders = 4;
+        for (int idx = threadIdx.x; idx < n * per_pair; idx += kThreads) {
+            const int i = idx / per_pair, rem = idx - i * per_pair, r = rem / (D / 4), c4 = rem % (D / 4);
+            const int* e = pend + 5 * i;
+            if (!last_s[i] || r >= rows_of(e[3], e[4])) continue;
+            const int slot0 = e[1] + e[0], parts = e[2] - e[1] + 1;
+            float mm = -INFINITY, ll = 0.f;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c0 = 0; c0 < parts; c0 += kHolders) {
+                float ms[kHolders], ls[kHolders];
+                float4 v[kHolders];
+#pragma unroll
+                for (int j = 0; j < kHolders; ++j) {
+                    const int slot = slot0 + min(c0 + j, parts - 1);   // past the last holder: a repeat, not used
+                    ms[j] = __ldcg(&p.part_m[slot * 16 + r]);
+                    ls[j] = __ldcg(&p.part_l[slot * 16 + r]);
+                    v[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D + c4 * 4));
+                }
+                float m_new = mm;
+#pragma unroll
+                for (int j = 0; j < kHolders; ++j) {
+                    if (c0 + j < parts) m_new = fmaxf(m_new, ms[j]);
+                }
+                const float base = m_new == -INFINITY ? 0.f : m_new, fa = fast_exp2(mm - base);
+                mm = m_new;
+                ll *= fa;
+                sum.x *= fa; sum.y *= fa; sum.z *= fa; sum.w *= fa;
+#pragma unroll
+                for (int j = 0; j < kHolders; ++j) {
+                    if (c0 + j >= parts) continue;
+                    const float fb = fast_exp2(ms[j] - base);
+                    ll = fmaf(ls[j], fb, ll);
+                    sum.x = fmaf(v[j].x, fb, sum.x); sum.y = fmaf(v[j].y, fb, sum.y);
+                    sum.z = fmaf(v[j].z, fb, sum.z); sum.w = fmaf(v[j].w, fb, sum.w);
+                }
+            }
+            write_row(e[3], e[4], r, c4, sum, ll);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) npend_s[0] = 0;
+        __syncthreads();
+    };
+
+    // The pages of this warp's blocks in the producer's next 32 tiles, a lane each.
+    int64_t page = -1;
+    int page_at = 32;
+    auto issue = [&](const Cursor& c, int st, bool fresh_pair) {
+        if (fresh_pair || page_at == 32) {
+            const int block = (c.tile + lane * step) * W + warp;
+            page = -1;
+            if (static_cast<int64_t>(block) * 16 < c.len) {
+                page = p.c.table[c.b * p.c.table_stride + block / p.page_blocks];
+                if (page < 0 || page >= p.c.pages) page = -1;   // no page: zeros
+            }
+            page_at = 0;
+        }
+        const int64_t pg = __shfl_sync(0xffffffffu, page, page_at);
+        ++page_at;
+        const int block = c.tile * W + warp, j0 = block * 16;
+        if (j0 >= c.len) return;
+        const bool there = pg >= 0;
+        const int hk = c.hk / p.row_tiles, in_page = block % p.page_blocks;
+        const unsigned char* kp = p.c.k + (there ? pg * p.c.ks[0] + hk * p.c.ks[1] : 0);
+        const unsigned char* vp = p.c.v + (there ? pg * p.c.vs[0] + hk * p.c.vs[1] : 0);
+        const uint32_t to = smem_u32(ring + st * S::kStage);
+        if constexpr (kBits == 16) {
+            constexpr int CH = D / 8;
+            const int left = c.len - j0;
+            kp += there ? in_page * 16 * p.c.ks[2] : 0;
+            vp += there ? in_page * 16 * p.c.vs[2] : 0;
+#pragma unroll
+            for (int it = 0; it < 16 * CH / 32; ++it) {
+                const int idx = it * 32 + lane, r = idx / CH, ch = idx % CH;
+                const bool ok = there && r < left;   // rows behind the last key are zeros, whatever the page holds
+                cp_async_16(to + swizzled<D>(r, ch * 8), kp + (ok ? r * p.c.ks[2] : 0) + (ok ? ch * 16 : 0), ok);
+                cp_async_16(to + 32 * D + swizzled<D>(r, ch * 8), vp + (ok ? r * p.c.vs[2] : 0) + (ok ? ch * 16 : 0), ok);
+            }
+        } else {
+            constexpr int kHalf = 9 * D / 16;   // 16-byte pieces of a block
+            kp += there ? in_page * (9 * D) : 0;
+            vp += there ? in_page * (9 * D) : 0;
+#pragma unroll
+            for (int it = 0; it < (2 * kHalf + 31) / 32; ++it) {
+                const int idx = it * 32 + lane;
+                if (idx < 2 * kHalf) {
+                    const unsigned char* from = idx < kHalf ? kp + (there ? idx * 16 : 0) : vp + (there ? (idx - kHalf) * 16 : 0);
+                    cp_async_16(to + idx * 16, from, there);
+                }
+            }
+        }
+    };
+
+    int up = 0;
+    bool fresh_prod = true;
+    auto produce = [&]() {
+        if (up < u1) {
+            issue(prod, up % NS, fresh_prod);
+            const int b = prod.b, hk = prod.hk;
+            next(prod);
+            fresh_prod = b != prod.b || hk != prod.hk;
+            ++up;
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) produce();
+
+    uint32_t qb[NT][MT][2];           // B operands of S^T: columns are query rows
+    float qsum[NT][G][2];             // 4 bits: sums of this thread's two columns by group of channels
+    int lim[NT][2], whole = 0;        // the last key that a column sees; that all columns see
+    float o[MT][NT][4], mid[NT][G][2], m_ref[NT][2], l_run[NT][2];
+    bool fresh = true;
+
+    for (int u = 0; u < u1; ++u) {
+        const int st = u % NS;
+        produce();
+        if (fresh) {
+            fresh = false;
+            const int hk = cons.hk / p.row_tiles, row0 = (cons.hk - hk * p.row_tiles) * kRows;
+            int64_t first;
+            const int n = tokens_of(p, cons.b, first), rows = p.group * n;
+            whole = p.causal ? cons.len - n : cons.len - 1;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int r = row0 + nt * 8 + g;
+                const bool ok = r < rows;
+                const int gi = ok ? r / n : 0, tq = ok ? r - gi * n : 0;
+                // (A row past the last reads the first and is zeroed after; without any row at all nothing is read.)
+                const __nv_bfloat16* from = p.q + (p.cu ? 0 : cons.b * p.qs[0]) + (hk * p.group + gi) * p.qs[1] + (rows > 0 ? first + tq : 0) * p.qs[2];
+                if constexpr (kBits == 16) {
+#pragma unroll
+                    for (int kk = 0; kk < MT; ++kk) {
+                        const uint32_t lo = *reinterpret_cast<const uint32_t*>(from + kk * 16 + t * 2), hi = *reinterpret_cast<const uint32_t*>(from + kk * 16 + 8 + t * 2);
+                        qb[nt][kk][0] = ok ? lo : 0u;
+                        qb[nt][kk][1] = ok ? hi : 0u;
+                    }
+                } else {
+                    // Channels 32 i + 8 t .. of a word's eight, four to a k step.
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t x = *reinterpret_cast<const uint32_t*>(from + 32 * i + 8 * t + 2 * e);
+                            qb[nt][2 * i + (e >> 1)][e & 1] = ok ? x : 0u;
+                        }
+                    }
+#pragma unroll
+                    for (int w = 0; w < G; ++w) {
+                        float sum = 0.f;
+#pragma unroll
+                        for (int kk = 4 * w; kk < 4 * w + 4; ++kk) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qb[nt][kk][e]));
+                                sum += x.x + x.y;
+                            }
+                        }
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                        qsum[nt][w][0] = __shfl_sync(0xffffffffu, sum, 8 * t);
+                        qsum[nt][w][1] = __shfl_sync(0xffffffffu, sum, 8 * t + 4);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int c = row0 + nt * 8 + 2 * t + e;
+                    lim[nt][e] = p.causal ? cons.len - n + (c < rows ? c % n : 0) : cons.len - 1;
+                    m_ref[nt][e] = -INFINITY;
+                    l_run[nt][e] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < G; ++w) mid[nt][w][e] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
+            }
+        }
+        cp_async_wait<NS - 1>();
+        __syncwarp();
+
+        const int j0 = (cons.tile * W + warp) * 16;
+        if (j0 < cons.len) {
+            const unsigned char* sk = ring + st * S::kStage;
+            const unsigned char* sv = sk + S::kStage / 2;
+            float x[NT][4];   // logits in base 2: key g of columns 2 t, 2 t + 1, then key g + 8
+            uint2 vstep[2];   // 4 bits: (step, least) of the two keys' values
+            if constexpr (kBits == 16) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+                const uint32_t base = smem_u32(sk);
+                const int r = (lane & 7) + ((lane >> 3) & 1) * 8, c = (lane >> 4) * 8;
+#pragma unroll
+                for (int kk = 0; kk < MT; ++kk) {
+                    uint32_t a[4];
+                    ldmatrix_x4(a, base + swizzled<D>(r, kk * 16 + c));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16(x[nt], a, qb[nt][kk][0], qb[nt][kk][1]);
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[nt][e] *= p.scale_log2;
+                }
+            } else {
+                uint32_t kw[2][D / 32];
+                uint2 kstep[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const unsigned char* row = sk + (g + 8 * h) * (D / 2);
+                    const unsigned char* steps = sk + 8 * D + (g + 8 * h) * (D / 16);
+                    const unsigned char* vsteps = sv + 8 * D + (g + 8 * h) * (D / 16);
+                    if constexpr (D == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * t);
+                        kw[h][0] = w.x; kw[h][1] = w.y; kw[h][2] = w.z; kw[h][3] = w.w;
+                        kstep[h] = *reinterpret_cast<const uint2*>(steps);
+                        vstep[h] = *reinterpret_cast<const uint2*>(vsteps);
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(row + 8 * t);
+                        kw[h][0] = w.x; kw[h][1] = w.y;
+                        kstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(steps), 0u);
+                        vstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(vsteps), 0u);
+                    }
+                    if (j0 + g + 8 * h >= cons.len) kstep[h] = vstep[h] = make_uint2(0u, 0u);   // whatever the page holds there
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+#pragma unroll
+                for (int w = 0; w < G; ++w) {
+                    float acc[NT][4];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+                    for (int i = 2 * w; i < 2 * w + 2; ++i) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t a[4] = {code_pair(kw[0][i] >> (8 * h)), code_pair(kw[1][i] >> (8 * h)), code_pair(kw[0][i] >> (8 * h + 4)), code_pair(kw[1][i] >> (8 * h + 4))};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], a, qb[nt][2 * i + h][0], qb[nt][2 * i + h][1]);
+                        }
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t pair = w ? kstep[h].y : kstep[h].x;
+                        const float ks = step_of(pair) * p.scale_log2, kl = fmaf(-128.f, ks, least_of(pair) * p.scale_log2);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) x[nt][2 * h + e] += fmaf(ks, acc[nt][2 * h + e], kl * qsum[nt][w][e]);
+                        }
+                    }
+                }
+            }
+            if (j0 + 15 > whole) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (j0 + g + 8 * (e >> 1) > lim[nt][e & 1]) x[nt][e] = -INFINITY;
+                    }
+                }
+            }
+            bool higher = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) higher |= x[nt][e] > m_ref[nt][e & 1] + 8.f;
+            }
+            if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(x[nt][e], x[nt][e + 2]);
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        top = fmaxf(top, m_ref[nt][e]);
+                        const float f = fast_exp2(m_ref[nt][e] - (top == -INFINITY ? 0.f : top));
+                        m_ref[nt][e] = top;
+                        l_run[nt][e] *= f;
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            o[mt][nt][e] *= f;
+                            o[mt][nt][e + 2] *= f;
+                        }
+#pragma unroll
+                        for (int w = 0; w < G; ++w) mid[nt][w][e] *= f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float ref = m_ref[nt][e & 1];
+                    x[nt][e] = fast_exp2(x[nt][e] - (ref == -INFINITY ? 0.f : ref));
+                    l_run[nt][e & 1] += x[nt][e];
+                }
+            }
+            if constexpr (kBits == 16) {
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    pb[nt][0] = transposed(pack_bf16(x[nt][0], x[nt][1]));
+                    pb[nt][1] = transposed(pack_bf16(x[nt][2], x[nt][3]));
+                }
+                const uint32_t base = smem_u32(sv);
+                const int r = (lane & 7) + (lane >> 4) * 8, c = ((lane >> 3) & 1) * 8;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    uint32_t a[4];
+                    ldmatrix_x4_trans(a, base + swizzled<D>(r, mt * 16 + c));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16(o[mt][nt], a, pb[nt][0], pb[nt][1]);
+                }
+            } else {
+                uint32_t pb[NT][G][2];
+#pragma unroll
+                for (int w = 0; w < G; ++w) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t pair = w ? vstep[h].y : vstep[h].x;
+                        const float vs = step_of(pair), vm = fmaf(8.f, vs, least_of(pair));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            pb[nt][w][h] = transposed(pack_bf16(x[nt][2 * h] * vs, x[nt][2 * h + 1] * vs));
+                            mid[nt][w][0] = fmaf(x[nt][2 * h], vm, mid[nt][w][0]);
+                            mid[nt][w][1] = fmaf(x[nt][2 * h + 1], vm, mid[nt][w][1]);
+                        }
+                    }
+                }
+                uint32_t vw[2][2][G];   // token pairs t and t + 4: even token's words, odd token's
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int pair = t + 4 * h, place = g ^ (D == 128 ? 2 * (pair & 3) : 4 * ((pair >> 1) & 1));
+                    const unsigned char* from = sv + (pair * 8 + place) * (8 * G);
+                    if constexpr (D == 128) {
+                        const uint4 w = *reinterpret_cast<const uint4*>(from);
+                        vw[h][0][0] = w.x; vw[h][0][G - 1] = w.y; vw[h][1][0] = w.z; vw[h][1][G - 1] = w.w;
+                    } else {
+                        const uint2 w = *reinterpret_cast<const uint2*>(from);
+                        vw[h][0][0] = w.x; vw[h][1][0] = w.y;
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < G; ++w) {
+                    const uint32_t lo0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x5410), hi0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x7632);
+                    const uint32_t lo1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x5410), hi1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x7632);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        // Row g: channel 64 w + 8 g + 2 i; row g + 8: the next one.
+                        const uint32_t a[4] = {about_middle(code_pair(lo0 >> (4 * i))), about_middle(code_pair(hi0 >> (4 * i))),
+                                               about_middle(code_pair(lo1 >> (4 * i))), about_middle(code_pair(hi1 >> (4 * i)))};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[4 * w + i][nt], a, pb[nt][w][0], pb[nt][w][1]);
+                    }
+                }
+            }
+        }
+        __syncwarp();   // all lanes are done with stage `st` before it is filled again
+
+        const bool last_of_pair = !kCluster && cons.tile + 1 == cons.ntiles;
+        if (last_of_pair || u + 1 == u1) {
+            // The warps' results to shared memory, each with its own reference; then their sum in the order of the warps.
+            float* slab = reinterpret_cast<float*>(kBits == 4 ? smem + S::kRing + warp * (kRows * D * 4) : ring + st * S::kStage);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float l = l_run[nt][e];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+                    const int r = nt * 8 + 2 * t + e;
+                    if (g == 0) {
+                        sm_m[warp * kRows + r] = m_ref[nt][e];
+                        sm_l[warp * kRows + r] = l;
+                    }
+                    if constexpr (kBits == 16) {
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const int c = mt * 16 + g + 8 * h;
+                                slab[r * D + slab_chunk(r, c >> 2) * 4 + (c & 3)] = o[mt][nt][e + 2 * h];
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < G; ++w) {
+                            float add = mid[nt][w][e];
+#pragma unroll
+                            for (int off = 4; off < 32; off <<= 1) add += __shfl_xor_sync(0xffffffffu, add, off);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const float4 y = make_float4(o[4 * w + 2 * h][nt][e] + add, o[4 * w + 2 * h][nt][e + 2] + add,
+                                                             o[4 * w + 2 * h + 1][nt][e] + add, o[4 * w + 2 * h + 1][nt][e + 2] + add);
+                                *reinterpret_cast<float4*>(slab + r * D + slab_chunk(r, 16 * w + 2 * g + h) * 4) = y;
+                            }
+                        }
+                    }
+                }
+            }
+            __syncthreads();
+            if (threadIdx.x < kRows) {
+                const int r = threadIdx.x;
+                float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+                for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm_m[w * kRows + r]);
+                const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float f = fast_exp2(sm_m[w * kRows + r] - base);
+                    sm_f[w * kRows + r] = f;
+                    ll = fmaf(sm_l[w * kRows + r], f, ll);
+                }
+                fin_m[r] = mm;
+                fin_l[r] = ll;
+            }
+            __syncthreads();
+            auto merged = [&](int r, int c4) {
+                const unsigned char* from = (kBits == 4 ? smem + S::kRing : smem + st * S::kStage) + (r * D + slab_chunk(r, c4) * 4) * 4;
+                constexpr int kNext = kBits == 4 ? kRows * D * 4 : NS * S::kStage;
+                float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const float4 y = *reinterpret_cast<const float4*>(from + w * kNext);
+                    const float f = sm_f[w * kRows + r];
+                    sum.x = fmaf(y.x, f, sum.x); sum.y = fmaf(y.y, f, sum.y);
+                    sum.z = fmaf(y.z, f, sum.z); sum.w = fmaf(y.w, f, sum.w);
+                }
+                return sum;
+            };
+            const int rows = rows_of(cons.b, cons.hk);
+            if constexpr (kCluster) {
+                for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
+                    const int r = idx / (D / 4), c4 = idx % (D / 4);
+                    const float4 sum = merged(r, c4);
+                    if (cons.ntiles == 1) write_row(cons.b, cons.hk, r, c4, sum, fin_l[r]);
+                    else reinterpret_cast<float4*>(part_s)[idx] = sum;
+                }
+                break;
+            }
+            const int pair = cons.b * p.kv_heads + cons.hk;
+            const int t0 = p.kv_heads * prefix_s[cons.b] + cons.hk * (cons.ntiles + kPairCost);   // the pair's first unit
+            const int c_first = t0 / upc, c_last = (t0 + cons.ntiles - 1) / upc;
+            if (c_first == c_last) {
+                for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
+                    const int r = idx / (D / 4), c4 = idx % (D / 4);
+                    write_row(cons.b, cons.hk, r, c4, merged(r, c4), fin_l[r]);
+                }
+            } else {
+                const int slot = blockIdx.x + pair;
+                for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
+                    const int r = idx / (D / 4), c4 = idx % (D / 4);
+                    reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D)[c4] = merged(r, c4);
+                }
+                if (threadIdx.x < kRows) {
+                    p.part_m[slot * 16 + threadIdx.x] = fin_m[threadIdx.x];
+                    p.part_l[slot * 16 + threadIdx.x] = fin_l[threadIdx.x];
+                }
+                if (threadIdx.x == 0) {
+                    int* e = pend + 5 * npend_s[0];
+                    e[0] = pair; e[1] = c_first; e[2] = c_last; e[3] = cons.b; e[4] = cons.hk;
+                    npend_s[0] += 1;
+                }
+                __syncthreads();
+                if (npend_s[0] == kMaxPending || u + 1 < u1) draw_tickets();
+            }
+            __syncthreads();
+            fresh = true;
+        }
+        next(cons);
+    }
+    cp_async_wait<0>();
+    if constexpr (kCluster) {
+        if (cons.ntiles == 1) return;   // one rank had all of it and has written it: nobody waits for anybody
+        cluster_meet();
+        // Every rank adds up its share of the output, the ranks that had a tile in their order.
+        const int rows = rows_of(cons.b, cons.hk);
+        const int parts = min(cons.ntiles, p.ranks), all = rows * (D / 4), share = (all + p.ranks - 1) / p.ranks;
+        const uint32_t at_m = smem_u32(fin_m), at_l = smem_u32(fin_l), at_o = smem_u32(part_s);
+        for (int idx = rank * share + threadIdx.x; idx < min((rank + 1) * share, all); idx += kThreads) {
+            const int r = idx / (D / 4), c4 = idx % (D / 4);
+            float ms[8], ls[8], mm = -INFINITY, ll = 0.f;
+            float4 v[8], sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {   // (ranks: 8 at most)
+                const int from = min(j, parts - 1);
+                ms[j] = ld_cluster(in_rank(at_m + r * 4, from));
+                ls[j] = ld_cluster(in_rank(at_l + r * 4, from));
+                v[j] = ld_cluster4(in_rank(at_o + idx * 16, from));
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mm = fmaxf(mm, ms[j]);
+            const float base = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (j >= parts) continue;
+                const float f = fast_exp2(ms[j] - base);
+                ll = fmaf(ls[j], f, ll);
+                sum.x = fmaf(v[j].x, f, sum.x); sum.y = fmaf(v[j].y, f, sum.y);
+                sum.z = fmaf(v[j].z, f, sum.z); sum.w = fmaf(v[j].w, f, sum.w);
+            }
+            write_row(cons.b, cons.hk, r, c4, sum, ll);
+        }
+        cluster_meet();   // nobody's shared memory goes away while another reads it
+    } else {
+        __syncthreads();
+        if (npend_s[0] > 0) draw_tickets();
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+int current_device() {
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64 ? dev : -1;
+}
+
+int sm_count(int dev) {
+    static std::atomic<int> known[64];
+    if (dev < 0) return 148;
+    const int sms = kept(known[dev], [&]() {
+        int n = 0;
+        return cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess ? n : -1;
+    });
+    return sms > 0 ? sms : 148;
+}
+
+template <int D, int kBits, int NT, bool kCluster>
+cudaLaunchConfig_t paged_config(int ctas, int ranks, cudaStream_t stream, cudaLaunchAttribute* attr) {
+    using S = Shape<D, kBits, NT>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(ctas));
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::smem(kCluster);
+    cfg.stream = stream;
+    if (kCluster) {
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = static_cast<unsigned>(ranks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.numAttrs = 1;
+    }
+    cfg.attrs = attr;
+    return cfg;
+}
+
+// Clusters of `ranks` CTAs that run at the same time on the current device; asked for once. -1: no answer now.
+template <int D, int kBits, int NT>
+int cluster_room(int dev, int ranks) {
+    static std::atomic<int> known[64][4];   // by log2 of the ranks
+    if (dev < 0) return -1;
+    int log = 0;
+    while ((1 << log) < ranks) ++log;
+    return kept(known[dev][log], [&]() {
+        auto kernel = paged_kernel<D, kBits, NT, true>;
+        cudaLaunchAttribute attr[1];
+        cudaLaunchConfig_t cfg = paged_config<D, kBits, NT, true>(ranks, ranks, nullptr, attr);
+        int n = 0;
+        if (raise_smem_limit(kernel, static_cast<int>(cfg.dynamicSmemBytes)) == cudaSuccess &&
+            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess) return n;
+        cudaGetLastError();   // not this call's failure
+        return -1;
+    });
+}
+
+// Set up once per device, by the first call of whatever size: both kernels' limits and the room for clusters.
+template <int D, int kBits, int NT>
+int paged_set_up(int dev) {
+    static std::atomic<int> done[64];
+    int rc = 0;
+    auto shares = [&]() { return rc = ensure_smem(paged_kernel<D, kBits, NT, false>, Shape<D, kBits, NT>::smem(false), "cudaFuncSetAttribute(paged)"); };
+    if (dev < 0) return shares();
+    kept(done[dev], [&]() {
+        int least = shares();
+        for (int ranks = 1; ranks <= 8; ranks *= 2) {
+            const int room = cluster_room<D, kBits, NT>(dev, ranks);
+            least = room < least ? room : least;
+        }
+        return least < 0 ? -1 : 0;
+    });
+    return rc;
+}
+
+// CTAs per pair where each has a cluster of its own; 0 where the pairs are cut into equal shares.
+template <int D, int kBits, int NT>
+int paged_ranks(int64_t pairs, int cap, int ctas, int dev) {
+    constexpr int kTile = Shape<D, kBits, NT>::kTile;
+    for (int ranks = 8; ranks >= 1; ranks /= 2) {
+        if (ranks > 1 && (ranks / 2) * kTile >= cap) continue;   // half as many have a tile each
+        if (pairs * ranks > ctas || cluster_room<D, kBits, NT>(dev, ranks) < pairs) continue;
+        const int64_t used = pairs * ranks * (ranks == 1 ? 7 : 6), all = static_cast<int64_t>(ctas) * 6, most = 16ll * kTile * ranks;
+        return cap <= most && (ranks == 8 || 2 * cap <= most || cap * all <= most * used) ? ranks : 0;
+    }
+    return 0;
+}
+
+struct Parts {
+    int64_t m_bytes, o_bytes, total;
+};
+Parts parts_of(int64_t pairs, int d, int ctas) {
+    Parts s;
+    const int64_t slots = ctas + pairs;
+    auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    s.m_bytes = up(slots * 16 * 4);
+    s.o_bytes = up(slots * 16 * d * 4);
+    s.total = 2 * s.m_bytes + s.o_bytes;
+    return s;
+}
+
+// Rows of a K / V head (its heads x tokens) up to which its keys are passed over once for every 8 or 16 of them; more
+// rows are a matter for the tensor path (below).
+constexpr int kFewRows = 64;
+
+// What a call will do, from its sizes alone.
+struct Plan {
+    bool few;
+    int nt, row_tiles, slice;   // sequences of a launch
+    int64_t bytes;              // of workspace
+};
+
+int64_t rows_per_head(const ktt_b200_paged_sdpa_args* a) { return static_cast<int64_t>(a->heads / a->cache.kv_heads) * a->sq; }
+
+Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
+    Plan s = {};
+    const int64_t rows = rows_per_head(a), hk = a->cache.kv_heads;
+    s.few = rows <= kFewRows;
+    if (s.few) {
+        s.nt = rows <= 8 ? 1 : 2;
+        s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
+        // Units of all pairs have to fit 30 bits.
+        int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 64 + 1 + kPairCost) * hk * s.row_tiles);
+        most = most < 1 ? 1 : (most > kMaxBatch ? kMaxBatch : most);
+        s.slice = static_cast<int>(a->batch < most ? a->batch : most);
+        s.bytes = parts_of(s.slice * hk * s.row_tiles, a->d, sms * 3).total;
+        return s;
+    }
+    // Dense rows of some sequences at a time: 1 GB, or one sequence.
+    const int64_t one = 4ll * c.cap * hk * a->d;
+    const int64_t most = (1ll << 30) / one;
+    s.slice = static_cast<int>(most < 1 ? 1 : (most < a->batch ? most : a->batch));
+    if (s.slice > kMaxBatch) s.slice = kMaxBatch;
+    s.bytes = s.slice * one + 4096;   // offsets of the slice's keys behind the rows
+    return s;
+}
+
+template <int D, int kBits, int NT>
+int run_few(PagedParams& p, cudaStream_t stream) {
+    using S = Shape<D, kBits, NT>;
+    const int dev = current_device();
+    if (int rc = paged_set_up<D, kBits, NT>(dev)) return rc;
+    int ctas = S::kCtas * sm_count(dev);
+    if (ctas > kMaxCtas) ctas = kMaxCtas;
+    const int64_t pairs = static_cast<int64_t>(p.batch) * p.kv_heads;
+    p.ranks = paged_ranks<D, kBits, NT>(pairs, p.c.cap, ctas, dev);
+    cudaLaunchAttribute attr[2];
+    auto go = [&](auto kernel, cudaLaunchConfig_t cfg) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+        ++cfg.numAttrs;
+        return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "paged_sdpa launch");
+    };
+    if (p.ranks > 0) return go(paged_kernel<D, kBits, NT, true>, paged_config<D, kBits, NT, true>(static_cast<int>(pairs) * p.ranks, p.ranks, stream, attr));
+    return go(paged_kernel<D, kBits, NT, false>, paged_config<D, kBits, NT, false>(ctas, 1, stream, attr));
+}
+
+template <int D, int kBits>
+int run_few(PagedParams& p, int nt, cudaStream_t stream) { return nt == 1 ? run_few<D, kBits, 1>(p, stream) : run_few<D, kBits, 2>(p, stream); }
+
+const char* sdpa_refusal(const ktt_b200_paged_sdpa_args* a, Pages& c) {
+    if (const char* why = pages_of(c, a->cache, a->d)) return why;
+    if (a->heads < 1 || a->heads % a->cache.kv_heads) return "K / V heads must divide Q heads";
+    if (a->heads > 65535 || a->batch > 65535) return "batch and heads must not exceed 65535";
+    if (!(a->scale > 0.f)) return "the softmax scale must be positive";
+    if (rows_per_head(a) >= (1ll << 31)) return "too many query rows";
+    for (int i = 0; i < 3; ++i) {
+        if (a->q_strides[i] % 2 || a->out_strides[i] % 4) return "q strides must be even and out strides multiples of 4";
+    }
+    if ((reinterpret_cast<uintptr_t>(a->q) & 3) || (reinterpret_cast<uintptr_t>(a->out) & 7)) return "q must be 4-byte and out 8-byte aligned";
+    if ((static_cast<int64_t>(c.cap) / 64 + 1 + kPairCost) * a->cache.kv_heads * 8 > (1ll << 30)) return "too many keys and heads";
+    return nullptr;
+}
+
+// A chunk of a prompt: the rows of a K / V head are many, so the work is in the products, which the tensor kernels of the
+// dense and packed forward do; the pages become dense bf16 rows for them first (2 x 2 D bytes written and read per key
+// and head, against 4 D operations per key and row).
+int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice, cudaStream_t stream) {
+    const int hk = a->cache.kv_heads, d = a->d;
+    const int64_t cap = p.c.cap, half = slice * cap * hk * d;
+    __nv_bfloat16* k = static_cast<__nv_bfloat16*>(a->workspace);
+    __nv_bfloat16* v = k + half;
+    int32_t* cu_k = reinterpret_cast<int32_t*>(v + half);
+    for (int b0 = 0; b0 < a->batch; b0 += slice) {
+        const int n = a->batch - b0 < slice ? a->batch - b0 : slice;
+        Pages c = p.c;
+        c.table += b0 * c.table_stride;
+        c.lengths += b0;
+        ktt_b200_attn_args f = {};
+        f.batch = n;
+        f.heads = a->heads;
+        f.kv_heads = hk;
+        f.sq = a->sq;
+        f.sk = static_cast<int32_t>(cap);
+        f.d = f.dv = d;
+        f.scale = a->scale;
+        f.q = p.q;
+        f.k = k;
+        f.v = v;
+        f.out = p.out;
+        f.lse_strides[2] = 1;
+        f.workspace = a->counters;
+        f.workspace_bytes = 256;
+        // All rows of a head together, sequence after sequence: a dense call's keys, and a packed one's.
+        const int64_t strides[3] = {cap * d, slice * cap * d, d};
+        for (int i = 0; i < 3; ++i) {
+            f.q_strides[i] = a->q_strides[i];
+            f.out_strides[i] = a->out_strides[i];
+            f.k_strides[i] = f.v_strides[i] = strides[i];
+        }
+        f.key_lengths = c.lengths;   // (a length of 0 counts as 1 there: a row of zeros)
+        f.causal = a->causal ? KTT_B200_CAUSAL_KEY_END : KTT_B200_CAUSAL_NONE;
+        if (a->cu_seqlens_q) {
+            f.total_q = a->total_q;
+            f.total_k = slice * cap;
+            f.cu_seqlens_q = a->cu_seqlens_q + b0;
+            f.cu_seqlens_k = cu_k;
+            f.q_strides[0] = f.out_strides[0] = f.k_strides[0] = f.v_strides[0] = 0;
+        } else {
+            f.q = p.q + b0 * a->q_strides[0];
+            f.out = p.out + b0 * a->out_strides[0];
+        }
+        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, a->cu_seqlens_q ? cu_k : nullptr, stream)) return rc;
+        if (int rc = ktt_b200_sdpa_forward(&f, stream)) return rc;
+    }
+    return 0;
+}
+
+}  // namespace
+}  // namespace ktt
+
+using namespace ktt;
+
+extern "C" int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args* a) {
+    Pages c = {};
+    if (!a || a->batch < 1 || a->sq < 0) {
+        fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: sizes must be positive");
+        return -1;
+    }
+    if (const char* why = sdpa_refusal(a, c)) {
+        fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: %s", why);
+        return -1;
+    }
+    return a->sq == 0 ? 0 : plan_of(a, c, sm_count(current_device())).bytes;
+}
+
+extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stream) {
+    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null arguments");
+    PagedParams p = {};
+    if (a->batch < 1 || a->sq < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: sizes must be positive");
+    if (const char* why = sdpa_refusal(a, p.c)) {
+        note_call(4);
+        return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: %s", why);
+    }
+    if (a->sq == 0) return 0;
+    if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || !a->q || !a->out) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null pointer");
+    }
+    const Plan s = plan_of(a, p.c, sm_count(current_device()));
+    if (!a->counters || !a->workspace || a->workspace_bytes < s.bytes) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: counters and %lld bytes of workspace are needed", static_cast<long long>(s.bytes));
+    }
+    if ((reinterpret_cast<uintptr_t>(a->counters) | reinterpret_cast<uintptr_t>(a->workspace)) & 15) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: counters and workspace must be 16-byte aligned");
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    if (!s.few) return run_many(a, p, s.slice, st);
+    p.heads = a->heads;
+    p.row_tiles = s.row_tiles;
+    p.kv_heads = a->cache.kv_heads * s.row_tiles;
+    p.group = a->heads / a->cache.kv_heads;
+    p.sq = a->sq;
+    p.causal = a->causal != 0;
+    p.page_blocks = a->cache.page_size / 16;
+    p.scale_log2 = a->scale * kLog2e;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a->q_strides[i];
+        p.os[i] = a->out_strides[i];
+    }
+    p.total_q = a->total_q;
+    const Parts parts = parts_of(static_cast<int64_t>(s.slice) * p.kv_heads, a->d, sm_count(current_device()) * 3);
+    unsigned char* base = static_cast<unsigned char*>(a->workspace);
+    p.counters = static_cast<int32_t*>(a->counters);
+    p.part_m = reinterpret_cast<float*>(base);
+    p.part_l = reinterpret_cast<float*>(base + parts.m_bytes);
+    p.part_o = reinterpret_cast<float*>(base + 2 * parts.m_bytes);
+    const Pages all = p.c;
+    note_call(3);
+    for (int b0 = 0; b0 < a->batch; b0 += s.slice) {
+        p.batch = a->batch - b0 < s.slice ? a->batch - b0 : s.slice;
+        p.c.table = all.table + b0 * all.table_stride;
+        p.c.lengths = all.lengths + b0;
+        p.cu = a->cu_seqlens_q ? a->cu_seqlens_q + b0 : nullptr;
+        p.q = static_cast<const __nv_bfloat16*>(a->q) + (p.cu ? 0 : b0 * a->q_strides[0]);
+        p.out = static_cast<__nv_bfloat16*>(a->out) + (p.cu ? 0 : b0 * a->out_strides[0]);
+        int rc;
+        if (a->cache.bits == 16) rc = a->d == 64 ? run_few<64, 16>(p, s.nt, st) : run_few<128, 16>(p, s.nt, st);
+        else rc = a->d == 64 ? run_few<64, 4>(p, s.nt, st) : run_few<128, 4>(p, s.nt, st);
+        if (rc) return rc;
+    }
+    return 0;
+}

@@ -141,6 +141,21 @@ def _read(k_pages, v_pages, block_table, lengths, max_k):
     return k, v
 
 
+_COUNTERS = {}
+
+
+def _counters(device):
+    """Tickets of the split over the keys: zero before a call, and after it. A buffer per device and stream; a
+    captured call has its own, which its graph fills at every replay."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros((4096,), dtype=torch.uint8, device=device)
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
+    buf = _COUNTERS.get(key)
+    if buf is None:
+        buf = _COUNTERS[key] = torch.zeros((4096,), dtype=torch.uint8, device=device)
+    return buf
+
+
 def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k):
     what = "sdpa_paged"
     ops._require_cuda(q)
@@ -151,6 +166,8 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
         raise ValueError("kohaku_tt_b200.sdpa_paged: q must be [B, H, Sq, D], or packed [T, H, D] with cu_seq_q")
     rows = q.shape[0] if packed else q.shape[2]
     q = _operand(q, "q", q.shape[1], k_pages, batch, rows, dim, packed, what)
+    if q.data_ptr() % 16 or any(x % 8 for x in q.stride()[:-1]):
+        q = q.clone(memory_format=torch.contiguous_format)   # (rows that the kernels cannot read in place)
     strides = ops._ths_strides if packed else ops._bhs_strides
     with torch.cuda.device(q.device):
         cu = None
@@ -167,6 +184,11 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
         a.q, a.out = q.data_ptr(), out.data_ptr()
         ops._set3(a.q_strides, strides(q))
         ops._set3(a.out_strides, strides(out))
+        need = _lib.lib().ktt_b200_paged_sdpa_workspace(ctypes.byref(a))
+        if need < 0:
+            _lib.check(_lib.ERR_UNSUPPORTED, what)
+        counters, work = _counters(q.device), torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
+        a.counters, a.workspace, a.workspace_bytes = counters.data_ptr(), work.data_ptr(), work.numel()
         _lib.check(_lib.lib().ktt_b200_paged_sdpa(ctypes.byref(a), ops._stream(q.device)), what)
     return out
 
@@ -254,7 +276,7 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
     device) count the keys with those of the call's own tokens, which are appended first. Under is_causal the
     diagonal is aligned to the end: query i of n sees keys 0 .. lengths[b] - n + i. A row that sees no key
     gets zeros. max_k: no sequence has more keys (default: what block_table has room for; longer ones are
-    cut). A key that some of a sequence's queries see and others do not must be finite. No gradients."""
+    cut); an entry of block_table within a length that is no page of the cache reads as zeros. A key that some of a sequence's queries see and others do not must be finite. No gradients."""
     causal = bool(is_causal)
     if torch.compiler.is_compiling():
         return torch.ops.ktt_b200._sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)

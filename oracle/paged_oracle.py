@@ -105,43 +105,47 @@ def values(pages, value):
     return worth(*unpack(pages, value)) if pages.dtype == torch.uint8 else pages.float()
 
 
-def sequence(pages, row, count, value):
-    """(float64 [Hk, count, D], bool [count]: whether the key has a page)."""
+def about_middle(pages):
+    """What pages of 4 bits hold beside the middle of their range: step * |code - 8|; 0 for bf16."""
+    if pages.dtype != torch.uint8:
+        return torch.zeros_like(pages, dtype=torch.float32)
+    code, step, _ = unpack(pages, True)
+    return worth(code - 8, step, torch.zeros_like(step)).abs()
+
+
+def sequence(pages, row, count, value, vals=None):
+    """float64 [Hk, count, D]; zeros where there is no page."""
     page = pages.shape[2]
-    got, there = [], []
-    vals = values(pages, value).double()
+    vals = (values(pages, value) if vals is None else vals).double()
+    got = torch.zeros((pages.shape[1], count, vals.shape[-1]), dtype=torch.float64)
     for j in range(count):
         p = int(row[j // page])
-        ok = 0 <= p < pages.shape[0]
-        there.append(ok)
-        got.append(vals[p if ok else 0, :, j % page])
-    d = vals.shape[-1]
-    k = torch.stack(got, 1) if got else torch.zeros((pages.shape[1], 0, d), dtype=torch.float64)
-    return k, torch.tensor(there, dtype=torch.bool)
+        if 0 <= p < pages.shape[0]:
+            got[:, j] = vals[p, :, j % page]
+    return got
 
 
 def attend(q, k_pages, v_pages, table_rows, lengths, causal, scale, counts=None):
-    """q: list of [H, n, D] float64 per sequence. Returns lists (out, sum p |v|, largest sum |q| |k| scale per
-    row) per sequence."""
+    """q: list of [H, n, D] float64 per sequence. Returns lists (out, sum p (|v| + step |code - 8|), largest
+    sum |q| |k| scale per row) per sequence."""
     outs, mags, sizes = [], [], []
     cap = table_rows.shape[1] * k_pages.shape[2]
     for b, x in enumerate(q):
         h, n, d = x.shape
         length = min(max(int(lengths[b]), 0), cap)
-        k, there = sequence(k_pages, table_rows[b], length, False)
-        v, _ = sequence(v_pages, table_rows[b], length, True)
+        k, v = sequence(k_pages, table_rows[b], length, False), sequence(v_pages, table_rows[b], length, True)
+        a = v.abs() + sequence(v_pages, table_rows[b], length, True, about_middle(v_pages))
         group = h // k.shape[0]
         o, m, z = torch.zeros_like(x), torch.zeros_like(x), torch.zeros((h, n), dtype=torch.float64)
         for i in range(n):
             last = min(length, length - n + i + 1) if causal else length
-            keep = there[:max(last, 0)].nonzero().flatten()
-            if keep.numel() == 0:
+            if last <= 0:
                 continue
             for head in range(h):
-                kk, vv = k[head // group][keep], v[head // group][keep]
+                kk, vv, aa = k[head // group][:last], v[head // group][:last], a[head // group][:last]
                 logits = kk @ x[head, i] * scale
                 p = torch.softmax(logits, 0)
-                o[head, i], m[head, i] = p @ vv, p @ vv.abs()
+                o[head, i], m[head, i] = p @ vv, p @ aa
                 z[head, i] = (kk.abs() @ x[head, i].abs()).max() * abs(scale)
         outs.append(o)
         mags.append(m)
