@@ -337,6 +337,12 @@ KTT_B200_API int ktt_b200_merge_partials(
  * keys and values in a static cache; what follows serves models that turn part of a head or pairs of neighbours, contexts
  * stretched past what a model was trained on, training through the rotation, and caches in pages. */
 
+/* The dim / 2 (256 at most) frequencies f_i of rotary tables, in 64 bits, and what cosines and sines are multiplied by. scaling:
+ * 0: f_i = base^(-2 i / dim). 1: f_i / factor. 2: with base factor^(dim / (dim - 2)). 3: pairs that turn `fast` times or more
+ * within `original` positions keep f_i, those that turn `slow` times or less get f_i / factor, those between a mixture by
+ * their turns; cosines and sines times 0.1 ln(factor) + 1. Host only; launches nothing. */
+KTT_B200_API int ktt_b200_rotary_frequencies(double* frequencies, double* scale, int32_t dim, double base, int32_t scaling, double factor, double original, double fast, double slow);
+
 /* cos / sin [positions][pairs] fp32, rows dense: scale * cos(p f_i), scale * sin(p f_i) for positions p = 0, 1, ... and the
  * `pairs` (at most 256) frequencies f_i, which are read from host memory during the call. Angles are taken in 64 bits. */
 KTT_B200_API int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, int32_t pairs, const double* frequencies, double scale, void* stream);

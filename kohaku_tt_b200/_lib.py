@@ -60,6 +60,7 @@ EXPORTS = (
     "ktt_b200_decode_static",
     "ktt_b200_decode_append",
     "ktt_b200_merge_partials",
+    "ktt_b200_rotary_frequencies",
     "ktt_b200_rotary_table",
     "ktt_b200_rotary",
     "ktt_b200_paged_append",
@@ -429,6 +430,7 @@ def lib():
     handle.ktt_b200_selftest_wait_timeout.argtypes = [_ptr]
     handle.ktt_b200_probe_read.argtypes = [_ptr, ctypes.c_int64, _ptr, _ptr]
     handle.ktt_b200_merge_partials.argtypes = [_ptr, _ptr, _ptr, _ptr, _i64, _i32, _i32, _ptr]
+    handle.ktt_b200_rotary_frequencies.argtypes = [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(ctypes.c_double), _i32, ctypes.c_double, _i32] + [ctypes.c_double] * 4
     handle.ktt_b200_rotary_table.argtypes = [_ptr, _ptr, _i64, _i32, ctypes.POINTER(ctypes.c_double), ctypes.c_double, _ptr]
     handle.ktt_b200_rotary.argtypes = [ctypes.POINTER(RotaryArgs), _ptr]
     handle.ktt_b200_paged_append.argtypes = [ctypes.POINTER(AppendArgs), _ptr]

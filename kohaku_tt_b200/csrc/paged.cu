@@ -39,7 +39,7 @@ struct AppendParams {
     Pages c;
     Turn turn;
     int batch, rows, heads, kv_heads;
-    int groups;            // blocks of the grid's y that rotate queries; the keys' and the values' follow
+    int groups;            // blocks of kHeads queries' heads; those of the keys and of the values follow in the grid's y
     int64_t tokens;        // rows of all sequences
     const __nv_bfloat16* q;
     __nv_bfloat16* q_out;
@@ -99,78 +99,87 @@ __device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, uns
     }
 }
 
-// A thread has eight columns of one token and head: of a query, a key or a value. No thread leaves before the
-// group's shuffles.
-template <int D, int kBits, bool kFast>
+// A thread has eight columns of kHeads heads of one token: of queries, keys or values. Its rows are requested before it
+// knows where they go (a packed row's sequence takes a search). No thread leaves before the groups' shuffles.
+template <int D, int kBits, bool kFast, int kHeads>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-    const int chunk = threadIdx.x, col = chunk * 8, y = blockIdx.y;
+    const int chunk = threadIdx.x, col = chunk * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (p.lengths_out && blockIdx.x == 0 && y == 0) {
+    if (p.lengths_out && blockIdx.x == 0 && blockIdx.y == 0) {
         for (int b = threadIdx.y * blockDim.x + threadIdx.x; b < p.batch; b += blockDim.x * blockDim.y) {
             const int64_t more = p.cu ? max(p.cu[b + 1] - p.cu[b], 0) : p.rows, all = cached_keys(p.c, b) + more;
             p.lengths_out[b] = static_cast<int32_t>(all < p.c.cap ? all : p.c.cap);
         }
     }
-    int b = -1;
-    int64_t r = 0, in = 0;   // row of the operands, and of the sequence's new ones
-    if (n < p.tokens) {
-        if (p.cu) {
-            b = sequence_of(p.cu, p.batch, n);
-            r = n;
-            in = b >= 0 ? n - p.cu[b] : 0;
-        } else {
-            b = static_cast<int>(n / p.rows);
-            r = in = n - static_cast<int64_t>(b) * p.rows;
+    // What the block has: queries, keys or values.
+    const int y = blockIdx.y, kv = (p.kv_heads + kHeads - 1) / kHeads;
+    const int what = y < p.groups ? 0 : y < p.groups + kv ? 1 : 2;
+    const int h0 = (y - (what == 0 ? 0 : what == 1 ? p.groups : p.groups + kv)) * kHeads, heads = what == 0 ? p.heads : p.kv_heads;
+    const __nv_bfloat16* from = what == 0 ? p.q : what == 1 ? p.k : p.v;
+    const int64_t sb = what == 0 ? p.qs[0] : what == 1 ? p.ks[0] : p.vs[0], sh = what == 0 ? p.qs[1] : what == 1 ? p.ks[1] : p.vs[1];
+    const int64_t sr = what == 0 ? p.qs[2] : what == 1 ? p.ks[2] : p.vs[2];
+    const bool in_range = n < p.tokens;
+    int b = in_range && !p.cu ? static_cast<int>(n / p.rows) : 0;
+    int64_t r = !in_range ? 0 : p.cu ? n : n - static_cast<int64_t>(b) * p.rows;
+    from += (p.cu ? 0 : b * sb) + r * sr;
+    Eight<__nv_bfloat16> x[kHeads], other[kHeads];
+    const int partner = what == 2 || !p.turn.cos || p.turn.interleaved || col >= 2 * p.turn.half ? -1 : col < p.turn.half ? col + p.turn.half : col - p.turn.half;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        if (!in_range || h0 + i >= heads) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i].set(e, __float2bfloat16_rn(0.f));
+            continue;
+        }
+        const __nv_bfloat16* row = from + (h0 + i) * sh;
+        if (p.vec) x[i].load(row + col); else x[i].load_some(row + col, 8);
+        if (kFast && partner >= 0) {
+            if (p.vec) other[i].load(row + partner); else other[i].load_some(row + partner, 8);
         }
     }
-    const bool row = b >= 0;
-    const int64_t pos = row ? cached_keys(p.c, b) + in : 0;
-    const int64_t batch = p.cu || !row ? 0 : b;
-    Eight<__nv_bfloat16> x, other;
-    if (y < p.groups) {
-        if (!row) return;
-        Turned<kFast> turned;
-        turned.load(p.turn, pos, col);
-        const __nv_bfloat16* from = p.q + batch * p.qs[0] + y * p.qs[1] + r * p.qs[2];
-        if (p.vec) x.load(from + col); else x.load_some(from + col, 8);
-        if (kFast && turned.partner >= 0) {
-            if (p.vec) other.load(from + turned.partner); else other.load_some(from + turned.partner, 8);
+    int64_t in = r;          // the row's place among the sequence's new ones
+    bool row_there = in_range;
+    if (in_range && p.cu) {
+        b = sequence_of(p.cu, p.batch, n);
+        row_there = b >= 0;
+        b = row_there ? b : 0;
+        in = n - p.cu[b];
+    }
+    const int64_t pos = row_there ? cached_keys(p.c, b) + in : 0;
+    Turned<kFast> turned;
+    turned.count = 0;
+    if (what != 2 && row_there) turned.load(p.turn, pos, col);
+    if (what == 0) {
+        if (!row_there) return;
+        __nv_bfloat16* to = p.q_out + (p.cu ? 0 : b * p.qos[0]) + r * p.qos[2] + col;
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            if (h0 + i >= heads) break;
+            turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
+            if (p.vec) x[i].store(to + (h0 + i) * p.qos[1]); else x[i].store_some(to + (h0 + i) * p.qos[1], 8);
         }
-        turned.apply(p.turn, x, other, from, col);
-        __nv_bfloat16* to = p.q_out + batch * p.qos[0] + y * p.qos[1] + r * p.qos[2] + col;
-        if (p.vec) x.store(to); else x.store_some(to, 8);
         return;
     }
-    const bool value = y >= p.groups + p.kv_heads;
-    const int head = y - p.groups - (value ? p.kv_heads : 0);
     int64_t page = -1;
-    if (row && pos < p.c.cap) page = page_of(p.c, b, static_cast<int>(pos));
+    if (row_there && pos < p.c.cap) page = page_of(p.c, b, static_cast<int>(pos));
     const bool there = page >= 0;
-    if (there) {
-        const __nv_bfloat16* from = value ? p.v + batch * p.vs[0] + head * p.vs[1] + r * p.vs[2] : p.k + batch * p.ks[0] + head * p.ks[1] + r * p.ks[2];
-        if (p.vec) x.load(from + col); else x.load_some(from + col, 8);
-        if (!value) {
-            Turned<kFast> turned;
-            turned.load(p.turn, pos, col);
-            if (kFast && turned.partner >= 0) {
-                if (p.vec) other.load(from + turned.partner); else other.load_some(from + turned.partner, 8);
-            }
-            turned.apply(p.turn, x, other, from, col);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x.set(e, __float2bfloat16_rn(0.f));
-    }
     const int at = static_cast<int>(pos % p.c.page_size);
-    unsigned char* base = there ? (value ? p.c.v + page * p.c.vs[0] + head * p.c.vs[1] : p.c.k + page * p.c.ks[0] + head * p.c.ks[1]) : nullptr;
-    if constexpr (kBits == 16) {
-        if (there) x.store(reinterpret_cast<__nv_bfloat16*>(base + at * (value ? p.c.vs[2] : p.c.ks[2])) + col);
-    } else {
-        unsigned char* block = base + (there ? (at >> 4) * (9 * D) : 0);
-        if (value) put_four_bits<D, true>(x, block, at & 15, chunk, there);
-        else put_four_bits<D, false>(x, block, at & 15, chunk, there);
+    unsigned char* base = !there ? nullptr : what == 2 ? p.c.v + page * p.c.vs[0] : p.c.k + page * p.c.ks[0];
+    const int64_t head_stride = what == 2 ? p.c.vs[1] : p.c.ks[1];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+        if (h0 + i >= heads) break;
+        if (there && what == 1) turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
+        unsigned char* to = there ? base + (h0 + i) * head_stride : nullptr;
+        if constexpr (kBits == 16) {
+            if (there) x[i].store(reinterpret_cast<__nv_bfloat16*>(to + at * (what == 2 ? p.c.vs[2] : p.c.ks[2])) + col);
+        } else {
+            if (there) to += (at >> 4) * (9 * D);
+            if (what == 2) put_four_bits<D, true>(x[i], to, at & 15, chunk, there);
+            else put_four_bits<D, false>(x[i], to, at & 15, chunk, there);
+        }
     }
 }
 
@@ -247,12 +256,23 @@ int launch_dependent(void (*kernel)(Params), const Params& p, dim3 grid, dim3 bl
 }
 
 template <int D, int kBits>
-int launch_append(const AppendParams& p, cudaStream_t stream) {
+int launch_append(const AppendParams& given, cudaStream_t stream) {
+    AppendParams p = given;
     const dim3 block(D / 8, 256 / (D / 8));
     const int64_t blocks = (p.tokens + block.y - 1) / block.y;   // one at least: it writes the new lengths
-    const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), static_cast<unsigned>(p.groups + 2 * p.kv_heads));
-    if (turn_is_fast(p.turn)) return launch_dependent(append_kernel<D, kBits, true>, p, grid, block, stream, "paged_append launch");
-    return launch_dependent(append_kernel<D, kBits, false>, p, grid, block, stream, "paged_append launch");
+    auto go = [&](auto kernel, int per) {
+        p.groups = (p.heads + per - 1) / per;
+        const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), static_cast<unsigned>(p.groups + 2 * ((p.kv_heads + per - 1) / per)));
+        return launch_dependent(kernel, p, grid, block, stream, "paged_append launch");
+    };
+    const bool fast = turn_is_fast(p.turn);
+    // Four heads to a thread once that fills the GPU.
+    if (p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads) >= 4 * 148 * 2048) {
+        if (fast) return go(append_kernel<D, kBits, true, 4>, 4);
+        return go(append_kernel<D, kBits, false, 4>, 4);
+    }
+    if (fast) return go(append_kernel<D, kBits, true, 1>, 1);
+    return go(append_kernel<D, kBits, false, 1>, 1);
 }
 
 template <int D, int kBits>
@@ -300,7 +320,7 @@ extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream
     p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, 0};
     p.batch = a->batch;
     p.rows = a->rows;
-    p.heads = p.groups = a->heads;
+    p.heads = a->heads;
     p.kv_heads = a->cache.kv_heads;
     p.tokens = a->cu_seqlens ? a->rows : static_cast<int64_t>(a->batch) * a->rows;
     if (p.tokens > (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: at most 2^31 rows");

@@ -1,4 +1,6 @@
 // Rotary positions: the tables of cosines and sines, and the rotation of queries and keys (its gradient too).
+#include <cmath>
+
 #include "rotary.cuh"
 
 namespace ktt {
@@ -17,22 +19,50 @@ struct TableParams {
     int64_t positions;
     int pairs;
     float scale;
+    int vec;                   // both tables start at 16 bytes
     double turns[kMaxPairs];   // f_i / 2 pi
 };
 
+constexpr int kTableRows = 32;   // positions of a block
+
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
-    const int64_t n = p.positions * p.pairs, step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-    for (int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; at < n; at += step) {
-        const int64_t pos = at / p.pairs;
-        const int i = static_cast<int>(at - pos * p.pairs);
-        double turn = static_cast<double>(pos) * p.turns[i];
-        turn = 2.0 * (turn - rint(turn));
-        const float h = static_cast<float>(turn);
-        const float r = static_cast<float>(turn - static_cast<double>(h)) * 3.14159265358979f;
-        float s, c;
-        sincospif(h, &s, &c);
-        p.cos[at] = p.scale * fmaf(-r, s, c);
-        p.sin[at] = p.scale * fmaf(r, c, s);
+    __shared__ double turns[kMaxPairs];   // (a warp's threads want different ones: no matter for constant memory)
+    for (int i = threadIdx.x; i < p.pairs; i += 256) turns[i] = p.turns[i];
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTableRows;
+    const int rows = static_cast<int>(p.positions - first < kTableRows ? p.positions - first : kTableRows), n = rows * p.pairs;
+    float* cos = p.cos + first * p.pairs;
+    float* sin = p.sin + first * p.pairs;
+    for (int at = threadIdx.x * 4; at < n; at += 1024) {
+        int row = at / p.pairs, i = at - row * p.pairs;
+        float c[4], s[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            double turn = static_cast<double>(first + row) * turns[i];
+            turn = 2.0 * (turn - rint(turn));
+            const float h = static_cast<float>(turn);
+            const float r = static_cast<float>(turn - static_cast<double>(h)) * 3.14159265358979f;
+            sincospif(h, &s[e], &c[e]);
+            const float x = p.scale * fmaf(-r, s[e], c[e]);
+            s[e] = p.scale * fmaf(r, c[e], s[e]);
+            c[e] = x;
+            if (++i == p.pairs) {
+                i = 0;
+                ++row;
+            }
+        }
+        if (p.vec && at + 4 <= n) {
+            *reinterpret_cast<float4*>(cos + at) = make_float4(c[0], c[1], c[2], c[3]);
+            *reinterpret_cast<float4*>(sin + at) = make_float4(s[0], s[1], s[2], s[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (at + e < n) {
+                    cos[at + e] = c[e];
+                    sin[at + e] = s[e];
+                }
+            }
+        }
     }
 }
 
@@ -94,6 +124,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     }
 }
 
+constexpr int64_t kManyThreads = 4 * 148 * 2048;
+
 template <typename T>
 int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
     RotaryParams p = given;
@@ -114,6 +146,11 @@ int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
         cfg.numAttrs = 1;
         return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "rotary launch");
     };
+    // Four heads to a thread once that fills the GPU.
+    if (p.tokens * chunks * (p.heads[0] + p.heads[1]) >= kManyThreads) {
+        if (fast) return go(rotary_kernel<T, true, 4>, 4);
+        return go(rotary_kernel<T, false, 4>, 4);
+    }
     if (fast) return go(rotary_kernel<T, true, 1>, 1);
     return go(rotary_kernel<T, false, 1>, 1);
 }
@@ -122,6 +159,31 @@ int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
 }  // namespace ktt
 
 using namespace ktt;
+
+extern "C" int ktt_b200_rotary_frequencies(double* f, double* scale, int32_t dim, double base, int32_t scaling, double factor, double original, double fast, double slow) {
+    if (!f || !scale) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_frequencies: null pointer");
+    if (dim < 2 || dim % 2 || dim > 2 * kMaxPairs) return fail(KTT_B200_ERR_BAD_ARGUMENT, "dim must be even, from 2 to %d", 2 * kMaxPairs);
+    if (scaling < 0 || scaling > 3) return fail(KTT_B200_ERR_BAD_ARGUMENT, "unknown scaling");
+    if (!(base > 0) || !(factor > 0) || std::isinf(base) || std::isinf(factor)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "base and factor must be positive");
+    if (scaling == 2) {
+        if (dim < 4) return fail(KTT_B200_ERR_BAD_ARGUMENT, "scaling of the base needs two pairs");
+        base *= std::pow(factor, static_cast<double>(dim) / (dim - 2));
+    }
+    if (scaling == 3 && (!(original >= 1) || !(fast > slow) || !(factor >= 1))) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "scaling by parts needs the original context's length, fast > slow and a factor of 1 or more");
+    }
+    for (int i = 0; i < dim / 2; ++i) {
+        f[i] = std::pow(base, -2.0 * i / dim);
+        if (scaling == 1) f[i] /= factor;
+        if (scaling == 3) {
+            double keep = (original * f[i] * 0.15915494309189533577 - slow) / (fast - slow);
+            keep = keep < 0 ? 0 : (keep > 1 ? 1 : keep);
+            f[i] = (1 - keep) * f[i] / factor + keep * f[i];
+        }
+    }
+    *scale = scaling == 3 ? 0.1 * std::log(factor) + 1.0 : 1.0;
+    return 0;
+}
 
 extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, int32_t pairs, const double* frequencies, double scale, void* stream) {
     if (!cos || !sin || !frequencies) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: null pointer");
@@ -134,8 +196,8 @@ extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, 
     p.pairs = pairs;
     p.scale = static_cast<float>(scale);
     for (int i = 0; i < pairs; ++i) p.turns[i] = frequencies[i] * 0.15915494309189533577;   // 1 / 2 pi
-    const int64_t blocks = (positions * pairs + 255) / 256;
-    rotary_table_kernel<<<static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    p.vec = ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15) == 0;
+    rotary_table_kernel<<<static_cast<unsigned>((positions + kTableRows - 1) / kTableRows), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return check_cuda(cudaGetLastError(), "rotary_table launch");
 }
 

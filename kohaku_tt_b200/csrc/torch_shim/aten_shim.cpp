@@ -11,7 +11,7 @@
 // torch::Library objects), so that a process can take the overloads out again.
 //
 // The file is also a Python extension module (`ktt_b200_native`): the eager fast paths of
-// F.scaled_dot_product_attention, sdpa(key_lengths=), sdpa_varlen and decode_step. Small calls are
+// F.scaled_dot_product_attention, sdpa(key_lengths=), sdpa_varlen, decode_step, rotary and the paged cache. Small calls are
 // bound by the host: through torch's composite (its backend choice, the conversion of a bool
 // mask to a padded additive one by three kernels), Python custom operators, Python autograd
 // functions and ctypes argument blocks they took 13, 57, 150 and 50 us a call.
@@ -192,6 +192,10 @@ ZeroedPool& forward_pool() {
     return *pool;
 }
 ZeroedPool& decode_pool() {
+    static ZeroedPool* pool = new ZeroedPool;
+    return *pool;
+}
+ZeroedPool& paged_pool() {
     static ZeroedPool* pool = new ZeroedPool;
     return *pool;
 }
@@ -918,9 +922,407 @@ PyObject* py_sdpa_varlen(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---- rotary positions and the paged cache -------------------------------------------------------
+//
+// The checks are those of rotary.py and paged.py, whose functions word the refusals: a call that fails one
+// goes there. Through Python's checks and ctypes blocks these calls took 20 to 37 us.
+
+struct Turn {
+    Tensor cos, sin, positions;   // positions: undefined without
+    bool interleaved = false, inverse = false;
+};
+
+bool turn_ok(const Turn& x, const Tensor& like, int64_t dim) {
+    for (const Tensor* t : {&x.cos, &x.sin}) {
+        if (!plain(*t) || t->scalar_type() != at::kFloat || t->dim() != 2 || t->device() != like.device() || t->stride(1) != 1 || t->requires_grad()) return false;
+    }
+    return x.cos.sizes() == x.sin.sizes() && x.cos.stride(0) == x.sin.stride(0) && x.cos.size(0) > 0 && x.cos.size(1) > 0 && 2 * x.cos.size(1) <= dim;
+}
+
+Tensor like_operand(const Tensor& x) {
+    if (x.is_contiguous()) return empty_cuda(x.sizes(), x.scalar_type(), x);
+    Tensor out = at::empty_like(x);
+    return out.stride(-1) == 1 ? out : empty_cuda(x.sizes(), x.scalar_type(), x);
+}
+
+// (batch, head, row) strides of [B, H, S, D], or of packed [T, H, D].
+void operand_strides(int64_t* dst, const Tensor& t) {
+    const bool packed = t.dim() == 3;
+    dst[0] = packed ? 0 : t.stride(0);
+    dst[1] = t.stride(1);
+    dst[2] = packed ? t.stride(0) : t.stride(2);
+}
+
+// The rotation of q and of k where that is defined.
+torch::autograd::variable_list run_rotary(const Tensor& q_, const Tensor& k_, const Turn& x) {
+    c10::cuda::CUDAGuard device(q_.device());
+    const Tensor q = rows_contiguous(q_), k = k_.defined() ? rows_contiguous(k_) : k_;
+    torch::autograd::variable_list out{like_operand(q)};
+    if (k.defined()) out.push_back(like_operand(k));
+    const bool packed = q.dim() == 3;
+    ktt_b200_rotary_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.batch = packed ? 1 : static_cast<int32_t>(q.size(0));
+    a.rows = static_cast<int32_t>(packed ? q.size(0) : q.size(2));
+    a.heads = static_cast<int32_t>(q.size(1));
+    a.d = static_cast<int32_t>(q.size(-1));
+    a.pairs = static_cast<int32_t>(x.cos.size(1));
+    a.interleaved = x.interleaved;
+    a.inverse = x.inverse;
+    a.dtype = q.scalar_type() == at::kFloat ? KTT_B200_MASK_F32 : q.scalar_type() == at::kHalf ? KTT_B200_MASK_F16 : KTT_B200_MASK_BF16;
+    a.q = q.data_ptr();
+    a.q_out = out[0].data_ptr();
+    operand_strides(a.q_strides, q);
+    operand_strides(a.q_out_strides, out[0]);
+    if (k.defined()) {
+        a.kv_heads = static_cast<int32_t>(k.size(1));
+        a.k = k.data_ptr();
+        a.k_out = out[1].data_ptr();
+        operand_strides(a.k_strides, k);
+        operand_strides(a.k_out_strides, out[1]);
+    }
+    a.cos = x.cos.data_ptr<float>();
+    a.sin = x.sin.data_ptr<float>();
+    a.table_stride = x.cos.stride(0);
+    a.table_rows = x.cos.size(0);
+    if (x.positions.defined()) {
+        const Tensor& p = x.positions;
+        a.positions = p.data_ptr();
+        a.positions_are_64 = p.scalar_type() == at::kLong;
+        a.position_strides[0] = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
+        a.position_strides[1] = p.stride(-1);
+    }
+    raise_status(ktt_b200_rotary(&a, at::cuda::getCurrentCUDAStream()), "rotary");
+    return out;
+}
+
+// Its gradient is the inverse rotation, by the same node.
+struct Rotation : torch::autograd::Function<Rotation> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const c10::optional<Tensor>& k, const Turn& x) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        ctx->save_for_backward({x.cos, x.sin, x.positions});
+        ctx->saved_data["how"] = std::vector<int64_t>{x.interleaved, x.inverse, k.has_value()};
+        ctx->set_materialize_grads(false);
+        return run_rotary(q, k.has_value() ? *k : Tensor(), x);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const auto how = ctx->saved_data["how"].toIntVector();
+        const Turn x{saved[0], saved[1], saved[2], how[0] != 0, how[1] == 0};
+        const Tensor dq = grads[0], dk = how[2] ? grads[1] : Tensor();
+        const Tensor &first = dq.defined() ? dq : dk, &second = dq.defined() ? dk : dq;
+        if (!first.defined()) return {Tensor(), Tensor(), Tensor()};
+        torch::autograd::variable_list out;
+        if (at::GradMode::is_enabled()) {
+            out = apply(first, second.defined() ? c10::optional<Tensor>(second) : c10::nullopt, x);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView guard;
+            out = run_rotary(first, second, x);
+        }
+        if (!dq.defined()) return {Tensor(), out[0], Tensor()};
+        return {out[0], dk.defined() ? out[1] : Tensor(), Tensor()};
+    }
+};
+
+// rotary(q, k or None, cos, sin, positions or None, interleaved): (q', k' or None), or None.
+PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *k = nullptr, *cos, *sin, *pos = nullptr;
+    if (n != 6 || !callable_now() || !(q = tensor_of(args[0])) || (args[1] != Py_None && !(k = tensor_of(args[1]))) || !(cos = tensor_of(args[2])) ||
+        !(sin = tensor_of(args[3])) || (args[4] != Py_None && !(pos = tensor_of(args[4])))) Py_RETURN_NONE;
+    const bool packed = q->dim() == 3;
+    if (!plain(*q) || (!packed && q->dim() != 4) || q->numel() == 0) Py_RETURN_NONE;
+    if (q->scalar_type() != at::kBFloat16 && q->scalar_type() != at::kHalf && q->scalar_type() != at::kFloat) Py_RETURN_NONE;
+    const int64_t rows = packed ? q->size(0) : q->size(2);
+    if (rows > INT32_MAX || q->size(0) > INT32_MAX || q->size(1) > 65535 || (k && k->dim() > 1 && k->size(1) > 65535)) Py_RETURN_NONE;
+    if (k) {
+        if (!plain(*k) || k->dim() != q->dim() || k->numel() == 0 || k->scalar_type() != q->scalar_type() || k->device() != q->device() || k->size(-1) != q->size(-1) ||
+            k->size(0) != q->size(0) || (!packed && k->size(2) != rows)) Py_RETURN_NONE;
+    }
+    Turn x{*cos, *sin, pos ? *pos : Tensor(), args[5] == Py_True, false};
+    if (!turn_ok(x, *q, q->size(-1))) Py_RETURN_NONE;
+    if (pos) {
+        if (!plain(*pos) || pos->device() != q->device() || (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)) Py_RETURN_NONE;
+        const bool flat = pos->dim() == 1 && pos->size(0) == rows;
+        if (!flat && (packed || pos->dim() != 2 || pos->size(1) != rows || (pos->size(0) != 1 && pos->size(0) != q->size(0)))) Py_RETURN_NONE;
+    } else if (cos->size(0) < rows) {
+        Py_RETURN_NONE;
+    }
+    torch::autograd::variable_list out;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        const Tensor second = k ? *k : Tensor();
+        if (at::GradMode::is_enabled() && (q->requires_grad() || (k && k->requires_grad()))) {
+            out = Rotation::apply(*q, k ? c10::optional<Tensor>(second) : c10::nullopt, x);
+        } else {
+            at::AutoDispatchBelowADInplaceOrView guard;
+            out = run_rotary(*q, second, x);
+        }
+    });
+    if (!done) Py_RETURN_NONE;
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(out[0]));
+    if (k) {
+        PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(out[1]));
+    } else {
+        Py_INCREF(Py_None);
+        PyTuple_SET_ITEM(pair, 1, Py_None);
+    }
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// rotary_table(positions, dim, base, scaling, factor, original, fast, slow, device index): (cos, sin).
+PyObject* py_rotary_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 9) Py_RETURN_NONE;
+    const int64_t positions = PyLong_AsLongLong(args[0]), dim = PyLong_AsLongLong(args[1]), scaling = PyLong_AsLongLong(args[3]), index = PyLong_AsLongLong(args[8]);
+    const double base = PyFloat_AsDouble(args[2]), factor = PyFloat_AsDouble(args[4]), original = PyFloat_AsDouble(args[5]), fast = PyFloat_AsDouble(args[6]),
+                 slow = PyFloat_AsDouble(args[7]);
+    if (PyErr_Occurred()) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    Tensor cos, sin;
+    {
+        pybind11::gil_scoped_release release;
+        double f[256], scale = 1.0;
+        raise_status(dim < 0 || dim > 512 ? ktt_b200_rotary_frequencies(f, &scale, 0, base, 0, factor, original, fast, slow)
+                                          : ktt_b200_rotary_frequencies(f, &scale, static_cast<int32_t>(dim), base, static_cast<int32_t>(scaling), factor, original, fast, slow),
+                     "rotary_table");
+        TORCH_CHECK_VALUE(positions > 0, "kohaku_tt_b200.rotary_table: one position at least");
+        const c10::Device device(c10::kCUDA, static_cast<c10::DeviceIndex>(index));
+        c10::cuda::CUDAGuard guard(device);
+        cos = at::detail::empty_cuda({positions, dim / 2}, at::kFloat, device, c10::nullopt);
+        sin = at::detail::empty_cuda({positions, dim / 2}, at::kFloat, device, c10::nullopt);
+        raise_status(ktt_b200_rotary_table(cos.data_ptr<float>(), sin.data_ptr<float>(), positions, static_cast<int32_t>(dim / 2), f, scale, at::cuda::getCurrentCUDAStream()),
+                     "rotary_table");
+    }
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(cos));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(sin));
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// A cache's argument block, its checks those of paged._pages.
+struct Cache {
+    ktt_b200_pages c;
+    int64_t dim = 0, batch = 0, cap = 0;
+};
+bool cache_of(Cache& x, PyObject* const* args, PyObject* max_k) {   // k_pages, v_pages, block_table, lengths
+    const Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+        if (!(t[i] = tensor_of(args[i])) || !plain(*t[i])) return false;
+    }
+    const Tensor &k = *t[0], &v = *t[1], &table = *t[2], &lengths = *t[3];
+    if (k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || k.device() != v.device() || k.numel() == 0) return false;
+    const bool four = k.scalar_type() == at::kByte;
+    if (four ? k.size(3) % 9 != 0 : k.scalar_type() != at::kBFloat16) return false;
+    x.dim = four ? k.size(3) / 9 * 16 : k.size(3);
+    for (const Tensor* p : {&k, &v}) {
+        if (p->stride(3) != 1 || (four && p->size(2) > 1 && p->stride(2) != p->size(3))) return false;
+    }
+    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(1) < 1 || table.stride(1) != 1 || table.device() != k.device()) return false;
+    if (!int32_vector(lengths, k, table.size(0))) return false;
+    x.batch = table.size(0);
+    x.cap = table.size(1) * k.size(2);
+    if (max_k != Py_None) {
+        const int64_t most = PyLong_AsLongLong(max_k);
+        if (PyErr_Occurred()) PyErr_Clear();
+        if (most < 1) return false;
+        x.cap = std::min(x.cap, most);
+    }
+    if (x.cap > (1 << 30) || x.batch > INT32_MAX || x.batch < 1) return false;
+    ktt_b200_pages& c = x.c;
+    std::memset(&c, 0, sizeof(c));
+    c.k = k.data_ptr();
+    c.v = v.data_ptr();
+    c.bits = four ? 4 : 16;
+    c.page_size = static_cast<int32_t>(k.size(2));
+    c.kv_heads = static_cast<int32_t>(k.size(1));
+    c.table_width = static_cast<int32_t>(table.size(1));
+    c.pages = k.size(0);
+    set3(c.k_strides, k);
+    set3(c.v_strides, v);
+    c.block_table = table.data_ptr<int32_t>();
+    c.table_stride = table.stride(0);
+    c.lengths = lengths.data_ptr<int32_t>();
+    c.max_keys = static_cast<int32_t>(x.cap);
+    return true;
+}
+
+// bf16 [B, heads, S, D], or packed [T, heads, D], that goes with a cache; heads < 0: any.
+bool cache_operand(const Tensor& t, const Cache& x, const Tensor& pages, bool packed, int64_t rows, int64_t heads) {
+    if (!plain(t) || t.scalar_type() != at::kBFloat16 || t.device() != pages.device() || t.dim() != (packed ? 3 : 4) || t.stride(-1) != 1 || t.size(-1) != x.dim) return false;
+    if (rows > INT32_MAX || t.size(1) > 65535 || (packed ? t.size(0) : t.size(2)) != rows || (!packed && t.size(0) != x.batch) || t.size(1) < 1) return false;
+    return heads < 0 || t.size(1) == heads;
+}
+
+// paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq (on the device), lengths_out):
+// the rotated queries or None; NotImplemented when the call is not one for the fast path.
+PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *k, *v, *q = nullptr, *cu = nullptr, *len_out = nullptr;
+    Cache x;
+    if (n != 12 || !callable_now() || !(k = tensor_of(args[0])) || !(v = tensor_of(args[1])) || !cache_of(x, args + 2, Py_None)) Py_RETURN_NOTIMPLEMENTED;
+    const Tensor& pages = *tensor_of(args[2]);
+    const bool packed = args[10] != Py_None, turns = args[6] != Py_None;
+    if (packed && (!(cu = tensor_of(args[10])) || !int32_vector(*cu, pages, x.batch + 1))) Py_RETURN_NOTIMPLEMENTED;
+    if (k->dim() != (packed ? 3 : 4) || k->numel() == 0) Py_RETURN_NOTIMPLEMENTED;
+    const int64_t rows = packed ? k->size(0) : k->size(2);
+    if (!cache_operand(*k, x, pages, packed, rows, x.c.kv_heads) || !cache_operand(*v, x, pages, packed, rows, x.c.kv_heads)) Py_RETURN_NOTIMPLEMENTED;
+    if (args[8] != Py_None && (!(q = tensor_of(args[8])) || !cache_operand(*q, x, pages, packed, rows, -1))) Py_RETURN_NOTIMPLEMENTED;
+    if (args[11] != Py_None && (!(len_out = tensor_of(args[11])) || !int32_vector(*len_out, pages, x.batch))) Py_RETURN_NOTIMPLEMENTED;
+    Turn turn;
+    if (turns != (args[7] != Py_None)) Py_RETURN_NOTIMPLEMENTED;
+    if (turns) {
+        const Tensor *cos = tensor_of(args[6]), *sin = tensor_of(args[7]);
+        if (!cos || !sin) Py_RETURN_NOTIMPLEMENTED;
+        turn = Turn{*cos, *sin, Tensor(), args[9] == Py_True, false};
+        if (!turn_ok(turn, pages, x.dim) || cos->size(0) < x.cap) Py_RETURN_NOTIMPLEMENTED;
+    }
+    Tensor out;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        c10::cuda::CUDAGuard device(pages.device());
+        ktt_b200_append_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.cache = x.c;
+        a.batch = static_cast<int32_t>(x.batch);
+        a.rows = static_cast<int32_t>(rows);
+        a.d = static_cast<int32_t>(x.dim);
+        a.k = k->data_ptr();
+        a.v = v->data_ptr();
+        operand_strides(a.k_strides, *k);
+        operand_strides(a.v_strides, *v);
+        if (q) {
+            out = like_operand(*q);
+            a.heads = static_cast<int32_t>(q->size(1));
+            a.q = q->data_ptr();
+            a.q_out = out.data_ptr();
+            operand_strides(a.q_strides, *q);
+            operand_strides(a.q_out_strides, out);
+        }
+        if (turns) {
+            a.pairs = static_cast<int32_t>(turn.cos.size(1));
+            a.interleaved = turn.interleaved;
+            a.cos = turn.cos.data_ptr<float>();
+            a.sin = turn.sin.data_ptr<float>();
+            a.table_stride = turn.cos.stride(0);
+            a.table_rows = turn.cos.size(0);
+        }
+        if (cu) a.cu_seqlens = cu->data_ptr<int32_t>();
+        if (len_out) a.lengths_out = len_out->data_ptr<int32_t>();
+        raise_status(ktt_b200_paged_append(&a, at::cuda::getCurrentCUDAStream()), "paged_append");
+    });
+    if (!done) Py_RETURN_NOTIMPLEMENTED;
+    if (!q) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_read(k_pages, v_pages, block_table, lengths, max_k): (k, v), or None.
+PyObject* py_paged_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Cache x;
+    if (n != 5 || !callable_now() || !cache_of(x, args, args[4])) Py_RETURN_NONE;
+    const Tensor& pages = *tensor_of(args[0]);
+    Tensor k, v;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        c10::cuda::CUDAGuard device(pages.device());
+        const std::vector<int64_t> sizes{x.batch, x.c.kv_heads, x.cap, x.dim};
+        k = empty_cuda(sizes, at::kBFloat16, pages);
+        v = empty_cuda(sizes, at::kBFloat16, pages);
+        ktt_b200_read_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.cache = x.c;
+        a.batch = static_cast<int32_t>(x.batch);
+        a.rows = static_cast<int32_t>(x.cap);
+        a.d = static_cast<int32_t>(x.dim);
+        a.k_out = k.data_ptr();
+        a.v_out = v.data_ptr();
+        set3(a.k_strides, k);
+        set3(a.v_strides, v);
+        raise_status(ktt_b200_paged_read(&a, at::cuda::getCurrentCUDAStream()), "paged_read");
+    });
+    if (!done) Py_RETURN_NONE;
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(k)));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(v)));
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
+// sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal, scale, cu_seq_q (on the device), max_q, max_k): the output,
+// or None.
+PyObject* py_sdpa_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *cu = nullptr;
+    Cache x;
+    c10::optional<double> scale;
+    if (n != 10 || !callable_now() || !(q = tensor_of(args[0])) || !scale_of(args[6], scale) || !cache_of(x, args + 1, args[9])) Py_RETURN_NONE;
+    const Tensor& pages = *tensor_of(args[1]);
+    const bool packed = args[7] != Py_None;
+    if (packed && (!(cu = tensor_of(args[7])) || !int32_vector(*cu, pages, x.batch + 1))) Py_RETURN_NONE;
+    if (q->dim() != (packed ? 3 : 4) || q->numel() == 0) Py_RETURN_NONE;
+    const int64_t rows = packed ? q->size(0) : q->size(2);
+    if (!cache_operand(*q, x, pages, packed, rows, -1) || (reinterpret_cast<uintptr_t>(q->data_ptr()) & 15)) Py_RETURN_NONE;
+    for (int64_t i = 0; i + 1 < q->dim(); ++i) {
+        if (q->stride(i) % 8) Py_RETURN_NONE;
+    }
+    int64_t longest = rows;
+    if (packed && args[8] != Py_None) {
+        longest = PyLong_AsLongLong(args[8]);
+        if (PyErr_Occurred()) PyErr_Clear();
+        if (longest < 1) Py_RETURN_NONE;
+        longest = std::min(longest, rows);
+    }
+    Tensor out;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        c10::cuda::CUDAGuard device(pages.device());
+        cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+        out = packed ? empty_cuda(q->sizes(), at::kBFloat16, *q) : out_like_query(*q, x.dim);
+        ktt_b200_paged_sdpa_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.cache = x.c;
+        a.batch = static_cast<int32_t>(x.batch);
+        a.heads = static_cast<int32_t>(q->size(1));
+        a.sq = static_cast<int32_t>(longest);
+        a.d = static_cast<int32_t>(x.dim);
+        a.total_q = packed ? rows : 0;
+        a.causal = args[5] == Py_True;
+        a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(x.dim)));
+        a.q = q->data_ptr();
+        a.out = out.data_ptr();
+        operand_strides(a.q_strides, *q);
+        operand_strides(a.out_strides, out);
+        if (cu) a.cu_seqlens_q = cu->data_ptr<int32_t>();
+        const int64_t need = ktt_b200_paged_sdpa_workspace(&a);
+        if (need < 0) raise_status(KTT_B200_ERR_UNSUPPORTED, "sdpa_paged");
+        const Tensor counters = paged_pool().get(4096, 4096, *q, stream), work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
+        a.counters = counters.data_ptr();
+        a.workspace = work.data_ptr();
+        a.workspace_bytes = need;
+        raise_status(ktt_b200_paged_sdpa(&a, stream), "sdpa_paged");
+    });
+    if (!done) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_drop_workspaces(PyObject*, PyObject*) {
     forward_pool().clear();
     decode_pool().clear();
+    paged_pool().clear();
     Py_RETURN_NONE;
 }
 
@@ -928,6 +1330,11 @@ PyMethodDef g_methods[] = {
     {"sdpa_lengths", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_sdpa_lengths)), METH_FASTCALL, nullptr},
     {"decode_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_decode_step)), METH_FASTCALL, nullptr},
     {"sdpa_varlen", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_sdpa_varlen)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rotary)), METH_FASTCALL, nullptr},
+    {"rotary_table", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rotary_table)), METH_FASTCALL, nullptr},
+    {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
+    {"paged_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_read)), METH_FASTCALL, nullptr},
+    {"sdpa_paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_sdpa_paged)), METH_FASTCALL, nullptr},
     {"drop_workspaces", py_drop_workspaces, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "ktt_b200_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -73,10 +73,16 @@ def _offsets(cu, batch, tokens, device, what):
 
 
 def _operand(t, name, heads, like, batch, rows, dim, packed, what):
+    if rows >= 2 ** 31 or heads > 65535:
+        raise _lib.UnsupportedAttention(f"kohaku_tt_b200.{what}: more rows or heads than the kernels count")
     shape = (rows, heads, dim) if packed else (batch, heads, rows, dim)
     if tuple(t.shape) != shape or t.dtype != torch.bfloat16 or t.device != like.device:
         raise ValueError(f"kohaku_tt_b200.{what}: {name} must be bf16 {list(shape)} on the pages' device, got {t.dtype} {list(t.shape)}")
     return ops._rows_contiguous(t)
+
+
+def _on_device(cu):
+    return cu is None or (isinstance(cu, torch.Tensor) and cu.is_cuda)
 
 
 def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out):
@@ -249,9 +255,16 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     q: bf16 [B, H, S, D] or [T, H, D]; returned rotated (None without q).
     Pages of 4 bits (paged_cache(bits=4)) hold each 64 channels of a row as codes 0 to 15 of
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
+    interleaved = bool(interleaved)
     if torch.compiler.is_compiling():
-        out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, bool(interleaved), cu_seq, lengths_out)
+        out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
         return out if q is not None else None
+    # Eager calls on plain CUDA tensors are served by C++ in one step.
+    eager = _lib.native()
+    if eager and _on_device(cu_seq):
+        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+        if out is not NotImplemented:
+            return out
     with torch.no_grad():
         return _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
 
@@ -262,6 +275,11 @@ def paged_read(k_pages, v_pages, block_table, lengths, max_k=None):
     capacity: block_table's, or max_k where that is less."""
     if torch.compiler.is_compiling():
         return torch.ops.ktt_b200._paged_read(k_pages, v_pages, block_table, lengths, max_k)
+    eager = _lib.native()
+    if eager:
+        out = eager.paged_read(k_pages, v_pages, block_table, lengths, max_k)
+        if out is not None:
+            return out
     with torch.no_grad():
         return _read(k_pages, v_pages, block_table, lengths, max_k)
 
@@ -280,5 +298,10 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
     causal = bool(is_causal)
     if torch.compiler.is_compiling():
         return torch.ops.ktt_b200._sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
+    eager = _lib.native()
+    if eager and _on_device(cu_seq_q):
+        out = eager.sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
+        if out is not None:
+            return out
     with torch.no_grad():
         return _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)

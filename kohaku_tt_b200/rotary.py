@@ -4,7 +4,6 @@ csrc/aten/nn/aten_fused.cpp:30-43, turns whole heads in the half layout; decode_
 that in its one launch.)"""
 
 import ctypes
-import math
 
 import torch
 
@@ -17,31 +16,16 @@ SCALINGS = (None, "linear", "base", "parts")
 def rotary_frequencies(dim, base=10000.0, scaling=None, factor=1.0, original=None, fast=32.0, slow=1.0):
     """(frequencies, scale): the angle per position of each of dim / 2 pairs as Python floats, and
     what the cosines and sines are multiplied by. See rotary_table."""
-    if dim < 2 or dim % 2 or dim > 512:
-        raise ValueError(f"kohaku_tt_b200.rotary_table: dim must be even, from 2 to 512, got {dim}")
-    if scaling not in SCALINGS:
-        raise ValueError(f"kohaku_tt_b200.rotary_table: scaling must be one of {SCALINGS}, got {scaling!r}")
-    if not (base > 0 and factor > 0 and math.isfinite(base) and math.isfinite(factor)):
-        raise ValueError("kohaku_tt_b200.rotary_table: base and factor must be positive")
-    if scaling == "base":
-        if dim < 4:
-            raise ValueError("kohaku_tt_b200.rotary_table: scaling 'base' needs two pairs")
-        base = base * factor ** (dim / (dim - 2))
-    f = [base ** (-i / dim) for i in range(0, dim, 2)]
-    if scaling == "linear":
-        f = [x / factor for x in f]
-    if scaling != "parts":
-        return f, 1.0
-    if original is None or original < 1 or not fast > slow:
-        raise ValueError("kohaku_tt_b200.rotary_table: scaling 'parts' needs the original context's length, and fast > slow")
-    if factor < 1:
-        raise ValueError("kohaku_tt_b200.rotary_table: scaling 'parts' stretches: factor must be 1 or more")
+    f, m = (ctypes.c_double * 256)(), ctypes.c_double()
+    _lib.check(_lib.lib().ktt_b200_rotary_frequencies(f, ctypes.byref(m), int(dim), base, _scaling(scaling), factor,
+                                                      0.0 if original is None else original, fast, slow), "rotary_table")
+    return f[:dim // 2], m.value
 
-    def part(x):
-        keep = min(1.0, max(0.0, (original * x / (2 * math.pi) - slow) / (fast - slow)))
-        return (1 - keep) * x / factor + keep * x
 
-    return [part(x) for x in f], 0.1 * math.log(factor) + 1.0
+def _scaling(name):
+    if name not in SCALINGS:
+        raise ValueError(f"kohaku_tt_b200.rotary_table: scaling must be one of {SCALINGS}, got {name!r}")
+    return SCALINGS.index(name)
 
 
 def rotary_table(positions, dim, base=10000.0, scaling=None, factor=1.0, original=None, fast=32.0, slow=1.0,
@@ -55,13 +39,19 @@ def rotary_table(positions, dim, base=10000.0, scaling=None, factor=1.0, origina
       "parts"   pairs that turn more than `fast` times within the `original` context keep their
                 frequency, those that turn less than `slow` times get f_i / factor, those between a
                 mixture; cos and sin are multiplied by 0.1 ln(factor) + 1."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise RuntimeError("kohaku_tt_b200: rotary tables are made on CUDA devices only; there is no CPU fallback")
+    eager = not torch.compiler.is_compiling() and _lib.native()
+    if eager:
+        index = torch.cuda.current_device() if device.index is None else device.index
+        out = eager.rotary_table(positions, dim, base, _scaling(scaling), factor, 0.0 if original is None else original, fast, slow, index)
+        if out is not None:
+            return out
     f, scale = rotary_frequencies(dim, base, scaling, factor, original, fast, slow)
     positions = int(positions)
     if positions < 1:
         raise ValueError("kohaku_tt_b200.rotary_table: one position at least")
-    device = torch.device(device)
-    if device.type != "cuda":
-        raise RuntimeError("kohaku_tt_b200: rotary tables are made on CUDA devices only; there is no CPU fallback")
     pairs = len(f)
     with torch.cuda.device(device):
         cos = torch.empty((positions, pairs), dtype=torch.float32, device=device)
@@ -108,6 +98,8 @@ def _check(q, k, cos, sin, positions):
         same = x.shape[-1] == q.shape[-1] and (x.shape[0] == q.shape[0] if x.dim() == 3 else x.shape[0] == q.shape[0] and x.shape[2] == q.shape[2])
         if not same:
             raise ValueError("kohaku_tt_b200.rotary: q and k differ in more than their heads")
+    if max(q.shape[:-1]) >= 2 ** 31 or q.shape[1] > 65535 or (k is not None and k.shape[1] > 65535):
+        raise _lib.UnsupportedAttention("kohaku_tt_b200.rotary: more rows or heads than the kernel counts")
     check_tables(cos, sin, q, q.shape[-1], what)
     rows = q.shape[0] if q.dim() == 3 else q.shape[2]
     if positions is None:
@@ -215,8 +207,14 @@ def rotary(q, k, cos, sin, positions=None, interleaved=False):
     in fp32, products and sum rounded one by one, the result once to q's type (bf16, fp16 or fp32).
     positions: int32 or int64 on the device, [S] or [B, S] (packed [T]), read by the kernel and clamped to
     the tables' rows; without them row s has position s."""
-    _check(q, k, cos, sin, positions)
     interleaved = bool(interleaved)
+    # Eager calls on plain CUDA tensors are served by C++ in one step (None: not such a call).
+    eager = not torch.compiler.is_compiling() and _lib.native()
+    if eager:
+        out = eager.rotary(q, k, cos, sin, positions, interleaved)
+        if out is not None:
+            return out
+    _check(q, k, cos, sin, positions)
     if torch.compiler.is_compiling():
         out = torch.ops.ktt_b200._rotary(q, k, cos, sin, positions, interleaved, False)
         return (out[0], None if k is None else out[1])
