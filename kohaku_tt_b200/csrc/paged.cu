@@ -63,46 +63,51 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int64_t
 }
 
 // Eight columns of one token in the cache's 4 bits. The 8 threads of a group of 64 columns are neighbours in a warp and
-// all arrive here; `there`: the row has a place. Sums and quotients round as fp32's own do: the codes are the
-// definition's to the bit.
+// all arrive here; `there`: the row has a place. The codes are those of (x - least) / step rounded as fp32 does, to the
+// bit: the quotient is the product with 1 / step, corrected by its remainder (Markstein's theorem: with 1 / step correctly
+// rounded and the remainder exact, the corrected quotient is the correctly rounded one), 5 operations for a column where a
+// division takes some 12; steps so small or large that the remainder could leave fp32's range are divided by.
 template <int D, bool kValue>
 __device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, unsigned char* block, int token, int chunk, bool there) {
-    float v[8], least = INFINITY, most = -INFINITY;
-    bool nan = false;
+    const __nv_bfloat162* pair = reinterpret_cast<const __nv_bfloat162*>(x.raw);
+    const __nv_bfloat162 lo = __hmin2_nan(__hmin2_nan(pair[0], pair[1]), __hmin2_nan(pair[2], pair[3]));
+    const __nv_bfloat162 hi = __hmax2_nan(__hmax2_nan(pair[0], pair[1]), __hmax2_nan(pair[2], pair[3]));
+    // (least, -most): a NaN anywhere makes both NaN.
+    __nv_bfloat162 ends = __halves2bfloat162(__hmin_nan(__low2bfloat16(lo), __high2bfloat16(lo)), __hneg(__hmax_nan(__low2bfloat16(hi), __high2bfloat16(hi))));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        v[e] = to_f32(x.get(e));
-        nan |= v[e] != v[e];
-        least = fminf(least, v[e]);
-        most = fmaxf(most, v[e]);
-    }
-#pragma unroll
-    for (int off = 1; off < 8; off <<= 1) {
-        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, off));
-        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-        nan |= __shfl_xor_sync(0xffffffffu, static_cast<int>(nan), off) != 0;
-    }
-    const __nv_bfloat16 step = __float2bfloat16_rn(nan ? NAN : __fmul_rn(__fsub_rn(most, least), 1.f / 15.f));
+    for (int off = 1; off < 8; off <<= 1) ends = __hmin2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, off));
+    const float least = __low2float(ends);
+    const __nv_bfloat16 step = __float2bfloat16_rn(__fmul_rn(__fsub_rn(-__high2float(ends), least), 1.f / 15.f));
     const float s = __bfloat162float(step);
     uint32_t word = 0;
+    if (s >= 0x1p-100f && s <= 0x1p100f) {
+        const float inv = __frcp_rn(s);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float c = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(v[e], least), s)), 0.f), 15.f) : 0.f;
-        word |= static_cast<uint32_t>(c) << (4 * ((e >> 1) + 4 * (e & 1)));
+        for (int e = 0; e < 8; ++e) {
+            const float d = __fsub_rn(to_f32(x.get(e)), least), q = d * inv;
+            const float t = fmaf(fmaf(-q, s, d), inv, q);
+            // To the nearest whole number in the low bits, ties to even; t is at most 15 (1 + 2^-8).
+            word |= (__float_as_uint(t + 8388608.f) & 15u) << (4 * ((e >> 1) + 4 * (e & 1)));
+        }
+    } else if (s > 0.f) {
+#pragma unroll 1
+        for (int e = 0; e < 8; ++e) {
+            const float c = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(to_f32(x.get(e)), least), s)), 0.f), 15.f);
+            word |= static_cast<uint32_t>(c) << (4 * ((e >> 1) + 4 * (e & 1)));
+        }
     }
     if (!there) return;
     uint32_t* to = reinterpret_cast<uint32_t*>(block);
     to[kValue ? value_word<D>(token, chunk) : key_word<D>(token, chunk)] = word;
     if (chunk % 8 == 0) {
-        const __nv_bfloat16 low = nan ? __float2bfloat16_rn(NAN) : __float2bfloat16_rn(least);
-        to[step_word<D>(token, chunk / 8)] = static_cast<uint32_t>(__bfloat16_as_ushort(step)) | static_cast<uint32_t>(__bfloat16_as_ushort(low)) << 16;
+        to[step_word<D>(token, chunk / 8)] = static_cast<uint32_t>(__bfloat16_as_ushort(step)) | static_cast<uint32_t>(__bfloat16_as_ushort(__low2bfloat16(ends))) << 16;
     }
 }
 
 // A thread has eight columns of kHeads heads of one token: of queries, keys or values. Its rows are requested before it
 // knows where they go (a packed row's sequence takes a search). No thread leaves before the groups' shuffles.
 template <int D, int kBits, bool kFast, int kHeads>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const __grid_constant__ AppendParams p) {
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const int chunk = threadIdx.x, col = chunk * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -121,7 +126,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
     const int64_t sb = what == 0 ? p.qs[0] : what == 1 ? p.ks[0] : p.vs[0], sh = what == 0 ? p.qs[1] : what == 1 ? p.ks[1] : p.vs[1];
     const int64_t sr = what == 0 ? p.qs[2] : what == 1 ? p.ks[2] : p.vs[2];
     const bool in_range = n < p.tokens;
-    int b = in_range && !p.cu ? static_cast<int>(n / p.rows) : 0;
+    int b = in_range && !p.cu ? static_cast<int>(static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows)) : 0;   // (2^31 tokens at most)
     int64_t r = !in_range ? 0 : p.cu ? n : n - static_cast<int64_t>(b) * p.rows;
     from += (p.cu ? 0 : b * sb) + r * sr;
     Eight<__nv_bfloat16> x[kHeads], other[kHeads];
@@ -134,10 +139,8 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
             continue;
         }
         const __nv_bfloat16* row = from + (h0 + i) * sh;
-        if (p.vec) x[i].load(row + col); else x[i].load_some(row + col, 8);
-        if (kFast && partner >= 0) {
-            if (p.vec) other[i].load(row + partner); else other[i].load_some(row + partner, 8);
-        }
+        if (kFast || p.vec) x[i].load(row + col); else x[i].load_some(row + col, 8);
+        if (kFast && partner >= 0) other[i].load(row + partner);
     }
     int64_t in = r;          // the row's place among the sequence's new ones
     bool row_there = in_range;
@@ -158,14 +161,14 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
         for (int i = 0; i < kHeads; ++i) {
             if (h0 + i >= heads) break;
             turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
-            if (p.vec) x[i].store(to + (h0 + i) * p.qos[1]); else x[i].store_some(to + (h0 + i) * p.qos[1], 8);
+            if (kFast || p.vec) x[i].store(to + (h0 + i) * p.qos[1]); else x[i].store_some(to + (h0 + i) * p.qos[1], 8);
         }
         return;
     }
     int64_t page = -1;
     if (row_there && pos < p.c.cap) page = page_of(p.c, b, static_cast<int>(pos));
     const bool there = page >= 0;
-    const int at = static_cast<int>(pos % p.c.page_size);
+    const int at = there ? static_cast<int>(pos) % p.c.page_size : 0;
     unsigned char* base = !there ? nullptr : what == 2 ? p.c.v + page * p.c.vs[0] : p.c.k + page * p.c.ks[0];
     const int64_t head_stride = what == 2 ? p.c.vs[1] : p.c.ks[1];
 #pragma unroll
@@ -192,53 +195,83 @@ struct ReadParams {
     int64_t ks[3], vs[3];
 };
 
-template <int D, bool kValue>
-__device__ __forceinline__ Eight<__nv_bfloat16> get_four_bits(const unsigned char* block, int token, int chunk) {
-    const uint32_t* from = reinterpret_cast<const uint32_t*>(block);
-    const uint32_t word = from[kValue ? value_word<D>(token, chunk) : key_word<D>(token, chunk)], pair = from[step_word<D>(token, chunk / 8)];
+// What eight codes are worth.
+__device__ __forceinline__ Eight<__nv_bfloat16> of_four_bits(uint32_t word, uint32_t pair) {
+    const float step = step_of(pair), least = least_of(pair);
     Eight<__nv_bfloat16> x;
+    uint32_t* to = reinterpret_cast<uint32_t*>(x.raw);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        // (step * code is exact in fp32: one rounding to fp32, one to bf16.)
-        x.set(e, __float2bfloat16_rn(fmaf(step_of(pair), static_cast<float>(nibble_of(word, e)), least_of(pair))));
+    for (int n = 0; n < 4; ++n) {
+        // Two codes as bf16 128 + c, whose fp32 is a shift away. (step * code is exact in fp32: one rounding to fp32, one to bf16.)
+        const uint32_t two = ((word >> (4 * n)) & 0x000f000fu) | 0x43004300u;
+        const float a = __uint_as_float(two << 16) - 128.f, b = __uint_as_float(two & 0xffff0000u) - 128.f;
+        to[n] = pack_bf16(fmaf(step, a, least), fmaf(step, b, least));
     }
     return x;
 }
 
-// A thread brings eight columns of one key and its value.
+// A thread brings eight columns of kReadRows keys and their values, all requested before the first is used.
+constexpr int kReadRows = 4;
+
 template <int D, int kBits>
 __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams p) {
-    const int j = blockIdx.x * blockDim.y + threadIdx.y, head = blockIdx.y, b = blockIdx.z;
-    const int chunk = threadIdx.x, col = chunk * 8;
+    constexpr int kChunks = D / 8, kTokens = 256 / kChunks;   // tokens of the block at a time
+    const int chunk = threadIdx.x % kChunks, col = chunk * 8, head = blockIdx.y, b = blockIdx.z;
+    const int first = blockIdx.x * (kReadRows * kTokens) + threadIdx.x / kChunks;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int len = cached_keys(p.c, b);
-    if (p.cu_k && blockIdx.x == 0 && head == 0 && threadIdx.x == 0 && threadIdx.y == 0) {
+    if (p.cu_k && blockIdx.x == 0 && head == 0 && threadIdx.x == 0) {
         p.cu_k[b] = b * p.rows;
         if (b == static_cast<int>(gridDim.z) - 1) p.cu_k[b + 1] = (b + 1) * p.rows;
     }
-    if (j >= p.rows) return;
-    Eight<__nv_bfloat16> k, v;
+    const unsigned char *kp[kReadRows], *vp[kReadRows];
+    int token[kReadRows];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        k.set(e, __float2bfloat16_rn(0.f));
-        v.set(e, __float2bfloat16_rn(0.f));
-    }
-    const int64_t page = j < len ? page_of(p.c, b, j) : -1;
-    if (page >= 0) {
-        const unsigned char* kp = p.c.k + page * p.c.ks[0] + head * p.c.ks[1];
-        const unsigned char* vp = p.c.v + page * p.c.vs[0] + head * p.c.vs[1];
-        const int at = j % p.c.page_size;
-        if constexpr (kBits == 16) {
-            k.load(reinterpret_cast<const __nv_bfloat16*>(kp + at * p.c.ks[2]) + col);
-            v.load(reinterpret_cast<const __nv_bfloat16*>(vp + at * p.c.vs[2]) + col);
-        } else {
-            k = get_four_bits<D, false>(kp + (at >> 4) * (9 * D), at & 15, chunk);
-            v = get_four_bits<D, true>(vp + (at >> 4) * (9 * D), at & 15, chunk);
+    for (int i = 0; i < kReadRows; ++i) {
+        const int j = first + i * kTokens, entry = j / p.c.page_size, at = j - entry * p.c.page_size;
+        int64_t page = -1;
+        if (j < len && j < p.rows) page = p.c.table[b * p.c.table_stride + entry];
+        kp[i] = vp[i] = nullptr;
+        token[i] = at & 15;
+        if (page >= 0 && page < p.c.pages) {
+            kp[i] = p.c.k + page * p.c.ks[0] + head * p.c.ks[1] + (kBits == 16 ? at * p.c.ks[2] : (at >> 4) * (9 * D));
+            vp[i] = p.c.v + page * p.c.vs[0] + head * p.c.vs[1] + (kBits == 16 ? at * p.c.vs[2] : (at >> 4) * (9 * D));
         }
     }
-    k.store(p.k + b * p.ks[0] + head * p.ks[1] + j * p.ks[2] + col);
-    v.store(p.v + b * p.vs[0] + head * p.vs[1] + j * p.vs[2] + col);
+    Eight<__nv_bfloat16> k[kReadRows], v[kReadRows];
+    uint32_t words[kReadRows][4];
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i) {
+        if constexpr (kBits == 16) {
+            k[i].zero();
+            v[i].zero();
+            if (kp[i]) {
+                k[i].load(reinterpret_cast<const __nv_bfloat16*>(kp[i]) + col);
+                v[i].load(reinterpret_cast<const __nv_bfloat16*>(vp[i]) + col);
+            }
+        } else {
+            words[i][0] = words[i][1] = words[i][2] = words[i][3] = 0;   // (worth zeros)
+            if (kp[i]) {
+                const uint32_t *kw = reinterpret_cast<const uint32_t*>(kp[i]), *vw = reinterpret_cast<const uint32_t*>(vp[i]);
+                words[i][0] = kw[key_word<D>(token[i], chunk)];
+                words[i][1] = kw[step_word<D>(token[i], chunk / 8)];
+                words[i][2] = vw[value_word<D>(token[i], chunk)];
+                words[i][3] = vw[step_word<D>(token[i], chunk / 8)];
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kReadRows; ++i) {
+        const int j = first + i * kTokens;
+        if (j >= p.rows) break;
+        if constexpr (kBits == 4) {
+            k[i] = of_four_bits(words[i][0], words[i][1]);
+            v[i] = of_four_bits(words[i][2], words[i][3]);
+        }
+        k[i].store(p.k + b * p.ks[0] + head * p.ks[1] + j * p.ks[2] + col);
+        v[i].store(p.v + b * p.vs[0] + head * p.vs[1] + j * p.vs[2] + col);
+    }
 }
 
 template <typename Params>
@@ -265,7 +298,7 @@ int launch_append(const AppendParams& given, cudaStream_t stream) {
         const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), static_cast<unsigned>(p.groups + 2 * ((p.kv_heads + per - 1) / per)));
         return launch_dependent(kernel, p, grid, block, stream, "paged_append launch");
     };
-    const bool fast = turn_is_fast(p.turn);
+    const bool fast = p.vec && turn_is_fast(p.turn);
     // Four heads to a thread once that fills the GPU.
     if (p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads) >= 4 * 148 * 2048) {
         if (fast) return go(append_kernel<D, kBits, true, 4>, 4);
@@ -277,9 +310,9 @@ int launch_append(const AppendParams& given, cudaStream_t stream) {
 
 template <int D, int kBits>
 int launch_read(const ReadParams& p, int batch, int kv_heads, cudaStream_t stream) {
-    const dim3 block(D / 8, 256 / (D / 8));
-    const dim3 grid(static_cast<unsigned>((p.rows + block.y - 1) / block.y), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
-    return launch_dependent(read_kernel<D, kBits>, p, grid, block, stream, "paged_read launch");
+    constexpr int kRows = kReadRows * (256 / (D / 8));
+    const dim3 grid(static_cast<unsigned>((p.rows + kRows - 1) / kRows), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
+    return launch_dependent(read_kernel<D, kBits>, p, grid, dim3(256), stream, "paged_read launch");
 }
 
 int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, cudaStream_t stream) {

@@ -33,7 +33,6 @@ __host__ __device__ __forceinline__ int step_word(int token, int group) {
     return 16 * (D / 8) + token * (D / 64) + group;
 }
 
-__device__ __forceinline__ int nibble_of(uint32_t word, int e) { return (word >> (4 * ((e >> 1) + 4 * (e & 1)))) & 15; }
 __device__ __forceinline__ float step_of(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float least_of(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }
 

@@ -16,10 +16,13 @@
 // 4 bits: a code c is worth least + step c per 64 channels. Codes become bf16 128 + c by one logic operation for two (the
 // pages' layout is made for it, paged.cuh) and never anything else:
 //   s_j   = sum_g step_jg (q_g . (128 + c_jg)) + (least_jg - 128 step_jg) sum(q_g): one product per group of channels g
-//   o_g  += (p_j step_jg) (c_jg - 8), and p_j (least_jg + 8 step_jg) once for all channels of the group: with codes about
-//           their middle, neither sum is large beside the result.
-// p_j step_jg is rounded to bf16 for the product, as p_j is over bf16 pages; all else is fp32.
+//   o_g  += (2 p_j step_jg) (8 + c_jg / 2) less 12 (2 p_j step_jg), by a product with the constant 12 whose rows are all
+//           alike, and p_j (least_jg + 8 step_jg) once for all channels of the group: what is left of both sums is about the
+//           middle of the codes, and neither is large beside the result. (8 + c / 2 is a code shifted into the mantissa of 8; with
+//           128 + c in its place the sums would be ten times as large and lose as much to fp32.)
+// 2 p_j step_jg is rounded to bf16 for the product, as p_j is over bf16 pages; all else is fp32.
 #include <atomic>
+#include <type_traits>
 
 #include "kept.h"
 #include "paged.cuh"
@@ -99,11 +102,22 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t word) {
     asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(y) : "r"(word));   // (word & mask) | 128
     return y;
 }
-// ... less 136: codes about their middle, exactly.
-__device__ __forceinline__ uint32_t about_middle(uint32_t pair) {
-    const __nv_bfloat162 x = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&pair), __floats2bfloat162_rn(136.f, 136.f));
-    return *reinterpret_cast<const uint32_t*>(&x);
+// The i-th of four pairs of codes (nibbles i and i + 4 of a word) as 8 + c / 2: in bits 3 to 6 of the mantissa; the
+// first pair by 128 + c times 1 / 2 less 56, which is exact.
+template <int i>
+__device__ __forceinline__ uint32_t half_code_pair(uint32_t word) {
+    uint32_t y;
+    if constexpr (i == 0) {
+        y = code_pair(word);
+        asm("fma.rn.bf16x2 %0, %0, %1, %2;" : "+r"(y) : "r"(0x3f003f00u), "r"(0xc260c260u));   // 0.5, -56
+    } else {
+        asm("lop3.b32 %0, %1, 0x00780078, 0x41004100, 0xea;" : "=r"(y) : "r"(word >> (4 * i - 3)));
+    }
+    return y;
 }
+constexpr uint32_t kTwelve = 0x41404140u;   // bf16 12, twice
+// The reference of a column that has seen no key: below every logit.
+constexpr float kNoKey = -3.0e38f;
 
 // Rows of a sequence's queries: how many tokens, and where they start.
 __device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& first) {
@@ -249,64 +263,66 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
         __syncthreads();
     };
 
-    // The pages of this warp's blocks in the producer's next 32 tiles, a lane each.
-    int64_t page = -1;
-    int page_at = 32;
+    // Where this warp's blocks of the producer's next 32 tiles lie, a lane each; null: no page.
+    const unsigned char *k_at = nullptr, *v_at = nullptr;
+    int at = 32;
     auto issue = [&](const Cursor& c, int st, bool fresh_pair) {
-        if (fresh_pair || page_at == 32) {
-            const int block = (c.tile + lane * step) * W + warp;
-            page = -1;
+        if (fresh_pair || at == 32) {
+            const int block = (c.tile + lane * step) * W + warp, hk = c.hk / p.row_tiles;
+            k_at = v_at = nullptr;
             if (static_cast<int64_t>(block) * 16 < c.len) {
-                page = p.c.table[c.b * p.c.table_stride + block / p.page_blocks];
-                if (page < 0 || page >= p.c.pages) page = -1;   // no page: zeros
+                const int entry = block / p.page_blocks, row = (block - entry * p.page_blocks) * (kBits == 16 ? 16 : 1);
+                const int64_t page = p.c.table[c.b * p.c.table_stride + entry];
+                if (page >= 0 && page < p.c.pages) {
+                    k_at = p.c.k + page * p.c.ks[0] + hk * p.c.ks[1] + row * (kBits == 16 ? p.c.ks[2] : 9 * D);
+                    v_at = p.c.v + page * p.c.vs[0] + hk * p.c.vs[1] + row * (kBits == 16 ? p.c.vs[2] : 9 * D);
+                }
             }
-            page_at = 0;
+            at = 0;
         }
-        const int64_t pg = __shfl_sync(0xffffffffu, page, page_at);
-        ++page_at;
-        const int block = c.tile * W + warp, j0 = block * 16;
+        const unsigned char* kp = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k_at), at));
+        const unsigned char* vp = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v_at), at));
+        ++at;
+        const int j0 = (c.tile * W + warp) * 16;
         if (j0 >= c.len) return;
-        const bool there = pg >= 0;
-        const int hk = c.hk / p.row_tiles, in_page = block % p.page_blocks;
-        const unsigned char* kp = p.c.k + (there ? pg * p.c.ks[0] + hk * p.c.ks[1] : 0);
-        const unsigned char* vp = p.c.v + (there ? pg * p.c.vs[0] + hk * p.c.vs[1] : 0);
+        const bool there = kp != nullptr;
+        if (!there) kp = p.c.k, vp = p.c.v;    // (not read: zeros are written)
         const uint32_t to = smem_u32(ring + st * S::kStage);
         if constexpr (kBits == 16) {
-            constexpr int CH = D / 8;
-            const int left = c.len - j0;
-            kp += there ? in_page * 16 * p.c.ks[2] : 0;
-            vp += there ? in_page * 16 * p.c.vs[2] : 0;
+            constexpr int CH = D / 8, kStep = 32 / CH;
+            const int left = there ? c.len - j0 : 0, r0 = lane / CH, ch = lane % CH;   // rows behind the last key are zeros, whatever the page holds
+            const unsigned char* kr = kp + ch * 16;
+            const unsigned char* vr = vp + ch * 16;
 #pragma unroll
-            for (int it = 0; it < 16 * CH / 32; ++it) {
-                const int idx = it * 32 + lane, r = idx / CH, ch = idx % CH;
-                const bool ok = there && r < left;   // rows behind the last key are zeros, whatever the page holds
-                cp_async_16(to + swizzled<D>(r, ch * 8), kp + (ok ? r * p.c.ks[2] : 0) + (ok ? ch * 16 : 0), ok);
-                cp_async_16(to + 32 * D + swizzled<D>(r, ch * 8), vp + (ok ? r * p.c.vs[2] : 0) + (ok ? ch * 16 : 0), ok);
+            for (int it = 0; it < 16 / kStep; ++it) {
+                const int r = it * kStep + r0;
+                const bool ok = r < left;
+                cp_async_16(to + swizzled<D>(r, ch * 8), kr + (ok ? r * p.c.ks[2] : 0), ok);
+                cp_async_16(to + 32 * D + swizzled<D>(r, ch * 8), vr + (ok ? r * p.c.vs[2] : 0), ok);
             }
         } else {
-            constexpr int kHalf = 9 * D / 16;   // 16-byte pieces of a block
-            kp += there ? in_page * (9 * D) : 0;
-            vp += there ? in_page * (9 * D) : 0;
+            constexpr int kPieces = 9 * D / 16;   // of 16 bytes, of keys and of values
+            kp += lane * 16;
+            vp += lane * 16;
 #pragma unroll
-            for (int it = 0; it < (2 * kHalf + 31) / 32; ++it) {
-                const int idx = it * 32 + lane;
-                if (idx < 2 * kHalf) {
-                    const unsigned char* from = idx < kHalf ? kp + (there ? idx * 16 : 0) : vp + (there ? (idx - kHalf) * 16 : 0);
-                    cp_async_16(to + idx * 16, from, there);
+            for (int it = 0; it < (kPieces + 31) / 32; ++it) {
+                if (32 * it + 32 <= kPieces || lane < kPieces - 32 * it) {
+                    cp_async_16(to + (it * 32 + lane) * 16, kp + it * 512, there);
+                    cp_async_16(to + (kPieces + it * 32 + lane) * 16, vp + it * 512, there);
                 }
             }
         }
     };
 
-    int up = 0;
+    int up = 0, up_st = 0;
     bool fresh_prod = true;
     auto produce = [&]() {
         if (up < u1) {
-            issue(prod, up % NS, fresh_prod);
-            const int b = prod.b, hk = prod.hk;
+            issue(prod, up_st, fresh_prod);
             next(prod);
-            fresh_prod = b != prod.b || hk != prod.hk;
+            fresh_prod = !kCluster && prod.tile == 0;
             ++up;
+            up_st = up_st + 1 == NS ? 0 : up_st + 1;
         }
         cp_async_commit();
     };
@@ -316,11 +332,14 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
     uint32_t qb[NT][MT][2];           // B operands of S^T: columns are query rows
     float qsum[NT][G][2];             // 4 bits: sums of this thread's two columns by group of channels
     int lim[NT][2], whole = 0;        // the last key that a column sees; that all columns see
-    float o[MT][NT][4], mid[NT][G][2], m_ref[NT][2], l_run[NT][2];
+    float o[MT][NT][4], mid[NT][G][2], m_ref[NT][2], bar[NT][2], l_run[NT][2];   // bar: the logit that moves the reference
+    float twelve[NT][G][4];           // 4 bits: 12 times the weights' sums
+    const float inv_scale = 1.f / p.scale_log2;
     bool fresh = true;
 
+    int st = NS - 1;
     for (int u = 0; u < u1; ++u) {
-        const int st = u % NS;
+        st = st + 1 == NS ? 0 : st + 1;
         produce();
         if (fresh) {
             fresh = false;
@@ -373,10 +392,11 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 for (int e = 0; e < 2; ++e) {
                     const int c = row0 + nt * 8 + 2 * t + e;
                     lim[nt][e] = p.causal ? cons.len - n + (c < rows ? c % n : 0) : cons.len - 1;
-                    m_ref[nt][e] = -INFINITY;
+                    m_ref[nt][e] = kNoKey;
+                    bar[nt][e] = -INFINITY;
                     l_run[nt][e] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < G; ++w) mid[nt][w][e] = 0.f;
+                    for (int w = 0; w < G; ++w) mid[nt][w][e] = twelve[nt][w][e] = twelve[nt][w][e + 2] = 0.f;
                 }
             }
 #pragma unroll
@@ -392,7 +412,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
         if (j0 < cons.len) {
             const unsigned char* sk = ring + st * S::kStage;
             const unsigned char* sv = sk + S::kStage / 2;
-            float x[NT][4];   // logits in base 2: key g of columns 2 t, 2 t + 1, then key g + 8
+            float x[NT][4];   // q k: key g of columns 2 t, 2 t + 1, then key g + 8
             uint2 vstep[2];   // 4 bits: (step, least) of the two keys' values
             if constexpr (kBits == 16) {
 #pragma unroll
@@ -405,11 +425,6 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                     ldmatrix_x4(a, base + swizzled<D>(r, kk * 16 + c));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma_bf16(x[nt], a, qb[nt][kk][0], qb[nt][kk][1]);
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[nt][e] *= p.scale_log2;
                 }
             } else {
                 uint32_t kw[2][D / 32];
@@ -430,10 +445,13 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                         kstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(steps), 0u);
                         vstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(vsteps), 0u);
                     }
-                    if (j0 + g + 8 * h >= cons.len) kstep[h] = vstep[h] = make_uint2(0u, 0u);   // whatever the page holds there
                 }
+                if (j0 + 16 > cons.len) {   // whatever the page holds behind the last key
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+                    for (int h = 0; h < 2; ++h) {
+                        if (j0 + g + 8 * h >= cons.len) kstep[h] = vstep[h] = make_uint2(0u, 0u);
+                    }
+                }
 #pragma unroll
                 for (int w = 0; w < G; ++w) {
                     float acc[NT][4];
@@ -451,11 +469,14 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t pair = w ? kstep[h].y : kstep[h].x;
-                        const float ks = step_of(pair) * p.scale_log2, kl = fmaf(-128.f, ks, least_of(pair) * p.scale_log2);
+                        const float ks = step_of(pair), kl = fmaf(-128.f, ks, least_of(pair));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) x[nt][2 * h + e] += fmaf(ks, acc[nt][2 * h + e], kl * qsum[nt][w][e]);
+                            for (int e = 0; e < 2; ++e) {
+                                const float at_zero = w ? fmaf(kl, qsum[nt][w][e], x[nt][2 * h + e]) : kl * qsum[nt][w][e];
+                                x[nt][2 * h + e] = fmaf(ks, acc[nt][2 * h + e], at_zero);
+                            }
                         }
                     }
                 }
@@ -473,7 +494,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) higher |= x[nt][e] > m_ref[nt][e & 1] + 8.f;
+                for (int e = 0; e < 4; ++e) higher |= x[nt][e] > bar[nt][e & 1];
             }
             if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
@@ -484,9 +505,10 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        top = fmaxf(top, m_ref[nt][e]);
-                        const float f = fast_exp2(m_ref[nt][e] - (top == -INFINITY ? 0.f : top));
+                        top = fmaxf(top * p.scale_log2, m_ref[nt][e]);
+                        const float f = fast_exp2(m_ref[nt][e] - top);
                         m_ref[nt][e] = top;
+                        bar[nt][e] = (top + 8.f) * inv_scale;
                         l_run[nt][e] *= f;
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
@@ -494,7 +516,11 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                             o[mt][nt][e + 2] *= f;
                         }
 #pragma unroll
-                        for (int w = 0; w < G; ++w) mid[nt][w][e] *= f;
+                        for (int w = 0; w < G; ++w) {
+                            mid[nt][w][e] *= f;
+                            twelve[nt][w][e] *= f;
+                            twelve[nt][w][e + 2] *= f;
+                        }
                     }
                 }
             }
@@ -502,8 +528,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float ref = m_ref[nt][e & 1];
-                    x[nt][e] = fast_exp2(x[nt][e] - (ref == -INFINITY ? 0.f : ref));
+                    x[nt][e] = fast_exp2(fmaf(x[nt][e], p.scale_log2, -m_ref[nt][e & 1]));
                     l_run[nt][e & 1] += x[nt][e];
                 }
             }
@@ -530,7 +555,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t pair = w ? vstep[h].y : vstep[h].x;
-                        const float vs = step_of(pair), vm = fmaf(8.f, vs, least_of(pair));
+                        const float vs = 2.f * step_of(pair), vm = fmaf(4.f, vs, least_of(pair));
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             pb[nt][w][h] = transposed(pack_bf16(x[nt][2 * h] * vs, x[nt][2 * h + 1] * vs));
@@ -556,14 +581,20 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 for (int w = 0; w < G; ++w) {
                     const uint32_t lo0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x5410), hi0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x7632);
                     const uint32_t lo1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x5410), hi1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x7632);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        // Row g: channel 64 w + 8 g + 2 i; row g + 8: the next one.
-                        const uint32_t a[4] = {about_middle(code_pair(lo0 >> (4 * i))), about_middle(code_pair(hi0 >> (4 * i))),
-                                               about_middle(code_pair(lo1 >> (4 * i))), about_middle(code_pair(hi1 >> (4 * i)))};
+                    // Rows g and g + 8 of instruction i: channels 64 w + 8 g + 2 i and the next one.
+                    auto product = [&](auto which) {
+                        constexpr int i = decltype(which)::value;
+                        const uint32_t a[4] = {half_code_pair<i>(lo0), half_code_pair<i>(hi0), half_code_pair<i>(lo1), half_code_pair<i>(hi1)};
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma_bf16(o[4 * w + i][nt], a, pb[nt][w][0], pb[nt][w][1]);
-                    }
+                    };
+                    product(std::integral_constant<int, 0>());
+                    product(std::integral_constant<int, 1>());
+                    product(std::integral_constant<int, 2>());
+                    product(std::integral_constant<int, 3>());
+                    const uint32_t a[4] = {kTwelve, kTwelve, kTwelve, kTwelve};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_bf16(twelve[nt][w], a, pb[nt][w][0], pb[nt][w][1]);
                 }
             }
         }
@@ -600,10 +631,11 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                             float add = mid[nt][w][e];
 #pragma unroll
                             for (int off = 4; off < 32; off <<= 1) add += __shfl_xor_sync(0xffffffffu, add, off);
+                            const float less = twelve[nt][w][e];   // (all rows alike)
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
-                                const float4 y = make_float4(o[4 * w + 2 * h][nt][e] + add, o[4 * w + 2 * h][nt][e + 2] + add,
-                                                             o[4 * w + 2 * h + 1][nt][e] + add, o[4 * w + 2 * h + 1][nt][e + 2] + add);
+                                const float4 y = make_float4((o[4 * w + 2 * h][nt][e] - less) + add, (o[4 * w + 2 * h][nt][e + 2] - less) + add,
+                                                             (o[4 * w + 2 * h + 1][nt][e] - less) + add, (o[4 * w + 2 * h + 1][nt][e + 2] - less) + add);
                                 *reinterpret_cast<float4*>(slab + r * D + slab_chunk(r, 16 * w + 2 * g + h) * 4) = y;
                             }
                         }

@@ -94,7 +94,8 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     if (n >= p.tokens) return;
     const int which = static_cast<int>(blockIdx.y) >= p.groups[0];
     const int h0 = (static_cast<int>(blockIdx.y) - (which ? p.groups[0] : 0)) * kHeads;
-    const int64_t b = n / p.rows, r = n - b * p.rows;
+    const uint32_t entry = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows);   // (2^31 tokens at most)
+    const int64_t b = entry, r = static_cast<uint32_t>(n) - entry * static_cast<uint32_t>(p.rows);
     int64_t pos = r;
     if (p.positions) {
         const int64_t at = b * p.ps[0] + r * p.ps[1];

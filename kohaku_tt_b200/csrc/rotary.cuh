@@ -40,6 +40,10 @@ struct Eight {
     uint4 raw[kPieces];
     __device__ __forceinline__ T get(int e) const { return reinterpret_cast<const T*>(raw)[e]; }
     __device__ __forceinline__ void set(int e, T x) { reinterpret_cast<T*>(raw)[e] = x; }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+    }
     __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
