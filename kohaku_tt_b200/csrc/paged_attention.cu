@@ -5,11 +5,11 @@
 // Bound: the reading of the pages, 4 D bytes per key and head in bf16, 9 / 8 D in 4 bits. So all query rows of a K / V head
 // (its group's heads x tokens, in tiles of 8 or 16 rows) share one pass over the keys, and the keys of all (sequence,
 // K / V head) pairs are laid end to end and cut into equal shares (split.cuh), as in decode.cu; where the pairs are few, a
-// cluster of CTAs has a pair to itself. Partial results of a pair meet behind a ticket in L2, or in the cluster's shared
+// cluster of CTAs has a pair to itself. Partial results of a pair meet in a small second launch, or in the cluster's shared
 // memory, and are added in a fixed order.
 //
-// A warp has 16 keys of a tile and a ring of stages of its own: one page, of which it needs one block. Both products have the
-// keys or channels as the rows of their matrix instruction (m16n8k16) and the queries as its 8 columns, so that a
+// A CTA's share of a pair is cut into equal runs of blocks (16 keys, which lie in one page), one to a warp; a warp has a ring of
+// stages of its own, each of a few blocks. Both products have the keys or channels as the rows of their matrix instruction (m16n8k16) and the queries as its 8 columns, so that a
 // group of 8 heads or fewer leaves nothing idle: S^T = K Q^T, then O^T += V^T P^T. P^T comes out of S^T's registers by
 // an 8 x 8 transpose (movmatrix). The reference of the exponentials moves when a score exceeds it by 2^8.
 //
@@ -47,33 +47,32 @@ struct PagedParams {
     int64_t qs[3], os[3];
     const int32_t* cu;       // packed queries
     int64_t total_q;
-    int32_t* counters;       // [kMaxCtas] tickets, zero between calls
-    float* part_m;           // [slots][16]
-    float* part_l;
+    int2* pieces;            // [pairs] first slot of a pair's partials, and how many it has (1: none, its result is written)
+    float2* part_ml;         // [slots][16] maximum and sum
     float* part_o;           // [slots][16][D]
     int ranks;               // CTAs of a cluster
 };
 
 constexpr int kMaxBatch = 512;    // lengths and their prefix sums live in shared memory
-constexpr int kMaxPending = 8;
-constexpr int kMaxCtas = 1024;
-constexpr int kPairCost = 4;      // what ending a pair costs a CTA, in tiles
-constexpr int kMinUnits = 2;
 
 // What a variant has: D, bits of the pages, NT column tiles of 8 query rows.
 template <int D, int kBits, int NT>
 struct Shape {
-    static constexpr int W = kBits == 4 && NT == 1 ? 8 : 4;       // warps
-    static constexpr int kThreads = 32 * W, kTile = 16 * W;       // keys of a tile
-    static constexpr int kStage = kBits == 4 ? 18 * D : 64 * D;   // bytes: 16 keys, then their values
-    static constexpr int NS = kBits == 4 ? (D == 64 ? 6 : 4) : (D == 64 ? 6 : 3);
+    static constexpr int W = 4;                                               // warps
+    static constexpr int kThreads = 32 * W;
+    static constexpr int kBlock = kBits == 4 ? 18 * D : 64 * D;               // bytes: 16 keys, then their values
+    static constexpr int NB = kBits == 16 ? 1 : (D == 128 && NT == 1 ? 2 : 4);   // blocks of a stage
+    static constexpr int PB = kBits == 4 && NT == 1 ? 2 : 1;                 // blocks that the products are of at a time
+    static constexpr int kStage = NB * kBlock;
+    static constexpr int NS = kBits == 4 ? 2 : (D == 64 ? 6 : 3);
     static constexpr int kRows = 8 * NT;
-    static constexpr int kCtas = kBits == 4 && NT == 2 ? 3 : 2;   // per SM
+    static constexpr int kPairCost = kBits == 4 ? 24 : (D == 64 ? 24 : 16);   // what ending a pair costs a CTA, in blocks
+    static constexpr int kCtas = kBits == 16 ? 2 : D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);   // per SM
     static constexpr int kRing = W * NS * kStage;
-    static constexpr int kSlab = kBits == 4 ? W * kRows * D * 4 : 0;   // bf16: in the stage just consumed
-    static constexpr int kStats = (3 * W + 2) * kRows * 4;
+    static constexpr int kStats = (3 * W + 2) * kRows * 4 + W * 4;
+    static_assert(kStage >= kRows * D * 4, "a warp leaves its result in the stage it consumed last");
     static constexpr int smem(bool cluster) {
-        return kRing + kSlab + kStats + (cluster ? kRows * D * 4 : (2 * kMaxBatch + 1 + 8 + 6 * kMaxPending + 3) * 4);
+        return kRing + kStats + (cluster ? kRows * D * 4 : (2 * kMaxBatch + 1 + 8) * 4);
     }
 };
 
@@ -132,145 +131,100 @@ __device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& f
     return static_cast<int>(hi - lo);
 }
 
+// One normalised chunk of 4 columns of (pair, row of its tile).
+__device__ __forceinline__ void write_row(const PagedParams& p, int b, int vh, int row_in_tile, int tile_rows, int c4, float4 sum, float ll) {
+    const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // (a NaN stays one)
+    const int hk = vh / p.row_tiles, row = (vh - hk * p.row_tiles) * tile_rows + row_in_tile;
+    int64_t first;
+    const int n = tokens_of(p, b, first);
+    const int gi = row / n, tq = row - gi * n;
+    __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + (hk * p.group + gi) * p.os[1] + (first + tq) * p.os[2] + c4 * 4;
+    uint2 packed;
+    packed.x = pack_bf16(sum.x * inv, sum.y * inv);
+    packed.y = pack_bf16(sum.z * inv, sum.w * inv);
+    *reinterpret_cast<uint2*>(to) = packed;
+}
+// Rows that a pair has in its tile.
+__device__ __forceinline__ int rows_of(const PagedParams& p, int b, int vh, int tile_rows) {
+    int64_t first;
+    const int all = p.group * tokens_of(p, b, first);
+    return max(min(all - (vh % p.row_tiles) * tile_rows, tile_rows), 0);
+}
+
 template <int D, int kBits, int NT, bool kCluster>
 __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBits, NT>::kCtas)) paged_kernel(const __grid_constant__ PagedParams p) {
     using S = Shape<D, kBits, NT>;
-    constexpr int W = S::W, NS = S::NS, kRows = S::kRows, kTile = S::kTile, kThreads = S::kThreads;
-    constexpr int G = D / 64, MT = D / 16;
+    constexpr int W = S::W, NS = S::NS, NB = S::NB, PB = S::PB, kRows = S::kRows, kThreads = S::kThreads;
+    constexpr int G = D / 64, MT = D / 16, kPairCost = S::kPairCost;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char* ring = smem + warp * NS * S::kStage;     // this warp's
-    float* sm_m = reinterpret_cast<float*>(smem + S::kRing + S::kSlab);   // [W][kRows]
+    float* sm_m = reinterpret_cast<float*>(smem + S::kRing);   // [W][kRows]
     float* sm_l = sm_m + W * kRows;
     float* sm_f = sm_l + W * kRows;    // a warp's weight in its CTA's sum
     float* fin_m = sm_f + W * kRows;   // [kRows]
     float* fin_l = fin_m + kRows;
-    int* prefix_s = reinterpret_cast<int*>(fin_l + kRows);       // [kMaxBatch + 1]
+    int* slab_s = reinterpret_cast<int*>(fin_l + kRows);       // [W] where a warp left its result
+    int* prefix_s = slab_s + W;        // [kMaxBatch + 1]
     int* lens_s = prefix_s + kMaxBatch + 1;
     int* misc = lens_s + kMaxBatch;
-    float* part_s = fin_l + kRows;     // kCluster: [kRows][D] this CTA's partial
+    float* part_s = reinterpret_cast<float*>(slab_s + W);      // kCluster: [kRows][D] this CTA's partial
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    Cursor prod, cons;
-    int u1, upc = 0, rank = 0;
-    const int step = kCluster ? p.ranks : 1;
+    // The blocks that this CTA streams: `left` of them from block `tile` of a pair on, through the pairs behind it.
+    struct Walk {
+        Cursor c;
+        int left, pos, end;   // pos .. end: this warp's blocks of the CTA's piece of the pair
+    } cons;
+    int upc = 0, rank = 0, ranks_used = 1;
     if constexpr (kCluster) {
         const int pair = static_cast<int>(blockIdx.x) / p.ranks;
         rank = static_cast<int>(blockIdx.x) - pair * p.ranks;
-        cons.b = pair / p.kv_heads;
-        cons.hk = pair - cons.b * p.kv_heads;
-        cons.tile = rank;
-        cons.len = cached_keys(p.c, cons.b);
-        cons.ntiles = max((cons.len + kTile - 1) / kTile, 1);
-        u1 = cons.ntiles > rank ? (cons.ntiles - rank + p.ranks - 1) / p.ranks : 0;
+        cons.c.b = pair / p.kv_heads;
+        cons.c.hk = pair - cons.c.b * p.kv_heads;
+        cons.c.len = cached_keys(p.c, cons.c.b);
+        cons.c.ntiles = max((cons.c.len + 15) / 16, 1);
+        // A rank has a block for each warp, or more.
+        const int each = max((cons.c.ntiles + p.ranks - 1) / p.ranks, W);
+        cons.c.tile = min(rank * each, cons.c.ntiles);
+        cons.left = min(each, cons.c.ntiles - cons.c.tile);
+        ranks_used = (cons.c.ntiles + each - 1) / each;
     } else {
-        scan_lengths<kThreads, kMaxBatch, kTile, kPairCost>(p.batch, [&](int b) { return cached_keys(p.c, b); }, prefix_s, lens_s, misc);
+        scan_lengths<kThreads, kMaxBatch, 16, kPairCost>(p.batch, [&](int b) { return cached_keys(p.c, b); }, prefix_s, lens_s, misc);
         const int total = p.kv_heads * prefix_s[p.batch];
-        upc = max(static_cast<int>((total + gridDim.x - 1) / gridDim.x), kMinUnits);
+        upc = max(static_cast<int>((total + gridDim.x - 1) / gridDim.x), 2 * W);
         const int64_t from = static_cast<int64_t>(blockIdx.x) * upc;
         const int first_unit = static_cast<int>(from < total ? from : total), end_unit = min(first_unit + upc, total);
-        u1 = tiles_before<kPairCost>(p, prefix_s, end_unit) - tiles_before<kPairCost>(p, prefix_s, first_unit);
-        if (u1 <= 0) return;
-        cursor_seek<kPairCost>(p, prefix_s, lens_s, cons, first_unit);
+        cons.left = tiles_before<kPairCost>(p, prefix_s, end_unit) - tiles_before<kPairCost>(p, prefix_s, first_unit);
+        if (cons.left <= 0) return;
+        cursor_seek<kPairCost>(p, prefix_s, lens_s, cons.c, first_unit);
     }
-    prod = cons;
-    auto next = [&](Cursor& c) {
-        if constexpr (kCluster) c.tile += p.ranks;
-        else cursor_next<kPairCost>(p, prefix_s, lens_s, c);
+    auto piece_of = [](const Walk& w) { return min(w.c.ntiles - w.c.tile, w.left); };
+    auto enter = [&](Walk& w) {
+        const int m = piece_of(w), each = m / W, more = m - each * W;
+        w.pos = w.c.tile + warp * each + min(warp, more);
+        w.end = w.pos + each + (warp < more ? 1 : 0);
     };
-
-    // One normalised chunk of 4 columns of (pair, row of its tile).
-    auto write_row = [&](int b, int vh, int r, int c4, float4 sum, float ll) {
-        const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // (a NaN stays one)
-        const int hk = vh / p.row_tiles, row = (vh - hk * p.row_tiles) * kRows + r;
-        int64_t first;
-        const int n = tokens_of(p, b, first);
-        const int gi = row / n, tq = row - gi * n;
-        __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + (hk * p.group + gi) * p.os[1] + (first + tq) * p.os[2] + c4 * 4;
-        uint2 packed;
-        packed.x = pack_bf16(sum.x * inv, sum.y * inv);
-        packed.y = pack_bf16(sum.z * inv, sum.w * inv);
-        *reinterpret_cast<uint2*>(to) = packed;
+    auto leave = [&](Walk& w) {   // to the next pair
+        w.left -= piece_of(w);
+        if (kCluster || w.left == 0) return;
+        w.c.tile = w.c.ntiles - 1;
+        cursor_next<kPairCost>(p, prefix_s, lens_s, w.c);
     };
-    // Rows that a pair has in its tile.
-    auto rows_of = [&](int b, int vh) {
-        int64_t first;
-        const int all = p.group * tokens_of(p, b, first);
-        return max(min(all - (vh % p.row_tiles) * kRows, kRows), 0);
-    };
+    enter(cons);
+    Walk prod = cons;
 
-    int* pend = misc + 8;            // [kMaxPending][5]: pair, first CTA, last CTA, batch, head of the pair
-    int* npend_s = pend + 5 * kMaxPending;
-    int* last_s = npend_s + 1;
-    if (!kCluster && threadIdx.x == 0) npend_s[0] = 0;
-
-    // Draws a ticket for each pending pair; the last holder adds the pair's partials up, in the order of the CTAs, and
-    // puts the counter back to zero. (The same as in decode.cu, which has the measurements.)
-    auto draw_tickets = [&]() {
-        __syncthreads();
-        const int n = npend_s[0];
-        if (static_cast<int>(threadIdx.x) < n) {
-            const int* e = pend + 5 * threadIdx.x;
-            const int parts = e[2] - e[1] + 1;
-            int ticket;
-            asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(ticket) : "l"(p.counters + e[1]) : "memory");
-            last_s[threadIdx.x] = ticket == parts - 1;
-            if (ticket == parts - 1) p.counters[e[1]] = 0;
-        }
-        __syncthreads();
-        constexpr int per_pair = kRows * (D / 4), kHolders = 4;
-        for (int idx = threadIdx.x; idx < n * per_pair; idx += kThreads) {
-            const int i = idx / per_pair, rem = idx - i * per_pair, r = rem / (D / 4), c4 = rem % (D / 4);
-            const int* e = pend + 5 * i;
-            if (!last_s[i] || r >= rows_of(e[3], e[4])) continue;
-            const int slot0 = e[1] + e[0], parts = e[2] - e[1] + 1;
-            float mm = -INFINITY, ll = 0.f;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int c0 = 0; c0 < parts; c0 += kHolders) {
-                float ms[kHolders], ls[kHolders];
-                float4 v[kHolders];
-#pragma unroll
-                for (int j = 0; j < kHolders; ++j) {
-                    const int slot = slot0 + min(c0 + j, parts - 1);   // past the last holder: a repeat, not used
-                    ms[j] = __ldcg(&p.part_m[slot * 16 + r]);
-                    ls[j] = __ldcg(&p.part_l[slot * 16 + r]);
-                    v[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D + c4 * 4));
-                }
-                float m_new = mm;
-#pragma unroll
-                for (int j = 0; j < kHolders; ++j) {
-                    if (c0 + j < parts) m_new = fmaxf(m_new, ms[j]);
-                }
-                const float base = m_new == -INFINITY ? 0.f : m_new, fa = fast_exp2(mm - base);
-                mm = m_new;
-                ll *= fa;
-                sum.x *= fa; sum.y *= fa; sum.z *= fa; sum.w *= fa;
-#pragma unroll
-                for (int j = 0; j < kHolders; ++j) {
-                    if (c0 + j >= parts) continue;
-                    const float fb = fast_exp2(ms[j] - base);
-                    ll = fmaf(ls[j], fb, ll);
-                    sum.x = fmaf(v[j].x, fb, sum.x); sum.y = fmaf(v[j].y, fb, sum.y);
-                    sum.z = fmaf(v[j].z, fb, sum.z); sum.w = fmaf(v[j].w, fb, sum.w);
-                }
-            }
-            write_row(e[3], e[4], r, c4, sum, ll);
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) npend_s[0] = 0;
-        __syncthreads();
-    };
-
-    // Where this warp's blocks of the producer's next 32 tiles lie, a lane each; null: no page.
+    // Where this warp's next 32 blocks lie, a lane each; null: no page.
     const unsigned char *k_at = nullptr, *v_at = nullptr;
     int at = 32;
-    auto issue = [&](const Cursor& c, int st, bool fresh_pair) {
-        if (fresh_pair || at == 32) {
-            const int block = (c.tile + lane * step) * W + warp, hk = c.hk / p.row_tiles;
+    auto issue = [&](int st, int count) {
+        const Cursor& c = prod.c;
+        if (at + count > 32) {   // (a batch's blocks are in one lot)
+            const int block = prod.pos + lane, hk = c.hk / p.row_tiles;
             k_at = v_at = nullptr;
-            if (static_cast<int64_t>(block) * 16 < c.len) {
+            if (block < prod.end && static_cast<int64_t>(block) * 16 < c.len) {
                 const int entry = block / p.page_blocks, row = (block - entry * p.page_blocks) * (kBits == 16 ? 16 : 1);
                 const int64_t page = p.c.table[c.b * p.c.table_stride + entry];
                 if (page >= 0 && page < p.c.pages) {
@@ -280,80 +234,86 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
             }
             at = 0;
         }
-        const unsigned char* kp = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k_at), at));
-        const unsigned char* vp = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v_at), at));
-        ++at;
-        const int j0 = (c.tile * W + warp) * 16;
-        if (j0 >= c.len) return;
-        const bool there = kp != nullptr;
-        if (!there) kp = p.c.k, vp = p.c.v;    // (not read: zeros are written)
         const uint32_t to = smem_u32(ring + st * S::kStage);
-        if constexpr (kBits == 16) {
-            constexpr int CH = D / 8, kStep = 32 / CH;
-            const int left = there ? c.len - j0 : 0, r0 = lane / CH, ch = lane % CH;   // rows behind the last key are zeros, whatever the page holds
-            const unsigned char* kr = kp + ch * 16;
-            const unsigned char* vr = vp + ch * 16;
 #pragma unroll
-            for (int it = 0; it < 16 / kStep; ++it) {
-                const int r = it * kStep + r0;
-                const bool ok = r < left;
-                cp_async_16(to + swizzled<D>(r, ch * 8), kr + (ok ? r * p.c.ks[2] : 0), ok);
-                cp_async_16(to + 32 * D + swizzled<D>(r, ch * 8), vr + (ok ? r * p.c.vs[2] : 0), ok);
-            }
-        } else {
-            constexpr int kPieces = 9 * D / 16;   // of 16 bytes, of keys and of values
-            kp += lane * 16;
-            vp += lane * 16;
+        for (int n = 0; n < NB; ++n) {
+            if (n >= count) break;
+            const unsigned char* kp = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(k_at), at + n));
+            const unsigned char* vp = reinterpret_cast<const unsigned char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(v_at), at + n));
+            const bool there = kp != nullptr;
+            if (!there) kp = p.c.k, vp = p.c.v;    // (not read: zeros are written)
+            if constexpr (kBits == 16) {
+                constexpr int CH = D / 8, kStep = 32 / CH;
+                const int left = there ? c.len - prod.pos * 16 : 0, r0 = lane / CH, ch = lane % CH;   // rows behind the last key are zeros, whatever the page holds
+                const unsigned char* kr = kp + ch * 16;
+                const unsigned char* vr = vp + ch * 16;
 #pragma unroll
-            for (int it = 0; it < (kPieces + 31) / 32; ++it) {
-                if (32 * it + 32 <= kPieces || lane < kPieces - 32 * it) {
-                    cp_async_16(to + (it * 32 + lane) * 16, kp + it * 512, there);
-                    cp_async_16(to + (kPieces + it * 32 + lane) * 16, vp + it * 512, there);
+                for (int it = 0; it < 16 / kStep; ++it) {
+                    const int r = it * kStep + r0;
+                    const bool ok = r < left;
+                    cp_async_16(to + swizzled<D>(r, ch * 8), kr + (ok ? r * p.c.ks[2] : 0), ok);
+                    cp_async_16(to + 32 * D + swizzled<D>(r, ch * 8), vr + (ok ? r * p.c.vs[2] : 0), ok);
+                }
+            } else {
+                constexpr int kPieces = 9 * D / 16;   // of 16 bytes, of keys and of values
+                kp += lane * 16;
+                vp += lane * 16;
+#pragma unroll
+                for (int it = 0; it < (kPieces + 31) / 32; ++it) {
+                    if (32 * it + 32 <= kPieces || lane < kPieces - 32 * it) {
+                        cp_async_16(to + n * S::kBlock + (it * 32 + lane) * 16, kp + it * 512, there);
+                        cp_async_16(to + n * S::kBlock + (kPieces + it * 32 + lane) * 16, vp + it * 512, there);
+                    }
                 }
             }
         }
+        at += count;
     };
 
-    int up = 0, up_st = 0;
-    bool fresh_prod = true;
+    int up_st = 0;
     auto produce = [&]() {
-        if (up < u1) {
-            issue(prod, up_st, fresh_prod);
-            next(prod);
-            fresh_prod = !kCluster && prod.tile == 0;
-            ++up;
+        while (prod.pos == prod.end && prod.left > 0) {
+            leave(prod);
+            if (prod.left > 0) {
+                enter(prod);
+                at = 32;
+            }
+        }
+        if (prod.left > 0) {
+            const int count = min(prod.end - prod.pos, NB);
+            issue(up_st, count);
+            prod.pos += count;
             up_st = up_st + 1 == NS ? 0 : up_st + 1;
         }
         cp_async_commit();
     };
+    if (cons.left > 0) {
 #pragma unroll
-    for (int s = 0; s < NS - 1; ++s) produce();
+        for (int s = 0; s < NS - 1; ++s) produce();
+    }
 
     uint32_t qb[NT][MT][2];           // B operands of S^T: columns are query rows
     float qsum[NT][G][2];             // 4 bits: sums of this thread's two columns by group of channels
-    int lim[NT][2], whole = 0;        // the last key that a column sees; that all columns see
+    // Of this warp's keys: their end, the last one that a column sees, and the last that all columns see.
+    int kend = 0, lim[NT][2], whole = 0;
     float o[MT][NT][4], mid[NT][G][2], m_ref[NT][2], bar[NT][2], l_run[NT][2];   // bar: the logit that moves the reference
     float twelve[NT][G][4];           // 4 bits: 12 times the weights' sums
     const float inv_scale = 1.f / p.scale_log2;
-    bool fresh = true;
-
-    int st = NS - 1;
-    for (int u = 0; u < u1; ++u) {
-        st = st + 1 == NS ? 0 : st + 1;
-        produce();
-        if (fresh) {
-            fresh = false;
-            const int hk = cons.hk / p.row_tiles, row0 = (cons.hk - hk * p.row_tiles) * kRows;
+    int st = NS - 1;                  // the stage consumed last
+    while (cons.left > 0) {           // pieces of pairs
+        {
+            const int hk = cons.c.hk / p.row_tiles, row0 = (cons.c.hk - hk * p.row_tiles) * kRows;
             int64_t first;
-            const int n = tokens_of(p, cons.b, first), rows = p.group * n;
-            whole = p.causal ? cons.len - n : cons.len - 1;
+            const int n = tokens_of(p, cons.c.b, first), rows = p.group * n;
+            kend = min(cons.c.len, cons.end * 16);
+            whole = min(p.causal ? cons.c.len - n : cons.c.len - 1, kend - 1);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 const int r = row0 + nt * 8 + g;
                 const bool ok = r < rows;
                 const int gi = ok ? r / n : 0, tq = ok ? r - gi * n : 0;
                 // (A row past the last reads the first and is zeroed after; without any row at all nothing is read.)
-                const __nv_bfloat16* from = p.q + (p.cu ? 0 : cons.b * p.qs[0]) + (hk * p.group + gi) * p.qs[1] + (rows > 0 ? first + tq : 0) * p.qs[2];
+                const __nv_bfloat16* from = p.q + (p.cu ? 0 : cons.c.b * p.qs[0]) + (hk * p.group + gi) * p.qs[1] + (rows > 0 ? first + tq : 0) * p.qs[2];
                 if constexpr (kBits == 16) {
 #pragma unroll
                     for (int kk = 0; kk < MT; ++kk) {
@@ -391,7 +351,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int c = row0 + nt * 8 + 2 * t + e;
-                    lim[nt][e] = p.causal ? cons.len - n + (c < rows ? c % n : 0) : cons.len - 1;
+                    lim[nt][e] = min(p.causal ? cons.c.len - n + (c < rows ? c % n : 0) : cons.c.len - 1, kend - 1);
                     m_ref[nt][e] = kNoKey;
                     bar[nt][e] = -INFINITY;
                     l_run[nt][e] = 0.f;
@@ -405,103 +365,120 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 for (int nt = 0; nt < NT; ++nt) o[mt][nt][0] = o[mt][nt][1] = o[mt][nt][2] = o[mt][nt][3] = 0.f;
             }
         }
+        for (; cons.pos < cons.end; cons.pos += NB) {   // batches of blocks
+        st = st + 1 == NS ? 0 : st + 1;
+        produce();
         cp_async_wait<NS - 1>();
         __syncwarp();
-
-        const int j0 = (cons.tile * W + warp) * 16;
-        if (j0 < cons.len) {
-            const unsigned char* sk = ring + st * S::kStage;
-            const unsigned char* sv = sk + S::kStage / 2;
-            float x[NT][4];   // q k: key g of columns 2 t, 2 t + 1, then key g + 8
-            uint2 vstep[2];   // 4 bits: (step, least) of the two keys' values
-            if constexpr (kBits == 16) {
+        const int count = min(cons.end - cons.pos, NB);
+#pragma unroll 1
+        for (int n = 0; n < count; n += PB) {
+            const int j0 = (cons.pos + n) * 16;
+            if (j0 >= kend) break;          // (an empty sequence)
+            const bool tail = j0 + 16 * PB - 1 > whole;
+            const unsigned char* stage = ring + st * S::kStage + n * S::kBlock;
+            float x[PB][NT][4];             // q k: key g of columns 2 t, 2 t + 1, then key g + 8
+            uint2 vstep[PB][2];             // 4 bits: (step, least) of the two keys' values
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
-                const uint32_t base = smem_u32(sk);
-                const int r = (lane & 7) + ((lane >> 3) & 1) * 8, c = (lane >> 4) * 8;
+            for (int i = 0; i < PB; ++i) {
+                const unsigned char *sk = stage + i * S::kBlock, *sv = sk + S::kBlock / 2;
+                if constexpr (kBits == 16) {
 #pragma unroll
-                for (int kk = 0; kk < MT; ++kk) {
-                    uint32_t a[4];
-                    ldmatrix_x4(a, base + swizzled<D>(r, kk * 16 + c));
+                    for (int nt = 0; nt < NT; ++nt) x[i][nt][0] = x[i][nt][1] = x[i][nt][2] = x[i][nt][3] = 0.f;
+                    const uint32_t base = smem_u32(sk);
+                    const int r = (lane & 7) + ((lane >> 3) & 1) * 8, c = (lane >> 4) * 8;
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_bf16(x[nt], a, qb[nt][kk][0], qb[nt][kk][1]);
-                }
-            } else {
-                uint32_t kw[2][D / 32];
-                uint2 kstep[2];
+                    for (int kk = 0; kk < MT; ++kk) {
+                        uint32_t a[4];
+                        ldmatrix_x4(a, base + swizzled<D>(r, kk * 16 + c));
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const unsigned char* row = sk + (g + 8 * h) * (D / 2);
-                    const unsigned char* steps = sk + 8 * D + (g + 8 * h) * (D / 16);
-                    const unsigned char* vsteps = sv + 8 * D + (g + 8 * h) * (D / 16);
-                    if constexpr (D == 128) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * t);
-                        kw[h][0] = w.x; kw[h][1] = w.y; kw[h][2] = w.z; kw[h][3] = w.w;
-                        kstep[h] = *reinterpret_cast<const uint2*>(steps);
-                        vstep[h] = *reinterpret_cast<const uint2*>(vsteps);
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(row + 8 * t);
-                        kw[h][0] = w.x; kw[h][1] = w.y;
-                        kstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(steps), 0u);
-                        vstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(vsteps), 0u);
+                        for (int nt = 0; nt < NT; ++nt) mma_bf16(x[i][nt], a, qb[nt][kk][0], qb[nt][kk][1]);
                     }
-                }
-                if (j0 + 16 > cons.len) {   // whatever the page holds behind the last key
+                } else {
+                    uint32_t kw[2][D / 32];
+                    uint2 kstep[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        if (j0 + g + 8 * h >= cons.len) kstep[h] = vstep[h] = make_uint2(0u, 0u);
+                        const unsigned char* row = sk + (g + 8 * h) * (D / 2);
+                        const unsigned char* steps = sk + 8 * D + (g + 8 * h) * (D / 16);
+                        const unsigned char* vsteps = sv + 8 * D + (g + 8 * h) * (D / 16);
+                        if constexpr (D == 128) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(row + 16 * t);
+                            kw[h][0] = w.x; kw[h][1] = w.y; kw[h][2] = w.z; kw[h][3] = w.w;
+                            kstep[h] = *reinterpret_cast<const uint2*>(steps);
+                            vstep[i][h] = *reinterpret_cast<const uint2*>(vsteps);
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(row + 8 * t);
+                            kw[h][0] = w.x; kw[h][1] = w.y;
+                            kstep[h] = make_uint2(*reinterpret_cast<const uint32_t*>(steps), 0u);
+                            vstep[i][h] = make_uint2(*reinterpret_cast<const uint32_t*>(vsteps), 0u);
+                        }
                     }
-                }
-#pragma unroll
-                for (int w = 0; w < G; ++w) {
-                    float acc[NT][4];
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
-#pragma unroll
-                    for (int i = 2 * w; i < 2 * w + 2; ++i) {
+                    if (tail) {   // whatever is behind the last key
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            const uint32_t a[4] = {code_pair(kw[0][i] >> (8 * h)), code_pair(kw[1][i] >> (8 * h)), code_pair(kw[0][i] >> (8 * h + 4)), code_pair(kw[1][i] >> (8 * h + 4))};
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], a, qb[nt][2 * i + h][0], qb[nt][2 * i + h][1]);
+                            if (j0 + 16 * i + g + 8 * h >= kend) kstep[h] = vstep[i][h] = make_uint2(0u, 0u);
                         }
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t pair = w ? kstep[h].y : kstep[h].x;
-                        const float ks = step_of(pair), kl = fmaf(-128.f, ks, least_of(pair));
+                    for (int w = 0; w < G; ++w) {
+                        float acc[NT][4];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
+                        for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const float at_zero = w ? fmaf(kl, qsum[nt][w][e], x[nt][2 * h + e]) : kl * qsum[nt][w][e];
-                                x[nt][2 * h + e] = fmaf(ks, acc[nt][2 * h + e], at_zero);
+                        for (int k = 2 * w; k < 2 * w + 2; ++k) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t a[4] = {code_pair(kw[0][k] >> (8 * h)), code_pair(kw[1][k] >> (8 * h)), code_pair(kw[0][k] >> (8 * h + 4)), code_pair(kw[1][k] >> (8 * h + 4))};
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma_bf16(acc[nt], a, qb[nt][2 * k + h][0], qb[nt][2 * k + h][1]);
+                            }
+                        }
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t pair = w ? kstep[h].y : kstep[h].x;
+                            const float ks = step_of(pair), kl = fmaf(-128.f, ks, least_of(pair));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const float at_zero = w ? fmaf(kl, qsum[nt][w][e], x[i][nt][2 * h + e]) : kl * qsum[nt][w][e];
+                                    x[i][nt][2 * h + e] = fmaf(ks, acc[nt][2 * h + e], at_zero);
+                                }
                             }
                         }
                     }
                 }
             }
-            if (j0 + 15 > whole) {
+            if (tail) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int i = 0; i < PB; ++i) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (j0 + g + 8 * (e >> 1) > lim[nt][e & 1]) x[nt][e] = -INFINITY;
+                    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            if (j0 + 16 * i + g + 8 * (e >> 1) > lim[nt][e & 1]) x[i][nt][e] = -INFINITY;
+                        }
                     }
                 }
             }
             bool higher = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            for (int i = 0; i < PB; ++i) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) higher |= x[nt][e] > bar[nt][e & 1];
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) higher |= x[i][nt][e] > bar[nt][e & 1];
+                }
             }
             if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float top = fmaxf(x[nt][e], x[nt][e + 2]);
+                        float top = fmaxf(x[0][nt][e], x[0][nt][e + 2]);
+#pragma unroll
+                        for (int i = 1; i < PB; ++i) top = fmaxf(top, fmaxf(x[i][nt][e], x[i][nt][e + 2]));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -525,85 +502,94 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 }
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[nt][e] = fast_exp2(fmaf(x[nt][e], p.scale_log2, -m_ref[nt][e & 1]));
-                    l_run[nt][e & 1] += x[nt][e];
-                }
-            }
-            if constexpr (kBits == 16) {
-                uint32_t pb[NT][2];
+            for (int i = 0; i < PB; ++i) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    pb[nt][0] = transposed(pack_bf16(x[nt][0], x[nt][1]));
-                    pb[nt][1] = transposed(pack_bf16(x[nt][2], x[nt][3]));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[i][nt][e] = fast_exp2(fmaf(x[i][nt][e], p.scale_log2, -m_ref[nt][e & 1]));
+                        l_run[nt][e & 1] += x[i][nt][e];
+                    }
                 }
-                const uint32_t base = smem_u32(sv);
-                const int r = (lane & 7) + (lane >> 4) * 8, c = ((lane >> 3) & 1) * 8;
+            }
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    uint32_t a[4];
-                    ldmatrix_x4_trans(a, base + swizzled<D>(r, mt * 16 + c));
+            for (int i = 0; i < PB; ++i) {
+                const unsigned char* sv = stage + i * S::kBlock + S::kBlock / 2;
+                if constexpr (kBits == 16) {
+                    uint32_t pb[NT][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_bf16(o[mt][nt], a, pb[nt][0], pb[nt][1]);
-                }
-            } else {
-                uint32_t pb[NT][G][2];
+                    for (int nt = 0; nt < NT; ++nt) {
+                        pb[nt][0] = transposed(pack_bf16(x[i][nt][0], x[i][nt][1]));
+                        pb[nt][1] = transposed(pack_bf16(x[i][nt][2], x[i][nt][3]));
+                    }
+                    const uint32_t base = smem_u32(sv);
+                    const int r = (lane & 7) + (lane >> 4) * 8, c = ((lane >> 3) & 1) * 8;
 #pragma unroll
-                for (int w = 0; w < G; ++w) {
+                    for (int mt = 0; mt < MT; ++mt) {
+                        uint32_t a[4];
+                        ldmatrix_x4_trans(a, base + swizzled<D>(r, mt * 16 + c));
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t pair = w ? vstep[h].y : vstep[h].x;
-                        const float vs = 2.f * step_of(pair), vm = fmaf(4.f, vs, least_of(pair));
+                        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[mt][nt], a, pb[nt][0], pb[nt][1]);
+                    }
+                } else {
+                    uint32_t pb[NT][G][2];
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) {
-                            pb[nt][w][h] = transposed(pack_bf16(x[nt][2 * h] * vs, x[nt][2 * h + 1] * vs));
-                            mid[nt][w][0] = fmaf(x[nt][2 * h], vm, mid[nt][w][0]);
-                            mid[nt][w][1] = fmaf(x[nt][2 * h + 1], vm, mid[nt][w][1]);
+                    for (int w = 0; w < G; ++w) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t pair = w ? vstep[i][h].y : vstep[i][h].x;
+                            const float vs = 2.f * step_of(pair), vm = fmaf(4.f, vs, least_of(pair));
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                pb[nt][w][h] = transposed(pack_bf16(x[i][nt][2 * h] * vs, x[i][nt][2 * h + 1] * vs));
+                                mid[nt][w][0] = fmaf(x[i][nt][2 * h], vm, mid[nt][w][0]);
+                                mid[nt][w][1] = fmaf(x[i][nt][2 * h + 1], vm, mid[nt][w][1]);
+                            }
                         }
                     }
-                }
-                uint32_t vw[2][2][G];   // token pairs t and t + 4: even token's words, odd token's
+                    uint32_t vw[2][2][G];   // token pairs t and t + 4: even token's words, odd token's
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int pair = t + 4 * h, place = g ^ (D == 128 ? 2 * (pair & 3) : 4 * ((pair >> 1) & 1));
-                    const unsigned char* from = sv + (pair * 8 + place) * (8 * G);
-                    if constexpr (D == 128) {
-                        const uint4 w = *reinterpret_cast<const uint4*>(from);
-                        vw[h][0][0] = w.x; vw[h][0][G - 1] = w.y; vw[h][1][0] = w.z; vw[h][1][G - 1] = w.w;
-                    } else {
-                        const uint2 w = *reinterpret_cast<const uint2*>(from);
-                        vw[h][0][0] = w.x; vw[h][1][0] = w.y;
+                    for (int h = 0; h < 2; ++h) {
+                        const int pair = t + 4 * h, place = g ^ (D == 128 ? 2 * (pair & 3) : 4 * ((pair >> 1) & 1));
+                        const unsigned char* from = sv + (pair * 8 + place) * (8 * G);
+                        if constexpr (D == 128) {
+                            const uint4 w = *reinterpret_cast<const uint4*>(from);
+                            vw[h][0][0] = w.x; vw[h][0][G - 1] = w.y; vw[h][1][0] = w.z; vw[h][1][G - 1] = w.w;
+                        } else {
+                            const uint2 w = *reinterpret_cast<const uint2*>(from);
+                            vw[h][0][0] = w.x; vw[h][1][0] = w.y;
+                        }
                     }
-                }
 #pragma unroll
-                for (int w = 0; w < G; ++w) {
-                    const uint32_t lo0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x5410), hi0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x7632);
-                    const uint32_t lo1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x5410), hi1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x7632);
-                    // Rows g and g + 8 of instruction i: channels 64 w + 8 g + 2 i and the next one.
-                    auto product = [&](auto which) {
-                        constexpr int i = decltype(which)::value;
-                        const uint32_t a[4] = {half_code_pair<i>(lo0), half_code_pair<i>(hi0), half_code_pair<i>(lo1), half_code_pair<i>(hi1)};
+                    for (int w = 0; w < G; ++w) {
+                        const uint32_t lo0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x5410), hi0 = __byte_perm(vw[0][0][w], vw[0][1][w], 0x7632);
+                        const uint32_t lo1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x5410), hi1 = __byte_perm(vw[1][0][w], vw[1][1][w], 0x7632);
+                        // Rows g and g + 8 of instruction k: channels 64 w + 8 g + 2 k and the next one.
+                        auto product = [&](auto which) {
+                            constexpr int k = decltype(which)::value;
+                            const uint32_t a[4] = {half_code_pair<k>(lo0), half_code_pair<k>(hi0), half_code_pair<k>(lo1), half_code_pair<k>(hi1)};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma_bf16(o[4 * w + i][nt], a, pb[nt][w][0], pb[nt][w][1]);
-                    };
-                    product(std::integral_constant<int, 0>());
-                    product(std::integral_constant<int, 1>());
-                    product(std::integral_constant<int, 2>());
-                    product(std::integral_constant<int, 3>());
-                    const uint32_t a[4] = {kTwelve, kTwelve, kTwelve, kTwelve};
+                            for (int nt = 0; nt < NT; ++nt) mma_bf16(o[4 * w + k][nt], a, pb[nt][w][0], pb[nt][w][1]);
+                        };
+                        product(std::integral_constant<int, 0>());
+                        product(std::integral_constant<int, 1>());
+                        product(std::integral_constant<int, 2>());
+                        product(std::integral_constant<int, 3>());
+                        const uint32_t a[4] = {kTwelve, kTwelve, kTwelve, kTwelve};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_bf16(twelve[nt][w], a, pb[nt][w][0], pb[nt][w][1]);
+                        for (int nt = 0; nt < NT; ++nt) mma_bf16(twelve[nt][w], a, pb[nt][w][0], pb[nt][w][1]);
+                    }
                 }
             }
         }
         __syncwarp();   // all lanes are done with stage `st` before it is filled again
+        }
 
-        const bool last_of_pair = !kCluster && cons.tile + 1 == cons.ntiles;
-        if (last_of_pair || u + 1 == u1) {
-            // The warps' results to shared memory, each with its own reference; then their sum in the order of the warps.
-            float* slab = reinterpret_cast<float*>(kBits == 4 ? smem + S::kRing + warp * (kRows * D * 4) : ring + st * S::kStage);
+        {
+            // The warps' results to shared memory, each with its own reference, in the stage that it consumed last (nothing is
+            // on its way there); then their sum in the order of the warps.
+            float* slab = reinterpret_cast<float*>(ring + st * S::kStage);
+            if (lane == 0) slab_s[warp] = warp * NS * S::kStage + st * S::kStage;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -660,35 +646,34 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
             }
             __syncthreads();
             auto merged = [&](int r, int c4) {
-                const unsigned char* from = (kBits == 4 ? smem + S::kRing : smem + st * S::kStage) + (r * D + slab_chunk(r, c4) * 4) * 4;
-                constexpr int kNext = kBits == 4 ? kRows * D * 4 : NS * S::kStage;
+                const unsigned char* from = smem + (r * D + slab_chunk(r, c4) * 4) * 4;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
-                    const float4 y = *reinterpret_cast<const float4*>(from + w * kNext);
+                    const float4 y = *reinterpret_cast<const float4*>(from + slab_s[w]);
                     const float f = sm_f[w * kRows + r];
                     sum.x = fmaf(y.x, f, sum.x); sum.y = fmaf(y.y, f, sum.y);
                     sum.z = fmaf(y.z, f, sum.z); sum.w = fmaf(y.w, f, sum.w);
                 }
                 return sum;
             };
-            const int rows = rows_of(cons.b, cons.hk);
+            const int rows = rows_of(p, cons.c.b, cons.c.hk, kRows);
             if constexpr (kCluster) {
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
                     const float4 sum = merged(r, c4);
-                    if (cons.ntiles == 1) write_row(cons.b, cons.hk, r, c4, sum, fin_l[r]);
+                    if (ranks_used == 1) write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, fin_l[r]);
                     else reinterpret_cast<float4*>(part_s)[idx] = sum;
                 }
                 break;
             }
-            const int pair = cons.b * p.kv_heads + cons.hk;
-            const int t0 = p.kv_heads * prefix_s[cons.b] + cons.hk * (cons.ntiles + kPairCost);   // the pair's first unit
-            const int c_first = t0 / upc, c_last = (t0 + cons.ntiles - 1) / upc;
+            const int pair = cons.c.b * p.kv_heads + cons.c.hk;
+            const int t0 = p.kv_heads * prefix_s[cons.c.b] + cons.c.hk * (cons.c.ntiles + kPairCost);   // the pair's first unit
+            const int c_first = t0 / upc, c_last = (t0 + cons.c.ntiles - 1) / upc;
             if (c_first == c_last) {
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
-                    write_row(cons.b, cons.hk, r, c4, merged(r, c4), fin_l[r]);
+                    write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, merged(r, c4), fin_l[r]);
                 }
             } else {
                 const int slot = blockIdx.x + pair;
@@ -697,29 +682,22 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                     reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D)[c4] = merged(r, c4);
                 }
                 if (threadIdx.x < kRows) {
-                    p.part_m[slot * 16 + threadIdx.x] = fin_m[threadIdx.x];
-                    p.part_l[slot * 16 + threadIdx.x] = fin_l[threadIdx.x];
+                    p.part_ml[slot * 16 + threadIdx.x] = make_float2(fin_m[threadIdx.x], fin_l[threadIdx.x]);
                 }
-                if (threadIdx.x == 0) {
-                    int* e = pend + 5 * npend_s[0];
-                    e[0] = pair; e[1] = c_first; e[2] = c_last; e[3] = cons.b; e[4] = cons.hk;
-                    npend_s[0] += 1;
-                }
-                __syncthreads();
-                if (npend_s[0] == kMaxPending || u + 1 < u1) draw_tickets();
             }
+            if (threadIdx.x == 0 && c_last == static_cast<int>(blockIdx.x)) p.pieces[pair] = make_int2(c_first + pair, c_last - c_first + 1);
             __syncthreads();
-            fresh = true;
         }
-        next(cons);
+        leave(cons);
+        if (cons.left > 0) enter(cons);
     }
     cp_async_wait<0>();
     if constexpr (kCluster) {
-        if (cons.ntiles == 1) return;   // one rank had all of it and has written it: nobody waits for anybody
+        if (ranks_used == 1) return;   // one rank had all of it and has written it: nobody waits for anybody
         cluster_meet();
         // Every rank adds up its share of the output, the ranks that had a tile in their order.
-        const int rows = rows_of(cons.b, cons.hk);
-        const int parts = min(cons.ntiles, p.ranks), all = rows * (D / 4), share = (all + p.ranks - 1) / p.ranks;
+        const int rows = rows_of(p, cons.c.b, cons.c.hk, kRows);
+        const int parts = ranks_used, all = rows * (D / 4), share = (all + p.ranks - 1) / p.ranks;
         const uint32_t at_m = smem_u32(fin_m), at_l = smem_u32(fin_l), at_o = smem_u32(part_s);
         for (int idx = rank * share + threadIdx.x; idx < min((rank + 1) * share, all); idx += kThreads) {
             const int r = idx / (D / 4), c4 = idx % (D / 4);
@@ -743,13 +721,77 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 sum.x = fmaf(v[j].x, f, sum.x); sum.y = fmaf(v[j].y, f, sum.y);
                 sum.z = fmaf(v[j].z, f, sum.z); sum.w = fmaf(v[j].w, f, sum.w);
             }
-            write_row(cons.b, cons.hk, r, c4, sum, ll);
+            write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
         }
         cluster_meet();   // nobody's shared memory goes away while another reads it
-    } else {
-        __syncthreads();
-        if (npend_s[0] > 0) draw_tickets();
     }
+}
+
+// The pairs that were cut: their partials, in the order of the CTAs that left them. A block has two rows of a pair; four
+// threads share four columns, each with every fourth partial, eight requested at a time. (A launch of its own, which starts
+// up while the stream drains: a last holder that adds them up behind a ticket keeps registers from the stream, whose
+// instructions were 30 % more for it.)
+template <int D>
+__global__ void __launch_bounds__(2 * D) merge_kernel(const __grid_constant__ PagedParams p, int tile_rows) {
+    __shared__ float4 sums[2][4][D / 4];
+    __shared__ float2 stats[2][4];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int pair = blockIdx.x, r = blockIdx.y * 2 + threadIdx.z, c4 = threadIdx.x, quarter = threadIdx.y;
+    const int2 piece = p.pieces[pair];
+    if (piece.y <= 1) return;
+    const int b = pair / p.kv_heads, vh = pair - b * p.kv_heads;
+    const bool there = r < rows_of(p, b, vh, tile_rows);
+    float mm = kNoKey, ll = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAhead = 8;
+    for (int c0 = quarter; there && c0 < piece.y; c0 += 4 * kAhead) {
+        float2 ml[kAhead];
+        float4 v[kAhead];
+        float top = mm;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            ml[j] = make_float2(kNoKey, 0.f);
+            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c0 + 4 * j < piece.y) {
+                const int64_t at = static_cast<int64_t>(piece.x + c0 + 4 * j) * 16 + r;
+                ml[j] = __ldcg(&p.part_ml[at]);
+                v[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + c4);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) top = fmaxf(top, ml[j].x);
+        const float f = fast_exp2(mm - top);
+        mm = top;
+        ll *= f;
+        sum.x *= f; sum.y *= f; sum.z *= f; sum.w *= f;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const float w = fast_exp2(ml[j].x - top);
+            ll = fmaf(ml[j].y, w, ll);
+            sum.x = fmaf(v[j].x, w, sum.x); sum.y = fmaf(v[j].y, w, sum.y);
+            sum.z = fmaf(v[j].z, w, sum.z); sum.w = fmaf(v[j].w, w, sum.w);
+        }
+    }
+    sums[threadIdx.z][quarter][c4] = sum;
+    if (c4 == 0) stats[threadIdx.z][quarter] = make_float2(mm, ll);
+    __syncthreads();
+    if (quarter || !there) return;
+    float2 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = stats[threadIdx.z][i];
+    const float top = fmaxf(fmaxf(s[0].x, s[1].x), fmaxf(s[2].x, s[3].x));
+    ll = 0.f;
+    sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float w = fast_exp2(s[i].x - top);
+        const float4 v = sums[threadIdx.z][i][c4];
+        ll = fmaf(s[i].y, w, ll);
+        sum.x = fmaf(v.x, w, sum.x); sum.y = fmaf(v.y, w, sum.y);
+        sum.z = fmaf(v.z, w, sum.z); sum.w = fmaf(v.w, w, sum.w);
+    }
+    write_row(p, b, vh, r, tile_rows, c4, sum, ll);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -827,7 +869,7 @@ int paged_set_up(int dev) {
 // CTAs per pair where each has a cluster of its own; 0 where the pairs are cut into equal shares.
 template <int D, int kBits, int NT>
 int paged_ranks(int64_t pairs, int cap, int ctas, int dev) {
-    constexpr int kTile = Shape<D, kBits, NT>::kTile;
+    constexpr int kTile = 16 * Shape<D, kBits, NT>::W;
     for (int ranks = 8; ranks >= 1; ranks /= 2) {
         if (ranks > 1 && (ranks / 2) * kTile >= cap) continue;   // half as many have a tile each
         if (pairs * ranks > ctas || cluster_room<D, kBits, NT>(dev, ranks) < pairs) continue;
@@ -838,15 +880,15 @@ int paged_ranks(int64_t pairs, int cap, int ctas, int dev) {
 }
 
 struct Parts {
-    int64_t m_bytes, o_bytes, total;
+    int64_t piece_bytes, ml_bytes, total;
 };
 Parts parts_of(int64_t pairs, int d, int ctas) {
     Parts s;
     const int64_t slots = ctas + pairs;
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    s.m_bytes = up(slots * 16 * 4);
-    s.o_bytes = up(slots * 16 * d * 4);
-    s.total = 2 * s.m_bytes + s.o_bytes;
+    s.piece_bytes = up(pairs * 8);
+    s.ml_bytes = up(slots * 16 * 8);
+    s.total = s.piece_bytes + s.ml_bytes + up(slots * 16 * d * 4);
     return s;
 }
 
@@ -871,10 +913,10 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
         s.nt = rows <= 8 ? 1 : 2;
         s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
         // Units of all pairs have to fit 30 bits.
-        int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 64 + 1 + kPairCost) * hk * s.row_tiles);
+        int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 16 + 32) * hk * s.row_tiles);
         most = most < 1 ? 1 : (most > kMaxBatch ? kMaxBatch : most);
         s.slice = static_cast<int>(a->batch < most ? a->batch : most);
-        s.bytes = parts_of(s.slice * hk * s.row_tiles, a->d, sms * 3).total;
+        s.bytes = parts_of(s.slice * hk * s.row_tiles, a->d, sms * 4).total;
         return s;
     }
     // Dense rows of some sequences at a time: 1 GB, or one sequence.
@@ -891,19 +933,24 @@ int run_few(PagedParams& p, cudaStream_t stream) {
     using S = Shape<D, kBits, NT>;
     const int dev = current_device();
     if (int rc = paged_set_up<D, kBits, NT>(dev)) return rc;
-    int ctas = S::kCtas * sm_count(dev);
-    if (ctas > kMaxCtas) ctas = kMaxCtas;
+    const int ctas = S::kCtas * sm_count(dev);
     const int64_t pairs = static_cast<int64_t>(p.batch) * p.kv_heads;
     p.ranks = paged_ranks<D, kBits, NT>(pairs, p.c.cap, ctas, dev);
     cudaLaunchAttribute attr[2];
-    auto go = [&](auto kernel, cudaLaunchConfig_t cfg) {
+    auto go = [&](cudaLaunchConfig_t cfg, auto kernel, auto... args) {
+        cfg.attrs = attr;
         attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
         ++cfg.numAttrs;
-        return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "paged_sdpa launch");
+        return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "paged_sdpa launch");
     };
-    if (p.ranks > 0) return go(paged_kernel<D, kBits, NT, true>, paged_config<D, kBits, NT, true>(static_cast<int>(pairs) * p.ranks, p.ranks, stream, attr));
-    return go(paged_kernel<D, kBits, NT, false>, paged_config<D, kBits, NT, false>(ctas, 1, stream, attr));
+    if (p.ranks > 0) return go(paged_config<D, kBits, NT, true>(static_cast<int>(pairs) * p.ranks, p.ranks, stream, attr), paged_kernel<D, kBits, NT, true>, p);
+    if (int rc = go(paged_config<D, kBits, NT, false>(ctas, 1, stream, attr), paged_kernel<D, kBits, NT, false>, p)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(pairs), S::kRows / 2);
+    cfg.blockDim = dim3(D / 4, 4, 2);
+    cfg.stream = stream;
+    return go(cfg, merge_kernel<D>, p, static_cast<int>(S::kRows));
 }
 
 template <int D, int kBits>
@@ -919,7 +966,7 @@ const char* sdpa_refusal(const ktt_b200_paged_sdpa_args* a, Pages& c) {
         if (a->q_strides[i] % 2 || a->out_strides[i] % 4) return "q strides must be even and out strides multiples of 4";
     }
     if ((reinterpret_cast<uintptr_t>(a->q) & 3) || (reinterpret_cast<uintptr_t>(a->out) & 7)) return "q must be 4-byte and out 8-byte aligned";
-    if ((static_cast<int64_t>(c.cap) / 64 + 1 + kPairCost) * a->cache.kv_heads * 8 > (1ll << 30)) return "too many keys and heads";
+    if ((static_cast<int64_t>(c.cap) / 16 + 32) * a->cache.kv_heads * 8 > (1ll << 30)) return "too many keys and heads";
     return nullptr;
 }
 
@@ -950,8 +997,8 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice,
         f.v = v;
         f.out = p.out;
         f.lse_strides[2] = 1;
-        f.workspace = a->counters;
-        f.workspace_bytes = 256;
+        f.workspace = a->counter;
+        f.workspace_bytes = a->counter ? 256 : 0;
         // All rows of a head together, sequence after sequence: a dense call's keys, and a packed one's.
         const int64_t strides[3] = {cap * d, slice * cap * d, d};
         for (int i = 0; i < 3; ++i) {
@@ -995,6 +1042,10 @@ extern "C" int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args*
     return a->sq == 0 ? 0 : plan_of(a, c, sm_count(current_device())).bytes;
 }
 
+extern "C" int ktt_b200_paged_sdpa_is_chunk(const ktt_b200_paged_sdpa_args* a) {
+    return a && a->cache.kv_heads > 0 && rows_per_head(a) > kFewRows;
+}
+
 extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stream) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null arguments");
     PagedParams p = {};
@@ -1008,11 +1059,11 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null pointer");
     }
     const Plan s = plan_of(a, p.c, sm_count(current_device()));
-    if (!a->counters || !a->workspace || a->workspace_bytes < s.bytes) {
-        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: counters and %lld bytes of workspace are needed", static_cast<long long>(s.bytes));
+    if (!a->workspace || a->workspace_bytes < s.bytes) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: workspace holds %lld bytes, %lld needed", static_cast<long long>(a->workspace_bytes), static_cast<long long>(s.bytes));
     }
-    if ((reinterpret_cast<uintptr_t>(a->counters) | reinterpret_cast<uintptr_t>(a->workspace)) & 15) {
-        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: counters and workspace must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(a->counter) | reinterpret_cast<uintptr_t>(a->workspace)) & 15) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: counter and workspace must be 16-byte aligned");
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     p.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -1031,12 +1082,11 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
         p.os[i] = a->out_strides[i];
     }
     p.total_q = a->total_q;
-    const Parts parts = parts_of(static_cast<int64_t>(s.slice) * p.kv_heads, a->d, sm_count(current_device()) * 3);
+    const Parts parts = parts_of(static_cast<int64_t>(s.slice) * p.kv_heads, a->d, sm_count(current_device()) * 4);
     unsigned char* base = static_cast<unsigned char*>(a->workspace);
-    p.counters = static_cast<int32_t*>(a->counters);
-    p.part_m = reinterpret_cast<float*>(base);
-    p.part_l = reinterpret_cast<float*>(base + parts.m_bytes);
-    p.part_o = reinterpret_cast<float*>(base + 2 * parts.m_bytes);
+    p.pieces = reinterpret_cast<int2*>(base);
+    p.part_ml = reinterpret_cast<float2*>(base + parts.piece_bytes);
+    p.part_o = reinterpret_cast<float*>(base + parts.piece_bytes + parts.ml_bytes);
     const Pages all = p.c;
     note_call(3);
     for (int b0 = 0; b0 < a->batch; b0 += s.slice) {

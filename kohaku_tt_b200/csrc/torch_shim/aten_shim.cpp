@@ -195,10 +195,6 @@ ZeroedPool& decode_pool() {
     static ZeroedPool* pool = new ZeroedPool;
     return *pool;
 }
-ZeroedPool& paged_pool() {
-    static ZeroedPool* pool = new ZeroedPool;
-    return *pool;
-}
 
 // The tcgen05 forward's workspace. Without a mask that has a row per query it is the counter the
 // CTAs draw their tiles from, which the kernel leaves zero. A plan of such a mask is up to 1 GB and
@@ -1308,8 +1304,12 @@ PyObject* py_sdpa_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (cu) a.cu_seqlens_q = cu->data_ptr<int32_t>();
         const int64_t need = ktt_b200_paged_sdpa_workspace(&a);
         if (need < 0) raise_status(KTT_B200_ERR_UNSUPPORTED, "sdpa_paged");
-        const Tensor counters = paged_pool().get(4096, 4096, *q, stream), work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
-        a.counters = counters.data_ptr();
+        const Tensor work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
+        Tensor counter;
+        if (ktt_b200_paged_sdpa_is_chunk(&a)) {
+            counter = forward_pool().get(kCounterBytes, kCounterBytes, *q, stream);
+            a.counter = counter.data_ptr();
+        }
         a.workspace = work.data_ptr();
         a.workspace_bytes = need;
         raise_status(ktt_b200_paged_sdpa(&a, stream), "sdpa_paged");
@@ -1322,7 +1322,6 @@ PyObject* py_sdpa_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* py_drop_workspaces(PyObject*, PyObject*) {
     forward_pool().clear();
     decode_pool().clear();
-    paged_pool().clear();
     Py_RETURN_NONE;
 }
 

@@ -150,15 +150,15 @@ def _read(k_pages, v_pages, block_table, lengths, max_k):
 _COUNTERS = {}
 
 
-def _counters(device):
-    """Tickets of the split over the keys: zero before a call, and after it. A buffer per device and stream; a
-    captured call has its own, which its graph fills at every replay."""
+def _counter(device):
+    """The work counter of the forward that does chunks of prompts: zero before a call, and after it. A buffer
+    per device and stream; a captured call has its own, which its graph fills at every replay."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros((4096,), dtype=torch.uint8, device=device)
+        return torch.zeros((256,), dtype=torch.uint8, device=device)
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
     buf = _COUNTERS.get(key)
     if buf is None:
-        buf = _COUNTERS[key] = torch.zeros((4096,), dtype=torch.uint8, device=device)
+        buf = _COUNTERS[key] = torch.zeros((256,), dtype=torch.uint8, device=device)
     return buf
 
 
@@ -193,8 +193,10 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
         need = _lib.lib().ktt_b200_paged_sdpa_workspace(ctypes.byref(a))
         if need < 0:
             _lib.check(_lib.ERR_UNSUPPORTED, what)
-        counters, work = _counters(q.device), torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
-        a.counters, a.workspace, a.workspace_bytes = counters.data_ptr(), work.data_ptr(), work.numel()
+        work = torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
+        counter = _counter(q.device) if _lib.lib().ktt_b200_paged_sdpa_is_chunk(ctypes.byref(a)) else None
+        a.counter = None if counter is None else counter.data_ptr()
         _lib.check(_lib.lib().ktt_b200_paged_sdpa(ctypes.byref(a), ops._stream(q.device)), what)
     return out
 
