@@ -35,6 +35,10 @@ int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int row
 
 namespace {
 
+// Partials: a CTA cuts two pairs at most, the one it starts in and the one it ends in. That one, where the pair starts in the
+// CTA, has the CTA's second slot, the other its first.
+__device__ __forceinline__ int slot_of(int cta, bool starts_here) { return 2 * cta + (starts_here ? 1 : 0); }
+
 struct PagedParams {
     Pages c;
     int batch, heads;
@@ -47,7 +51,7 @@ struct PagedParams {
     int64_t qs[3], os[3];
     const int32_t* cu;       // packed queries
     int64_t total_q;
-    int2* pieces;            // [pairs] first slot of a pair's partials, and how many it has (1: none, its result is written)
+    int2* pieces;            // [pairs] the first CTA of a pair, and how many have a piece of it (1: its result is written)
     float2* part_ml;         // [slots][16] maximum and sum
     float* part_o;           // [slots][16][D]
     int ranks;               // CTAs of a cluster
@@ -676,7 +680,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                     write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, merged(r, c4), fin_l[r]);
                 }
             } else {
-                const int slot = blockIdx.x + pair;
+                const int slot = slot_of(blockIdx.x, c_first == static_cast<int>(blockIdx.x));
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
                     reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D)[c4] = merged(r, c4);
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                     p.part_ml[slot * 16 + threadIdx.x] = make_float2(fin_m[threadIdx.x], fin_l[threadIdx.x]);
                 }
             }
-            if (threadIdx.x == 0 && c_last == static_cast<int>(blockIdx.x)) p.pieces[pair] = make_int2(c_first + pair, c_last - c_first + 1);
+            if (threadIdx.x == 0 && c_last == static_cast<int>(blockIdx.x)) p.pieces[pair] = make_int2(c_first, c_last - c_first + 1);
             __syncthreads();
         }
         leave(cons);
@@ -753,8 +757,9 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const __grid_constant__ Pa
         for (int j = 0; j < kAhead; ++j) {
             ml[j] = make_float2(kNoKey, 0.f);
             v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (c0 + 4 * j < piece.y) {
-                const int64_t at = static_cast<int64_t>(piece.x + c0 + 4 * j) * 16 + r;
+            const int i = c0 + 4 * j;
+            if (i < piece.y) {
+                const int64_t at = static_cast<int64_t>(slot_of(piece.x + i, i == 0)) * 16 + r;
                 ml[j] = __ldcg(&p.part_ml[at]);
                 v[j] = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D) + c4);
             }
@@ -884,7 +889,7 @@ struct Parts {
 };
 Parts parts_of(int64_t pairs, int d, int ctas) {
     Parts s;
-    const int64_t slots = ctas + pairs;
+    const int64_t slots = 2 * static_cast<int64_t>(ctas);
     auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
     s.piece_bytes = up(pairs * 8);
     s.ml_bytes = up(slots * 16 * 8);
@@ -892,9 +897,12 @@ Parts parts_of(int64_t pairs, int d, int ctas) {
     return s;
 }
 
-// Rows of a K / V head (its heads x tokens) up to which its keys are passed over once for every 8 or 16 of them; more
-// rows are a matter for the tensor path (below).
-constexpr int kFewRows = 64;
+// Tokens of a sequence up to which a K / V head's keys are passed over once for every 8 or 16 of its rows (heads x tokens);
+// more are a matter for the tensor path (below), which takes 128 tokens of one head at a time, full or not. Measured, us, this
+// pass and that path, bf16 and 4 bits: 32 x 16 heads x up to 1,024 keys, D 64, 16 tokens 31 and 70, 25 and 64, 64 tokens 92 and 72,
+// 75 and 66; 32 x 32 heads over 8 x 2,048, D 128, 16 tokens 104 and 164, 95 and 161; 1 x 32 over 8 x 8,192, 32 tokens 26 and 48,
+// 25 and 49, 128 tokens 72 and 49, 71 and 51.
+constexpr int kFewTokens = 48;
 
 // What a call will do, from its sizes alone.
 struct Plan {
@@ -908,7 +916,7 @@ int64_t rows_per_head(const ktt_b200_paged_sdpa_args* a) { return static_cast<in
 Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     Plan s = {};
     const int64_t rows = rows_per_head(a), hk = a->cache.kv_heads;
-    s.few = rows <= kFewRows;
+    s.few = a->sq <= kFewTokens;
     if (s.few) {
         s.nt = rows <= 8 ? 1 : 2;
         s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
@@ -1043,7 +1051,7 @@ extern "C" int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args*
 }
 
 extern "C" int ktt_b200_paged_sdpa_is_chunk(const ktt_b200_paged_sdpa_args* a) {
-    return a && a->cache.kv_heads > 0 && rows_per_head(a) > kFewRows;
+    return a && a->sq > kFewTokens;
 }
 
 extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stream) {

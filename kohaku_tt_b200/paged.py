@@ -147,18 +147,15 @@ def _read(k_pages, v_pages, block_table, lengths, max_k):
     return k, v
 
 
-_COUNTERS = {}
-
-
 def _counter(device):
-    """The work counter of the forward that does chunks of prompts: zero before a call, and after it. A buffer
-    per device and stream; a captured call has its own, which its graph fills at every replay."""
+    """The work counter of the forward that does chunks of prompts (ops.forward_workspace's); a captured call has its
+    own, which its graph fills at every replay."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros((256,), dtype=torch.uint8, device=device)
+        return torch.zeros((ops._COUNTER_BYTES,), dtype=torch.uint8, device=device)
     key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    buf = _COUNTERS.get(key)
+    buf = ops._FORWARD_WORKSPACE.get(key)
     if buf is None:
-        buf = _COUNTERS[key] = torch.zeros((256,), dtype=torch.uint8, device=device)
+        buf = ops._FORWARD_WORKSPACE[key] = torch.zeros((ops._COUNTER_BYTES,), dtype=torch.uint8, device=device)
     return buf
 
 
@@ -248,13 +245,13 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     (and the step's queries alongside), in one launch.
 
     k, v: bf16 [B, Hk, S, D], or packed [T, Hk, D] with cu_seq (B + 1 offsets, a list, or int32 on the
-    device; rows that no sequence covers are left alone). Row i of sequence b goes to place lengths[b] + i:
+    device; rows that no sequence covers are not read). No two sequences may append to one page in one call. Row i of sequence b goes to place lengths[b] + i:
     row p % page_size of page block_table[b, p // page_size]. An entry that is no page of the cache (-1, say)
     takes nothing, nor does a place past the table. lengths: int32 [B] on the device, keys cached so far; they
     are not changed, lengths_out (optional, another buffer) receives the new ones.
     cos, sin: rotary_table's, one row per place of the cache; without them keys go in as they are. Rotation as
     in `rotary` (interleaved; columns past 2 * pairs are copied), the result in bf16.
-    q: bf16 [B, H, S, D] or [T, H, D]; returned rotated (None without q).
+    q: bf16 [B, H, S, D] or [T, H, D]; returned rotated (None without q; packed rows of no sequence undefined).
     Pages of 4 bits (paged_cache(bits=4)) hold each 64 channels of a row as codes 0 to 15 of
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
     interleaved = bool(interleaved)
