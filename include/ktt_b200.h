@@ -440,14 +440,12 @@ typedef struct ktt_b200_paged_sdpa_args {
     void* out;
     int64_t q_strides[3], out_strides[3];
     const int32_t* cu_seqlens_q;
-    void* counter;                 /* optional, 256 bytes as ktt_b200_attn_args.workspace has them: chunks of prompts */
     void* workspace;               /* ktt_b200_paged_sdpa_workspace() bytes, 16-byte aligned, of any content */
     int64_t workspace_bytes;
 } ktt_b200_paged_sdpa_args;
 /* Bytes of workspace of a call of these sizes; -1: refused. Chunks of prompts take dense rows of some sequences' keys there, 1 GB
- * or one sequence's at most. ktt_b200_paged_sdpa_is_chunk: 1 where the call is one of those (its `counter` is used), else 0. */
+ * or one sequence's at most. */
 KTT_B200_API int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args* args);
-KTT_B200_API int ktt_b200_paged_sdpa_is_chunk(const ktt_b200_paged_sdpa_args* args);
 KTT_B200_API int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* args, void* stream);
 
 #ifdef __cplusplus

@@ -67,7 +67,6 @@ EXPORTS = (
     "ktt_b200_paged_read",
     "ktt_b200_paged_sdpa",
     "ktt_b200_paged_sdpa_workspace",
-    "ktt_b200_paged_sdpa_is_chunk",
 )
 
 _i32, _i64, _f32, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -274,7 +273,6 @@ class PagedSdpaArgs(ctypes.Structure):
         ("q_strides", _i64 * 3),
         ("out_strides", _i64 * 3),
         ("cu_seqlens_q", _ptr),
-        ("counter", _ptr),
         ("workspace", _ptr),
         ("workspace_bytes", _i64),
     ]
@@ -438,7 +436,6 @@ def lib():
     handle.ktt_b200_paged_read.argtypes = [ctypes.POINTER(ReadArgs), _ptr]
     handle.ktt_b200_paged_sdpa_workspace.argtypes = [ctypes.POINTER(PagedSdpaArgs)]
     handle.ktt_b200_paged_sdpa_workspace.restype = _i64
-    handle.ktt_b200_paged_sdpa_is_chunk.argtypes = [ctypes.POINTER(PagedSdpaArgs)]
     handle.ktt_b200_paged_sdpa.argtypes = [ctypes.POINTER(PagedSdpaArgs), _ptr]
     if handle.ktt_b200_abi_version() != 1:
         raise RuntimeError("kohaku_tt_b200: libktt_b200.so has another ABI version")

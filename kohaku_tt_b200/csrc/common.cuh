@@ -33,6 +33,9 @@ struct AttnParams {
     const int32_t* key_lengths;
     const int32_t* cu_q;
     const int32_t* cu_k;
+    // Forward, head dim 128, optional (with a work counter): batch entries by falling length, the order in which their tiles
+    // are drawn.
+    const int32_t* order;
     // backward
     const __nv_bfloat16* dout;
     __nv_bfloat16* dq;
@@ -221,6 +224,8 @@ int ensure_smem(K kernel, int bytes, const char* what) {
     return check_cuda(raise_smem_limit(kernel, bytes), what);
 }
 
+// ktt_b200_sdpa_forward, with an order of the batch entries (AttnParams.order, or null).
+int forward_in_order(const ktt_b200_attn_args* a, const int32_t* order, cudaStream_t stream);
 // Launchers (one per kernel family).
 int launch_forward_mma(const AttnParams& p, cudaStream_t stream);
 int launch_backward_mma(const AttnParams& p, cudaStream_t stream);

@@ -156,6 +156,7 @@ __device__ __forceinline__ Work decode_work(const Tc5Params& tp, int w) {
         k.b = div_by(pair, tp.by_kv_heads);
         k.h = (pair - k.b * p.kv_heads) * group + (r - tile * group);
         qb = tp.q_tiles - 1 - tile;
+        if (p.order) k.b = p.order[k.b];   // (the longest sequence's tiles first)
     } else {
         const int t = div_by(w, tp.by_heads), level = div_by(t, tp.by_batch);
         k.h = w - t * p.heads;
@@ -1079,7 +1080,7 @@ int launch_tc5(const AttnParams& p, cudaStream_t stream) {
     const bool explicit_counter = p.fwd_work_counter && !p.fwd_done_counter;
     tp.work_counter = (large || explicit_counter) ? p.fwd_work_counter : nullptr;
     tp.done_counter = tp.work_counter ? p.fwd_done_counter : nullptr;
-    tp.grouped = (tp.work_counter && large) ? 1 : 0;
+    tp.grouped = (tp.work_counter && (large || p.order)) ? 1 : 0;
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const int grid = tp.work < sms ? tp.work : sms;  // persistent: one CTA per SM

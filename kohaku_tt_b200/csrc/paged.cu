@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
 struct ReadParams {
     Pages c;
     int rows;
-    int32_t* cu_k;   // optional: gets 0, rows, 2 rows, ...
+    int32_t* head;   // optional: 64 words that are cleared, then 0, rows, 2 rows, ..., then the sequences by falling length
     __nv_bfloat16* k;
     __nv_bfloat16* v;
     int64_t ks[3], vs[3];
@@ -214,10 +214,23 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int len = cached_keys(p.c, b);
-    if (p.cu_k && blockIdx.x == 0 && head == 0 && threadIdx.x == 0) {
-        p.cu_k[b] = b * p.rows;
-        if (b == static_cast<int>(gridDim.z) - 1) p.cu_k[b + 1] = (b + 1) * p.rows;
+    if (p.head && blockIdx.x == 0 && head == 0) {
+        if (threadIdx.x == 0) {
+            p.head[64 + b] = b * p.rows;
+            if (b == static_cast<int>(gridDim.z) - 1) p.head[64 + b + 1] = (b + 1) * p.rows;
+        }
+        if (b == 0 && threadIdx.x < 64) p.head[threadIdx.x] = 0;
+        const int batch = gridDim.z;
+        int place = 0;
+        for (int i0 = 0; i0 < batch; i0 += 256) {
+            const int i = i0 + threadIdx.x, other = i < batch ? cached_keys(p.c, i) : -1;
+            place += __syncthreads_count(other > len || (other == len && i < b));
+        }
+        if (threadIdx.x == 0) p.head[64 + batch + 1 + place] = b;
     }
+    // For the forward's sake no row behind a length is written, but one of a sequence without keys, which counts as one there.
+    const int rows = p.head ? min(max(len, 1), p.rows) : p.rows;
+    if (blockIdx.x * (kReadRows * kTokens) >= rows) return;
     const unsigned char *kp[kReadRows], *vp[kReadRows];
     int token[kReadRows];
 #pragma unroll
@@ -257,7 +270,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
 #pragma unroll
     for (int i = 0; i < kReadRows; ++i) {
         const int j = first + i * kTokens;
-        if (j >= p.rows) break;
+        if (j >= rows) break;
         if constexpr (kBits == 4) {
             k[i] = of_four_bits(words[i][0], words[i][1]);
             v[i] = of_four_bits(words[i][2], words[i][3]);
@@ -317,11 +330,11 @@ int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, c
 
 }  // namespace
 
-int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* cu_k, cudaStream_t stream) {
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, cudaStream_t stream) {
     ReadParams p = {};
     p.c = c;
     p.rows = rows;
-    p.cu_k = cu_k;
+    p.head = head;
     p.k = static_cast<__nv_bfloat16*>(k);
     p.v = static_cast<__nv_bfloat16*>(v);
     for (int i = 0; i < 3; ++i) p.ks[i] = p.vs[i] = strides[i];

@@ -30,8 +30,9 @@
 
 namespace ktt {
 
-// paged.cu: dense rows of the cache for a chunk of a prompt; cu_k (optional) gets the offsets 0, rows, 2 rows, ...
-int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* cu_k, cudaStream_t stream);
+// paged.cu: dense rows of the cache for a chunk of a prompt; 64 words of `head` are cleared, behind them go the offsets 0, rows,
+// 2 rows, ... (batch + 1), and the sequences by falling length.
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, cudaStream_t stream);
 
 namespace {
 
@@ -68,10 +69,10 @@ struct Shape {
     static constexpr int NB = kBits == 16 ? 1 : (D == 128 && NT == 1 ? 2 : 4);   // blocks of a stage
     static constexpr int PB = kBits == 4 && NT == 1 ? 2 : 1;                 // blocks that the products are of at a time
     static constexpr int kStage = NB * kBlock;
-    static constexpr int NS = kBits == 4 ? 2 : (D == 64 ? 6 : 3);
+    static constexpr int NS = kBits == 4 ? 2 : NT == 1 ? (D == 64 ? 3 : 2) : (D == 64 ? 6 : 3);
     static constexpr int kRows = 8 * NT;
     static constexpr int kPairCost = kBits == 4 ? 24 : (D == 64 ? 24 : 16);   // what ending a pair costs a CTA, in blocks
-    static constexpr int kCtas = kBits == 16 ? 2 : D == 64 ? (NT == 1 ? 4 : 3) : (NT == 1 ? 3 : 2);   // per SM
+    static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : kBits == 4 ? 3 : 2) : (kBits == 4 && NT == 1 ? 3 : 2);   // per SM
     static constexpr int kRing = W * NS * kStage;
     static constexpr int kStats = (3 * W + 2) * kRows * 4 + W * 4;
     static_assert(kStage >= kRows * D * 4, "a warp leaves its result in the stage it consumed last");
@@ -932,7 +933,7 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     const int64_t most = (1ll << 30) / one;
     s.slice = static_cast<int>(most < 1 ? 1 : (most < a->batch ? most : a->batch));
     if (s.slice > kMaxBatch) s.slice = kMaxBatch;
-    s.bytes = s.slice * one + 4096;   // offsets of the slice's keys behind the rows
+    s.bytes = s.slice * one + (64 + 2 * kMaxBatch + 1) * 4;   // and what is behind the rows (run_many)
     return s;
 }
 
@@ -986,7 +987,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice,
     const int64_t cap = p.c.cap, half = slice * cap * hk * d;
     __nv_bfloat16* k = static_cast<__nv_bfloat16*>(a->workspace);
     __nv_bfloat16* v = k + half;
-    int32_t* cu_k = reinterpret_cast<int32_t*>(v + half);
+    int32_t* head = reinterpret_cast<int32_t*>(v + half);   // the forward's work counter, the offsets of the dense rows, the order
     for (int b0 = 0; b0 < a->batch; b0 += slice) {
         const int n = a->batch - b0 < slice ? a->batch - b0 : slice;
         Pages c = p.c;
@@ -1005,8 +1006,13 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice,
         f.v = v;
         f.out = p.out;
         f.lse_strides[2] = 1;
-        f.workspace = a->counter;
-        f.workspace_bytes = a->counter ? 256 : 0;
+        // Sequences differ in length: their tiles are drawn, the longest sequence's first. (The head-dim-128 kernel does so with a
+        // counter of fewer than 256 bytes, which has to be zero before the call, and an order; the head-dim-64 kernel takes 256
+        // bytes and its own order.) 4 sequences of up to 512 tokens and 8,192 keys, 16 heads over 4, D 128, dealt in the order of the
+        // batch, drawn in it, and drawn by length: 121, 122 and 111 us.
+        const bool several = n > 1;
+        f.workspace = d == 64 || several ? head : nullptr;
+        f.workspace_bytes = d == 64 ? 256 : several ? 16 : 0;
         // All rows of a head together, sequence after sequence: a dense call's keys, and a packed one's.
         const int64_t strides[3] = {cap * d, slice * cap * d, d};
         for (int i = 0; i < 3; ++i) {
@@ -1020,14 +1026,14 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice,
             f.total_q = a->total_q;
             f.total_k = slice * cap;
             f.cu_seqlens_q = a->cu_seqlens_q + b0;
-            f.cu_seqlens_k = cu_k;
+            f.cu_seqlens_k = head + 64;
             f.q_strides[0] = f.out_strides[0] = f.k_strides[0] = f.v_strides[0] = 0;
         } else {
             f.q = p.q + b0 * a->q_strides[0];
             f.out = p.out + b0 * a->out_strides[0];
         }
-        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, a->cu_seqlens_q ? cu_k : nullptr, stream)) return rc;
-        if (int rc = ktt_b200_sdpa_forward(&f, stream)) return rc;
+        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, stream)) return rc;
+        if (int rc = forward_in_order(&f, d == 128 && several ? head + 64 + n + 1 : nullptr, stream)) return rc;
     }
     return 0;
 }
@@ -1050,10 +1056,6 @@ extern "C" int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args*
     return a->sq == 0 ? 0 : plan_of(a, c, sm_count(current_device())).bytes;
 }
 
-extern "C" int ktt_b200_paged_sdpa_is_chunk(const ktt_b200_paged_sdpa_args* a) {
-    return a && a->sq > kFewTokens;
-}
-
 extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stream) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null arguments");
     PagedParams p = {};
@@ -1070,9 +1072,7 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
     if (!a->workspace || a->workspace_bytes < s.bytes) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: workspace holds %lld bytes, %lld needed", static_cast<long long>(a->workspace_bytes), static_cast<long long>(s.bytes));
     }
-    if ((reinterpret_cast<uintptr_t>(a->counter) | reinterpret_cast<uintptr_t>(a->workspace)) & 15) {
-        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: counter and workspace must be 16-byte aligned");
-    }
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: the workspace must be 16-byte aligned");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     p.q = static_cast<const __nv_bfloat16*>(a->q);
     p.out = static_cast<__nv_bfloat16*>(a->out);

@@ -1305,11 +1305,6 @@ PyObject* py_sdpa_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t need = ktt_b200_paged_sdpa_workspace(&a);
         if (need < 0) raise_status(KTT_B200_ERR_UNSUPPORTED, "sdpa_paged");
         const Tensor work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
-        Tensor counter;
-        if (ktt_b200_paged_sdpa_is_chunk(&a)) {
-            counter = forward_pool().get(kCounterBytes, kCounterBytes, *q, stream);
-            a.counter = counter.data_ptr();
-        }
         a.workspace = work.data_ptr();
         a.workspace_bytes = need;
         raise_status(ktt_b200_paged_sdpa(&a, stream), "sdpa_paged");

@@ -147,18 +147,6 @@ def _read(k_pages, v_pages, block_table, lengths, max_k):
     return k, v
 
 
-def _counter(device):
-    """The work counter of the forward that does chunks of prompts (ops.forward_workspace's); a captured call has its
-    own, which its graph fills at every replay."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.zeros((ops._COUNTER_BYTES,), dtype=torch.uint8, device=device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream)
-    buf = ops._FORWARD_WORKSPACE.get(key)
-    if buf is None:
-        buf = ops._FORWARD_WORKSPACE[key] = torch.zeros((ops._COUNTER_BYTES,), dtype=torch.uint8, device=device)
-    return buf
-
-
 def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k):
     what = "sdpa_paged"
     ops._require_cuda(q)
@@ -192,8 +180,6 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
             _lib.check(_lib.ERR_UNSUPPORTED, what)
         work = torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
         a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
-        counter = _counter(q.device) if _lib.lib().ktt_b200_paged_sdpa_is_chunk(ctypes.byref(a)) else None
-        a.counter = None if counter is None else counter.data_ptr()
         _lib.check(_lib.lib().ktt_b200_paged_sdpa(ctypes.byref(a), ops._stream(q.device)), what)
     return out
 
