@@ -46,6 +46,7 @@ struct PagedParams {
     int kv_heads;            // of the pairs: K / V heads x row tiles
     int row_tiles, group, sq, causal;
     int page_blocks;         // blocks of 16 keys in a page
+    int table_width;
     float scale_log2;
     const __nv_bfloat16* q;
     __nv_bfloat16* out;
@@ -74,7 +75,7 @@ struct Shape {
     static constexpr int kPairCost = kBits == 4 ? 24 : (D == 64 ? 24 : 16);   // what ending a pair costs a CTA, in blocks
     static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : kBits == 4 ? 3 : 2) : (kBits == 4 && NT == 1 ? 3 : 2);   // per SM
     static constexpr int kRing = W * NS * kStage;
-    static constexpr int kStats = (3 * W + 2) * kRows * 4 + W * 4;
+    static constexpr int kStats = (2 * W + 2) * kRows * 4 + W * 4;
     static_assert(kStage >= kRows * D * 4, "a warp leaves its result in the stage it consumed last");
     static constexpr int smem(bool cluster) {
         return kRing + kStats + (cluster ? kRows * D * 4 : (2 * kMaxBatch + 1 + 8) * 4);
@@ -166,8 +167,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
     unsigned char* ring = smem + warp * NS * S::kStage;     // this warp's
     float* sm_m = reinterpret_cast<float*>(smem + S::kRing);   // [W][kRows]
     float* sm_l = sm_m + W * kRows;
-    float* sm_f = sm_l + W * kRows;    // a warp's weight in its CTA's sum
-    float* fin_m = sm_f + W * kRows;   // [kRows]
+    float* fin_m = sm_l + W * kRows;   // [kRows]: kCluster, the CTA's
     float* fin_l = fin_m + kRows;
     int* slab_s = reinterpret_cast<int*>(fin_l + kRows);       // [W] where a warp left its result
     int* prefix_s = slab_s + W;        // [kMaxBatch + 1]
@@ -189,6 +189,8 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
         rank = static_cast<int>(blockIdx.x) - pair * p.ranks;
         cons.c.b = pair / p.kv_heads;
         cons.c.hk = pair - cons.c.b * p.kv_heads;
+        // The sequence's row of the table comes along with its length.
+        if (lane * 32 < p.table_width) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.c.table + cons.c.b * p.c.table_stride + lane * 32));
         cons.c.len = cached_keys(p.c, cons.c.b);
         cons.c.ntiles = max((cons.c.len + 15) / 16, 1);
         // A rank has a block for each warp, or more.
@@ -634,29 +636,19 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 }
             }
             __syncthreads();
-            if (threadIdx.x < kRows) {
-                const int r = threadIdx.x;
-                float mm = -INFINITY, ll = 0.f;
-#pragma unroll
-                for (int w = 0; w < W; ++w) mm = fmaxf(mm, sm_m[w * kRows + r]);
-                const float base = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-                for (int w = 0; w < W; ++w) {
-                    const float f = fast_exp2(sm_m[w * kRows + r] - base);
-                    sm_f[w * kRows + r] = f;
-                    ll = fmaf(sm_l[w * kRows + r], f, ll);
-                }
-                fin_m[r] = mm;
-                fin_l[r] = ll;
-            }
-            __syncthreads();
-            auto merged = [&](int r, int c4) {
+            // Four columns of a row, its maximum and its sum: of all warps.
+            auto merged = [&](int r, int c4, float& mm, float& ll) {
                 const unsigned char* from = smem + (r * D + slab_chunk(r, c4) * 4) * 4;
                 float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+                mm = sm_m[r];
+                ll = 0.f;
+#pragma unroll
+                for (int w = 1; w < W; ++w) mm = fmaxf(mm, sm_m[w * kRows + r]);
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     const float4 y = *reinterpret_cast<const float4*>(from + slab_s[w]);
-                    const float f = sm_f[w * kRows + r];
+                    const float f = fast_exp2(sm_m[w * kRows + r] - mm);
+                    ll = fmaf(sm_l[w * kRows + r], f, ll);
                     sum.x = fmaf(y.x, f, sum.x); sum.y = fmaf(y.y, f, sum.y);
                     sum.z = fmaf(y.z, f, sum.z); sum.w = fmaf(y.w, f, sum.w);
                 }
@@ -666,9 +658,17 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
             if constexpr (kCluster) {
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
-                    const float4 sum = merged(r, c4);
-                    if (ranks_used == 1) write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, fin_l[r]);
-                    else reinterpret_cast<float4*>(part_s)[idx] = sum;
+                    float mm, ll;
+                    const float4 sum = merged(r, c4, mm, ll);
+                    if (ranks_used == 1) {
+                        write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
+                        continue;
+                    }
+                    reinterpret_cast<float4*>(part_s)[idx] = sum;
+                    if (c4 == 0) {
+                        fin_m[r] = mm;
+                        fin_l[r] = ll;
+                    }
                 }
                 break;
             }
@@ -678,16 +678,17 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
             if (c_first == c_last) {
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
-                    write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, merged(r, c4), fin_l[r]);
+                    float mm, ll;
+                    const float4 sum = merged(r, c4, mm, ll);
+                    write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
                 }
             } else {
                 const int slot = slot_of(blockIdx.x, c_first == static_cast<int>(blockIdx.x));
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
-                    reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D)[c4] = merged(r, c4);
-                }
-                if (threadIdx.x < kRows) {
-                    p.part_ml[slot * 16 + threadIdx.x] = make_float2(fin_m[threadIdx.x], fin_l[threadIdx.x]);
+                    float mm, ll;
+                    reinterpret_cast<float4*>(p.part_o + (static_cast<int64_t>(slot) * 16 + r) * D)[c4] = merged(r, c4, mm, ll);
+                    if (c4 == 0) p.part_ml[slot * 16 + r] = make_float2(mm, ll);
                 }
             }
             if (threadIdx.x == 0 && c_last == static_cast<int>(blockIdx.x)) p.pieces[pair] = make_int2(c_first, c_last - c_first + 1);
@@ -1084,6 +1085,7 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
     p.sq = a->sq;
     p.causal = a->causal != 0;
     p.page_blocks = a->cache.page_size / 16;
+    p.table_width = a->cache.table_width;
     p.scale_log2 = a->scale * kLog2e;
     for (int i = 0; i < 3; ++i) {
         p.qs[i] = a->q_strides[i];
