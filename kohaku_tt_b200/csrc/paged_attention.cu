@@ -61,18 +61,27 @@ struct PagedParams {
 
 constexpr int kMaxBatch = 512;    // lengths and their prefix sums live in shared memory
 
-// What a variant has: D, bits of the pages, NT column tiles of 8 query rows.
+// What a variant has: D, bits of the pages, NT column tiles of 8 query rows. Measured, us, 64 sequences, 16 heads over 2, D 128,
+// lengths U[n / 8, n], unless it says otherwise:
+//   4 bits, n 16,384, one column tile: two blocks at a time, 4 warps, 3 CTAs 53.2; one block at a time 55.7; 8 warps, 2 CTAs (128
+//   registers) 56.6; 4 warps, 4 CTAs 56.0. Loads alone 39.4, products alone as long as both: the stream is bound by the issue of
+//   some 390 instructions a block, half of them on the integer pipe. D 64, 32 heads over 8, n 512: 4 CTAs 10.0, 3 CTAs 15.3.
+//   Two column tiles, 16 x 4 tokens, n 8,192: 2 CTAs 28.7, 3 (spills) 58.
+//   bf16, n 4,096: 2 stages 34.3, 3 stages 34.7, 3 CTAs 34.8 (4.8 TB/s, 73 % of a copy's rate). D 64, 32 x 14 heads over 2, n 8,192: 4 CTAs of
+//   3 stages 20.9, 2 of 6 22.7, 3 of 4 25.9; 64 x 32 over 8, n 512: 11.2, 18.1, 16.6.
+//   What ending a pair costs, 4 bits, n 4,096 and 16,384, for 8, 12, 24, 40 blocks: 24.5, 24.2, 23.6, 24.4 and 54.8, 54.1, 53.3, 54.4; bf16,
+//   n 4,096, for 4, 8, 16, 24, 32: 34.9, 34.5, 34.1, 34.1, 34.4.
 template <int D, int kBits, int NT>
 struct Shape {
     static constexpr int W = 4;                                               // warps
     static constexpr int kThreads = 32 * W;
     static constexpr int kBlock = kBits == 4 ? 18 * D : 64 * D;               // bytes: 16 keys, then their values
     static constexpr int NB = kBits == 16 ? 1 : (D == 128 && NT == 1 ? 2 : 4);   // blocks of a stage
-    static constexpr int PB = kBits == 4 && NT == 1 ? 2 : 1;                 // blocks that the products are of at a time
+    static constexpr int PB = kBits == 4 && NT == 1 ? 2 : 1;                  // blocks that the products are of at a time
     static constexpr int kStage = NB * kBlock;
     static constexpr int NS = kBits == 4 ? 2 : NT == 1 ? (D == 64 ? 3 : 2) : (D == 64 ? 6 : 3);
     static constexpr int kRows = 8 * NT;
-    static constexpr int kPairCost = kBits == 4 ? 24 : (D == 64 ? 24 : 16);   // what ending a pair costs a CTA, in blocks
+    static constexpr int kPairCost = kBits == 4 ? 24 : 16;                    // what ending a pair costs a CTA, in blocks
     static constexpr int kCtas = D == 64 ? (NT == 1 ? 4 : kBits == 4 ? 3 : 2) : (kBits == 4 && NT == 1 ? 3 : 2);   // per SM
     static constexpr int kRing = W * NS * kStage;
     static constexpr int kStats = (2 * W + 2) * kRows * 4 + W * 4;
@@ -873,15 +882,21 @@ int paged_set_up(int dev) {
     return rc;
 }
 
-// CTAs per pair where each has a cluster of its own; 0 where the pairs are cut into equal shares.
+// CTAs per pair where each has a cluster of its own; 0 where the pairs are cut into equal shares. A cluster has no lengths to
+// scan and nothing to add up behind the stream, 1.5 to 3 us less; but a pair is as long as it is, and CTAs that clusters leave
+// out have no share. So a rank has 1,024 keys at most, and beyond 512 as many times fewer as clusters use fewer CTAs than there are
+// (less a fifth). Measured, us, clusters and shares, lengths U[n / 8, n], 16 heads over 2, bf16, D 64: 1 x 1,024 6.1 and 7.4, 1 x 4,096
+// 8.1 and 8.0, 4 x 4,096 8.5 and 9.2, 4 x 8,192 11.6 and 11.1, 32 x 2,048 9.2 and 11.7, 32 x 8,192 20.7 and 25.7, 64 x 4,096 (4 ranks) 19.6 and
+// 23.7; D 128: 1 x 8,192 11.8 and 9.9, 16 x 4,096 14.4 and 16.6, 64 x 2,048 21.5 and 22.6, 64 x 4,096 (2 ranks) 35.5 and 34.0; 4 bits, D 128: 1 x 1,024
+// 7.3 and 8.0, 16 x 2,048 10.7 and 12.2, 16 x 8,192 19.9 and 17.7, 64 x 1,024 14.2 and 15.2, 64 x 2,048 20.1 and 18.0.
 template <int D, int kBits, int NT>
 int paged_ranks(int64_t pairs, int cap, int ctas, int dev) {
     constexpr int kTile = 16 * Shape<D, kBits, NT>::W;
     for (int ranks = 8; ranks >= 1; ranks /= 2) {
-        if (ranks > 1 && (ranks / 2) * kTile >= cap) continue;   // half as many have a tile each
+        if (ranks > 1 && (ranks / 2) * kTile >= cap) continue;   // half as many have a block for every warp
         if (pairs * ranks > ctas || cluster_room<D, kBits, NT>(dev, ranks) < pairs) continue;
-        const int64_t used = pairs * ranks * (ranks == 1 ? 7 : 6), all = static_cast<int64_t>(ctas) * 6, most = 16ll * kTile * ranks;
-        return cap <= most && (ranks == 8 || 2 * cap <= most || cap * all <= most * used) ? ranks : 0;
+        const int64_t used = pairs * ranks, all = ctas, most = 1024ll * ranks;
+        return cap <= most && (2 * cap <= most || 4 * cap * all <= 5 * most * used) ? ranks : 0;
     }
     return 0;
 }
