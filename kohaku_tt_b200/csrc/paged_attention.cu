@@ -888,10 +888,13 @@ int paged_set_up(int dev) {
 // (less a fifth). Measured, us, clusters and shares, lengths U[n / 8, n], 16 heads over 2, bf16, D 64: 1 x 1,024 6.1 and 7.4, 1 x 4,096
 // 8.1 and 8.0, 4 x 4,096 8.5 and 9.2, 4 x 8,192 11.6 and 11.1, 32 x 2,048 9.2 and 11.7, 32 x 8,192 20.7 and 25.7, 64 x 4,096 (4 ranks) 19.6 and
 // 23.7; D 128: 1 x 8,192 11.8 and 9.9, 16 x 4,096 14.4 and 16.6, 64 x 2,048 21.5 and 22.6, 64 x 4,096 (2 ranks) 35.5 and 34.0; 4 bits, D 128: 1 x 1,024
-// 7.3 and 8.0, 16 x 2,048 10.7 and 12.2, 16 x 8,192 19.9 and 17.7, 64 x 1,024 14.2 and 15.2, 64 x 2,048 20.1 and 18.0.
+// 7.3 and 8.0, 16 x 2,048 10.7 and 12.2, 16 x 8,192 19.9 and 17.7, 64 x 1,024 14.2 and 15.2, 64 x 2,048 20.1 and 18.0. Pairs that outnumber the
+// CTAs follow one another, up to 2,048 keys each: 64 x 16 heads, D 64, bf16, 128, 1,024 and 2,048 keys 10.2 and 15.8, 29.0 and 32.8, 52.4 and
+// 57.7; 4 bits 10.3 and 15.9, 24.4 and 28.4, 40.3 and 41.2; 64 x 12, D 128, 4 bits, 2,048 49.1 and 47.9.
 template <int D, int kBits, int NT>
 int paged_ranks(int64_t pairs, int cap, int ctas, int dev) {
     constexpr int kTile = 16 * Shape<D, kBits, NT>::W;
+    if (pairs > ctas && cap <= 2048) return 1;
     for (int ranks = 8; ranks >= 1; ranks /= 2) {
         if (ranks > 1 && (ranks / 2) * kTile >= cap) continue;   // half as many have a block for every warp
         if (pairs * ranks > ctas || cluster_room<D, kBits, NT>(dev, ranks) < pairs) continue;
