@@ -307,6 +307,15 @@ def test_more_sequences_than_a_launch_takes(cuda, bits):
 
 
 @pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_more_pairs_than_ctas(cuda, bits, d):
+    """One after another, whole, where no sequence is long; equal shares where one may be."""
+    lengths = [(7 * i) % 50 for i in range(60)]
+    _check(cuda, bits, d, 16, 16, 16, 1, lengths)
+    _check(cuda, bits, d, 16, 16, 16, 1, lengths, wide=130)
+
+
+@pytest.mark.parametrize("bits", BITS)
 def test_one_long_sequence_among_short_ones(cuda, bits):
     _check(cuda, bits, 64, 4, 2, 16, 1, [3000, 1, 16, 40, 0, 500], seed=2)
 
