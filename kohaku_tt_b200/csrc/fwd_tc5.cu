@@ -842,15 +842,19 @@ EncodeFn encode_fn() {
 
 int* status_word(int** device_view) {
     // One pinned, device-mapped word per process: kernels record a wait that ran out
-    // there and the host reads it without a synchronisation.
+    // there and the host reads it without a synchronisation. A first call may come inside a stream
+    // capture, where this thread's own allocations are allowed only in the relaxed mode.
     static int* host = nullptr;
     static int* dev = nullptr;
     static std::once_flag once;
     std::call_once(once, [] {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        const bool relaxed = cudaThreadExchangeStreamCaptureMode(&mode) == cudaSuccess;
         if (cudaHostAlloc(reinterpret_cast<void**>(&host), sizeof(int), cudaHostAllocMapped) == cudaSuccess) {
             *host = 0;
             if (cudaHostGetDevicePointer(reinterpret_cast<void**>(&dev), host, 0) != cudaSuccess) dev = nullptr;
         }
+        if (relaxed) cudaThreadExchangeStreamCaptureMode(&mode);
     });
     if (device_view) *device_view = dev;
     return host;

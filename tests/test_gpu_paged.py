@@ -483,6 +483,41 @@ def test_two_streams_and_two_graphs_at_once(cuda, bits, n):
             assert torch.equal(e, w) and torch.equal(o, w)
 
 
+@pytest.mark.parametrize("bits", BITS)
+def test_first_call_of_a_kind_inside_a_capture(cuda, bits):
+    """What a kernel needs set up can be set up while a stream captures: a process of its own, whose first calls are
+    captured ones."""
+    import subprocess
+    import sys
+
+    code = f"""
+import torch, kohaku_tt_b200 as ktt
+dev = torch.device("cuda:0")
+kp, vp = ktt.paged_cache(8, 2, 16, 64, bits={bits}, device=dev)
+table = torch.arange(8, dtype=torch.int32, device=dev).view(2, 4)
+lens, after = torch.tensor([3, 40], dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+x = [torch.randn(2, h, n, 64, device=dev).bfloat16() for n in (1, 3, 50) for h in (2, 2, 8)]
+cos, sin = ktt.rotary_table(64, 64, device=dev)
+torch.cuda.synchronize()
+def run():
+    outs = []
+    for i in range(3):
+        q = ktt.paged_append(x[3 * i], x[3 * i + 1], kp, vp, table, lens, cos, sin, q=x[3 * i + 2], lengths_out=after)
+        outs += [q, ktt.sdpa_paged(q, kp, vp, table, after), *ktt.paged_read(kp, vp, table, after), *ktt.rotary(q, x[3 * i], cos, sin)]
+    return outs
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = run()
+graph.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+assert all(torch.equal(a, b) for a, b in zip(got, run()))
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stdout + done.stderr[-3000:]
+
+
 def test_compiled(cuda):
     kp, vp, table = _cache(16, 64, 2, 16, [20, 33], wide=4)
     kp, vp, table = kp.nan_to_num(0.0).to(cuda), vp.nan_to_num(0.0).to(cuda), table.clamp(min=0).to(cuda)
