@@ -184,14 +184,18 @@ def _(q, k, cos, sin, positions, interleaved, inverse):
 def _setup(ctx, inputs, output):
     _, k, cos, sin, positions, interleaved, inverse = inputs
     ctx.save_for_backward(cos, sin, positions)
-    ctx.how = (interleaved, inverse, k is None)
+    ctx.how = (interleaved, inverse, [x.shape for x in output])
 
 
 def _op_backward(ctx, grads):
     cos, sin, positions = ctx.saved_tensors
-    interleaved, inverse, alone = ctx.how
-    got = torch.ops.ktt_b200._rotary(grads[0], None if alone else grads[1], cos, sin, positions, interleaved, not inverse)
-    return got[0], None if alone else got[1], None, None, None, None, None
+    interleaved, inverse, shapes = ctx.how
+    some = next((g for g in grads if g is not None), None)
+    if some is None:
+        return (None,) * 7
+    grads = [some.new_zeros(shape) if g is None else g for g, shape in zip(grads, shapes)]
+    got = torch.ops.ktt_b200._rotary(grads[0], grads[1] if len(grads) > 1 else None, cos, sin, positions, interleaved, not inverse)
+    return got[0], got[1] if len(got) > 1 else None, None, None, None, None, None
 
 
 _rotary_op.register_autograd(_op_backward, setup_context=_setup)

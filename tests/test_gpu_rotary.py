@@ -199,6 +199,19 @@ def test_compiled(cuda):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     (g,) = torch.autograd.grad(got[0], leaf, q)
     assert torch.equal(g, ktt.rotary(q, None, cos, -sin, interleaved=True)[0])
+    for use in (lambda a, b: ktt.rotary(a, b, cos, sin)[1], lambda a, b: ktt.rotary(b, a, cos, sin)[0]):   # one output alone
+        kl = k.clone().requires_grad_()
+        (g,) = torch.autograd.grad(torch.compile(use, fullgraph=True)(q, kl), kl, k)
+        assert torch.equal(g, ktt.rotary(k, None, cos, -sin)[0])
+
+
+def test_the_operator_s_gradient_where_one_output_is_used(cuda):
+    cos, sin = ktt.rotary_table(16, 64, device=cuda)
+    q, k = _x(2, 4, 16, 64).to(cuda).requires_grad_(), _x(2, 2, 16, 64, seed=1).to(cuda).requires_grad_()
+    want = ktt.rotary(k.detach(), None, cos, -sin)[0]
+    out = torch.ops.ktt_b200._rotary(q, k, cos, sin, None, False, False)
+    gq, gk = torch.autograd.grad(out[1], (q, k), k.detach(), allow_unused=True)
+    assert torch.equal(gk, want) and (gq is None or not gq.any())
 
 
 def test_refusals(cuda):
