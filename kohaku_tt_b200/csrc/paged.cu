@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
         if constexpr (kBits == 16) {
             if (there) x[i].store(reinterpret_cast<__nv_bfloat16*>(to + at * (what == 2 ? p.c.vs[2] : p.c.ks[2])) + col);
         } else {
-            if (there) to += (at >> 4) * (9 * D);
+            if (there) to += static_cast<int64_t>(at >> 4) * (9 * D);
             put_four_bits<D>(x[i], to, what == 2, at & 15, chunk, there);
         }
     }
@@ -241,8 +241,8 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
         kp[i] = vp[i] = nullptr;
         token[i] = at & 15;
         if (page >= 0 && page < p.c.pages) {
-            kp[i] = p.c.k + page * p.c.ks[0] + head * p.c.ks[1] + (kBits == 16 ? at * p.c.ks[2] : (at >> 4) * (9 * D));
-            vp[i] = p.c.v + page * p.c.vs[0] + head * p.c.vs[1] + (kBits == 16 ? at * p.c.vs[2] : (at >> 4) * (9 * D));
+            kp[i] = p.c.k + page * p.c.ks[0] + head * p.c.ks[1] + (kBits == 16 ? at * p.c.ks[2] : static_cast<int64_t>(at >> 4) * (9 * D));
+            vp[i] = p.c.v + page * p.c.vs[0] + head * p.c.vs[1] + (kBits == 16 ? at * p.c.vs[2] : static_cast<int64_t>(at >> 4) * (9 * D));
         }
     }
     Eight<__nv_bfloat16> k[kReadRows], v[kReadRows];

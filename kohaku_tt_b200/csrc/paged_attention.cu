@@ -244,8 +244,8 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 const int entry = block / p.page_blocks, row = (block - entry * p.page_blocks) * (kBits == 16 ? 16 : 1);
                 const int64_t page = p.c.table[c.b * p.c.table_stride + entry];
                 if (page >= 0 && page < p.c.pages) {
-                    k_at = p.c.k + page * p.c.ks[0] + hk * p.c.ks[1] + row * (kBits == 16 ? p.c.ks[2] : 9 * D);
-                    v_at = p.c.v + page * p.c.vs[0] + hk * p.c.vs[1] + row * (kBits == 16 ? p.c.vs[2] : 9 * D);
+                    k_at = p.c.k + page * p.c.ks[0] + hk * p.c.ks[1] + row * (kBits == 16 ? p.c.ks[2] : static_cast<int64_t>(9 * D));
+                    v_at = p.c.v + page * p.c.vs[0] + hk * p.c.vs[1] + row * (kBits == 16 ? p.c.vs[2] : static_cast<int64_t>(9 * D));
                 }
             }
             at = 0;
@@ -936,20 +936,20 @@ int64_t rows_per_head(const ktt_b200_paged_sdpa_args* a) { return static_cast<in
 Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     Plan s = {};
     const int64_t rows = rows_per_head(a), hk = a->cache.kv_heads;
-    s.few = a->sq <= kFewTokens;
+    s.nt = rows <= 8 ? 1 : 2;
+    s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
+    // Units of all pairs of a launch have to fit 30 bits.
+    int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 16 + 32) * hk * s.row_tiles);
+    s.few = a->sq <= kFewTokens && most > 0;
     if (s.few) {
-        s.nt = rows <= 8 ? 1 : 2;
-        s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
-        // Units of all pairs have to fit 30 bits.
-        int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 16 + 32) * hk * s.row_tiles);
-        most = most < 1 ? 1 : (most > kMaxBatch ? kMaxBatch : most);
+        if (most > kMaxBatch) most = kMaxBatch;
         s.slice = static_cast<int>(a->batch < most ? a->batch : most);
         s.bytes = parts_of(s.slice * hk * s.row_tiles, a->d, sms * 4).total;
         return s;
     }
     // Dense rows of some sequences at a time: 1 GB, or one sequence.
     const int64_t one = 4ll * c.cap * hk * a->d;
-    const int64_t most = (1ll << 30) / one;
+    most = (1ll << 30) / one;
     s.slice = static_cast<int>(most < 1 ? 1 : (most < a->batch ? most : a->batch));
     if (s.slice > kMaxBatch) s.slice = kMaxBatch;
     s.bytes = s.slice * one + (64 + 2 * kMaxBatch + 1) * 4;   // and what is behind the rows (run_many)
@@ -994,7 +994,6 @@ const char* sdpa_refusal(const ktt_b200_paged_sdpa_args* a, Pages& c) {
         if (a->q_strides[i] % 2 || a->out_strides[i] % 4) return "q strides must be even and out strides multiples of 4";
     }
     if ((reinterpret_cast<uintptr_t>(a->q) & 3) || (reinterpret_cast<uintptr_t>(a->out) & 7)) return "q must be 4-byte and out 8-byte aligned";
-    if ((static_cast<int64_t>(c.cap) / 16 + 32) * a->cache.kv_heads * 8 > (1ll << 30)) return "too many keys and heads";
     return nullptr;
 }
 

@@ -273,7 +273,8 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
                max_k=None):
     """Attention of q [B, H, Sq, D] over the first lengths[b] keys of each sequence's pages; Sq may be one
     token, a few, or a chunk of a prompt. Packed: q [T, H, D] with cu_seq_q (B + 1 offsets, a list, or int32 on
-    the device, then best with max_q, the longest sequence); rows that no sequence covers are left undefined.
+    the device, then best with max_q, no less than the longest sequence); rows that no sequence covers are left
+    undefined.
 
     Pages as in paged_append, bf16 or 4 bits, D 64 or 128, H a multiple of Hk. lengths (int32 [B] on the
     device) count the keys with those of the call's own tokens, which are appended first. Under is_causal the
