@@ -357,7 +357,9 @@ extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream
     if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || (a->heads && a->rows && (!a->q || !a->q_out)) || (a->rows && (!a->k || !a->v))) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: null pointer");
     }
-    if (a->lengths_out && a->lengths_out == a->cache.lengths) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: lengths_out must not be the lengths themselves");
+    if (a->lengths_out && a->lengths_out < a->cache.lengths + a->batch && a->cache.lengths < a->lengths_out + a->batch) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: lengths_out must not overlap the lengths");
+    }
     p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, 0};
     p.batch = a->batch;
     p.rows = a->rows;

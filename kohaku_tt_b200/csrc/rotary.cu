@@ -165,7 +165,8 @@ int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
         cfg.numAttrs = 1;
         return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "rotary launch");
     };
-    // Four heads to a thread once that fills the GPU.
+    // Four heads to a thread once that fills the GPU: a row's position and table entries are read once for all of them.
+    // 4 x 4,096 tokens, 32 heads over 8, D 128, bf16, forward and gradient, us for 1 and 4 heads: 671 and 400.
     if (p.tokens * chunks * (p.heads[0] + p.heads[1]) >= kManyThreads) {
         if (fast) return go(rotary_kernel<T, true, 4>, 4);
         return go(rotary_kernel<T, false, 4>, 4);
@@ -217,7 +218,8 @@ extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, 
     for (int i = 0; i < pairs; ++i) {
         if (!std::isfinite(frequencies[i])) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: frequencies must be finite");
         const long double turns = frequencies[i] * 0.159154943091895335768883763372514362L;   // f / 2 pi
-        p.turns[i] = static_cast<uint64_t>((turns - std::floor(turns)) * 0x1p64L);
+        const long double part = turns - std::floor(turns);
+        p.turns[i] = part < 1 ? static_cast<uint64_t>(part * 0x1p64L) : 0;   // (1: a frequency just below 0)
     }
     p.vec = ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15) == 0;
     rotary_table_kernel<<<static_cast<unsigned>((positions + kTableRows - 1) / kTableRows), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);

@@ -336,6 +336,36 @@ def _cut(cuda, bits, max_k):
 
 
 @pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("d,hk", [(128, 8), (64, 16)])
+def test_chunks_over_more_room_than_one_launch_takes(cuda, bits, packed, d, hk):
+    """Room for 65,536 keys: the dense rows of 4 sequences are 1 GB, so 6 are two launches of 4 and 2."""
+    counts = [60, 49, 0, 130, 7, 64] if packed else 60
+    _check(cuda, bits, d, hk, hk, 64, counts, [100, 49, 3, 257, 0, 64], packed=packed, wide=1024, dense_four_bits=bits == 4)
+
+
+@pytest.mark.parametrize("bits", BITS)
+def test_pages_past_32_bits_of_a_pool(cuda, bits):
+    """The same cache at the front of a small pool and at the end of one of over 4 GB."""
+    d, h, hk, page, b = 128, 16, 8, 16, 2
+    many = 140_000 if bits == 16 else 480_000
+    small, large = (ktt.paged_cache(n, hk, page, d, bits=bits, device=cuda) for n in (8, many))
+    assert large[0].numel() * large[0].element_size() > 2 ** 32
+    table = torch.arange(8, dtype=torch.int32, device=cuda).view(b, 4)
+    lens = torch.tensor([0, 3], dtype=torch.int32, device=cuda)
+    outs = []
+    for (kp, vp), t in ((small, table), (large, table + (many - 8))):
+        state, out = lens, []
+        for n in (50, 3, 1):
+            after = torch.empty_like(state)
+            ktt.paged_append(_x(b, hk, n, d, seed=n).to(cuda), _x(b, hk, n, d, seed=n + 1).to(cuda), kp, vp, t, state, lengths_out=after)
+            out.append(ktt.sdpa_paged(_x(b, h, n, d, seed=n + 2).to(cuda), kp, vp, t, after))
+            state = after
+        outs.append(out + list(ktt.paged_read(kp, vp, t, state)))
+    assert all(torch.equal(x, y) for x, y in zip(*outs)) and bool(outs[0][0].any())
+
+
+@pytest.mark.parametrize("bits", BITS)
 @pytest.mark.parametrize("n", [1, 4, 140])
 def test_keys_without_a_page_are_zeros(cuda, bits, n):
     d, h, hk, page = 64, 4, 2, 16

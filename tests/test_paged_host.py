@@ -74,7 +74,7 @@ def test_append_refusals(built_lib):
         return a
 
     for kw in (dict(batch=0), dict(rows=-1), dict(k=None), dict(heads=2), dict(cos=4096), dict(cos=4096, sin=4096, pairs=65, table_rows=4),
-               dict(cos=4096, sin=4096, pairs=4, table_rows=0), dict(lengths_out=4096)):
+               dict(cos=4096, sin=4096, pairs=4, table_rows=0), dict(lengths_out=4096), dict(batch=4, lengths_out=4096 + 12), dict(batch=4, lengths_out=4096 - 12)):
         assert built_lib.ktt_b200_paged_append(ctypes.byref(args(**kw)), None) == _lib.ERR_BAD_ARGUMENT, kw
     assert built_lib.ktt_b200_paged_append(ctypes.byref(args(rows=0)), None) == 0      # nothing to do
     assert built_lib.ktt_b200_paged_append(None, None) == _lib.ERR_BAD_ARGUMENT
@@ -92,6 +92,26 @@ def test_attention_refusals(built_lib):
                    (dict(batch=0), _lib.ERR_BAD_ARGUMENT), (dict(q=None), _lib.ERR_BAD_ARGUMENT), (dict(sq=-1), _lib.ERR_BAD_ARGUMENT)):
         assert built_lib.ktt_b200_paged_sdpa(ctypes.byref(args(**kw)), None) == rc, kw
     assert built_lib.ktt_b200_paged_sdpa(ctypes.byref(args(sq=0)), None) == 0
+
+
+def test_a_diagonal_at_the_key_lengths_end_is_the_forward_s_alone(built_lib):
+    """causal 3 needs key lengths; packed calls with key lengths take it or none; the backward takes neither."""
+    def args(**kw):
+        a = _lib.AttnArgs()
+        a.batch, a.heads, a.kv_heads, a.sq, a.sk, a.d, a.dv, a.scale = 1, 1, 1, 8, 8, 64, 64, 0.1
+        a.q = a.k = a.v = a.out = a.key_lengths = 4096
+        for name, x in kw.items():
+            setattr(a, name, x)
+        return ctypes.byref(a)
+
+    packed = dict(cu_seqlens_q=4096, cu_seqlens_k=4096, total_q=8, total_k=8)
+    assert built_lib.ktt_b200_sdpa_supported(args(causal=3)) and built_lib.ktt_b200_sdpa_supported(args(causal=3, **packed))
+    for kw in (dict(causal=3, key_lengths=None), dict(causal=2, **packed), dict(causal=4), dict(causal=-1)):
+        assert not built_lib.ktt_b200_sdpa_supported(args(**kw)), kw
+        assert built_lib.ktt_b200_sdpa_forward(args(**kw), None) == _lib.ERR_UNSUPPORTED, kw
+    for kw in (dict(causal=3), dict(causal=3, **packed), dict(causal=0, **packed)):
+        assert not built_lib.ktt_b200_sdpa_backward_supported(args(**kw)), kw
+        assert built_lib.ktt_b200_sdpa_backward(args(**kw), None) == _lib.ERR_UNSUPPORTED, kw
 
 
 def test_rotary_refusals(built_lib):
