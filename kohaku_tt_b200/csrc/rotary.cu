@@ -12,10 +12,16 @@ namespace {
 // per position, f / 2 pi, is a whole number of 2^-64 turns, and its multiples modulo 2^64 lose nothing, whole turns fall off
 // by themselves, and the quarter turn nearest to what is left stands in two bits. The rest, at most an eighth of a turn, is
 // read from the bits as a mantissa of 23 and a remainder of 23 more; sine and cosine of it are their Taylor sums to the 9th and
-// 10th power (the next terms are 2^-29 and 2^-33 of the value). Bound: the writing of the tables, in 16-byte pieces; in 64-bit
-// floating point, whose conversions run at an eighth of this rate, 131,072 x 64 took 24.6 us; now 22.6, of which a fill of
-// the same 67 MB takes 12.4, the rest being some 60 instructions a pair.
+// 10th power (the next terms are 2^-29 and 2^-33 of the value).
+// That is some 80 instructions a pair, so a block takes it for the first of every kSteps of its positions and for the first
+// kSteps alone, each as an fp32 value and what it leaves, and the others by
+//     cos(a + b) = cos a cos b - sin a sin b,   sin(a + b) = sin a cos b + cos a sin b
+// with the leavings' products: 12 operations, two roundings that count (the larger product's sum and the result's), where each
+// position by itself took 60 and had three. Bound: the writing of the tables, in 16-byte pieces.
 constexpr int kMaxPairs = 256;
+// Pairs in all from which a block has 256 positions, not 64. us for 64 and 256: 4,096 x 64 3.3 and 5.5, 16,384 x 64 4.3 and 5.5,
+// 32,768 x 64 6.5 and 5.7, 131,072 x 64 17.2 and 14.0 (two fills of the same 67 MB 11.1; every position by itself 20.2).
+constexpr int64_t kLargeTable = 3 << 19;
 struct TableParams {
     float* cos;
     float* sin;
@@ -26,10 +32,23 @@ struct TableParams {
     uint64_t turns[kMaxPairs];   // f_i / 2 pi in 2^-64 turns
 };
 
-constexpr int kTableRows = 64;   // positions of a block (16 to 128: 24.9, 22.7, 22.6, 22.6 us for 131,072 x 64)
+constexpr int kTablePairs = 64;   // of a block
+
+// An fp32 value and what it leaves of a number.
+struct Two {
+    float hi, lo;
+};
+__device__ __forceinline__ Two two_of(float hi, float lo) {
+    const float s = hi + lo;
+    return {s, lo - (s - hi)};
+}
+__device__ __forceinline__ Two times(const Two& x, float y) {
+    const float h = x.hi * y;
+    return {h, fmaf(x.hi, y, -h) + x.lo * y};
+}
 
 // Cosine and sine of an angle of `turn` 2^-64 turns.
-__device__ __forceinline__ void cos_sin(uint64_t turn, float& c, float& s) {
+__device__ __forceinline__ void cos_sin(uint64_t turn, Two& c, Two& s) {
     const uint64_t z = turn + (1ull << 61);
     const uint32_t quarter = static_cast<uint32_t>(z >> 62);
     // The rest and 2^61, as 62 bits: the upper 23 and the next 23 as fractions.
@@ -39,47 +58,98 @@ __device__ __forceinline__ void cos_sin(uint64_t turn, float& c, float& s) {
     constexpr float kQuarter = 1.57079632679489662f, kQuarterRest = -4.37113882867379e-8f;
     const float x = hi * kQuarter;
     const float rest = fmaf(lo, kQuarter * 0x1p-23f, fmaf(hi, kQuarterRest, fmaf(hi, kQuarter, -x)));
-    const float q = x * x;
-    const float sx = fmaf(x * q, fmaf(q, fmaf(q, fmaf(q, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6), x);
-    const float cx = fmaf(q, fmaf(q, fmaf(q, fmaf(q, fmaf(q, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24), -0.5f), 1.f);
-    const float sr = fmaf(rest, cx, sx), cr = fmaf(-rest, sx, cx);
-    const float a = quarter & 1 ? sr : cr, b = quarter & 1 ? cr : sr;
-    c = quarter == 1 || quarter == 2 ? -a : a;
-    s = quarter & 2 ? -b : b;
+    const float q = x * x, more = fmaf(x, x, -q);   // (x^2 and its rounding)
+    const float st = x * q * fmaf(q, fmaf(q, fmaf(q, 1.f / 362880, -1.f / 5040), 1.f / 120), -1.f / 6);
+    const float ct = q * q * fmaf(q, fmaf(q, fmaf(q, -1.f / 3628800, 1.f / 40320), -1.f / 720), 1.f / 24);
+    const float half = fmaf(q, -0.5f, 1.f), left = (1.f - half) - 0.5f * q;
+    const Two sr = two_of(x, fmaf(rest, half, st)), cr = two_of(half, left + fmaf(more, -0.5f, fmaf(-rest, x, ct)));
+    c = quarter & 1 ? sr : cr;
+    s = quarter & 1 ? cr : sr;
+    if (quarter == 1 || quarter == 2) c = {-c.hi, -c.lo};
+    if (quarter & 2) s = {-s.hi, -s.lo};
 }
 
+// The angles of a block, by pair: those of positions first + kSteps u, times the scale, then those of 0, 1, .. kSteps - 1.
+template <int kSteps>
+struct TableShared {
+    alignas(16) float ch[2 * kSteps][kTablePairs], cl[2 * kSteps][kTablePairs], sh[2 * kSteps][kTablePairs], sl[2 * kSteps][kTablePairs];
+};
+
+template <int kVec>
+__device__ __forceinline__ void table_load(float (&to)[kVec], const float* from) {
+    if constexpr (kVec == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from);
+        to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
+    } else if constexpr (kVec == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(from);
+        to[0] = x.x; to[1] = x.y;
+    } else {
+        to[0] = *from;
+    }
+}
+template <int kVec>
+__device__ __forceinline__ void table_store(float* to, const float (&x)[kVec]) {
+    if constexpr (kVec == 4) *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+    else if constexpr (kVec == 2) *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+    else *to = x[0];
+}
+
+// A block has kSteps * kSteps positions of up to 64 pairs; a thread kVec pairs of every position first + kSteps u + w of some
+// of its (u, w).
+template <int kSteps, int kVec>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ TableParams p) {
-    __shared__ uint64_t turns[kMaxPairs];   // (a warp's threads want different ones: no matter for constant memory)
-    for (int i = threadIdx.x; i < p.pairs; i += 256) turns[i] = p.turns[i];
+    __shared__ TableShared<kSteps> sm;
+    __shared__ uint64_t turns[kTablePairs];   // (a warp's threads want different ones: no matter for constant memory)
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * (kSteps * kSteps);
+    const int rows = static_cast<int>(p.positions - first < kSteps * kSteps ? p.positions - first : kSteps * kSteps);
+    const int pair0 = blockIdx.y * kTablePairs, pairs = min(p.pairs - pair0, kTablePairs);
+    if (threadIdx.x < pairs) turns[threadIdx.x] = p.turns[pair0 + threadIdx.x];
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kTableRows;
-    const int rows = static_cast<int>(p.positions - first < kTableRows ? p.positions - first : kTableRows), n = rows * p.pairs;
-    float* cos = p.cos + first * p.pairs;
-    float* sin = p.sin + first * p.pairs;
-    for (int at = threadIdx.x * 4; at < n; at += 1024) {
-        int row = at / p.pairs, i = at - row * p.pairs;
-        float c[4], s[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            cos_sin(static_cast<uint64_t>(first + row) * turns[i], c[e], s[e]);
-            c[e] *= p.scale;
-            s[e] *= p.scale;
-            if (++i == p.pairs) {
-                i = 0;
-                ++row;
-            }
+    for (int at = threadIdx.x; at < 2 * kSteps * kTablePairs; at += 256) {
+        const int row = at / kTablePairs, i = at % kTablePairs;
+        if (i >= pairs) continue;
+        const uint64_t pos = row < kSteps ? first + row * kSteps : row - kSteps;
+        Two c, s;
+        cos_sin(pos * turns[i], c, s);
+        if (row < kSteps) {
+            c = times(c, p.scale);
+            s = times(s, p.scale);
         }
-        if (p.vec && at + 4 <= n) {
-            *reinterpret_cast<float4*>(cos + at) = make_float4(c[0], c[1], c[2], c[3]);
-            *reinterpret_cast<float4*>(sin + at) = make_float4(s[0], s[1], s[2], s[3]);
-        } else {
+        sm.ch[row][i] = c.hi;
+        sm.cl[row][i] = c.lo;
+        sm.sh[row][i] = s.hi;
+        sm.sl[row][i] = s.lo;
+    }
+    __syncthreads();
+    const int chunks = pairs / kVec;   // (kVec divides the pairs)
+    // Threads that share a u take every `parts`-th w.
+    const int parts = min(max(256 / (kSteps * chunks), 1), kSteps);
+    for (int at = threadIdx.x; at < kSteps * parts * chunks; at += 256) {
+        const int group = at / chunks, i = (at - group * chunks) * kVec, u = group / parts;
+        float ch[kVec], cl[kVec], sh[kVec], sl[kVec];
+        table_load(ch, &sm.ch[u][i]);
+        table_load(cl, &sm.cl[u][i]);
+        table_load(sh, &sm.sh[u][i]);
+        table_load(sl, &sm.sl[u][i]);
+#pragma unroll 2
+        for (int w = group - u * parts; w < kSteps; w += parts) {
+            const int row = u * kSteps + w;
+            if (row >= rows) break;
+            float dh[kVec], dl[kVec], th[kVec], tl[kVec], c[kVec], s[kVec];
+            table_load(dh, &sm.ch[kSteps + w][i]);
+            table_load(dl, &sm.cl[kSteps + w][i]);
+            table_load(th, &sm.sh[kSteps + w][i]);
+            table_load(tl, &sm.sl[kSteps + w][i]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (at + e < n) {
-                    cos[at + e] = c[e];
-                    sin[at + e] = s[e];
-                }
+            for (int e = 0; e < kVec; ++e) {
+                const float cr = fmaf(ch[e], dl[e], fmaf(cl[e], dh[e], fmaf(-sh[e], tl[e], -sl[e] * th[e])));
+                const float sr = fmaf(sh[e], dl[e], fmaf(sl[e], dh[e], fmaf(ch[e], tl[e], cl[e] * th[e])));
+                c[e] = fmaf(ch[e], dh[e], fmaf(-sh[e], th[e], cr));
+                s[e] = fmaf(sh[e], dh[e], fmaf(ch[e], th[e], sr));
             }
+            const int64_t to = (first + row) * p.pairs + pair0 + i;
+            table_store(p.cos + to, c);
+            table_store(p.sin + to, s);
         }
     }
 }
@@ -222,7 +292,13 @@ extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, 
         p.turns[i] = part < 1 ? static_cast<uint64_t>(part * 0x1p64L) : 0;   // (1: a frequency just below 0)
     }
     p.vec = ((reinterpret_cast<uintptr_t>(cos) | reinterpret_cast<uintptr_t>(sin)) & 15) == 0;
-    rotary_table_kernel<<<static_cast<unsigned>((positions + kTableRows - 1) / kTableRows), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    auto go = [&](auto kernel, int rows) {
+        const dim3 grid(static_cast<unsigned>((positions + rows - 1) / rows), static_cast<unsigned>((pairs + kTablePairs - 1) / kTablePairs));
+        kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
+    };
+    const int vec = !p.vec ? 1 : pairs % 4 == 0 ? 4 : pairs % 2 == 0 ? 2 : 1;
+    if (positions * pairs >= kLargeTable) go(vec == 4 ? rotary_table_kernel<16, 4> : vec == 2 ? rotary_table_kernel<16, 2> : rotary_table_kernel<16, 1>, 256);
+    else go(vec == 4 ? rotary_table_kernel<8, 4> : vec == 2 ? rotary_table_kernel<8, 2> : rotary_table_kernel<8, 1>, 64);
     return check_cuda(cudaGetLastError(), "rotary_table launch");
 }
 

@@ -34,7 +34,7 @@ def test_tables(cuda, positions, dim, base, how):
     cos, sin = ktt.rotary_table(positions, dim, base=base, device=cuda, **how)
     assert cos.shape == sin.shape == (positions, dim // 2) and cos.dtype == torch.float32
     want_c, want_s = po.table(positions, *rotary_frequencies(dim, base, **how))
-    # sincospif (2 ulp) of an angle split in two: 3 ulp of values up to the scale, which is at most 2.
+    # Sines and cosines of two parts of an angle, multiplied and added: 3 ulp of values up to the scale, which is at most 2.
     for got, want in ((cos, want_c), (sin, want_s)):
         assert (got.double().cpu() - want).abs().max() <= 3 * 2.0 ** -23 * max(1.0, want.abs().max().item())
 
