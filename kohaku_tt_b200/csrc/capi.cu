@@ -309,9 +309,9 @@ extern "C" int ktt_b200_sdpa_backward_supported(const ktt_b200_attn_args* a) {
 
 static bool row_per_query(const AttnParams& p) { return p.mask_dtype != KTT_B200_MASK_NONE && p.ms[2] != 0 && p.sq > 1; }
 
-extern "C" int ktt_b200_sdpa_forward(const ktt_b200_attn_args* a, void* stream) { return forward_in_order(a, nullptr, static_cast<cudaStream_t>(stream)); }
+extern "C" int ktt_b200_sdpa_forward(const ktt_b200_attn_args* a, void* stream) { return forward_in_parts(a, {}, static_cast<cudaStream_t>(stream)); }
 
-int ktt::forward_in_order(const ktt_b200_attn_args* a, const int32_t* order, cudaStream_t stream) {
+int ktt::forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cudaStream_t stream) {
     if (const char* why = forward_refusal(a)) {
         note_call(4);
         return fail(KTT_B200_ERR_UNSUPPORTED, "sdpa_forward: %s", why);
@@ -321,7 +321,11 @@ int ktt::forward_in_order(const ktt_b200_attn_args* a, const int32_t* order, cud
     }
     AttnParams p;
     to_params(a, p);
-    p.order = order;
+    p.order = x.order;
+    p.parts = x.parts;
+    p.most_parts = x.most_parts;
+    p.part_o = x.part_o;
+    p.part_lse = x.part_lse;
     cudaStream_t st = stream;
     const char* why = nullptr;
     const bool tc5 = forward_tc5_takes(p, &why);

@@ -33,9 +33,15 @@ struct AttnParams {
     const int32_t* key_lengths;
     const int32_t* cu_q;
     const int32_t* cu_k;
-    // Forward, head dim 128, optional (with a work counter): batch entries by falling length, the order in which their tiles
-    // are drawn.
+    // Forward (fwd_tc5.cu, with a work counter; null without). order: batch entries by falling length, the order in which their
+    // tiles are drawn. parts, on the device: (n, span): tiles are cut along the keys into up to n <= most_parts parts of `span` keys
+    // (whole blocks); a part of a sequence of more than one leaves its normalised rows in part_o [parts][rows][heads][d] and
+    // their base-2 lse in part_lse [parts][rows][heads], rows = total_q or batch * sq, for the caller to merge.
     const int32_t* order;
+    const int32_t* parts;
+    int most_parts;
+    float* part_o;
+    float* part_lse;
     // backward
     const __nv_bfloat16* dout;
     __nv_bfloat16* dq;
@@ -224,8 +230,15 @@ int ensure_smem(K kernel, int bytes, const char* what) {
     return check_cuda(raise_smem_limit(kernel, bytes), what);
 }
 
-// ktt_b200_sdpa_forward, with an order of the batch entries (AttnParams.order, or null).
-int forward_in_order(const ktt_b200_attn_args* a, const int32_t* order, cudaStream_t stream);
+// ktt_b200_sdpa_forward, with AttnParams' order and parts.
+struct ForwardParts {
+    const int32_t* order;
+    const int32_t* parts;
+    int most_parts;
+    float* part_o;
+    float* part_lse;
+};
+int forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cudaStream_t stream);
 // Launchers (one per kernel family).
 int launch_forward_mma(const AttnParams& p, cudaStream_t stream);
 int launch_backward_mma(const AttnParams& p, cudaStream_t stream);

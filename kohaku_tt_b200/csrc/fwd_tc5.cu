@@ -114,6 +114,7 @@ struct Tc5Params {
     int* done_counter;  // with it: producers that have drawn their last; the last one puts both back to zero
     int grouped;        // item order (decode_work): 1 with a counter
     Divisor by_heads, by_batch, by_kv_heads, by_group, by_per_pair;   // group: query heads per K/V head; per_pair: q_tiles * group
+    Divisor by_part;    // kSplit: work, the items of one part
 };
 
 // Profiling zones (the counterpart of the reference's FLASH_PROFILE device zones,
@@ -135,6 +136,7 @@ struct Work {
     int b, h, q0, nblocks;
     SeqInfo si;
     bool valid;  // false: the tile lies past the end of its sequence
+    int part;    // kSplit: which part of its keys; -1: all of them
 };
 
 // Two orders of the items. Fixed deal (no counter): consecutive items are the heads of one
@@ -145,12 +147,17 @@ struct Work {
 // of (batch, head) pairs, which stay in L2, instead of one tile of every pair in the launch
 // (measured on the packed 65,536-token batch, 537 MB of K / V: 4.85 GB of DRAM reads per
 // launch for 1.07 GB of operands with the first order). The counter keeps the load even.
-__device__ __forceinline__ Work decode_work(const Tc5Params& tp, int w) {
+template <bool kSplit>
+__device__ __forceinline__ Work decode_work(const Tc5Params& tp, int w, int span) {
     const AttnParams& p = tp.a;
     Work k;
-    int qb;
-    if (tp.grouped) {
+    int qb, part = 0;
+    if (kSplit || tp.grouped) {
         const int group = static_cast<int>(tp.by_group.d);
+        if (kSplit) {   // a part of all tiles before the next one
+            part = div_by(w, tp.by_part);
+            w -= part * static_cast<int>(tp.by_part.d);
+        }
         const int pair = div_by(w, tp.by_per_pair), r = w - pair * static_cast<int>(tp.by_per_pair.d);
         const int tile = div_by(r, tp.by_group);
         k.b = div_by(pair, tp.by_kv_heads);
@@ -166,6 +173,14 @@ __device__ __forceinline__ Work decode_work(const Tc5Params& tp, int w) {
     k.si = seq_info(p, k.b);
     k.q0 = qb * kBM;
     k.valid = k.q0 < k.si.lq;
+    if (kSplit) {
+        const int start = part * span;
+        k.valid = k.valid && start < k.si.klen;
+        k.part = k.si.klen > span ? part : -1;
+        k.si.k_off += start;
+        k.si.klen = min(k.si.klen - start, span);
+        k.si.shift -= start;
+    }
     int kend = k.si.klen;
     if (p.causal) kend = min(kend, min(k.q0 + kBM, k.si.lq) - 1 + k.si.shift + 1);
     k.nblocks = (k.valid && kend > 0) ? (kend + kBN - 1) / kBN : 0;
@@ -180,7 +195,7 @@ __device__ __forceinline__ int work_of(int round, int cta, int ctas) {
 
 // ---- the kernel ------------------------------------------------------------------------
 
-template <int D, bool kTrace, bool kMask>
+template <int D, bool kTrace, bool kMask, bool kSplit = false>
 __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const Tc5Params tp) {
@@ -261,6 +276,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
     // items with at least one key block, `blk` the key blocks of all items so far. Ring
     // stages, S buffers and barrier parities are functions of those.
     int blocks_done = 0;
+    const int span = kSplit ? p.parts[1] : 0, work = kSplit ? tp.work * p.parts[0] : tp.work;
 
     // The n-th item of this CTA: -1 = no more, -2 = nothing at this position. Without a
     // counter every role computes the same snake order by itself. With one, the producer
@@ -269,9 +285,9 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
     // two-slot queue in shared memory.
     const bool dynamic = tp.work_counter != nullptr;
     auto static_item = [&](int n) -> int {
-        if (static_cast<int64_t>(n) * gridDim.x >= tp.work) return -1;
+        if (static_cast<int64_t>(n) * gridDim.x >= work) return -1;
         const int w = work_of(n, blockIdx.x, gridDim.x);
-        return w < tp.work ? w : -2;
+        return w < work ? w : -2;
     };
     auto draw_item = [&](int n, bool& ok) -> int {   // producer warp, converged
         if (!dynamic) return static_item(n);
@@ -287,11 +303,11 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             w = 0;
             if (lane == 0) w = atomicAdd(tp.work_counter, 1);
             w = __shfl_sync(0xffffffffu, w, 0);
-            if (w >= tp.work) {
+            if (w >= work) {
                 w = -1;
                 break;
             }
-            if (decode_work(tp, w).valid) break;
+            if (decode_work<kSplit>(tp, w, span).valid) break;
         }
         if (lane == 0) {
             work_slot[slot] = w;
@@ -316,15 +332,17 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
         bool ok = true;
         // Drawn items are fetched one ahead: the trip to the counter (and the positions past
         // the end of short sequences that a draw skips) then hides behind a whole item's loads
-        // instead of standing between two items.
+        // instead of standing between two items. (kSplit: behind the item's last loads, for as many CTAs to have a first
+        // item as there are items: with one drawn ahead half of them would have two.)
         int w_next = draw_item(0, ok);
         for (int n = 0; ok; ++n) {
+            if (kSplit && n > 0) w_next = draw_item(n, ok);
             const int w = w_next;
             if (w == -1) break;
-            w_next = draw_item(n + 1, ok);
+            if (!kSplit) w_next = draw_item(n + 1, ok);
             if (!ok) break;
             if (w == -2) continue;
-            const Work k = decode_work(tp, w);
+            const Work k = decode_work<kSplit>(tp, w, span);
             if (k.nblocks == 0) continue;
             const int hk = div_by(k.h, tp.by_group);
             int c[4], cv[4];
@@ -402,7 +420,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             const int w = take_item(n, ok, true);
             if (w == -1) break;
             if (w == -2) continue;
-            const Work k = decode_work(tp, w);
+            const Work k = decode_work<kSplit>(tp, w, span);
             if (k.nblocks == 0) continue;
             const bool mtracer = first_item && lane == 0 && blockIdx.x == 0;
             zone<kTrace>(tp, mtracer, 61, 0);
@@ -498,15 +516,23 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             const int w = take_item(n, ok, true);
             if (w == -1) break;
             if (w == -2) continue;
-            const Work k = decode_work(tp, w);
+            const Work k = decode_work<kSplit>(tp, w, span);
             if (!k.valid) continue;
             const SeqInfo& si = k.si;
             const int qi = k.q0 + row;                  // row inside the sequence
             const bool real = qi < si.lq;
+            // kSplit: the row's place among the parts (AttnParams), -1 where the sequence has only one.
+            int64_t place = -1;
+            if (kSplit && k.part >= 0) {
+                const int64_t rows = p.cu_q ? p.total_q : static_cast<int64_t>(p.batch) * p.sq;
+                place = ((k.part * rows) + (p.cu_q ? 0 : static_cast<int64_t>(k.b) * p.sq) + si.q_off + qi) * p.heads + k.h;
+            }
             __nv_bfloat16* og = p.out + k.b * p.os[0] + k.h * p.os[1] + static_cast<int64_t>(si.q_off + qi) * p.os[2] + g * (D / G);
             if (k.nblocks == 0) {
                 // No key is visible to this tile: zeros, lse = -inf. No barrier is involved.
-                if (real) {
+                if (kSplit && place >= 0) {
+                    if (real && g == 0) p.part_lse[place] = -INFINITY;   // (its rows of part_o are not read)
+                } else if (real) {
 #pragma unroll
                     for (int c = 0; c < D / G / 8; ++c) *reinterpret_cast<uint4*>(og + c * 8) = make_uint4(0u, 0u, 0u, 0u);
                     if (g == 0 && p.lse) p.lse[k.b * p.ls[0] + k.h * p.ls[1] + (si.q_off + qi) * p.ls[2]] = -INFINITY;
@@ -757,7 +783,13 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                         tc_fence_before();
                         mbar_arrive_warp(bar(P::bOFree));
                     }
-                    if (real) {
+                    if (kSplit && place >= 0) {
+                        if (real) {
+                            float4* to = reinterpret_cast<float4*>(p.part_o + place * D + g * kOut + c * kChunk);
+#pragma unroll
+                            for (int e = 0; e < kChunk / 4; ++e) to[e] = make_float4(acc[4 * e], acc[4 * e + 1], acc[4 * e + 2], acc[4 * e + 3]);
+                        }
+                    } else if (real) {
 #pragma unroll
                         for (int e = 0; e < kChunk / 16; ++e) {
                             uint32_t w[8];
@@ -768,7 +800,9 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                     }
                 }
                 zone<kTrace>(tp, tracer && g == 0, 60, 3);
-                if (real && g == 0 && p.lse) {
+                if (kSplit && place >= 0) {
+                    if (real && g == 0) p.part_lse[place] = l_sum > 0.f ? m_all + log2f(l_sum) : -INFINITY;   // (base 2)
+                } else if (real && g == 0 && p.lse) {
                     p.lse[k.b * p.ls[0] + k.h * p.ls[1] + (si.q_off + qi) * p.ls[2]] =
                         l_sum > 0.f ? kLn2 * (m_all + log2f(l_sum)) : -INFINITY;
                 }
@@ -1063,6 +1097,11 @@ int launch_tc5(const AttnParams& p, cudaStream_t stream) {
     const bool masked = p.mask_dtype != KTT_B200_MASK_NONE;
     auto kernel = masked ? (tp.trace ? fwd_tc5_kernel<D, true, true> : fwd_tc5_kernel<D, false, true>)
                          : (tp.trace ? fwd_tc5_kernel<D, true, false> : fwd_tc5_kernel<D, false, false>);
+    const bool split = p.parts != nullptr;
+    if (split) {
+        if (masked || !p.fwd_work_counter || p.most_parts < 1 || !p.part_o || !p.part_lse) return fail(KTT_B200_ERR_BAD_ARGUMENT, "tcgen05 forward: parts without their places");
+        kernel = fwd_tc5_kernel<D, false, false, true>;
+    }
     if (int rc = ensure_smem(kernel, smem, "cudaFuncSetAttribute(fwd_tc5)")) return rc;
     tp.q_tiles = (p.sq + kBM - 1) / kBM;
     tp.by_heads = divisor_of(p.heads);
@@ -1070,9 +1109,10 @@ int launch_tc5(const AttnParams& p, cudaStream_t stream) {
     tp.by_kv_heads = divisor_of(p.kv_heads);
     tp.by_group = divisor_of(p.heads / p.kv_heads);
     tp.by_per_pair = divisor_of(tp.q_tiles > 0 ? tp.q_tiles * (p.heads / p.kv_heads) : 1);
-    const int64_t work = static_cast<int64_t>(p.heads) * p.batch * tp.q_tiles;
-    if (work > 0x7fffffff) return fail(KTT_B200_ERR_UNSUPPORTED, "tcgen05 forward: too many query tiles");
+    const int64_t work = static_cast<int64_t>(p.heads) * p.batch * tp.q_tiles, all = work * (split ? p.most_parts : 1);
+    if (all > 0x7fffffff) return fail(KTT_B200_ERR_UNSUPPORTED, "tcgen05 forward: too many query tiles");
     tp.work = static_cast<int>(work);
+    tp.by_part = divisor_of(work > 0 ? tp.work : 1);
     // K / V that fit L2 comfortably (126 MB on B200) are read from HBM once whatever the
     // order, and the fixed deal of the length-sorted list is then the faster one (measured:
     // 940 against 857 TFLOP/s on 67 MB of K / V). Larger problems take the grouped order,
@@ -1084,10 +1124,10 @@ int launch_tc5(const AttnParams& p, cudaStream_t stream) {
     const bool explicit_counter = p.fwd_work_counter && !p.fwd_done_counter;
     tp.work_counter = (large || explicit_counter) ? p.fwd_work_counter : nullptr;
     tp.done_counter = tp.work_counter ? p.fwd_done_counter : nullptr;
-    tp.grouped = (tp.work_counter && (large || p.order)) ? 1 : 0;
+    tp.grouped = (tp.work_counter && (large || p.order || split)) ? 1 : 0;
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const int grid = tp.work < sms ? tp.work : sms;  // persistent: one CTA per SM
+    const int grid = all < sms ? static_cast<int>(all) : sms;  // persistent: one CTA per SM
     kernel<<<grid, P::kThreads, smem, stream>>>(mq, mk, mv, tp);
     return check_cuda(cudaGetLastError(), "fwd_tc5 launch");
 }

@@ -51,17 +51,6 @@ struct AppendParams {
     int vec;
 };
 
-// The sequence of packed row n, or -1: offsets do not decrease, sequences may be empty.
-__device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int64_t n) {
-    if (n < cu[0] || n >= cu[batch]) return -1;
-    int lo = 0, hi = batch - 1;   // the last b with cu[b] <= n
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (cu[mid] <= n) lo = mid; else hi = mid - 1;
-    }
-    return lo;
-}
-
 // Eight columns of one token in the cache's 4 bits. The 8 threads of a group of 64 columns are neighbours in a warp and
 // all arrive here; `there`: the row has a place. The codes are those of (x - least) / step rounded as fp32 does, to the
 // bit: the quotient is the product with 1 / step, corrected by its remainder (Markstein's theorem: with 1 / step correctly
@@ -182,7 +171,8 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
 struct ReadParams {
     Pages c;
     int rows;
-    int32_t* head;   // optional: 64 words that are cleared, then 0, rows, 2 rows, ..., then the sequences by falling length
+    int32_t* head;   // optional (kHeadWords)
+    int tiles, most_parts, sms, d;   // with it: what parts_of_chunk goes by; most_parts 0: no parts
     __nv_bfloat16* k;
     __nv_bfloat16* v;
     int64_t ks[3], vs[3];
@@ -216,17 +206,22 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
     const int len = cached_keys(p.c, b);
     if (p.head && blockIdx.x == 0 && head == 0) {
         if (threadIdx.x == 0) {
-            p.head[64 + b] = b * p.rows;
-            if (b == static_cast<int>(gridDim.z) - 1) p.head[64 + b + 1] = (b + 1) * p.rows;
+            p.head[kHeadWords + b] = b * p.rows;
+            if (b == static_cast<int>(gridDim.z) - 1) p.head[kHeadWords + b + 1] = (b + 1) * p.rows;
         }
-        if (b == 0 && threadIdx.x < 64) p.head[threadIdx.x] = 0;
+        if (b == 0 && threadIdx.x < kHeadWords && (threadIdx.x == 0 || threadIdx.x > 2 || !p.most_parts)) p.head[threadIdx.x] = 0;
         const int batch = gridDim.z;
         int place = 0;
         for (int i0 = 0; i0 < batch; i0 += 256) {
             const int i = i0 + threadIdx.x, other = i < batch ? cached_keys(p.c, i) : -1;
             place += __syncthreads_count(other > len || (other == len && i < b));
         }
-        if (threadIdx.x == 0) p.head[64 + batch + 1 + place] = b;
+        if (threadIdx.x == 0) p.head[kHeadWords + batch + 1 + place] = b;
+        if (threadIdx.x == 0 && place == 0 && p.most_parts) {   // (the longest)
+            const int blocks = (max(len, 1) + 127) / 128, parts = parts_of_chunk(p.tiles, blocks, p.sms, p.d, p.most_parts);
+            p.head[1] = parts;
+            p.head[2] = (blocks + parts - 1) / parts * 128;
+        }
     }
     // For the forward's sake no row behind a length is written, but one of a sequence without keys, which counts as one there.
     const int rows = p.head ? min(max(len, 1), p.rows) : p.rows;
@@ -330,11 +325,15 @@ int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, c
 
 }  // namespace
 
-int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, cudaStream_t stream) {
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, int tiles, int most_parts, int sms, cudaStream_t stream) {
     ReadParams p = {};
     p.c = c;
     p.rows = rows;
     p.head = head;
+    p.tiles = tiles;
+    p.most_parts = most_parts;
+    p.sms = sms;
+    p.d = d;
     p.k = static_cast<__nv_bfloat16*>(k);
     p.v = static_cast<__nv_bfloat16*>(v);
     for (int i = 0; i < 3; ++i) p.ks[i] = p.vs[i] = strides[i];

@@ -59,6 +59,41 @@ __device__ __forceinline__ int64_t page_of(const Pages& c, int b, int j) {
     return page >= 0 && page < c.pages ? page : -1;
 }
 
+// The sequence of packed row n, or -1: offsets do not decrease, sequences may be empty.
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int64_t n) {
+    if (n < cu[0] || n >= cu[batch]) return -1;
+    int lo = 0, hi = batch - 1;   // the last b with cu[b] <= n
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (cu[mid] <= n) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+// What the chunk path needs behind its dense rows (int32 words): a work counter and, from word 1, the parts that tiles are cut
+// into and the keys of a part; from kHeadWords the offsets of the dense rows, then the sequences by falling length.
+constexpr int kHeadWords = 64;
+
+// Parts (1 to `most`) that the keys of a chunk's tiles are cut into: `tiles` of 128 rows over up to `blocks` blocks of 128 keys,
+// on `sms` SMs that take an item each. In tenths of a microsecond: a block, an item's start and end, and what adding up the parts
+// costs (a launch, another kernel than whole tiles may take, and rows written and read at some 4 TB/s). Measured, us a call of bf16
+// pages, whole and in parts: 32 heads over 8, D 128, 64 tokens x 8,192 keys 74.0 and 34.8, 128 x 8,192 75.2 and 38.3, 256 x 4,096 45.6 and
+// 38.2; 2 x 16 over 2, D 64, 200 x 4,096 37.8 and 29.0; 14 over 2, D 64, 100 x 1,024 15.4 and 17.5 (left whole).
+__host__ __device__ inline int parts_of_chunk(int64_t tiles, int blocks, int sms, int d, int most) {
+    const int64_t block = d == 128 ? 10 : 7, item = 25;
+    int best = 1;
+    int64_t least = (tiles + sms - 1) / sms * (blocks * block + item);
+    for (int n = 2; n <= most; ++n) {
+        const int span = (blocks + n - 1) / n;
+        const int64_t cost = (tiles * n + sms - 1) / sms * (span * block + item) + 60 + n * tiles * d / 390;
+        if (cost < least) {
+            least = cost;
+            best = n;
+        }
+    }
+    return best;
+}
+
 // Fills the cache's fields from an argument block after its checks (paged.cu); null, or why not.
 const char* pages_of(Pages& c, const ktt_b200_pages& a, int d);
 

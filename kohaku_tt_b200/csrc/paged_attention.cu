@@ -32,7 +32,7 @@ namespace ktt {
 
 // paged.cu: dense rows of the cache for a chunk of a prompt; 64 words of `head` are cleared, behind them go the offsets 0, rows,
 // 2 rows, ... (batch + 1), and the sequences by falling length.
-int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, cudaStream_t stream);
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, int tiles, int most_parts, int sms, cudaStream_t stream);
 
 namespace {
 
@@ -929,9 +929,18 @@ struct Plan {
     bool few;
     int nt, row_tiles, slice;   // sequences of a launch
     int64_t bytes;              // of workspace
+    int tiles, parts;           // chunks: tiles of 128 rows of a launch, and the most parts that their keys are cut into (0: none)
+    int64_t parts_at;           // where in the workspace the parts' rows are
 };
 
+// Tiles that are too few for the SMs are cut along their keys where that pays for the longest sequence that the table has room
+// for; into how many parts then goes by the longest there is (parts_of_chunk, in read_pages), of which there may be two for every SM.
+constexpr int kMostParts = 16;
+
 int64_t rows_per_head(const ktt_b200_paged_sdpa_args* a) { return static_cast<int64_t>(a->heads / a->cache.kv_heads) * a->sq; }
+
+// Rows of a launch over `batch` sequences that parts have a place for.
+int64_t part_rows(const ktt_b200_paged_sdpa_args* a, int batch) { return a->cu_seqlens_q ? a->total_q : static_cast<int64_t>(batch) * a->sq; }
 
 Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     Plan s = {};
@@ -952,7 +961,19 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     most = (1ll << 30) / one;
     s.slice = static_cast<int>(most < 1 ? 1 : (most < a->batch ? most : a->batch));
     if (s.slice > kMaxBatch) s.slice = kMaxBatch;
-    s.bytes = s.slice * one + (64 + 2 * kMaxBatch + 1) * 4;   // and what is behind the rows (run_many)
+    s.parts_at = s.slice * one + ((kHeadWords + 2 * kMaxBatch + 1) * 4 + 255) / 256 * 256;
+    s.bytes = s.parts_at;
+    const bool packed = a->cu_seqlens_q != nullptr;
+    int64_t tiles = s.slice * static_cast<int64_t>((a->sq + 127) / 128);
+    if (packed && a->total_q / 128 + s.slice < tiles) tiles = a->total_q / 128 + s.slice;
+    tiles *= a->heads;
+    int64_t parts = 2 * sms / tiles;
+    if (parts > kMostParts) parts = kMostParts;
+    if (parts > 1 && parts_of_chunk(tiles, (c.cap + 127) / 128, sms, a->d, static_cast<int>(parts)) > 1) {
+        s.tiles = static_cast<int>(tiles);
+        s.parts = static_cast<int>(parts);
+        s.bytes += parts * part_rows(a, s.slice) * a->heads * (a->d + 1) * 4;
+    }
     return s;
 }
 
@@ -997,11 +1018,87 @@ const char* sdpa_refusal(const ktt_b200_paged_sdpa_args* a, Pages& c) {
     return nullptr;
 }
 
+// Rows of chunks whose sequence has more than one part: the parts' rows, each with its base-2 logarithm of the sum of weights,
+// added up. D / 4 threads have a row of a head.
+struct MergeParams {
+    Pages c;
+    const float* o;      // [parts][rows][heads][D]
+    const float* lse;    // [parts][rows][heads]
+    const int32_t* cu;   // packed
+    const int32_t* parts;   // (parts, keys of a part)
+    int64_t rows;
+    int batch, heads, sq;
+    __nv_bfloat16* out;
+    int64_t os[3];
+};
+template <int D>
+__global__ void __launch_bounds__(256) merge_parts_kernel(const __grid_constant__ MergeParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y, row = n / p.heads;
+    if (row >= p.rows) return;
+    const int h = static_cast<int>(n - row * p.heads), c4 = threadIdx.x;
+    const int b = p.cu ? sequence_of(p.cu, p.batch, row) : static_cast<int>(row / p.sq);
+    if (b < 0) return;
+    const int span = p.parts[1], parts = (cached_keys(p.c, b) + span - 1) / span;
+    if (parts <= 1) return;
+    const int64_t step = p.rows * p.heads;
+    float m = -INFINITY, sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    constexpr int kAhead = 4;
+    for (int i0 = 0; i0 < parts; i0 += kAhead) {
+        float l[kAhead], top = m;
+        float4 v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            l[j] = -INFINITY;
+            v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i0 + j < parts) {
+                const int64_t at = (i0 + j) * step + n;
+                l[j] = __ldcg(p.lse + at);
+                v[j] = __ldcg(reinterpret_cast<const float4*>(p.o + at * D) + c4);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) top = fmaxf(top, l[j]);
+        if (top == -INFINITY) continue;
+        const float f = fast_exp2(m - top);
+        m = top;
+        sum *= f;
+        acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (l[j] == -INFINITY) continue;   // (a part that the row sees nothing of has written no row)
+            const float w = fast_exp2(l[j] - top);
+            sum += w;
+            acc.x = fmaf(v[j].x, w, acc.x); acc.y = fmaf(v[j].y, w, acc.y);
+            acc.z = fmaf(v[j].z, w, acc.z); acc.w = fmaf(v[j].w, w, acc.w);
+        }
+    }
+    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const int64_t r = p.cu ? row : row - static_cast<int64_t>(b) * p.sq;
+    __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + h * p.os[1] + r * p.os[2] + 4 * c4;
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+}
+
+int merge_parts(const MergeParams& p, int d, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(static_cast<unsigned>(d / 4), static_cast<unsigned>(1024 / d));
+    cfg.gridDim = dim3(static_cast<unsigned>((p.rows * p.heads + cfg.blockDim.y - 1) / cfg.blockDim.y));
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, d == 64 ? merge_parts_kernel<64> : merge_parts_kernel<128>, p), "paged_sdpa merge launch");
+}
+
 // A chunk of a prompt: the rows of a K / V head are many, so the work is in the products, which the tensor kernels of the
 // dense and packed forward do; the pages become dense bf16 rows for them first (2 x 2 D bytes written and read per key
 // and head, against 4 D operations per key and row).
-int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice, cudaStream_t stream) {
-    const int hk = a->cache.kv_heads, d = a->d;
+int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan& plan, cudaStream_t stream) {
+    const int hk = a->cache.kv_heads, d = a->d, slice = plan.slice;
     const int64_t cap = p.c.cap, half = slice * cap * hk * d;
     __nv_bfloat16* k = static_cast<__nv_bfloat16*>(a->workspace);
     __nv_bfloat16* v = k + half;
@@ -1044,14 +1141,42 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, int slice,
             f.total_q = a->total_q;
             f.total_k = slice * cap;
             f.cu_seqlens_q = a->cu_seqlens_q + b0;
-            f.cu_seqlens_k = head + 64;
+            f.cu_seqlens_k = head + kHeadWords;
             f.q_strides[0] = f.out_strides[0] = f.k_strides[0] = f.v_strides[0] = 0;
         } else {
             f.q = p.q + b0 * a->q_strides[0];
             f.out = p.out + b0 * a->out_strides[0];
         }
-        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, stream)) return rc;
-        if (int rc = forward_in_order(&f, d == 128 && several ? head + 64 + n + 1 : nullptr, stream)) return rc;
+        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, plan.tiles, plan.parts, sm_count(current_device()), stream)) return rc;
+        ForwardParts x = {};
+        bool parts = plan.parts > 0;
+        if (parts) {
+            f.kernel = KTT_B200_KERNEL_TC5_WIDE;
+            parts = ktt_b200_sdpa_supported(&f) != 0;   // (else its copies cannot address the operands)
+            if (!parts) f.kernel = KTT_B200_KERNEL_AUTO;
+            f.workspace = parts ? head : nullptr;
+            f.workspace_bytes = parts ? 4 : 0;
+        }
+        if (parts || (d == 128 && several)) x.order = head + kHeadWords + n + 1;
+        MergeParams m = {};
+        if (parts) {
+            m.c = c;
+            m.cu = f.cu_seqlens_q;
+            m.rows = part_rows(a, n);
+            x.parts = m.parts = head + 1;
+            x.most_parts = plan.parts;
+            m.o = x.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + plan.parts_at);
+            m.lse = x.part_lse = x.part_o + plan.parts * m.rows * a->heads * d;
+            m.batch = n;
+            m.heads = a->heads;
+            m.sq = a->sq;
+            m.out = static_cast<__nv_bfloat16*>(f.out);
+            for (int i = 0; i < 3; ++i) m.os[i] = f.out_strides[i];
+        }
+        if (int rc = forward_in_parts(&f, x, stream)) return rc;
+        if (parts) {
+            if (int rc = merge_parts(m, d, stream)) return rc;
+        }
     }
     return 0;
 }
@@ -1094,7 +1219,7 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     p.q = static_cast<const __nv_bfloat16*>(a->q);
     p.out = static_cast<__nv_bfloat16*>(a->out);
-    if (!s.few) return run_many(a, p, s.slice, st);
+    if (!s.few) return run_many(a, p, s, st);
     p.heads = a->heads;
     p.row_tiles = s.row_tiles;
     p.kv_heads = a->cache.kv_heads * s.row_tiles;

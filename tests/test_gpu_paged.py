@@ -337,6 +337,18 @@ def _cut(cuda, bits, max_k):
 
 @pytest.mark.parametrize("bits", BITS)
 @pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("d,causal", [(64, True), (64, False), (128, True), (128, False)])
+def test_chunks_cut_along_their_keys(cuda, bits, packed, d, causal):
+    """Few tiles and many keys: parts that end in a tile's diagonal, that no row or only some rows see, that hold one key, and
+    sequences of one part or none beside them. Parts are added up in fp32: no rounding more than _near counts."""
+    counts = [130, 60, 1, 0, 256, 49] if packed else 130
+    _check(cuda, bits, d, 2, 1, 32, counts, [3000, 1025, 2048, 700, 2049, 49], packed=packed, causal=causal, dense_four_bits=bits == 4)
+    _check(cuda, bits, d, 4, 2, 64, 1100, [1100], causal=causal, dense_four_bits=bits == 4, seed=3)
+    _check(cuda, bits, d, 3, 3, 16, 50, [0, 2500], causal=causal, dense_four_bits=bits == 4, seed=4)
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("packed", [False, True])
 @pytest.mark.parametrize("d,hk", [(128, 8), (64, 16)])
 def test_chunks_over_more_room_than_one_launch_takes(cuda, bits, packed, d, hk):
     """Room for 65,536 keys: the dense rows of 4 sequences are 1 GB, so 6 are two launches of 4 and 2."""
@@ -402,7 +414,7 @@ def test_pages_and_queries_in_other_orders(cuda, n):
 
 
 @pytest.mark.parametrize("bits", BITS)
-@pytest.mark.parametrize("b,n,cap", [(1, 1, 4096), (64, 1, 1024), (3, 2, 600), (2, 200, 500)])
+@pytest.mark.parametrize("b,n,cap", [(1, 1, 4096), (64, 1, 1024), (3, 2, 600), (2, 200, 500), (2, 100, 6000)])
 def test_the_same_bits_every_time(cuda, bits, b, n, cap):
     """No result goes by the order in which parts of a sequence are done."""
     g = torch.Generator().manual_seed(b)
