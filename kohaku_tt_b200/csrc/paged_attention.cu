@@ -917,12 +917,21 @@ Parts parts_of(int64_t pairs, int d, int ctas) {
     return s;
 }
 
-// Tokens of a sequence up to which a K / V head's keys are passed over once for every 8 or 16 of its rows (heads x tokens);
-// more are a matter for the tensor path (below), which takes 128 tokens of one head at a time, full or not. Measured, us, this
-// pass and that path, bf16 and 4 bits: 32 x 16 heads x up to 1,024 keys, D 64, 16 tokens 31 and 70, 25 and 64, 64 tokens 92 and 72,
-// 75 and 66; 32 x 32 heads over 8 x 2,048, D 128, 16 tokens 104 and 164, 95 and 161; 1 x 32 over 8 x 8,192, 32 tokens 26 and 48,
-// 25 and 49, 128 tokens 72 and 49, 71 and 51.
-constexpr int kFewTokens = 48;
+// Up to kFewTokens tokens of a sequence there are two ways: the pass above over a K / V head's keys for every 8 or 16 of its rows
+// (heads x tokens), and the tensor path below, which makes dense rows of the keys and takes 128 tokens of one head at a time, full
+// or not. Which is the shorter goes by what each costs for a K / V head and 128 keys: the pass, rows / 16 times `pass`; the tensor
+// path, `dense` for the rows and `tile` for each head; and by 9 and 12 us that they take whatever the sizes. Measured, us, pass and
+// tensor path, bf16, D 128: 32 heads over 8, 1 x 8,192, 24 tokens 29.9 and 33.9, 48 tokens 49.4 and 34.5; 4 x 4,096, 24 tokens 54 and 59,
+// 48 tokens 96 and 60; 32 x 2,048, 24 tokens 184 and 208, 32 tokens 220 and 208; 8 x 16 heads x 4,096, 48 tokens 122 and 134, 64 tokens
+// 159 and 134; D 64: 32 x 16
+// heads x 1,024, 48 tokens 81 and 88, 64 tokens 96 and 89, with 4 bits 77 and 79; 14 heads over 2, 1 x 4,096, 48 tokens 16 and 19.
+constexpr int kFewTokens = 64;
+bool pass_pays(int bits, int d, int64_t heads, int64_t kv_heads, int64_t batch, int64_t row_tiles, int64_t blocks) {
+    const double pass = d == 128 ? (bits == 16 ? 0.0075 : 0.0066) : (bits == 16 ? 0.0053 : 0.0042);
+    const double tile = d == 128 ? 0.006 : 0.004, dense = d == 128 ? 0.023 : 0.015;
+    const double units = static_cast<double>(batch * kv_heads) * blocks;
+    return 9 + units * pass * row_tiles <= 12 + units * (tile * (heads / kv_heads) + dense);
+}
 
 // What a call will do, from its sizes alone.
 struct Plan {
@@ -949,7 +958,7 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     s.row_tiles = static_cast<int>((rows + 8 * s.nt - 1) / (8 * s.nt));
     // Units of all pairs of a launch have to fit 30 bits.
     int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 16 + 32) * hk * s.row_tiles);
-    s.few = a->sq <= kFewTokens && most > 0;
+    s.few = a->sq <= kFewTokens && most > 0 && pass_pays(a->cache.bits, a->d, a->heads, hk, a->batch, (rows + 15) / 16, (c.cap + 127) / 128);
     if (s.few) {
         if (most > kMaxBatch) most = kMaxBatch;
         s.slice = static_cast<int>(a->batch < most ? a->batch : most);

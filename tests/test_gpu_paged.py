@@ -298,6 +298,14 @@ def test_both_sides_of_the_choice_by_tokens(cuda, bits, n):
 
 
 @pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("n", [24, 40, 64, 65])
+def test_both_sides_of_the_choice_by_rows(cuda, bits, n):
+    """Eight rows to a token of a K / V head, over room for many keys, and one."""
+    _check(cuda, bits, 128, 16, 2, 32, n, [60, 300, 1], wide=256, dense_four_bits=bits == 4)
+    _check(cuda, bits, 64, 3, 3, 32, n, [60, 300, 1], wide=256, dense_four_bits=bits == 4)
+
+
+@pytest.mark.parametrize("bits", BITS)
 def test_more_sequences_than_a_launch_takes(cuda, bits):
     """Over 512 sequences are several launches, dense and packed."""
     b = 700
