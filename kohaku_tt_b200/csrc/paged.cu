@@ -71,13 +71,17 @@ __device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, uns
     uint32_t word = 0;
     if (s > 0.f && s < INFINITY) {   // (else all codes are 0)
         const float even = s < 0x1p-60f ? 0x1p100f : (s > 0x1p60f ? 0x1p-100f : 1.f), r = s * even, inv = __frcp_rn(r);
+        const Pair least2(least), even2(even), inv2(inv), r2(-r), whole2(8388608.f);
+        Pair codes(0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float d = __fsub_rn(to_f32(x.get(e)), least) * even, q = d * inv;
-            const float t = fmaf(fmaf(-q, r, d), inv, q);
-            // To the nearest whole number in the low bits, ties to even; t is at most 15 (1 + 2^-8).
-            word |= (__float_as_uint(t + 8388608.f) & 15u) << (4 * ((e >> 1) + 4 * (e & 1)));
+        for (int n = 3; n >= 0; --n) {
+            const Pair d = sub(Pair(to_f32(x.get(2 * n)), to_f32(x.get(2 * n + 1))), least2) * even2, q = d * inv2;
+            const Pair t = fma(fma(q, r2, d), inv2, q);
+            // To the nearest whole number, ties to even (t is at most 15 (1 + 2^-8)); four of them make one of 16 bits.
+            codes = fma(codes, Pair(16.f), sub(t + whole2, whole2));
         }
+        codes = codes + whole2;
+        word = __byte_perm(__float_as_uint(codes.low()), __float_as_uint(codes.high()), 0x5410);
     }
     if (!there) return;
     uint32_t* to = reinterpret_cast<uint32_t*>(block);
@@ -178,17 +182,17 @@ struct ReadParams {
     int64_t ks[3], vs[3];
 };
 
-// What eight codes are worth.
+// What eight codes are worth: bf16 products and sums of pairs, rounded once. (An fp32 sum rounded to bf16 is the same: where step
+// is under 2^-15 of least's power of two, so that fp32 cannot hold the sum, all 15 steps are less than half of bf16's.)
 __device__ __forceinline__ Eight<__nv_bfloat16> of_four_bits(uint32_t word, uint32_t pair) {
-    const float step = step_of(pair), least = least_of(pair);
+    const __nv_bfloat162 ends = *reinterpret_cast<const __nv_bfloat162*>(&pair), step = __low2bfloat162(ends), least = __high2bfloat162(ends);
+    const __nv_bfloat162 zero = __float2bfloat162_rn(128.f);
     Eight<__nv_bfloat16> x;
-    uint32_t* to = reinterpret_cast<uint32_t*>(x.raw);
+    __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(x.raw);
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        // Two codes as bf16 128 + c, whose fp32 is a shift away. (step * code is exact in fp32: one rounding to fp32, one to bf16.)
-        const uint32_t two = ((word >> (4 * n)) & 0x000f000fu) | 0x43004300u;
-        const float a = __uint_as_float(two << 16) - 128.f, b = __uint_as_float(two & 0xffff0000u) - 128.f;
-        to[n] = pack_bf16(fmaf(step, a, least), fmaf(step, b, least));
+        const uint32_t two = ((word >> (4 * n)) & 0x000f000fu) | 0x43004300u;   // two codes as bf16 128 + c
+        to[n] = __hfma2(step, __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&two), zero), least);
     }
     return x;
 }
