@@ -140,6 +140,33 @@ def test_append(cuda, bits, packed, d, r, interleaved, page, hk, h, new, lengths
 
 
 @pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_appends_of_many_sequences(cuda, bits, d):
+    """Over 31 sequences, empty ones among them, with rows before the first and behind the last, against two calls of fewer."""
+    hk, page, b = 2, 16, 40
+    counts, lens = [(7 * i) % 4 for i in range(b)], [(5 * i) % 40 for i in range(b)]
+    starts = [3]
+    for n in counts:
+        starts.append(starts[-1] + n)
+    t = starts[-1] + 5
+    k, v, q = (_x(t, h, d, seed=h + i).to(cuda) for i, h in enumerate((hk, hk, 6)))
+    cos, sin = ktt.rotary_table(64, d, device=cuda)
+    table = torch.randperm(b * 4, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(b, 4).to(cuda)
+    lengths = torch.tensor(lens, dtype=torch.int32, device=cuda)
+    cu = torch.tensor(starts, dtype=torch.int32, device=cuda)
+    outs = []
+    for parts in ([(0, b)], [(0, 17), (17, 31), (31, b)]):
+        kp, vp = ktt.paged_cache(b * 4, hk, page, d, bits=bits, device=cuda)
+        after, rows = torch.zeros(b, dtype=torch.int32, device=cuda), torch.zeros_like(q)
+        for lo, hi in parts:
+            got = ktt.paged_append(k, v, kp, vp, table[lo:hi], lengths[lo:hi], cos, sin, q=q, cu_seq=cu[lo:hi + 1], lengths_out=after[lo:hi])
+            rows[starts[lo]:starts[hi]] = got[starts[lo]:starts[hi]]
+        outs.append((kp, vp, after, rows))
+    assert all(torch.equal(x, y) for x, y in zip(*outs))
+    assert outs[0][2].tolist() == [x + y for x, y in zip(lens, counts)]
+
+
+@pytest.mark.parametrize("bits", BITS)
 def test_rows_without_a_page_go_nowhere(cuda, bits):
     """Holes in the table, a table that ends, lengths out of range: no other byte of the pool changes."""
     d, hk, page = 64, 2, 16
