@@ -236,7 +236,8 @@ int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
         return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "rotary launch");
     };
     // Four heads to a thread once that fills the GPU: a row's position and table entries are read once for all of them.
-    // 4 x 4,096 tokens, 32 heads over 8, D 128, bf16, forward and gradient, us for 1 and 4 heads: 671 and 400.
+    // 4 x 4,096 tokens, 32 heads over 8, D 128, bf16, forward and gradient, us for 1 and 4 heads: 671 and 400. (Of the latter's
+    // bytes 92 to 95 % of a copy's rate: forward alone, 16 x 4,096 tokens, 16 + 16 heads, 175.7 us, 6.1 TB/s.)
     if (p.tokens * chunks * (p.heads[0] + p.heads[1]) >= kManyThreads) {
         if (fast) return go(rotary_kernel<T, true, 4>, 4);
         return go(rotary_kernel<T, false, 4>, 4);
