@@ -7,8 +7,6 @@
 #pragma once
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 #include "common.cuh"
 
 namespace ktt {
@@ -35,7 +33,8 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// Two fp32 values that one instruction works on, each rounded as by itself.
+// Two fp32 values that one instruction works on, each rounded as by itself; but a product and a sum behind it are joined into
+// one rounding by the compiler, whatever the instructions say, so what rounds them one by one stays with __fmul_rn and __fadd_rn.
 struct Pair {
     unsigned long long v;
     __device__ __forceinline__ Pair() {}
@@ -72,14 +71,6 @@ struct Eight {
     uint4 raw[kPieces];
     __device__ __forceinline__ T get(int e) const { return reinterpret_cast<const T*>(raw)[e]; }
     __device__ __forceinline__ void set(int e, T x) { reinterpret_cast<T*>(raw)[e] = x; }
-    __device__ __forceinline__ void set2(int e, float a, float b) {
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            reinterpret_cast<__nv_bfloat162*>(raw)[e / 2] = __floats2bfloat162_rn(a, b);
-        } else {
-            set(e, from_f32<T>(a));
-            set(e + 1, from_f32<T>(b));
-        }
-    }
     __device__ __forceinline__ void zero() {
 #pragma unroll
         for (int i = 0; i < kPieces; ++i) raw[i] = make_uint4(0, 0, 0, 0);
@@ -161,23 +152,14 @@ struct Turned {
     __device__ __forceinline__ void apply(const Turn& t, Eight<T>& x, const Eight<T>& other, const T* row, int col) const {
         if (count == 0) return;
         const Eight<T> old = x;
-        if (kFast) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float a = to_f32(old.get(e)), b = to_f32(old.get(e + 1));
-                const Pair p = t.interleaved ? Pair(b, a) : Pair(to_f32(other.get(e)), to_f32(other.get(e + 1)));
-                const Pair y = Pair(a, b) * Pair(c[e], c[e + 1]) + p * Pair(s[e], s[e + 1]);
-                x.set2(e, y.low(), y.high());
-            }
-            return;
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float p;
             if (t.interleaved) p = to_f32(old.get(e ^ 1));
+            else if (kFast) p = to_f32(other.get(e));
             else p = e < count ? to_f32(row[col + e < t.half ? col + e + t.half : col + e - t.half]) : 0.f;
             // A column that does not turn is copied, whatever its neighbours hold.
-            if (e < count) x.set(e, from_f32<T>(__fadd_rn(__fmul_rn(to_f32(old.get(e)), c[e]), __fmul_rn(p, s[e]))));
+            if (kFast || e < count) x.set(e, from_f32<T>(__fadd_rn(__fmul_rn(to_f32(old.get(e)), c[e]), __fmul_rn(p, s[e]))));
         }
     }
 };

@@ -77,6 +77,20 @@ def test_rotation_and_gradient(cuda, h, hk, n, d, r, interleaved, dtype):
 
 
 @pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("b,s,d", [(1, 70, 64), (4, 4096, 128), (2, 500, 50)])
+def test_products_and_sum_are_rounded_one_by_one(cuda, b, s, d, dtype, interleaved):
+    """To the bit: what separate fp32 operators give. One thread's heads are four in the large call, one in the others."""
+    q = _x(b, 8, s, d, dtype=dtype).to(cuda)
+    cos, sin = ktt.rotary_table(s, d, device=cuda)
+    x = q.float()
+    x1, x2 = (x[..., ::2], x[..., 1::2]) if interleaved else (x[..., :d // 2], x[..., d // 2:])
+    y1, y2 = x1 * cos - x2 * sin, x2 * cos + x1 * sin
+    want = torch.stack((y1, y2), -1).flatten(-2) if interleaved else torch.cat((y1, y2), -1)
+    assert torch.equal(ktt.rotary(q, None, cos, sin, interleaved=interleaved)[0], want.to(dtype))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
 def test_gradient_against_differences(cuda, interleaved):
     """fp32: the loss is linear in x, so a difference quotient is exact up to rounding: 2^-24 of the loss's terms
     over the step."""
