@@ -325,8 +325,8 @@ int launch_append(const AppendParams& given, cudaStream_t stream) {
     };
     const bool fast = p.vec && turn_is_fast(p.turn);
     // Four heads to a thread once that fills the GPU: a token's place, page and table rows are looked up once for all of
-    // them. 10,240 packed tokens, 32 heads over 8, D 128, us for 1, 2, 4 and 8 heads: bf16 pages 94.8, 69.7, 50.8, 48.4
-    // (5.0 TB/s at 4); 4 bits 102.6, 77.3, 59.3, 58.6, of which keys and values 28 (queries alone run at a copy's rate).
+    // them. 10,240 packed tokens, 32 heads over 8, D 128, us for 1, 2, 4 and 8 heads: bf16 pages 94.8, 69.7, 51.3, 48.4
+    // (4.9 TB/s at 4); 4 bits 102.6, 77.3, 60.1, 58.6, of which keys and values 28 (queries alone run at a copy's rate).
     if (p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads) >= 4 * 148 * 2048) {
         if (fast) return go(append_kernel<D, kBits, true, 4>, 4);
         return go(append_kernel<D, kBits, false, 4>, 4);
