@@ -801,7 +801,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                 }
                 zone<kTrace>(tp, tracer && g == 0, 60, 3);
                 if (kSplit && place >= 0) {
-                    if (real && g == 0) p.part_lse[place] = l_sum > 0.f ? m_all + log2f(l_sum) : -INFINITY;   // (base 2)
+                    if (real && g == 0) p.part_lse[place] = l_sum == 0.f ? -INFINITY : m_all + log2f(l_sum);   // (base 2; a NaN stays one)
                 } else if (real && g == 0 && p.lse) {
                     p.lse[k.b * p.ls[0] + k.h * p.ls[1] + (si.q_off + qi) * p.ls[2]] =
                         l_sum > 0.f ? kLn2 * (m_all + log2f(l_sum)) : -INFINITY;

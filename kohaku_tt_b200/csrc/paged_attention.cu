@@ -1068,23 +1068,27 @@ __global__ void __launch_bounds__(256) merge_parts_kernel(const __grid_constant_
                 v[j] = __ldcg(reinterpret_cast<const float4*>(p.o + at * D) + c4);
             }
         }
+        bool seen = false;   // (a NaN is seen, though it is no maximum)
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) top = fmaxf(top, l[j]);
-        if (top == -INFINITY) continue;
-        const float f = fast_exp2(m - top);
+        for (int j = 0; j < kAhead; ++j) {
+            top = fmaxf(top, l[j]);
+            seen |= !(l[j] == -INFINITY);
+        }
+        if (!seen) continue;
+        const float base = top == -INFINITY ? 0.f : top, f = fast_exp2(m - base);
         m = top;
         sum *= f;
         acc.x *= f; acc.y *= f; acc.z *= f; acc.w *= f;
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             if (l[j] == -INFINITY) continue;   // (a part that the row sees nothing of has written no row)
-            const float w = fast_exp2(l[j] - top);
+            const float w = fast_exp2(l[j] - base);
             sum += w;
             acc.x = fmaf(v[j].x, w, acc.x); acc.y = fmaf(v[j].y, w, acc.y);
             acc.z = fmaf(v[j].z, w, acc.z); acc.w = fmaf(v[j].w, w, acc.w);
         }
     }
-    const float inv = sum > 0.f ? 1.f / sum : 0.f;
+    const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // (a NaN stays one)
     const int64_t r = p.cu ? row : row - static_cast<int64_t>(b) * p.sq;
     __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + h * p.os[1] + r * p.os[2] + 4 * c4;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
