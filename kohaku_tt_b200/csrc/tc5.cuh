@@ -246,11 +246,20 @@ __device__ __forceinline__ float exp2_poly(float x) {
 }
 
 // The same for two values at once on the packed fp32 pipe (fma.rn.f32x2 / add.f32x2 halve
-// the instruction count of the softmax loop, which is issue-bound).
+// the instruction count of the softmax loop, which is issue-bound). kNan: a NaN comes out as the
+// largest fp32 value, whose weight and sum leave the row nothing finite (the integer step that adds
+// the exponent turns a NaN into that; a maximum that drops it would make it 2^-125 instead, and the
+// row a softmax without the key). Both maxima are one instruction.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+template <bool kNan = true>
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
     const float2 magic = make_float2(12582912.f, 12582912.f);
-    x.x = fmaxf(x.x, -125.f);
-    x.y = fmaxf(x.y, -125.f);
+    x.x = kNan ? max_nan(x.x, -125.f) : fmaxf(x.x, -125.f);
+    x.y = kNan ? max_nan(x.y, -125.f) : fmaxf(x.y, -125.f);
     const float2 t = __fadd2_rn(x, magic);
     const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
     const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
@@ -266,7 +275,7 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
 // exp2_poly2 with exact zeros: anything below 2^-120 (a row whose lse is +inf, i.e. one that
 // does not exist or saw no key) gives 0, as MUFU's 2^-inf does.
 __device__ __forceinline__ float2 exp2_poly2_zero(float2 x) {
-    float2 r = exp2_poly2(x);
+    float2 r = exp2_poly2<false>(x);
     r.x = x.x < -120.f ? 0.f : r.x;
     r.y = x.y < -120.f ? 0.f : r.y;
     return r;

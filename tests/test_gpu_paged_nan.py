@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import kohaku_tt_b200 as ktt
+from kohaku_tt_b200 import ops
 from oracle import paged_oracle as po
 from tests.launched import launched
 from tests.test_gpu_paged import _poison, _store, _table, _x
@@ -90,6 +91,23 @@ def _places(n, length):
     return [j for j in (0, 21, 38, 63, 64, 77, 101, 127, 128, 700, 1500, length - n) if j <= length - n]
 
 
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("d,h,hk,n,lengths,cut", CASES)
+def test_keys_that_all_rows_see(cuda, bits, packed, d, h, hk, n, lengths, cut):
+    """A NaN in a key of one K / V head: none of its query heads' rows has a finite value, all others keep their bits."""
+    run = _Run(cuda, bits, d, h, hk, n, lengths, packed)
+    clean, group = run(), h // hk
+    for j in _places(n, lengths[0]):
+        page, row = run.at(0, j)
+        k = run.k.clone()
+        k[page, 0, row, 5] = NAN
+        got = run(k=k)
+        assert not torch.isfinite(got[0, :group]).any(), j
+        got[0, :group] = clean[0, :group]
+        assert torch.equal(got, clean), j
+
+
 @pytest.mark.parametrize("packed", [False, True])
 @pytest.mark.parametrize("d,h,hk,n,lengths,cut", CASES)
 def test_an_infinite_key(cuda, packed, d, h, hk, n, lengths, cut):
@@ -109,3 +127,13 @@ def test_an_infinite_key(cuda, packed, d, h, hk, n, lengths, cut):
         off = (got[~up].double() - want[0][:group][~up]).abs()
         # Half a step of bf16 weights and of the result, of |v| <= 6 (and sums and logits in fp32: less than that once more).
         assert off.max() <= 3 * 2.0 ** -8 * run.v.abs().max()
+
+
+@pytest.mark.parametrize("kernel,d", [("flash", 64), ("flash_wide", 64), ("flash_wide", 128), ("flash_pair", 64), ("flash_pair", 80), ("flash_pair", 128), ("mma", 64)])
+def test_keys_of_the_dense_forward(cuda, kernel, d):
+    """The kernels that chunks run on, over plain keys: a NaN at every place of two blocks, a head each."""
+    h, n = 256, 256
+    q, k, v = (_x(1, h, n, d, seed=i).to(cuda) for i in range(3))
+    k[0, torch.arange(h), torch.arange(n), 3] = NAN
+    out, _ = ops.sdpa_forward(q, k, v, kernel=kernel)
+    assert not torch.isfinite(out).any()
