@@ -429,7 +429,7 @@ KTT_B200_API int ktt_b200_paged_read(const ktt_b200_read_args* args, void* strea
 /* Attention over the cache: q dense [B, H, sq, D] or packed [total_q, H, D] (cu_seqlens_q int32 [batch + 1] on the device, sq
  * = the longest, batch stride 0), D 64 or 128. `lengths` count the keys with those of the call's own tokens. causal (1):
  * query i of n sees keys j <= length - n + i; a row that sees none gets zeros. Packed rows that no sequence covers are
- * left as they were. */
+ * left as they were; offsets outside of [0, total_q] are taken as its ends. */
 typedef struct ktt_b200_paged_sdpa_args {
     ktt_b200_pages cache;
     int32_t batch, heads, sq, d;

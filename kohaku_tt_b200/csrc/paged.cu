@@ -195,8 +195,7 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
 struct ReadParams {
     Pages c;
     int rows;
-    int32_t* head;   // optional (kHeadWords)
-    int tiles, most_parts, sms, d;   // with it: what parts_of_chunk goes by; most_parts 0: no parts
+    ChunkHead head;
     __nv_bfloat16* k;
     __nv_bfloat16* v;
     int64_t ks[3], vs[3];
@@ -228,27 +227,32 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int len = cached_keys(p.c, b);
-    if (p.head && blockIdx.x == 0 && head == 0) {
-        if (threadIdx.x == 0) {
-            p.head[kHeadWords + b] = b * p.rows;
-            if (b == static_cast<int>(gridDim.z) - 1) p.head[kHeadWords + b + 1] = (b + 1) * p.rows;
-        }
-        if (b == 0 && threadIdx.x < kHeadWords && (threadIdx.x == 0 || threadIdx.x > 2 || !p.most_parts)) p.head[threadIdx.x] = 0;
+    if (p.head.words && blockIdx.x == 0 && head == 0) {
         const int batch = gridDim.z;
+        if (threadIdx.x == 0) {
+            const bool last = b == batch - 1;
+            p.head.offsets()[b] = b * p.rows;
+            if (last) p.head.offsets()[batch] = batch * p.rows;
+            if (p.head.cu_q) {
+                p.head.query_offsets(batch)[b] = row_offset(p.head.cu_q, b, p.head.total_q);
+                if (last) p.head.query_offsets(batch)[batch] = row_offset(p.head.cu_q, batch, p.head.total_q);
+            }
+        }
+        if (b == 0 && threadIdx.x < kHeadWords && (threadIdx.x == 0 || threadIdx.x > 2 || !p.head.most_parts)) p.head.words[threadIdx.x] = 0;
         int place = 0;
         for (int i0 = 0; i0 < batch; i0 += 256) {
             const int i = i0 + threadIdx.x, other = i < batch ? cached_keys(p.c, i) : -1;
             place += __syncthreads_count(other > len || (other == len && i < b));
         }
-        if (threadIdx.x == 0) p.head[kHeadWords + batch + 1 + place] = b;
-        if (threadIdx.x == 0 && place == 0 && p.most_parts) {   // (the longest)
-            const int blocks = (max(len, 1) + 127) / 128, parts = parts_of_chunk(p.tiles, blocks, p.sms, p.d, p.most_parts);
-            p.head[1] = parts;
-            p.head[2] = (blocks + parts - 1) / parts * 128;
+        if (threadIdx.x == 0) p.head.order(batch)[place] = b;
+        if (threadIdx.x == 0 && place == 0 && p.head.most_parts) {   // (the longest)
+            const int blocks = (max(len, 1) + 127) / 128, parts = parts_of_chunk(p.head.tiles, blocks, p.head.sms, p.head.d, p.head.most_parts);
+            p.head.words[1] = parts;
+            p.head.words[2] = (blocks + parts - 1) / parts * 128;
         }
     }
     // For the forward's sake no row behind a length is written, but one of a sequence without keys, which counts as one there.
-    const int rows = p.head ? min(max(len, 1), p.rows) : p.rows;
+    const int rows = p.head.words ? min(max(len, 1), p.rows) : p.rows;
     if (blockIdx.x * (kReadRows * kTokens) >= rows) return;
     const unsigned char *kp[kReadRows], *vp[kReadRows];
     int token[kReadRows];
@@ -349,15 +353,11 @@ int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, c
 
 }  // namespace
 
-int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, int tiles, int most_parts, int sms, cudaStream_t stream) {
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], const ChunkHead& head, cudaStream_t stream) {
     ReadParams p = {};
     p.c = c;
     p.rows = rows;
     p.head = head;
-    p.tiles = tiles;
-    p.most_parts = most_parts;
-    p.sms = sms;
-    p.d = d;
     p.k = static_cast<__nv_bfloat16*>(k);
     p.v = static_cast<__nv_bfloat16*>(v);
     for (int i = 0; i < 3; ++i) p.ks[i] = p.vs[i] = strides[i];

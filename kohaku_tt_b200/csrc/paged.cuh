@@ -71,8 +71,25 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int64_t
 }
 
 // What the chunk path needs behind its dense rows (int32 words): a work counter and, from word 1, the parts that tiles are cut
-// into and the keys of a part; from kHeadWords the offsets of the dense rows, then the sequences by falling length.
+// into and the keys of a part; from kHeadWords the offsets of the dense rows (batch + 1), the sequences by falling length (batch),
+// and for packed queries their offsets (batch + 1), none of them outside of the rows there are.
 constexpr int kHeadWords = 64;
+__host__ __device__ constexpr int64_t head_words(int64_t batch) { return kHeadWords + 3 * batch + 2; }
+struct ChunkHead {
+    int32_t* words;         // null: no chunk
+    const int32_t* cu_q;    // packed queries: their offsets as they were given
+    int64_t total_q;
+    int tiles, most_parts, sms, d;   // what parts_of_chunk goes by; most_parts 0: no parts
+    __host__ __device__ int32_t* offsets() const { return words + kHeadWords; }
+    __host__ __device__ int32_t* order(int batch) const { return offsets() + batch + 1; }
+    __host__ __device__ int32_t* query_offsets(int batch) const { return order(batch) + batch; }
+};
+
+// An offset of packed rows, given on the device and not checked there: inside of the `total` rows there are.
+__device__ __forceinline__ int row_offset(const int32_t* cu, int b, int64_t total) {
+    const int64_t x = cu[b];
+    return static_cast<int>(x < 0 ? 0 : (x > total ? total : x));
+}
 
 // Parts (1 to `most`) that the keys of a chunk's tiles are cut into: `tiles` of 128 rows over up to `blocks` blocks of 128 keys,
 // on `sms` SMs that take an item each. In tenths of a microsecond: a block, an item's start and end, and what adding up the parts

@@ -30,9 +30,9 @@
 
 namespace ktt {
 
-// paged.cu: dense rows of the cache for a chunk of a prompt; 64 words of `head` are cleared, behind them go the offsets 0, rows,
-// 2 rows, ... (batch + 1), and the sequences by falling length.
-int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], int32_t* head, int tiles, int most_parts, int sms, cudaStream_t stream);
+// paged.cu: dense rows of the cache for a chunk of a prompt, and what the forward over them goes by (ChunkHead; its first words are
+// cleared, the offsets of the dense rows are 0, rows, 2 rows, ...).
+int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], const ChunkHead& head, cudaStream_t stream);
 
 namespace {
 
@@ -139,11 +139,9 @@ __device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& f
         first = 0;
         return p.sq;
     }
-    int64_t lo = p.cu[b], hi = p.cu[b + 1];
-    lo = lo < 0 ? 0 : (lo > p.total_q ? p.total_q : lo);
-    hi = hi < lo ? lo : (hi > p.total_q ? p.total_q : hi);
+    const int lo = row_offset(p.cu, b, p.total_q), hi = row_offset(p.cu, b + 1, p.total_q);
     first = lo;
-    return static_cast<int>(hi - lo);
+    return max(hi - lo, 0);
 }
 
 // One normalised chunk of 4 columns of (pair, row of its tile).
@@ -970,7 +968,7 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     most = (1ll << 30) / one;
     s.slice = static_cast<int>(most < 1 ? 1 : (most < a->batch ? most : a->batch));
     if (s.slice > kMaxBatch) s.slice = kMaxBatch;
-    s.parts_at = s.slice * one + ((kHeadWords + 2 * kMaxBatch + 1) * 4 + 255) / 256 * 256;
+    s.parts_at = s.slice * one + (head_words(kMaxBatch) * 4 + 255) / 256 * 256;
     s.bytes = s.parts_at;
     const bool packed = a->cu_seqlens_q != nullptr;
     int64_t tiles = s.slice * static_cast<int64_t>((a->sq + 127) / 128);
@@ -1117,7 +1115,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
     const int64_t cap = p.c.cap, half = slice * cap * hk * d;
     __nv_bfloat16* k = static_cast<__nv_bfloat16*>(a->workspace);
     __nv_bfloat16* v = k + half;
-    int32_t* head = reinterpret_cast<int32_t*>(v + half);   // the forward's work counter, the offsets of the dense rows, the order
+    int32_t* words = reinterpret_cast<int32_t*>(v + half);
     for (int b0 = 0; b0 < a->batch; b0 += slice) {
         const int n = a->batch - b0 < slice ? a->batch - b0 : slice;
         Pages c = p.c;
@@ -1141,7 +1139,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
         // bytes and its own order.) 4 sequences of up to 512 tokens and 8,192 keys, 16 heads over 4, D 128, dealt in the order of the
         // batch, drawn in it, and drawn by length: 121, 122 and 111 us.
         const bool several = n > 1;
-        f.workspace = d == 64 || several ? head : nullptr;
+        f.workspace = d == 64 || several ? words : nullptr;
         f.workspace_bytes = d == 64 ? 256 : several ? 16 : 0;
         // All rows of a head together, sequence after sequence: a dense call's keys, and a packed one's.
         const int64_t strides[3] = {cap * d, slice * cap * d, d};
@@ -1152,33 +1150,35 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
         }
         f.key_lengths = c.lengths;   // (a length of 0 counts as 1 there: a row of zeros)
         f.causal = a->causal ? KTT_B200_CAUSAL_KEY_END : KTT_B200_CAUSAL_NONE;
+        ChunkHead head = {words, nullptr, a->total_q, plan.tiles, plan.parts, sm_count(current_device()), d};
         if (a->cu_seqlens_q) {
             f.total_q = a->total_q;
             f.total_k = slice * cap;
-            f.cu_seqlens_q = a->cu_seqlens_q + b0;
-            f.cu_seqlens_k = head + kHeadWords;
+            head.cu_q = a->cu_seqlens_q + b0;
+            f.cu_seqlens_q = head.query_offsets(n);   // (the forward writes what they say)
+            f.cu_seqlens_k = head.offsets();
             f.q_strides[0] = f.out_strides[0] = f.k_strides[0] = f.v_strides[0] = 0;
         } else {
             f.q = p.q + b0 * a->q_strides[0];
             f.out = p.out + b0 * a->out_strides[0];
         }
-        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, plan.tiles, plan.parts, sm_count(current_device()), stream)) return rc;
+        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, stream)) return rc;
         ForwardParts x = {};
         bool parts = plan.parts > 0;
         if (parts) {
             f.kernel = KTT_B200_KERNEL_TC5_WIDE;
             parts = ktt_b200_sdpa_supported(&f) != 0;   // (else its copies cannot address the operands)
             if (!parts) f.kernel = KTT_B200_KERNEL_AUTO;
-            f.workspace = parts ? head : nullptr;
+            f.workspace = parts ? words : nullptr;
             f.workspace_bytes = parts ? 4 : 0;
         }
-        if (parts || (d == 128 && several)) x.order = head + kHeadWords + n + 1;
+        if (parts || (d == 128 && several)) x.order = head.order(n);
         MergeParams m = {};
         if (parts) {
             m.c = c;
             m.cu = f.cu_seqlens_q;
             m.rows = part_rows(a, n);
-            x.parts = m.parts = head + 1;
+            x.parts = m.parts = words + 1;
             x.most_parts = plan.parts;
             m.o = x.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + plan.parts_at);
             m.lse = x.part_lse = x.part_o + plan.parts * m.rows * a->heads * d;
