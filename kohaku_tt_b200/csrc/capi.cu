@@ -101,6 +101,7 @@ void to_params(const ktt_b200_attn_args* a, AttnParams& p) {
     p.mask_dtype = a->mask_dtype;
     for (int i = 0; i < 4; ++i) p.ms[i] = a->mask_strides[i];
     p.key_lengths = a->key_lengths;
+    p.least_keys = 1;
     p.cu_q = a->cu_seqlens_q;
     p.cu_k = a->cu_seqlens_k;
     p.dout = static_cast<const __nv_bfloat16*>(a->dout);
@@ -321,6 +322,7 @@ int ktt::forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cu
     }
     AttnParams p;
     to_params(a, p);
+    p.least_keys = x.empty ? 0 : 1;
     p.order = x.order;
     p.parts = x.parts;
     p.most_parts = x.most_parts;

@@ -42,6 +42,7 @@ struct AttnParams {
     int most_parts;
     float* part_o;
     float* part_lse;
+    int least_keys;   // what a smaller key length counts as: 1, or 0 where a sequence may have no key
     // backward
     const __nv_bfloat16* dout;
     __nv_bfloat16* dq;
@@ -86,7 +87,7 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnParams& p, int b) {
     s.klen = s.lk;
     if (p.key_lengths) {
         int l = p.key_lengths[b];
-        l = l < 1 ? 1 : l;
+        l = l < p.least_keys ? p.least_keys : l;
         s.klen = l > s.lk ? s.lk : l;
     }
     s.shift = p.causal == KTT_B200_CAUSAL_BOTTOM_RIGHT ? s.lk - s.lq : p.causal == KTT_B200_CAUSAL_KEY_END ? s.klen - s.lq : 0;
@@ -230,8 +231,9 @@ int ensure_smem(K kernel, int bytes, const char* what) {
     return check_cuda(raise_smem_limit(kernel, bytes), what);
 }
 
-// ktt_b200_sdpa_forward, with AttnParams' order and parts.
+// ktt_b200_sdpa_forward, with AttnParams' order and parts; `empty`: sequences of key length 0 have no key.
 struct ForwardParts {
+    bool empty;
     const int32_t* order;
     const int32_t* parts;
     int most_parts;

@@ -175,7 +175,7 @@ __device__ __forceinline__ Work decode_work(const Tc5Params& tp, int w, int span
     k.valid = k.q0 < k.si.lq;
     if (kSplit) {
         const int start = part * span;
-        k.valid = k.valid && start < k.si.klen;
+        k.valid = k.valid && (start < k.si.klen || part == 0);   // (without a key: one part, of zeros)
         k.part = k.si.klen > span ? part : -1;
         k.si.k_off += start;
         k.si.klen = min(k.si.klen - start, span);

@@ -251,8 +251,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
             p.head.words[2] = (blocks + parts - 1) / parts * 128;
         }
     }
-    // For the forward's sake no row behind a length is written, but one of a sequence without keys, which counts as one there.
-    const int rows = p.head.words ? min(max(len, 1), p.rows) : p.rows;
+    const int rows = p.head.words ? min(len, p.rows) : p.rows;   // (what lies behind a length is nothing to the forward)
     if (blockIdx.x * (kReadRows * kTokens) >= rows) return;
     const unsigned char *kp[kReadRows], *vp[kReadRows];
     int token[kReadRows];

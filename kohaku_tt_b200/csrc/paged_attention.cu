@@ -1148,7 +1148,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
             f.out_strides[i] = a->out_strides[i];
             f.k_strides[i] = f.v_strides[i] = strides[i];
         }
-        f.key_lengths = c.lengths;   // (a length of 0 counts as 1 there: a row of zeros)
+        f.key_lengths = c.lengths;
         f.causal = a->causal ? KTT_B200_CAUSAL_KEY_END : KTT_B200_CAUSAL_NONE;
         ChunkHead head = {words, nullptr, a->total_q, plan.tiles, plan.parts, sm_count(current_device()), d};
         if (a->cu_seqlens_q) {
@@ -1164,6 +1164,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
         }
         if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, stream)) return rc;
         ForwardParts x = {};
+        x.empty = true;
         bool parts = plan.parts > 0;
         if (parts) {
             f.kernel = KTT_B200_KERNEL_TC5_WIDE;
