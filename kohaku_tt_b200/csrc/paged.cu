@@ -234,8 +234,8 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
             p.head.offsets()[b] = b * p.rows;
             if (last) p.head.offsets()[batch] = batch * p.rows;
             if (p.head.cu_q) {
-                p.head.query_offsets(batch)[b] = row_offset(p.head.cu_q, b, p.head.total_q);
-                if (last) p.head.query_offsets(batch)[batch] = row_offset(p.head.cu_q, batch, p.head.total_q);
+                p.head.query_offsets(batch)[b] = static_cast<int32_t>(row_offset(p.head.cu_q, b, p.head.total_q));
+                if (last) p.head.query_offsets(batch)[batch] = static_cast<int32_t>(row_offset(p.head.cu_q, batch, p.head.total_q));
             }
         }
         if (b == 0 && threadIdx.x < kHeadWords && (threadIdx.x == 0 || threadIdx.x > 2 || !p.head.most_parts)) p.head.words[threadIdx.x] = 0;

@@ -86,9 +86,9 @@ struct ChunkHead {
 };
 
 // An offset of packed rows, given on the device and not checked there: inside of the `total` rows there are.
-__device__ __forceinline__ int row_offset(const int32_t* cu, int b, int64_t total) {
+__device__ __forceinline__ int64_t row_offset(const int32_t* cu, int b, int64_t total) {
     const int64_t x = cu[b];
-    return static_cast<int>(x < 0 ? 0 : (x > total ? total : x));
+    return x < 0 ? 0 : (x > total ? total : x);
 }
 
 // Parts (1 to `most`) that the keys of a chunk's tiles are cut into: `tiles` of 128 rows over up to `blocks` blocks of 128 keys,

@@ -139,9 +139,9 @@ __device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& f
         first = 0;
         return p.sq;
     }
-    const int lo = row_offset(p.cu, b, p.total_q), hi = row_offset(p.cu, b + 1, p.total_q);
-    first = lo;
-    return max(hi - lo, 0);
+    const int64_t hi = row_offset(p.cu, b + 1, p.total_q);
+    first = row_offset(p.cu, b, p.total_q);
+    return static_cast<int>(hi < first ? 0 : hi - first);
 }
 
 // One normalised chunk of 4 columns of (pair, row of its tile).
