@@ -1,6 +1,7 @@
 // The paged cache: appending rows (with the rotation of the keys and of the step's queries) and reading it back.
-#include "paged.cuh"
+#include <type_traits>
 
+#include "paged.cuh"
 #include "rotary.cuh"
 
 namespace ktt {
@@ -69,20 +70,25 @@ __device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, uns
     const __nv_bfloat16 step = __float2bfloat16_rn(__fmul_rn(__fsub_rn(-__high2float(ends), least), 1.f / 15.f));
     const float s = __bfloat162float(step);
     uint32_t word = 0;
-    if (s > 0.f && s < INFINITY) {   // (else all codes are 0)
+    auto encode = [&](auto coarse) {
         const float even = s < 0x1p-60f ? 0x1p100f : (s > 0x1p60f ? 0x1p-100f : 1.f), r = s * even, inv = __frcp_rn(r);
         const Pair least2(least), even2(even), inv2(inv), r2(-r), whole2(8388608.f);
         Pair codes(0.f);
 #pragma unroll
         for (int n = 3; n >= 0; --n) {
             const Pair d = sub(Pair(to_f32(x.get(2 * n)), to_f32(x.get(2 * n + 1))), least2) * even2, q = d * inv2;
-            const Pair t = fma(fma(q, r2, d), inv2, q);
-            // To the nearest whole number, ties to even (t is at most 15 (1 + 2^-8)); four of them make one of 16 bits.
+            Pair t = fma(fma(q, r2, d), inv2, q);
+            if constexpr (decltype(coarse)::value) t = Pair(fminf(t.low(), 15.f), fminf(t.high(), 15.f));
+            // To the nearest whole number, ties to even; four of them make one of 16 bits.
             codes = fma(codes, Pair(16.f), sub(t + whole2, whole2));
         }
         codes = codes + whole2;
         word = __byte_perm(__float_as_uint(codes.low()), __float_as_uint(codes.high()), 0x5410);
-    }
+    };
+    // t is at most 15 (1 + 2^-8), by half of a bf16 step's rounding; a subnormal step, which is rounded by up to half of 2^-133, can leave
+    // values as far as 22 steps from the least, whose code is 15. (Else all codes are 0.)
+    if (s >= 0x1p-126f && s < INFINITY) encode(std::false_type());
+    else if (s > 0.f && s < INFINITY) encode(std::true_type());
     if (!there) return;
     uint32_t* to = reinterpret_cast<uint32_t*>(block);
     to[value ? value_word<D>(token, chunk) : key_word<D>(token, chunk)] = word;
