@@ -328,6 +328,8 @@ int ktt::forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cu
     p.most_parts = x.most_parts;
     p.part_o = x.part_o;
     p.part_lse = x.part_lse;
+    p.part_rows = x.part_rows;
+    p.part_stride = x.part_stride;
     cudaStream_t st = stream;
     const char* why = nullptr;
     const bool tc5 = forward_tc5_takes(p, &why);

@@ -35,13 +35,16 @@ struct AttnParams {
     const int32_t* cu_k;
     // Forward (fwd_tc5.cu, with a work counter; null without). order: batch entries by falling length, the order in which their
     // tiles are drawn. parts, on the device: (n, span): tiles are cut along the keys into up to n <= most_parts parts of `span` keys
-    // (whole blocks); a part of a sequence of more than one leaves its normalised rows in part_o [parts][rows][heads][d] and
-    // their base-2 lse in part_lse [parts][rows][heads], rows = total_q or batch * sq, for the caller to merge.
+    // (whole blocks); a part of a sequence of more than one leaves its normalised rows in part_o [parts][part_rows][heads][d] and
+    // their base-2 lse in part_lse [parts][part_rows][heads], for the caller to merge. Row i of sequence b has place
+    // b * part_stride + i there, or that of the packed row where part_stride is 0; rows past sq have none.
     const int32_t* order;
     const int32_t* parts;
     int most_parts;
     float* part_o;
     float* part_lse;
+    int64_t part_rows;
+    int part_stride;
     int least_keys;   // what a smaller key length counts as: 1, or 0 where a sequence may have no key
     // backward
     const __nv_bfloat16* dout;
@@ -239,6 +242,8 @@ struct ForwardParts {
     int most_parts;
     float* part_o;
     float* part_lse;
+    int64_t part_rows;
+    int part_stride;
 };
 int forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cudaStream_t stream);
 // Launchers (one per kernel family).

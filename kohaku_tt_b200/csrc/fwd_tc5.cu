@@ -520,13 +520,13 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             if (!k.valid) continue;
             const SeqInfo& si = k.si;
             const int qi = k.q0 + row;                  // row inside the sequence
-            const bool real = qi < si.lq;
             // kSplit: the row's place among the parts (AttnParams), -1 where the sequence has only one.
             int64_t place = -1;
             if (kSplit && k.part >= 0) {
-                const int64_t rows = p.cu_q ? p.total_q : static_cast<int64_t>(p.batch) * p.sq;
-                place = ((k.part * rows) + (p.cu_q ? 0 : static_cast<int64_t>(k.b) * p.sq) + si.q_off + qi) * p.heads + k.h;
+                const int64_t at = (p.part_stride ? static_cast<int64_t>(k.b) * p.part_stride : si.q_off) + qi;
+                place = (k.part * p.part_rows + at) * p.heads + k.h;
             }
+            const bool real = qi < (kSplit ? min(si.lq, p.sq) : si.lq);
             __nv_bfloat16* og = p.out + k.b * p.os[0] + k.h * p.os[1] + static_cast<int64_t>(si.q_off + qi) * p.os[2] + g * (D / G);
             if (k.nblocks == 0) {
                 // No key is visible to this tile: zeros, lse = -inf. No barrier is involved.
@@ -1099,7 +1099,7 @@ int launch_tc5(const AttnParams& p, cudaStream_t stream) {
                          : (tp.trace ? fwd_tc5_kernel<D, true, false> : fwd_tc5_kernel<D, false, false>);
     const bool split = p.parts != nullptr;
     if (split) {
-        if (masked || !p.fwd_work_counter || p.most_parts < 1 || !p.part_o || !p.part_lse) return fail(KTT_B200_ERR_BAD_ARGUMENT, "tcgen05 forward: parts without their places");
+        if (masked || !p.fwd_work_counter || p.most_parts < 1 || !p.part_o || !p.part_lse || p.part_rows < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "tcgen05 forward: parts without their places");
         kernel = fwd_tc5_kernel<D, false, false, true>;
     }
     if (int rc = ensure_smem(kernel, smem, "cudaFuncSetAttribute(fwd_tc5)")) return rc;

@@ -946,8 +946,12 @@ constexpr int kMostParts = 16;
 
 int64_t rows_per_head(const ktt_b200_paged_sdpa_args* a) { return static_cast<int64_t>(a->heads / a->cache.kv_heads) * a->sq; }
 
-// Rows of a launch over `batch` sequences that parts have a place for.
-int64_t part_rows(const ktt_b200_paged_sdpa_args* a, int batch) { return a->cu_seqlens_q ? a->total_q : static_cast<int64_t>(batch) * a->sq; }
+// Rows that parts have a place for in a launch over `batch` sequences: sq for each, or the packed rows where those are fewer (the
+// launches of a call share them, and a padded buffer has more than its sequences). Parts are at most two tiles' worth for every SM.
+int64_t part_rows(const ktt_b200_paged_sdpa_args* a, int batch) {
+    const int64_t rows = static_cast<int64_t>(batch) * a->sq;
+    return a->cu_seqlens_q && a->total_q < rows ? a->total_q : rows;
+}
 
 Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     Plan s = {};
@@ -1033,7 +1037,8 @@ struct MergeParams {
     const float* lse;    // [parts][rows][heads]
     const int32_t* cu;   // packed
     const int32_t* parts;   // (parts, keys of a part)
-    int64_t rows;
+    int64_t rows;        // that parts have a place for
+    int stride;          // places of a sequence; 0: those of the packed rows
     int batch, heads, sq;
     __nv_bfloat16* out;
     int64_t os[3];
@@ -1042,11 +1047,18 @@ template <int D>
 __global__ void __launch_bounds__(256) merge_parts_kernel(const __grid_constant__ MergeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y, row = n / p.heads;
-    if (row >= p.rows) return;
-    const int h = static_cast<int>(n - row * p.heads), c4 = threadIdx.x;
-    const int b = p.cu ? sequence_of(p.cu, p.batch, row) : static_cast<int>(row / p.sq);
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y, place = n / p.heads;
+    if (place >= p.rows) return;
+    const int h = static_cast<int>(n - place * p.heads), c4 = threadIdx.x;
+    const int b = p.stride ? static_cast<int>(place / p.stride) : sequence_of(p.cu, p.batch, place);
     if (b < 0) return;
+    int64_t row = place - static_cast<int64_t>(b) * p.stride;   // in the sequence, then of the operands
+    if (p.cu) {
+        const int64_t first = p.cu[b], n_rows = p.cu[b + 1] - first;
+        if (!p.stride) row -= first;
+        if (row >= n_rows || row >= p.sq) return;
+        row += first;
+    }
     const int span = p.parts[1], parts = (cached_keys(p.c, b) + span - 1) / span;
     if (parts <= 1) return;
     const int64_t step = p.rows * p.heads;
@@ -1087,8 +1099,7 @@ __global__ void __launch_bounds__(256) merge_parts_kernel(const __grid_constant_
         }
     }
     const float inv = sum > 0.f ? 1.f / sum : (sum == 0.f ? 0.f : sum);   // (a NaN stays one)
-    const int64_t r = p.cu ? row : row - static_cast<int64_t>(b) * p.sq;
-    __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + h * p.os[1] + r * p.os[2] + 4 * c4;
+    __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + h * p.os[1] + row * p.os[2] + 4 * c4;
     *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
@@ -1178,7 +1189,8 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
         if (parts) {
             m.c = c;
             m.cu = f.cu_seqlens_q;
-            m.rows = part_rows(a, n);
+            x.part_rows = m.rows = part_rows(a, n);
+            x.part_stride = m.stride = m.cu && m.rows == a->total_q ? 0 : a->sq;
             x.parts = m.parts = words + 1;
             x.most_parts = plan.parts;
             m.o = x.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + plan.parts_at);
