@@ -27,7 +27,7 @@ struct TableParams {
     float* sin;
     int64_t positions;
     int pairs;
-    float scale;
+    float scale, scale_rest;   // as fp32, and what that leaves
     int vec;                   // both tables start at 16 bytes
     uint64_t turns[kMaxPairs];   // f_i / 2 pi in 2^-64 turns
 };
@@ -42,9 +42,9 @@ __device__ __forceinline__ Two two_of(float hi, float lo) {
     const float s = hi + lo;
     return {s, lo - (s - hi)};
 }
-__device__ __forceinline__ Two times(const Two& x, float y) {
-    const float h = x.hi * y;
-    return {h, fmaf(x.hi, y, -h) + x.lo * y};
+__device__ __forceinline__ Two times(const Two& x, const Two& y) {
+    const float h = x.hi * y.hi;
+    return {h, fmaf(x.hi, y.hi, -h) + fmaf(x.lo, y.hi, x.hi * y.lo)};
 }
 
 // Cosine and sine of an angle of `turn` 2^-64 turns.
@@ -112,8 +112,9 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
         Two c, s;
         cos_sin(pos * turns[i], c, s);
         if (row < kSteps) {
-            c = times(c, p.scale);
-            s = times(s, p.scale);
+            const Two scale = {p.scale, p.scale_rest};
+            c = times(c, scale);
+            s = times(s, scale);
         }
         sm.ch[row][i] = c.hi;
         sm.cl[row][i] = c.lo;
@@ -280,12 +281,14 @@ extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, 
     if (!cos || !sin || !frequencies) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: null pointer");
     if (positions < 1 || pairs < 1 || pairs > kMaxPairs) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: 1 or more positions and 1 to %d pairs", kMaxPairs);
     if (positions > (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary_table: at most 2^31 positions");
+    if (!std::isfinite(static_cast<float>(scale))) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: the scale must be finite");
     TableParams p = {};
     p.cos = cos;
     p.sin = sin;
     p.positions = positions;
     p.pairs = pairs;
     p.scale = static_cast<float>(scale);
+    p.scale_rest = static_cast<float>(scale - p.scale);
     for (int i = 0; i < pairs; ++i) {
         if (!std::isfinite(frequencies[i])) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary_table: frequencies must be finite");
         const long double turns = frequencies[i] * 0.159154943091895335768883763372514362L;   // f / 2 pi
