@@ -1069,10 +1069,10 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// rotary_table(positions, dim, base, scaling, factor, original, fast, slow, device index): (cos, sin).
+// rotary_table(positions, dim, base, scaling, factor, original, fast, slow, device index): (cos, sin), or None.
 PyObject* py_rotary_table(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    if (n != 9) Py_RETURN_NONE;
+    if (n != 9 || !callable_now()) Py_RETURN_NONE;
     const int64_t positions = PyLong_AsLongLong(args[0]), dim = PyLong_AsLongLong(args[1]), scaling = PyLong_AsLongLong(args[3]), index = PyLong_AsLongLong(args[8]);
     const double base = PyFloat_AsDouble(args[2]), factor = PyFloat_AsDouble(args[4]), original = PyFloat_AsDouble(args[5]), fast = PyFloat_AsDouble(args[6]),
                  slow = PyFloat_AsDouble(args[7]);

@@ -42,14 +42,21 @@ def rotary_table(positions, dim, base=10000.0, scaling=None, factor=1.0, origina
     device = torch.device(device)
     if device.type != "cuda":
         raise RuntimeError("kohaku_tt_b200: rotary tables are made on CUDA devices only; there is no CPU fallback")
+    scalars = (base, _scaling(scaling), factor, 0.0 if original is None else original, fast, slow)
     eager = not torch.compiler.is_compiling() and _lib.native()
     if eager:
         index = torch.cuda.current_device() if device.index is None else device.index
-        out = eager.rotary_table(positions, dim, base, _scaling(scaling), factor, 0.0 if original is None else original, fast, slow, index)
+        out = eager.rotary_table(positions, dim, *scalars, index)
         if out is not None:
             return out
-    f, scale = rotary_frequencies(dim, base, scaling, factor, original, fast, slow)
-    positions = int(positions)
+    return torch.ops.ktt_b200._rotary_table(int(positions), int(dim), *scalars, device)
+
+
+@torch.library.custom_op("ktt_b200::_rotary_table", mutates_args=(), device_types="cuda")
+def _table_op(positions: int, dim: int, base: float, scaling: int, factor: float, original: float, fast: float, slow: float,
+              device: torch.device) -> tuple[torch.Tensor, torch.Tensor]:
+    """The tables as an operator, for compiled graphs and for modes that watch operators."""
+    f, scale = rotary_frequencies(dim, base, SCALINGS[scaling], factor, original, fast, slow)
     if positions < 1:
         raise ValueError("kohaku_tt_b200.rotary_table: one position at least")
     pairs = len(f)
@@ -60,6 +67,12 @@ def rotary_table(positions, dim, base=10000.0, scaling=None, factor=1.0, origina
         _lib.check(_lib.lib().ktt_b200_rotary_table(cos.data_ptr(), sin.data_ptr(), positions, pairs, host, scale,
                                                     ops._stream(cos.device)), "rotary_table")
     return cos, sin
+
+
+@_table_op.register_fake
+def _(positions, dim, base, scaling, factor, original, fast, slow, device):
+    shape = (positions, dim // 2)
+    return torch.empty(shape, dtype=torch.float32, device=device), torch.empty(shape, dtype=torch.float32, device=device)
 
 
 def check_tables(cos, sin, like, dim, what):

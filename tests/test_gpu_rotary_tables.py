@@ -1,4 +1,4 @@
-"""What scaled tables are off by."""
+"""What scaled tables are off by, and tables made inside of compiled and traced code."""
 
 import pytest
 import torch
@@ -24,3 +24,52 @@ def test_the_scale_is_not_rounded_before_the_entries_are(cuda, positions, factor
     want = torch.stack(po.table(positions, f, scale))
     off = torch.stack([cos, sin]).double().cpu() - want
     assert abs((off * want).sum() / (want * want).sum()) <= 2.0 ** -27.5
+
+
+def test_compiled(cuda):
+    x = torch.randn((1, 2, 16, 64), device=cuda).bfloat16()
+    how = dict(base=1e6, scaling="parts", factor=4.0, original=8)
+
+    def turned(x):
+        cos, sin = ktt.rotary_table(16, 64, device=x.device, **how)
+        return ktt.rotary(x, None, cos, sin)[0], cos, sin
+
+    want = turned(x)
+    for a, b in zip(torch.compile(turned, fullgraph=True)(x), want):
+        assert torch.equal(a, b)
+
+
+def test_fake_tables_are_fake(cuda):
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    for device in ("cuda", cuda):
+        with FakeTensorMode():
+            cos, sin = ktt.rotary_table(16, 64, device=device)
+        for t in (cos, sin):
+            assert isinstance(t, FakeTensor) and t.shape == (16, 32) and t.dtype == torch.float32 and t.device == cuda
+
+
+def test_modes_that_watch_calls(cuda):
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Functions(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    seen = []
+
+    class Operators(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    want = ktt.rotary_table(16, 64, device=cuda)
+    for mode in (Functions(), Operators()):
+        with mode:
+            got = ktt.rotary_table(16, 64, device=cuda)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert any("_rotary_table" in name for name in seen)
+    for bad in (dict(positions=0, dim=64), dict(positions=4, dim=63), dict(positions=4, dim=514), dict(positions=4, dim=64, scaling="parts", factor=2.0)):
+        with Operators(), pytest.raises(ValueError):
+            ktt.rotary_table(**bad)
