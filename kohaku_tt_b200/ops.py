@@ -62,6 +62,12 @@ def _rows_contiguous(t):
     return t if t.stride(-1) == 1 else t.contiguous()
 
 
+def _empty_like_rows(t):
+    """An output for `t`: laid out like it where its innermost stride is one, else contiguous."""
+    out = torch.empty_like(_rows_contiguous(t))
+    return out if out.stride(-1) == 1 or out.numel() == 0 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _bhs_strides(t):
     """(batch, head, row) element strides of a [B, H, S, D] tensor."""
     return (t.stride(0), t.stride(1), t.stride(2))

@@ -115,9 +115,7 @@ def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleav
             if q.dim() != k.dim() or q.shape[1] < 1:
                 raise ValueError("kohaku_tt_b200.paged_append: q must be laid out like k, with its own heads")
             q = _operand(q, "q", q.shape[1], k_pages, batch, rows, dim, packed, what)
-            q_out = torch.empty_like(q)
-            if q_out.stride(-1) != 1:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            q_out = ops._empty_like_rows(q)
             a.heads, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
             ops._set3(a.q_strides, strides(q))
             ops._set3(a.q_out_strides, strides(q_out))
@@ -147,6 +145,11 @@ def _read(k_pages, v_pages, block_table, lengths, max_k):
     return k, v
 
 
+def _attention_out(q, packed):
+    """The output of sdpa_paged, by the queries that the caller gave (whose place in memory a graph does not know)."""
+    return q.new_empty(q.shape) if packed else ops._out_like_query(ops._rows_contiguous(q), q.shape[-1])
+
+
 def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k):
     what = "sdpa_paged"
     ops._require_cuda(q)
@@ -157,6 +160,7 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
         raise ValueError("kohaku_tt_b200.sdpa_paged: q must be [B, H, Sq, D], or packed [T, H, D] with cu_seq_q")
     rows = q.shape[0] if packed else q.shape[2]
     q = _operand(q, "q", q.shape[1], k_pages, batch, rows, dim, packed, what)
+    out = _attention_out(q, packed)
     if q.data_ptr() % 16 or any(x % 8 for x in q.stride()[:-1]):
         q = q.clone(memory_format=torch.contiguous_format)   # (rows that the kernels cannot read in place)
     strides = ops._ths_strides if packed else ops._bhs_strides
@@ -169,7 +173,6 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
             if max_q < 0 or (longest is not None and max_q < longest):
                 raise ValueError("kohaku_tt_b200.sdpa_paged: max_q is less than the longest sequence")
             max_q = min(max_q, rows)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if packed else ops._out_like_query(q, dim)
         a.batch, a.heads, a.sq, a.d = batch, q.shape[1], max_q if packed else rows, dim
         a.causal, a.scale = int(causal), float(scale) if scale is not None else 1.0 / math.sqrt(dim)
         a.q, a.out = q.data_ptr(), out.data_ptr()
@@ -196,7 +199,7 @@ def _append_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages:
 
 @_append_op.register_fake
 def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out):
-    return k.new_empty((0,)) if q is None else torch.empty_like(q)
+    return k.new_empty((0,)) if q is None else ops._empty_like_rows(q)
 
 
 @torch.library.custom_op("ktt_b200::_paged_read", mutates_args=(), device_types="cuda")
@@ -220,7 +223,7 @@ def _sdpa_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, bloc
 
 @_sdpa_op.register_fake
 def _(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k):
-    return q.new_empty(q.shape) if cu_seq_q is not None else ops._out_like_query(q, q.shape[3])
+    return _attention_out(q, cu_seq_q is not None)
 
 
 # ---- the entry points ------------------------------------------------------------------------

@@ -94,11 +94,6 @@ def dense_tables(cos, sin):
     return cos, sin
 
 
-def _like(x):
-    out = torch.empty_like(x)
-    return out if out.stride(-1) == 1 or out.numel() == 0 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
 def _check(q, k, cos, sin, positions):
     what = "rotary"
     for x in (q, k):
@@ -134,7 +129,7 @@ def _run(q, k, cos, sin, positions, interleaved, inverse):
     cos, sin = dense_tables(cos, sin)
     strides = ops._ths_strides if q.dim() == 3 else ops._bhs_strides
     with torch.cuda.device(q.device):
-        q_out, k_out = _like(q), None if k is None else _like(k)
+        q_out, k_out = ops._empty_like_rows(q), None if k is None else ops._empty_like_rows(k)
         if q.numel() == 0 and (k is None or k.numel() == 0):
             return q_out, k_out
         a = _lib.RotaryArgs()
@@ -191,7 +186,7 @@ def _rotary_op(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: 
 
 @_rotary_op.register_fake
 def _(q, k, cos, sin, positions, interleaved, inverse):
-    return [_like(q)] if k is None else [_like(q), _like(k)]
+    return [ops._empty_like_rows(x) for x in (q, k) if x is not None]
 
 
 def _setup(ctx, inputs, output):
