@@ -444,7 +444,8 @@ typedef struct ktt_b200_paged_sdpa_args {
     int64_t workspace_bytes;
 } ktt_b200_paged_sdpa_args;
 /* Bytes of workspace of a call of these sizes; -1: refused. Chunks of prompts take dense rows of some sequences' capacity
- * there, 1 GB or one sequence's at most, and 20 MB at most for the parts that their keys may be cut into. */
+ * there, 1 GB or one sequence's at most, 20 MB at most for the parts that their keys may be cut into, and over 4 bits
+ * a copy of the queries (2 D + 4 bytes for each row and head). */
 KTT_B200_API int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args* args);
 KTT_B200_API int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* args, void* stream);
 

@@ -330,6 +330,9 @@ int ktt::forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cu
     p.part_lse = x.part_lse;
     p.part_rows = x.part_rows;
     p.part_stride = x.part_stride;
+    p.q_power = x.q_power;
+    p.kv_powers = x.kv_powers;
+    p.chunks = x.chunks;
     cudaStream_t st = stream;
     const char* why = nullptr;
     const bool tc5 = forward_tc5_takes(p, &why);

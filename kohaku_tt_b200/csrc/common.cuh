@@ -1,6 +1,7 @@
 // Shared device helpers and the kernel-side parameter block.
 #pragma once
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -45,6 +46,12 @@ struct AttnParams {
     float* part_lse;
     int64_t part_rows;
     int part_stride;
+    // Operands in fp16 (fwd_tc5.cu without a mask; null: bf16), none of 2^15 or more: rows of q divided by the power of two
+    // q_power[row][head] (rows: packed, or batch * sq), keys and values 64 c .. of a sequence by 2^k and 2^v, the low and the high half of
+    // kv_powers[kv head][batch][c], of `chunks` for each. Weights are fp16 then too.
+    const float* q_power;
+    const int32_t* kv_powers;
+    int chunks;
     int least_keys;   // what a smaller key length counts as: 1, or 0 where a sequence may have no key
     // backward
     const __nv_bfloat16* dout;
@@ -165,6 +172,14 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<uint32_t*>(&t);
 }
 
+// 2^n, n from -126 to 127.
+__device__ __forceinline__ float power_of_two(int n) { return __int_as_float((127 + n) << 23); }
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    __half2 t = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&t);
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -234,7 +249,7 @@ int ensure_smem(K kernel, int bytes, const char* what) {
     return check_cuda(raise_smem_limit(kernel, bytes), what);
 }
 
-// ktt_b200_sdpa_forward, with AttnParams' order and parts; `empty`: sequences of key length 0 have no key.
+// ktt_b200_sdpa_forward, with AttnParams' order, parts and operands in fp16; `empty`: sequences of key length 0 have no key.
 struct ForwardParts {
     bool empty;
     const int32_t* order;
@@ -244,6 +259,9 @@ struct ForwardParts {
     float* part_lse;
     int64_t part_rows;
     int part_stride;
+    const float* q_power;
+    const int32_t* kv_powers;
+    int chunks;
 };
 int forward_in_parts(const ktt_b200_attn_args* a, const ForwardParts& x, cudaStream_t stream);
 // Launchers (one per kernel family).

@@ -40,6 +40,8 @@ namespace {
 
 constexpr int kTmemCols = 512;    // two S / P buffers, one O accumulator per softmax group
 constexpr float kRescaleGap = 8.f;  // in log2 units
+// fp16 weights are 2^7 times as large: with the gap 2^15 at most, and what is lost below the least of them is under 2^-31 of the largest.
+constexpr float kHalfLift = 7.f;
 
 // ---- shared-memory plan -----------------------------------------------------------------
 
@@ -137,6 +139,7 @@ struct Work {
     SeqInfo si;
     bool valid;  // false: the tile lies past the end of its sequence
     int part;    // kSplit: which part of its keys; -1: all of them
+    int start;   // the first of its keys
 };
 
 // Two orders of the items. Fixed deal (no counter): consecutive items are the heads of one
@@ -173,8 +176,9 @@ __device__ __forceinline__ Work decode_work(const Tc5Params& tp, int w, int span
     k.si = seq_info(p, k.b);
     k.q0 = qb * kBM;
     k.valid = k.q0 < k.si.lq;
+    k.start = 0;
     if (kSplit) {
-        const int start = part * span;
+        const int start = k.start = part * span;
         k.valid = k.valid && (start < k.si.klen || part == 0);   // (without a key: one part, of zeros)
         k.part = k.si.klen > span ? part : -1;
         k.si.k_off += start;
@@ -195,7 +199,11 @@ __device__ __forceinline__ int work_of(int round, int cta, int ctas) {
 
 // ---- the kernel ------------------------------------------------------------------------
 
-template <int D, bool kTrace, bool kMask, bool kSplit = false>
+// kHalf: operands in fp16, each query row and every 64 keys and values (a softmax group's of a block) with a power of two of their own
+// (AttnParams), and P in fp16: an eighth of bf16's rounding. The rows' and the keys' powers are part of a block's logit scale; the values' is
+// part of the exponents, and of what the running maximum is of, so that no product is out of range, and the sum of weights takes
+// it out again where it changes.
+template <int D, bool kTrace, bool kMask, bool kSplit = false, bool kHalf = false>
 __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
     const __grid_constant__ CUtensorMap map_v, const Tc5Params tp) {
@@ -393,8 +401,8 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
         }
     } else if (warp == P::kMmaWarp) {
         // ---------------- MMA issuer (whole warp, converged) ----------------
-        constexpr uint32_t idesc_s = instr_desc(kBN, false);
-        constexpr uint32_t idesc_o = instr_desc(D, true);
+        constexpr uint32_t idesc_s = instr_desc(kBN, false, kHalf);
+        constexpr uint32_t idesc_o = instr_desc(D, true, kHalf);
         // Descriptors differ only in their 14-bit start-address field (bytes / 16):
         // build each base once and add constants per MMA.
         const uint64_t q_desc = smem_desc(sbase + P::kQ, 16, 1024);
@@ -541,7 +549,20 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             }
             const bool tracer = first_item && row == 0 && blockIdx.x == 0;
             float m_ref = -INFINITY;  // this half's reference maximum (base-2 logits), moved lazily
-            float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // running sums, 4 lanes
+            float2 l2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};  // running sums, 4 lanes (kHalf: of blocks with one power)
+            float l_run = 0.f;                                              // kHalf: of the blocks before
+            const int32_t* powers = nullptr;
+            int now = 0, next = 0;
+            float row_scale = p.scale_log2, block_scale = p.scale_log2;     // kHalf: with the row's power, and with the keys'
+            float v_power = 0.f, v_inverse = 1.f;
+            if constexpr (kHalf) {
+                static_assert(!kMask && CG == 64, "a power for each group's keys of a block");
+                powers = p.kv_powers + (static_cast<int64_t>(div_by(k.h, tp.by_group)) * p.batch + k.b) * p.chunks + k.start / CG + g;
+                next = *powers;
+                now = ~next;
+                const int64_t at = (p.cu_q ? 0 : static_cast<int64_t>(k.b) * p.sq) + si.q_off + qi;
+                row_scale *= real ? p.q_power[at * p.heads + k.h] : 0.f;   // (a row of no sequence moves no reference)
+            }
             // Keys this row may see: [0, row_limit).
             int row_limit = si.klen;
             if (p.causal) row_limit = min(row_limit, qi + si.shift + 1);
@@ -549,6 +570,16 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             for (int j = 0; ok && j < k.nblocks; ++j) {
                 const int gb = blk + j;
                 const uint32_t s_addr = tmem + (gb & 1) * 128 + g * CG + lane_addr;
+                if (kHalf && next != now) {   // (seldom: powers are multiples of 4)
+                    l_run = fmaf((l2[0].x + l2[0].y) + (l2[1].x + l2[1].y), v_inverse, l_run);
+                    l2[0] = l2[1] = make_float2(0.f, 0.f);
+                    now = next;
+                    // (Neither 0 nor infinite: a masked column's -inf and a score of 0 stay what they are.)
+                    block_scale = fminf(fmaxf(row_scale * power_of_two(static_cast<int16_t>(now)), 0x1p-126f), 0x1p127f);
+                    v_power = static_cast<float>(now >> 16);
+                    v_inverse = power_of_two(-(now >> 16));
+                }
+                if (kHalf && j + 1 < k.nblocks) next = powers[(j + 1) * G];
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(P::bSFull + (gb & 1)), (gb >> 1) & 1, abort_flag, 300 + g, tp.status));
                 if (!ok) break;
                 tc_fence_after();
@@ -613,7 +644,8 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                         mx4[e & 3] = fmaxf(mx4[e & 3], s[e]);
                     }
                 }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (kMask ? 1.f : p.scale_log2);
+                float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * (kMask ? 1.f : block_scale);
+                if (kHalf) mx += v_power;
                 zone<kTrace>(tp, tracer && g == 0, j, 1);
 
                 // Lazy rescale: move the reference only when this block exceeds it by 2^8.
@@ -625,6 +657,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                         m_ref = mx;
                         l2[0] = __fmul2_rn(l2[0], make_float2(f, f));
                         l2[1] = __fmul2_rn(l2[1], make_float2(f, f));
+                        if (kHalf) l_run *= f;
                     }
                     if (j > 0) {
                         // O of this half holds blocks [0, j): wait for block j - 1's P V.
@@ -659,8 +692,9 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                 // P = 2^(s * scale - m) as packed bf16 pairs, two values per instruction where
                 // the packed fp32 pipe allows.
                 uint32_t wv[CG / 2];
-                const float sc1 = kMask ? 1.f : p.scale_log2;  // masked logits are already scaled
-                const float2 sc2 = make_float2(sc1, sc1), nm2 = make_float2(-m_use, -m_use);
+                const float sc1 = kMask ? 1.f : block_scale;  // masked logits are already scaled
+                const float nm = kHalf ? (kHalfLift + v_power) - m_use : -m_use;
+                const float2 sc2 = make_float2(sc1, sc1), nm2 = make_float2(nm, nm);
                 if (whole) {
                     // Every column visible. kPolyPairs of this thread's pairs take the polynomial
                     // on the FMA pipe, the rest MUFU; odd groups start with the polynomial and
@@ -679,7 +713,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                                 pr.y = fast_exp2(x.y);
                             }
                             l2[e & 1] = __fadd2_rn(l2[e & 1], pr);
-                            wv[e] = pack_bf16(pr.x, pr.y);
+                            wv[e] = kHalf ? pack_f16(pr.x, pr.y) : pack_bf16(pr.x, pr.y);
                         }
                     };
                     if (g & 1) {
@@ -694,7 +728,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                         const float2 x = __ffma2_rn(make_float2(s[2 * e], s[2 * e + 1]), sc2, nm2);
                         const float2 pr = make_float2(fast_exp2(x.x), fast_exp2(x.y));
                         l2[e & 1] = __fadd2_rn(l2[e & 1], pr);
-                        wv[e] = pack_bf16(pr.x, pr.y);
+                        wv[e] = kHalf ? pack_f16(pr.x, pr.y) : pack_bf16(pr.x, pr.y);
                     }
                 }
                 zone<kTrace>(tp, tracer && g == 0, j, 2);
@@ -719,7 +753,7 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
             // passed this item's accumulator hand-over (bOFree), which comes after its reads here.
             zone<kTrace>(tp, tracer && g == 0, 60, 0);
             float2* ml = ml_base;
-            const float l_mine = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
+            const float l_mine = fmaf((l2[0].x + l2[0].y) + (l2[1].x + l2[1].y), v_inverse, l_run);
             ml[g * 128 + row] = make_float2(m_ref, l_mine);
             if (lane == 0) ok_flags[warp] = ok;
             // A bounded wait like every other in this kernel: no warp can be left behind at a
@@ -801,10 +835,10 @@ __global__ void __launch_bounds__(Plan<D>::kThreads, 1) fwd_tc5_kernel(
                 }
                 zone<kTrace>(tp, tracer && g == 0, 60, 3);
                 if (kSplit && place >= 0) {
-                    if (real && g == 0) p.part_lse[place] = l_sum == 0.f ? -INFINITY : m_all + log2f(l_sum);   // (base 2; a NaN stays one)
+                    if (real && g == 0) p.part_lse[place] = l_sum == 0.f ? -INFINITY : m_all - (kHalf ? kHalfLift : 0.f) + log2f(l_sum);   // (base 2; a NaN stays one)
                 } else if (real && g == 0 && p.lse) {
                     p.lse[k.b * p.ls[0] + k.h * p.ls[1] + (si.q_off + qi) * p.ls[2]] =
-                        l_sum > 0.f ? kLn2 * (m_all + log2f(l_sum)) : -INFINITY;
+                        l_sum > 0.f ? kLn2 * (m_all - (kHalf ? kHalfLift : 0.f) + log2f(l_sum)) : -INFINITY;
                 }
             } else {
                 break;
@@ -1101,6 +1135,10 @@ int launch_tc5(const AttnParams& p, cudaStream_t stream) {
     if (split) {
         if (masked || !p.fwd_work_counter || p.most_parts < 1 || !p.part_o || !p.part_lse || p.part_rows < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "tcgen05 forward: parts without their places");
         kernel = fwd_tc5_kernel<D, false, false, true>;
+    }
+    if (p.kv_powers) {
+        if (masked || !p.q_power) return fail(KTT_B200_ERR_BAD_ARGUMENT, "tcgen05 forward: fp16 operands without their powers");
+        kernel = split ? fwd_tc5_kernel<D, false, false, true, true> : fwd_tc5_kernel<D, false, false, false, true>;
     }
     if (int rc = ensure_smem(kernel, smem, "cudaFuncSetAttribute(fwd_tc5)")) return rc;
     tp.q_tiles = (p.sq + kBM - 1) / kBM;

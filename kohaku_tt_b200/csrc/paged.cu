@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
 
 struct ReadParams {
     Pages c;
-    int rows;
+    int batch, rows;
     ChunkHead head;
     __nv_bfloat16* k;
     __nv_bfloat16* v;
@@ -222,19 +222,70 @@ __device__ __forceinline__ Eight<__nv_bfloat16> of_four_bits(uint32_t word, uint
     return x;
 }
 
+// The same in fp16, of a step and a least value times a power of two that leaves none of the sums at 2^15 or above. Both have 8 bits, so
+// they are fp16's too but where they are under 2^-17, which is nothing beside 2^15; the sums are rounded once, by 2^-11 of them at most.
+__device__ __forceinline__ Eight<__half> of_four_bits_f16(uint32_t word, uint32_t pair, float power) {
+    const __half2 step = __float2half2_rn(step_of(pair) * power), least = __float2half2_rn(least_of(pair) * power), zero = __float2half2_rn(1024.f);
+    Eight<__half> x;
+    __half2* to = reinterpret_cast<__half2*>(x.raw);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const uint32_t two = ((word >> (4 * n)) & 0x000f000fu) | 0x64006400u;   // two codes as fp16 1024 + c
+        to[n] = __hfma2(step, __hsub2(*reinterpret_cast<const __half2*>(&two), zero), least);
+    }
+    return x;
+}
+
 // A thread brings eight columns of kReadRows keys and their values, all requested before the first is used.
 constexpr int kReadRows = 4;
+// The power of two that brings numbers of up to this exponent (fp32's 8 bits) under 2^15: a multiple of 4, so that it changes
+// seldom, 116 at most. Numbers under 2^-65 lose bits of theirs, so that the sum of 2^30 weights over their power stays in range. (Keys whose
+// values are all under 2^-110 of others' of the head weigh nothing beside them, in the sum of weights too.)
+__device__ __forceinline__ int f16_power(int exponent) { return max((exponent - 127 + 1 - 15 + 3) & ~3, -80); }
 
-template <int D, int kBits>
+// Queries in fp16 as the forward takes them beside such keys: rows [row][head][D], each times a power of two, by the blocks of a grid's planes
+// from z on. D / 8 threads have one.
+template <int D>
+__device__ __forceinline__ void f16_queries(const ChunkHead& p, int z) {
+    constexpr int kThreads = D / 8;
+    const int col = threadIdx.x % kThreads * 8;
+    const int64_t all = p.q_rows * p.heads, plane = static_cast<int64_t>(gridDim.x) * gridDim.y, step = plane * (gridDim.z - z) * (256 / kThreads);
+    for (int64_t n0 = ((blockIdx.z - z) * plane + static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * (256 / kThreads); n0 < all; n0 += step) {
+        const int64_t n = n0 + threadIdx.x / kThreads, row = n / p.heads, b = p.sq ? row / p.sq : 0;
+        Eight<__nv_bfloat16> x;
+        x.zero();
+        if (n < all) {
+            const __nv_bfloat16* from = p.q + b * p.qs[0] + (n - row * p.heads) * p.qs[1] + (row - b * p.sq) * p.qs[2] + col;
+            if (p.q_vec) x.load(from); else x.load_some(from, 8);
+        }
+        float top = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(__bfloat162float(x.get(e))));
+#pragma unroll
+        for (int off = 1; off < kThreads; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        if (n >= all) continue;   // (the last in any case)
+        const int power = f16_power(__float_as_int(top) >> 23);
+        const float by = power_of_two(-power);
+        Eight<__half> y;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y.set(e, __float2half_rn(__bfloat162float(x.get(e)) * by));
+        y.store(p.q_out + n * D + col);
+        if (col == 0) p.q_power[n] = power_of_two(power);
+    }
+}
+
+// kHalf: 4-bit keys and values as fp16 with powers of two for each 64 keys, for the forward (ChunkHead); else bf16.
+template <int D, int kBits, bool kHalf>
 __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadParams p) {
     constexpr int kChunks = D / 8, kTokens = 256 / kChunks;   // tokens of the block at a time
     const int chunk = threadIdx.x % kChunks, col = chunk * 8, head = blockIdx.y, b = blockIdx.z;
     const int first = blockIdx.x * (kReadRows * kTokens) + threadIdx.x / kChunks;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int batch = p.batch;
+    if (kHalf && b >= batch) return f16_queries<D>(p.head, batch);
     const int len = cached_keys(p.c, b);
     if (p.head.words && blockIdx.x == 0 && head == 0) {
-        const int batch = gridDim.z;
         if (threadIdx.x == 0) {
             const bool last = b == batch - 1;
             p.head.offsets()[b] = b * p.rows;
@@ -295,6 +346,43 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
             }
         }
     }
+    if constexpr (kHalf) {
+        // The powers of each 64 keys, and of their values, from the largest end of a group among them (its exponent, over the block).
+        constexpr int kKeys = 64, kOf = kReadRows * kTokens / kKeys, kEach = kReadRows / kOf;   // chunks of the block, a thread's keys of each
+        static_assert(kKeys % kTokens == 0 && kOf >= 1, "a thread's keys are of whole chunks");
+        __shared__ int tops[2 * kOf];
+        if (threadIdx.x < 2 * kOf) tops[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2 * kOf; ++c) {   // keys of each chunk, then values
+            float top = 0.f;
+#pragma unroll
+            for (int i = (c % kOf) * kEach; i < (c % kOf + 1) * kEach; ++i) {
+                const uint32_t pair = words[i][c < kOf ? 1 : 3];
+                top = fmaxf(top, fmaxf(fabsf(least_of(pair)), fabsf(fmaf(15.f, step_of(pair), least_of(pair)))));
+            }
+            const int most = __reduce_max_sync(0xffffffffu, __float_as_int(top) >> 23);
+            if ((threadIdx.x & 31) == 0) atomicMax(&tops[c], most);
+        }
+        __syncthreads();
+        const int first_chunk = blockIdx.x * kOf;
+        int32_t* powers = p.head.powers + (static_cast<int64_t>(head) * batch + b) * p.head.chunks + first_chunk;
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int c = 0; c < kOf; ++c) powers[c] = static_cast<int>(__byte_perm(f16_power(tops[c]), f16_power(tops[kOf + c]), 0x5410));
+            // The forward looks at chunks by two; the block of one without a key does not get here.
+            if (kOf == 1 && !(first_chunk & 1) && (first_chunk + 1) * kKeys >= rows) powers[1] = powers[0];
+        }
+#pragma unroll
+        for (int i = 0; i < kReadRows; ++i) {
+            const int j = first + i * kTokens;
+            if (j >= rows) break;
+            const float kp2 = power_of_two(-f16_power(tops[i / kEach])), vp2 = power_of_two(-f16_power(tops[kOf + i / kEach]));
+            of_four_bits_f16(words[i][0], words[i][1], kp2).store(reinterpret_cast<__half*>(p.k) + b * p.ks[0] + head * p.ks[1] + j * p.ks[2] + col);
+            of_four_bits_f16(words[i][2], words[i][3], vp2).store(reinterpret_cast<__half*>(p.v) + b * p.vs[0] + head * p.vs[1] + j * p.vs[2] + col);
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < kReadRows; ++i) {
         const int j = first + i * kTokens;
@@ -345,15 +433,20 @@ int launch_append(const AppendParams& given, cudaStream_t stream) {
 }
 
 template <int D, int kBits>
-int launch_read(const ReadParams& p, int batch, int kv_heads, cudaStream_t stream) {
+int launch_read(const ReadParams& p, int kv_heads, cudaStream_t stream) {
     constexpr int kRows = kReadRows * (256 / (D / 8));
-    const dim3 grid(static_cast<unsigned>((p.rows + kRows - 1) / kRows), static_cast<unsigned>(kv_heads), static_cast<unsigned>(batch));
-    return launch_dependent(read_kernel<D, kBits>, p, grid, dim3(256), stream, "paged_read launch");
+    dim3 grid(static_cast<unsigned>((p.rows + kRows - 1) / kRows), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.batch));
+    if (p.head.q_rows > 0) {   // planes for the queries: two rows to a thread's place
+        const int64_t one = static_cast<int64_t>(grid.x) * grid.y * (2 * 256 / (D / 8)), planes = (p.head.q_rows * p.head.heads + one - 1) / one;
+        grid.z += static_cast<unsigned>(planes < 32768 ? planes : 32768);
+    }
+    if (kBits == 4 && p.head.powers) return launch_dependent(read_kernel<D, 4, true>, p, grid, dim3(256), stream, "paged_read launch");
+    return launch_dependent(read_kernel<D, kBits, false>, p, grid, dim3(256), stream, "paged_read launch");
 }
 
-int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, cudaStream_t stream) {
-    if (bits == 16) return d == 64 ? launch_read<64, 16>(p, batch, kv_heads, stream) : launch_read<128, 16>(p, batch, kv_heads, stream);
-    return d == 64 ? launch_read<64, 4>(p, batch, kv_heads, stream) : launch_read<128, 4>(p, batch, kv_heads, stream);
+int launch_read(const ReadParams& p, int bits, int d, int kv_heads, cudaStream_t stream) {
+    if (bits == 16) return d == 64 ? launch_read<64, 16>(p, kv_heads, stream) : launch_read<128, 16>(p, kv_heads, stream);
+    return d == 64 ? launch_read<64, 4>(p, kv_heads, stream) : launch_read<128, 4>(p, kv_heads, stream);
 }
 
 }  // namespace
@@ -361,12 +454,13 @@ int launch_read(const ReadParams& p, int bits, int d, int batch, int kv_heads, c
 int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], const ChunkHead& head, cudaStream_t stream) {
     ReadParams p = {};
     p.c = c;
+    p.batch = batch;
     p.rows = rows;
     p.head = head;
     p.k = static_cast<__nv_bfloat16*>(k);
     p.v = static_cast<__nv_bfloat16*>(v);
     for (int i = 0; i < 3; ++i) p.ks[i] = p.vs[i] = strides[i];
-    return launch_read(p, bits, d, batch, kv_heads, stream);
+    return launch_read(p, bits, d, kv_heads, stream);
 }
 
 }  // namespace ktt
@@ -427,6 +521,7 @@ extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_read: null pointer");
     }
     uintptr_t low = reinterpret_cast<uintptr_t>(a->k_out) | reinterpret_cast<uintptr_t>(a->v_out);
+    p.batch = a->batch;
     p.rows = a->rows;
     p.k = static_cast<__nv_bfloat16*>(a->k_out);
     p.v = static_cast<__nv_bfloat16*>(a->v_out);
@@ -435,5 +530,5 @@ extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {
         low |= static_cast<uintptr_t>((p.ks[i] | p.vs[i]) * 2);
     }
     if (low & 15) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_read: outputs must be 16-byte aligned in every row");
-    return launch_read(p, a->cache.bits, a->d, a->batch, a->cache.kv_heads, static_cast<cudaStream_t>(stream));
+    return launch_read(p, a->cache.bits, a->d, a->cache.kv_heads, static_cast<cudaStream_t>(stream));
 }

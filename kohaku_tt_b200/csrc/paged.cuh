@@ -79,6 +79,14 @@ struct ChunkHead {
     int32_t* words;         // null: no chunk
     const int32_t* cu_q;    // packed queries: their offsets as they were given
     int64_t total_q;
+    int32_t* powers;        // 4 bits: keys and values in fp16, divided by powers of two (AttnParams::kv_powers); null: bf16
+    int chunks;
+    // With them, unless q_rows is 0: the queries in fp16 too, [row][head][D], and each row's power.
+    const __nv_bfloat16* q;
+    int64_t qs[3], q_rows;
+    int heads, sq, q_vec;   // sq: rows of a batch entry, 0: packed
+    __half* q_out;
+    float* q_power;
     int tiles, most_parts, sms, d;   // what parts_of_chunk goes by; most_parts 0: no parts
     __host__ __device__ int32_t* offsets() const { return words + kHeadWords; }
     __host__ __device__ int32_t* order(int batch) const { return offsets() + batch + 1; }

@@ -31,7 +31,7 @@
 namespace ktt {
 
 // paged.cu: dense rows of the cache for a chunk of a prompt, and what the forward over them goes by (ChunkHead; its first words are
-// cleared, the offsets of the dense rows are 0, rows, 2 rows, ...).
+// cleared, the offsets of the dense rows are 0, rows, 2 rows, ..., queries are written where there are rows of them).
 int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int rows, void* k, void* v, const int64_t (&strides)[3], const ChunkHead& head, cudaStream_t stream);
 
 namespace {
@@ -937,7 +937,7 @@ struct Plan {
     int nt, row_tiles, slice;   // sequences of a launch
     int64_t bytes;              // of workspace
     int tiles, parts;           // chunks: tiles of 128 rows of a launch, and the most parts that their keys are cut into (0: none)
-    int64_t parts_at;           // where in the workspace the parts' rows are
+    int64_t powers_at, q_at, q_powers_at, parts_at;   // where in the workspace the keys' powers of two, fp16 queries and theirs, and parts are
 };
 
 // Tiles that are too few for the SMs are cut along their keys where that pays for the longest sequence that the table has room
@@ -952,6 +952,9 @@ int64_t part_rows(const ktt_b200_paged_sdpa_args* a, int batch) {
     const int64_t rows = static_cast<int64_t>(batch) * a->sq;
     return a->cu_seqlens_q && a->total_q < rows ? a->total_q : rows;
 }
+
+// Groups of 64 keys that a sequence has powers of two for, in whole blocks of 128.
+int chunks_of(const Pages& c) { return (c.cap + 127) / 128 * 2; }
 
 Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     Plan s = {};
@@ -972,7 +975,12 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     most = (1ll << 30) / one;
     s.slice = static_cast<int>(most < 1 ? 1 : (most < a->batch ? most : a->batch));
     if (s.slice > kMaxBatch) s.slice = kMaxBatch;
-    s.parts_at = s.slice * one + (head_words(kMaxBatch) * 4 + 255) / 256 * 256;
+    auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+    const int64_t rows_heads = a->cache.bits == 4 ? (a->cu_seqlens_q ? a->total_q : static_cast<int64_t>(a->batch) * a->sq) * a->heads : 0;
+    s.powers_at = s.slice * one + up(head_words(kMaxBatch) * 4);
+    s.q_at = s.powers_at + (a->cache.bits == 4 ? up(s.slice * hk * chunks_of(c) * 4) : 0);
+    s.q_powers_at = s.q_at + up(rows_heads * a->d * 2);
+    s.parts_at = s.q_powers_at + up(rows_heads * 4);
     s.bytes = s.parts_at;
     const bool packed = a->cu_seqlens_q != nullptr;
     int64_t tiles = s.slice * static_cast<int64_t>((a->sq + 127) / 128);
@@ -1117,14 +1125,17 @@ int merge_parts(const MergeParams& p, int d, cudaStream_t stream) {
 }
 
 // A chunk of a prompt: the rows of a K / V head are many, so the work is in the products, which the tensor kernels of the
-// dense and packed forward do; the pages become dense bf16 rows for them first (2 x 2 D bytes written and read per key
-// and head, against 4 D operations per key and row). Over 4 bits that rounds each key and value once more (2^-8 of it at most: the
-// tensor instructions' operands are 16 bits, and a code's worth, an 8-bit step times 4 bits and a sum, is not): against float64 the
-// result is off by 3.3e-3, where the pass, which multiplies codes, is by 2.4e-3 and bf16 pages by 2.3e-3 (root mean squares).
+// dense and packed forward do; the pages become dense rows for them first (2 x 2 D bytes written and read per key
+// and head, against 4 D operations per key and row). Those are bf16. Over 4 bits they are fp16, and so are the queries and the weights: a
+// code's worth is an 8-bit step times 4 bits and a sum, which bf16 rounds by as much as it does the weights. Powers of two, of each query row
+// and of each 64 keys and values, keep all magnitudes in fp16's range. Off against float64 (root mean squares of the result): 1.7e-3, all of
+// it the result's own rounding, where it was 3.3e-3 with everything in bf16; the pass, which multiplies codes by bf16 weights, 2.4e-3,
+// bf16 pages 2.3e-3. 4 sequences of up to 512 tokens and 8,192 keys, 16 heads over 4, D 128: 103 us, 101 in bf16, the queries' copy 2.5 of it.
 int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan& plan, cudaStream_t stream) {
     const int hk = a->cache.kv_heads, d = a->d, slice = plan.slice;
     const int64_t cap = p.c.cap, half = slice * cap * hk * d;
-    __nv_bfloat16* k = static_cast<__nv_bfloat16*>(a->workspace);
+    unsigned char* base = static_cast<unsigned char*>(a->workspace);
+    __nv_bfloat16* k = reinterpret_cast<__nv_bfloat16*>(base);
     __nv_bfloat16* v = k + half;
     int32_t* words = reinterpret_cast<int32_t*>(v + half);
     for (int b0 = 0; b0 < a->batch; b0 += slice) {
@@ -1145,13 +1156,6 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
         f.v = v;
         f.out = p.out;
         f.lse_strides[2] = 1;
-        // Sequences differ in length: their tiles are drawn, the longest sequence's first. (The head-dim-128 kernel does so with a
-        // counter of fewer than 256 bytes, which has to be zero before the call, and an order; the head-dim-64 kernel takes 256
-        // bytes and its own order.) 4 sequences of up to 512 tokens and 8,192 keys, 16 heads over 4, D 128, dealt in the order of the
-        // batch, drawn in it, and drawn by length: 121, 122 and 111 us.
-        const bool several = n > 1;
-        f.workspace = d == 64 || several ? words : nullptr;
-        f.workspace_bytes = d == 64 ? 256 : several ? 16 : 0;
         // All rows of a head together, sequence after sequence: a dense call's keys, and a packed one's.
         const int64_t strides[3] = {cap * d, slice * cap * d, d};
         for (int i = 0; i < 3; ++i) {
@@ -1161,7 +1165,13 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
         }
         f.key_lengths = c.lengths;
         f.causal = a->causal ? KTT_B200_CAUSAL_KEY_END : KTT_B200_CAUSAL_NONE;
-        ChunkHead head = {words, nullptr, a->total_q, plan.tiles, plan.parts, sm_count(current_device()), d};
+        ChunkHead head = {};
+        head.words = words;
+        head.total_q = a->total_q;
+        head.tiles = plan.tiles;
+        head.most_parts = plan.parts;
+        head.sms = sm_count(current_device());
+        head.d = d;
         if (a->cu_seqlens_q) {
             f.total_q = a->total_q;
             f.total_k = slice * cap;
@@ -1173,18 +1183,54 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
             f.q = p.q + b0 * a->q_strides[0];
             f.out = p.out + b0 * a->out_strides[0];
         }
-        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, stream)) return rc;
+        // The kernel of one tile per CTA takes parts, an order of its tiles and operands in fp16 (unless its copies cannot address the
+        // operands, or the output is not aligned for it). Head dim 128 is that kernel's anyway.
+        const bool several = n > 1, four = a->cache.bits == 4;
+        bool wide = plan.parts > 0 || four;
+        if (wide) {
+            const ktt_b200_attn_args given = f;
+            f.kernel = KTT_B200_KERNEL_TC5_WIDE;
+            if (four) {
+                f.q = base + plan.q_at + (a->cu_seqlens_q ? 0 : static_cast<int64_t>(b0) * a->sq * a->heads * d * 2);
+                f.q_strides[0] = a->cu_seqlens_q ? 0 : static_cast<int64_t>(a->sq) * a->heads * d;
+                f.q_strides[1] = d;
+                f.q_strides[2] = static_cast<int64_t>(a->heads) * d;
+            }
+            wide = ktt_b200_sdpa_supported(&f) != 0;
+            if (!wide) f = given;
+        }
+        const bool parts = wide && plan.parts > 0;
+        if (!parts) head.most_parts = 0;
         ForwardParts x = {};
         x.empty = true;
-        bool parts = plan.parts > 0;
-        if (parts) {
-            f.kernel = KTT_B200_KERNEL_TC5_WIDE;
-            parts = ktt_b200_sdpa_supported(&f) != 0;   // (else its copies cannot address the operands)
-            if (!parts) f.kernel = KTT_B200_KERNEL_AUTO;
-            f.workspace = parts ? words : nullptr;
-            f.workspace_bytes = parts ? 4 : 0;
+        if (wide && four) {
+            x.kv_powers = head.powers = reinterpret_cast<int32_t*>(base + plan.powers_at);
+            x.chunks = head.chunks = chunks_of(c);
+            float* q_power = reinterpret_cast<float*>(base + plan.q_powers_at);
+            x.q_power = q_power + (a->cu_seqlens_q ? 0 : static_cast<int64_t>(b0) * a->sq * a->heads);
+            if (b0 == 0) {   // of all launches
+                head.q = static_cast<const __nv_bfloat16*>(a->q);
+                head.q_rows = a->cu_seqlens_q ? a->total_q : static_cast<int64_t>(a->batch) * a->sq;
+                head.heads = a->heads;
+                head.sq = a->cu_seqlens_q ? 0 : a->sq;
+                head.q_vec = (reinterpret_cast<uintptr_t>(a->q) & 15) == 0;
+                for (int i = 0; i < 3; ++i) {
+                    head.qs[i] = a->q_strides[i];
+                    head.q_vec = head.q_vec && a->q_strides[i] % 8 == 0;
+                }
+                head.q_out = reinterpret_cast<__half*>(base + plan.q_at);
+                head.q_power = q_power;
+            }
         }
-        if (parts || (d == 128 && several)) x.order = head.order(n);
+        // Sequences differ in length: their tiles are drawn, the longest sequence's first. (That kernel does so with a
+        // counter of fewer than 256 bytes, which has to be zero before the call, and an order; the head-dim-64 kernel takes 256
+        // bytes and its own order.) 4 sequences of up to 512 tokens and 8,192 keys, 16 heads over 4, D 128, dealt in the order of the
+        // batch, drawn in it, and drawn by length: 121, 122 and 111 us.
+        const bool drawn = parts || ((d == 128 || wide) && several);
+        if (drawn) x.order = head.order(n);
+        f.workspace = drawn || d == 64 ? words : nullptr;
+        f.workspace_bytes = drawn ? 4 : d == 64 && !wide ? 256 : 0;
+        if (int rc = read_pages(c, a->cache.bits, d, n, hk, static_cast<int>(cap), k, v, strides, head, stream)) return rc;
         MergeParams m = {};
         if (parts) {
             m.c = c;
@@ -1193,7 +1239,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
             x.part_stride = m.stride = m.cu && m.rows == a->total_q ? 0 : a->sq;
             x.parts = m.parts = words + 1;
             x.most_parts = plan.parts;
-            m.o = x.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(a->workspace) + plan.parts_at);
+            m.o = x.part_o = reinterpret_cast<float*>(base + plan.parts_at);
             m.lse = x.part_lse = x.part_o + plan.parts * m.rows * a->heads * d;
             m.batch = n;
             m.heads = a->heads;

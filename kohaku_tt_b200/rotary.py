@@ -42,14 +42,14 @@ def rotary_table(positions, dim, base=10000.0, scaling=None, factor=1.0, origina
     device = torch.device(device)
     if device.type != "cuda":
         raise RuntimeError("kohaku_tt_b200: rotary tables are made on CUDA devices only; there is no CPU fallback")
-    scalars = (base, _scaling(scaling), factor, 0.0 if original is None else original, fast, slow)
+    scaling, original = _scaling(scaling), 0.0 if original is None else original
     eager = not torch.compiler.is_compiling() and _lib.native()
     if eager:
         index = torch.cuda.current_device() if device.index is None else device.index
-        out = eager.rotary_table(positions, dim, *scalars, index)
+        out = eager.rotary_table(positions, dim, base, scaling, factor, original, fast, slow, index)
         if out is not None:
             return out
-    return torch.ops.ktt_b200._rotary_table(int(positions), int(dim), *scalars, device)
+    return torch.ops.ktt_b200._rotary_table(int(positions), int(dim), base, scaling, factor, original, fast, slow, device)
 
 
 @torch.library.custom_op("ktt_b200::_rotary_table", mutates_args=(), device_types="cuda")
