@@ -244,33 +244,43 @@ constexpr int kReadRows = 4;
 __device__ __forceinline__ int f16_power(int exponent) { return max((exponent - 127 + 1 - 15 + 3) & ~3, -80); }
 
 // Queries in fp16 as the forward takes them beside such keys: rows [row][head][D], each times a power of two, by the blocks of a grid's planes
-// from z on. D / 8 threads have one.
+// from z on. D / 8 threads have kQueries of them.
+constexpr int kQueries = 4;
 template <int D>
 __device__ __forceinline__ void f16_queries(const ChunkHead& p, int z) {
-    constexpr int kThreads = D / 8;
+    constexpr int kThreads = D / 8, kRows = 256 / kThreads;
     const int col = threadIdx.x % kThreads * 8;
-    const int64_t all = p.q_rows * p.heads, plane = static_cast<int64_t>(gridDim.x) * gridDim.y, step = plane * (gridDim.z - z) * (256 / kThreads);
-    for (int64_t n0 = ((blockIdx.z - z) * plane + static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * (256 / kThreads); n0 < all; n0 += step) {
-        const int64_t n = n0 + threadIdx.x / kThreads, row = n / p.heads, b = p.sq ? row / p.sq : 0;
-        Eight<__nv_bfloat16> x;
-        x.zero();
-        if (n < all) {
+    const int64_t all = p.q_rows * p.heads, plane = static_cast<int64_t>(gridDim.x) * gridDim.y, step = plane * (gridDim.z - z) * (kQueries * kRows);
+    for (int64_t n0 = ((blockIdx.z - z) * plane + static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * (kQueries * kRows); n0 < all; n0 += step) {
+        Eight<__nv_bfloat16> x[kQueries];
+#pragma unroll
+        for (int i = 0; i < kQueries; ++i) {   // (all requested before the first is used)
+            const int64_t n = n0 + i * kRows + threadIdx.x / kThreads;
+            x[i].zero();
+            if (n >= all) continue;
+            // (64-bit quotients take some hundred instructions)
+            const int64_t row = all >> 32 ? n / p.heads : static_cast<uint32_t>(n) / static_cast<uint32_t>(p.heads);
+            const int64_t b = !p.sq ? 0 : all >> 32 ? row / p.sq : static_cast<uint32_t>(row) / static_cast<uint32_t>(p.sq);
             const __nv_bfloat16* from = p.q + b * p.qs[0] + (n - row * p.heads) * p.qs[1] + (row - b * p.sq) * p.qs[2] + col;
-            if (p.q_vec) x.load(from); else x.load_some(from, 8);
+            if (p.q_vec) x[i].load(from); else x[i].load_some(from, 8);
         }
-        float top = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(__bfloat162float(x.get(e))));
+        for (int i = 0; i < kQueries; ++i) {
+            const int64_t n = n0 + i * kRows + threadIdx.x / kThreads;
+            float top = 0.f;
 #pragma unroll
-        for (int off = 1; off < kThreads; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-        if (n >= all) continue;   // (the last in any case)
-        const int power = f16_power(__float_as_int(top) >> 23);
-        const float by = power_of_two(-power);
-        Eight<__half> y;
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(__bfloat162float(x[i].get(e))));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y.set(e, __float2half_rn(__bfloat162float(x.get(e)) * by));
-        y.store(p.q_out + n * D + col);
-        if (col == 0) p.q_power[n] = power_of_two(power);
+            for (int off = 1; off < kThreads; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            if (n >= all) continue;   // (the last in any case)
+            const int power = f16_power(__float_as_int(top) >> 23);
+            const float by = power_of_two(-power);
+            Eight<__half> y;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y.set(e, __float2half_rn(__bfloat162float(x[i].get(e)) * by));
+            y.store(p.q_out + n * D + col);
+            if (col == 0) p.q_power[n] = power_of_two(power);
+        }
     }
 }
 
@@ -436,8 +446,8 @@ template <int D, int kBits>
 int launch_read(const ReadParams& p, int kv_heads, cudaStream_t stream) {
     constexpr int kRows = kReadRows * (256 / (D / 8));
     dim3 grid(static_cast<unsigned>((p.rows + kRows - 1) / kRows), static_cast<unsigned>(kv_heads), static_cast<unsigned>(p.batch));
-    if (p.head.q_rows > 0) {   // planes for the queries: two rows to a thread's place
-        const int64_t one = static_cast<int64_t>(grid.x) * grid.y * (2 * 256 / (D / 8)), planes = (p.head.q_rows * p.head.heads + one - 1) / one;
+    if (p.head.q_rows > 0) {   // planes for the queries
+        const int64_t one = static_cast<int64_t>(grid.x) * grid.y * (kQueries * 256 / (D / 8)), planes = (p.head.q_rows * p.head.heads + one - 1) / one;
         grid.z += static_cast<unsigned>(planes < 32768 ? planes : 32768);
     }
     if (kBits == 4 && p.head.powers) return launch_dependent(read_kernel<D, 4, true>, p, grid, dim3(256), stream, "paged_read launch");
