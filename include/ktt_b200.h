@@ -397,7 +397,7 @@ typedef struct ktt_b200_pages {
  * q (optional, heads 0 without) is rotated alongside into q_out. Dense: [B, H, rows, D]; packed (cu_seqlens int32
  * [batch + 1] on the device): [rows, H, D] with batch strides 0, rows that no sequence covers are neither read nor
  * written. lengths_out (optional, another buffer than lengths) receives the new lengths. No two sequences may append to one
- * page in one call. */
+ * page in one call; q_out may not overlap q (a row's threads read what others of them write). */
 typedef struct ktt_b200_append_args {
     ktt_b200_pages cache;
     int32_t batch, rows, heads, d;  /* packed: rows = all rows of q, k and v */
@@ -429,7 +429,7 @@ KTT_B200_API int ktt_b200_paged_read(const ktt_b200_read_args* args, void* strea
 /* Attention over the cache: q dense [B, H, sq, D] or packed [total_q, H, D] (cu_seqlens_q int32 [batch + 1] on the device, sq
  * = the longest, batch stride 0), D 64 or 128. `lengths` count the keys with those of the call's own tokens. causal (1):
  * query i of n sees keys j <= length - n + i; a row that sees none gets zeros. Packed rows that no sequence covers are
- * left as they were; offsets outside of [0, total_q] are taken as its ends. */
+ * left as they were; offsets outside of [0, total_q] are taken as its ends. out may not overlap q: many blocks read a row of it. */
 typedef struct ktt_b200_paged_sdpa_args {
     ktt_b200_pages cache;
     int32_t batch, heads, sq, d;

@@ -492,6 +492,7 @@ extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream
     if (a->lengths_out && a->lengths_out < a->cache.lengths + a->batch && a->cache.lengths < a->lengths_out + a->batch) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: lengths_out must not overlap the lengths");
     }
+    if (a->heads && a->rows && a->q == a->q_out) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: q_out must not overlap q");
     p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, 0};
     p.batch = a->batch;
     p.rows = a->rows;

@@ -1285,6 +1285,7 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
     if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || !a->q || !a->out) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null pointer");
     }
+    if (a->q == a->out) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: out must not overlap q");
     const Plan s = plan_of(a, p.c, sm_count(current_device()));
     if (!a->workspace || a->workspace_bytes < s.bytes) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: workspace holds %lld bytes, %lld needed", static_cast<long long>(a->workspace_bytes), static_cast<long long>(s.bytes));

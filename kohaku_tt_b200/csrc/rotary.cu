@@ -318,6 +318,7 @@ extern "C" int ktt_b200_rotary(const ktt_b200_rotary_args* a, void* stream) {
     if (tokens > (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary: at most 2^31 tokens");
     if (!a->q || !a->q_out || !a->cos || !a->sin || (a->kv_heads && (!a->k || !a->k_out))) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: null pointer");
     if (a->table_rows < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: the tables have no rows");
+    if (a->q == a->q_out || (a->kv_heads && a->k == a->k_out)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: outputs must not overlap inputs");
     RotaryParams p = {};
     p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, a->inverse};
     p.x[0] = a->q; p.x[1] = a->k;
