@@ -207,8 +207,9 @@ struct ReadParams {
     int64_t ks[3], vs[3];
 };
 
-// What eight codes are worth: bf16 products and sums of pairs, rounded once. (An fp32 sum rounded to bf16 is the same: where step
-// is under 2^-15 of least's power of two, so that fp32 cannot hold the sum, all 15 steps are less than half of bf16's.)
+// What eight codes are worth: bf16 products and sums of pairs, rounded once. (An fp32 sum rounded to bf16 would be the same but where the
+// least value is under 2^-19 of the step: the sum then drops it, and a product that lies halfway between two bf16 values goes to the even one
+// instead of to the side that the least value is on.)
 __device__ __forceinline__ Eight<__nv_bfloat16> of_four_bits(uint32_t word, uint32_t pair) {
     const __nv_bfloat162 ends = *reinterpret_cast<const __nv_bfloat162*>(&pair), step = __low2bfloat162(ends), least = __high2bfloat162(ends);
     const __nv_bfloat162 zero = __float2bfloat162_rn(128.f);

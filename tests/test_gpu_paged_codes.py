@@ -1,5 +1,5 @@
 """Codes of groups whose steps are subnormal: a step of a few of the least bf16 values is rounded by as much as half of one, and
-the farthest values then lie past 15 of them."""
+the farthest values then lie past 15 of them; and what codes are worth where the least value is far below the step."""
 
 import pytest
 import torch
@@ -31,3 +31,31 @@ def test_ranges_of_a_few_of_the_least_values(cuda, d, least):
         got = po.unpack(pages.cpu(), value)
         for a, b in zip(got, want):
             assert torch.equal(a.transpose(1, 2).reshape(b.shape), b)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_code_s_worth_is_rounded_once(cuda, d):
+    """least + step * code of all 16 codes, least values of 2^-12 to 2^-40 of the step on both sides: against the sum in 64 bits, rounded to the
+    nearest bf16, ties to even."""
+    n = 256
+    x = torch.zeros((n, 1, d), dtype=torch.bfloat16)
+    steps = 1 + torch.arange(n) % 128 / 128.0
+    for g in range(0, d, 64):
+        for c in range(64):
+            x[:, 0, g + c] = ((c % 16) * steps).to(torch.bfloat16)
+    pages = {value: po.pack(x.view(n // 16, 16, 1, d).transpose(1, 2), value) for value in (False, True)}
+    least = (2.0 ** -(12 + torch.arange(n) % 29).double() * (1 - 2 * (torch.arange(n) // 29 % 2))).to(torch.bfloat16)
+    for pool in pages.values():     # the least values themselves, beside the codes
+        words = pool.view(n // 16, 1, 1, 16 * (d // 2 + d // 16))[..., 8 * d:].view(torch.bfloat16)
+        words[..., 1::2] = least.view(n // 16, 1, 1, 16, 1).expand(-1, -1, -1, -1, d // 64).reshape(n // 16, 1, 1, -1)
+    table = torch.arange(n // 16, dtype=torch.int32, device=cuda)[None]
+    lens = torch.tensor([n], dtype=torch.int32, device=cuda)
+    got = ktt.paged_read(pages[False].to(cuda), pages[True].to(cuda), table, lens)
+    for out, value in zip(got, (False, True)):
+        code, step, low = (t.double().transpose(1, 2).reshape(n, -1) for t in po.unpack(pages[value], value))
+        exact = (low.unsqueeze(-1) + step.unsqueeze(-1) * code.view(n, -1, 64)).reshape(n, d)
+        have = out[0, 0].cpu()
+        bits = have.view(torch.int16)
+        for other in ((bits + 1).view(torch.bfloat16), (bits - 1).view(torch.bfloat16)):     # no neighbour is nearer
+            near, far = (have.double() - exact).abs(), (other.double() - exact).abs()
+            assert ((near < far) | ((near == far) & (bits & 1 == 0)) | (have == 0)).all()
