@@ -82,3 +82,46 @@ def test_pages_and_queries_in_other_orders(cuda, n):
     want = ktt.sdpa_paged(q, kp.to(cuda), vp.to(cuda), table.to(cuda), lens)
     got = ktt.sdpa_paged(q.transpose(1, 2).contiguous().transpose(1, 2), both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2), table.to(cuda), lens)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("bits", BITS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_process_s_first_chunk_inside_a_capture(cuda, bits, d):
+    """Chunks that are cut and whole, captured before any call has run; then two replays at once with calls on a third stream."""
+    import subprocess
+    import sys
+
+    code = f"""
+import torch, kohaku_tt_b200 as ktt
+dev = torch.device("cuda:0")
+kp, vp = ktt.paged_cache(188, 2, 16, {d}, bits={bits}, device=dev)
+table = torch.arange(188, dtype=torch.int32, device=dev).view(2, 94)
+zero, lens = torch.zeros(2, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+k, v = (torch.randn(2, 2, 1500, {d}, device=dev).bfloat16() for _ in range(2))
+qs = [torch.randn(2, h, 140, {d}, device=dev).bfloat16() for h in (2, 16)]
+torch.cuda.synchronize()
+graphs, got = [], []
+for q in qs:
+    graphs.append(torch.cuda.CUDAGraph())
+    with torch.cuda.graph(graphs[-1]):
+        ktt.paged_append(k, v, kp, vp, table, zero, lengths_out=lens)
+        got.append(ktt.sdpa_paged(q, kp, vp, table, lens))
+for g in graphs:
+    g.replay()
+torch.cuda.synchronize()
+assert lens.tolist() == [1500, 1500]
+want = [ktt.sdpa_paged(q, kp, vp, table, lens) for q in qs]
+streams = [torch.cuda.Stream() for _ in range(3)]
+for _ in range(5):
+    torch.cuda.synchronize()
+    for s, g in zip(streams, graphs):
+        with torch.cuda.stream(s):
+            g.replay()
+    with torch.cuda.stream(streams[2]):
+        eager = [ktt.sdpa_paged(q, kp, vp, table, lens) for q in qs]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) and torch.equal(c, b) and b.isfinite().all() for a, b, c in zip(got, want, eager))
+print("same")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "same" in done.stdout, done.stdout + done.stderr[-3000:]
