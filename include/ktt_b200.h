@@ -339,8 +339,8 @@ KTT_B200_API int ktt_b200_merge_partials(
 
 /* The dim / 2 (256 at most) frequencies f_i of rotary tables, in 64 bits, and what cosines and sines are multiplied by. scaling:
  * 0: f_i = base^(-2 i / dim). 1: f_i / factor. 2: with base factor^(dim / (dim - 2)). 3: pairs that turn `fast` times or more
- * within `original` positions keep f_i, those that turn `slow` times or less get f_i / factor, those between a mixture by
- * their turns; cosines and sines times 0.1 ln(factor) + 1. Host only; launches nothing. */
+ * within `original` positions keep f_i, those that turn `slow` times or less get f_i / factor, those between a mixture linear
+ * in their turns; cosines and sines times 0.1 ln(factor) + 1. Host only; launches nothing. */
 KTT_B200_API int ktt_b200_rotary_frequencies(double* frequencies, double* scale, int32_t dim, double base, int32_t scaling, double factor, double original, double fast, double slow);
 
 /* cos / sin [positions][pairs] fp32, rows dense: scale * cos(p f_i), scale * sin(p f_i) for positions p = 0, 1, ... and the

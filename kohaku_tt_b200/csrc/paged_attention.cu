@@ -64,8 +64,8 @@ constexpr int kMaxBatch = 512;    // lengths and their prefix sums live in share
 // What a variant has: D, bits of the pages, NT column tiles of 8 query rows. Measured, us, 64 sequences, 16 heads over 2, D 128,
 // lengths U[n / 8, n], unless it says otherwise:
 //   4 bits, n 16,384, one column tile: two blocks at a time, 4 warps, 3 CTAs 53.2; one block at a time 55.7; 8 warps, 2 CTAs (128
-//   registers) 56.6; 4 warps, 4 CTAs 56.0. Loads alone 39.4, products alone as long as both: the stream is bound by the issue of
-//   some 390 instructions a block, half of them on the integer pipe. D 64, 32 heads over 8, n 512: 4 CTAs 10.0, 3 CTAs 15.3.
+//   registers) 56.6; 4 warps, 4 CTAs 56.0. Loads alone 39.4, products alone as long as both: the stream is bound by the
+//   chains between some 390 instructions a block (0.55 issued per scheduler and cycle, no pipe over 54 %). D 64, 32 heads over 8, n 512: 4 CTAs 10.0, 3 CTAs 15.3.
 //   Two column tiles, 16 x 4 tokens, n 8,192: 2 CTAs 28.7, 3 (spills) 58.
 //   bf16, n 4,096: 2 stages 34.3, 3 stages 34.7, 3 CTAs 34.8 (4.8 TB/s, 73 % of a copy's rate). D 64, 32 x 14 heads over 2, n 8,192: 4 CTAs of
 //   3 stages 20.9, 2 of 6 22.7, 3 of 4 25.9; 64 x 32 over 8, n 512: 11.2, 18.1, 16.6.

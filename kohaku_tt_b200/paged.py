@@ -276,14 +276,15 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
                max_k=None):
     """Attention of q [B, H, Sq, D] over the first lengths[b] keys of each sequence's pages; Sq may be one
     token, a few, or a chunk of a prompt. Packed: q [T, H, D] with cu_seq_q (B + 1 offsets, a list, or int32 on
-    the device, then best with max_q, no less than the longest sequence); rows that no sequence covers are left
-    undefined.
+    the device, then best with max_q, no less than the longest sequence, and taken inside of the T rows); rows that no
+    sequence covers are left undefined.
 
     Pages as in paged_append, bf16 or 4 bits, D 64 or 128, H a multiple of Hk. lengths (int32 [B] on the
     device) count the keys with those of the call's own tokens, which are appended first. Under is_causal the
     diagonal is aligned to the end: query i of n sees keys 0 .. lengths[b] - n + i. A row that sees no key
     gets zeros. max_k: no sequence has more keys (default: what block_table has room for; longer ones are
-    cut); an entry of block_table within a length that is no page of the cache reads as zeros. A key that some of a sequence's queries see and others do not must be finite. No gradients."""
+    cut); an entry of block_table within a length that is no page of the cache reads as zeros. A key that some of a sequence's queries see and others do not must be finite. Weights are
+    rounded to bf16 for their product with the values, to fp16 in chunks of prompts over 4-bit pages. No gradients."""
     causal = bool(is_causal)
     if torch.compiler.is_compiling():
         return torch.ops.ktt_b200._sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)

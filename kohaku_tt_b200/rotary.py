@@ -36,9 +36,10 @@ def rotary_table(positions, dim, base=10000.0, scaling=None, factor=1.0, origina
     scaling, for contexts `factor` times as long as a model was trained for:
       "linear"  f_i / factor: positions are interpolated;
       "base"    base times factor^(dim / (dim - 2)): the slowest pair is interpolated, the fastest kept;
-      "parts"   pairs that turn more than `fast` times within the `original` context keep their
-                frequency, those that turn less than `slow` times get f_i / factor, those between a
-                mixture; cos and sin are multiplied by 0.1 ln(factor) + 1."""
+      "parts"   pairs that turn `fast` times or more within the `original` context keep their
+                frequency, those that turn `slow` times or less get f_i / factor; one that turns r times
+                between them keeps (r - slow) / (fast - slow) of it and has f_i / factor for the rest
+                (a ramp in the turns, not in i); cos and sin are multiplied by 0.1 ln(factor) + 1."""
     device = torch.device(device)
     if device.type != "cuda":
         raise RuntimeError("kohaku_tt_b200: rotary tables are made on CUDA devices only; there is no CPU fallback")
