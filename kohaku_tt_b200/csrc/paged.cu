@@ -370,7 +370,8 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
 #pragma unroll
             for (int i = (c % kOf) * kEach; i < (c % kOf + 1) * kEach; ++i) {
                 const uint32_t pair = words[i][c < kOf ? 1 : 3];
-                top = fmaxf(top, fmaxf(fabsf(least_of(pair)), fabsf(fmaf(15.f, step_of(pair), least_of(pair)))));
+                const float end = fmaxf(fabsf(least_of(pair)), fabsf(fmaf(15.f, step_of(pair), least_of(pair))));
+                if (end < INFINITY) top = fmaxf(top, end);   // (an infinity has no power, and takes none from the others)
             }
             const int most = __reduce_max_sync(0xffffffffu, __float_as_int(top) >> 23);
             if ((threadIdx.x & 31) == 0) atomicMax(&tops[c], most);
