@@ -240,8 +240,9 @@ __device__ __forceinline__ Eight<__half> of_four_bits_f16(uint32_t word, uint32_
 // A thread brings eight columns of kReadRows keys and their values, all requested before the first is used.
 constexpr int kReadRows = 4;
 // The power of two that brings numbers of up to this exponent (fp32's 8 bits) under 2^15: a multiple of 4, so that it changes
-// seldom, 116 at most. Numbers under 2^-65 lose bits of theirs, so that the sum of 2^30 weights over their power stays in range. (Keys whose
-// values are all under 2^-110 of others' of the head weigh nothing beside them, in the sum of weights too.)
+// seldom, 116 at most. What shares a power (a query row, 64 keys, 64 values) has 11 bits down to 2^-25 of the largest and fewer below, and
+// under 2^-65 in any case, so that the sum of 2^30 weights over their power stays in range. (Keys whose values are all under 2^-110 of others' of
+// the head weigh nothing beside them, in the sum of weights too.)
 __device__ __forceinline__ int f16_power(int exponent) { return max((exponent - 127 + 1 - 15 + 3) & ~3, -80); }
 
 // Queries in fp16 as the forward takes them beside such keys: rows [row][head][D], each times a power of two, by the blocks of a grid's planes
