@@ -1184,7 +1184,7 @@ int run_many(const ktt_b200_paged_sdpa_args* a, const PagedParams& p, const Plan
             f.out = p.out + b0 * a->out_strides[0];
         }
         // The kernel of one tile per CTA takes parts, an order of its tiles and operands in fp16 (unless its copies cannot address the
-        // operands, or the output is not aligned for it). Head dim 128 is that kernel's anyway.
+        // operands, or the output is not aligned for it: dense rows are bf16 then, over 4 bits too). Head dim 128 is that kernel's anyway.
         const bool several = n > 1, four = a->cache.bits == 4;
         bool wide = plan.parts > 0 || four;
         if (wide) {
