@@ -370,6 +370,18 @@ typedef struct ktt_b200_rotary_args {
 } ktt_b200_rotary_args;
 KTT_B200_API int ktt_b200_rotary(const ktt_b200_rotary_args* args, void* stream);
 
+/* Positions of several axes (time, height, width of pictures and video): pair i of a row turns by the table row of the row's
+ * position on axis of_pair[i]. positions [axis, batch, row] on the device with element strides, clamped like those of one axis. */
+typedef struct ktt_b200_axes {
+    int32_t axes;                  /* 1 to 4 */
+    int32_t positions_are_64;      /* int64, else int32 */
+    const void* positions;
+    int64_t strides[3];            /* (axis, batch, row); packed rows: batch 0 */
+    const uint8_t* of_pair;        /* host memory, one byte for each pair of columns, read during the call; NULL: axis 0 */
+} ktt_b200_axes;
+/* ktt_b200_rotary by such positions; those of args are not used. */
+KTT_B200_API int ktt_b200_rotary_axes(const ktt_b200_rotary_args* args, const ktt_b200_axes* axes, void* stream);
+
 /* A cache in pages: key j of sequence b is row j % page_size of page block_table[b][j / page_size]. An entry outside
  * [0, pages) names no page: rows appended there go nowhere, keys and values read there are zeros. page_size is a multiple of
  * 16. bits 16: bf16 rows of D values, (page, head, row) strides in elements, multiples of 8. bits 4: bytes, of which each 16
@@ -390,6 +402,32 @@ typedef struct ktt_b200_pages {
     const int32_t* lengths;        /* int32 [batch] on the device: keys in the cache, clamped to [0, capacity] */
     int32_t max_keys;              /* capacity of a sequence where it is less than table_width * page_size; 0: that */
 } ktt_b200_pages;
+
+/* Block tables kept on the device. free_pages[0 .. *count) are the pages that no sequence has; a call reads *count and leaves the new
+ * number in *count_out (another word). Sequence b has pages in the first ceil(lengths[b] / page_size) entries of its row. */
+typedef struct ktt_b200_tables {
+    int32_t batch, table_width, page_size;   /* batch: 4096 at most */
+    int32_t* block_table;          /* int32 [batch][table_width] */
+    int64_t table_stride;
+    const int32_t* lengths;        /* int32 [batch], clamped to [0, table_width * page_size] */
+    int32_t* free_pages;           /* int32 [pool] */
+    int64_t pool;
+    const int32_t* count;
+    int32_t* count_out;
+} ktt_b200_tables;
+
+/* Pages for added[b] new keys of each sequence (int32 [batch] on the device), from the end of the list on: the i-th that the call
+ * takes, sequence by sequence and entry by entry, is free_pages[*count - 1 - i]. The first sequence that the list (or its row of
+ * the table) has no room for gets none, and none of those behind it do: their new entries are -1. The list is only read. Outputs,
+ * each of which may be NULL: granted int32 [batch] (added[b], or 0); cu_seqlens int32 [batch + 1], the sums of added; and of each
+ * of `tokens` packed rows, row i of sequence b being cu_seqlens[b] + i: positions int32, lengths[b] + i, and slots int64, page *
+ * page_size + row in the page; both -1 behind the last sequence's rows, slots also of sequences that got nothing. */
+KTT_B200_API int ktt_b200_paged_reserve(const ktt_b200_tables* args, const int32_t* added, int64_t tokens, int32_t* cu_seqlens, int32_t* positions, int64_t* slots, int32_t* granted, void* stream);
+
+/* Cuts sequences back to kept[b] keys (int32 [batch] on the device, clamped to [0, lengths[b]]; 0: all of its pages): the pages behind those
+ * go to free_pages[*count ..], sequence by sequence and entry by entry, and their entries become -1. Entries outside [0, pool) give
+ * nothing; pages past the list's end are dropped. */
+KTT_B200_API int ktt_b200_paged_release(const ktt_b200_tables* args, const int32_t* kept, void* stream);
 
 /* Appends rows lengths[b] .. of sequence b: k rotated (as above, at the position it is cached at; cos NULL: as it is) and
  * rounded to bf16, v as it is; 4-bit pages hold step = bf16((most - least) / 15), code = (x - least) / step to the nearest
@@ -414,6 +452,60 @@ typedef struct ktt_b200_append_args {
     int32_t* lengths_out;
 } ktt_b200_append_args;
 KTT_B200_API int ktt_b200_paged_append(const ktt_b200_append_args* args, void* stream);
+
+/* Bounds of pages: bf16 [pages][kv heads][2][D], the least and the largest value of each channel over a page's keys, as
+ * ktt_b200_paged_read gives them (a NaN among them stays one); (page, head, edge) strides in elements, multiples of 8, 16-byte aligned. */
+
+/* ktt_b200_paged_append with rows turned by positions of their own instead of their places in the cache (positions.positions NULL: the
+ * places; packed rows: batch stride 0), and with the bounds of the pages that the new keys lie in (bounds NULL: none). Bounds of a page
+ * that held keys before have to be those of these keys. */
+typedef struct ktt_b200_append_at_args {
+    ktt_b200_append_args base;
+    ktt_b200_axes positions;
+    void* bounds;
+    int64_t bounds_strides[3];
+} ktt_b200_append_at_args;
+KTT_B200_API int ktt_b200_paged_append_at(const ktt_b200_append_at_args* args, void* stream);
+
+/* Bounds of the pages that keys since[b] .. lengths[b] - 1 of each sequence lie in (since int32 [batch] on the device, or NULL: all
+ * pages); where since[b] lies inside a page, those that the page has already are kept and widened. cache.v is not used. */
+typedef struct ktt_b200_bounds_args {
+    ktt_b200_pages cache;
+    int32_t batch, d;
+    const int32_t* since;
+    void* bounds;
+    int64_t bounds_strides[3];
+} ktt_b200_bounds_args;
+KTT_B200_API int ktt_b200_paged_bounds(const ktt_b200_bounds_args* args, void* stream);
+
+/* The `top` pages of its sequence that each query token goes to, for each K / V head: the first `first`, the last `last` (first + last
+ * <= top, last >= 1), and of the others those of the largest score, ties to the lower place. A page's score is the largest logit that a key
+ * between its bounds could have, over the queries q_h of the head's group: max_h sum_d max(q_hd least_d, q_hd largest_d), of which the exact
+ * value decides; one that is no number counts as infinite, that of an entry that names no page as 0. q dense [B, H, sq, D] or packed
+ * [total_q, H, D] (cu_seqlens_q); lengths count the keys with those of the call's own tokens, and query i of n sees keys
+ * 0 .. length - n + i, and the pages these lie in. chosen int32 [tokens][kv_heads][top]: the pages' names in the order of their places, -1 behind
+ * them; keys int32 [tokens][kv_heads]: how many keys they hold that the token sees (0: none). Tokens: batch * sq, or total_q. */
+typedef struct ktt_b200_select_args {
+    int32_t batch, heads, kv_heads, sq, d;
+    int64_t total_q;
+    int32_t page_size, table_width;
+    int64_t pages;
+    const int32_t* block_table;
+    int64_t table_stride;
+    const int32_t* lengths;
+    int32_t top, first, last;
+    const void* q;
+    int64_t q_strides[3];
+    const int32_t* cu_seqlens_q;
+    const void* bounds;
+    int64_t bounds_strides[3];
+    int32_t* chosen;
+    int32_t* keys;
+    void* workspace;               /* ktt_b200_paged_select_workspace() bytes, 16-byte aligned, of any content */
+    int64_t workspace_bytes;
+} ktt_b200_select_args;
+KTT_B200_API int64_t ktt_b200_paged_select_workspace(const ktt_b200_select_args* args);
+KTT_B200_API int ktt_b200_paged_select(const ktt_b200_select_args* args, void* stream);
 
 /* The cache as dense bf16 k_out / v_out [batch, kv heads, rows, D] with (batch, head, row) strides: rows past a sequence's
  * length, and those that have no page, are zero. */
@@ -448,6 +540,12 @@ typedef struct ktt_b200_paged_sdpa_args {
  * a copy of the queries (2 D + 4 bytes for each row and head). */
 KTT_B200_API int64_t ktt_b200_paged_sdpa_workspace(const ktt_b200_paged_sdpa_args* args);
 KTT_B200_API int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* args, void* stream);
+
+/* Attention where each query token has a table of its own for each K / V head: cache.block_table [batch * sq][kv heads][table_width] with
+ * table_stride values from a head's row to the next, cache.lengths [batch * sq][kv heads] the keys behind it, all of which the token sees
+ * (causal is not used). q dense [B, H, sq, D]; packed tokens: batch 1, sq tokens. */
+KTT_B200_API int64_t ktt_b200_paged_sdpa_chosen_workspace(const ktt_b200_paged_sdpa_args* args);
+KTT_B200_API int ktt_b200_paged_sdpa_chosen(const ktt_b200_paged_sdpa_args* args, void* stream);
 
 #ifdef __cplusplus
 }

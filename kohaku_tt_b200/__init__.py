@@ -8,6 +8,8 @@
     cos, sin = ktt.rotary_table(positions, dim); q, k = ktt.rotary(q, k, cos, sin)
     q = ktt.paged_append(k, v, k_pages, v_pages, table, lengths, cos, sin, q=q, lengths_out=n)
     y = ktt.sdpa_paged(q, k_pages, v_pages, table, n)
+    cu, positions, slots, granted = ktt.paged_reserve(table, lengths, added, free, count, page_size, tokens, left)
+    pages, keys = ktt.paged_select(q, bounds, table, n, page_size, top=64); y = ktt.sdpa_paged(q, k_pages, v_pages, pages, keys)
 
 Everything runs on hand-written sm_100a CUDA in lib/libktt_b200.so (C ABI in
 include/ktt_b200.h); there is no CPU or PyTorch-math fallback.
@@ -21,7 +23,9 @@ from .attention import decode_step, sdpa, sdpa_varlen
 from .numerics import KERNELS, sdpa_kernel
 from .paged import paged_append, paged_cache, paged_read, sdpa_paged
 from .rotary import rotary, rotary_table
+from .selection import paged_bounds, paged_select
 from .stats import diff_stats, format_stats, rel_rms
+from .tables import paged_release, paged_reserve
 from .trace import debug_flash_dump
 
 AVAILABLE = True
@@ -53,8 +57,12 @@ __all__ = [
     "sdpa_kernel",
     "debug_flash_dump",
     "paged_append",
+    "paged_bounds",
     "paged_cache",
     "paged_read",
+    "paged_release",
+    "paged_reserve",
+    "paged_select",
     "rotary",
     "rotary_table",
     "sdpa_paged",

@@ -67,6 +67,15 @@ EXPORTS = (
     "ktt_b200_paged_read",
     "ktt_b200_paged_sdpa",
     "ktt_b200_paged_sdpa_workspace",
+    "ktt_b200_rotary_axes",
+    "ktt_b200_paged_reserve",
+    "ktt_b200_paged_release",
+    "ktt_b200_paged_append_at",
+    "ktt_b200_paged_bounds",
+    "ktt_b200_paged_select",
+    "ktt_b200_paged_select_workspace",
+    "ktt_b200_paged_sdpa_chosen",
+    "ktt_b200_paged_sdpa_chosen_workspace",
 )
 
 _i32, _i64, _f32, _ptr = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
@@ -278,6 +287,90 @@ class PagedSdpaArgs(ctypes.Structure):
     ]
 
 
+class Axes(ctypes.Structure):
+    """struct ktt_b200_axes."""
+
+    _fields_ = [
+        ("axes", _i32),
+        ("positions_are_64", _i32),
+        ("positions", _ptr),
+        ("strides", _i64 * 3),
+        ("of_pair", ctypes.c_char_p),
+    ]
+
+
+class Tables(ctypes.Structure):
+    """struct ktt_b200_tables."""
+
+    _fields_ = [
+        ("batch", _i32),
+        ("table_width", _i32),
+        ("page_size", _i32),
+        ("block_table", _ptr),
+        ("table_stride", _i64),
+        ("lengths", _ptr),
+        ("free_pages", _ptr),
+        ("pool", _i64),
+        ("count", _ptr),
+        ("count_out", _ptr),
+    ]
+
+
+class AppendAtArgs(ctypes.Structure):
+    """struct ktt_b200_append_at_args."""
+
+    _fields_ = [
+        ("base", AppendArgs),
+        ("positions", Axes),
+        ("bounds", _ptr),
+        ("bounds_strides", _i64 * 3),
+    ]
+
+
+class BoundsArgs(ctypes.Structure):
+    """struct ktt_b200_bounds_args."""
+
+    _fields_ = [
+        ("cache", Pages),
+        ("batch", _i32),
+        ("d", _i32),
+        ("since", _ptr),
+        ("bounds", _ptr),
+        ("bounds_strides", _i64 * 3),
+    ]
+
+
+class SelectArgs(ctypes.Structure):
+    """struct ktt_b200_select_args."""
+
+    _fields_ = [
+        ("batch", _i32),
+        ("heads", _i32),
+        ("kv_heads", _i32),
+        ("sq", _i32),
+        ("d", _i32),
+        ("total_q", _i64),
+        ("page_size", _i32),
+        ("table_width", _i32),
+        ("pages", _i64),
+        ("block_table", _ptr),
+        ("table_stride", _i64),
+        ("lengths", _ptr),
+        ("top", _i32),
+        ("first", _i32),
+        ("last", _i32),
+        ("q", _ptr),
+        ("q_strides", _i64 * 3),
+        ("cu_seqlens_q", _ptr),
+        ("bounds", _ptr),
+        ("bounds_strides", _i64 * 3),
+        ("chosen", _ptr),
+        ("keys", _ptr),
+        ("workspace", _ptr),
+        ("workspace_bytes", _i64),
+    ]
+
+
 def sources():
     return sorted(
         os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".cu")
@@ -437,6 +530,17 @@ def lib():
     handle.ktt_b200_paged_sdpa_workspace.argtypes = [ctypes.POINTER(PagedSdpaArgs)]
     handle.ktt_b200_paged_sdpa_workspace.restype = _i64
     handle.ktt_b200_paged_sdpa.argtypes = [ctypes.POINTER(PagedSdpaArgs), _ptr]
+    handle.ktt_b200_rotary_axes.argtypes = [ctypes.POINTER(RotaryArgs), ctypes.POINTER(Axes), _ptr]
+    handle.ktt_b200_paged_reserve.argtypes = [ctypes.POINTER(Tables), _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr]
+    handle.ktt_b200_paged_release.argtypes = [ctypes.POINTER(Tables), _ptr, _ptr]
+    handle.ktt_b200_paged_append_at.argtypes = [ctypes.POINTER(AppendAtArgs), _ptr]
+    handle.ktt_b200_paged_bounds.argtypes = [ctypes.POINTER(BoundsArgs), _ptr]
+    handle.ktt_b200_paged_select_workspace.argtypes = [ctypes.POINTER(SelectArgs)]
+    handle.ktt_b200_paged_select_workspace.restype = _i64
+    handle.ktt_b200_paged_select.argtypes = [ctypes.POINTER(SelectArgs), _ptr]
+    handle.ktt_b200_paged_sdpa_chosen_workspace.argtypes = [ctypes.POINTER(PagedSdpaArgs)]
+    handle.ktt_b200_paged_sdpa_chosen_workspace.restype = _i64
+    handle.ktt_b200_paged_sdpa_chosen.argtypes = [ctypes.POINTER(PagedSdpaArgs), _ptr]
     if handle.ktt_b200_abi_version() != 1:
         raise RuntimeError("kohaku_tt_b200: libktt_b200.so has another ABI version")
     _LIB = handle

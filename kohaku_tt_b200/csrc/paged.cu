@@ -1,8 +1,7 @@
 // The paged cache: appending rows (with the rotation of the keys and of the step's queries) and reading it back.
 #include <type_traits>
 
-#include "paged.cuh"
-#include "rotary.cuh"
+#include "four_bits.cuh"
 
 namespace ktt {
 
@@ -51,14 +50,20 @@ struct AppendParams {
     int32_t* lengths_out;
     int vec;
 };
+// With positions of their own, and with bounds that a key of a sequence goes into on the way (one row for each sequence).
+struct AppendAtParams : AppendParams {
+    Placed positions;
+    PairAxes axes;
+    Bounds bounds;
+};
 
 // Eight columns of one token in the cache's 4 bits. The 8 threads of a group of 64 columns are neighbours in a warp and
-// all arrive here; `there`: the row has a place. The codes are those of (x - least) / step rounded as fp32 does, to the
+// all arrive here; `there`: the row has a place. Returns the codes and (step, least). The codes are those of (x - least) / step rounded as fp32 does, to the
 // bit: the quotient is the product with 1 / step, corrected by its remainder (Markstein's theorem: with 1 / step correctly
 // rounded and the remainder exact, the corrected quotient is the correctly rounded one), 6 operations for a column where a
 // division takes some 12; a power of two keeps steps near the ends of fp32's range from taking the remainder out of it.
 template <int D>
-__device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, unsigned char* block, bool value, int token, int chunk, bool there) {
+__device__ __forceinline__ uint2 put_four_bits(const Eight<__nv_bfloat16>& x, unsigned char* block, bool value, int token, int chunk, bool there) {
     const __nv_bfloat162* pair = reinterpret_cast<const __nv_bfloat162*>(x.raw);
     const __nv_bfloat162 lo = __hmin2_nan(__hmin2_nan(pair[0], pair[1]), __hmin2_nan(pair[2], pair[3]));
     const __nv_bfloat162 hi = __hmax2_nan(__hmax2_nan(pair[0], pair[1]), __hmax2_nan(pair[2], pair[3]));
@@ -89,18 +94,19 @@ __device__ __forceinline__ void put_four_bits(const Eight<__nv_bfloat16>& x, uns
     // values as far as 22 steps from the least, whose code is 15. (Else all codes are 0.)
     if (s >= 0x1p-126f && s < INFINITY) encode(std::false_type());
     else if (s > 0.f && s < INFINITY) encode(std::true_type());
-    if (!there) return;
+    const uint2 held = make_uint2(word, static_cast<uint32_t>(__bfloat16_as_ushort(step)) | static_cast<uint32_t>(__bfloat16_as_ushort(__low2bfloat16(ends))) << 16);
+    if (!there) return held;
     uint32_t* to = reinterpret_cast<uint32_t*>(block);
-    to[value ? value_word<D>(token, chunk) : key_word<D>(token, chunk)] = word;
-    if (chunk % 8 == 0) {
-        to[step_word<D>(token, chunk / 8)] = static_cast<uint32_t>(__bfloat16_as_ushort(step)) | static_cast<uint32_t>(__bfloat16_as_ushort(__low2bfloat16(ends))) << 16;
-    }
+    to[value ? value_word<D>(token, chunk) : key_word<D>(token, chunk)] = held.x;
+    if (chunk % 8 == 0) to[step_word<D>(token, chunk / 8)] = held.y;
+    return held;
 }
 
 // A thread has eight columns of kHeads heads of one token: of queries, keys or values. Its rows are requested before it
 // knows where they go (a packed row's sequence takes a search). No thread leaves before the groups' shuffles.
-template <int D, int kBits, bool kFast, int kHeads>
-__global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const __grid_constant__ AppendParams p) {
+template <int D, int kBits, bool kFast, int kHeads, typename Params>
+__global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const __grid_constant__ Params p) {
+    constexpr bool kAt = std::is_same_v<Params, AppendAtParams>;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const int chunk = threadIdx.x, col = chunk * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -166,7 +172,17 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
     const int64_t pos = row_there ? cached + in : 0;
     Turned<kFast> turned;
     turned.count = 0;
-    if (what != 2 && row_there) turned.load(p.turn, pos, col);
+    if constexpr (kAt) {
+        if (what != 2 && row_there) {
+            // (Packed rows have one batch entry's positions; without any, the place is the only axis, and all pairs are of axis 0.)
+            Positions<true> at = {};
+            if (p.positions.at) at = p.positions.all(p.axes.axes, p.cu ? 0 : b, r);
+            else at.at[0] = pos;
+            turned.load(p.turn, p.axes, at, col);
+        }
+    } else {
+        if (what != 2 && row_there) turned.load(p.turn, pos, col);
+    }
     if (what == 0) {
         if (!row_there) return;
         __nv_bfloat16* to = p.q_out + (p.cu ? 0 : b * p.qos[0]) + r * p.qos[2] + col;
@@ -193,7 +209,25 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
             if (there) x[i].store(reinterpret_cast<__nv_bfloat16*>(to + at * (what == 2 ? p.c.vs[2] : p.c.ks[2])) + col);
         } else {
             if (there) to += static_cast<int64_t>(at >> 4) * (9 * D);
-            put_four_bits<D>(x[i], to, what == 2, at & 15, chunk, there);
+            const uint2 held = put_four_bits<D>(x[i], to, what == 2, at & 15, chunk, there);
+            if constexpr (kAt) {
+                if (p.bounds.at && what == 1) x[i] = of_four_bits(held.x, held.y);
+            }
+        }
+        if constexpr (kAt) {
+            // The sequence's only new key: no other thread has these channels of its page's bounds.
+            if (p.bounds.at && what == 1 && there) {
+                Edges e = {x[i], x[i]};
+                __nv_bfloat16 *lo = p.bounds.edge(page, h0 + i, 0) + col, *hi = p.bounds.edge(page, h0 + i, 1) + col;
+                if (at > 0) {
+                    Edges old;
+                    old.lo.load(lo);
+                    old.hi.load(hi);
+                    e.with(old.lo, old.hi);
+                }
+                e.lo.store(lo);
+                e.hi.store(hi);
+            }
         }
     }
 }
@@ -206,22 +240,6 @@ struct ReadParams {
     __nv_bfloat16* v;
     int64_t ks[3], vs[3];
 };
-
-// What eight codes are worth: bf16 products and sums of pairs, rounded once. (An fp32 sum rounded to bf16 would be the same but where the
-// least value is under 2^-19 of the step: the sum then drops it, and a product that lies halfway between two bf16 values goes to the even one
-// instead of to the side that the least value is on.)
-__device__ __forceinline__ Eight<__nv_bfloat16> of_four_bits(uint32_t word, uint32_t pair) {
-    const __nv_bfloat162 ends = *reinterpret_cast<const __nv_bfloat162*>(&pair), step = __low2bfloat162(ends), least = __high2bfloat162(ends);
-    const __nv_bfloat162 zero = __float2bfloat162_rn(128.f);
-    Eight<__nv_bfloat16> x;
-    __nv_bfloat162* to = reinterpret_cast<__nv_bfloat162*>(x.raw);
-#pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const uint32_t two = ((word >> (4 * n)) & 0x000f000fu) | 0x43004300u;   // two codes as bf16 128 + c
-        to[n] = __hfma2(step, __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&two), zero), least);
-    }
-    return x;
-}
 
 // The same in fp16, of a step and a least value times a power of two that leaves none of the sums at 2^15 or above. Both have 8 bits, so
 // they are fp16's too but where they are under 2^-17, which is nothing beside 2^15; the sums are rounded once, by 2^-11 of them at most.
@@ -409,23 +427,9 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ ReadP
     }
 }
 
-template <typename Params>
-int launch_dependent(void (*kernel)(Params), const Params& p, dim3 grid, dim3 block, cudaStream_t stream, const char* what) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), what);
-}
-
-template <int D, int kBits>
-int launch_append(const AppendParams& given, cudaStream_t stream) {
-    AppendParams p = given;
+template <int D, int kBits, typename Params>
+int launch_append(const Params& given, cudaStream_t stream) {
+    Params p = given;
     const dim3 block(D / 8, 256 / (D / 8));
     const int64_t blocks = (p.tokens + block.y - 1) / block.y;   // one at least: it writes the new lengths
     auto go = [&](auto kernel, int per) {
@@ -438,11 +442,11 @@ int launch_append(const AppendParams& given, cudaStream_t stream) {
     // them. 10,240 packed tokens, 32 heads over 8, D 128, us for 1, 2, 4 and 8 heads: bf16 pages 94.8, 69.7, 51.3, 48.4
     // (4.9 TB/s at 4); 4 bits 102.6, 77.3, 60.1, 58.6, of which keys and values 28 (queries alone run at a copy's rate).
     if (p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads) >= 4 * 148 * 2048) {
-        if (fast) return go(append_kernel<D, kBits, true, 4>, 4);
-        return go(append_kernel<D, kBits, false, 4>, 4);
+        if (fast) return go(append_kernel<D, kBits, true, 4, Params>, 4);
+        return go(append_kernel<D, kBits, false, 4, Params>, 4);
     }
-    if (fast) return go(append_kernel<D, kBits, true, 1>, 1);
-    return go(append_kernel<D, kBits, false, 1>, 1);
+    if (fast) return go(append_kernel<D, kBits, true, 1, Params>, 1);
+    return go(append_kernel<D, kBits, false, 1, Params>, 1);
 }
 
 template <int D, int kBits>
@@ -480,9 +484,13 @@ int read_pages(const Pages& c, int bits, int d, int batch, int kv_heads, int row
 
 using namespace ktt;
 
-extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream) {
+namespace {
+
+// The checks of an append and its parameters; go: whether there is anything to launch.
+template <typename Params>
+int fill(Params& p, const ktt_b200_append_args* a, bool& go) {
+    go = false;
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: null arguments");
-    AppendParams p = {};
     if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: %s", why);
     if (a->batch < 1 || a->rows < 0 || a->heads < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: sizes must be positive");
     if (a->heads > 32768) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: at most 32768 heads");
@@ -518,11 +526,51 @@ extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream
     p.vec = vec;
     p.cu = a->cu_seqlens;
     p.lengths_out = a->lengths_out;
-    if (p.tokens == 0 && !p.lengths_out) return 0;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->cache.bits == 16) return a->d == 64 ? launch_append<64, 16>(p, st) : launch_append<128, 16>(p, st);
-    return a->d == 64 ? launch_append<64, 4>(p, st) : launch_append<128, 4>(p, st);
+    go = p.tokens > 0 || p.lengths_out;
+    return 0;
 }
+
+template <typename Params>
+int launch(const Params& p, int bits, int d, cudaStream_t st) {
+    if (bits == 16) return d == 64 ? launch_append<64, 16>(p, st) : launch_append<128, 16>(p, st);
+    return d == 64 ? launch_append<64, 4>(p, st) : launch_append<128, 4>(p, st);
+}
+
+}  // namespace
+
+extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream) {
+    AppendParams p = {};
+    bool go;
+    if (int rc = fill(p, a, go)) return rc;
+    return go ? launch(p, a->cache.bits, a->d, static_cast<cudaStream_t>(stream)) : 0;
+}
+
+extern "C" int ktt_b200_paged_append_at(const ktt_b200_append_at_args* x, void* stream) {
+    if (!x) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: null arguments");
+    const ktt_b200_append_args* a = &x->base;
+    AppendAtParams p = {};
+    bool go;
+    if (int rc = fill(p, a, go)) return rc;
+    if (!go) return 0;
+    p.axes.axes = 1;
+    if (x->positions.positions && a->cos) {
+        if (const char* why = axes_of(p.axes, x->positions, a->pairs)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: %s", why);
+        p.positions = {x->positions.positions, x->positions.positions_are_64, {x->positions.strides[0], x->positions.strides[1], x->positions.strides[2]}};
+    }
+    Bounds bounds = {};
+    if (x->bounds) {
+        if (const char* why = bounds_of(bounds, x->bounds, x->bounds_strides)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: %s", why);
+        if (a->batch > 65535) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: at most 65535 sequences with bounds");
+    }
+    // One new key of each sequence goes into its page's bounds as it passes; of several, those of a page meet in a launch behind this one, which
+    // reads them back.
+    const bool passing = !a->cu_seqlens && a->rows == 1;
+    if (passing) p.bounds = bounds;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (int rc = launch(p, a->cache.bits, a->d, st)) return rc;
+    return bounds.at && !passing ? keep_bounds(p.c, a->cache.bits, a->d, p.kv_heads, bounds, a->batch, a->rows, a->cu_seqlens, st) : 0;
+}
+
 
 extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_read: null arguments");

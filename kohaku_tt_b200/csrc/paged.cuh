@@ -122,4 +122,20 @@ __host__ __device__ inline int parts_of_chunk(int64_t tiles, int blocks, int sms
 // Fills the cache's fields from an argument block after its checks (paged.cu); null, or why not.
 const char* pages_of(Pages& c, const ktt_b200_pages& a, int d);
 
+// A launch that may start while the one before it ends (its kernel waits for that by griddepcontrol).
+template <typename Params>
+int launch_dependent(void (*kernel)(Params), const Params& p, dim3 grid, dim3 block, cudaStream_t stream, const char* what, int smem = 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), what);
+}
+
 }  // namespace ktt

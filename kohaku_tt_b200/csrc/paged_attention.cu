@@ -53,6 +53,7 @@ struct PagedParams {
     int64_t qs[3], os[3];
     const int32_t* cu;       // packed queries
     int64_t total_q;
+    int own_heads, entry0;   // kOwn: K / V heads of the cache, and the first entry of this launch
     int2* pieces;            // [pairs] the first CTA of a pair, and how many have a piece of it (1: its result is written)
     float2* part_ml;         // [slots][16] maximum and sum
     float* part_o;           // [slots][16][D]
@@ -133,8 +134,26 @@ constexpr uint32_t kTwelve = 0x41404140u;   // bf16 12, twice
 // The reference of a column that has seen no key: below every logit.
 constexpr float kNoKey = -3.0e38f;
 
+// kOwn: a batch entry is a query token and K / V head with a table and a length of its own; sq are the tokens of a row of q's batch.
+struct Owner {
+    int b, s, hk;   // of q: batch entry and row; K / V head
+};
+__device__ __forceinline__ Owner owner_of(const PagedParams& p, int entry) {
+    const uint32_t n = static_cast<uint32_t>(p.entry0) + static_cast<uint32_t>(entry), token = n / static_cast<uint32_t>(p.own_heads);
+    Owner x;
+    x.hk = static_cast<int>(n - token * p.own_heads);
+    x.b = static_cast<int>(token / static_cast<uint32_t>(p.sq));
+    x.s = static_cast<int>(token - static_cast<uint32_t>(x.b) * p.sq);
+    return x;
+}
+
 // Rows of a sequence's queries: how many tokens, and where they start.
+template <bool kOwn>
 __device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& first) {
+    if constexpr (kOwn) {
+        first = 0;
+        return 1;
+    }
     if (!p.cu) {
         first = 0;
         return p.sq;
@@ -145,26 +164,34 @@ __device__ __forceinline__ int tokens_of(const PagedParams& p, int b, int64_t& f
 }
 
 // One normalised chunk of 4 columns of (pair, row of its tile).
+template <bool kOwn>
 __device__ __forceinline__ void write_row(const PagedParams& p, int b, int vh, int row_in_tile, int tile_rows, int c4, float4 sum, float ll) {
     const float inv = ll > 0.f ? 1.f / ll : (ll == 0.f ? 0.f : ll);   // (a NaN stays one)
     const int hk = vh / p.row_tiles, row = (vh - hk * p.row_tiles) * tile_rows + row_in_tile;
     int64_t first;
-    const int n = tokens_of(p, b, first);
+    const int n = tokens_of<kOwn>(p, b, first);
     const int gi = row / n, tq = row - gi * n;
-    __nv_bfloat16* to = p.out + (p.cu ? 0 : b * p.os[0]) + (hk * p.group + gi) * p.os[1] + (first + tq) * p.os[2] + c4 * 4;
+    __nv_bfloat16* to;
+    if constexpr (kOwn) {
+        const Owner x = owner_of(p, b);
+        to = p.out + x.b * p.os[0] + (x.hk * p.group + row) * p.os[1] + x.s * p.os[2] + c4 * 4;
+    } else {
+        to = p.out + (p.cu ? 0 : b * p.os[0]) + (hk * p.group + gi) * p.os[1] + (first + tq) * p.os[2] + c4 * 4;
+    }
     uint2 packed;
     packed.x = pack_bf16(sum.x * inv, sum.y * inv);
     packed.y = pack_bf16(sum.z * inv, sum.w * inv);
     *reinterpret_cast<uint2*>(to) = packed;
 }
 // Rows that a pair has in its tile.
+template <bool kOwn>
 __device__ __forceinline__ int rows_of(const PagedParams& p, int b, int vh, int tile_rows) {
     int64_t first;
-    const int all = p.group * tokens_of(p, b, first);
+    const int all = p.group * tokens_of<kOwn>(p, b, first);
     return max(min(all - (vh % p.row_tiles) * tile_rows, tile_rows), 0);
 }
 
-template <int D, int kBits, int NT, bool kCluster>
+template <int D, int kBits, int NT, bool kCluster, bool kOwn>
 __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBits, NT>::kCtas)) paged_kernel(const __grid_constant__ PagedParams p) {
     using S = Shape<D, kBits, NT>;
     constexpr int W = S::W, NS = S::NS, NB = S::NB, PB = S::PB, kRows = S::kRows, kThreads = S::kThreads;
@@ -236,7 +263,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
     auto issue = [&](int st, int count) {
         const Cursor& c = prod.c;
         if (at + count > 32) {   // (a batch's blocks are in one lot)
-            const int block = prod.pos + lane, hk = c.hk / p.row_tiles;
+            const int block = prod.pos + lane, hk = kOwn ? owner_of(p, c.b).hk : c.hk / p.row_tiles;
             k_at = v_at = nullptr;
             if (block < prod.end && static_cast<int64_t>(block) * 16 < c.len) {
                 const int entry = block / p.page_blocks, row = (block - entry * p.page_blocks) * (kBits == 16 ? 16 : 1);
@@ -318,7 +345,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
         {
             const int hk = cons.c.hk / p.row_tiles, row0 = (cons.c.hk - hk * p.row_tiles) * kRows;
             int64_t first;
-            const int n = tokens_of(p, cons.c.b, first), rows = p.group * n;
+            const int n = tokens_of<kOwn>(p, cons.c.b, first), rows = p.group * n;
             kend = min(cons.c.len, cons.end * 16);
             whole = min(p.causal ? cons.c.len - n : cons.c.len - 1, kend - 1);
 #pragma unroll
@@ -327,7 +354,13 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 const bool ok = r < rows;
                 const int gi = ok ? r / n : 0, tq = ok ? r - gi * n : 0;
                 // (A row past the last reads the first and is zeroed after; without any row at all nothing is read.)
-                const __nv_bfloat16* from = p.q + (p.cu ? 0 : cons.c.b * p.qs[0]) + (hk * p.group + gi) * p.qs[1] + (rows > 0 ? first + tq : 0) * p.qs[2];
+                const __nv_bfloat16* from;
+                if constexpr (kOwn) {
+                    const Owner x = owner_of(p, cons.c.b);
+                    from = p.q + x.b * p.qs[0] + (x.hk * p.group + gi) * p.qs[1] + x.s * p.qs[2];
+                } else {
+                    from = p.q + (p.cu ? 0 : cons.c.b * p.qs[0]) + (hk * p.group + gi) * p.qs[1] + (rows > 0 ? first + tq : 0) * p.qs[2];
+                }
                 if constexpr (kBits == 16) {
 #pragma unroll
                     for (int kk = 0; kk < MT; ++kk) {
@@ -661,14 +694,14 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 }
                 return sum;
             };
-            const int rows = rows_of(p, cons.c.b, cons.c.hk, kRows);
+            const int rows = rows_of<kOwn>(p, cons.c.b, cons.c.hk, kRows);
             if constexpr (kCluster) {
                 for (int idx = threadIdx.x; idx < rows * (D / 4); idx += kThreads) {
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
                     float mm, ll;
                     const float4 sum = merged(r, c4, mm, ll);
                     if (ranks_used == 1) {
-                        write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
+                        write_row<kOwn>(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
                         continue;
                     }
                     reinterpret_cast<float4*>(part_s)[idx] = sum;
@@ -687,7 +720,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                     const int r = idx / (D / 4), c4 = idx % (D / 4);
                     float mm, ll;
                     const float4 sum = merged(r, c4, mm, ll);
-                    write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
+                    write_row<kOwn>(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
                 }
             } else {
                 const int slot = slot_of(blockIdx.x, c_first == static_cast<int>(blockIdx.x));
@@ -709,7 +742,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
         if (ranks_used == 1) return;   // one rank had all of it and has written it: nobody waits for anybody
         cluster_meet();
         // Every rank adds up its share of the output, the ranks that had a tile in their order.
-        const int rows = rows_of(p, cons.c.b, cons.c.hk, kRows);
+        const int rows = rows_of<kOwn>(p, cons.c.b, cons.c.hk, kRows);
         const int parts = ranks_used, all = rows * (D / 4), share = (all + p.ranks - 1) / p.ranks;
         const uint32_t at_m = smem_u32(fin_m), at_l = smem_u32(fin_l), at_o = smem_u32(part_s);
         for (int idx = rank * share + threadIdx.x; idx < min((rank + 1) * share, all); idx += kThreads) {
@@ -734,7 +767,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
                 sum.x = fmaf(v[j].x, f, sum.x); sum.y = fmaf(v[j].y, f, sum.y);
                 sum.z = fmaf(v[j].z, f, sum.z); sum.w = fmaf(v[j].w, f, sum.w);
             }
-            write_row(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
+            write_row<kOwn>(p, cons.c.b, cons.c.hk, r, kRows, c4, sum, ll);
         }
         cluster_meet();   // nobody's shared memory goes away while another reads it
     }
@@ -744,7 +777,7 @@ __global__ void __launch_bounds__((Shape<D, kBits, NT>::kThreads), (Shape<D, kBi
 // threads share four columns, each with every fourth partial, eight requested at a time. (A launch of its own, which starts
 // up while the stream drains: a last holder that adds them up behind a ticket keeps registers from the stream, whose
 // instructions were 30 % more for it.)
-template <int D>
+template <int D, bool kOwn>
 __global__ void __launch_bounds__(2 * D) merge_kernel(const __grid_constant__ PagedParams p, int tile_rows) {
     __shared__ float4 sums[2][4][D / 4];
     __shared__ float2 stats[2][4];
@@ -754,7 +787,7 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const __grid_constant__ Pa
     const int2 piece = p.pieces[pair];
     if (piece.y <= 1) return;
     const int b = pair / p.kv_heads, vh = pair - b * p.kv_heads;
-    const bool there = r < rows_of(p, b, vh, tile_rows);
+    const bool there = r < rows_of<kOwn>(p, b, vh, tile_rows);
     float mm = kNoKey, ll = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int kAhead = 8;
@@ -805,7 +838,7 @@ __global__ void __launch_bounds__(2 * D) merge_kernel(const __grid_constant__ Pa
         sum.x = fmaf(v.x, w, sum.x); sum.y = fmaf(v.y, w, sum.y);
         sum.z = fmaf(v.z, w, sum.z); sum.w = fmaf(v.w, w, sum.w);
     }
-    write_row(p, b, vh, r, tile_rows, c4, sum, ll);
+    write_row<kOwn>(p, b, vh, r, tile_rows, c4, sum, ll);
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -844,14 +877,14 @@ cudaLaunchConfig_t paged_config(int ctas, int ranks, cudaStream_t stream, cudaLa
 }
 
 // Clusters of `ranks` CTAs that run at the same time on the current device; asked for once. -1: no answer now.
-template <int D, int kBits, int NT>
+template <int D, int kBits, int NT, bool kOwn>
 int cluster_room(int dev, int ranks) {
     static std::atomic<int> known[64][4];   // by log2 of the ranks
     if (dev < 0) return -1;
     int log = 0;
     while ((1 << log) < ranks) ++log;
     return kept(known[dev][log], [&]() {
-        auto kernel = paged_kernel<D, kBits, NT, true>;
+        auto kernel = paged_kernel<D, kBits, NT, true, kOwn>;
         cudaLaunchAttribute attr[1];
         cudaLaunchConfig_t cfg = paged_config<D, kBits, NT, true>(ranks, ranks, nullptr, attr);
         int n = 0;
@@ -863,16 +896,16 @@ int cluster_room(int dev, int ranks) {
 }
 
 // Set up once per device, by the first call of whatever size: both kernels' limits and the room for clusters.
-template <int D, int kBits, int NT>
+template <int D, int kBits, int NT, bool kOwn>
 int paged_set_up(int dev) {
     static std::atomic<int> done[64];
     int rc = 0;
-    auto shares = [&]() { return rc = ensure_smem(paged_kernel<D, kBits, NT, false>, Shape<D, kBits, NT>::smem(false), "cudaFuncSetAttribute(paged)"); };
+    auto shares = [&]() { return rc = ensure_smem(paged_kernel<D, kBits, NT, false, kOwn>, Shape<D, kBits, NT>::smem(false), "cudaFuncSetAttribute(paged)"); };
     if (dev < 0) return shares();
     kept(done[dev], [&]() {
         int least = shares();
         for (int ranks = 1; ranks <= 8; ranks *= 2) {
-            const int room = cluster_room<D, kBits, NT>(dev, ranks);
+            const int room = cluster_room<D, kBits, NT, kOwn>(dev, ranks);
             least = room < least ? room : least;
         }
         return least < 0 ? -1 : 0;
@@ -889,13 +922,13 @@ int paged_set_up(int dev) {
 // 7.3 and 8.0, 16 x 2,048 10.7 and 12.2, 16 x 8,192 19.9 and 17.7, 64 x 1,024 14.2 and 15.2, 64 x 2,048 20.1 and 18.0. Pairs that outnumber the
 // CTAs follow one another, up to 2,048 keys each: 64 x 16 heads, D 64, bf16, 128, 1,024 and 2,048 keys 10.2 and 15.8, 29.0 and 32.8, 52.4 and
 // 57.7; 4 bits 10.3 and 15.9, 24.4 and 28.4, 40.3 and 41.2; 64 x 12, D 128, 4 bits, 2,048 49.1 and 47.9.
-template <int D, int kBits, int NT>
+template <int D, int kBits, int NT, bool kOwn>
 int paged_ranks(int64_t pairs, int cap, int ctas, int dev) {
     constexpr int kTile = 16 * Shape<D, kBits, NT>::W;
     if (pairs > ctas && cap <= 2048) return 1;
     for (int ranks = 8; ranks >= 1; ranks /= 2) {
         if (ranks > 1 && (ranks / 2) * kTile >= cap) continue;   // half as many have a block for every warp
-        if (pairs * ranks > ctas || cluster_room<D, kBits, NT>(dev, ranks) < pairs) continue;
+        if (pairs * ranks > ctas || cluster_room<D, kBits, NT, kOwn>(dev, ranks) < pairs) continue;
         const int64_t used = pairs * ranks, all = ctas, most = 1024ll * ranks;
         return cap <= most && (2 * cap <= most || 4 * cap * all <= 5 * most * used) ? ranks : 0;
     }
@@ -996,14 +1029,14 @@ Plan plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
     return s;
 }
 
-template <int D, int kBits, int NT>
+template <int D, int kBits, int NT, bool kOwn>
 int run_few(PagedParams& p, cudaStream_t stream) {
     using S = Shape<D, kBits, NT>;
     const int dev = current_device();
-    if (int rc = paged_set_up<D, kBits, NT>(dev)) return rc;
+    if (int rc = paged_set_up<D, kBits, NT, kOwn>(dev)) return rc;
     const int ctas = S::kCtas * sm_count(dev);
     const int64_t pairs = static_cast<int64_t>(p.batch) * p.kv_heads;
-    p.ranks = paged_ranks<D, kBits, NT>(pairs, p.c.cap, ctas, dev);
+    p.ranks = paged_ranks<D, kBits, NT, kOwn>(pairs, p.c.cap, ctas, dev);
     cudaLaunchAttribute attr[2];
     auto go = [&](cudaLaunchConfig_t cfg, auto kernel, auto... args) {
         cfg.attrs = attr;
@@ -1012,17 +1045,44 @@ int run_few(PagedParams& p, cudaStream_t stream) {
         ++cfg.numAttrs;
         return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "paged_sdpa launch");
     };
-    if (p.ranks > 0) return go(paged_config<D, kBits, NT, true>(static_cast<int>(pairs) * p.ranks, p.ranks, stream, attr), paged_kernel<D, kBits, NT, true>, p);
-    if (int rc = go(paged_config<D, kBits, NT, false>(ctas, 1, stream, attr), paged_kernel<D, kBits, NT, false>, p)) return rc;
+    if (p.ranks > 0) return go(paged_config<D, kBits, NT, true>(static_cast<int>(pairs) * p.ranks, p.ranks, stream, attr), paged_kernel<D, kBits, NT, true, kOwn>, p);
+    if (int rc = go(paged_config<D, kBits, NT, false>(ctas, 1, stream, attr), paged_kernel<D, kBits, NT, false, kOwn>, p)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(pairs), S::kRows / 2);
     cfg.blockDim = dim3(D / 4, 4, 2);
     cfg.stream = stream;
-    return go(cfg, merge_kernel<D>, p, static_cast<int>(S::kRows));
+    return go(cfg, merge_kernel<D, kOwn>, p, static_cast<int>(S::kRows));
 }
 
-template <int D, int kBits>
-int run_few(PagedParams& p, int nt, cudaStream_t stream) { return nt == 1 ? run_few<D, kBits, 1>(p, stream) : run_few<D, kBits, 2>(p, stream); }
+// Tables of each token's and head's own: entries (token, K / V head) of one query token each, by the pass.
+struct OwnPlan {
+    int nt, row_tiles;
+    int64_t entries, slice, bytes;
+};
+OwnPlan own_plan_of(const ktt_b200_paged_sdpa_args* a, const Pages& c, int sms) {
+    OwnPlan s = {};
+    const int64_t group = a->heads / a->cache.kv_heads;
+    s.nt = group <= 8 ? 1 : 2;
+    s.row_tiles = static_cast<int>((group + 8 * s.nt - 1) / (8 * s.nt));
+    s.entries = static_cast<int64_t>(a->batch) * a->sq * a->cache.kv_heads;
+    // Units of all pairs of a launch have to fit 30 bits, and the scan of their lengths shared memory. Where they outnumber the CTAs and follow
+    // one another whole (paged_ranks) nothing is scanned, and a launch has as many as there are.
+    int64_t most = (1ll << 30) / ((static_cast<int64_t>(c.cap) / 16 + 32) * s.row_tiles);
+    if (most < 1) most = 1;
+    const bool whole = c.cap <= 2048 && s.entries * s.row_tiles > 4ll * sms;
+    const int64_t scanned = most < kMaxBatch ? most : kMaxBatch, all = whole ? s.entries : scanned;
+    s.slice = s.entries < all ? s.entries : all;
+    s.bytes = parts_of((s.slice < scanned ? s.slice : scanned) * s.row_tiles, a->d, sms * 4).total;
+    return s;
+}
+
+template <int D, int kBits, bool kOwn>
+int run_few(PagedParams& p, int nt, cudaStream_t stream) { return nt == 1 ? run_few<D, kBits, 1, kOwn>(p, stream) : run_few<D, kBits, 2, kOwn>(p, stream); }
+template <bool kOwn>
+int run_few(PagedParams& p, int bits, int d, int nt, cudaStream_t stream) {
+    if (bits == 16) return d == 64 ? run_few<64, 16, kOwn>(p, nt, stream) : run_few<128, 16, kOwn>(p, nt, stream);
+    return d == 64 ? run_few<64, 4, kOwn>(p, nt, stream) : run_few<128, 4, kOwn>(p, nt, stream);
+}
 
 const char* sdpa_refusal(const ktt_b200_paged_sdpa_args* a, Pages& c) {
     if (const char* why = pages_of(c, a->cache, a->d)) return why;
@@ -1323,10 +1383,82 @@ extern "C" int ktt_b200_paged_sdpa(const ktt_b200_paged_sdpa_args* a, void* stre
         p.cu = a->cu_seqlens_q ? a->cu_seqlens_q + b0 : nullptr;
         p.q = static_cast<const __nv_bfloat16*>(a->q) + (p.cu ? 0 : b0 * a->q_strides[0]);
         p.out = static_cast<__nv_bfloat16*>(a->out) + (p.cu ? 0 : b0 * a->out_strides[0]);
-        int rc;
-        if (a->cache.bits == 16) rc = a->d == 64 ? run_few<64, 16>(p, s.nt, st) : run_few<128, 16>(p, s.nt, st);
-        else rc = a->d == 64 ? run_few<64, 4>(p, s.nt, st) : run_few<128, 4>(p, s.nt, st);
-        if (rc) return rc;
+        if (int rc = run_few<false>(p, a->cache.bits, a->d, s.nt, st)) return rc;
+    }
+    return 0;
+}
+
+namespace {
+
+const char* chosen_refusal(const ktt_b200_paged_sdpa_args* a, Pages& c) {
+    if (const char* why = sdpa_refusal(a, c)) return why;
+    if (a->cu_seqlens_q) return "packed tokens are one batch entry here";
+    // (a row tile of a K / V head has 8 query heads at least, or all of them; so that a launch has all pairs)
+    if (static_cast<int64_t>(a->batch) * a->sq * (a->cache.kv_heads + a->heads / 8) > (1ll << 28)) return "at most 2^28 pairs of a token and a K / V head";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" int64_t ktt_b200_paged_sdpa_chosen_workspace(const ktt_b200_paged_sdpa_args* a) {
+    Pages c = {};
+    if (!a || a->batch < 1 || a->sq < 0) {
+        fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: sizes must be positive");
+        return -1;
+    }
+    if (const char* why = chosen_refusal(a, c)) {
+        fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: %s", why);
+        return -1;
+    }
+    return a->sq == 0 ? 0 : own_plan_of(a, c, sm_count(current_device())).bytes;
+}
+
+extern "C" int ktt_b200_paged_sdpa_chosen(const ktt_b200_paged_sdpa_args* a, void* stream) {
+    if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null arguments");
+    PagedParams p = {};
+    if (a->batch < 1 || a->sq < 0) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: sizes must be positive");
+    if (const char* why = chosen_refusal(a, p.c)) {
+        note_call(4);
+        return fail(KTT_B200_ERR_UNSUPPORTED, "paged_sdpa: %s", why);
+    }
+    if (a->sq == 0) return 0;
+    if (!a->cache.k || !a->cache.v || !a->cache.block_table || !a->cache.lengths || !a->q || !a->out) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: null pointer");
+    }
+    if (a->q == a->out) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: out must not overlap q");
+    const OwnPlan s = own_plan_of(a, p.c, sm_count(current_device()));
+    if (!a->workspace || a->workspace_bytes < s.bytes) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: workspace holds %lld bytes, %lld needed", static_cast<long long>(a->workspace_bytes), static_cast<long long>(s.bytes));
+    }
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_sdpa: the workspace must be 16-byte aligned");
+    p.q = static_cast<const __nv_bfloat16*>(a->q);
+    p.out = static_cast<__nv_bfloat16*>(a->out);
+    p.heads = a->heads;
+    p.row_tiles = p.kv_heads = s.row_tiles;
+    p.own_heads = a->cache.kv_heads;
+    p.group = a->heads / a->cache.kv_heads;
+    p.sq = a->sq;
+    p.page_blocks = a->cache.page_size / 16;
+    p.table_width = a->cache.table_width;
+    p.scale_log2 = a->scale * kLog2e;
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = a->q_strides[i];
+        p.os[i] = a->out_strides[i];
+    }
+    const int64_t scanned = s.slice < kMaxBatch ? s.slice : kMaxBatch;
+    const Parts parts = parts_of(scanned * s.row_tiles, a->d, sm_count(current_device()) * 4);
+    unsigned char* base = static_cast<unsigned char*>(a->workspace);
+    p.pieces = reinterpret_cast<int2*>(base);
+    p.part_ml = reinterpret_cast<float2*>(base + parts.piece_bytes);
+    p.part_o = reinterpret_cast<float*>(base + parts.piece_bytes + parts.ml_bytes);
+    const Pages all = p.c;
+    note_call(3);
+    for (int64_t e0 = 0; e0 < s.entries; e0 += s.slice) {
+        p.batch = static_cast<int>(s.entries - e0 < s.slice ? s.entries - e0 : s.slice);
+        p.entry0 = static_cast<int>(e0);
+        p.c.table = all.table + e0 * all.table_stride;
+        p.c.lengths = all.lengths + e0;
+        if (int rc = run_few<true>(p, a->cache.bits, a->d, s.nt, static_cast<cudaStream_t>(stream))) return rc;
     }
     return 0;
 }

@@ -1,9 +1,22 @@
 // Rotary positions: the tables of cosines and sines, and the rotation of queries and keys (its gradient too).
 #include <cmath>
+#include <type_traits>
 
 #include "rotary.cuh"
 
 namespace ktt {
+
+const char* axes_of(PairAxes& x, const ktt_b200_axes& given, int pairs) {
+    if (given.axes < 1 || given.axes > kMaxAxes) return "positions have 1 to 4 axes";
+    if (!given.positions || (!given.of_pair && given.axes > 1)) return "null pointer";
+    x.axes = given.axes;
+    for (int i = 0; i < pairs && given.of_pair; ++i) {
+        if (given.of_pair[i] >= given.axes) return "a pair's axis must be one of the positions'";
+        x.of[i >> 4] |= static_cast<uint32_t>(given.of_pair[i]) << (2 * (i & 15));
+    }
+    return nullptr;
+}
+
 namespace {
 
 // ---- tables ----------------------------------------------------------------------------------
@@ -166,16 +179,17 @@ struct RotaryParams {
     int64_t tokens;          // of all batch entries
     int rows;                // of one
     int d;
-    const void* positions;   // null: the row
-    int wide_positions;      // int64, else int32
-    int64_t ps[2];           // (batch, row) strides
+    Placed positions;        // none: the row
     int vec;                 // rows may be read and written in 16-byte pieces
+};
+struct RotaryAxesParams : RotaryParams {
+    PairAxes axes;
 };
 
 // A thread turns eight columns of kHeads heads of one token: the table is read once for all of them. A thread reads
 // its partner columns too (its neighbour in the block brings the same line, so they come from L1).
-template <typename T, bool kFast, int kHeads>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+template <typename T, bool kFast, int kHeads, typename Params>
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Params p) {
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const int col = threadIdx.x * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -185,13 +199,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     const int h0 = (static_cast<int>(blockIdx.y) - (which ? p.groups[0] : 0)) * kHeads;
     const uint32_t entry = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows);   // (2^31 tokens at most)
     const int64_t b = entry, r = static_cast<uint32_t>(n) - entry * static_cast<uint32_t>(p.rows);
-    int64_t pos = r;
-    if (p.positions) {
-        const int64_t at = b * p.ps[0] + r * p.ps[1];
-        pos = p.wide_positions ? static_cast<const int64_t*>(p.positions)[at] : static_cast<const int32_t*>(p.positions)[at];
-    }
     Turned<kFast> turned;
-    turned.load(p.turn, pos, col);
+    if constexpr (std::is_same_v<Params, RotaryAxesParams>) turned.load(p.turn, p.axes, p.positions.all(p.axes.axes, b, r), col);
+    else turned.load(p.turn, p.positions.at ? p.positions.get(0, b, r) : r, col);
     const T* x = static_cast<const T*>(p.x[which]) + b * p.xs[which][0] + r * p.xs[which][2];
     T* y = static_cast<T*>(p.y[which]) + b * p.ys[which][0] + r * p.ys[which][2];
     const int left = p.d - col;
@@ -216,9 +226,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
 
 constexpr int64_t kManyThreads = 4 * 148 * 2048;
 
-template <typename T>
-int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
-    RotaryParams p = given;
+template <typename T, typename Params>
+int launch_rotary(const Params& given, cudaStream_t stream) {
+    Params p = given;
     const int chunks = (p.d + 7) / 8;
     const int tokens_per_block = 256 / chunks > 0 ? 256 / chunks : 1;
     const int64_t blocks = (p.tokens + tokens_per_block - 1) / tokens_per_block;
@@ -242,11 +252,11 @@ int launch_rotary(const RotaryParams& given, cudaStream_t stream) {
     // Where the pairs of the half layout are no multiple of 8 a thread goes for its columns' partners one by one, and reads the tables so:
     // 4 x 16 heads x 4,096, D 128, bf16, all columns turning 25.1, 20 or 40 of them 38.6; neighbours 24.3, and 26.3 with 20 columns.
     if (p.tokens * chunks * (p.heads[0] + p.heads[1]) >= kManyThreads) {
-        if (fast) return go(rotary_kernel<T, true, 4>, 4);
-        return go(rotary_kernel<T, false, 4>, 4);
+        if (fast) return go(rotary_kernel<T, true, 4, Params>, 4);
+        return go(rotary_kernel<T, false, 4, Params>, 4);
     }
-    if (fast) return go(rotary_kernel<T, true, 1>, 1);
-    return go(rotary_kernel<T, false, 1>, 1);
+    if (fast) return go(rotary_kernel<T, true, 1, Params>, 1);
+    return go(rotary_kernel<T, false, 1, Params>, 1);
 }
 
 }  // namespace
@@ -308,7 +318,12 @@ extern "C" int ktt_b200_rotary_table(float* cos, float* sin, int64_t positions, 
     return check_cuda(cudaGetLastError(), "rotary_table launch");
 }
 
-extern "C" int ktt_b200_rotary(const ktt_b200_rotary_args* a, void* stream) {
+namespace {
+
+// The checks of a rotation and its parameters; go: whether there is anything to launch.
+template <typename Params>
+int fill(Params& p, const ktt_b200_rotary_args* a, bool& go) {
+    go = false;
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: null arguments");
     if (a->batch < 0 || a->rows < 0 || a->heads < 1 || a->kv_heads < 0 || a->d < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: sizes must be positive");
     if (a->d > 1024) return fail(KTT_B200_ERR_UNSUPPORTED, "rotary: head dims above 1024 are not taken");
@@ -321,7 +336,6 @@ extern "C" int ktt_b200_rotary(const ktt_b200_rotary_args* a, void* stream) {
     if (!a->q || !a->q_out || !a->cos || !a->sin || (a->kv_heads && (!a->k || !a->k_out))) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: null pointer");
     if (a->table_rows < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: the tables have no rows");
     if (a->q == a->q_out || (a->kv_heads && a->k == a->k_out)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: outputs must not overlap inputs");
-    RotaryParams p = {};
     p.turn = {a->cos, a->sin, a->table_stride, a->table_rows, a->pairs, a->interleaved, a->inverse};
     p.x[0] = a->q; p.x[1] = a->k;
     p.y[0] = a->q_out; p.y[1] = a->k_out;
@@ -339,12 +353,36 @@ extern "C" int ktt_b200_rotary(const ktt_b200_rotary_args* a, void* stream) {
     p.tokens = tokens;
     p.rows = a->rows;
     p.d = a->d;
-    p.positions = a->positions;
-    p.wide_positions = a->positions_are_64;
-    p.ps[0] = a->position_strides[0]; p.ps[1] = a->position_strides[1];
+    p.positions = {a->positions, a->positions_are_64, {0, a->position_strides[0], a->position_strides[1]}};
     p.vec = vec;
+    go = true;
+    return 0;
+}
+
+template <typename Params>
+int launch(const Params& p, int dtype, void* stream) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->dtype == KTT_B200_MASK_F32) return launch_rotary<float>(p, st);
-    if (a->dtype == KTT_B200_MASK_F16) return launch_rotary<__half>(p, st);
+    if (dtype == KTT_B200_MASK_F32) return launch_rotary<float>(p, st);
+    if (dtype == KTT_B200_MASK_F16) return launch_rotary<__half>(p, st);
     return launch_rotary<__nv_bfloat16>(p, st);
+}
+
+}  // namespace
+
+extern "C" int ktt_b200_rotary(const ktt_b200_rotary_args* a, void* stream) {
+    RotaryParams p = {};
+    bool go;
+    if (int rc = fill(p, a, go)) return rc;
+    return go ? launch(p, a->dtype, stream) : 0;
+}
+
+extern "C" int ktt_b200_rotary_axes(const ktt_b200_rotary_args* a, const ktt_b200_axes* axes, void* stream) {
+    RotaryAxesParams p = {};
+    bool go;
+    if (int rc = fill(p, a, go)) return rc;
+    if (!go) return 0;
+    if (!axes) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: null axes");
+    if (const char* why = axes_of(p.axes, *axes, a->pairs)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "rotary: %s", why);
+    p.positions = {axes->positions, axes->positions_are_64, {axes->strides[0], axes->strides[1], axes->strides[2]}};
+    return launch(p, a->dtype, stream);
 }

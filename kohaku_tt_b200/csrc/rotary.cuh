@@ -4,12 +4,24 @@
 // (x1, x2) at position p becomes (x1 c - x2 s, x2 c + x1 s) with c = cos[p][i], s = sin[p][i]; its gradient is the
 // same with -s. Column by column that is y = x c + x' s', x' the other column of the pair and s' = -s or s: products
 // and sum are rounded one by one in fp32 (as separate operators round them), the result once to the row's type.
+//
+// Positions may have several axes (time, height, width): pair i then turns by cos[p_a][i], s[p_a][i], p_a the row's position on
+// that pair's axis a.
 #pragma once
 #include <cuda_fp16.h>
 
 #include "common.cuh"
 
 namespace ktt {
+
+constexpr int kMaxAxes = 4;
+constexpr int kMaxTurnPairs = 512;   // of rows of 1,024 columns
+
+// The axis of each pair, in two bits.
+struct PairAxes {
+    uint32_t of[kMaxTurnPairs / 16];
+    int axes;
+};
 
 // Tables and layout of a rotation, as the kernels read them.
 struct Turn {
@@ -96,6 +108,12 @@ struct Eight {
     }
 };
 
+// The positions of a row: one, or one for each axis.
+template <bool kAxes>
+struct Positions {
+    int64_t at[kAxes ? kMaxAxes : 1];
+};
+
 // The turn of columns [col, col + 8) at one position: kept in registers over the heads of a token.
 // kFast: the columns all turn or none does, their partners are eight neighbours too, and table rows are read in
 // 16-byte pieces.
@@ -104,6 +122,67 @@ struct Turned {
     float c[8], s[8];
     int partner;     // kFast: column of the first partner (half layout), or -1: in the same eight columns
     int count;       // columns of the eight that turn
+
+    static __device__ __forceinline__ int64_t row_of(const Turn& t, int64_t position) {
+        return (position < 0 ? 0 : (position >= t.rows ? t.rows - 1 : position)) * t.stride;
+    }
+
+    // Several axes. kFast: of each axis that the eight columns' pairs have, its table rows' pieces, of which the pairs of that axis
+    // are taken: pairs of one axis lie together in most layouts (one piece), and where they take turns three pieces of 16 bytes
+    // are fewer trips through the cache than eight words.
+    __device__ __forceinline__ void load(const Turn& t, const PairAxes& x, const Positions<true>& positions, int col) {
+        const int part = t.cos ? 2 * t.half : 0;
+        count = min(max(part - col, 0), 8);
+        partner = -1;
+        if (count == 0) return;
+        const float flip = t.inverse ? -1.f : 1.f;
+        if (kFast) {
+            const bool low = t.interleaved || col < t.half;
+            const int at = t.interleaved ? col / 2 : (low ? col : col - t.half);
+            if (!t.interleaved) partner = low ? col + t.half : at;
+            const uint32_t word = x.of[at >> 4] >> (2 * (at & 15));   // (eight pairs from a multiple of 8 on, or four from one of 4)
+            float cs[8], sn[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) cs[e] = sn[e] = 0.f;
+#pragma unroll
+            for (int a = 0; a < kMaxAxes; ++a) {
+                const uint32_t other = word ^ (a * 0x5555u), mine = ~(other | other >> 1) & (t.interleaved ? 0x55u : 0x5555u);
+                if (!mine) continue;
+                const int64_t row = row_of(t, positions.at[a]) + at;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (i && t.interleaved) break;
+                    const float4 u = *reinterpret_cast<const float4*>(t.cos + row + 4 * i), v = *reinterpret_cast<const float4*>(t.sin + row + 4 * i);
+                    const float uc[4] = {u.x, u.y, u.z, u.w}, us[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const bool take = mine >> (2 * (4 * i + e)) & 1;
+                        cs[4 * i + e] = take ? uc[e] : cs[4 * i + e];
+                        sn[4 * i + e] = take ? us[e] : sn[4 * i + e];
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                c[e] = t.interleaved ? cs[e >> 1] : cs[e];
+                s[e] = t.interleaved ? (e & 1 ? flip : -flip) * sn[e >> 1] : (low ? -flip : flip) * sn[e];
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int i = col + e;
+                const bool low = t.interleaved ? !(i & 1) : i < t.half;
+                const int at = e < count ? (t.interleaved ? i >> 1 : (low ? i : i - t.half)) : 0;
+                const int axis = x.of[at >> 4] >> (2 * (at & 15)) & 3;
+                int64_t position = positions.at[0];
+#pragma unroll
+                for (int a = 1; a < kMaxAxes; ++a) position = axis == a ? positions.at[a] : position;
+                const int64_t row = row_of(t, position) + at;
+                c[e] = e < count ? t.cos[row] : 1.f;
+                s[e] = e < count ? (low ? -flip : flip) * t.sin[row] : 0.f;
+            }
+        }
+    }
 
     __device__ __forceinline__ void load(const Turn& t, int64_t position, int col) {
         const int part = t.cos ? 2 * t.half : 0;
@@ -163,6 +242,26 @@ struct Turned {
         }
     }
 };
+
+// Positions as a caller gives them: of 32 or 64 bits, (axis, batch entry, row) strides.
+struct Placed {
+    const void* at;   // null: none
+    int wide;
+    int64_t stride[3];
+    __device__ __forceinline__ int64_t get(int axis, int64_t b, int64_t r) const {
+        const int64_t i = axis * stride[0] + b * stride[1] + r * stride[2];
+        return wide ? static_cast<const int64_t*>(at)[i] : static_cast<const int32_t*>(at)[i];
+    }
+    __device__ __forceinline__ Positions<true> all(int axes, int64_t b, int64_t r) const {
+        Positions<true> p;
+#pragma unroll
+        for (int a = 0; a < kMaxAxes; ++a) p.at[a] = a < axes ? get(a, b, r) : 0;
+        return p;
+    }
+};
+
+// Axes of `pairs` pairs from the caller's bytes; null, or why not (rotary.cu).
+const char* axes_of(PairAxes& x, const ktt_b200_axes& given, int pairs);
 
 // Whether Turned<true> may be used for columns of rows like these.
 inline bool turn_is_fast(const Turn& t) {

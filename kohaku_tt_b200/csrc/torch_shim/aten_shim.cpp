@@ -926,7 +926,57 @@ PyObject* py_sdpa_varlen(PyObject*, PyObject* const* args, Py_ssize_t n) {
 struct Turn {
     Tensor cos, sin, positions;   // positions: undefined without
     bool interleaved = false, inverse = false;
+    std::string axes;             // of each pair, a byte each; empty: positions have one
 };
+
+// A sequence of `pairs` axes, 0 to 3.
+bool axes_of(PyObject* given, int64_t pairs, std::string& to) {
+    if (!PyTuple_CheckExact(given) && !PyList_CheckExact(given)) return false;
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(given);
+    if (n != pairs || n == 0) return false;
+    to.resize(static_cast<size_t>(n));
+    PyObject** items = PySequence_Fast_ITEMS(given);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        if (!PyLong_CheckExact(items[i])) return false;
+        const long axis = PyLong_AsLong(items[i]);
+        if (axis < 0 || axis > 3) {
+            PyErr_Clear();
+            return false;
+        }
+        to[static_cast<size_t>(i)] = static_cast<char>(axis);
+    }
+    return true;
+}
+
+// positions [rows] or [1 or batch, rows], with axes one dimension more in front.
+bool positions_ok(const Tensor& p, const std::string& axes, const Tensor& like, bool packed, int64_t batch, int64_t rows) {
+    if (!plain(p) || p.device() != like.device() || (p.scalar_type() != at::kInt && p.scalar_type() != at::kLong)) return false;
+    const int64_t front = axes.empty() ? 0 : 1, dims = p.dim() - front;
+    if (front) {
+        if (p.dim() < 1 || p.size(0) > 4) return false;
+        for (const char axis : axes) {
+            if (axis >= p.size(0)) return false;
+        }
+    }
+    if (dims == 1) return p.size(front) == rows;
+    return !packed && dims == 2 && p.size(front + 1) == rows && (p.size(front) == 1 || p.size(front) == batch);
+}
+
+ktt_b200_axes axes_block(const Turn& x) {
+    const Tensor& p = x.positions;
+    const int64_t at = p.dim() - 2;
+    const bool front = !x.axes.empty();
+    ktt_b200_axes a;
+    std::memset(&a, 0, sizeof(a));
+    a.axes = front ? static_cast<int32_t>(p.size(0)) : 1;
+    a.positions_are_64 = p.scalar_type() == at::kLong;
+    a.positions = p.data_ptr();
+    a.strides[0] = front ? p.stride(0) : 0;
+    a.strides[1] = at >= front && p.size(at) > 1 ? p.stride(at) : 0;
+    a.strides[2] = p.stride(-1);
+    a.of_pair = front ? reinterpret_cast<const uint8_t*>(x.axes.data()) : nullptr;
+    return a;
+}
 
 bool turn_ok(const Turn& x, const Tensor& like, int64_t dim) {
     for (const Tensor* t : {&x.cos, &x.sin}) {
@@ -981,6 +1031,11 @@ torch::autograd::variable_list run_rotary(const Tensor& q_, const Tensor& k_, co
     a.sin = x.sin.data_ptr<float>();
     a.table_stride = x.cos.stride(0);
     a.table_rows = x.cos.size(0);
+    if (!x.axes.empty()) {
+        const ktt_b200_axes axes = axes_block(x);
+        raise_status(ktt_b200_rotary_axes(&a, &axes, at::cuda::getCurrentCUDAStream()), "rotary");
+        return out;
+    }
     if (x.positions.defined()) {
         const Tensor& p = x.positions;
         a.positions = p.data_ptr();
@@ -998,13 +1053,15 @@ struct Rotation : torch::autograd::Function<Rotation> {
         at::AutoDispatchBelowADInplaceOrView guard;
         ctx->save_for_backward({x.cos, x.sin, x.positions});
         ctx->saved_data["how"] = std::vector<int64_t>{x.interleaved, x.inverse, k.has_value()};
+        if (!x.axes.empty()) ctx->saved_data["axes"] = x.axes;
         ctx->set_materialize_grads(false);
         return run_rotary(q, k.has_value() ? *k : Tensor(), x);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
         const auto saved = ctx->get_saved_variables();
         const auto how = ctx->saved_data["how"].toIntVector();
-        const Turn x{saved[0], saved[1], saved[2], how[0] != 0, how[1] == 0};
+        const auto axes = ctx->saved_data.find("axes");
+        const Turn x{saved[0], saved[1], saved[2], how[0] != 0, how[1] == 0, axes == ctx->saved_data.end() ? std::string() : axes->second.toStringRef()};
         const Tensor dq = grads[0], dk = how[2] ? grads[1] : Tensor();
         const Tensor &first = dq.defined() ? dq : dk, &second = dq.defined() ? dk : dq;
         if (!first.defined()) return {Tensor(), Tensor(), Tensor()};
@@ -1020,11 +1077,11 @@ struct Rotation : torch::autograd::Function<Rotation> {
     }
 };
 
-// rotary(q, k or None, cos, sin, positions or None, interleaved): (q', k' or None), or None.
+// rotary(q, k or None, cos, sin, positions or None, interleaved, axes or None): (q', k' or None), or None.
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     const Tensor *q, *k = nullptr, *cos, *sin, *pos = nullptr;
-    if (n != 6 || !callable_now() || !(q = tensor_of(args[0])) || (args[1] != Py_None && !(k = tensor_of(args[1]))) || !(cos = tensor_of(args[2])) ||
+    if (n != 7 || !callable_now() || !(q = tensor_of(args[0])) || (args[1] != Py_None && !(k = tensor_of(args[1]))) || !(cos = tensor_of(args[2])) ||
         !(sin = tensor_of(args[3])) || (args[4] != Py_None && !(pos = tensor_of(args[4])))) Py_RETURN_NONE;
     const bool packed = q->dim() == 3;
     if (!plain(*q) || (!packed && q->dim() != 4) || q->numel() == 0) Py_RETURN_NONE;
@@ -1035,15 +1092,10 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!plain(*k) || k->dim() != q->dim() || k->numel() == 0 || k->scalar_type() != q->scalar_type() || k->device() != q->device() || k->size(-1) != q->size(-1) ||
             k->size(0) != q->size(0) || (!packed && k->size(2) != rows)) Py_RETURN_NONE;
     }
-    Turn x{*cos, *sin, pos ? *pos : Tensor(), args[5] == Py_True, false};
+    Turn x{*cos, *sin, pos ? *pos : Tensor(), args[5] == Py_True, false, std::string()};
     if (!turn_ok(x, *q, q->size(-1))) Py_RETURN_NONE;
-    if (pos) {
-        if (!plain(*pos) || pos->device() != q->device() || (pos->scalar_type() != at::kInt && pos->scalar_type() != at::kLong)) Py_RETURN_NONE;
-        const bool flat = pos->dim() == 1 && pos->size(0) == rows;
-        if (!flat && (packed || pos->dim() != 2 || pos->size(1) != rows || (pos->size(0) != 1 && pos->size(0) != q->size(0)))) Py_RETURN_NONE;
-    } else if (cos->size(0) < rows) {
-        Py_RETURN_NONE;
-    }
+    if (args[6] != Py_None && (!pos || !axes_of(args[6], cos->size(1), x.axes))) Py_RETURN_NONE;
+    if (pos ? !positions_ok(*pos, x.axes, *q, packed, q->size(0), rows) : cos->size(0) < rows) Py_RETURN_NONE;
     torch::autograd::variable_list out;
     const bool done = attempted([&] {
         pybind11::gil_scoped_release release;
@@ -1108,12 +1160,8 @@ struct Cache {
     ktt_b200_pages c;
     int64_t dim = 0, batch = 0, cap = 0;
 };
-bool cache_of(Cache& x, PyObject* const* args, PyObject* max_k) {   // k_pages, v_pages, block_table, lengths
-    const Tensor* t[4];
-    for (int i = 0; i < 4; ++i) {
-        if (!(t[i] = tensor_of(args[i])) || !plain(*t[i])) return false;
-    }
-    const Tensor &k = *t[0], &v = *t[1], &table = *t[2], &lengths = *t[3];
+bool cache_of(Cache& x, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, PyObject* max_k) {
+    if (!plain(k) || !plain(v) || !plain(table) || !plain(lengths)) return false;
     if (k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || k.device() != v.device() || k.numel() == 0) return false;
     const bool four = k.scalar_type() == at::kByte;
     if (four ? k.size(3) % 9 != 0 : k.scalar_type() != at::kBFloat16) return false;
@@ -1150,6 +1198,14 @@ bool cache_of(Cache& x, PyObject* const* args, PyObject* max_k) {   // k_pages, 
     return true;
 }
 
+bool cache_of(Cache& x, PyObject* const* args, PyObject* max_k) {   // k_pages, v_pages, block_table, lengths
+    const Tensor* t[4];
+    for (int i = 0; i < 4; ++i) {
+        if (!(t[i] = tensor_of(args[i]))) return false;
+    }
+    return cache_of(x, *t[0], *t[1], *t[2], *t[3], max_k);
+}
+
 // bf16 [B, heads, S, D], or packed [T, heads, D], that goes with a cache; heads < 0: any.
 bool cache_operand(const Tensor& t, const Cache& x, const Tensor& pages, bool packed, int64_t rows, int64_t heads) {
     if (!plain(t) || t.scalar_type() != at::kBFloat16 || t.device() != pages.device() || t.dim() != (packed ? 3 : 4) || t.stride(-1) != 1 || t.size(-1) != x.dim) return false;
@@ -1157,13 +1213,21 @@ bool cache_operand(const Tensor& t, const Cache& x, const Tensor& pages, bool pa
     return heads < 0 || t.size(1) == heads;
 }
 
-// paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq (on the device), lengths_out):
+// A cache's bounds: bf16 [pages, Hk, 2, D] with dense rows.
+const Tensor* bounds_of(PyObject* o, const Tensor& like, int64_t pages, int64_t heads, int64_t dim) {
+    const Tensor* t = tensor_of(o);
+    if (!t || !plain(*t) || t->scalar_type() != at::kBFloat16 || t->dim() != 4 || t->device() != like.device() || t->size(0) != pages || t->size(1) != heads ||
+        t->size(2) != 2 || t->size(3) != dim || t->stride(3) != 1) return nullptr;
+    return t;
+}
+
+// paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq (on the device), lengths_out, positions, axes, bounds):
 // the rotated queries or None; NotImplemented when the call is not one for the fast path.
 PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *k, *v, *q = nullptr, *cu = nullptr, *len_out = nullptr;
+    const Tensor *k, *v, *q = nullptr, *cu = nullptr, *len_out = nullptr, *pos = nullptr, *bounds = nullptr;
     Cache x;
-    if (n != 12 || !callable_now() || !(k = tensor_of(args[0])) || !(v = tensor_of(args[1])) || !cache_of(x, args + 2, Py_None)) Py_RETURN_NOTIMPLEMENTED;
+    if (n != 15 || !callable_now() || !(k = tensor_of(args[0])) || !(v = tensor_of(args[1])) || !cache_of(x, args + 2, Py_None)) Py_RETURN_NOTIMPLEMENTED;
     const Tensor& pages = *tensor_of(args[2]);
     const bool packed = args[10] != Py_None, turns = args[6] != Py_None;
     if (packed && (!(cu = tensor_of(args[10])) || !int32_vector(*cu, pages, x.batch + 1))) Py_RETURN_NOTIMPLEMENTED;
@@ -1177,16 +1241,24 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (turns) {
         const Tensor *cos = tensor_of(args[6]), *sin = tensor_of(args[7]);
         if (!cos || !sin) Py_RETURN_NOTIMPLEMENTED;
-        turn = Turn{*cos, *sin, Tensor(), args[9] == Py_True, false};
-        if (!turn_ok(turn, pages, x.dim) || cos->size(0) < x.cap) Py_RETURN_NOTIMPLEMENTED;
+        turn = Turn{*cos, *sin, Tensor(), args[9] == Py_True, false, std::string()};
+        if (!turn_ok(turn, pages, x.dim) || (args[12] == Py_None && cos->size(0) < x.cap)) Py_RETURN_NOTIMPLEMENTED;
     }
+    if (args[12] == Py_None ? args[13] != Py_None : !turns) Py_RETURN_NOTIMPLEMENTED;
+    if (args[12] != Py_None) {
+        if (!(pos = tensor_of(args[12])) || (args[13] != Py_None && !axes_of(args[13], turn.cos.size(1), turn.axes))) Py_RETURN_NOTIMPLEMENTED;
+        if (!positions_ok(*pos, turn.axes, *k, packed, x.batch, rows)) Py_RETURN_NOTIMPLEMENTED;
+        turn.positions = *pos;
+    }
+    if (args[14] != Py_None && !(bounds = bounds_of(args[14], pages, x.c.pages, x.c.kv_heads, x.dim))) Py_RETURN_NOTIMPLEMENTED;
     Tensor out;
     const bool done = attempted([&] {
         pybind11::gil_scoped_release release;
         at::AutoDispatchBelowADInplaceOrView guard;
         c10::cuda::CUDAGuard device(pages.device());
-        ktt_b200_append_args a;
-        std::memset(&a, 0, sizeof(a));
+        ktt_b200_append_at_args placed;
+        std::memset(&placed, 0, sizeof(placed));
+        ktt_b200_append_args& a = placed.base;
         a.cache = x.c;
         a.batch = static_cast<int32_t>(x.batch);
         a.rows = static_cast<int32_t>(rows);
@@ -1213,7 +1285,12 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         }
         if (cu) a.cu_seqlens = cu->data_ptr<int32_t>();
         if (len_out) a.lengths_out = len_out->data_ptr<int32_t>();
-        raise_status(ktt_b200_paged_append(&a, at::cuda::getCurrentCUDAStream()), "paged_append");
+        if (pos) placed.positions = axes_block(turn);
+        if (bounds) {
+            placed.bounds = bounds->data_ptr();
+            set3(placed.bounds_strides, *bounds);
+        }
+        raise_status(pos || bounds ? ktt_b200_paged_append_at(&placed, at::cuda::getCurrentCUDAStream()) : ktt_b200_paged_append(&a, at::cuda::getCurrentCUDAStream()), "paged_append");
     });
     if (!done) Py_RETURN_NOTIMPLEMENTED;
     if (!q) Py_RETURN_NONE;
@@ -1314,6 +1391,234 @@ PyObject* py_sdpa_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// sdpa_paged_chosen(q, k_pages, v_pages, block_table [tokens, Hk, pages], lengths [tokens, Hk], scale, max_k): the output, or None.
+PyObject* py_sdpa_paged_chosen(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *k, *v, *table, *keys;
+    c10::optional<double> scale;
+    if (n != 7 || !callable_now() || !(q = tensor_of(args[0])) || !(k = tensor_of(args[1])) || !(v = tensor_of(args[2])) || !(table = tensor_of(args[3])) ||
+        !(keys = tensor_of(args[4])) || !scale_of(args[5], scale)) Py_RETURN_NONE;
+    if (!plain(*table) || table->scalar_type() != at::kInt || table->dim() != 3 || !table->is_contiguous() || table->numel() == 0 || !plain(*keys) ||
+        keys->scalar_type() != at::kInt || keys->dim() != 2 || !keys->is_contiguous() || keys->size(0) != table->size(0) || keys->size(1) != table->size(1)) Py_RETURN_NONE;
+    if (k->dim() != 4 || k->size(1) != table->size(1) || table->size(0) > INT32_MAX / table->size(1)) Py_RETURN_NONE;
+    // As a cache of one sequence for each token and head, whose checks are the same.
+    Tensor rows_table, rows_keys;
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        rows_table = table->view({-1, table->size(2)});
+        rows_keys = keys->view({-1});
+    }
+    Cache x;
+    if (!cache_of(x, *k, *v, rows_table, rows_keys, args[6])) Py_RETURN_NONE;
+    const bool packed = q->dim() == 3;
+    if ((!packed && q->dim() != 4) || q->numel() == 0) Py_RETURN_NONE;
+    const int64_t rows = packed ? q->size(0) : q->size(2), batch = packed ? 1 : q->size(0);
+    x.batch = batch;
+    if (batch * rows != table->size(0) || !cache_operand(*q, x, *k, packed, rows, -1) || (reinterpret_cast<uintptr_t>(q->data_ptr()) & 15)) Py_RETURN_NONE;
+    for (int64_t i = 0; i + 1 < q->dim(); ++i) {
+        if (q->stride(i) % 8) Py_RETURN_NONE;
+    }
+    Tensor out;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        c10::cuda::CUDAGuard device(k->device());
+        out = packed ? empty_cuda(q->sizes(), at::kBFloat16, *q) : out_like_query(*q, x.dim);
+        ktt_b200_paged_sdpa_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.cache = x.c;
+        a.batch = static_cast<int32_t>(batch);
+        a.heads = static_cast<int32_t>(q->size(1));
+        a.sq = static_cast<int32_t>(rows);
+        a.d = static_cast<int32_t>(x.dim);
+        a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(x.dim)));
+        a.q = q->data_ptr();
+        a.out = out.data_ptr();
+        operand_strides(a.q_strides, *q);
+        operand_strides(a.out_strides, out);
+        const int64_t need = ktt_b200_paged_sdpa_chosen_workspace(&a);
+        if (need < 0) raise_status(KTT_B200_ERR_UNSUPPORTED, "sdpa_paged");
+        const Tensor work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
+        a.workspace = work.data_ptr();
+        a.workspace_bytes = need;
+        raise_status(ktt_b200_paged_sdpa_chosen(&a, at::cuda::getCurrentCUDAStream()), "sdpa_paged");
+    });
+    if (!done) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// A whole number; false where it is none or does not fit 32 bits.
+bool int32_of(PyObject* o, int32_t& to) {
+    if (!PyLong_CheckExact(o)) return false;
+    const long long x = PyLong_AsLongLong(o);
+    if ((x == -1 && PyErr_Occurred()) || x < INT32_MIN || x > INT32_MAX) {
+        PyErr_Clear();
+        return false;
+    }
+    to = static_cast<int32_t>(x);
+    return true;
+}
+
+// A block table, its checks those of tables._tables: block_table, lengths, added or kept, free, count, page_size; count_out apart.
+bool tables_of(ktt_b200_tables& a, PyObject* const* args, PyObject* count_out) {
+    const Tensor* t[6];
+    for (int i = 0; i < 6; ++i) {
+        if (!(t[i] = tensor_of(i < 5 ? args[i] : count_out)) || !plain(*t[i]) || t[i]->scalar_type() != at::kInt) return false;
+    }
+    const Tensor& table = *t[0];
+    if (table.dim() != 2 || table.size(0) < 1 || table.size(1) < 1 || table.size(0) > INT32_MAX || table.size(1) > INT32_MAX || table.stride(1) != 1) return false;
+    for (int i = 1; i < 6; ++i) {
+        const int64_t size = i < 3 ? table.size(0) : i == 3 ? t[3]->numel() : 1;
+        if (!int32_vector(*t[i], table, size)) return false;
+    }
+    std::memset(&a, 0, sizeof(a));
+    if (!int32_of(args[5], a.page_size)) return false;
+    a.batch = static_cast<int32_t>(table.size(0));
+    a.table_width = static_cast<int32_t>(table.size(1));
+    a.block_table = table.data_ptr<int32_t>();
+    a.table_stride = table.stride(0);
+    a.lengths = t[1]->data_ptr<int32_t>();
+    a.free_pages = t[3]->data_ptr<int32_t>();
+    a.pool = t[3]->numel();
+    a.count = t[4]->data_ptr<int32_t>();
+    a.count_out = t[5]->data_ptr<int32_t>();
+    return true;
+}
+
+// paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out): (cu_seq, positions, slots, granted), or None.
+PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    ktt_b200_tables a;
+    int32_t tokens;
+    if (n != 8 || !callable_now() || !tables_of(a, args, args[7]) || !int32_of(args[6], tokens) || tokens < 0) Py_RETURN_NONE;
+    const Tensor& table = *tensor_of(args[0]);
+    Tensor out[4];
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        c10::cuda::CUDAGuard device(table.device());
+        out[0] = empty_cuda({a.batch + 1}, at::kInt, table);
+        out[1] = empty_cuda({tokens}, at::kInt, table);
+        out[2] = empty_cuda({tokens}, at::kLong, table);
+        out[3] = empty_cuda({a.batch}, at::kInt, table);
+        raise_status(ktt_b200_paged_reserve(&a, tensor_of(args[2])->data_ptr<int32_t>(), tokens, out[0].data_ptr<int32_t>(), out[1].data_ptr<int32_t>(),
+                                            out[2].data_ptr<int64_t>(), out[3].data_ptr<int32_t>(), at::cuda::getCurrentCUDAStream()),
+                     "paged_reserve");
+    });
+    if (!done) Py_RETURN_NONE;
+    PyObject* all = PyTuple_New(4);
+    if (!all) return nullptr;
+    for (int i = 0; i < 4; ++i) PyTuple_SET_ITEM(all, i, THPVariable_Wrap(std::move(out[i])));
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_release(block_table, lengths, kept, free, count, page_size, count_out): True, or None.
+PyObject* py_paged_release(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    ktt_b200_tables a;
+    if (n != 7 || !callable_now() || !tables_of(a, args, args[6])) Py_RETURN_NONE;
+    const Tensor& table = *tensor_of(args[0]);
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        c10::cuda::CUDAGuard device(table.device());
+        raise_status(ktt_b200_paged_release(&a, tensor_of(args[2])->data_ptr<int32_t>(), at::cuda::getCurrentCUDAStream()), "paged_release");
+    });
+    if (!done) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_bounds(k_pages, block_table, lengths, bounds, since or None): True, or None.
+PyObject* py_paged_bounds(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *k, *table, *lengths, *bounds, *since = nullptr;
+    if (n != 5 || !callable_now() || !(k = tensor_of(args[0])) || !(table = tensor_of(args[1])) || !(lengths = tensor_of(args[2]))) Py_RETURN_NONE;
+    Cache x;
+    if (!cache_of(x, *k, *k, *table, *lengths, Py_None) || !(bounds = bounds_of(args[3], *k, x.c.pages, x.c.kv_heads, x.dim))) Py_RETURN_NONE;
+    if (args[4] != Py_None && (!(since = tensor_of(args[4])) || !int32_vector(*since, *k, x.batch))) Py_RETURN_NONE;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        c10::cuda::CUDAGuard device(k->device());
+        ktt_b200_bounds_args a;
+        std::memset(&a, 0, sizeof(a));
+        a.cache = x.c;
+        a.batch = static_cast<int32_t>(x.batch);
+        a.d = static_cast<int32_t>(x.dim);
+        a.since = since ? since->data_ptr<int32_t>() : nullptr;
+        a.bounds = bounds->data_ptr();
+        set3(a.bounds_strides, *bounds);
+        raise_status(ktt_b200_paged_bounds(&a, at::cuda::getCurrentCUDAStream()), "paged_bounds");
+    });
+    if (!done) Py_RETURN_NONE;
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq_q (on the device)): (chosen, keys), or None.
+PyObject* py_paged_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const Tensor *q, *bounds, *table, *lengths, *cu = nullptr;
+    ktt_b200_select_args a;
+    std::memset(&a, 0, sizeof(a));
+    if (n != 9 || !callable_now() || !(q = tensor_of(args[0])) || !(bounds = tensor_of(args[1])) || !(table = tensor_of(args[2])) || !(lengths = tensor_of(args[3])) ||
+        !int32_of(args[4], a.page_size) || !int32_of(args[5], a.top) || !int32_of(args[6], a.first) || !int32_of(args[7], a.last)) Py_RETURN_NONE;
+    if (bounds->dim() != 4 || !bounds_of(args[1], *q, bounds->size(0), bounds->size(1), bounds->size(3)) || bounds->numel() == 0 || bounds->size(1) > INT32_MAX) Py_RETURN_NONE;
+    if (!plain(*table) || table->scalar_type() != at::kInt || table->dim() != 2 || table->size(0) < 1 || table->size(0) > INT32_MAX || table->size(1) < 1 ||
+        table->size(1) > INT32_MAX || table->stride(1) != 1 || table->device() != q->device()) Py_RETURN_NONE;
+    const int64_t batch = table->size(0);
+    if (!int32_vector(*lengths, *table, batch)) Py_RETURN_NONE;
+    const bool packed = args[8] != Py_None;
+    if (packed && (!(cu = tensor_of(args[8])) || !int32_vector(*cu, *table, batch + 1))) Py_RETURN_NONE;
+    if (!plain(*q) || q->scalar_type() != at::kBFloat16 || q->dim() != (packed ? 3 : 4) || q->numel() == 0 || q->size(-1) != bounds->size(3) || q->stride(-1) != 1 ||
+        (reinterpret_cast<uintptr_t>(q->data_ptr()) & 15) || (!packed && q->size(0) != batch) || q->size(1) > 65535) Py_RETURN_NONE;
+    for (int64_t i = 0; i + 1 < q->dim(); ++i) {
+        if (q->stride(i) % 8) Py_RETURN_NONE;
+    }
+    const int64_t rows = packed ? q->size(0) : q->size(2), tokens = packed ? rows : batch * rows;
+    if (tokens > INT32_MAX || a.top < 1) Py_RETURN_NONE;
+    Tensor chosen, keys;
+    const bool done = attempted([&] {
+        pybind11::gil_scoped_release release;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        c10::cuda::CUDAGuard device(q->device());
+        a.batch = static_cast<int32_t>(batch);
+        a.heads = static_cast<int32_t>(q->size(1));
+        a.kv_heads = static_cast<int32_t>(bounds->size(1));
+        a.sq = packed ? 0 : static_cast<int32_t>(rows);
+        a.d = static_cast<int32_t>(q->size(-1));
+        a.total_q = packed ? rows : 0;
+        a.table_width = static_cast<int32_t>(table->size(1));
+        a.pages = bounds->size(0);
+        a.block_table = table->data_ptr<int32_t>();
+        a.table_stride = table->stride(0);
+        a.lengths = lengths->data_ptr<int32_t>();
+        a.q = q->data_ptr();
+        operand_strides(a.q_strides, *q);
+        if (cu) a.cu_seqlens_q = cu->data_ptr<int32_t>();
+        a.bounds = bounds->data_ptr();
+        set3(a.bounds_strides, *bounds);
+        const int64_t need = ktt_b200_paged_select_workspace(&a);
+        if (need < 0) raise_status(KTT_B200_ERR_UNSUPPORTED, "paged_select");
+        chosen = empty_cuda({tokens, a.kv_heads, a.top}, at::kInt, *q);
+        keys = empty_cuda({tokens, a.kv_heads}, at::kInt, *q);
+        const Tensor work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
+        a.chosen = chosen.data_ptr<int32_t>();
+        a.keys = keys.data_ptr<int32_t>();
+        a.workspace = work.data_ptr();
+        a.workspace_bytes = need;
+        raise_status(ktt_b200_paged_select(&a, at::cuda::getCurrentCUDAStream()), "paged_select");
+    });
+    if (!done) Py_RETURN_NONE;
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(chosen)));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(keys)));
+    return pair;
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* py_drop_workspaces(PyObject*, PyObject*) {
     forward_pool().clear();
     decode_pool().clear();
@@ -1329,6 +1634,11 @@ PyMethodDef g_methods[] = {
     {"paged_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_append)), METH_FASTCALL, nullptr},
     {"paged_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_read)), METH_FASTCALL, nullptr},
     {"sdpa_paged", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_sdpa_paged)), METH_FASTCALL, nullptr},
+    {"sdpa_paged_chosen", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_sdpa_paged_chosen)), METH_FASTCALL, nullptr},
+    {"paged_reserve", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_reserve)), METH_FASTCALL, nullptr},
+    {"paged_release", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_release)), METH_FASTCALL, nullptr},
+    {"paged_bounds", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_bounds)), METH_FASTCALL, nullptr},
+    {"paged_select", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_select)), METH_FASTCALL, nullptr},
     {"drop_workspaces", py_drop_workspaces, METH_NOARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "ktt_b200_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};

@@ -5,11 +5,12 @@ times as many keys in it.)"""
 
 import ctypes
 import math
+from collections.abc import Sequence
 
 import torch
 
 from . import _lib, attention, ops
-from .rotary import check_tables, dense_tables
+from .rotary import check_positions, check_tables, dense_tables, fill_axes, pair_axes
 
 
 def paged_cache(pages, kv_heads, page_size, dim, bits=16, device="cuda"):
@@ -85,10 +86,19 @@ def _on_device(cu):
     return cu is None or (isinstance(cu, torch.Tensor) and cu.is_cuda)
 
 
-def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out):
+def check_bounds(bounds, like, pages, hk, dim, what):
+    """The rules of a cache's bounds."""
+    if tuple(bounds.shape) != (pages, hk, 2, dim) or bounds.dtype != torch.bfloat16 or bounds.device != like.device:
+        raise ValueError(f"kohaku_tt_b200.{what}: bounds must be bf16 {[pages, hk, 2, dim]} on the pages' device, got {bounds.dtype} {list(bounds.shape)}")
+    if bounds.stride(3) != 1:
+        raise _lib.UnsupportedAttention(f"kohaku_tt_b200.{what}: the rows of bounds must be dense")
+
+
+def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions=None, axes=None, bounds=None):
     what = "paged_append"
-    ops._require_cuda(k, v, q, cos, sin, lengths_out)
-    a = _lib.AppendArgs()
+    ops._require_cuda(k, v, q, cos, sin, lengths_out, positions, bounds)
+    at = _lib.AppendAtArgs()
+    a = at.base
     dim, batch, cap = _pages(a.cache, k_pages, v_pages, block_table, lengths, None, what)
     packed = cu_seq is not None
     if k.dim() != (3 if packed else 4):
@@ -106,10 +116,22 @@ def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleav
             raise ValueError("kohaku_tt_b200.paged_append: cos and sin go together")
         if cos is not None:
             a.pairs = check_tables(cos, sin, k_pages, dim, what)
-            if cos.shape[0] < cap:
+            if positions is None and cos.shape[0] < cap:
                 raise ValueError("kohaku_tt_b200.paged_append: the rotary tables must cover every cache position")
             cos, sin = dense_tables(cos, sin)
             a.cos, a.sin, a.table_stride, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
+        if positions is None and axes is not None:
+            raise ValueError("kohaku_tt_b200.paged_append: axes need positions")
+        if positions is not None:
+            if cos is None:
+                raise ValueError("kohaku_tt_b200.paged_append: positions need rotary tables")
+            axes = pair_axes(axes, cos.shape[1], what)
+            check_positions(positions, axes, k, rows, what)
+            fill_axes(at.positions, positions, axes)
+        if bounds is not None:
+            check_bounds(bounds, k_pages, k_pages.shape[0], hk, dim, what)
+            at.bounds = bounds.data_ptr()
+            ops._set3(at.bounds_strides, bounds.stride()[:3])
         q_out = None
         if q is not None:
             if q.dim() != k.dim() or q.shape[1] < 1:
@@ -127,7 +149,10 @@ def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleav
         a.k, a.v = k.data_ptr(), v.data_ptr()
         ops._set3(a.k_strides, strides(k))
         ops._set3(a.v_strides, strides(v))
-        _lib.check(_lib.lib().ktt_b200_paged_append(ctypes.byref(a), ops._stream(k_pages.device)), what)
+        if positions is not None or bounds is not None:
+            _lib.check(_lib.lib().ktt_b200_paged_append_at(ctypes.byref(at), ops._stream(k_pages.device)), what)
+        else:
+            _lib.check(_lib.lib().ktt_b200_paged_append(ctypes.byref(a), ops._stream(k_pages.device)), what)
     return q_out
 
 
@@ -187,18 +212,56 @@ def _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, ma
     return out
 
 
+def _chosen(q, k_pages, v_pages, chosen, keys, scale, max_k):
+    """sdpa_paged with a table of each token's and K / V head's own."""
+    what = "sdpa_paged"
+    ops._require_cuda(q, chosen, keys)
+    if chosen.dim() != 3 or chosen.dtype != torch.int32 or chosen.shape[2] < 1 or chosen.shape[1] != k_pages.shape[1]:
+        raise ValueError("kohaku_tt_b200.sdpa_paged: block_table of three dimensions must be int32 [tokens, Hk, pages]")
+    if keys.dtype != torch.int32 or keys.shape != chosen.shape[:2]:
+        raise ValueError("kohaku_tt_b200.sdpa_paged: lengths must be int32 [tokens, Hk] there")
+    if q.dim() not in (3, 4):
+        raise ValueError("kohaku_tt_b200.sdpa_paged: q must be [B, H, Sq, D] or [T, H, D]")
+    packed = q.dim() == 3
+    batch, rows = (1, q.shape[0]) if packed else (q.shape[0], q.shape[2])
+    if batch * rows != chosen.shape[0]:
+        raise ValueError(f"kohaku_tt_b200.sdpa_paged: tables of {chosen.shape[0]} tokens for {batch * rows}")
+    chosen, keys = chosen.contiguous(), keys.contiguous()
+    a = _lib.PagedSdpaArgs()
+    dim, _, _ = _pages(a.cache, k_pages, v_pages, chosen.view(-1, chosen.shape[2]), keys.view(-1), max_k, what)
+    q = _operand(q, "q", q.shape[1], k_pages, batch, rows, dim, packed, what)
+    out = _attention_out(q, packed)
+    if q.data_ptr() % 16 or any(x % 8 for x in q.stride()[:-1]):
+        q = q.clone(memory_format=torch.contiguous_format)
+    strides = ops._ths_strides if packed else ops._bhs_strides
+    with torch.cuda.device(q.device):
+        a.batch, a.heads, a.sq, a.d = batch, q.shape[1], rows, dim
+        a.scale = float(scale) if scale is not None else 1.0 / math.sqrt(dim)
+        a.q, a.out = q.data_ptr(), out.data_ptr()
+        ops._set3(a.q_strides, strides(q))
+        ops._set3(a.out_strides, strides(out))
+        need = _lib.lib().ktt_b200_paged_sdpa_chosen_workspace(ctypes.byref(a))
+        if need < 0:
+            _lib.check(_lib.ERR_UNSUPPORTED, what)
+        work = torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
+        _lib.check(_lib.lib().ktt_b200_paged_sdpa_chosen(ctypes.byref(a), ops._stream(q.device)), what)
+    return out
+
+
 # ---- operators for compiled graphs (which pass tensors, not lists) ---------------------------
 
-@torch.library.custom_op("ktt_b200::_paged_append", mutates_args=("k_pages", "v_pages", "lengths_out"), device_types="cuda")
+@torch.library.custom_op("ktt_b200::_paged_append", mutates_args=("k_pages", "v_pages", "lengths_out", "bounds"), device_types="cuda")
 def _append_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
                cos: torch.Tensor | None, sin: torch.Tensor | None, q: torch.Tensor | None, interleaved: bool, cu_seq: torch.Tensor | None,
-               lengths_out: torch.Tensor | None) -> torch.Tensor:
-    out = _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+               lengths_out: torch.Tensor | None, positions: torch.Tensor | None = None, axes: Sequence[int] | None = None,
+               bounds: torch.Tensor | None = None) -> torch.Tensor:
+    out = _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
     return k.new_empty((0,)) if out is None else out
 
 
 @_append_op.register_fake
-def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out):
+def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions=None, axes=None, bounds=None):
     return k.new_empty((0,)) if q is None else ops._empty_like_rows(q)
 
 
@@ -226,10 +289,21 @@ def _(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q,
     return _attention_out(q, cu_seq_q is not None)
 
 
+@torch.library.custom_op("ktt_b200::_sdpa_paged_chosen", mutates_args=(), device_types="cuda")
+def _chosen_op(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, chosen: torch.Tensor, keys: torch.Tensor, scale: float | None,
+               max_k: int | None) -> torch.Tensor:
+    return _chosen(q, k_pages, v_pages, chosen, keys, scale, max_k)
+
+
+@_chosen_op.register_fake
+def _(q, k_pages, v_pages, chosen, keys, scale, max_k):
+    return _attention_out(q, q.dim() == 3)
+
+
 # ---- the entry points ------------------------------------------------------------------------
 
 def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=None, q=None, interleaved=False,
-                 cu_seq=None, lengths_out=None):
+                 cu_seq=None, lengths_out=None, positions=None, axes=None, bounds=None):
     """Writes new keys and values behind what sequences have in a paged cache, the keys rotated on the way
     (and the step's queries alongside), in one launch.
 
@@ -241,20 +315,25 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     cos, sin: rotary_table's, one row per place of the cache; without them keys go in as they are. Rotation as
     in `rotary` (interleaved; columns past 2 * pairs are copied), the result in bf16.
     q: bf16 [B, H, S, D] or [T, H, D]; returned rotated (None without q; packed rows of no sequence undefined).
+    positions, axes: as in `rotary`, where rows turn by positions other than their places (pictures in a
+    prompt; packed rows: [T], or [axes, T]); the tables then need not cover the places.
+    bounds: a cache's bounds (paged_bounds), which are kept up to date for the pages that the new keys go to;
+    what those held before must be in the bounds already.
     Pages of 4 bits (paged_cache(bits=4)) hold each 64 channels of a row as codes 0 to 15 of
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
     interleaved = bool(interleaved)
     if torch.compiler.is_compiling():
-        out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+        out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out,
+                                               positions, axes, bounds)
         return out if q is not None else None
     # Eager calls on plain CUDA tensors are served by C++ in one step.
     eager = _lib.native()
     if eager and _on_device(cu_seq):
-        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
         if out is not NotImplemented:
             return out
     with torch.no_grad():
-        return _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+        return _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
 
 
 def paged_read(k_pages, v_pages, block_table, lengths, max_k=None):
@@ -284,8 +363,24 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
     diagonal is aligned to the end: query i of n sees keys 0 .. lengths[b] - n + i. A row that sees no key
     gets zeros. max_k: no sequence has more keys (default: what block_table has room for; longer ones are
     cut); an entry of block_table within a length that is no page of the cache reads as zeros. A key that some of a sequence's queries see and others do not must be finite. Weights are
-    rounded to bf16 for their product with the values, to fp16 in chunks of prompts over 4-bit pages. No gradients."""
+    rounded to bf16 for their product with the values, to fp16 in chunks of prompts over 4-bit pages. No gradients.
+
+    block_table [tokens, Hk, pages] with lengths [tokens, Hk] (paged_select's): each query token has its own pages
+    for each K / V head, and sees the first lengths[t, h] keys of them; q [B, H, Sq, D] (token b * Sq + s) or
+    [T, H, D], without offsets."""
     causal = bool(is_causal)
+    if block_table.dim() == 3:
+        if cu_seq_q is not None or max_q is not None:
+            raise ValueError("kohaku_tt_b200.sdpa_paged: with a table for each token there are no offsets")
+        if torch.compiler.is_compiling():
+            return torch.ops.ktt_b200._sdpa_paged_chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
+        eager = _lib.native()
+        if eager:
+            out = eager.sdpa_paged_chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
+            if out is not None:
+                return out
+        with torch.no_grad():
+            return _chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
     if torch.compiler.is_compiling():
         return torch.ops.ktt_b200._sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
     eager = _lib.native()

@@ -4,6 +4,7 @@ csrc/aten/nn/aten_fused.cpp:30-43, turns whole heads in the half layout; decode_
 that in its one launch.)"""
 
 import ctypes
+from collections.abc import Sequence
 
 import torch
 
@@ -95,7 +96,43 @@ def dense_tables(cos, sin):
     return cos, sin
 
 
-def _check(q, k, cos, sin, positions):
+def pair_axes(axes, pairs, what):
+    """The axis of each pair as a tuple; None without axes."""
+    if axes is None:
+        return None
+    axes = tuple(int(a) for a in axes)
+    if len(axes) != pairs or any(a < 0 or a > 3 for a in axes):
+        raise ValueError(f"kohaku_tt_b200.{what}: axes must name an axis (0 to 3) for each of the {pairs} pairs that turn")
+    return axes
+
+
+def check_positions(positions, axes, q, rows, what):
+    """The rules of positions for rows of q [B, H, S, D] or [T, H, D]; with axes they have a dimension more in front."""
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
+        raise ValueError(f"kohaku_tt_b200.{what}: positions must be an int32 or int64 tensor on the operands' device")
+    shape = tuple(positions.shape)
+    if axes is not None:
+        if not shape or not max(axes) < shape[0] <= 4:
+            raise ValueError(f"kohaku_tt_b200.{what}: positions must have a row for each axis, 4 at most, got {shape}")
+        shape = shape[1:]
+    if not (shape == (rows,) or (q.dim() == 4 and shape in ((q.shape[0], rows), (1, rows)))):
+        raise ValueError(f"kohaku_tt_b200.{what}: one position per row ([{rows}], or [batch, {rows}]{', for each axis' if axes is not None else ''}), got {tuple(positions.shape)}")
+
+
+def position_strides(positions, axes):
+    """(axis, batch, row) strides."""
+    at = positions.dim() - 2
+    batch = positions.stride(at) if at >= (axes is not None) and positions.shape[at] > 1 else 0
+    return (positions.stride(0) if axes is not None else 0, batch, positions.stride(-1))
+
+
+def fill_axes(x, positions, axes):
+    x.axes, x.positions, x.positions_are_64 = 1 if axes is None else positions.shape[0], positions.data_ptr(), int(positions.dtype == torch.int64)
+    ops._set3(x.strides, position_strides(positions, axes))
+    x.of_pair = None if axes is None else bytes(axes)
+
+
+def _check(q, k, cos, sin, positions, axes):
     what = "rotary"
     for x in (q, k):
         if x is None:
@@ -112,17 +149,15 @@ def _check(q, k, cos, sin, positions):
     check_tables(cos, sin, q, q.shape[-1], what)
     rows = q.shape[0] if q.dim() == 3 else q.shape[2]
     if positions is None:
+        if axes is not None:
+            raise ValueError("kohaku_tt_b200.rotary: axes need positions")
         if cos.shape[0] < rows:
             raise ValueError(f"kohaku_tt_b200.rotary: tables of {cos.shape[0]} positions for {rows} rows")
         return
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64) or positions.device != q.device:
-        raise ValueError("kohaku_tt_b200.rotary: positions must be an int32 or int64 tensor on the operands' device")
-    fits = positions.shape == (rows,) or (q.dim() == 4 and positions.shape in ((q.shape[0], rows), (1, rows)))
-    if not fits:
-        raise ValueError(f"kohaku_tt_b200.rotary: one position per row ([{rows}], or [batch, {rows}]), got {tuple(positions.shape)}")
+    check_positions(positions, axes, q, rows, what)
 
 
-def _run(q, k, cos, sin, positions, interleaved, inverse):
+def _run(q, k, cos, sin, positions, interleaved, inverse, axes=None):
     """The launch, after the checks: (q', k' or None)."""
     ops._require_cuda(q, k, cos, sin, positions)
     q = ops._rows_contiguous(q)
@@ -145,10 +180,14 @@ def _run(q, k, cos, sin, positions, interleaved, inverse):
             ops._set3(a.k_strides, strides(k))
             ops._set3(a.k_out_strides, strides(k_out))
         a.cos, a.sin, a.table_stride, a.table_rows = cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0]
+        if axes is not None:
+            x = _lib.Axes()
+            fill_axes(x, positions, axes)
+            _lib.check(_lib.lib().ktt_b200_rotary_axes(ctypes.byref(a), ctypes.byref(x), ops._stream(q.device)), "rotary")
+            return q_out, k_out
         if positions is not None:
             a.positions, a.positions_are_64 = positions.data_ptr(), int(positions.dtype == torch.int64)
-            a.position_strides[0] = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-            a.position_strides[1] = positions.stride(-1)
+            a.position_strides[0], a.position_strides[1] = position_strides(positions, None)[1:]
         _lib.check(_lib.lib().ktt_b200_rotary(ctypes.byref(a), ops._stream(q.device)), "rotary")
     return q_out, k_out
 
@@ -158,59 +197,59 @@ class _Rotary(torch.autograd.Function):
     differentiated again)."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse):
+    def forward(ctx, q, k, cos, sin, positions, interleaved, inverse, axes):
         ctx.save_for_backward(cos, sin, positions)
-        ctx.how = (interleaved, inverse)
+        ctx.how = (interleaved, inverse, axes)
         ctx.set_materialize_grads(False)
-        return _run(q, k, cos, sin, positions, interleaved, inverse)
+        return _run(q, k, cos, sin, positions, interleaved, inverse, axes)
 
     @staticmethod
     def backward(ctx, dq, dk):
         cos, sin, positions = ctx.saved_tensors
-        interleaved, inverse = ctx.how
-        rest = (cos, sin, positions, interleaved, not inverse)
+        interleaved, inverse, axes = ctx.how
+        rest = (cos, sin, positions, interleaved, not inverse, axes)
         if dq is None and dk is None:
-            return (None,) * 7
+            return (None,) * 8
         if dq is None:
-            return (None, _Rotary.apply(dk, None, *rest)[0], None, None, None, None, None)
+            return (None, _Rotary.apply(dk, None, *rest)[0], None, None, None, None, None, None)
         dq, dk = _Rotary.apply(dq, dk, *rest)
-        return dq, dk, None, None, None, None, None
+        return dq, dk, None, None, None, None, None, None
 
 
 @torch.library.custom_op("ktt_b200::_rotary", mutates_args=(), device_types="cuda")
 def _rotary_op(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None,
-               interleaved: bool, inverse: bool) -> list[torch.Tensor]:
+               interleaved: bool, inverse: bool, axes: Sequence[int] | None = None) -> list[torch.Tensor]:
     """The rotation as an operator, for compiled graphs."""
-    q_out, k_out = _run(q, k, cos, sin, positions, interleaved, inverse)
+    q_out, k_out = _run(q, k, cos, sin, positions, interleaved, inverse, None if axes is None else tuple(axes))
     return [q_out] if k_out is None else [q_out, k_out]
 
 
 @_rotary_op.register_fake
-def _(q, k, cos, sin, positions, interleaved, inverse):
+def _(q, k, cos, sin, positions, interleaved, inverse, axes=None):
     return [ops._empty_like_rows(x) for x in (q, k) if x is not None]
 
 
 def _setup(ctx, inputs, output):
-    _, k, cos, sin, positions, interleaved, inverse = inputs
+    _, k, cos, sin, positions, interleaved, inverse, axes = inputs
     ctx.save_for_backward(cos, sin, positions)
-    ctx.how = (interleaved, inverse, [x.shape for x in output])
+    ctx.how = (interleaved, inverse, axes, [x.shape for x in output])
 
 
 def _op_backward(ctx, grads):
     cos, sin, positions = ctx.saved_tensors
-    interleaved, inverse, shapes = ctx.how
+    interleaved, inverse, axes, shapes = ctx.how
     some = next((g for g in grads if g is not None), None)
     if some is None:
-        return (None,) * 7
+        return (None,) * 8
     grads = [some.new_zeros(shape) if g is None else g for g, shape in zip(grads, shapes)]
-    got = torch.ops.ktt_b200._rotary(grads[0], grads[1] if len(grads) > 1 else None, cos, sin, positions, interleaved, not inverse)
-    return got[0], got[1] if len(got) > 1 else None, None, None, None, None, None
+    got = torch.ops.ktt_b200._rotary(grads[0], grads[1] if len(grads) > 1 else None, cos, sin, positions, interleaved, not inverse, axes)
+    return got[0], got[1] if len(got) > 1 else None, None, None, None, None, None, None
 
 
 _rotary_op.register_autograd(_op_backward, setup_context=_setup)
 
 
-def rotary(q, k, cos, sin, positions=None, interleaved=False):
+def rotary(q, k, cos, sin, positions=None, interleaved=False, axes=None):
     """Rotary positions of q [B, H, S, D] and k [B, Hk, S, D] (packed: [T, H, D] and [T, Hk, D]; k may be
     None): (q', k'), new tensors laid out like q and k, with gradients.
 
@@ -219,16 +258,21 @@ def rotary(q, k, cos, sin, positions=None, interleaved=False):
         y1 = x1 cos - x2 sin,  y2 = x2 cos + x1 sin
     in fp32, products and sum rounded one by one, the result once to q's type (bf16, fp16 or fp32).
     positions: int32 or int64 on the device, [S] or [B, S] (packed [T]), read by the kernel and clamped to
-    the tables' rows; without them row s has position s."""
+    the tables' rows; without them row s has position s.
+    axes: for positions of several axes (time, height and width of pictures and video), the axis of each of
+    the R / 2 pairs, 0 to 3: (0,) * 16 + (1,) * 24 + (2,) * 24, say. positions then have a dimension more in
+    front, [axes, S] or [axes, B, S] (packed [axes, T]), and pair i turns by row positions[axes[i]] of the
+    tables."""
     interleaved = bool(interleaved)
     # Eager calls on plain CUDA tensors are served by C++ in one step (None: not such a call).
     eager = not torch.compiler.is_compiling() and _lib.native()
     if eager:
-        out = eager.rotary(q, k, cos, sin, positions, interleaved)
+        out = eager.rotary(q, k, cos, sin, positions, interleaved, axes)
         if out is not None:
             return out
-    _check(q, k, cos, sin, positions)
+    axes = pair_axes(axes, cos.shape[-1], "rotary")
+    _check(q, k, cos, sin, positions, axes)
     if torch.compiler.is_compiling():
-        out = torch.ops.ktt_b200._rotary(q, k, cos, sin, positions, interleaved, False)
+        out = torch.ops.ktt_b200._rotary(q, k, cos, sin, positions, interleaved, False, None if axes is None else list(axes))
         return (out[0], None if k is None else out[1])
-    return _Rotary.apply(q, k, cos, sin, positions, interleaved, False)
+    return _Rotary.apply(q, k, cos, sin, positions, interleaved, False, axes)
