@@ -1,0 +1,161 @@
+"""Rotation by positions of several axes, forward and gradient, alone and in the append, against float64."""
+
+import pytest
+import torch
+
+import kohaku_tt_b200 as ktt
+from kohaku_tt_b200 import _lib
+from oracle import paged_oracle as po
+from oracle import serving_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch):
+    """Through the C++ edge, and through Python's."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_NATIVE", False)
+
+
+def _x(*shape, dtype=torch.bfloat16, seed=0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype)
+
+
+def _near(got, want, size):
+    """A result rounded once to its type, of three fp32 operations: half a step of the value, and 4 x 2^-24 of
+    the terms' magnitudes (two products, a sum, and room for the type's own subnormals)."""
+    got, half = got.double().cpu(), torch.finfo(got.dtype).eps / 2
+    off = (got - want).abs()
+    room = half * (want.abs() + 2.0 ** -22 * size) + 2.0 ** -22 * size + torch.finfo(torch.float16).smallest_normal * 2.0 ** -11 * (half < 2.0 ** -8)
+    assert bool((off <= room).all()), (off - room).max()
+
+
+def _axes(kind, pairs, axes):
+    g = torch.Generator().manual_seed(pairs)
+    if kind == "runs":
+        return tuple(min(axes - 1, i * axes // pairs) for i in range(pairs))
+    if kind == "turns":
+        return tuple(i % axes for i in range(pairs))
+    return tuple(torch.randint(0, axes, (pairs,), generator=g).tolist())
+
+
+# heads, kv heads, rows, D, R, interleaved
+SHAPES = [(14, 2, 77, 64, 64, False), (4, 4, 1, 128, 128, True), (3, 1, 9, 128, 64, False), (2, 2, 33, 96, 96, True), (5, 5, 7, 80, 80, False),
+          (2, 1, 5, 64, 6, False), (2, 1, 5, 64, 10, True), (1, 1, 3, 7, 6, True), (3, 2, 4, 2, 2, False), (1, 1, 2, 1024, 1024, False)]
+
+
+@pytest.mark.parametrize("h,hk,n,d,r,interleaved", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("kind,axes", [("runs", 3), ("turns", 3), ("any", 4), ("any", 2), ("runs", 1)])
+def test_rotation_and_gradient(cuda, path, h, hk, n, d, r, interleaved, dtype, kind, axes):
+    b = 2
+    q, k, dq, dk = (_x(b, x, n, d, dtype=dtype, seed=i) for i, x in enumerate((h, hk, h, hk)))
+    cos, sin = ktt.rotary_table(200, min(r, 512), device=cuda)
+    if r > 512:
+        cos, sin = (torch.cat([t, t.flip(0)], 1) for t in (cos, sin))
+    of_pair = _axes(kind, r // 2, axes)
+    pos = torch.randint(-3, 203, (axes, b, n), generator=torch.Generator().manual_seed(9))     # (clamped to the tables)
+    qd, kd = q.to(cuda).requires_grad_(), k.to(cuda).requires_grad_()
+    yq, yk = ktt.rotary(qd, kd, cos, sin, positions=pos.to(cuda), interleaved=interleaved, axes=of_pair)
+    gq, gk = torch.autograd.grad((yq, yk), (qd, kd), (dq.to(cuda), dk.to(cuda)))
+    c, s = (t[:, None] for t in so.axis_rows(cos.cpu(), sin.cpu(), pos, of_pair))
+    for got, x, inverse in ((yq, q, False), (yk, k, False), (gq, dq, True), (gk, dk, True)):
+        assert got.dtype == dtype and got.shape == x.shape
+        _near(got.detach(), *po.turn(x, c, s, interleaved, inverse))
+        assert torch.equal(got.detach().cpu()[..., r:], x[..., r:])
+    assert torch.equal(yq.detach().cpu(), po.turn_fp32(q, c, s, interleaved))      # to the bit
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_many_rows(cuda, interleaved):
+    """As many threads as have four heads each; packed, positions of 64 bits and of any strides, queries and keys in one storage."""
+    t, h, hk, d = 5000, 12, 4, 128
+    both = _x(t, h + hk, d, seed=1)
+    of_pair, pos = _axes("turns", 32, 3), torch.randint(0, 300, (t, 3), generator=torch.Generator().manual_seed(2))
+    cos, sin = ktt.rotary_table(300, 64, device=cuda)
+    x = both.to(cuda)
+    yq, yk = ktt.rotary(x[:, :h], x[:, h:], cos, sin, positions=pos.to(cuda).t(), interleaved=interleaved, axes=of_pair)
+    c, s = (y[:, None] for y in so.axis_rows(cos.cpu(), sin.cpu(), pos.t(), of_pair))
+    assert torch.equal(torch.cat([yq, yk], 1).cpu(), po.turn_fp32(both, c, s, interleaved))
+
+
+def test_alike_positions_are_those_of_one_axis(cuda, path):
+    """Text: all axes count on together. [axes, S] and [axes, 1, S] serve all batch entries."""
+    q, k = _x(3, 8, 40, 64, seed=1).to(cuda), _x(3, 2, 40, 64, seed=2).to(cuda)
+    cos, sin = ktt.rotary_table(64, 64, device=cuda)
+    at = torch.arange(7, 47, dtype=torch.int32, device=cuda)
+    want = ktt.rotary(q, k, cos, sin, positions=at)
+    for pos in (at.expand(3, 40), at.expand(3, 1, 40), at.expand(3, 3, 40), at.expand(4, 40).long()):
+        got = ktt.rotary(q, k, cos, sin, positions=pos, axes=[i % 3 for i in range(32)])
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_gradient_by_differences_and_of_the_gradient(cuda, path):
+    """The rotation is linear: differences are exact up to rounding, and the gradient's gradient is the rotation."""
+    q = _x(1, 2, 6, 16, dtype=torch.float32, seed=3).to(cuda).requires_grad_()
+    cos, sin = ktt.rotary_table(32, 12, device=cuda)
+    pos, of_pair = torch.randint(0, 32, (3, 6), generator=torch.Generator().manual_seed(4)).to(cuda), (0, 1, 2, 2, 1, 0)
+    w = _x(1, 2, 6, 16, dtype=torch.float32, seed=5).to(cuda)
+
+    def f(x):
+        return ktt.rotary(x, None, cos, sin, positions=pos, axes=of_pair)[0]
+
+    (g,) = torch.autograd.grad(f(q), q, w, create_graph=True)
+    step = _x(1, 2, 6, 16, dtype=torch.float32, seed=6).to(cuda)
+    with torch.no_grad():
+        change = ((f(q + step) - f(q - step)).double() * w.double()).sum() / 2
+        # (192 terms, each off by some 2^-22 of products of about 1)
+        assert abs(change - (g.double() * step.double()).sum()) <= 192 * 2.0 ** -20
+    v = w.clone().requires_grad_()
+    (g2,) = torch.autograd.grad(f(q), q, v, create_graph=True)
+    (back,) = torch.autograd.grad(g2, v, step)
+    assert torch.equal(back, f(step))
+    (only,) = torch.autograd.grad(ktt.rotary(q, q.detach(), cos, sin, positions=pos, axes=of_pair)[0].sum(), q)
+    assert torch.equal(only, torch.autograd.grad(f(q).sum(), q)[0])
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,pairs,interleaved", [(128, 64, False), (64, 16, True), (64, 5, False)])
+@pytest.mark.parametrize("packed", [False, True])
+def test_append(cuda, path, bits, d, pairs, interleaved, packed):
+    """Rows turned by their own positions, one axis and three, are those that `rotary` makes, at their places."""
+    b, n, h, hk, page = 3, 19, 6, 2, 16
+    lengths = torch.tensor([0, 15, 33], dtype=torch.int32, device=cuda)
+    k, v, q = _x(b * n, hk, d, seed=1).to(cuda), _x(b * n, hk, d, seed=2).to(cuda), _x(b * n, h, d, seed=3).to(cuda)
+    cos, sin = ktt.rotary_table(20, 2 * pairs, device=cuda)      # (fewer rows than places)
+    table = torch.randperm(24, generator=torch.Generator().manual_seed(4)).view(3, 8)[:, :4].to(device=cuda, dtype=torch.int32).contiguous()
+    three = torch.randint(0, 20, (3, b * n), generator=torch.Generator().manual_seed(5)).to(cuda)
+    for pos, axes in ((three[0].int(), None), (three, _axes("any", pairs, 3))):
+        want_q, want_k = ktt.rotary(q, k, cos, sin, positions=pos, interleaved=interleaved, axes=axes)
+        plain = ktt.paged_cache(24, hk, page, d, bits=bits, device=cuda)
+        got = ktt.paged_cache(24, hk, page, d, bits=bits, device=cuda)
+        cu = torch.arange(0, b * n + 1, n, dtype=torch.int32, device=cuda)
+        ktt.paged_append(want_k, v, *plain, table, lengths, cu_seq=cu)
+        if packed:
+            out = ktt.paged_append(k, v, *got, table, lengths, cos, sin, q=q, interleaved=interleaved, cu_seq=cu, positions=pos, axes=axes)
+        else:
+            rows = [x.view(b, n, -1, d).transpose(1, 2) for x in (k, v, q)]
+            out = ktt.paged_append(rows[0], rows[1], *got, table, lengths, cos, sin, q=rows[2], interleaved=interleaved, axes=axes,
+                                   positions=pos.view(*pos.shape[:-1], b, n))
+            out = out.transpose(1, 2).reshape(b * n, h, d)
+        assert torch.equal(out, want_q)
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(plain, got))
+
+
+def test_refusals(cuda, path):
+    q = _x(2, 2, 5, 8).to(cuda)
+    cos, sin = ktt.rotary_table(9, 8, device=cuda)
+    at = torch.zeros((3, 5), dtype=torch.int32, device=cuda)
+    for kw in (dict(axes=(0, 1, 2, 0)), dict(axes=(0, 1, 2), positions=at), dict(axes=(0, 1, 3, 0), positions=at), dict(axes=(0, -1, 0, 0), positions=at),
+               dict(axes=(0, 1, 2, 0), positions=at.float()), dict(axes=(0, 1, 2, 0), positions=at[:, :4]), dict(axes=(0, 1, 2, 0), positions=at[0]),
+               dict(positions=at), dict(axes=(0, 0, 0, 0), positions=torch.zeros((5, 5), dtype=torch.int32, device=cuda))):
+        with pytest.raises(ValueError):
+            ktt.rotary(q, None, cos, sin, **kw)
+    pages, table, n = ktt.paged_cache(4, 2, 16, 64, device=cuda), torch.zeros((2, 2), dtype=torch.int32, device=cuda), torch.zeros(2, dtype=torch.int32, device=cuda)
+    k, (cos, sin) = _x(2, 2, 5, 64).to(cuda), ktt.rotary_table(32, 8, device=cuda)
+    for kw in (dict(positions=at[0]), dict(cos=cos, sin=sin, axes=(0, 1, 2, 0)), dict(cos=cos, sin=sin, positions=at[0], axes=(0, 0, 0)),
+               dict(cos=cos, sin=sin, positions=at[0, :3]), dict(bounds=torch.zeros((4, 2, 2, 64), device=cuda)),
+               dict(bounds=torch.zeros((4, 2, 2, 128), dtype=torch.bfloat16, device=cuda))):
+        with pytest.raises(ValueError):
+            ktt.paged_append(k, k, *pages, table, n, **kw)
