@@ -9,7 +9,7 @@
 // at most e = 2^-17 max_h sum_d |q_hd| max |bound| (products of bf16 values are exact in fp32; the 2 D / 16 instructions that add up a
 // score round, or cut off, by some 2^-23 of the magnitudes each, together 2^-19; measured 2^-21 at most). The value t of the last page selected
 // lies within e of the last by fp32. So pages more than 2 e above or below are in or out, and those between, a few, get their scores in 64 bits.
-#include <cfloat>
+#include <algorithm>
 
 #include "four_bits.cuh"
 
@@ -220,11 +220,19 @@ __device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t x) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// A warp takes `each` blocks of 16 pages of a (token, K / V head): its lanes load both bounds of pages g and g + 8 in pieces of 16 bytes
-// as they lie (lane (g, t): channels 32 j + 8 t ..), which are the operands of m16n8k16 with the channels in that order; q+ and q- of 8 heads are
-// its columns. Nothing goes through shared memory: no two warps read the same bounds.
+// Both bounds of 16 pages as a warp's lanes load them: lane (g, t) has pages g and g + 8, channels 32 j + 8 t .., in pieces of 16 bytes.
 template <int D>
-__global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ SelectParams p) {
+struct Sixteen {
+    static constexpr int J = D / 32;
+    uint4 lo[J][2], hi[J][2];
+};
+
+// A warp takes up to kEach blocks of 16 pages of a (token, K / V head), one on its way while another is multiplied. Its lanes load the bounds as
+// they lie, which are the operands of m16n8k16 with the channels in that order; q+ and q- of 8 heads are its columns. Nothing goes
+// through shared memory: no two warps read the same bounds. The products of a block are four sums, for the latency of one.
+constexpr int kEach = 4;
+template <int D>
+__global__ void __launch_bounds__(128, 2) score_kernel(const __grid_constant__ SelectParams p) {
     constexpr int J = D / 32;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -236,9 +244,35 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Sele
     const int count = (tok.seen + p.page_size - 1) / p.page_size;
     if (count <= p.top) return;   // (all of them)
     const int block0 = ((static_cast<int>(blockIdx.x) - static_cast<int>(pair) * p.lots) * 4 + warp) * p.each;
-    const int block1 = min(block0 + p.each, (count + 15) / 16);
+    const int blocks = min(p.each, (count + 15) / 16 - block0);
+    if (blocks <= 0) return;
+    // The names of all its pages, two to a lane.
+    int names[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int e = block0 * 16 + 32 * i + lane;
+        names[i] = 32 * i < blocks * 16 && e < count ? p.table[tok.b * p.table_stride + e] : -1;
+    }
+    auto load = [&](Sixteen<D>& x, int block) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int from = (block & 1) * 16 + g + 8 * i;
+            const int n0 = __shfl_sync(0xffffffffu, names[0], from), n1 = __shfl_sync(0xffffffffu, names[1], from), name = block & 2 ? n1 : n0;
+            const bool there = name >= 0 && name < p.pages;
+            const __nv_bfloat16* at = p.bounds.edge(there ? name : 0, hk, 0) + 8 * t;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                x.lo[j][i] = x.hi[j][i] = make_uint4(0u, 0u, 0u, 0u);
+                if (there) {
+                    x.lo[j][i] = *reinterpret_cast<const uint4*>(at + 32 * j);
+                    x.hi[j][i] = *reinterpret_cast<const uint4*>(at + p.bounds.stride[2] + 32 * j);
+                }
+            }
+        }
+    };
     for (int h0 = 0; h0 < p.group; h0 += 8) {   // (more than 8 heads: the bounds come from the cache again)
-        if (block0 >= block1) return;
+        Sixteen<D> x[2];
+        load(x[0], 0);
         uint32_t up[J][4], down[J][4];
         {
             const bool there = h0 + g < p.group;
@@ -246,8 +280,8 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Sele
             const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                const uint4 x = *reinterpret_cast<const uint4*>(from + 32 * j);
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                const uint4 y4 = *reinterpret_cast<const uint4*>(from + 32 * j);
+                const uint32_t w[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(&w[i]), u = __hmax2_nan(y, zero), v = __hmin2_nan(y, zero);
@@ -256,49 +290,37 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Sele
                 }
             }
         }
-        for (int block = block0; block < block1; ++block) {
-            const __nv_bfloat16* at[2];
+        auto score = [&](const Sixteen<D>& x, int block) {
+            float acc[4][4];
+            uint32_t most[4];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int e = block * 16 + g + 8 * i;
-                const int64_t page = e < count ? p.table[tok.b * p.table_stride + e] : -1;
-                at[i] = page >= 0 && page < p.pages ? p.bounds.edge(page, hk, 0) + 8 * t : nullptr;
+            for (int i = 0; i < 4; ++i) {
+                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+                most[i] = 0u;
             }
-            uint4 lo[J][2], hi[J][2];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    lo[j][i] = hi[j][i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (at[i]) {
-                        lo[j][i] = *reinterpret_cast<const uint4*>(at[i] + 32 * j);
-                        hi[j][i] = *reinterpret_cast<const uint4*>(at[i] + p.bounds.stride[2] + 32 * j);
-                    }
-                }
-            }
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            uint32_t most = 0u;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                auto product = [&](const uint4& x, const uint4& y, const uint32_t (&b)[4]) {
+                auto product = [&](const uint4& x, const uint4& y, const uint32_t (&b)[4], int sum) {
                     const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
-                    mma_bf16(acc, a0, b[0], b[1]);
-                    mma_bf16(acc, a1, b[2], b[3]);
+                    mma_bf16(acc[sum], a0, b[0], b[1]);
+                    mma_bf16(acc[sum + 1], a1, b[2], b[3]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) most = max_magnitude(max_magnitude(most, a0[i]), a1[i]);
+                    for (int i = 0; i < 4; ++i) most[i] = max_magnitude(max_magnitude(most[i], a0[i]), a1[i]);
                 };
-                product(hi[j][0], hi[j][1], up[j]);
-                product(lo[j][0], lo[j][1], down[j]);
+                product(x.hi[j][0], x.hi[j][1], up[j], 0);
+                product(x.lo[j][0], x.lo[j][1], down[j], 2);
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[0][i] = (acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]);
             // The largest of the columns that are heads.
             const bool c0 = h0 + 2 * t < p.group, c1 = h0 + 2 * t + 1 < p.group;
-            float s[2] = {fmaxf(c0 ? acc[0] : -INFINITY, c1 ? acc[1] : -INFINITY), fmaxf(c0 ? acc[2] : -INFINITY, c1 ? acc[3] : -INFINITY)};
+            float s[2] = {fmaxf(c0 ? acc[0][0] : -INFINITY, c1 ? acc[0][1] : -INFINITY), fmaxf(c0 ? acc[0][2] : -INFINITY, c1 ? acc[0][3] : -INFINITY)};
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 1));
                 s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 2));
             }
-            float* to = p.scores + (pair * p.blocks + block) * 16;
+            float* to = p.scores + (pair * p.blocks + block0 + block) * 16;
             if (t == 0) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
@@ -307,30 +329,38 @@ __global__ void __launch_bounds__(128) score_kernel(const __grid_constant__ Sele
                 }
             }
             if (h0 == 0) {
+                uint32_t m = max_magnitude(max_magnitude(most[0], most[1]), max_magnitude(most[2], most[3]));
 #pragma unroll
-                for (int off = 1; off < 32; off <<= 1) most = max_magnitude(most, __shfl_xor_sync(0xffffffffu, most, off));
-                const __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&most);
-                if (lane == 0) p.most[pair * p.blocks + block] = __bfloat162float(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m)));
+                for (int off = 1; off < 32; off <<= 1) m = max_magnitude(m, __shfl_xor_sync(0xffffffffu, m, off));
+                const __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162*>(&m);
+                if (lane == 0) p.most[pair * p.blocks + block0 + block] = __bfloat162float(__hmax_nan(__low2bfloat16(m2), __high2bfloat16(m2)));
             }
+        };
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (i >= blocks) break;
+            if (i + 1 < blocks) load(x[(i + 1) & 1], i + 1);
+            score(x[i & 1], i);
         }
     }
 }
 
 // ---- the selection -----------------------------------------------------------------------------
 
-constexpr int kBins = 1024;
+constexpr int kBins = 512;
 constexpr int kFew = 256;        // pages between in and out that are ranked one against the others
 
 struct SelectShared {
-    int bins[kBins];
-    float fwarps[32];
-    int iwarps[32];
+    int bins[kBins + kBins / 16];   // (a place more for every 16: warp 0 reads 16 to a lane)
+    float warps[4][32];
+    int sums[32];
+    float ranked[32];
     int few_at[kFew];
     double few[kFew];
-    float lo, hi;                // fp32 scores that the last one selected lies between
-    int lo_bits, hi_bits, need, above, in_bin, count;
-    unsigned long long value;
+    int bin, in_bin, need, count, found, all_in, lo_bits, hi_bits;
+    unsigned long long exact;
 };
+__device__ __forceinline__ int bin_at(int bin) { return bin + (bin >> 4); }
 
 // Order of floats as that of integers.
 __device__ __forceinline__ int ordered(float x) {
@@ -342,38 +372,46 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
     const unsigned long long i = __double_as_longlong(x);
     return i >> 63 ? ~i : i | 1ull << 63;
 }
+__device__ __forceinline__ float larger(float a, float b) { return a != a || a > b ? a : b; }   // (a NaN stays)
 
-template <typename T, typename Op>
-__device__ __forceinline__ T over_block(T x, T* warps, Op op) {
+// Exclusive sum of x over the CTA, and that of all. Two barriers.
+__device__ __forceinline__ int sum_before(int x, int* warps, int& all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
+    int sum = x;
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) x = op(x, __shfl_xor_sync(0xffffffffu, x, off));
+    for (int off = 1; off < 32; off <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, sum, off);
+        if (lane >= off) sum += y;
+    }
+    if (lane == 31) warps[warp] = sum;
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = x;
+    const int other = lane < n ? warps[lane] : 0;
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0);
+    all = __reduce_add_sync(0xffffffffu, other);
     __syncthreads();
-    x = warps[0];
-    for (int w = 1; w < blockDim.x / 32; ++w) x = op(x, warps[w]);
-    return x;
+    return before + sum - x;
 }
 
 // The exact score of a page: 64-bit sums of products that are exact themselves. By one warp.
 template <int D>
 __device__ __forceinline__ double exact_score(const SelectParams& p, const Token& tok, int hk, int e) {
     const int lane = threadIdx.x & 31;
-    constexpr int kEach = D / 32;
+    constexpr int kMine = D / 32;
     const int64_t page = p.table[tok.b * p.table_stride + e];
     if (page < 0 || page >= p.pages) return 0.0;
-    double lo[kEach], hi[kEach];
+    double lo[kMine], hi[kMine];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
+    for (int i = 0; i < kMine; ++i) {
         lo[i] = __bfloat162float(p.bounds.edge(page, hk, 0)[lane + 32 * i]);
         hi[i] = __bfloat162float(p.bounds.edge(page, hk, 1)[lane + 32 * i]);
     }
     double best = -INFINITY;
+#pragma unroll 4
     for (int h = 0; h < p.group; ++h) {
         const __nv_bfloat16* q = tok.q + static_cast<int64_t>(hk * p.group + h) * p.qs[1];
         double sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
+        for (int i = 0; i < kMine; ++i) {
             const double x = __bfloat162float(q[lane + 32 * i]), a = x * lo[i], b = x * hi[i];
             sum += a != a || a > b ? a : b;   // (a NaN of either stays)
         }
@@ -385,15 +423,15 @@ __device__ __forceinline__ double exact_score(const SelectParams& p, const Token
     return best + 0.0;   // (no -0)
 }
 
-// One CTA for a (token, K / V head). The fp32 scores lie in shared memory where they fit, else where they were written; `in` has a bit for each
-// page that is selected.
-template <int D>
-__global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ SelectParams p, int in_shared) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
+// One CTA for a (token, K / V head); a thread has kItems neighbouring pages, their scores and names in registers (0: as many as there are, which
+// it reads again each time). The k-th largest of the scores is found by bins of equal width between the least and the largest, then by
+// rank among the few of its bin. Bound: latency, some ten barriers and two trips to memory.
+template <int D, int kItems>
+__global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ SelectParams p) {
     __shared__ SelectShared sm;
-    uint32_t* in = reinterpret_cast<uint32_t*>(dynamic);
-    const int words = (p.blocks + 1) / 2;
     const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
+    for (int i = tid; i < kBins + kBins / 16; i += threads) sm.bins[i] = 0;
+    if (tid == 0) sm.count = sm.found = sm.all_in = 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t pair = blockIdx.x, local = pair / p.kv_heads, t = p.token0 + local;
@@ -411,223 +449,243 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
         return;
     }
     const float* given = p.scores + pair * p.blocks * 16;
-    float* held = reinterpret_cast<float*>(in + words);
-    const float* s = in_shared ? held : given;
-    const int begin = p.first, end = count - p.last, k = top - p.first - p.last;   // of [begin, end), more than k
-    for (int w = tid; w < words; w += threads) in[w] = 0u;
-    for (int i = tid; i < kBins; i += threads) sm.bins[i] = 0;
-    if (tid == 0) {
-        sm.need = k;
-        sm.count = 0;
-    }
-    // The error of the fp32 scores.
-    float norm = 0.f, most = 0.f, lo = INFINITY, hi = -INFINITY;
-    constexpr int kHeadThreads = D / 8;
-    for (int h0 = 0; h0 < p.group; h0 += threads / kHeadThreads) {
-        const int h = h0 + tid / kHeadThreads;
-        float sum = 0.f;
-        if (h < p.group) {
-            Eight<__nv_bfloat16> x;
-            x.load(tok.q + static_cast<int64_t>(hk * p.group + h) * p.qs[1] + (tid % kHeadThreads) * 8);
+    const int begin = p.first, end = count - p.last, k = top - p.first - p.last;   // the k largest of [begin, end), which are more
+    const int mine = kItems ? kItems : ((count + threads - 1) / threads + 3) & ~3, first = tid * mine;
+    // All its pages: f(page, score, place among its own).
+    float held[kItems ? kItems : 1];
+    if constexpr (kItems > 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum += fabsf(__bfloat162float(x.get(e)));
+        for (int i = 0; i < kItems; i += 4) {
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (first + i < count) x = *reinterpret_cast<const float4*>(given + first + i);   // (whole blocks of 16 are written)
+            held[i] = x.x; held[i + 1] = x.y; held[i + 2] = x.z; held[i + 3] = x.w;
+        }
+    }
+    auto each = [&](auto f) {
+        if constexpr (kItems > 0) {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) {
+                if (first + i >= begin && first + i < end) f(first + i, held[i]);
+            }
+        } else {
+            for (int e = max(first, begin); e < min(first + mine, end); ++e) f(e, given[e]);
+        }
+    };
+    // The least and the largest, and what the scores may be off by.
+    float lo = INFINITY, hi = -INFINITY, most = 0.f, norm = 0.f;
+    for (int h = warp; h < p.group; h += warps) {
+        const __nv_bfloat16* q = tok.q + static_cast<int64_t>(hk * p.group + h) * p.qs[1] + lane * (D / 32);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 32; i += 2) {
+            const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(q + i));
+            sum += fabsf(y.x) + fabsf(y.y);
         }
 #pragma unroll
-        for (int off = 1; off < kHeadThreads; off <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        norm = sum > norm || sum != sum ? sum : norm;
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        norm = larger(sum, norm);
     }
-    auto larger = [](float a, float b) { return a != a || a > b ? a : b; };   // (a NaN stays)
     for (int i = tid; i < (count + 15) / 16; i += threads) most = larger(p.most[pair * p.blocks + i], most);
-    for (int e = begin + tid; e < end; e += threads) {
-        const float x = given[e];
-        if (in_shared) held[e] = x;
+    each([&](int, float x) {
         lo = fminf(lo, x);
         hi = fmaxf(hi, x);
+    });
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        most = larger(most, __shfl_xor_sync(0xffffffffu, most, off));
     }
-    norm = over_block(norm, sm.fwarps, larger);
-    most = over_block(most, sm.fwarps, larger);
-    lo = over_block(lo, sm.fwarps, [](float a, float b) { return fminf(a, b); });
-    hi = over_block(hi, sm.fwarps, [](float a, float b) { return fmaxf(a, b); });
+    if (lane == 0) {
+        sm.warps[0][warp] = lo;
+        sm.warps[1][warp] = hi;
+        sm.warps[2][warp] = most;
+        sm.warps[3][warp] = norm;
+    }
+    __syncthreads();
+    lo = lane < warps ? sm.warps[0][lane] : INFINITY;
+    hi = lane < warps ? sm.warps[1][lane] : -INFINITY;
+    most = lane < warps ? sm.warps[2][lane] : 0.f;
+    norm = lane < warps ? sm.warps[3][lane] : 0.f;
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        most = larger(most, __shfl_xor_sync(0xffffffffu, most, off));
+        norm = larger(norm, __shfl_xor_sync(0xffffffffu, norm, off));
+    }
     const float mass = norm * most;
     // (What the products could lose below fp32's least normal number is in the last terms.)
     const float off = fmaf(mass, 0x1p-17f, fmaf(norm + most, 0x1p-110f, 0x1p-110f));
     const bool sure = mass < 0x1p120f;   // else, and where it is no number: all in 64 bits
-    // The value of the k-th largest is between lo and hi: bins of equal width, of which the one that has it is cut again while it holds many.
+    int need = k;
     for (int round = 0; round < 4 && sure && k > 0 && hi - lo > 4.f * off; ++round) {
         const float by = (kBins - 0.5f) / (hi - lo);
         if (!(by < 0x1p100f)) break;
-        for (int e = begin + tid; e < end; e += threads) {
-            const float x = s[e];
-            if (x >= lo && x <= hi) atomicAdd(&sm.bins[static_cast<int>((x - lo) * by)], 1);
-        }
+        auto bin_of = [&](float x) { return static_cast<int>((x - lo) * by); };   // (falls nowhere as x rises)
+        each([&](int, float x) {
+            if (x >= lo && x <= hi) atomicAdd(&sm.bins[bin_at(bin_of(x))], 1);
+        });
         __syncthreads();
         if (warp == 0) {
-            // From the top: lane l has bins [kBins - 32 (l + 1), kBins - 32 l), summed up.
-            int sum = 0;
-            for (int i = 0; i < kBins / 32; ++i) sum += sm.bins[kBins - 1 - (lane * (kBins / 32) + i)];
+            // Lane l has the 16 bins from kBins - 16 l down: those above the one that has the need-th, and it.
+            int own[16], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum += own[i] = sm.bins[bin_at(kBins - 1 - 16 * lane - i)];
             int upto = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int y = __shfl_up_sync(0xffffffffu, upto, o);
                 if (lane >= o) upto += y;
             }
-            const int need = sm.need;
-            __syncwarp();
-            if (upto - sum < need && upto >= need) {
-                int above = upto - sum, bin = kBins - 1 - lane * (kBins / 32);
-                while (above + sm.bins[bin] < need) above += sm.bins[bin--];
-                sm.above = bin;
-                sm.in_bin = sm.bins[bin];
-                sm.need = need - above;
+            int above = upto - sum;
+            if (above < need && upto >= need) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    if (above < need && above + own[i] >= need) {
+                        sm.bin = kBins - 1 - 16 * lane - i;
+                        sm.in_bin = own[i];
+                        sm.need = need - above;
+                    }
+                    above += own[i];
+                }
+            }
+            if (lane == 0) {
                 sm.lo_bits = 0x7fffffff;
                 sm.hi_bits = static_cast<int>(0x80000000);
             }
         }
         __syncthreads();
-        const int bin = sm.above;
-        for (int e = begin + tid; e < end; e += threads) {
-            const float x = s[e];
-            if (x >= lo && x <= hi && static_cast<int>((x - lo) * by) == bin) {
+        const int bin = sm.bin, many = sm.in_bin;
+        need = sm.need;
+        if (many <= 32) {
+            each([&](int, float x) {
+                if (x >= lo && x <= hi && bin_of(x) == bin) sm.ranked[atomicAdd(&sm.found, 1)] = x;
+            });
+            __syncthreads();
+            // The need-th largest of them (equal ones in any order): every warp for itself.
+            const float x = lane < many ? sm.ranked[lane] : -INFINITY;
+            int better = 0;
+            for (int i = 0; i < many; ++i) {
+                const float y = __shfl_sync(0xffffffffu, x, i);
+                better += y > x || (y == x && i < lane);
+            }
+            const uint32_t it = __ballot_sync(0xffffffffu, lane < many && better == need - 1);
+            lo = hi = __shfl_sync(0xffffffffu, x, __ffs(it) - 1);
+            break;
+        }
+        each([&](int, float x) {
+            if (x >= lo && x <= hi && bin_of(x) == bin) {
                 atomicMin(&sm.lo_bits, ordered(x));
                 atomicMax(&sm.hi_bits, ordered(x));
             }
-        }
-        for (int i = tid; i < kBins; i += threads) sm.bins[i] = 0;
+        });
+        for (int i = tid; i < kBins + kBins / 16; i += threads) sm.bins[i] = 0;
         __syncthreads();
         lo = from_ordered(sm.lo_bits);
         hi = from_ordered(sm.hi_bits);
-        const int many = sm.in_bin;
         __syncthreads();
-        if (many <= 32) break;
     }
-    // Pages above are in, pages below are out.
+    // Pages above are in, pages below are out; those between are counted, and listed while they are few.
     const float above = sure ? hi + 2.f * off : INFINITY, below = sure ? lo - 2.f * off : -INFINITY;
-    int mine = 0, doubtful = 0;
+    auto surely = [&](float x) { return sure && x > above; };
+    auto doubtful = [&](float x) { return !surely(x) && !(x < below); };
+    int in = 0, some = 0;
     if (k > 0) {
-        for (int e0 = begin & ~31; e0 < end; e0 += threads) {
-            const int e = e0 + tid;
-            bool take = e < p.first || (e >= end && e < count);
-            if (e >= begin && e < end) {
-                const float x = s[e];
-                take = sure && x > above;
-                mine += take;
-                if (!take && !(x < below)) {
-                    const int at = atomicAdd(&sm.count, 1);
-                    if (at < kFew) sm.few_at[at] = e;
-                    ++doubtful;
-                }
+        each([&](int e, float x) {
+            in += surely(x);
+            if (doubtful(x)) {
+                ++some;
+                const int at = atomicAdd(&sm.count, 1);
+                if (at < kFew) sm.few_at[at] = e;
             }
-            const uint32_t bits = __ballot_sync(0xffffffffu, take);
-            if (lane == 0 && e < count) in[e >> 5] = bits;
-        }
+        });
     }
-    mine = over_block(mine, sm.iwarps, [](int a, int b) { return a + b; });
-    for (int e = tid; e < p.first + p.last; e += threads) {   // (those that were not in a word above)
-        const int at = e < p.first ? e : end + e - p.first;
-        atomicOr(&in[at >> 5], 1u << (at & 31));
-    }
-    const int rest = k - mine, some = sm.count;
-    if (k > 0 && some <= kFew) {
-        if (some == rest) {
-            for (int i = tid; i < some; i += threads) atomicOr(&in[sm.few_at[i] >> 5], 1u << (sm.few_at[i] & 31));
-        } else {
-            for (int i = warp; i < some; i += warps) {
+    const int warp_in = __reduce_add_sync(0xffffffffu, in);
+    if (lane == 0 && warp_in > 0) atomicAdd(&sm.all_in, warp_in);
+    __syncthreads();
+    const int all_some = sm.count, rest = k - sm.all_in;   // so many of the doubtful ones are in
+    const bool everything = all_some == rest;
+    int some_before = 0;
+    double* exact = p.exact + pair * p.blocks * 16;
+    unsigned long long value = 0;
+    int ties = 0;
+    if (k > 0 && !everything) {
+        if (all_some <= kFew) {
+            for (int i = warp; i < all_some; i += warps) {
                 const double x = exact_score<D>(p, tok, hk, sm.few_at[i]);
                 if (lane == 0) sm.few[i] = x;
             }
             __syncthreads();
-            for (int i = tid; i < some; i += threads) {
+            // The rest-th in the order of score and place: pages at or before it are in.
+            for (int i = tid; i < all_some; i += threads) {
                 const double x = sm.few[i];
                 const int e = sm.few_at[i];
                 int better = 0;
-                for (int j = 0; j < some; ++j) better += sm.few[j] > x || (sm.few[j] == x && sm.few_at[j] < e);
-                if (better < rest) atomicOr(&in[e >> 5], 1u << (e & 31));
-            }
-        }
-    } else if (k > 0) {
-        // Many that differ by less than the error (alike, most of them): the rest-th largest of their exact scores, bits by bits from the top, then
-        // those above it and, of its own value, the first.
-        double* exact = p.exact + pair * p.blocks * 16;
-        auto doubt = [&](int e) {
-            const float x = s[e];
-            return !(sure && x > above) && !(x < below);
-        };
-        for (int e = begin + warp; e < end; e += warps) {
-            if (!doubt(e)) continue;
-            const double x = exact_score<D>(p, tok, hk, e);
-            if (lane == 0) exact[e] = x;
-        }
-        __syncthreads();
-        int need = rest;
-        unsigned long long value = 0;
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += threads) sm.bins[i] = 0;
-            __syncthreads();
-            for (int e = begin + tid; e < end; e += threads) {
-                if (!doubt(e)) continue;
-                const unsigned long long x = ordered(exact[e]);
-                if (shift == 56 || x >> (shift + 8) == value >> (shift + 8)) atomicAdd(&sm.bins[x >> shift & 255], 1);
+                for (int j = 0; j < all_some; ++j) better += sm.few[j] > x || (sm.few[j] == x && sm.few_at[j] < e);
+                exact[e] = better < rest ? 1.0 : 0.0;
             }
             __syncthreads();
-            if (tid == 0) {
-                int bin = 255, left = need;
-                while (sm.bins[bin] < left) left -= sm.bins[bin--];
-                sm.need = left;
-                sm.value = value | static_cast<unsigned long long>(bin) << shift;
+        } else {
+            // Many that differ by less than the error (alike, most of them): the rest-th largest of their exact scores, eight bits at a time, then
+            // those above it and, of its own value, the first.
+            for (int e = begin + warp; e < end; e += warps) {
+                if (!doubtful(given[e])) continue;
+                const double x = exact_score<D>(p, tok, hk, e);
+                if (lane == 0) exact[e] = x;
             }
             __syncthreads();
-            need = sm.need;
-            value = sm.value;
-            __syncthreads();
-        }
-        // need: how many of the value itself, in the order of their places.
-        if (tid == 0) sm.count = 0;
-        __syncthreads();
-        for (int e0 = begin & ~31; e0 < end; e0 += threads) {
-            const int e = e0 + tid;
-            const bool here = e >= begin && e < end && doubt(e);
-            const unsigned long long x = here ? ordered(exact[e]) : 0;
-            const uint32_t ties = __ballot_sync(0xffffffffu, here && x == value);
-            if (lane == 0) sm.iwarps[warp] = __popc(ties);
-            __syncthreads();
-            int before = sm.count + __popc(ties & ((1u << lane) - 1));
-            for (int w = 0; w < warp; ++w) before += sm.iwarps[w];
-            const bool take = here && (x > value || (x == value && before < need));
-            const uint32_t bits = __ballot_sync(0xffffffffu, take);
-            if (lane == 0 && bits) atomicOr(&in[e >> 5], bits);
-            __syncthreads();
-            if (tid == 0) {
-                for (int w = 0; w < warps; ++w) sm.count += sm.iwarps[w];
+            ties = rest;
+            for (int shift = 56; shift >= 0; shift -= 8) {
+                for (int i = tid; i < 256; i += threads) sm.bins[i] = 0;
+                __syncthreads();
+                each([&](int e, float x) {
+                    if (!doubtful(x)) return;
+                    const unsigned long long y = ordered(exact[e]);
+                    if (shift == 56 || y >> (shift + 8) == value >> (shift + 8)) atomicAdd(&sm.bins[y >> shift & 255], 1);
+                });
+                __syncthreads();
+                if (tid == 0) {
+                    int bin = 255, left = ties;
+                    while (sm.bins[bin] < left) left -= sm.bins[bin--];
+                    sm.need = left;
+                    sm.exact = value | static_cast<unsigned long long>(bin) << shift;
+                }
+                __syncthreads();
+                ties = sm.need;
+                value = sm.exact;
+                __syncthreads();
             }
-            __syncthreads();
+            // Of this thread's pages: those of the value itself, of which the first `ties` of all are in.
+            int equal = 0, all;
+            each([&](int e, float x) { equal += doubtful(x) && ordered(exact[e]) == value; });
+            some_before = sum_before(equal, sm.sums, all);
         }
     }
-    __syncthreads();
-    // The bits in order: a thread has a word of 32 pages.
-    int before = 0;
-    for (int w0 = 0; w0 < words; w0 += threads) {
-        const uint32_t bits = w0 + tid < words ? in[w0 + tid] : 0u;
-        const int own = __popc(bits);
-        int sum = own;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += y;
-        }
-        if (lane == 31) sm.iwarps[warp] = sum;
-        __syncthreads();
-        int at = before + sum - own;
-        for (int w = 0; w < warps; ++w) {
-            const int x = sm.iwarps[w];
-            at += w < warp ? x : 0;
-            before += x;
-        }
-        for (uint32_t left = bits; left; left &= left - 1) {
-            const int e = (w0 + tid) * 32 + __ffs(left) - 1;
-            to[at++] = row[e];
-        }
-        __syncthreads();
+    // Whether a doubtful page is in; asked in the order of a thread's pages.
+    int equal = some_before;
+    auto among = [&](int e) {
+        if (everything) return true;
+        if (all_some <= kFew) return exact[e] != 0.0;
+        const unsigned long long y = ordered(exact[e]);
+        return y > value || (y == value && equal++ < ties);
+    };
+    // The pages that are in, in their order: the first, those of [begin, end), the last.
+    int own = in, all;
+    if (some > 0) {
+        each([&](int e, float x) {
+            if (doubtful(x)) own += among(e);
+        });
     }
+    int at = p.first + sum_before(own, sm.sums, all);
+    equal = some_before;
+    if (own > 0) {
+        each([&](int e, float x) {
+            if (surely(x) || (doubtful(x) && among(e))) to[at++] = row[e];
+        });
+    }
+    for (int i = tid; i < p.first; i += threads) to[i] = row[i];
+    for (int i = tid; i < p.last; i += threads) to[top - p.last + i] = row[end + i];
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -677,34 +735,18 @@ SelectPlan plan_of(const ktt_b200_select_args* a) {
 
 template <int D>
 int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t stream) {
-    const int threads = width <= 512 ? 256 : (width <= 2048 ? 512 : 1024);
-    const int bits = (plan.blocks + 1) / 2 * 4, scores = plan.blocks * 64;
-    constexpr int kMost = 200 * 1024;
-    const bool in_shared = bits + scores <= kMost;
-    const int smem = bits + (in_shared ? scores : 0);
-    if (smem > 32 * 1024) {
-        if (int rc = ensure_smem(select_kernel<D>, kMost, "cudaFuncSetAttribute(select)")) return rc;
-    }
+    const int items = width <= 4096 ? 4 : (width <= 16384 ? 16 : 0);
+    const int threads = items ? std::max(128, (width + 32 * items - 1) / (32 * items) * 32) : 1024;
     for (int64_t t0 = 0; t0 < plan.tokens; t0 += plan.slice) {
         const int64_t n = plan.tokens - t0 < plan.slice ? plan.tokens - t0 : plan.slice, pairs = n * p.kv_heads;
         p.token0 = t0;
-        // Blocks of a warp: as many warps as the GPU holds, and no more than four blocks one after another until it is full.
-        const int64_t all = pairs * plan.blocks, warps = 148 * 16;
-        const int64_t each = (all + warps - 1) / warps;
-        p.each = static_cast<int>(each > 4 ? 4 : each);
+        // Blocks of a warp: as few as there are warps for at a time (8 on an SM).
+        const int64_t all = pairs * plan.blocks, warps = 148 * 8, each = (all + warps - 1) / warps;
+        p.each = static_cast<int>(each > kEach ? kEach : each);
         p.lots = (plan.blocks + 4 * p.each - 1) / (4 * p.each);
         if (int rc = launch_dependent(score_kernel<D>, p, dim3(static_cast<unsigned>(pairs * p.lots)), dim3(128), stream, "paged_select launch")) return rc;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(static_cast<unsigned>(pairs));
-        cfg.blockDim = dim3(static_cast<unsigned>(threads));
-        cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-        cfg.stream = stream;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[0].val.programmaticStreamSerializationAllowed = 1;
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        if (int rc = check_cuda(cudaLaunchKernelEx(&cfg, select_kernel<D>, p, static_cast<int>(in_shared)), "paged_select launch")) return rc;
+        auto kernel = items == 4 ? select_kernel<D, 4> : (items == 16 ? select_kernel<D, 16> : select_kernel<D, 0>);
+        if (int rc = launch_dependent(kernel, p, dim3(static_cast<unsigned>(pairs)), dim3(static_cast<unsigned>(threads)), stream, "paged_select launch")) return rc;
     }
     return 0;
 }
