@@ -9,9 +9,8 @@
 // at most e = 2^-17 max_h sum_d |q_hd| max |bound| (products of bf16 values are exact in fp32; the 2 D / 16 instructions that add up a
 // score round, or cut off, by some 2^-23 of the magnitudes each, together 2^-19; measured 2^-21 at most). The value t of the last page selected
 // lies within e of the last by fp32. So pages more than 2 e above or below are in or out, and those between, a few, get their scores in 64 bits.
-#include <algorithm>
-
 #include "four_bits.cuh"
+#include "split.cuh"
 
 namespace ktt {
 
@@ -176,15 +175,14 @@ struct SelectParams {
     int page_size, cap;
     int top, first, last;
     int blocks;               // of 16 pages, that the table has
-    int lots, each;           // CTAs of a pair, and blocks of a warp of them
-    float* scores;            // [pairs][blocks][16]
-    float* most;              // [pairs][blocks] the largest magnitude among a block's bounds
-    double* exact;            // [pairs][blocks][16]
+    int ranks;                // CTAs of a pair
+    float* scores;            // [pairs][blocks][16]; null: in shared memory
+    double* exact;            // [pairs][blocks][16], of the pages that need them
     int32_t* chosen;
     int32_t* keys;
 };
 
-// A query token: its row of q, its sequence (-1: none), and the keys it sees.
+// A query token: its row of q, its sequence (-1: none), and the keys it sees. By whole warps.
 struct Token {
     const __nv_bfloat16* q;
     int b, seen;
@@ -194,7 +192,18 @@ __device__ __forceinline__ Token token_of(const SelectParams& p, int64_t t) {
     int64_t row = t, place;
     int n;
     if (p.cu) {
-        x.b = sequence_of(p.cu, p.batch, t);
+        // The last sequence that starts at or before t: a warp's lanes look at 32 offsets that are evenly spaced, then between two of them.
+        const int lane = threadIdx.x & 31;
+        int from = 0, many = p.batch + 1;   // offsets that it is among; cu[batch] too, where t lies behind all
+        while (many > 1) {
+            const int step = (many + 31) / 32, i = lane * step;
+            const uint32_t before = __ballot_sync(0xffffffffu, i < many && p.cu[from + min(i, many - 1)] <= t);
+            if (!before) break;   // (t lies before all)
+            const int at = (31 - __clz(before)) * step;
+            from += at;
+            many = min(step, many - at);
+        }
+        x.b = from < p.batch && p.cu[from] <= t ? from : -1;
         x.q = p.q + t * p.qs[2];
         if (x.b < 0) {
             x.seen = 0;
@@ -202,8 +211,13 @@ __device__ __forceinline__ Token token_of(const SelectParams& p, int64_t t) {
         }
         place = t - p.cu[x.b];
         n = p.cu[x.b + 1] - p.cu[x.b];
+        if (place >= n) {   // (offsets that decrease)
+            x.b = -1;
+            x.seen = 0;
+            return x;
+        }
     } else {
-        x.b = static_cast<int>(t / p.sq);
+        x.b = static_cast<int>(static_cast<uint32_t>(t) / static_cast<uint32_t>(p.sq));
         place = row = t - static_cast<int64_t>(x.b) * p.sq;
         n = p.sq;
         x.q = p.q + x.b * p.qs[0] + row * p.qs[2];
@@ -214,153 +228,33 @@ __device__ __forceinline__ Token token_of(const SelectParams& p, int64_t t) {
     return x;
 }
 
-__device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t x) {
-    const uint32_t y = x & 0x7fff7fffu;
-    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&y));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// Both bounds of 16 pages as a warp's lanes load them: lane (g, t) has pages g and g + 8, channels 32 j + 8 t .., in pieces of 16 bytes.
-template <int D>
-struct Sixteen {
-    static constexpr int J = D / 32;
-    uint4 lo[J][2], hi[J][2];
-};
-
-// A warp takes up to kEach blocks of 16 pages of a (token, K / V head), one on its way while another is multiplied. Its lanes load the bounds as
-// they lie, which are the operands of m16n8k16 with the channels in that order; q+ and q- of 8 heads are its columns. Nothing goes
-// through shared memory: no two warps read the same bounds. The products of a block are four sums, for the latency of one.
-constexpr int kEach = 4;
-template <int D>
-__global__ void __launch_bounds__(128, 2) score_kernel(const __grid_constant__ SelectParams p) {
-    constexpr int J = D / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t pair = blockIdx.x / p.lots;
-    const int64_t local = pair / p.kv_heads;
-    const int hk = static_cast<int>(pair - local * p.kv_heads);
-    const Token tok = token_of(p, p.token0 + local);
-    const int count = (tok.seen + p.page_size - 1) / p.page_size;
-    if (count <= p.top) return;   // (all of them)
-    const int block0 = ((static_cast<int>(blockIdx.x) - static_cast<int>(pair) * p.lots) * 4 + warp) * p.each;
-    const int blocks = min(p.each, (count + 15) / 16 - block0);
-    if (blocks <= 0) return;
-    // The names of all its pages, two to a lane.
-    int names[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int e = block0 * 16 + 32 * i + lane;
-        names[i] = 32 * i < blocks * 16 && e < count ? p.table[tok.b * p.table_stride + e] : -1;
-    }
-    auto load = [&](Sixteen<D>& x, int block) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int from = (block & 1) * 16 + g + 8 * i;
-            const int n0 = __shfl_sync(0xffffffffu, names[0], from), n1 = __shfl_sync(0xffffffffu, names[1], from), name = block & 2 ? n1 : n0;
-            const bool there = name >= 0 && name < p.pages;
-            const __nv_bfloat16* at = p.bounds.edge(there ? name : 0, hk, 0) + 8 * t;
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                x.lo[j][i] = x.hi[j][i] = make_uint4(0u, 0u, 0u, 0u);
-                if (there) {
-                    x.lo[j][i] = *reinterpret_cast<const uint4*>(at + 32 * j);
-                    x.hi[j][i] = *reinterpret_cast<const uint4*>(at + p.bounds.stride[2] + 32 * j);
-                }
-            }
-        }
-    };
-    for (int h0 = 0; h0 < p.group; h0 += 8) {   // (more than 8 heads: the bounds come from the cache again)
-        Sixteen<D> x[2];
-        load(x[0], 0);
-        uint32_t up[J][4], down[J][4];
-        {
-            const bool there = h0 + g < p.group;
-            const __nv_bfloat16* from = tok.q + static_cast<int64_t>(hk * p.group + (there ? h0 + g : 0)) * p.qs[1] + 8 * t;
-            const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                const uint4 y4 = *reinterpret_cast<const uint4*>(from + 32 * j);
-                const uint32_t w[4] = {y4.x, y4.y, y4.z, y4.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(&w[i]), u = __hmax2_nan(y, zero), v = __hmin2_nan(y, zero);
-                    up[j][i] = there ? *reinterpret_cast<const uint32_t*>(&u) : 0u;
-                    down[j][i] = there ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
-                }
-            }
-        }
-        auto score = [&](const Sixteen<D>& x, int block) {
-            float acc[4][4];
-            uint32_t most[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-                most[i] = 0u;
-            }
-#pragma unroll
-            for (int j = 0; j < J; ++j) {
-                auto product = [&](const uint4& x, const uint4& y, const uint32_t (&b)[4], int sum) {
-                    const uint32_t a0[4] = {x.x, y.x, x.y, y.y}, a1[4] = {x.z, y.z, x.w, y.w};
-                    mma_bf16(acc[sum], a0, b[0], b[1]);
-                    mma_bf16(acc[sum + 1], a1, b[2], b[3]);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) most[i] = max_magnitude(max_magnitude(most[i], a0[i]), a1[i]);
-                };
-                product(x.hi[j][0], x.hi[j][1], up[j], 0);
-                product(x.lo[j][0], x.lo[j][1], down[j], 2);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[0][i] = (acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]);
-            // The largest of the columns that are heads.
-            const bool c0 = h0 + 2 * t < p.group, c1 = h0 + 2 * t + 1 < p.group;
-            float s[2] = {fmaxf(c0 ? acc[0][0] : -INFINITY, c1 ? acc[0][1] : -INFINITY), fmaxf(c0 ? acc[0][2] : -INFINITY, c1 ? acc[0][3] : -INFINITY)};
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 1));
-                s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 2));
-            }
-            float* to = p.scores + (pair * p.blocks + block0 + block) * 16;
-            if (t == 0) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    if (h0 > 0) s[i] = fmaxf(s[i], to[g + 8 * i]);
-                    to[g + 8 * i] = s[i];
-                }
-            }
-            if (h0 == 0) {
-                uint32_t m = max_magnitude(max_magnitude(most[0], most[1]), max_magnitude(most[2], most[3]));
-#pragma unroll
-                for (int off = 1; off < 32; off <<= 1) m = max_magnitude(m, __shfl_xor_sync(0xffffffffu, m, off));
-                const __nv_bfloat162 m2 = *reinterpret_cast<const __nv_bfloat162*>(&m);
-                if (lane == 0) p.most[pair * p.blocks + block0 + block] = __bfloat162float(__hmax_nan(__low2bfloat16(m2), __high2bfloat16(m2)));
-            }
-        };
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            if (i >= blocks) break;
-            if (i + 1 < blocks) load(x[(i + 1) & 1], i + 1);
-            score(x[i & 1], i);
-        }
-    }
-}
-
-// ---- the selection -----------------------------------------------------------------------------
-
-constexpr int kBins = 512;
+constexpr int kWarps = 4;        // of a CTA
+constexpr int kMaxRanks = 8;
 constexpr int kFew = 256;        // pages between in and out that are ranked one against the others
 
+// A warp's ring: blocks of 16 pages' bounds, a row of 4 D bytes each and 16 more, so that eight rows of a matrix lie in different banks.
+template <int D>
+struct Ring {
+    static constexpr int kRow = 4 * D + 16;
+    static constexpr int kBlock = 16 * kRow;
+    static constexpr int kStages = D == 128 ? 3 : 4;
+    static constexpr int kBytes = kWarps * kStages * kBlock;
+};
+
 struct SelectShared {
-    int bins[kBins + kBins / 16];   // (a place more for every 16: warp 0 reads 16 to a lane)
-    float warps[4][32];
-    int sums[32];
-    float ranked[32];
-    int few_at[kFew];
-    double few[kFew];
-    int bin, in_bin, need, count, found, all_in, lo_bits, hi_bits;
+    uint32_t most[kMaxRanks * kWarps];   // magnitudes among the bounds, by warp
+    int4 counts[2][kWarps];
+    int ends[2][2][kWarps];
+    int sums[kWarps];
+    int count, all_in, need;
     unsigned long long exact;
 };
-__device__ __forceinline__ int bin_at(int bin) { return bin + (bin >> 4); }
+// Of the selection, where the ring was.
+struct SelectLater {
+    double few[kFew];
+    int few_at[kFew];
+    int bins[256];
+};
 
 // Order of floats as that of integers.
 __device__ __forceinline__ int ordered(float x) {
@@ -372,11 +266,10 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
     const unsigned long long i = __double_as_longlong(x);
     return i >> 63 ? ~i : i | 1ull << 63;
 }
-__device__ __forceinline__ float larger(float a, float b) { return a != a || a > b ? a : b; }   // (a NaN stays)
 
-// Exclusive sum of x over the CTA, and that of all. Two barriers.
-__device__ __forceinline__ int sum_before(int x, int* warps, int& all) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = blockDim.x >> 5;
+// Exclusive sum of x over the CTA. Two barriers.
+__device__ __forceinline__ int sum_before(int x, int* warps) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int sum = x;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -385,16 +278,18 @@ __device__ __forceinline__ int sum_before(int x, int* warps, int& all) {
     }
     if (lane == 31) warps[warp] = sum;
     __syncthreads();
-    const int other = lane < n ? warps[lane] : 0;
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? other : 0);
-    all = __reduce_add_sync(0xffffffffu, other);
+    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? warps[lane] : 0);
     __syncthreads();
     return before + sum - x;
 }
 
+// Stores to shared memory of the cluster's first CTA.
+__device__ __forceinline__ void to_first(uint32_t at, float x) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
+__device__ __forceinline__ void to_first(uint32_t at, int x) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); }
+
 // The exact score of a page: 64-bit sums of products that are exact themselves. By one warp.
 template <int D>
-__device__ __forceinline__ double exact_score(const SelectParams& p, const Token& tok, int hk, int e) {
+__device__ __noinline__ double exact_score(const SelectParams& p, const Token& tok, int hk, int e) {
     const int lane = threadIdx.x & 31;
     constexpr int kMine = D / 32;
     const int64_t page = p.table[tok.b * p.table_stride + e];
@@ -423,35 +318,174 @@ __device__ __forceinline__ double exact_score(const SelectParams& p, const Token
     return best + 0.0;   // (no -0)
 }
 
-// One CTA for a (token, K / V head); a thread has kItems neighbouring pages, their scores and names in registers (0: as many as there are, which
-// it reads again each time). The k-th largest of the scores is found by bins of equal width between the least and the largest, then by
-// rank among the few of its bin. Bound: latency, some ten barriers and two trips to memory.
-template <int D, int kItems>
-__global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ SelectParams p) {
+// A cluster of `ranks` CTAs has a (token, K / V head): all of their warps score its pages, the first selects.
+//
+// Scores: a warp takes neighbouring blocks of 16 pages through a ring of its own, two or three on their way while one is multiplied: pages are the
+// rows of m16n8k16, q+ and q- of 8 heads its columns. (Bounds in registers as they come, two blocks to a warp, were no faster than one after the
+// other: 16 us for 38 MB.) The products of a block are four sums, for the latency of one.
+//
+// Selection: the value of the k-th largest score by quarters of an interval, with counts of what lies above; a thread has kItems
+// neighbouring pages in registers (0: reads them each time). kNear: scores and names lie in shared memory, else scores where the workspace is.
+// Measured, us: 8 pairs of 1,024 pages, D 128, and 128 of 128 to 1,024: 10.3 and 23.8 in two launches, scores through memory and bins of
+// equal width for the k-th.
+template <int D, int kItems, bool kNear>
+__global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_constant__ SelectParams p) {
+    using R = Ring<D>;
+    constexpr int K = D / 16, NS = R::kStages;
+    extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ SelectShared sm;
-    const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = threads / 32;
-    for (int i = tid; i < kBins + kBins / 16; i += threads) sm.bins[i] = 0;
-    if (tid == 0) sm.count = sm.found = sm.all_in = 0;
+    SelectLater& later = *reinterpret_cast<SelectLater*>(dynamic);
+    static_assert(sizeof(SelectLater) <= R::kBytes, "where the ring was");
+    float* score_s = reinterpret_cast<float*>(dynamic + R::kBytes);           // kNear: [blocks][16]
+    int* name_s = reinterpret_cast<int*>(score_s + p.blocks * 16);
+    constexpr int threads = 32 * kWarps, warps = kWarps;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
+    if (tid == 0) sm.count = sm.all_in = 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t pair = blockIdx.x, local = pair / p.kv_heads, t = p.token0 + local;
-    const int hk = static_cast<int>(pair - local * p.kv_heads);
+    const uint32_t pair = blockIdx.x / static_cast<uint32_t>(p.ranks), local = pair / static_cast<uint32_t>(p.kv_heads);
+    const int rank = static_cast<int>(blockIdx.x - pair * p.ranks), hk = static_cast<int>(pair - local * p.kv_heads);
+    const int64_t t = p.token0 + local;
     const Token tok = token_of(p, t);
-    const int count = (tok.seen + p.page_size - 1) / p.page_size, top = p.top;
+    const int count = static_cast<int>((static_cast<uint32_t>(tok.seen) + p.page_size - 1) / static_cast<uint32_t>(p.page_size)), top = p.top;
     int32_t* to = p.chosen + (t * p.kv_heads + hk) * top;
     const int32_t* row = p.table + max(tok.b, 0) * p.table_stride;
-    if (tid == 0) {
+    if (rank == 0 && tid == 0) {
         const int many = min(count, top);
         p.keys[t * p.kv_heads + hk] = many > 0 ? (many - 1) * p.page_size + (tok.seen - 1) % p.page_size + 1 : 0;
     }
-    if (count <= top) {
-        for (int i = tid; i < top; i += threads) to[i] = i < count ? row[i] : -1;
+    if (count <= top) {   // all of them
+        for (int i = rank * threads + tid; i < top; i += threads * p.ranks) to[i] = i < count ? row[i] : -1;
         return;
     }
-    const float* given = p.scores + pair * p.blocks * 16;
+    float* given = kNear ? score_s : p.scores + static_cast<int64_t>(pair) * p.blocks * 16;
+
+    // ---- scores
+    float norm = 0.f;        // the largest sum of magnitudes of a head's query
+    {
+        const int all = (count + 15) / 16, each = (all + p.ranks * warps - 1) / (p.ranks * warps);
+        const int block0 = (rank * warps + warp) * each, blocks = min(each, all - block0);
+        const uint32_t ring = smem_u32(dynamic + warp * NS * R::kBlock), first_scores = in_rank(smem_u32(score_s), 0), first_names = in_rank(smem_u32(name_s), 0);
+        // Names of two blocks, a lane each.
+        auto names_of = [&](int block) {
+            const int i = (block0 + block) * 16 + lane;
+            return block < blocks && lane < (blocks - block) * 16 && i < count ? row[i] : -1;
+        };
+        int names = names_of(0), next = names_of(2);
+        int issued = 0;
+        auto issue = [&]() {   // a block's bounds, a page's with one instruction (D 64: two pages' with one)
+            if (issued < blocks) {
+                const int half = issued & 1;
+                const uint32_t to = ring + (issued % NS) * R::kBlock;
+                constexpr int kLanes = D / 4, kPages = 32 / kLanes;   // lanes to a page
+                const int at = lane % kLanes * 8, edge = at / D;
+                const __nv_bfloat16* from = p.bounds.at + hk * p.bounds.stride[1] + edge * p.bounds.stride[2] + (at - edge * D);
+#pragma unroll
+                for (int i = 0; i < 16; i += kPages) {
+                    const int r = i + lane / kLanes, name = __shfl_sync(0xffffffffu, names, half * 16 + r);
+                    const bool there = name >= 0 && name < p.pages;
+                    cp_async_16(to + r * R::kRow + at * 2, from + (there ? name : 0) * p.bounds.stride[0], there);
+                }
+                if constexpr (kNear) {
+                    if ((lane >> 4) == half) to_first(first_names + ((block0 + issued) * 16 + (lane & 15)) * 4, names);
+                }
+                ++issued;
+                if (half) {
+                    names = next;
+                    next = names_of(issued + 2);
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) issue();
+        uint32_t up[K][2], down[K][2];
+        auto queries = [&](int h0) {   // of heads h0 .. h0 + 7
+            const bool there = h0 + g < p.group;
+            const __nv_bfloat16* from = tok.q + static_cast<int64_t>(hk * p.group + (there ? h0 + g : 0)) * p.qs[1] + 2 * t4;
+            const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(from + 16 * k + 8 * i), u = __hmax2_nan(y, zero), v = __hmin2_nan(y, zero);
+                    up[k][i] = there ? *reinterpret_cast<const uint32_t*>(&u) : 0u;
+                    down[k][i] = there ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
+                    const float2 f = __bfloat1622float2(y);
+                    sum += there ? fabsf(f.x) + fabsf(f.y) : 0.f;
+                }
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            // (as an integer, which a NaN is the largest of)
+            norm = __uint_as_float(__reduce_max_sync(0xffffffffu, max(__float_as_uint(sum), __float_as_uint(norm))));
+        };
+        for (int h0 = (p.group - 1) / 8 * 8; h0 >= 0; h0 -= 8) queries(h0);   // (of all for the norm, which all warps need)
+        __nv_bfloat162 largest[2], least[2];
+        largest[0] = largest[1] = least[0] = least[1] = __float2bfloat162_rn(0.f);
+        for (int block = 0; block < blocks; ++block) {
+            issue();
+            cp_async_wait<NS - 1>();
+            __syncwarp();
+            const uint32_t from = ring + (block % NS) * R::kBlock + ((lane & 7) + ((lane >> 3) & 1) * 8) * R::kRow + (lane >> 4) * 16;
+            float s[2] = {-INFINITY, -INFINITY};
+            for (int h0 = 0; h0 < p.group; h0 += 8) {
+                if (p.group > 8) queries(h0);
+                float acc[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    uint32_t lo[4], hi[4];
+                    ldmatrix_x4(lo, from + k * 32);
+                    ldmatrix_x4(hi, from + 2 * D + k * 32);
+                    mma_bf16(acc[k & 1], hi, up[k][0], up[k][1]);
+                    mma_bf16(acc[2 + (k & 1)], lo, down[k][0], down[k][1]);
+                    if (h0 == 0) {   // (the largest magnitude is that of a largest or a least value)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            largest[i & 1] = __hmax2_nan(largest[i & 1], *reinterpret_cast<const __nv_bfloat162*>(&hi[i]));
+                            least[i & 1] = __hmin2_nan(least[i & 1], *reinterpret_cast<const __nv_bfloat162*>(&lo[i]));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[0][i] = (acc[0][i] + acc[1][i]) + (acc[2][i] + acc[3][i]);
+                // The largest of the columns that are heads.
+                const bool c0 = h0 + 2 * t4 < p.group, c1 = h0 + 2 * t4 + 1 < p.group;
+                s[0] = fmaxf(s[0], fmaxf(c0 ? acc[0][0] : -INFINITY, c1 ? acc[0][1] : -INFINITY));
+                s[1] = fmaxf(s[1], fmaxf(c0 ? acc[0][2] : -INFINITY, c1 ? acc[0][3] : -INFINITY));
+            }
+            __syncwarp();   // (all lanes are done with the stage before it is filled again)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 1));
+                s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 2));
+            }
+            if (t4 == 0) {
+                const int e = (block0 + block) * 16 + g;
+                if constexpr (kNear) {
+                    to_first(first_scores + e * 4, s[0]);
+                    to_first(first_scores + (e + 8) * 4, s[1]);
+                } else {
+                    given[e] = s[0];
+                    given[e + 8] = s[1];
+                }
+            }
+        }
+        cp_async_wait<0>();
+        const __nv_bfloat162 high = __hmax2_nan(__hmax2_nan(largest[0], largest[1]), __hneg2(__hmin2_nan(least[0], least[1])));
+        const uint32_t bits = *reinterpret_cast<const uint32_t*>(&high) & 0x7fff7fffu;
+        const uint32_t most = __reduce_max_sync(0xffffffffu, max(bits & 0xffffu, bits >> 16)) << 16;   // (bf16 magnitudes as integers, a NaN above all)
+        if (lane == 0) to_first(in_rank(smem_u32(&sm.most[rank * warps + warp]), 0), static_cast<int>(most));
+    }
+    if (p.ranks > 1) cluster_meet(); else __syncthreads();
+    if (rank > 0) return;   // (nobody looks at its shared memory)
+
+    // ---- the selection, by the first CTA
     const int begin = p.first, end = count - p.last, k = top - p.first - p.last;   // the k largest of [begin, end), which are more
     const int mine = kItems ? kItems : ((count + threads - 1) / threads + 3) & ~3, first = tid * mine;
-    // All its pages: f(page, score, place among its own).
     float held[kItems ? kItems : 1];
     if constexpr (kItems > 0) {
 #pragma unroll
@@ -461,7 +495,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
             held[i] = x.x; held[i + 1] = x.y; held[i + 2] = x.z; held[i + 3] = x.w;
         }
     }
-    auto each = [&](auto f) {
+    auto each = [&](auto f) {   // its pages and their scores
         if constexpr (kItems > 0) {
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
@@ -471,120 +505,72 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
             for (int e = max(first, begin); e < min(first + mine, end); ++e) f(e, given[e]);
         }
     };
-    // The least and the largest, and what the scores may be off by.
-    float lo = INFINITY, hi = -INFINITY, most = 0.f, norm = 0.f;
-    for (int h = warp; h < p.group; h += warps) {
-        const __nv_bfloat16* q = tok.q + static_cast<int64_t>(hk * p.group + h) * p.qs[1] + lane * (D / 32);
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 32; i += 2) {
-            const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(q + i));
-            sum += fabsf(y.x) + fabsf(y.y);
+    auto name_of = [&](int e) { return kNear ? name_s[e] : row[e]; };
+    // The least and the largest of the CTA.
+    auto ends_of = [&](float& lo, float& hi, int which) {
+        const int a = __reduce_min_sync(0xffffffffu, ordered(lo)), b = __reduce_max_sync(0xffffffffu, ordered(hi));
+        if (lane == 0) {
+            sm.ends[which][0][warp] = a;
+            sm.ends[which][1][warp] = b;
         }
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        norm = larger(sum, norm);
-    }
-    for (int i = tid; i < (count + 15) / 16; i += threads) most = larger(p.most[pair * p.blocks + i], most);
+        __syncthreads();
+        lo = from_ordered(__reduce_min_sync(0xffffffffu, sm.ends[which][0][lane % warps]));
+        hi = from_ordered(__reduce_max_sync(0xffffffffu, sm.ends[which][1][lane % warps]));
+    };
+    float lo = INFINITY, hi = -INFINITY;
     each([&](int, float x) {
         lo = fminf(lo, x);
         hi = fmaxf(hi, x);
     });
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-        most = larger(most, __shfl_xor_sync(0xffffffffu, most, off));
-    }
-    if (lane == 0) {
-        sm.warps[0][warp] = lo;
-        sm.warps[1][warp] = hi;
-        sm.warps[2][warp] = most;
-        sm.warps[3][warp] = norm;
-    }
-    __syncthreads();
-    lo = lane < warps ? sm.warps[0][lane] : INFINITY;
-    hi = lane < warps ? sm.warps[1][lane] : -INFINITY;
-    most = lane < warps ? sm.warps[2][lane] : 0.f;
-    norm = lane < warps ? sm.warps[3][lane] : 0.f;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-        most = larger(most, __shfl_xor_sync(0xffffffffu, most, off));
-        norm = larger(norm, __shfl_xor_sync(0xffffffffu, norm, off));
-    }
-    const float mass = norm * most;
-    // (What the products could lose below fp32's least normal number is in the last terms.)
+    ends_of(lo, hi, 0);
+    const uint32_t largest = __reduce_max_sync(0xffffffffu, lane < p.ranks * warps ? sm.most[lane] : 0u);
+    const float most = __uint_as_float(largest), mass = norm * most;
+    // What the fp32 scores may be off by. (What the products could lose below fp32's least normal number is in the last terms.)
     const float off = fmaf(mass, 0x1p-17f, fmaf(norm + most, 0x1p-110f, 0x1p-110f));
     const bool sure = mass < 0x1p120f;   // else, and where it is no number: all in 64 bits
-    int need = k;
-    for (int round = 0; round < 4 && sure && k > 0 && hi - lo > 4.f * off; ++round) {
-        const float by = (kBins - 0.5f) / (hi - lo);
-        if (!(by < 0x1p100f)) break;
-        auto bin_of = [&](float x) { return static_cast<int>((x - lo) * by); };   // (falls nowhere as x rises)
-        each([&](int, float x) {
-            if (x >= lo && x <= hi) atomicAdd(&sm.bins[bin_at(bin_of(x))], 1);
-        });
-        __syncthreads();
-        if (warp == 0) {
-            // Lane l has the 16 bins from kBins - 16 l down: those above the one that has the need-th, and it.
-            int own[16], sum = 0;
+    if (sure && k > 0) {
+        // The k-th largest is in (a, b], and `between` scores are.
+        float a = lo - off, b = hi;
+        int above_a = end - begin, above_b = 0;
+        for (int round = 0; round < 24 && above_a - above_b > 1 && b - a > off; ++round) {
+            const float w = b - a, c[3] = {fmaf(w, 0.25f, a), fmaf(w, 0.5f, a), fmaf(w, 0.75f, a)};
+            int n[3] = {0, 0, 0};
+            each([&](int, float x) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum += own[i] = sm.bins[bin_at(kBins - 1 - 16 * lane - i)];
-            int upto = sum;
+                for (int i = 0; i < 3; ++i) n[i] += x > c[i];
+            });
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += y;
-            }
-            int above = upto - sum;
-            if (above < need && upto >= need) {
+            for (int i = 0; i < 3; ++i) n[i] = __reduce_add_sync(0xffffffffu, n[i]);
+            if (lane == 0) sm.counts[round & 1][warp] = make_int4(n[0], n[1], n[2], 0);
+            __syncthreads();
+            const int4 other = lane < warps ? sm.counts[round & 1][lane] : make_int4(0, 0, 0, 0);
+            n[0] = __reduce_add_sync(0xffffffffu, other.x);
+            n[1] = __reduce_add_sync(0xffffffffu, other.y);
+            n[2] = __reduce_add_sync(0xffffffffu, other.z);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    if (above < need && above + own[i] >= need) {
-                        sm.bin = kBins - 1 - 16 * lane - i;
-                        sm.in_bin = own[i];
-                        sm.need = need - above;
-                    }
-                    above += own[i];
+            for (int i = 0; i < 3; ++i) {   // (n falls)
+                if (n[i] >= k) {
+                    a = c[i];
+                    above_a = n[i];
                 }
             }
-            if (lane == 0) {
-                sm.lo_bits = 0x7fffffff;
-                sm.hi_bits = static_cast<int>(0x80000000);
+#pragma unroll
+            for (int i = 2; i >= 0; --i) {
+                if (n[i] < k) {
+                    b = c[i];
+                    above_b = n[i];
+                }
             }
         }
-        __syncthreads();
-        const int bin = sm.bin, many = sm.in_bin;
-        need = sm.need;
-        if (many <= 32) {
-            each([&](int, float x) {
-                if (x >= lo && x <= hi && bin_of(x) == bin) sm.ranked[atomicAdd(&sm.found, 1)] = x;
-            });
-            __syncthreads();
-            // The need-th largest of them (equal ones in any order): every warp for itself.
-            const float x = lane < many ? sm.ranked[lane] : -INFINITY;
-            int better = 0;
-            for (int i = 0; i < many; ++i) {
-                const float y = __shfl_sync(0xffffffffu, x, i);
-                better += y > x || (y == x && i < lane);
-            }
-            const uint32_t it = __ballot_sync(0xffffffffu, lane < many && better == need - 1);
-            lo = hi = __shfl_sync(0xffffffffu, x, __ffs(it) - 1);
-            break;
-        }
+        lo = INFINITY;
+        hi = -INFINITY;
         each([&](int, float x) {
-            if (x >= lo && x <= hi && bin_of(x) == bin) {
-                atomicMin(&sm.lo_bits, ordered(x));
-                atomicMax(&sm.hi_bits, ordered(x));
+            if (x > a && x <= b) {
+                lo = fminf(lo, x);
+                hi = fmaxf(hi, x);
             }
         });
-        for (int i = tid; i < kBins + kBins / 16; i += threads) sm.bins[i] = 0;
-        __syncthreads();
-        lo = from_ordered(sm.lo_bits);
-        hi = from_ordered(sm.hi_bits);
-        __syncthreads();
+        ends_of(lo, hi, 1);
     }
     // Pages above are in, pages below are out; those between are counted, and listed while they are few.
     const float above = sure ? hi + 2.f * off : INFINITY, below = sure ? lo - 2.f * off : -INFINITY;
@@ -597,7 +583,7 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
             if (doubtful(x)) {
                 ++some;
                 const int at = atomicAdd(&sm.count, 1);
-                if (at < kFew) sm.few_at[at] = e;
+                if (at < kFew) later.few_at[at] = e;
             }
         });
     }
@@ -607,22 +593,22 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
     const int all_some = sm.count, rest = k - sm.all_in;   // so many of the doubtful ones are in
     const bool everything = all_some == rest;
     int some_before = 0;
-    double* exact = p.exact + pair * p.blocks * 16;
+    double* exact = p.exact + static_cast<int64_t>(pair) * p.blocks * 16;
     unsigned long long value = 0;
     int ties = 0;
     if (k > 0 && !everything) {
         if (all_some <= kFew) {
             for (int i = warp; i < all_some; i += warps) {
-                const double x = exact_score<D>(p, tok, hk, sm.few_at[i]);
-                if (lane == 0) sm.few[i] = x;
+                const double x = exact_score<D>(p, tok, hk, later.few_at[i]);
+                if (lane == 0) later.few[i] = x;
             }
             __syncthreads();
-            // The rest-th in the order of score and place: pages at or before it are in.
+            // In the order of score and place, the first `rest` are in.
             for (int i = tid; i < all_some; i += threads) {
-                const double x = sm.few[i];
-                const int e = sm.few_at[i];
+                const double x = later.few[i];
+                const int e = later.few_at[i];
                 int better = 0;
-                for (int j = 0; j < all_some; ++j) better += sm.few[j] > x || (sm.few[j] == x && sm.few_at[j] < e);
+                for (int j = 0; j < all_some; ++j) better += later.few[j] > x || (later.few[j] == x && later.few_at[j] < e);
                 exact[e] = better < rest ? 1.0 : 0.0;
             }
             __syncthreads();
@@ -637,17 +623,17 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
             __syncthreads();
             ties = rest;
             for (int shift = 56; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += threads) sm.bins[i] = 0;
+                for (int i = tid; i < 256; i += threads) later.bins[i] = 0;
                 __syncthreads();
                 each([&](int e, float x) {
                     if (!doubtful(x)) return;
                     const unsigned long long y = ordered(exact[e]);
-                    if (shift == 56 || y >> (shift + 8) == value >> (shift + 8)) atomicAdd(&sm.bins[y >> shift & 255], 1);
+                    if (shift == 56 || y >> (shift + 8) == value >> (shift + 8)) atomicAdd(&later.bins[y >> shift & 255], 1);
                 });
                 __syncthreads();
                 if (tid == 0) {
                     int bin = 255, left = ties;
-                    while (sm.bins[bin] < left) left -= sm.bins[bin--];
+                    while (later.bins[bin] < left) left -= later.bins[bin--];
                     sm.need = left;
                     sm.exact = value | static_cast<unsigned long long>(bin) << shift;
                 }
@@ -657,9 +643,9 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
                 __syncthreads();
             }
             // Of this thread's pages: those of the value itself, of which the first `ties` of all are in.
-            int equal = 0, all;
+            int equal = 0;
             each([&](int e, float x) { equal += doubtful(x) && ordered(exact[e]) == value; });
-            some_before = sum_before(equal, sm.sums, all);
+            some_before = sum_before(equal, sm.sums);
         }
     }
     // Whether a doubtful page is in; asked in the order of a thread's pages.
@@ -671,21 +657,21 @@ __global__ void __launch_bounds__(1024) select_kernel(const __grid_constant__ Se
         return y > value || (y == value && equal++ < ties);
     };
     // The pages that are in, in their order: the first, those of [begin, end), the last.
-    int own = in, all;
+    int own = in;
     if (some > 0) {
         each([&](int e, float x) {
             if (doubtful(x)) own += among(e);
         });
     }
-    int at = p.first + sum_before(own, sm.sums, all);
+    int at = p.first + sum_before(own, sm.sums);
     equal = some_before;
     if (own > 0) {
         each([&](int e, float x) {
-            if (surely(x) || (doubtful(x) && among(e))) to[at++] = row[e];
+            if (surely(x) || (doubtful(x) && among(e))) to[at++] = name_of(e);
         });
     }
-    for (int i = tid; i < p.first; i += threads) to[i] = row[i];
-    for (int i = tid; i < p.last; i += threads) to[top - p.last + i] = row[end + i];
+    for (int i = tid; i < p.first; i += threads) to[i] = name_of(i);
+    for (int i = tid; i < p.last; i += threads) to[top - p.last + i] = name_of(end + i);
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -696,8 +682,10 @@ constexpr int64_t kWorkspace = 256ll << 20;        // bytes of scores at a time
 struct SelectPlan {
     int64_t tokens, slice;   // of all, of a launch
     int blocks;
-    int64_t most_at, exact_at, bytes;
+    bool near;               // scores and names in shared memory
+    int64_t exact_at, bytes;
 };
+constexpr int kNearBytes = 64 * 1024;   // 8,192 pages
 
 const char* select_refusal(const ktt_b200_select_args* a) {
     if (a->d != 64 && a->d != 128) return "head dim 64 or 128";
@@ -720,33 +708,51 @@ SelectPlan plan_of(const ktt_b200_select_args* a) {
     SelectPlan s = {};
     s.tokens = a->cu_seqlens_q ? a->total_q : static_cast<int64_t>(a->batch) * a->sq;
     s.blocks = (a->table_width + 15) / 16;
-    const int64_t one = static_cast<int64_t>(a->kv_heads) * s.blocks * (16 * 12 + 4);   // (scores, exact ones, magnitudes)
+    s.near = s.blocks * 128 <= kNearBytes;
+    const int64_t one = static_cast<int64_t>(a->kv_heads) * s.blocks * 16 * (s.near ? 8 : 12);   // exact scores, and others
     int64_t most = kWorkspace / one;
-    const int64_t pairs = (1ll << 30) / (static_cast<int64_t>(a->kv_heads) * s.blocks);   // CTAs of a launch
-    if (most > pairs) most = pairs;
+    const int64_t ctas = (1ll << 30) / (static_cast<int64_t>(a->kv_heads) * kMaxRanks);   // of a launch
+    if (most > ctas) most = ctas;
     s.slice = most < 1 ? 1 : (most < s.tokens ? most : s.tokens);
-    auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
-    const int64_t n = s.slice * a->kv_heads * s.blocks;
-    s.exact_at = up(n * 64);
-    s.most_at = s.exact_at + up(n * 128);
-    s.bytes = s.most_at + up(n * 4);
+    const int64_t n = s.slice * a->kv_heads * s.blocks * 16;
+    s.exact_at = s.near ? 0 : (n * 4 + 255) / 256 * 256;
+    s.bytes = s.exact_at + n * 8;
     return s;
+}
+
+template <int D, int kItems, bool kNear>
+int launch_select(const SelectParams& p, int64_t pairs, cudaStream_t stream) {
+    auto kernel = select_kernel<D, kItems, kNear>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.ranks));
+    cfg.blockDim = dim3(32 * kWarps);
+    cfg.dynamicSmemBytes = Ring<D>::kBytes + (kNear ? static_cast<size_t>(p.blocks) * 128 : 0);
+    cfg.stream = stream;
+    if (int rc = ensure_smem(kernel, Ring<D>::kBytes + (kNear ? kNearBytes : 0), "cudaFuncSetAttribute(select)")) return rc;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(p.ranks);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "paged_select launch");
 }
 
 template <int D>
 int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t stream) {
-    const int items = width <= 4096 ? 4 : (width <= 16384 ? 16 : 0);
-    const int threads = items ? std::max(128, (width + 32 * items - 1) / (32 * items) * 32) : 1024;
     for (int64_t t0 = 0; t0 < plan.tokens; t0 += plan.slice) {
         const int64_t n = plan.tokens - t0 < plan.slice ? plan.tokens - t0 : plan.slice, pairs = n * p.kv_heads;
         p.token0 = t0;
-        // Blocks of a warp: as few as there are warps for at a time (8 on an SM).
-        const int64_t all = pairs * plan.blocks, warps = 148 * 8, each = (all + warps - 1) / warps;
-        p.each = static_cast<int>(each > kEach ? kEach : each);
-        p.lots = (plan.blocks + 4 * p.each - 1) / (4 * p.each);
-        if (int rc = launch_dependent(score_kernel<D>, p, dim3(static_cast<unsigned>(pairs * p.lots)), dim3(128), stream, "paged_select launch")) return rc;
-        auto kernel = items == 4 ? select_kernel<D, 4> : (items == 16 ? select_kernel<D, 16> : select_kernel<D, 0>);
-        if (int rc = launch_dependent(kernel, p, dim3(static_cast<unsigned>(pairs)), dim3(static_cast<unsigned>(threads)), stream, "paged_select launch")) return rc;
+        // Two CTAs to an SM: as many to a pair as there is room for and blocks for all their warps.
+        p.ranks = 1;
+        while (p.ranks < kMaxRanks && pairs * p.ranks * 2 <= 2 * 148 && p.ranks * kWarps < plan.blocks) p.ranks *= 2;
+        int rc;
+        if (!plan.near) rc = launch_select<D, 0, false>(p, pairs, stream);
+        else if (width <= 8 * 32 * kWarps) rc = launch_select<D, 8, true>(p, pairs, stream);
+        else rc = launch_select<D, 0, true>(p, pairs, stream);
+        if (rc) return rc;
     }
     return 0;
 }
@@ -830,9 +836,8 @@ extern "C" int ktt_b200_paged_select(const ktt_b200_select_args* a, void* stream
     p.last = a->last;
     p.blocks = s.blocks;
     unsigned char* base = static_cast<unsigned char*>(a->workspace);
-    p.scores = reinterpret_cast<float*>(base);
+    p.scores = s.near ? nullptr : reinterpret_cast<float*>(base);
     p.exact = reinterpret_cast<double*>(base + s.exact_at);
-    p.most = reinterpret_cast<float*>(base + s.most_at);
     p.chosen = a->chosen;
     p.keys = a->keys;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
