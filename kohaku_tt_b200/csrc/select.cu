@@ -5,10 +5,11 @@
 // so the scores of all pages are two matrix products with the queries of a K / V head's group as columns. Bound: the reading of the
 // bounds, 4 D bytes a page and head (1 / P of the cache in bf16, for pages of P keys).
 //
-// What is selected is decided by the exact scores, so that it does not depend on an order of summation: the products' sums are fp32, off by
-// at most e = 2^-17 max_h sum_d |q_hd| max |bound| (products of bf16 values are exact in fp32; the 2 D / 16 instructions that add up a
-// score round, or cut off, by some 2^-23 of the magnitudes each, together 2^-19; measured 2^-21 at most). The value t of the last page selected
-// lies within e of the last by fp32. So pages more than 2 e above or below are in or out, and those between, a few, get their scores in 64 bits.
+// What is selected is decided by the exact scores, so that it does not depend on an order of summation. The products of bf16 values are exact in
+// fp32; a score is the sum of four sums of up to 4 matrix instructions each, of which every one is off by 2^-22 of the magnitudes that it adds
+// up at most (two bits more than a sum of fp32 rounds by), all in all by e = 2^-19 max_h sum_d |q_hd| max |bound|. So the value of the
+// last page selected lies within e of the last by fp32: pages more than 2 e above or below are in or out, and those between, one or a few, get their
+// scores in 64 bits where they are not all in. (2 to 5 in 100 selections among 1,024 pages.)
 #include "four_bits.cuh"
 #include "split.cuh"
 
@@ -174,7 +175,7 @@ struct SelectParams {
     int64_t pages;
     int page_size, cap;
     int top, first, last;
-    int blocks;               // of 16 pages, that the table has
+    int width, blocks;        // pages that the table has, and blocks of 16
     int ranks;                // CTAs of a pair
     float* scores;            // [pairs][blocks][16]; null: in shared memory
     double* exact;            // [pairs][blocks][16], of the pages that need them
@@ -182,15 +183,14 @@ struct SelectParams {
     int32_t* keys;
 };
 
-// A query token: its row of q, its sequence (-1: none), and the keys it sees. By whole warps.
+// A query token: its row of q, its sequence (-1: none), and where in it. By whole warps.
 struct Token {
     const __nv_bfloat16* q;
-    int b, seen;
+    int b;
+    int64_t place, of;   // the how-many-th of its sequence's tokens, and how many there are
 };
 __device__ __forceinline__ Token token_of(const SelectParams& p, int64_t t) {
     Token x;
-    int64_t row = t, place;
-    int n;
     if (p.cu) {
         // The last sequence that starts at or before t: a warp's lanes look at 32 offsets that are evenly spaced, then between two of them.
         const int lane = threadIdx.x & 31;
@@ -203,29 +203,28 @@ __device__ __forceinline__ Token token_of(const SelectParams& p, int64_t t) {
             from += at;
             many = min(step, many - at);
         }
-        x.b = from < p.batch && p.cu[from] <= t ? from : -1;
         x.q = p.q + t * p.qs[2];
-        if (x.b < 0) {
-            x.seen = 0;
-            return x;
-        }
-        place = t - p.cu[x.b];
-        n = p.cu[x.b + 1] - p.cu[x.b];
-        if (place >= n) {   // (offsets that decrease)
-            x.b = -1;
-            x.seen = 0;
-            return x;
+        x.b = -1;
+        x.place = x.of = 0;
+        if (from < p.batch && p.cu[from] <= t) {
+            x.place = t - p.cu[from];
+            x.of = p.cu[from + 1] - p.cu[from];
+            if (x.place < x.of) x.b = from;   // (offsets that decrease)
         }
     } else {
         x.b = static_cast<int>(static_cast<uint32_t>(t) / static_cast<uint32_t>(p.sq));
-        place = row = t - static_cast<int64_t>(x.b) * p.sq;
-        n = p.sq;
-        x.q = p.q + x.b * p.qs[0] + row * p.qs[2];
+        x.place = t - static_cast<int64_t>(x.b) * p.sq;
+        x.of = p.sq;
+        x.q = p.q + x.b * p.qs[0] + x.place * p.qs[2];
     }
-    const int len = min(max(p.lengths[x.b], 0), p.cap);
-    const int64_t seen = len - n + place + 1;
-    x.seen = static_cast<int>(seen < 0 || place < 0 ? 0 : (seen < len ? seen : len));
     return x;
+}
+// The keys that it sees.
+__device__ __forceinline__ int seen_by(const SelectParams& p, const Token& x) {
+    if (x.b < 0) return 0;
+    const int len = min(max(p.lengths[x.b], 0), p.cap);
+    const int64_t seen = len - x.of + x.place + 1;
+    return static_cast<int>(seen < 0 ? 0 : (seen < len ? seen : len));
 }
 
 constexpr int kWarps = 4;        // of a CTA
@@ -237,22 +236,25 @@ template <int D>
 struct Ring {
     static constexpr int kRow = 4 * D + 16;
     static constexpr int kBlock = 16 * kRow;
-    static constexpr int kStages = D == 128 ? 3 : 4;
+    static constexpr int kStages = 3;
     static constexpr int kBytes = kWarps * kStages * kBlock;
 };
 
 struct SelectShared {
-    uint32_t most[kMaxRanks * kWarps];   // magnitudes among the bounds, by warp
-    int4 counts[2][kWarps];
-    int ends[2][2][kWarps];
-    int sums[kWarps];
-    int count, all_in, need;
+    int of_warp[3][kMaxRanks * kWarps];   // by warp: the largest magnitude among the bounds, the least and the largest score (ordered)
+    int counts[2][kWarps][32];
+    int sums[2][kWarps];
+    int found, count, need;
+    float value;
     unsigned long long exact;
 };
 // Of the selection, where the ring was.
+constexpr int kRanked = 32 * kWarps;     // scores that are ranked one against the others
 struct SelectLater {
+    float ranked[kRanked];
     double few[kFew];
     int few_at[kFew];
+    int few_in[kFew];
     int bins[256];
 };
 
@@ -267,8 +269,8 @@ __device__ __forceinline__ unsigned long long ordered(double x) {
     return i >> 63 ? ~i : i | 1ull << 63;
 }
 
-// Exclusive sum of x over the CTA. Two barriers.
-__device__ __forceinline__ int sum_before(int x, int* warps) {
+// Exclusive sum of x over the CTA, and that of all; warps: not in use by another sum before the next barrier.
+__device__ __forceinline__ int sum_before(int x, int* warps, int& all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int sum = x;
 #pragma unroll
@@ -278,8 +280,14 @@ __device__ __forceinline__ int sum_before(int x, int* warps) {
     }
     if (lane == 31) warps[warp] = sum;
     __syncthreads();
-    const int before = __reduce_add_sync(0xffffffffu, lane < warp ? warps[lane] : 0);
-    __syncthreads();
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        const int y = warps[w];
+        before += w < warp ? y : 0;
+        all += y;
+    }
     return before + sum - x;
 }
 
@@ -287,33 +295,58 @@ __device__ __forceinline__ int sum_before(int x, int* warps) {
 __device__ __forceinline__ void to_first(uint32_t at, float x) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
 __device__ __forceinline__ void to_first(uint32_t at, int x) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); }
 
-// The exact score of a page: 64-bit sums of products that are exact themselves. By one warp.
+// The exact score of a page: 64-bit sums of products that are exact themselves. By one warp, a lane D / 32 neighbouring channels; eight heads at a
+// time, whose sums over the lanes halve the heads of a lane before its lanes.
 template <int D>
-__device__ __noinline__ double exact_score(const SelectParams& p, const Token& tok, int hk, int e) {
+__device__ __forceinline__ double exact_score(const SelectParams& p, const Token& tok, int hk, int64_t page) {
     const int lane = threadIdx.x & 31;
     constexpr int kMine = D / 32;
-    const int64_t page = p.table[tok.b * p.table_stride + e];
     if (page < 0 || page >= p.pages) return 0.0;
-    double lo[kMine], hi[kMine];
+    auto load = [&](double (&to)[kMine], const __nv_bfloat16* from) {
+        __nv_bfloat162 x[kMine / 2];
+        if constexpr (kMine == 4) *reinterpret_cast<uint2*>(x) = *reinterpret_cast<const uint2*>(from);
+        else x[0] = *reinterpret_cast<const __nv_bfloat162*>(from);
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) {
-        lo[i] = __bfloat162float(p.bounds.edge(page, hk, 0)[lane + 32 * i]);
-        hi[i] = __bfloat162float(p.bounds.edge(page, hk, 1)[lane + 32 * i]);
-    }
-    double best = -INFINITY;
-#pragma unroll 4
-    for (int h = 0; h < p.group; ++h) {
-        const __nv_bfloat16* q = tok.q + static_cast<int64_t>(hk * p.group + h) * p.qs[1];
-        double sum = 0.0;
+        for (int i = 0; i < kMine / 2; ++i) {
+            const float2 f = __bfloat1622float2(x[i]);
+            to[2 * i] = f.x;
+            to[2 * i + 1] = f.y;
+        }
+    };
+    double lo[kMine], hi[kMine], best = -INFINITY;
+    load(lo, p.bounds.edge(page, hk, 0) + lane * kMine);
+    load(hi, p.bounds.edge(page, hk, 1) + lane * kMine);
+    for (int h0 = 0; h0 < p.group; h0 += 8) {
+        double sum[8];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-            const double x = __bfloat162float(q[lane + 32 * i]), a = x * lo[i], b = x * hi[i];
-            sum += a != a || a > b ? a : b;   // (a NaN of either stays)
+        for (int h = 0; h < 8; ++h) {   // (heads past the last: it again)
+            double q[kMine];
+            load(q, tok.q + static_cast<int64_t>(hk * p.group + min(h0 + h, p.group - 1)) * p.qs[1] + lane * kMine);
+            sum[h] = 0.0;
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+                const double a = q[i] * lo[i], b = q[i] * hi[i];
+                sum[h] += a != a || a > b ? a : b;   // (a NaN of either stays)
+            }
         }
 #pragma unroll
-        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        if (sum != sum) sum = INFINITY;
-        best = sum > best ? sum : best;
+        for (int n = 4; n > 0; n /= 2) {
+            const bool upper = lane & (4 * n);
+#pragma unroll
+            for (int h = 0; h < n; ++h) {
+                const double keep = upper ? sum[h + n] : sum[h], give = upper ? sum[h] : sum[h + n];
+                sum[h] = keep + __shfl_xor_sync(0xffffffffu, give, 4 * n);
+            }
+        }
+        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 2);
+        sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], 1);
+        double x = sum[0] != sum[0] ? INFINITY : sum[0];
+#pragma unroll
+        for (int off = 16; off >= 4; off /= 2) {
+            const double y = __shfl_xor_sync(0xffffffffu, x, off);
+            x = y > x ? y : x;
+        }
+        best = x > best ? x : best;
     }
     return best + 0.0;   // (no -0)
 }
@@ -324,14 +357,15 @@ __device__ __noinline__ double exact_score(const SelectParams& p, const Token& t
 // rows of m16n8k16, q+ and q- of 8 heads its columns. (Bounds in registers as they come, two blocks to a warp, were no faster than one after the
 // other: 16 us for 38 MB.) The products of a block are four sums, for the latency of one.
 //
-// Selection: the value of the k-th largest score by quarters of an interval, with counts of what lies above; a thread has kItems
-// neighbouring pages in registers (0: reads them each time). kNear: scores and names lie in shared memory, else scores where the workspace is.
-// Measured, us: 8 pairs of 1,024 pages, D 128, and 128 of 128 to 1,024: 10.3 and 23.8 in two launches, scores through memory and bins of
-// equal width for the k-th.
+// Selection: the value of the k-th largest score. 32 thresholds cut the range evenly, one to a lane, and a warp's lanes count over its share of
+// the scores what lies above theirs; the interval that has the k-th is cut again while it holds many, and those of the last are ranked one
+// against the others. (A round is some 600 clocks of 1,024 scores. Four to a round, each by a sum over the CTA, were 950 a round and five rounds;
+// bins of equal width, by atomics, 3,000 in all.) Then a thread has kItems neighbouring pages in registers (0: reads them each time), and a sum
+// over the CTA places those that are in. kNear: scores and names lie in shared memory, else scores where the workspace is.
 template <int D, int kItems, bool kNear>
 __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_constant__ SelectParams p) {
     using R = Ring<D>;
-    constexpr int K = D / 16, NS = R::kStages;
+    constexpr int K = D / 16, NS = R::kStages;   // (two blocks on their way)
     extern __shared__ __align__(128) unsigned char dynamic[];
     __shared__ SelectShared sm;
     SelectLater& later = *reinterpret_cast<SelectLater*>(dynamic);
@@ -340,76 +374,77 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     int* name_s = reinterpret_cast<int*>(score_s + p.blocks * 16);
     constexpr int threads = 32 * kWarps, warps = kWarps;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
-    if (tid == 0) sm.count = sm.all_in = 0;
+    if (tid == 0) sm.found = sm.count = 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t pair = blockIdx.x / static_cast<uint32_t>(p.ranks), local = pair / static_cast<uint32_t>(p.kv_heads);
     const int rank = static_cast<int>(blockIdx.x - pair * p.ranks), hk = static_cast<int>(pair - local * p.kv_heads);
     const int64_t t = p.token0 + local;
     const Token tok = token_of(p, t);
-    const int count = static_cast<int>((static_cast<uint32_t>(tok.seen) + p.page_size - 1) / static_cast<uint32_t>(p.page_size)), top = p.top;
-    int32_t* to = p.chosen + (t * p.kv_heads + hk) * top;
     const int32_t* row = p.table + max(tok.b, 0) * p.table_stride;
+    // Requested before the length is known: the queries of the first 8 heads, and (for the cache) the table's row.
+    uint32_t up[K][2], down[K][2];
+    const __nv_bfloat16* queries_at = tok.q + static_cast<int64_t>(hk * p.group + min(g, p.group - 1)) * p.qs[1] + 2 * t4;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) up[k][i] = *reinterpret_cast<const uint32_t*>(queries_at + 16 * k + 8 * i);
+    }
+    if (warp == 0 && lane * 32 < p.blocks * 16) asm volatile("prefetch.global.L1 [%0];" ::"l"(row + min(lane * 32, p.width - 1)));
+    // Blocks are dealt to all warps of the cluster in turn; the first ones' bounds are requested too (names past the length: of pages of others, or none).
+    const int step = p.ranks * warps, own_block = rank * warps + warp;
+    const uint32_t ring = smem_u32(dynamic + warp * NS * R::kBlock), first_scores = in_rank(smem_u32(score_s), 0), first_names = in_rank(smem_u32(name_s), 0);
+    auto names_of = [&](int i, int limit) {   // of this warp's blocks i and i + 1, a lane each
+        const int e = (own_block + (i + (lane >> 4)) * step) * 16 + (lane & 15);
+        return e < limit ? row[e] : -1;
+    };
+    auto issue = [&](int i, int names) {   // a block's bounds, a page's with one instruction (D 64: two pages' with one)
+        const uint32_t to = ring + (i % NS) * R::kBlock;
+        constexpr int kLanes = D / 4, kPages = 32 / kLanes;   // lanes to a page
+        const int at = lane % kLanes * 8, edge = at / D;
+        const __nv_bfloat16* from = p.bounds.at + hk * p.bounds.stride[1] + edge * p.bounds.stride[2] + (at - edge * D);
+#pragma unroll
+        for (int j = 0; j < 16; j += kPages) {
+            const int r = j + lane / kLanes, name = __shfl_sync(0xffffffffu, names, (i & 1) * 16 + r);
+            const bool there = name >= 0 && name < p.pages;
+            cp_async_16(to + r * R::kRow + at * 2, from + (there ? name : 0) * p.bounds.stride[0], there);
+        }
+    };
+    int names = names_of(0, p.width), next = names_of(2, p.width);
+    const int seen = seen_by(p, tok);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (own_block + i * step < p.blocks) issue(i, names);
+        cp_async_commit();
+    }
+    const int count = static_cast<int>((static_cast<uint32_t>(seen) + p.page_size - 1) / static_cast<uint32_t>(p.page_size)), top = p.top;
+    int32_t* to = p.chosen + (t * p.kv_heads + hk) * top;
     if (rank == 0 && tid == 0) {
         const int many = min(count, top);
-        p.keys[t * p.kv_heads + hk] = many > 0 ? (many - 1) * p.page_size + (tok.seen - 1) % p.page_size + 1 : 0;
+        p.keys[t * p.kv_heads + hk] = many > 0 ? (many - 1) * p.page_size + (seen - 1) % p.page_size + 1 : 0;
     }
     if (count <= top) {   // all of them
+        cp_async_wait<0>();
         for (int i = rank * threads + tid; i < top; i += threads * p.ranks) to[i] = i < count ? row[i] : -1;
         return;
     }
     float* given = kNear ? score_s : p.scores + static_cast<int64_t>(pair) * p.blocks * 16;
+    const int begin = p.first, end = count - p.last, k = top - p.first - p.last;   // the k largest of [begin, end), which are more
 
     // ---- scores
     float norm = 0.f;        // the largest sum of magnitudes of a head's query
     {
-        const int all = (count + 15) / 16, each = (all + p.ranks * warps - 1) / (p.ranks * warps);
-        const int block0 = (rank * warps + warp) * each, blocks = min(each, all - block0);
-        const uint32_t ring = smem_u32(dynamic + warp * NS * R::kBlock), first_scores = in_rank(smem_u32(score_s), 0), first_names = in_rank(smem_u32(name_s), 0);
-        // Names of two blocks, a lane each.
-        auto names_of = [&](int block) {
-            const int i = (block0 + block) * 16 + lane;
-            return block < blocks && lane < (blocks - block) * 16 && i < count ? row[i] : -1;
-        };
-        int names = names_of(0), next = names_of(2);
-        int issued = 0;
-        auto issue = [&]() {   // a block's bounds, a page's with one instruction (D 64: two pages' with one)
-            if (issued < blocks) {
-                const int half = issued & 1;
-                const uint32_t to = ring + (issued % NS) * R::kBlock;
-                constexpr int kLanes = D / 4, kPages = 32 / kLanes;   // lanes to a page
-                const int at = lane % kLanes * 8, edge = at / D;
-                const __nv_bfloat16* from = p.bounds.at + hk * p.bounds.stride[1] + edge * p.bounds.stride[2] + (at - edge * D);
-#pragma unroll
-                for (int i = 0; i < 16; i += kPages) {
-                    const int r = i + lane / kLanes, name = __shfl_sync(0xffffffffu, names, half * 16 + r);
-                    const bool there = name >= 0 && name < p.pages;
-                    cp_async_16(to + r * R::kRow + at * 2, from + (there ? name : 0) * p.bounds.stride[0], there);
-                }
-                if constexpr (kNear) {
-                    if ((lane >> 4) == half) to_first(first_names + ((block0 + issued) * 16 + (lane & 15)) * 4, names);
-                }
-                ++issued;
-                if (half) {
-                    names = next;
-                    next = names_of(issued + 2);
-                }
-            }
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < NS - 1; ++i) issue();
-        uint32_t up[K][2], down[K][2];
-        auto queries = [&](int h0) {   // of heads h0 .. h0 + 7
+        const int all = (count + 15) / 16, blocks = all > own_block ? (all - own_block + step - 1) / step : 0;
+        // up: heads h0 .. h0 + 7 as they are; then q+ and q-, and the sums of their magnitudes.
+        auto split = [&](int h0) {
             const bool there = h0 + g < p.group;
-            const __nv_bfloat16* from = tok.q + static_cast<int64_t>(hk * p.group + (there ? h0 + g : 0)) * p.qs[1] + 2 * t4;
             const __nv_bfloat162 zero = __float2bfloat162_rn(0.f);
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(from + 16 * k + 8 * i), u = __hmax2_nan(y, zero), v = __hmin2_nan(y, zero);
+                    const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(&up[k][i]), u = __hmax2_nan(y, zero), v = __hmin2_nan(y, zero);
                     up[k][i] = there ? *reinterpret_cast<const uint32_t*>(&u) : 0u;
                     down[k][i] = there ? *reinterpret_cast<const uint32_t*>(&v) : 0u;
                     const float2 f = __bfloat1622float2(y);
@@ -421,17 +456,47 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
             // (as an integer, which a NaN is the largest of)
             norm = __uint_as_float(__reduce_max_sync(0xffffffffu, max(__float_as_uint(sum), __float_as_uint(norm))));
         };
-        for (int h0 = (p.group - 1) / 8 * 8; h0 >= 0; h0 -= 8) queries(h0);   // (of all for the norm, which all warps need)
+        auto queries = [&](int h0) {
+            const __nv_bfloat16* from = tok.q + static_cast<int64_t>(hk * p.group + min(h0 + g, p.group - 1)) * p.qs[1] + 2 * t4;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) up[k][i] = *reinterpret_cast<const uint32_t*>(from + 16 * k + 8 * i);
+            }
+            split(h0);
+        };
+        split(0);
+        for (int h0 = 8; h0 < p.group; h0 += 8) queries(h0);   // (of all for the norm, which all warps need)
         __nv_bfloat162 largest[2], least[2];
         largest[0] = largest[1] = least[0] = least[1] = __float2bfloat162_rn(0.f);
+        float lo = INFINITY, hi = -INFINITY;
         for (int block = 0; block < blocks; ++block) {
-            issue();
-            cp_async_wait<NS - 1>();
+            // Two ahead. Names of a pair of blocks are those of the next two once their own are on their way.
+            if (block & 1) {
+                if (block + 2 < blocks) issue(block + 2, names);
+            } else {
+                if constexpr (kNear) {
+                    const int of = block + (lane >> 4);
+                    if (of < blocks) to_first(first_names + ((own_block + of * step) * 16 + (lane & 15)) * 4, names);
+                }
+                names = next;
+                if (block + 2 < blocks) issue(block + 2, names);
+                next = names_of(block + 4, count);
+            }
+            cp_async_commit();
+            cp_async_wait<2>();
             __syncwarp();
+            const int behind = (own_block + block * step + 1) * 16 - count;
+            if (behind > 0) {   // rows past the last page count for nothing
+                for (int i = lane; i < behind * (4 * D / 16); i += 32) {
+                    *reinterpret_cast<uint4*>(dynamic + (warp * NS + block % NS) * R::kBlock + (15 - i / (4 * D / 16)) * R::kRow + i % (4 * D / 16) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                __syncwarp();
+            }
             const uint32_t from = ring + (block % NS) * R::kBlock + ((lane & 7) + ((lane >> 3) & 1) * 8) * R::kRow + (lane >> 4) * 16;
             float s[2] = {-INFINITY, -INFINITY};
             for (int h0 = 0; h0 < p.group; h0 += 8) {
-                if (p.group > 8) queries(h0);
+                if (p.group > 8) queries(h0);   // (more than 8 heads: each tile's again)
                 float acc[4][4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -463,8 +528,21 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
                 s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 1));
                 s[i] = fmaxf(s[i], __shfl_xor_sync(0xffffffffu, s[i], 2));
             }
+            // What is not asked about is below everything.
+            const int e = (own_block + block * step) * 16 + g;
+            if (e >= begin && e < end) {
+                lo = fminf(lo, s[0]);
+                hi = fmaxf(hi, s[0]);
+            } else {
+                s[0] = -INFINITY;
+            }
+            if (e + 8 >= begin && e + 8 < end) {
+                lo = fminf(lo, s[1]);
+                hi = fmaxf(hi, s[1]);
+            } else {
+                s[1] = -INFINITY;
+            }
             if (t4 == 0) {
-                const int e = (block0 + block) * 16 + g;
                 if constexpr (kNear) {
                     to_first(first_scores + e * 4, s[0]);
                     to_first(first_scores + (e + 8) * 4, s[1]);
@@ -478,24 +556,39 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         const __nv_bfloat162 high = __hmax2_nan(__hmax2_nan(largest[0], largest[1]), __hneg2(__hmin2_nan(least[0], least[1])));
         const uint32_t bits = *reinterpret_cast<const uint32_t*>(&high) & 0x7fff7fffu;
         const uint32_t most = __reduce_max_sync(0xffffffffu, max(bits & 0xffffu, bits >> 16)) << 16;   // (bf16 magnitudes as integers, a NaN above all)
-        if (lane == 0) to_first(in_rank(smem_u32(&sm.most[rank * warps + warp]), 0), static_cast<int>(most));
+        const int least_score = __reduce_min_sync(0xffffffffu, ordered(lo)), largest_score = __reduce_max_sync(0xffffffffu, ordered(hi));
+        if (lane < 3) {
+            const uint32_t slot = in_rank(smem_u32(&sm.of_warp[lane][own_block]), 0);
+            to_first(slot, lane == 0 ? static_cast<int>(most) : lane == 1 ? least_score : largest_score);
+        }
     }
     if (p.ranks > 1) cluster_meet(); else __syncthreads();
     if (rank > 0) return;   // (nobody looks at its shared memory)
 
     // ---- the selection, by the first CTA
-    const int begin = p.first, end = count - p.last, k = top - p.first - p.last;   // the k largest of [begin, end), which are more
+    const int share = ((count + 15) / 16 + kWarps - 1) / kWarps * 16;
+    auto each_of = [&](auto f) {   // this warp's share of the scores, for all lanes, 16 at a time
+        const int last = min((warp + 1) * share, (count + 15) / 16 * 16);
+#pragma unroll 2
+        for (int e = warp * share; e < last; e += 16) {
+            float4 x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = reinterpret_cast<const float4*>(given + e)[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f(i, x[i]);
+        }
+    };
     const int mine = kItems ? kItems : ((count + threads - 1) / threads + 3) & ~3, first = tid * mine;
     float held[kItems ? kItems : 1];
     if constexpr (kItems > 0) {
 #pragma unroll
         for (int i = 0; i < kItems; i += 4) {
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
             if (first + i < count) x = *reinterpret_cast<const float4*>(given + first + i);   // (whole blocks of 16 are written)
             held[i] = x.x; held[i + 1] = x.y; held[i + 2] = x.z; held[i + 3] = x.w;
         }
     }
-    auto each = [&](auto f) {   // its pages and their scores
+    auto each = [&](auto f) {   // this thread's pages and their scores
         if constexpr (kItems > 0) {
 #pragma unroll
             for (int i = 0; i < kItems; ++i) {
@@ -506,172 +599,174 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         }
     };
     auto name_of = [&](int e) { return kNear ? name_s[e] : row[e]; };
-    // The least and the largest of the CTA.
-    auto ends_of = [&](float& lo, float& hi, int which) {
-        const int a = __reduce_min_sync(0xffffffffu, ordered(lo)), b = __reduce_max_sync(0xffffffffu, ordered(hi));
-        if (lane == 0) {
-            sm.ends[which][0][warp] = a;
-            sm.ends[which][1][warp] = b;
-        }
-        __syncthreads();
-        lo = from_ordered(__reduce_min_sync(0xffffffffu, sm.ends[which][0][lane % warps]));
-        hi = from_ordered(__reduce_max_sync(0xffffffffu, sm.ends[which][1][lane % warps]));
-    };
-    float lo = INFINITY, hi = -INFINITY;
-    each([&](int, float x) {
-        lo = fminf(lo, x);
-        hi = fmaxf(hi, x);
-    });
-    ends_of(lo, hi, 0);
-    const uint32_t largest = __reduce_max_sync(0xffffffffu, lane < p.ranks * warps ? sm.most[lane] : 0u);
-    const float most = __uint_as_float(largest), mass = norm * most;
+    const bool slot = lane < step;
+    const float most = __int_as_float(__reduce_max_sync(0xffffffffu, slot ? sm.of_warp[0][lane] : 0)), mass = norm * most;
+    float lo = from_ordered(__reduce_min_sync(0xffffffffu, slot ? sm.of_warp[1][lane] : 0x7fffffff)), hi = from_ordered(__reduce_max_sync(0xffffffffu, slot ? sm.of_warp[2][lane] : static_cast<int>(0x80000000)));
     // What the fp32 scores may be off by. (What the products could lose below fp32's least normal number is in the last terms.)
-    const float off = fmaf(mass, 0x1p-17f, fmaf(norm + most, 0x1p-110f, 0x1p-110f));
+    const float off = fmaf(mass, 0x1p-19f, fmaf(norm + most, 0x1p-110f, 0x1p-110f));
     const bool sure = mass < 0x1p120f;   // else, and where it is no number: all in 64 bits
     if (sure && k > 0) {
-        // The k-th largest is in (a, b], and `between` scores are.
+        // The k-th largest is in (a, b].
         float a = lo - off, b = hi;
         int above_a = end - begin, above_b = 0;
-        for (int round = 0; round < 24 && above_a - above_b > 1 && b - a > off; ++round) {
-            const float w = b - a, c[3] = {fmaf(w, 0.25f, a), fmaf(w, 0.5f, a), fmaf(w, 0.75f, a)};
-            int n[3] = {0, 0, 0};
-            each([&](int, float x) {
-#pragma unroll
-                for (int i = 0; i < 3; ++i) n[i] += x > c[i];
-            });
-#pragma unroll
-            for (int i = 0; i < 3; ++i) n[i] = __reduce_add_sync(0xffffffffu, n[i]);
-            if (lane == 0) sm.counts[round & 1][warp] = make_int4(n[0], n[1], n[2], 0);
+        for (int round = 0; round < 8 && above_a - above_b > kRanked && b - a > off; ++round) {
+            const float c = fmaf(b - a, (lane + 1) * 0x1p-5f, a);   // (the last: b)
+            int some[4] = {0, 0, 0, 0};
+            each_of([&](int i, const float4& x) { some[i] += (x.x > c) + (x.y > c) + (x.z > c) + (x.w > c); });
+            sm.counts[round & 1][warp][lane] = (some[0] + some[1]) + (some[2] + some[3]);
             __syncthreads();
-            const int4 other = lane < warps ? sm.counts[round & 1][lane] : make_int4(0, 0, 0, 0);
-            n[0] = __reduce_add_sync(0xffffffffu, other.x);
-            n[1] = __reduce_add_sync(0xffffffffu, other.y);
-            n[2] = __reduce_add_sync(0xffffffffu, other.z);
+            int n = 0;
 #pragma unroll
-            for (int i = 0; i < 3; ++i) {   // (n falls)
-                if (n[i] >= k) {
-                    a = c[i];
-                    above_a = n[i];
-                }
+            for (int w = 0; w < kWarps; ++w) n += sm.counts[round & 1][w][lane];
+            // n falls from lane to lane: the first threshold with fewer than k above it, and the one before.
+            const uint32_t fewer = __ballot_sync(0xffffffffu, n < k || lane == 31);
+            const int at = __ffs(fewer) - 1;
+            const float upper = __shfl_sync(0xffffffffu, c, at), lower = __shfl_sync(0xffffffffu, c, max(at - 1, 0));
+            const int n_upper = __shfl_sync(0xffffffffu, n, at), n_lower = __shfl_sync(0xffffffffu, n, max(at - 1, 0));
+            if (at < 31) {   // (b stays else, and what lies above it)
+                b = upper;
+                above_b = n_upper;
             }
-#pragma unroll
-            for (int i = 2; i >= 0; --i) {
-                if (n[i] < k) {
-                    b = c[i];
-                    above_b = n[i];
-                }
+            if (at > 0) {
+                a = lower;
+                above_a = n_lower;
             }
         }
-        lo = INFINITY;
-        hi = -INFINITY;
-        each([&](int, float x) {
-            if (x > a && x <= b) {
-                lo = fminf(lo, x);
-                hi = fmaxf(hi, x);
+        if (above_a - above_b <= kRanked) {
+            const int many = above_a - above_b, need = k - above_b;
+            if (tid >= many) later.ranked[tid] = -INFINITY;
+            each([&](int, float x) {
+                if (x > a && x <= b) later.ranked[atomicAdd(&sm.found, 1)] = x;
+            });
+            __syncthreads();
+            // Equal ones in any order.
+            const float x = tid < many ? later.ranked[tid] : 0.f;
+            int better = 0;
+#pragma unroll 4
+            for (int i = 0; i < many; i += 4) {
+                const float4 y = *reinterpret_cast<const float4*>(later.ranked + i);
+                better += (y.x > x || (y.x == x && i < tid)) + (y.y > x || (y.y == x && i + 1 < tid)) + (y.z > x || (y.z == x && i + 2 < tid)) + (y.w > x || (y.w == x && i + 3 < tid));
             }
-        });
-        ends_of(lo, hi, 1);
+            if (tid < many && better == need - 1) sm.value = x;
+            __syncthreads();
+            lo = hi = sm.value;
+        } else {
+            lo = a;
+            hi = b;
+        }
     }
-    // Pages above are in, pages below are out; those between are counted, and listed while they are few.
+    // Pages above are in, pages below are out, those between are counted.
     const float above = sure ? hi + 2.f * off : INFINITY, below = sure ? lo - 2.f * off : -INFINITY;
-    auto surely = [&](float x) { return sure && x > above; };
-    auto doubtful = [&](float x) { return !surely(x) && !(x < below); };
+    auto surely = [&](float x) { return x > above; };
+    auto doubtful = [&](float x) { return !(x > above) && !(x < below); };
     int in = 0, some = 0;
     if (k > 0) {
-        each([&](int e, float x) {
+        each([&](int, float x) {
             in += surely(x);
-            if (doubtful(x)) {
-                ++some;
-                const int at = atomicAdd(&sm.count, 1);
-                if (at < kFew) later.few_at[at] = e;
-            }
+            some += doubtful(x);
         });
     }
-    const int warp_in = __reduce_add_sync(0xffffffffu, in);
-    if (lane == 0 && warp_in > 0) atomicAdd(&sm.all_in, warp_in);
-    __syncthreads();
-    const int all_some = sm.count, rest = k - sm.all_in;   // so many of the doubtful ones are in
-    const bool everything = all_some == rest;
-    int some_before = 0;
+    int at, all_in, all_some;
+    if (kItems > 0) {   // (fewer than 2^16 of either)
+        at = sum_before(in | some << 16, sm.sums[0], all_in);
+        all_some = all_in >> 16;
+        all_in &= 0xffff;
+        at = (at & 0xffff) + (at >> 16);
+    } else {
+        at = sum_before(in, sm.sums[0], all_in);
+        at += sum_before(some, sm.sums[1], all_some);
+    }
+    const int rest = k - all_in;   // so many of the doubtful ones are in
+    for (int i = tid; i < p.first; i += threads) to[i] = name_of(i);
+    for (int i = tid; i < p.last; i += threads) to[top - p.last + i] = name_of(end + i);
+    to += p.first;
+    if (k == 0) return;
+    if (all_some == rest) {
+        if (in + some > 0) {
+            each([&](int e, float x) {
+                if (!(x < below)) to[at++] = name_of(e);
+            });
+        }
+        return;
+    }
+    // Some of those between are in, by their exact scores.
     double* exact = p.exact + static_cast<int64_t>(pair) * p.blocks * 16;
     unsigned long long value = 0;
-    int ties = 0;
-    if (k > 0 && !everything) {
-        if (all_some <= kFew) {
-            for (int i = warp; i < all_some; i += warps) {
-                const double x = exact_score<D>(p, tok, hk, later.few_at[i]);
-                if (lane == 0) later.few[i] = x;
-            }
-            __syncthreads();
-            // In the order of score and place, the first `rest` are in.
-            for (int i = tid; i < all_some; i += threads) {
-                const double x = later.few[i];
-                const int e = later.few_at[i];
-                int better = 0;
-                for (int j = 0; j < all_some; ++j) better += later.few[j] > x || (later.few[j] == x && later.few_at[j] < e);
-                exact[e] = better < rest ? 1.0 : 0.0;
-            }
-            __syncthreads();
-        } else {
-            // Many that differ by less than the error (alike, most of them): the rest-th largest of their exact scores, eight bits at a time, then
-            // those above it and, of its own value, the first.
-            for (int e = begin + warp; e < end; e += warps) {
-                if (!doubtful(given[e])) continue;
-                const double x = exact_score<D>(p, tok, hk, e);
-                if (lane == 0) exact[e] = x;
-            }
-            __syncthreads();
-            ties = rest;
-            for (int shift = 56; shift >= 0; shift -= 8) {
-                for (int i = tid; i < 256; i += threads) later.bins[i] = 0;
-                __syncthreads();
-                each([&](int e, float x) {
-                    if (!doubtful(x)) return;
-                    const unsigned long long y = ordered(exact[e]);
-                    if (shift == 56 || y >> (shift + 8) == value >> (shift + 8)) atomicAdd(&later.bins[y >> shift & 255], 1);
-                });
-                __syncthreads();
-                if (tid == 0) {
-                    int bin = 255, left = ties;
-                    while (later.bins[bin] < left) left -= later.bins[bin--];
-                    sm.need = left;
-                    sm.exact = value | static_cast<unsigned long long>(bin) << shift;
-                }
-                __syncthreads();
-                ties = sm.need;
-                value = sm.exact;
-                __syncthreads();
-            }
-            // Of this thread's pages: those of the value itself, of which the first `ties` of all are in.
-            int equal = 0;
-            each([&](int e, float x) { equal += doubtful(x) && ordered(exact[e]) == value; });
-            some_before = sum_before(equal, sm.sums);
+    int ties = 0, ties_before = 0;
+    if (all_some <= kFew) {
+        each([&](int e, float x) {
+            if (doubtful(x)) later.few_at[atomicAdd(&sm.count, 1)] = e;
+        });
+        __syncthreads();
+        for (int i = warp; i < all_some; i += warps) {
+            const double x = exact_score<D>(p, tok, hk, name_of(later.few_at[i]));
+            if (lane == 0) later.few[i] = x;
         }
+        __syncthreads();
+        // In the order of score and place, the first `rest` are in.
+        for (int i = tid; i < all_some; i += threads) {
+            const double x = later.few[i];
+            const int e = later.few_at[i];
+            int better = 0;
+            for (int j = 0; j < all_some; ++j) better += later.few[j] > x || (later.few[j] == x && later.few_at[j] < e);
+            later.few_in[i] = better < rest;
+        }
+        __syncthreads();
+    } else {
+        // Many that differ by less than the error (alike, most of them): the rest-th largest of their exact scores, eight bits at a time, then
+        // those above it and, of its own value, the first.
+        for (int e = begin + warp; e < end; e += warps) {
+            if (!doubtful(given[e])) continue;
+            const double x = exact_score<D>(p, tok, hk, name_of(e));
+            if (lane == 0) exact[e] = x;
+        }
+        __syncthreads();
+        ties = rest;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            for (int i = tid; i < 256; i += threads) later.bins[i] = 0;
+            __syncthreads();
+            each([&](int e, float x) {
+                if (!doubtful(x)) return;
+                const unsigned long long y = ordered(exact[e]);
+                if (shift == 56 || y >> (shift + 8) == value >> (shift + 8)) atomicAdd(&later.bins[y >> shift & 255], 1);
+            });
+            __syncthreads();
+            if (tid == 0) {
+                int bin = 255, left = ties;
+                while (later.bins[bin] < left) left -= later.bins[bin--];
+                sm.need = left;
+                sm.exact = value | static_cast<unsigned long long>(bin) << shift;
+            }
+            __syncthreads();
+            ties = sm.need;
+            value = sm.exact;
+            __syncthreads();
+        }
+        // Of this thread's pages: those of the value itself, of which the first `ties` of all are in.
+        int equal = 0, all;
+        each([&](int e, float x) { equal += doubtful(x) && ordered(exact[e]) == value; });
+        ties_before = sum_before(equal, sm.sums[0], all);
     }
     // Whether a doubtful page is in; asked in the order of a thread's pages.
-    int equal = some_before;
+    int equal = ties_before;
     auto among = [&](int e) {
-        if (everything) return true;
-        if (all_some <= kFew) return exact[e] != 0.0;
+        if (all_some <= kFew) {
+            int i = 0;
+            while (later.few_at[i] != e) ++i;
+            return later.few_in[i] != 0;
+        }
         const unsigned long long y = ordered(exact[e]);
         return y > value || (y == value && equal++ < ties);
     };
-    // The pages that are in, in their order: the first, those of [begin, end), the last.
-    int own = in;
-    if (some > 0) {
-        each([&](int e, float x) {
-            if (doubtful(x)) own += among(e);
-        });
-    }
-    int at = p.first + sum_before(own, sm.sums);
-    equal = some_before;
-    if (own > 0) {
-        each([&](int e, float x) {
-            if (surely(x) || (doubtful(x) && among(e))) to[at++] = name_of(e);
-        });
-    }
-    for (int i = tid; i < p.first; i += threads) to[i] = name_of(i);
-    for (int i = tid; i < p.last; i += threads) to[top - p.last + i] = name_of(end + i);
+    int own = in, all;
+    each([&](int e, float x) {
+        if (doubtful(x)) own += among(e);
+    });
+    at = sum_before(own, sm.sums[1], all);
+    equal = ties_before;
+    each([&](int e, float x) {
+        if (surely(x) || (doubtful(x) && among(e))) to[at++] = name_of(e);
+    });
 }
 
 // ---- host --------------------------------------------------------------------------------------
@@ -835,6 +930,7 @@ extern "C" int ktt_b200_paged_select(const ktt_b200_select_args* a, void* stream
     p.first = a->first;
     p.last = a->last;
     p.blocks = s.blocks;
+    p.width = a->table_width;
     unsigned char* base = static_cast<unsigned char*>(a->workspace);
     p.scores = s.near ? nullptr : reinterpret_cast<float*>(base);
     p.exact = reinterpret_cast<double*>(base + s.exact_at);
