@@ -181,13 +181,14 @@ struct RotaryParams {
     int d;
     Placed positions;        // none: the row
     int vec;                 // rows may be read and written in 16-byte pieces
+    int loops;               // groups of kHeads that a thread goes through
 };
 struct RotaryAxesParams : RotaryParams {
     PairAxes axes;
 };
 
-// A thread turns eight columns of kHeads heads of one token: the table is read once for all of them. A thread reads
-// its partner columns too (its neighbour in the block brings the same line, so they come from L1).
+// A thread turns eight columns of kHeads heads of one token, and of the next kHeads, `loops` times: the table is read once for all of them. A thread
+// reads its partner columns too (its neighbour in the block brings the same line, so they come from L1).
 template <typename T, bool kFast, int kHeads, typename Params>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Params p) {
     const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
@@ -196,31 +197,90 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Par
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (n >= p.tokens) return;
     const int which = static_cast<int>(blockIdx.y) >= p.groups[0];
-    const int h0 = (static_cast<int>(blockIdx.y) - (which ? p.groups[0] : 0)) * kHeads;
+    const int loops = kHeads == 1 ? 1 : p.loops;
+    int h0 = (static_cast<int>(blockIdx.y) - (which ? p.groups[0] : 0)) * (kHeads * loops);
     const uint32_t entry = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows);   // (2^31 tokens at most)
     const int64_t b = entry, r = static_cast<uint32_t>(n) - entry * static_cast<uint32_t>(p.rows);
+    const T* x = static_cast<const T*>(p.x[which]) + b * p.xs[which][0] + r * p.xs[which][2];
+    T* y = static_cast<T*>(p.y[which]) + b * p.ys[which][0] + r * p.ys[which][2];
+    const int left = p.d - col, heads = p.heads[which], half = p.turn.half;
+    const int partner = p.turn.interleaved || col >= 2 * half ? -1 : col < half ? col + half : col - half;
+    Eight<T> v[kHeads], o[kHeads];
+    auto rows_of = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const T* row = x + static_cast<int64_t>(min(h0 + i, heads - 1)) * p.xs[which][1];
+            if (kFast || p.vec) v[i].load(row + col);
+            else v[i].load_some(row + col, left);
+            if (kFast && partner >= 0) o[i].load(row + partner);
+        }
+    };
+    if (kHeads == 1) rows_of(h0);   // (requested before the positions, which the table's rows wait for)
     Turned<kFast> turned;
     if constexpr (std::is_same_v<Params, RotaryAxesParams>) turned.load(p.turn, p.axes, p.positions.all(p.axes.axes, b, r), col);
     else turned.load(p.turn, p.positions.at ? p.positions.get(0, b, r) : r, col);
+    for (int loop = 0; loop < loops && h0 < heads; ++loop, h0 += kHeads) {
+        if (kHeads > 1) rows_of(h0);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const int h = h0 + i;
+            if (h >= heads) break;
+            turned.apply(p.turn, v[i], o[i], x + h * p.xs[which][1], col);
+            T* to = y + h * p.ys[which][1] + col;
+            if (kFast || p.vec) v[i].store(to);
+            else v[i].store_some(to, left);
+        }
+    }
+}
+
+// Half layout: a thread has eight pairs, both columns of each, so that no column is read twice and the table's entries are those of 16 columns; behind
+// the pairs it copies 16 columns.
+template <typename T, typename Params>
+__global__ void __launch_bounds__(256) rotary_pairs_kernel(const __grid_constant__ Params p) {
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+    const int half = p.turn.half, pair = threadIdx.x * 8;
+    const bool turns = pair < half;
+    const int col = turns ? pair : 2 * pair, other = turns ? pair + half : 2 * pair + 8;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (n >= p.tokens) return;
+    const int which = static_cast<int>(blockIdx.y) >= p.groups[0];
+    const uint32_t entry = static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows);   // (2^31 tokens at most)
+    const int64_t b = entry, r = static_cast<uint32_t>(n) - entry * static_cast<uint32_t>(p.rows);
+    Turned<true> turned;   // (of the first columns; the others' sines have the other sign)
+    if (turns) {
+        if constexpr (std::is_same_v<Params, RotaryAxesParams>) turned.load(p.turn, p.axes, p.positions.all(p.axes.axes, b, r), col);
+        else turned.load(p.turn, p.positions.at ? p.positions.get(0, b, r) : r, col);
+    }
     const T* x = static_cast<const T*>(p.x[which]) + b * p.xs[which][0] + r * p.xs[which][2];
     T* y = static_cast<T*>(p.y[which]) + b * p.ys[which][0] + r * p.ys[which][2];
-    const int left = p.d - col;
-    Eight<T> v[kHeads], o[kHeads];
+    constexpr int kHeads = 4;
+    const int heads = p.heads[which];
+    int h0 = (static_cast<int>(blockIdx.y) - (which ? p.groups[0] : 0)) * (kHeads * p.loops);
+    for (int loop = 0; loop < p.loops && h0 < heads; ++loop, h0 += kHeads) {
+        Eight<T> lo[kHeads], hi[kHeads];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const T* row = x + static_cast<int64_t>(min(h0 + i, p.heads[which] - 1)) * p.xs[which][1];
-        if (kFast || p.vec) v[i].load(row + col);
-        else v[i].load_some(row + col, left);
-        if (kFast && turned.partner >= 0) o[i].load(row + turned.partner);
-    }
+        for (int j = 0; j < kHeads; ++j) {
+            const T* row = x + static_cast<int64_t>(min(h0 + j, heads - 1)) * p.xs[which][1];
+            lo[j].load(row + col);
+            hi[j].load(row + other);
+        }
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const int h = h0 + i;
-        if (h >= p.heads[which]) break;
-        turned.apply(p.turn, v[i], o[i], x + h * p.xs[which][1], col);
-        T* to = y + h * p.ys[which][1] + col;
-        if (kFast || p.vec) v[i].store(to);
-        else v[i].store_some(to, left);
+        for (int j = 0; j < kHeads; ++j) {
+            if (h0 + j >= heads) break;
+            if (turns) {
+                const Eight<T> first = lo[j];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float u = to_f32(first.get(e)), v = to_f32(hi[j].get(e)), c = turned.c[e], s = turned.s[e];
+                    lo[j].set(e, from_f32<T>(__fadd_rn(__fmul_rn(u, c), __fmul_rn(v, s))));
+                    hi[j].set(e, from_f32<T>(__fadd_rn(__fmul_rn(v, c), __fmul_rn(u, -s))));
+                }
+            }
+            T* to = y + (h0 + j) * p.ys[which][1];
+            lo[j].store(to + col);
+            hi[j].store(to + other);
+        }
     }
 }
 
@@ -229,15 +289,14 @@ constexpr int64_t kManyThreads = 4 * 148 * 2048;
 template <typename T, typename Params>
 int launch_rotary(const Params& given, cudaStream_t stream) {
     Params p = given;
-    const int chunks = (p.d + 7) / 8;
-    const int tokens_per_block = 256 / chunks > 0 ? 256 / chunks : 1;
-    const int64_t blocks = (p.tokens + tokens_per_block - 1) / tokens_per_block;
     const bool fast = p.vec && turn_is_fast(p.turn);
-    auto go = [&](auto kernel, int per) {
+    constexpr bool kAxes = std::is_same_v<Params, RotaryAxesParams>;
+    auto go = [&](auto kernel, int columns, int per) {   // of a thread
+        const int x = (p.d + columns - 1) / columns, y = 256 / x > 0 ? 256 / x : 1;
         for (int i = 0; i < 2; ++i) p.groups[i] = (p.heads[i] + per - 1) / per;
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(p.groups[0] + p.groups[1]));
-        cfg.blockDim = dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(tokens_per_block));
+        cfg.gridDim = dim3(static_cast<unsigned>((p.tokens + y - 1) / y), static_cast<unsigned>(p.groups[0] + p.groups[1]));
+        cfg.blockDim = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
         cfg.stream = stream;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -246,17 +305,32 @@ int launch_rotary(const Params& given, cudaStream_t stream) {
         cfg.numAttrs = 1;
         return check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "rotary launch");
     };
-    // Four heads to a thread once that fills the GPU: a row's position and table entries are read once for all of them.
-    // 4 x 4,096 tokens, 32 heads over 8, D 128, bf16, forward and gradient, us for 1 and 4 heads: 671 and 400. (Of the latter's
-    // bytes 92 to 95 % of a copy's rate: forward alone, 16 x 4,096 tokens, 16 + 16 heads, 175.7 us, 6.1 TB/s.)
-    // Where the pairs of the half layout are no multiple of 8 a thread goes for its columns' partners one by one, and reads the tables so:
-    // 4 x 16 heads x 4,096, D 128, bf16, all columns turning 25.1, 20 or 40 of them 38.6; neighbours 24.3, and 26.3 with 20 columns.
-    if (p.tokens * chunks * (p.heads[0] + p.heads[1]) >= kManyThreads) {
-        if (fast) return go(rotary_kernel<T, true, 4, Params>, 4);
-        return go(rotary_kernel<T, false, 4, Params>, 4);
+    // Half layout: 16 columns and four heads to a thread as soon as that makes some 2^15 threads (one axis: 2^16), more heads one after another as
+    // there are more. us for the pairs' kernel and the other, bf16, three axes taking turns: 512 rows, 32 heads over 8, D 128: 5.1 and 8.6; 2,048:
+    // 8.2 and 11.0; 2,048 of 14 over 2, D 64: 5.3 and 6.4, with one axis 4.2 and 3.8; 77 of them 3.5 and 2.9. One, two and four
+    // times four heads, three axes (one): 2,048 rows, 32 over 8, D 128: 8.2, 7.5, 11.5 (6.5, 6.4, 10.6); 8,192: 31.6, 30.3, 30.5 (28.0, 28.2, 29.0);
+    // 65,536 of 16 + 16: 207, 170, 165 (182, 161, 163; a copy of the same bytes 165; the other kernel 264 and 215).
+    p.loops = 1;
+    if (fast && !p.turn.interleaved && p.d % 16 == 0) {
+        const int64_t threads = p.tokens * (p.d / 16) * ((p.heads[0] + 3) / 4 + (p.heads[1] + 3) / 4);
+        if (threads >= (kAxes ? 1 << 15 : 1 << 16)) {
+            p.loops = threads < 1 << 19 ? 1 : (kAxes && threads >= 1 << 21 ? 4 : 2);
+            return go(rotary_pairs_kernel<T, Params>, 16, 4 * p.loops);
+        }
     }
-    if (fast) return go(rotary_kernel<T, true, 1, Params>, 1);
-    return go(rotary_kernel<T, false, 1, Params>, 1);
+    // Else four heads to a thread once that fills the GPU: a row's position and table entries are read once for all of them; and for the next four,
+    // and as many again. 65,536 rows, 16 + 16 heads, D 128, neighbours, three axes (one), us for 4, 8 and 16 heads: 249, 191, 168 (211, 175, 162); 2,048 of
+    // 32 over 8: 9.6, 8.1, 9.7 (7.1, 6.7, 8.8).
+    // Where the pairs of the half layout are no multiple of 8 a thread goes for its columns' partners one by one, and reads the tables so:
+    // 65,536 rows, 16 + 16 heads, D 128, 20 columns: 569, 406, 325 (443, 345, 296).
+    const int64_t threads = p.tokens * ((p.d + 7) / 8) * (p.heads[0] + p.heads[1]);
+    if (threads >= kManyThreads) {
+        p.loops = threads < 1 << 21 ? 2 : 4;
+        if (fast) return go(rotary_kernel<T, true, 4, Params>, 8, 4 * p.loops);
+        return go(rotary_kernel<T, false, 4, Params>, 8, 4 * p.loops);
+    }
+    if (fast) return go(rotary_kernel<T, true, 1, Params>, 8, 1);
+    return go(rotary_kernel<T, false, 1, Params>, 8, 1);
 }
 
 }  // namespace

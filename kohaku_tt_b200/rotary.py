@@ -218,19 +218,32 @@ class _Rotary(torch.autograd.Function):
 
 @torch.library.custom_op("ktt_b200::_rotary", mutates_args=(), device_types="cuda")
 def _rotary_op(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None,
-               interleaved: bool, inverse: bool, axes: Sequence[int] | None = None) -> list[torch.Tensor]:
+               interleaved: bool, inverse: bool) -> list[torch.Tensor]:
     """The rotation as an operator, for compiled graphs."""
-    q_out, k_out = _run(q, k, cos, sin, positions, interleaved, inverse, None if axes is None else tuple(axes))
+    q_out, k_out = _run(q, k, cos, sin, positions, interleaved, inverse)
+    return [q_out] if k_out is None else [q_out, k_out]
+
+
+@torch.library.custom_op("ktt_b200::_rotary_axes", mutates_args=(), device_types="cuda")
+def _axes_op(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+             interleaved: bool, inverse: bool, axes: Sequence[int]) -> list[torch.Tensor]:
+    """That by positions of several axes. (One operator with axes of None by default would lose them on their way to its gradient.)"""
+    q_out, k_out = _run(q, k, cos, sin, positions, interleaved, inverse, tuple(axes))
     return [q_out] if k_out is None else [q_out, k_out]
 
 
 @_rotary_op.register_fake
-def _(q, k, cos, sin, positions, interleaved, inverse, axes=None):
+def _(q, k, cos, sin, positions, interleaved, inverse):
+    return [ops._empty_like_rows(x) for x in (q, k) if x is not None]
+
+
+@_axes_op.register_fake
+def _(q, k, cos, sin, positions, interleaved, inverse, axes):
     return [ops._empty_like_rows(x) for x in (q, k) if x is not None]
 
 
 def _setup(ctx, inputs, output):
-    _, k, cos, sin, positions, interleaved, inverse, axes = inputs
+    _, k, cos, sin, positions, interleaved, inverse, *axes = inputs
     ctx.save_for_backward(cos, sin, positions)
     ctx.how = (interleaved, inverse, axes, [x.shape for x in output])
 
@@ -238,15 +251,18 @@ def _setup(ctx, inputs, output):
 def _op_backward(ctx, grads):
     cos, sin, positions = ctx.saved_tensors
     interleaved, inverse, axes, shapes = ctx.how
+    rest = (None,) * (5 + len(axes))
     some = next((g for g in grads if g is not None), None)
     if some is None:
-        return (None,) * 8
+        return (None, None, *rest)
     grads = [some.new_zeros(shape) if g is None else g for g, shape in zip(grads, shapes)]
-    got = torch.ops.ktt_b200._rotary(grads[0], grads[1] if len(grads) > 1 else None, cos, sin, positions, interleaved, not inverse, axes)
-    return got[0], got[1] if len(got) > 1 else None, None, None, None, None, None, None
+    turn = torch.ops.ktt_b200._rotary_axes if axes else torch.ops.ktt_b200._rotary
+    got = turn(grads[0], grads[1] if len(grads) > 1 else None, cos, sin, positions, interleaved, not inverse, *axes)
+    return (got[0], got[1] if len(got) > 1 else None, *rest)
 
 
 _rotary_op.register_autograd(_op_backward, setup_context=_setup)
+_axes_op.register_autograd(_op_backward, setup_context=_setup)
 
 
 def rotary(q, k, cos, sin, positions=None, interleaved=False, axes=None):
@@ -273,6 +289,9 @@ def rotary(q, k, cos, sin, positions=None, interleaved=False, axes=None):
     axes = pair_axes(axes, cos.shape[-1], "rotary")
     _check(q, k, cos, sin, positions, axes)
     if torch.compiler.is_compiling():
-        out = torch.ops.ktt_b200._rotary(q, k, cos, sin, positions, interleaved, False, None if axes is None else list(axes))
+        if axes is None:
+            out = torch.ops.ktt_b200._rotary(q, k, cos, sin, positions, interleaved, False)
+        else:
+            out = torch.ops.ktt_b200._rotary_axes(q, k, cos, sin, positions, interleaved, False, list(axes))
         return (out[0], None if k is None else out[1])
     return _Rotary.apply(q, k, cos, sin, positions, interleaved, False, axes)

@@ -80,6 +80,24 @@ def test_many_rows(cuda, interleaved):
     assert torch.equal(torch.cat([yq, yk], 1).cpu(), po.turn_fp32(both, c, s, interleaved))
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("t,h,hk,d,r,dtype", [(5200, 13, 3, 128, 128, torch.bfloat16), (70000, 9, 5, 64, 64, torch.float16), (80000, 18, 3, 128, 96, torch.bfloat16),
+                                              (40000, 5, 1, 80, 80, torch.float32), (30000, 33, 1, 72, 64, torch.bfloat16), (20000, 10, 10, 64, 20, torch.bfloat16)])
+def test_threads_with_many_heads_are_threads_with_one(cuda, interleaved, t, h, hk, d, r, dtype):
+    """Rows in one call, whose threads go through several groups of heads, against the same rows a few at a time; one axis and three."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    q, k = torch.randn((t, h, d), generator=g, device=cuda).to(dtype), torch.randn((t, hk, d), generator=g, device=cuda).to(dtype)
+    cos, sin = ktt.rotary_table(500, r, device=cuda)
+    pos, some = torch.randint(0, 500, (3, t), generator=g, device=cuda), torch.tensor([0, 1, t // 2, t - 2, t - 1], device=cuda)
+    for at, axes in ((pos[0], None), (pos, _axes("turns", r // 2, 3))):
+        got = ktt.rotary(q, k, cos, sin, positions=at, interleaved=interleaved, axes=axes)
+        want = ktt.rotary(q[some], k[some], cos, sin, positions=at[..., some], interleaved=interleaved, axes=axes)
+        assert torch.equal(got[0][some], want[0]) and torch.equal(got[1][some], want[1])
+        c, s = (cos[at], sin[at]) if axes is None else so.axis_rows(cos, sin, at, axes)
+        whole = [po.turn_fp32(x, c[:, None], s[:, None], interleaved) for x in (q, k)]
+        assert torch.equal(got[0], whole[0]) and torch.equal(got[1], whole[1])
+
+
 def test_alike_positions_are_those_of_one_axis(cuda, path):
     """Text: all axes count on together. [axes, S] and [axes, 1, S] serve all batch entries."""
     q, k = _x(3, 8, 40, 64, seed=1).to(cuda), _x(3, 2, 40, 64, seed=2).to(cuda)
@@ -141,6 +159,27 @@ def test_append(cuda, path, bits, d, pairs, interleaved, packed):
             out = out.transpose(1, 2).reshape(b * n, h, d)
         assert torch.equal(out, want_q)
         assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(plain, got))
+
+
+def test_compiled(cuda):
+    """One graph, queries and keys, both gradients and one alone."""
+    cos, sin = ktt.rotary_table(16, 64, device=cuda)
+    q, k = _x(2, 4, 16, 64).to(cuda), _x(2, 2, 16, 64, seed=1).to(cuda)
+    at, axes = torch.randint(0, 16, (3, 2, 16), generator=torch.Generator().manual_seed(2)).to(cuda), _axes("turns", 32, 3)
+
+    def turned(a, b):
+        return ktt.rotary(a, b, cos, sin, positions=at, axes=axes)
+
+    ql, kl = q.clone().requires_grad_(), k.clone().requires_grad_()
+    want = turned(ql, kl)
+    got = torch.compile(turned, fullgraph=True)(ql, kl)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    a, b = torch.autograd.grad(want, (ql, kl), (q, k), retain_graph=True), torch.autograd.grad(got, (ql, kl), (q, k))
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    (a,), (b,) = torch.autograd.grad(want[1], kl, k), torch.autograd.grad(torch.compile(lambda x: turned(q, x)[1], fullgraph=True)(kl), kl, k)
+    assert torch.equal(a, b)
+    out = torch.ops.ktt_b200._rotary_axes(ql, kl, cos, sin, at, False, False, list(axes))
+    assert torch.equal(torch.autograd.grad(out[1], kl, k)[0], a)
 
 
 def test_refusals(cuda, path):
