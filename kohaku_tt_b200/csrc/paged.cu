@@ -39,7 +39,8 @@ struct AppendParams {
     Pages c;
     Turn turn;
     int batch, rows, heads, kv_heads;
-    int groups;            // blocks of kHeads queries' heads; those of the keys and of the values follow in the grid's y
+    int groups;            // blocks of `loops` times kHeads queries' heads; those of the keys and of the values follow in the grid's y
+    int loops;
     int64_t tokens;        // rows of all sequences
     const __nv_bfloat16* q;
     __nv_bfloat16* q_out;
@@ -102,8 +103,8 @@ __device__ __forceinline__ uint2 put_four_bits(const Eight<__nv_bfloat16>& x, un
     return held;
 }
 
-// A thread has eight columns of kHeads heads of one token: of queries, keys or values. Its rows are requested before it
-// knows where they go (a packed row's sequence takes a search). No thread leaves before the groups' shuffles.
+// A thread has eight columns of kHeads heads of one token, and of the next kHeads, `loops` times: of queries, keys or values. Its first rows are
+// requested before it knows where they go (a packed row's sequence takes a search). No thread leaves before the groups' shuffles.
 template <int D, int kBits, bool kFast, int kHeads, typename Params>
 __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const __grid_constant__ Params p) {
     constexpr bool kAt = std::is_same_v<Params, AppendAtParams>;
@@ -118,9 +119,11 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
         }
     }
     // What the block has: queries, keys or values.
-    const int y = blockIdx.y, kv = (p.kv_heads + kHeads - 1) / kHeads;
+    const int loops = kHeads == 1 ? 1 : p.loops, per = kHeads * loops;
+    const int y = blockIdx.y, kv = (p.kv_heads + per - 1) / per;
     const int what = y < p.groups ? 0 : y < p.groups + kv ? 1 : 2;
-    const int h0 = (y - (what == 0 ? 0 : what == 1 ? p.groups : p.groups + kv)) * kHeads, heads = what == 0 ? p.heads : p.kv_heads;
+    int h0 = (y - (what == 0 ? 0 : what == 1 ? p.groups : p.groups + kv)) * per;
+    const int heads = what == 0 ? p.heads : p.kv_heads;
     const __nv_bfloat16* from = what == 0 ? p.q : what == 1 ? p.k : p.v;
     const int64_t sb = what == 0 ? p.qs[0] : what == 1 ? p.ks[0] : p.vs[0], sh = what == 0 ? p.qs[1] : what == 1 ? p.ks[1] : p.vs[1];
     const int64_t sr = what == 0 ? p.qs[2] : what == 1 ? p.ks[2] : p.vs[2];
@@ -130,17 +133,20 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
     from += (p.cu ? 0 : b * sb) + r * sr;
     Eight<__nv_bfloat16> x[kHeads], other[kHeads];
     const int partner = what == 2 || !p.turn.cos || p.turn.interleaved || col >= 2 * p.turn.half ? -1 : col < p.turn.half ? col + p.turn.half : col - p.turn.half;
+    auto rows_of = [&](int h0) {
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        if (!in_range || h0 + i >= heads) {
+        for (int i = 0; i < kHeads; ++i) {
+            if (!in_range || h0 + i >= heads) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i].set(e, __float2bfloat16_rn(0.f));
-            continue;
+                for (int e = 0; e < 8; ++e) x[i].set(e, __float2bfloat16_rn(0.f));
+                continue;
+            }
+            const __nv_bfloat16* row = from + (h0 + i) * sh;
+            if (kFast || p.vec) x[i].load(row + col); else x[i].load_some(row + col, 8);
+            if (kFast && partner >= 0) other[i].load(row + partner);
         }
-        const __nv_bfloat16* row = from + (h0 + i) * sh;
-        if (kFast || p.vec) x[i].load(row + col); else x[i].load_some(row + col, 8);
-        if (kFast && partner >= 0) other[i].load(row + partner);
-    }
+    };
+    rows_of(h0);
     int64_t in = r;          // the row's place among the sequence's new ones
     bool row_there = in_range;
     int cached = 0;
@@ -186,11 +192,14 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
     if (what == 0) {
         if (!row_there) return;
         __nv_bfloat16* to = p.q_out + (p.cu ? 0 : b * p.qos[0]) + r * p.qos[2] + col;
+        for (int loop = 0; loop < loops && h0 < heads; ++loop, h0 += kHeads) {
+            if (loop) rows_of(h0);
 #pragma unroll
-        for (int i = 0; i < kHeads; ++i) {
-            if (h0 + i >= heads) break;
-            turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
-            if (kFast || p.vec) x[i].store(to + (h0 + i) * p.qos[1]); else x[i].store_some(to + (h0 + i) * p.qos[1], 8);
+            for (int i = 0; i < kHeads; ++i) {
+                if (h0 + i >= heads) break;
+                turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
+                if (kFast || p.vec) x[i].store(to + (h0 + i) * p.qos[1]); else x[i].store_some(to + (h0 + i) * p.qos[1], 8);
+            }
         }
         return;
     }
@@ -200,33 +209,36 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
     const int at = there ? static_cast<int>(pos) % p.c.page_size : 0;
     unsigned char* base = !there ? nullptr : what == 2 ? p.c.v + page * p.c.vs[0] : p.c.k + page * p.c.ks[0];
     const int64_t head_stride = what == 2 ? p.c.vs[1] : p.c.ks[1];
+    for (int loop = 0; loop < loops && h0 < heads; ++loop, h0 += kHeads) {
+        if (loop) rows_of(h0);
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        if (h0 + i >= heads) break;
-        if (there && what == 1) turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
-        unsigned char* to = there ? base + (h0 + i) * head_stride : nullptr;
-        if constexpr (kBits == 16) {
-            if (there) x[i].store(reinterpret_cast<__nv_bfloat16*>(to + at * (what == 2 ? p.c.vs[2] : p.c.ks[2])) + col);
-        } else {
-            if (there) to += static_cast<int64_t>(at >> 4) * (9 * D);
-            const uint2 held = put_four_bits<D>(x[i], to, what == 2, at & 15, chunk, there);
-            if constexpr (kAt) {
-                if (p.bounds.at && what == 1) x[i] = of_four_bits(held.x, held.y);
-            }
-        }
-        if constexpr (kAt) {
-            // The sequence's only new key: no other thread has these channels of its page's bounds.
-            if (p.bounds.at && what == 1 && there) {
-                Edges e = {x[i], x[i]};
-                __nv_bfloat16 *lo = p.bounds.edge(page, h0 + i, 0) + col, *hi = p.bounds.edge(page, h0 + i, 1) + col;
-                if (at > 0) {
-                    Edges old;
-                    old.lo.load(lo);
-                    old.hi.load(hi);
-                    e.with(old.lo, old.hi);
+        for (int i = 0; i < kHeads; ++i) {
+            if (h0 + i >= heads) break;
+            if (there && what == 1) turned.apply(p.turn, x[i], other[i], from + (h0 + i) * sh, col);
+            unsigned char* to = there ? base + (h0 + i) * head_stride : nullptr;
+            if constexpr (kBits == 16) {
+                if (there) x[i].store(reinterpret_cast<__nv_bfloat16*>(to + at * (what == 2 ? p.c.vs[2] : p.c.ks[2])) + col);
+            } else {
+                if (there) to += static_cast<int64_t>(at >> 4) * (9 * D);
+                const uint2 held = put_four_bits<D>(x[i], to, what == 2, at & 15, chunk, there);
+                if constexpr (kAt) {
+                    if (p.bounds.at && what == 1) x[i] = of_four_bits(held.x, held.y);
                 }
-                e.lo.store(lo);
-                e.hi.store(hi);
+            }
+            if constexpr (kAt) {
+                // The sequence's only new key: no other thread has these channels of its page's bounds.
+                if (p.bounds.at && what == 1 && there) {
+                    Edges e = {x[i], x[i]};
+                    __nv_bfloat16 *lo = p.bounds.edge(page, h0 + i, 0) + col, *hi = p.bounds.edge(page, h0 + i, 1) + col;
+                    if (at > 0) {
+                        Edges old;
+                        old.lo.load(lo);
+                        old.hi.load(hi);
+                        e.with(old.lo, old.hi);
+                    }
+                    e.lo.store(lo);
+                    e.hi.store(hi);
+                }
             }
         }
     }
@@ -433,15 +445,20 @@ int launch_append(const Params& given, cudaStream_t stream) {
     const dim3 block(D / 8, 256 / (D / 8));
     const int64_t blocks = (p.tokens + block.y - 1) / block.y;   // one at least: it writes the new lengths
     auto go = [&](auto kernel, int per) {
+        per *= p.loops;
         p.groups = (p.heads + per - 1) / per;
         const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), static_cast<unsigned>(p.groups + 2 * ((p.kv_heads + per - 1) / per)));
         return launch_dependent(kernel, p, grid, block, stream, "paged_append launch");
     };
     const bool fast = p.vec && turn_is_fast(p.turn);
-    // Four heads to a thread once that fills the GPU: a token's place, page and table rows are looked up once for all of
-    // them. 10,240 packed tokens, 32 heads over 8, D 128, us for 1, 2, 4 and 8 heads: bf16 pages 94.8, 69.7, 51.3, 48.4
-    // (4.9 TB/s at 4); 4 bits 102.6, 77.3, 60.1, 58.6, of which keys and values 28 (queries alone run at a copy's rate).
-    if (p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads) >= 4 * 148 * 2048) {
+    // Four heads to a thread once that makes threads enough, and four more after them: a token's place, page and table rows are looked up once for
+    // all of them. 32 heads over 8, D 128, us for 1 and 4 heads: 256 tokens, 4 bits 4.6 and 5.4; 512, bf16 6.0 and 3.9; 1,024, 4 bits 11.5 and 8.2. For
+    // 4, 8, 16 and 32 heads: 2,048 tokens, bf16 12.2, 10.8, 10.1, 16.0; 10,240 packed ones, bf16 52.3, 46.2, 44.5, 43.7 (5.4 TB/s), 4 bits 61.2, 54.1, 52.6,
+    // 51.0, and by positions of three axes 88, 70, 65, 61.
+    p.loops = 1;
+    const int64_t threads = p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads);
+    if (threads >= 3 << 17) {
+        p.loops = threads < 1 << 20 ? 1 : (threads < 1 << 22 ? 4 : 8);
         if (fast) return go(append_kernel<D, kBits, true, 4, Params>, 4);
         return go(append_kernel<D, kBits, false, 4, Params>, 4);
     }

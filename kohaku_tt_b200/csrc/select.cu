@@ -10,6 +10,8 @@
 // up at most (two bits more than a sum of fp32 rounds by), all in all by e = 2^-19 max_h sum_d |q_hd| max |bound|. So the value of the
 // last page selected lies within e of the last by fp32: pages more than 2 e above or below are in or out, and those between, one or a few, get their
 // scores in 64 bits where they are not all in. (2 to 5 in 100 selections among 1,024 pages.)
+#include <type_traits>
+
 #include "four_bits.cuh"
 #include "split.cuh"
 
@@ -39,16 +41,16 @@ struct BoundsParams {
 
 constexpr int kLotOfTokens = 16;   // packed rows that a warp looks for pages in
 
-// A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, eight rows requested before the first is used.
+// A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, 16 or 8 rows requested before the first is used.
 // Packed rows: a warp looks at 16 of them and has the pages that begin among them, or in which a sequence's rows begin.
 template <int D, int kBits, bool kPacked>
 __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ BoundsParams p) {
-    constexpr int kChunks = D / 8, kStep = 32 / kChunks, kAhead = 8;
+    constexpr int kChunks = D / 8, kStep = 32 / kChunks;
     const int lane = threadIdx.x & 31, chunk = lane % kChunks, page_size = p.c.page_size;
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t lot = unit / p.kv_heads;
+    const int64_t lot = unit >> 32 ? unit / p.kv_heads : static_cast<uint32_t>(unit) / static_cast<uint32_t>(p.kv_heads);
     const int head = static_cast<int>(unit - lot * p.kv_heads);
 
     // Rows begin .. end - 1 of a page, into what the page has if begin > 0.
@@ -68,7 +70,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
             old.lo.load(p.bounds.edge(page, head, 0) + chunk * 8);
             old.hi.load(p.bounds.edge(page, head, 1) + chunk * 8);
         }
-        for (int r0 = begin + lane / kChunks; r0 < end; r0 += kAhead * kStep) {
+        auto rows = [&](auto ahead, int r0) {
+            constexpr int kAhead = decltype(ahead)::value;
             if constexpr (kBits == 16) {
                 Eight<__nv_bfloat16> x[kAhead];
 #pragma unroll
@@ -92,7 +95,11 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
                     e.with(y, y);
                 }
             }
-        }
+        };
+        // (Whole lots while there are any, then as many as are left.)
+        int r0 = begin + lane / kChunks;
+        for (; r0 + 15 * kStep < end; r0 += 16 * kStep) rows(std::integral_constant<int, 16>(), r0);
+        for (; r0 < end; r0 += 8 * kStep) rows(std::integral_constant<int, 8>(), r0);
 #pragma unroll
         for (int off = kChunks; off < 32; off <<= 1) {
             Edges other;
@@ -114,14 +121,33 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
         const int64_t n = lot * kLotOfTokens + lane;
         int b = -1, place = 0, end = 0;
         bool leads = false;
-        if (lane < kLotOfTokens && n < p.rows) {
-            b = sequence_of(p.cu, p.batch, n);
-            if (b >= 0 && n >= p.cu[b]) {   // (offsets that decrease)
-                const int64_t in = n - p.cu[b], at = cached_keys(p.c, b) + in, all = at + (p.cu[b + 1] - n);
-                end = static_cast<int>(all < p.c.cap ? all : p.c.cap);
-                leads = at < end && (in == 0 || at % page_size == 0);
-                place = leads ? static_cast<int>(at) : 0;
+        const bool mine = lane < kLotOfTokens && n < p.rows;
+        int64_t start = 0, behind = 0;
+        int keys = 0;
+        if (p.batch < 32) {   // a lane looks at a sequence, its length with it, in one trip
+            const int offset = p.cu[min(lane, p.batch)], have = cached_keys(p.c, min(lane, p.batch - 1));
+#pragma unroll
+            for (int i = 0; i < kLotOfTokens; ++i) {   // (the last that starts at or before the token)
+                const uint32_t before = __ballot_sync(0xffffffffu, lane <= p.batch && offset <= lot * kLotOfTokens + i);
+                if (i == lane) b = 31 - __clz(before);
             }
+            if (!mine || b < 0 || b >= p.batch) b = -1;
+            start = __shfl_sync(0xffffffffu, offset, max(b, 0));
+            behind = __shfl_sync(0xffffffffu, offset, max(b, 0) + 1);
+            keys = __shfl_sync(0xffffffffu, have, max(b, 0));
+        } else if (mine) {
+            b = sequence_of(p.cu, p.batch, n);
+            if (b >= 0) {
+                start = p.cu[b];
+                behind = p.cu[b + 1];
+                keys = cached_keys(p.c, b);
+            }
+        }
+        if (b >= 0 && n >= start) {   // (offsets that decrease)
+            const int64_t in = n - start, at = keys + in, all = at + (behind - n);
+            end = static_cast<int>(all < p.c.cap ? all : p.c.cap);
+            leads = at < end && (in == 0 || static_cast<uint32_t>(at) % static_cast<uint32_t>(page_size) == 0);   // (at < end: 2^30 at most)
+            place = leads ? static_cast<int>(at) : 0;
         }
         uint32_t leaders = __ballot_sync(0xffffffffu, leads);
         while (leaders) {
