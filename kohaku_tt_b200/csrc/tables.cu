@@ -32,73 +32,100 @@ struct ReserveParams {
 };
 
 __device__ __forceinline__ int clamped(int x, int64_t most) { return x < 0 ? 0 : (x > most ? static_cast<int>(most) : x); }
-__device__ __forceinline__ int pages_for(int64_t keys, int page_size) { return static_cast<int>((keys + page_size - 1) / page_size); }
-
-// Exclusive sum of x over the CTA's threads.
-template <int N>
-__device__ __forceinline__ int64_t sum_before(int64_t x, int64_t* warps) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t sum = x;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, sum, off);
-        if (lane >= off) sum += y;
-    }
-    if (lane == 31) warps[warp] = sum;
-    __syncthreads();
-    int64_t before = sum - x;
-#pragma unroll
-    for (int w = 0; w < N / 32; ++w) before += w < warp ? warps[w] : 0;
-    __syncthreads();
-    return before;
+__device__ __forceinline__ int pages_for(int64_t keys, int page_size) {   // (2^30 keys at most)
+    return static_cast<int>((static_cast<uint32_t>(keys) + page_size - 1) / static_cast<uint32_t>(page_size));
 }
 
-// The last b with sums[b] <= n, of `batch` sequences; sums do not decrease.
-__device__ __forceinline__ int holder_of(const int* sums, int batch, int n) {
-    int lo = 0, hi = batch - 1;
+// Exclusive sums of x and y over the CTA's threads.
+template <int N, typename X, typename Y>
+__device__ __forceinline__ void sums_before(X& x, Y& y, X* x_warps, Y* y_warps) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    X sx = x;
+    Y sy = y;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const X u = __shfl_up_sync(0xffffffffu, sx, off);
+        const Y v = __shfl_up_sync(0xffffffffu, sy, off);
+        if (lane >= off) {
+            sx += u;
+            sy += v;
+        }
+    }
+    if (lane == 31) {
+        x_warps[warp] = sx;
+        y_warps[warp] = sy;
+    }
+    __syncthreads();
+    x = sx - x;
+    y = sy - y;
+#pragma unroll
+    for (int w = 0; w < N / 32; ++w) {
+        x += w < warp ? x_warps[w] : 0;
+        y += w < warp ? y_warps[w] : 0;
+    }
+}
+
+// The last b with sums[b] <= n, of sequences lo to hi; sums do not decrease.
+__device__ __forceinline__ int holder_of(const int* sums, int lo, int hi, int n) {
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (sums[mid] <= n) lo = mid; else hi = mid - 1;
     }
     return lo;
 }
+// That of n + lane: a warp's lanes look at 32 sums that are evenly spaced, then between two of them, for the first; unless that has all of
+// them, each lane for itself.
+__device__ __forceinline__ int holders_of(const int* sums, int batch, int n) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, many = batch;
+    while (many > 1) {
+        const int step = (many + 31) / 32, i = lane * step;
+        const uint32_t before = __ballot_sync(0xffffffffu, i < many && sums[lo + min(i, many - 1)] <= n);
+        const int at = before ? (31 - __clz(before)) * step : 0;
+        lo += at;
+        many = min(step, many - at);
+    }
+    return n <= sums[lo + 1] - 32 ? lo : holder_of(sums, lo, batch - 1, n + lane);
+}
 
 __global__ void __launch_bounds__(kThreads) reserve_kernel(const __grid_constant__ ReserveParams p) {
     __shared__ int pages_s[kMaxSequences + 1], rows_s[kMaxSequences + 1];
-    __shared__ int64_t warps[kThreads / 32];
+    __shared__ int page_warps[kThreads / 32];
+    __shared__ int64_t row_warps[kThreads / 32];
     __shared__ int short_s;   // the first sequence that gets nothing
+    const int batch = p.batch;
+    if (threadIdx.x == 0) short_s = batch;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int batch = p.batch;
     const int count = clamped(*p.count, p.pool);
-    if (threadIdx.x == 0) short_s = batch;
     // Consecutive sequences to a thread; their pages and rows, then the sums before them.
-    const int per = (batch + kThreads - 1) / kThreads, first = threadIdx.x * per;
-    int64_t pages = 0, rows = 0;
-    int over = batch;
-    for (int i = 0; i < per; ++i) {
-        const int b = first + i;
-        if (b >= batch) break;
-        const int len = clamped(p.lengths[b], p.cap), more = max(p.added[b], 0);
+    const int per = (batch + kThreads - 1) / kThreads, first = threadIdx.x * per, last = min(first + per, batch);
+    auto wanted = [&](int b, int& len, int& more) {   // pages
+        len = clamped(p.lengths[b], p.cap);
+        more = max(p.added[b], 0);
         const int64_t all = static_cast<int64_t>(len) + more;
-        if (all > p.cap && over == batch) over = b;
-        pages += pages_for(all < p.cap ? all : p.cap, p.page_size) - pages_for(len, p.page_size);
+        return pages_for(all < p.cap ? all : p.cap, p.page_size) - pages_for(len, p.page_size);
+    };
+    int pages = 0;   // (under 2^31: a table of fewer entries)
+    int64_t rows = 0;
+    int len = 0, more = 0, one = 0;
+    for (int b = first; b < last; ++b) {
+        one = wanted(b, len, more);
+        pages += one;
         rows += more;
     }
-    int64_t pages_at = sum_before<kThreads>(pages, warps), rows_at = sum_before<kThreads>(rows, warps);
-    for (int i = 0; i < per; ++i) {
-        const int b = first + i;
-        if (b >= batch) break;
-        pages_s[b] = static_cast<int>(pages_at);   // (under 2^31: a table of fewer entries)
-        rows_s[b] = static_cast<int>(rows_at < INT32_MAX ? rows_at : INT32_MAX);
-        const int len = clamped(p.lengths[b], p.cap), more = max(p.added[b], 0);
-        const int64_t all = static_cast<int64_t>(len) + more;
-        pages_at += pages_for(all < p.cap ? all : p.cap, p.page_size) - pages_for(len, p.page_size);
-        rows_at += more;
-        if (pages_at > count && over == batch) over = b;
+    sums_before<kThreads>(pages, rows, page_warps, row_warps);
+    int over = batch;
+    for (int b = first; b < last; ++b) {
+        if (per > 1) one = wanted(b, len, more);
+        pages_s[b] = pages;
+        rows_s[b] = static_cast<int>(rows < INT32_MAX ? rows : INT32_MAX);
+        pages += one;
+        rows += more;
+        if ((pages > count || static_cast<int64_t>(len) + more > p.cap) && over == batch) over = b;
         if (b == batch - 1) {
-            pages_s[batch] = static_cast<int>(pages_at);
-            rows_s[batch] = static_cast<int>(rows_at < INT32_MAX ? rows_at : INT32_MAX);
+            pages_s[batch] = pages;
+            rows_s[batch] = static_cast<int>(rows < INT32_MAX ? rows : INT32_MAX);
         }
     }
     if (over < batch) atomicMin(&short_s, over);
@@ -114,30 +141,36 @@ __global__ void __launch_bounds__(kThreads) reserve_kernel(const __grid_constant
             *p.count_out = count - pages_s[end];
         }
     }
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kThreads;
-    const int taken = pages_s[batch];
-    for (int64_t n = at; n < taken; n += step) {
-        const int i = static_cast<int>(n), b = holder_of(pages_s, batch, i);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads, warp_at = static_cast<int64_t>(blockIdx.x) * kThreads + (threadIdx.x & ~31);
+    const int lane = threadIdx.x & 31, taken = pages_s[batch];
+    for (int64_t n = warp_at; n < taken; n += step) {
+        const int i = static_cast<int>(n) + lane, b = holders_of(pages_s, batch, static_cast<int>(n));
+        if (i >= taken) continue;
         const int entry = pages_for(clamped(p.lengths[b], p.cap), p.page_size) + i - pages_s[b];
         p.table[b * p.table_stride + entry] = b < end ? p.free_pages[count - 1 - i] : -1;
     }
     if (!p.positions && !p.slots) return;
-    for (int64_t n = at; n < p.tokens; n += step) {
+    const int packed = rows_s[batch];
+    for (int64_t n = warp_at; n < p.tokens; n += step) {
+        const int64_t row = n + lane;
         int position = -1;
         int64_t slot = -1;
-        if (n < rows_s[batch]) {
-            const int b = holder_of(rows_s, batch, static_cast<int>(n));
-            const int len = clamped(p.lengths[b], p.cap);
-            const int64_t place = len + n - rows_s[b];
-            position = static_cast<int>(place < INT32_MAX ? place : INT32_MAX);
-            if (b < end) {
-                const int entry = position / p.page_size, held = pages_for(len, p.page_size);
-                const int64_t page = entry < held ? p.table[b * p.table_stride + entry] : p.free_pages[count - 1 - pages_s[b] - (entry - held)];
-                if (page >= 0) slot = page * p.page_size + (position - entry * p.page_size);
+        if (n < packed) {
+            const int b = holders_of(rows_s, batch, static_cast<int>(n));
+            if (row < packed) {
+                const int keys = clamped(p.lengths[b], p.cap);
+                const int64_t to = keys + row - rows_s[b];
+                position = static_cast<int>(to < INT32_MAX ? to : INT32_MAX);
+                if (b < end) {
+                    const int entry = static_cast<int>(static_cast<uint32_t>(position) / static_cast<uint32_t>(p.page_size)), held = pages_for(keys, p.page_size);
+                    const int64_t page = *(entry < held ? p.table + b * p.table_stride + entry : p.free_pages + (count - 1 - pages_s[b] - (entry - held)));
+                    if (page >= 0) slot = page * p.page_size + (position - entry * p.page_size);
+                }
             }
         }
-        if (p.positions) p.positions[n] = position;
-        if (p.slots) p.slots[n] = slot;
+        if (row >= p.tokens) continue;
+        if (p.positions) p.positions[row] = position;
+        if (p.slots) p.slots[row] = slot;
     }
 }
 
@@ -176,7 +209,7 @@ __device__ __forceinline__ void ctas_meet() {
 __global__ void __cluster_dims__(kReleaseCtas, 1, 1) __launch_bounds__(kReleaseThreads) release_kernel(const __grid_constant__ ReleaseParams p) {
     __shared__ int entries_s[kMaxSequences + 1];
     __shared__ int64_t warps[kReleaseThreads / 32];
-    __shared__ int found_s;
+    __shared__ int none_warps[kReleaseThreads / 32], found_s;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int batch = p.batch, count = clamped(*p.count, p.pool);
@@ -192,7 +225,10 @@ __global__ void __cluster_dims__(kReleaseCtas, 1, 1) __launch_bounds__(kReleaseT
         const int begin = first_free(b, end);
         mine += end - begin;
     }
-    int64_t before = sum_before<kReleaseThreads>(mine, warps);
+    int64_t before = mine;
+    int none = 0;
+    sums_before<kReleaseThreads>(before, none, warps, none_warps);
+    __syncthreads();
     for (int b = first; b < min(first + per, batch); ++b) {
         int end;
         const int begin = first_free(b, end);
@@ -206,7 +242,7 @@ __global__ void __cluster_dims__(kReleaseCtas, 1, 1) __launch_bounds__(kReleaseT
     const int n0 = static_cast<int>(from < all ? from : all), n1 = min(n0 + each, all);
     auto visit = [&](auto use) {   // this thread's entries
         if (n0 >= n1) return;
-        int b = holder_of(entries_s, batch, n0), end, entry = first_free(b, end) + n0 - entries_s[b];
+        int b = holder_of(entries_s, 0, batch - 1, n0), end, entry = first_free(b, end) + n0 - entries_s[b];
         for (int n = n0; n < n1; ++n, ++entry) {
             while (entry >= end) entry = first_free(++b, end);
             use(p.table + b * p.table_stride + entry);
@@ -214,7 +250,8 @@ __global__ void __cluster_dims__(kReleaseCtas, 1, 1) __launch_bounds__(kReleaseT
     };
     int found = 0;
     visit([&](const int32_t* e) { found += *e >= 0 && *e < p.pool; });
-    int64_t at = sum_before<kReleaseThreads>(found, warps);
+    int64_t at = found;
+    sums_before<kReleaseThreads>(at, none, warps, none_warps);
     if (threadIdx.x == kReleaseThreads - 1) found_s = static_cast<int>(at) + found;
     ctas_meet();
     int in_all = 0;
@@ -275,10 +312,11 @@ extern "C" int ktt_b200_paged_reserve(const ktt_b200_tables* a, const int32_t* a
     p.positions = positions;
     p.slots = slots;
     p.granted = granted;
-    // Four rows to a thread, two CTAs to an SM at most.
-    const int64_t blocks = (tokens + 4 * kThreads - 1) / (4 * kThreads);
-    const unsigned grid = static_cast<unsigned>(blocks < 1 ? 1 : (blocks > 296 ? 296 : blocks));
-    return launch_dependent(reserve_kernel, p, dim3(grid), dim3(kThreads), static_cast<cudaStream_t>(stream), "paged_reserve launch");
+    // A row to a thread at a time, two CTAs to an SM at most. 164,000 rows of 128 sequences, us with 1, 2, 4 and 6: 6.3, 5.1, 6.0, 5.6; with four rows to a
+    // thread, looked up together, 7.1 with one and 8.2 with two.
+    const int64_t blocks = (tokens + kThreads - 1) / kThreads;
+    const dim3 grid(static_cast<unsigned>(blocks < 1 ? 1 : (blocks > 2 * 148 ? 2 * 148 : blocks)));
+    return launch_dependent(reserve_kernel, p, grid, dim3(kThreads), static_cast<cudaStream_t>(stream), "paged_reserve launch");
 }
 
 extern "C" int ktt_b200_paged_release(const ktt_b200_tables* a, const int32_t* kept, void* stream) {

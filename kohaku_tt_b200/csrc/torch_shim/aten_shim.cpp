@@ -1486,6 +1486,14 @@ bool tables_of(ktt_b200_tables& a, PyObject* const* args, PyObject* count_out) {
     return true;
 }
 
+// A vector in the memory of `whole`, from a byte on.
+Tensor part_of(const Tensor& whole, int64_t byte, int64_t size, at::ScalarType type) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+    return t;
+}
+
 // paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out): (cu_seq, positions, slots, granted), or None.
 PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
@@ -1498,10 +1506,13 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
         pybind11::gil_scoped_release release;
         at::AutoDispatchBelowADInplaceOrView guard;
         c10::cuda::CUDAGuard device(table.device());
-        out[0] = empty_cuda({a.batch + 1}, at::kInt, table);
-        out[1] = empty_cuda({tokens}, at::kInt, table);
-        out[2] = empty_cuda({tokens}, at::kLong, table);
-        out[3] = empty_cuda({a.batch}, at::kInt, table);
+        // In one allocation, slots first.
+        const int64_t slots = (8 * static_cast<int64_t>(tokens) + 15) / 16 * 16, positions = (4 * static_cast<int64_t>(tokens) + 15) / 16 * 16, cu = (4 * (static_cast<int64_t>(a.batch) + 1) + 15) / 16 * 16;
+        const Tensor all = empty_cuda({slots + positions + cu + 4 * static_cast<int64_t>(a.batch)}, at::kByte, table);
+        out[0] = part_of(all, slots + positions, a.batch + 1, at::kInt);
+        out[1] = part_of(all, slots, tokens, at::kInt);
+        out[2] = part_of(all, 0, tokens, at::kLong);
+        out[3] = part_of(all, slots + positions + cu, a.batch, at::kInt);
         raise_status(ktt_b200_paged_reserve(&a, tensor_of(args[2])->data_ptr<int32_t>(), tokens, out[0].data_ptr<int32_t>(), out[1].data_ptr<int32_t>(),
                                             out[2].data_ptr<int64_t>(), out[3].data_ptr<int32_t>(), at::cuda::getCurrentCUDAStream()),
                      "paged_reserve");
