@@ -501,7 +501,7 @@ typedef struct ktt_b200_select_args {
     int64_t bounds_strides[3];
     int32_t* chosen;
     int32_t* keys;
-    void* workspace;               /* ktt_b200_paged_select_workspace() bytes, 16-byte aligned, of any content */
+    void* workspace;               /* ktt_b200_paged_select_workspace() bytes (0 but for long tables), 16-byte aligned, of any content */
     int64_t workspace_bytes;
 } ktt_b200_select_args;
 KTT_B200_API int64_t ktt_b200_paged_select_workspace(const ktt_b200_select_args* args);

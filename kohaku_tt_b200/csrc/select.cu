@@ -187,7 +187,22 @@ int launch_bounds(const BoundsParams& p, int bits, int d, cudaStream_t stream) {
 
 // ---- scores ------------------------------------------------------------------------------------
 
+// Division of numbers under 2^31 by one that the host knows, d: with 2^s the power of two at or above it, n / d is n ceil(2^(31 + s) / d) / 2^(31 + s),
+// whole part, as the product is off by less than n / 2^(31 + s) < 1 / d. (A division of 32 bits takes some 20 dependent instructions, and a
+// selection has five.)
+struct Divisor {
+    uint32_t by, times;
+    int shift;
+    explicit Divisor(int64_t d = 1) : by(static_cast<uint32_t>(d)), shift(31) {
+        while ((1ll << (shift - 31)) < d) ++shift;
+        times = static_cast<uint32_t>(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { return static_cast<uint32_t>(static_cast<uint64_t>(n) * times >> shift); }
+    __device__ __forceinline__ uint32_t rest(uint32_t n) const { return n - (*this)(n) * by; }
+};
+
 struct SelectParams {
+    Divisor by_page, by_sq, by_heads, by_ranks;   // page_size, sq, kv_heads, ranks
     const __nv_bfloat16* q;
     int64_t qs[3];
     const int32_t* cu;
@@ -204,7 +219,7 @@ struct SelectParams {
     int width, blocks;        // pages that the table has, and blocks of 16
     int ranks;                // CTAs of a pair
     float* scores;            // [pairs][blocks][16]; null: in shared memory
-    double* exact;            // [pairs][blocks][16], of the pages that need them
+    double* exact;            // [pairs][blocks][16], of the pages that need them; null: in shared memory, where the rings were
     int32_t* chosen;
     int32_t* keys;
 };
@@ -238,7 +253,7 @@ __device__ __forceinline__ Token token_of(const SelectParams& p, int64_t t) {
             if (x.place < x.of) x.b = from;   // (offsets that decrease)
         }
     } else {
-        x.b = static_cast<int>(static_cast<uint32_t>(t) / static_cast<uint32_t>(p.sq));
+        x.b = static_cast<int>(p.by_sq(static_cast<uint32_t>(t)));
         x.place = t - static_cast<int64_t>(x.b) * p.sq;
         x.of = p.sq;
         x.q = p.q + x.b * p.qs[0] + x.place * p.qs[2];
@@ -255,6 +270,7 @@ __device__ __forceinline__ int seen_by(const SelectParams& p, const Token& x) {
 
 constexpr int kWarps = 4;        // of a CTA
 constexpr int kMaxRanks = 8;
+constexpr int kBins = 128;       // that scores are counted in
 constexpr int kFew = 256;        // pages between in and out that are ranked one against the others
 
 // A warp's ring: blocks of 16 pages' bounds, a row of 4 D bytes each and 16 more, so that eight rows of a matrix lie in different banks.
@@ -268,9 +284,9 @@ struct Ring {
 
 struct SelectShared {
     int of_warp[3][kMaxRanks * kWarps];   // by warp: the largest magnitude among the bounds, the least and the largest score (ordered)
-    int counts[2][kWarps][32];
+    alignas(16) int bins[kBins];
     int sums[2][kWarps];
-    int found, count, need;
+    int found, count, need, least, largest;
     float value;
     unsigned long long exact;
 };
@@ -383,11 +399,11 @@ __device__ __forceinline__ double exact_score(const SelectParams& p, const Token
 // rows of m16n8k16, q+ and q- of 8 heads its columns. (Bounds in registers as they come, two blocks to a warp, were no faster than one after the
 // other: 16 us for 38 MB.) The products of a block are four sums, for the latency of one.
 //
-// Selection: the value of the k-th largest score. 32 thresholds cut the range evenly, one to a lane, and a warp's lanes count over its share of
-// the scores what lies above theirs; the interval that has the k-th is cut again while it holds many, and those of the last are ranked one
-// against the others. (A round is some 600 clocks of 1,024 scores. Four to a round, each by a sum over the CTA, were 950 a round and five rounds;
-// bins of equal width, by atomics, 3,000 in all.) Then a thread has kItems neighbouring pages in registers (0: reads them each time), and a sum
-// over the CTA places those that are in. kNear: scores and names lie in shared memory, else scores where the workspace is.
+// Selection: the value of the k-th largest score, by counts in bins of equal width, of which the one that has it is cut again while it holds many,
+// and by rank among those of the last. A thread has kItems neighbouring pages in registers (0: reads them each time), and a sum over the
+// CTA places those that are in. (32 thresholds, one to a lane whose warp goes through its share of the scores, were 1,700 clocks a round of 1,024
+// scores, four at a time, each by a sum over the CTA, 950 and five rounds.) kNear: scores, names and exact scores lie in shared memory,
+// else scores and exact ones in the workspace.
 template <int D, int kItems, bool kNear>
 __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_constant__ SelectParams p) {
     using R = Ring<D>;
@@ -401,11 +417,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     constexpr int threads = 32 * kWarps, warps = kWarps;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     if (tid == 0) sm.found = sm.count = 0;
+    for (int i = tid; i < kBins; i += threads) sm.bins[i] = 0;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint32_t pair = blockIdx.x / static_cast<uint32_t>(p.ranks), local = pair / static_cast<uint32_t>(p.kv_heads);
+    const uint32_t pair = p.by_ranks(blockIdx.x), local = p.by_heads(pair);
     const int rank = static_cast<int>(blockIdx.x - pair * p.ranks), hk = static_cast<int>(pair - local * p.kv_heads);
-    const int64_t t = p.token0 + local;
+    const int64_t t = p.token0 + local;   // (under 2^31)
     const Token tok = token_of(p, t);
     const int32_t* row = p.table + max(tok.b, 0) * p.table_stride;
     // Requested before the length is known: the queries of the first 8 heads, and (for the cache) the table's row.
@@ -443,11 +460,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         if (own_block + i * step < p.blocks) issue(i, names);
         cp_async_commit();
     }
-    const int count = static_cast<int>((static_cast<uint32_t>(seen) + p.page_size - 1) / static_cast<uint32_t>(p.page_size)), top = p.top;
+    const int count = static_cast<int>(p.by_page(static_cast<uint32_t>(seen) + p.page_size - 1)), top = p.top;
     int32_t* to = p.chosen + (t * p.kv_heads + hk) * top;
     if (rank == 0 && tid == 0) {
         const int many = min(count, top);
-        p.keys[t * p.kv_heads + hk] = many > 0 ? (many - 1) * p.page_size + (seen - 1) % p.page_size + 1 : 0;
+        p.keys[t * p.kv_heads + hk] = many > 0 ? (many - 1) * p.page_size + static_cast<int>(p.by_page.rest(static_cast<uint32_t>(seen - 1))) + 1 : 0;
     }
     if (count <= top) {   // all of them
         cp_async_wait<0>();
@@ -592,38 +609,17 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     if (rank > 0) return;   // (nobody looks at its shared memory)
 
     // ---- the selection, by the first CTA
-    const int share = ((count + 15) / 16 + kWarps - 1) / kWarps * 16;
-    auto each_of = [&](auto f) {   // this warp's share of the scores, for all lanes, 16 at a time
-        const int last = min((warp + 1) * share, (count + 15) / 16 * 16);
-#pragma unroll 2
-        for (int e = warp * share; e < last; e += 16) {
-            float4 x[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = reinterpret_cast<const float4*>(given + e)[i];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) f(i, x[i]);
-        }
-    };
-    const int mine = kItems ? kItems : ((count + threads - 1) / threads + 3) & ~3, first = tid * mine;
+    const int mine = kItems ? kItems : (count + threads - 1) / threads | 1, first = tid * mine;   // (odd: neighbours in different banks)
     float held[kItems ? kItems : 1];
+    int held_bin[kItems ? kItems : 1];
     if constexpr (kItems > 0) {
 #pragma unroll
         for (int i = 0; i < kItems; i += 4) {
             float4 x = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-            if (first + i < count) x = *reinterpret_cast<const float4*>(given + first + i);   // (whole blocks of 16 are written)
+            if (first + i < count) x = *reinterpret_cast<const float4*>(given + first + i);   // (whole blocks of 16 are written, below everything past the end)
             held[i] = x.x; held[i + 1] = x.y; held[i + 2] = x.z; held[i + 3] = x.w;
         }
     }
-    auto each = [&](auto f) {   // this thread's pages and their scores
-        if constexpr (kItems > 0) {
-#pragma unroll
-            for (int i = 0; i < kItems; ++i) {
-                if (first + i >= begin && first + i < end) f(first + i, held[i]);
-            }
-        } else {
-            for (int e = max(first, begin); e < min(first + mine, end); ++e) f(e, given[e]);
-        }
-    };
     auto name_of = [&](int e) { return kNear ? name_s[e] : row[e]; };
     const bool slot = lane < step;
     const float most = __int_as_float(__reduce_max_sync(0xffffffffu, slot ? sm.of_warp[0][lane] : 0)), mass = norm * most;
@@ -631,69 +627,121 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     // What the fp32 scores may be off by. (What the products could lose below fp32's least normal number is in the last terms.)
     const float off = fmaf(mass, 0x1p-19f, fmaf(norm + most, 0x1p-110f, 0x1p-110f));
     const bool sure = mass < 0x1p120f;   // else, and where it is no number: all in 64 bits
-    if (sure && k > 0) {
-        // The k-th largest is in (a, b].
-        float a = lo - off, b = hi;
-        int above_a = end - begin, above_b = 0;
-        for (int round = 0; round < 8 && above_a - above_b > kRanked && b - a > off; ++round) {
-            const float c = fmaf(b - a, (lane + 1) * 0x1p-5f, a);   // (the last: b)
-            int some[4] = {0, 0, 0, 0};
-            each_of([&](int i, const float4& x) { some[i] += (x.x > c) + (x.y > c) + (x.z > c) + (x.w > c); });
-            sm.counts[round & 1][warp][lane] = (some[0] + some[1]) + (some[2] + some[3]);
-            __syncthreads();
-            int n = 0;
+    // This thread's pages and their scores, and (kItems) pages that are not asked about, whose scores are below all: f(page, score, bin).
+    auto each = [&](auto f) {
+        if constexpr (kItems > 0) {
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) n += sm.counts[round & 1][w][lane];
-            // n falls from lane to lane: the first threshold with fewer than k above it, and the one before.
-            const uint32_t fewer = __ballot_sync(0xffffffffu, n < k || lane == 31);
-            const int at = __ffs(fewer) - 1;
-            const float upper = __shfl_sync(0xffffffffu, c, at), lower = __shfl_sync(0xffffffffu, c, max(at - 1, 0));
-            const int n_upper = __shfl_sync(0xffffffffu, n, at), n_lower = __shfl_sync(0xffffffffu, n, max(at - 1, 0));
-            if (at < 31) {   // (b stays else, and what lies above it)
-                b = upper;
-                above_b = n_upper;
+            for (int i = 0; i < kItems; ++i) f(first + i, held[i], held_bin[i]);
+        } else {
+            int bin = 0;
+            for (int e = max(first, begin); e < min(first + mine, end); ++e) f(e, sure ? given[e] : 0.f, bin);
+        }
+    };
+    // Of those for which pick(page, score, bin) holds: use(page). The few there are, one after another, so that a warp goes through as many as its lane
+    // with the most has, not through all pages of a lane.
+    auto each_of = [&](auto pick, auto use) {
+        if constexpr (kItems > 0) {
+#pragma unroll
+            for (int i0 = 0; i0 < kItems; i0 += 32) {
+                uint32_t mask = 0u;
+#pragma unroll
+                for (int i = i0; i < i0 + 32 && i < kItems; ++i) mask |= static_cast<uint32_t>(pick(first + i, held[i], held_bin[i])) << (i - i0);
+                for (; mask; mask &= mask - 1) use(first + i0 + __ffs(mask) - 1);
             }
-            if (at > 0) {
-                a = lower;
-                above_a = n_lower;
+        } else {
+            each([&](int e, float x, int& bin) {
+                if (pick(e, x, bin)) use(e);
+            });
+        }
+    };
+    int need = k;
+    for (int round = 0; round < 6 && sure && k > 0 && hi - lo > 4.f * off; ++round) {
+        const float by = (kBins - 0.5f) / (hi - lo), low = lo, high = hi;
+        if (!(by < 0x1p100f)) break;
+        // (falls nowhere as x rises; -1 and below: outside)
+        auto bin_of = [&](float x) { return x <= high ? static_cast<int>(floorf((x - low) * by)) : -1; };
+        each([&](int, float x, int& bin) {
+            bin = bin_of(x);
+            if (bin >= 0) atomicAdd(&sm.bins[bin], 1);
+        });
+        __syncthreads();
+        // Every warp for itself: lane l has 4 bins from the top, kBins - 4 (l + 1) .., and looks for the one that has the need-th.
+        const int4 own4 = reinterpret_cast<const int4*>(sm.bins)[kBins / 4 - 1 - lane];
+        const int own[4] = {own4.w, own4.z, own4.y, own4.x}, sum = (own[0] + own[1]) + (own[2] + own[3]);
+        int upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        int above = upto - sum, which = 0, many = own[0];
+        const bool holds = above < need && upto >= need;
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            if (above + many < need) {   // (only the lane that holds it matters)
+                above += many;
+                many = own[i];
+                which = i;
             }
         }
-        if (above_a - above_b <= kRanked) {
-            const int many = above_a - above_b, need = k - above_b;
+        const int holder = __ffs(__ballot_sync(0xffffffffu, holds)) - 1;
+        const int bin = __shfl_sync(0xffffffffu, kBins - 1 - 4 * lane - which, holder);
+        many = __shfl_sync(0xffffffffu, many, holder);
+        need -= __shfl_sync(0xffffffffu, above, holder);
+        if (many <= kRanked) {
             if (tid >= many) later.ranked[tid] = -INFINITY;
-            each([&](int, float x) {
-                if (x > a && x <= b) later.ranked[atomicAdd(&sm.found, 1)] = x;
-            });
+            each_of([&](int, float x, int of) { return (kItems > 0 ? of : bin_of(x)) == bin; }, [&](int e) { later.ranked[atomicAdd(&sm.found, 1)] = given[e]; });
             __syncthreads();
-            // Equal ones in any order.
-            const float x = tid < many ? later.ranked[tid] : 0.f;
-            int better = 0;
-#pragma unroll 4
-            for (int i = 0; i < many; i += 4) {
-                const float4 y = *reinterpret_cast<const float4*>(later.ranked + i);
-                better += (y.x > x || (y.x == x && i < tid)) + (y.y > x || (y.y == x && i + 1 < tid)) + (y.z > x || (y.z == x && i + 2 < tid)) + (y.w > x || (y.w == x && i + 3 < tid));
+            // The need-th of them, equal ones in any order.
+            if (tid < many) {
+                const float x = later.ranked[tid];
+                int better = 0;
+                for (int i = 0; i < many; i += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(later.ranked + i);
+                    better += (y.x > x || (y.x == x && i < tid)) + (y.y > x || (y.y == x && i + 1 < tid)) + (y.z > x || (y.z == x && i + 2 < tid)) + (y.w > x || (y.w == x && i + 3 < tid));
+                }
+                if (better == need - 1) sm.value = x;
             }
-            if (tid < many && better == need - 1) sm.value = x;
             __syncthreads();
             lo = hi = sm.value;
-        } else {
-            lo = a;
-            hi = b;
+            break;
+        }
+        __syncthreads();   // (all have looked at the bins)
+        for (int i = tid; i < kBins; i += threads) sm.bins[i] = 0;
+        if (tid == 0) {
+            sm.least = 0x7fffffff;
+            sm.largest = static_cast<int>(0x80000000);
+        }
+        __syncthreads();
+        each_of([&](int, float x, int of) { return (kItems > 0 ? of : bin_of(x)) == bin; }, [&](int e) {
+            atomicMin(&sm.least, ordered(given[e]));
+            atomicMax(&sm.largest, ordered(given[e]));
+        });
+        __syncthreads();
+        lo = from_ordered(sm.least);
+        hi = from_ordered(sm.largest);
+    }
+    // Pages above are in, pages below are out, those between are counted. (Where nothing is sure all are between, whatever their scores.)
+    const float above = sure ? hi + 2.f * off : 1.f, below = sure ? lo - 2.f * off : 0.f;
+    if constexpr (kItems > 0) {
+        if (!sure) {
+#pragma unroll
+            for (int i = 0; i < kItems; ++i) held[i] = first + i >= begin && first + i < end ? 0.f : -INFINITY;
         }
     }
-    // Pages above are in, pages below are out, those between are counted.
-    const float above = sure ? hi + 2.f * off : INFINITY, below = sure ? lo - 2.f * off : -INFINITY;
+    auto score_of = [&](int e) { return sure ? given[e] : 0.f; };
     auto surely = [&](float x) { return x > above; };
-    auto doubtful = [&](float x) { return !(x > above) && !(x < below); };
+    auto doubtful = [&](float x) { return x >= below && !(x > above); };
     int in = 0, some = 0;
     if (k > 0) {
-        each([&](int, float x) {
-            in += surely(x);
-            some += doubtful(x);
+        each([&](int, float x, int&) {
+            in += x > above;
+            some += x >= below;
         });
+        some -= in;
     }
     int at, all_in, all_some;
-    if (kItems > 0) {   // (fewer than 2^16 of either)
+    if (kItems > 0) {   // (fewer than 2^15 of either)
         at = sum_before(in | some << 16, sm.sums[0], all_in);
         all_some = all_in >> 16;
         all_in &= 0xffff;
@@ -708,21 +756,15 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     to += p.first;
     if (k == 0) return;
     if (all_some == rest) {
-        if (in + some > 0) {
-            each([&](int e, float x) {
-                if (!(x < below)) to[at++] = name_of(e);
-            });
-        }
+        each_of([&](int, float x, int) { return x >= below; }, [&](int e) { to[at++] = name_of(e); });
         return;
     }
     // Some of those between are in, by their exact scores.
-    double* exact = p.exact + static_cast<int64_t>(pair) * p.blocks * 16;
+    double* exact = kNear ? reinterpret_cast<double*>(dynamic + sizeof(SelectLater)) : p.exact + static_cast<int64_t>(pair) * p.blocks * 16;
     unsigned long long value = 0;
     int ties = 0, ties_before = 0;
     if (all_some <= kFew) {
-        each([&](int e, float x) {
-            if (doubtful(x)) later.few_at[atomicAdd(&sm.count, 1)] = e;
-        });
+        each_of([&](int, float x, int) { return doubtful(x); }, [&](int e) { later.few_at[atomicAdd(&sm.count, 1)] = e; });
         __syncthreads();
         for (int i = warp; i < all_some; i += warps) {
             const double x = exact_score<D>(p, tok, hk, name_of(later.few_at[i]));
@@ -742,7 +784,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         // Many that differ by less than the error (alike, most of them): the rest-th largest of their exact scores, eight bits at a time, then
         // those above it and, of its own value, the first.
         for (int e = begin + warp; e < end; e += warps) {
-            if (!doubtful(given[e])) continue;
+            if (!doubtful(score_of(e))) continue;
             const double x = exact_score<D>(p, tok, hk, name_of(e));
             if (lane == 0) exact[e] = x;
         }
@@ -751,8 +793,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         for (int shift = 56; shift >= 0; shift -= 8) {
             for (int i = tid; i < 256; i += threads) later.bins[i] = 0;
             __syncthreads();
-            each([&](int e, float x) {
-                if (!doubtful(x)) return;
+            each_of([&](int, float x, int) { return doubtful(x); }, [&](int e) {
                 const unsigned long long y = ordered(exact[e]);
                 if (shift == 56 || y >> (shift + 8) == value >> (shift + 8)) atomicAdd(&later.bins[y >> shift & 255], 1);
             });
@@ -770,7 +811,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         }
         // Of this thread's pages: those of the value itself, of which the first `ties` of all are in.
         int equal = 0, all;
-        each([&](int e, float x) { equal += doubtful(x) && ordered(exact[e]) == value; });
+        each_of([&](int, float x, int) { return doubtful(x); }, [&](int e) { equal += ordered(exact[e]) == value; });
         ties_before = sum_before(equal, sm.sums[0], all);
     }
     // Whether a doubtful page is in; asked in the order of a thread's pages.
@@ -785,13 +826,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         return y > value || (y == value && equal++ < ties);
     };
     int own = in, all;
-    each([&](int e, float x) {
-        if (doubtful(x)) own += among(e);
-    });
+    each_of([&](int, float x, int) { return doubtful(x); }, [&](int e) { own += among(e); });
     at = sum_before(own, sm.sums[1], all);
     equal = ties_before;
-    each([&](int e, float x) {
-        if (surely(x) || (doubtful(x) && among(e))) to[at++] = name_of(e);
+    each_of([&](int, float x, int) { return x >= below; }, [&](int e) {
+        if (surely(score_of(e)) || among(e)) to[at++] = name_of(e);
     });
 }
 
@@ -806,7 +845,9 @@ struct SelectPlan {
     bool near;               // scores and names in shared memory
     int64_t exact_at, bytes;
 };
-constexpr int kNearBytes = 64 * 1024;   // 8,192 pages
+// Pages whose scores, names and exact scores have room in shared memory.
+template <int D>
+constexpr int kNearPages = D == 128 ? 8192 : 4096;
 
 const char* select_refusal(const ktt_b200_select_args* a) {
     if (a->d != 64 && a->d != 128) return "head dim 64 or 128";
@@ -829,15 +870,15 @@ SelectPlan plan_of(const ktt_b200_select_args* a) {
     SelectPlan s = {};
     s.tokens = a->cu_seqlens_q ? a->total_q : static_cast<int64_t>(a->batch) * a->sq;
     s.blocks = (a->table_width + 15) / 16;
-    s.near = s.blocks * 128 <= kNearBytes;
-    const int64_t one = static_cast<int64_t>(a->kv_heads) * s.blocks * 16 * (s.near ? 8 : 12);   // exact scores, and others
-    int64_t most = kWorkspace / one;
+    s.near = s.blocks * 16 <= (a->d == 64 ? kNearPages<64> : kNearPages<128>);
+    const int64_t one = static_cast<int64_t>(a->kv_heads) * s.blocks * 16 * 12;   // scores, and exact ones
+    int64_t most = s.near ? s.tokens : kWorkspace / one;
     const int64_t ctas = (1ll << 30) / (static_cast<int64_t>(a->kv_heads) * kMaxRanks);   // of a launch
     if (most > ctas) most = ctas;
     s.slice = most < 1 ? 1 : (most < s.tokens ? most : s.tokens);
     const int64_t n = s.slice * a->kv_heads * s.blocks * 16;
-    s.exact_at = s.near ? 0 : (n * 4 + 255) / 256 * 256;
-    s.bytes = s.exact_at + n * 8;
+    s.exact_at = (n * 4 + 255) / 256 * 256;
+    s.bytes = s.near ? 0 : s.exact_at + n * 8;
     return s;
 }
 
@@ -847,9 +888,10 @@ int launch_select(const SelectParams& p, int64_t pairs, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(pairs * p.ranks));
     cfg.blockDim = dim3(32 * kWarps);
+    static_assert(!kNear || sizeof(SelectLater) + kNearPages<D> * 8 <= Ring<D>::kBytes, "exact scores lie where the rings were");
     cfg.dynamicSmemBytes = Ring<D>::kBytes + (kNear ? static_cast<size_t>(p.blocks) * 128 : 0);
     cfg.stream = stream;
-    if (int rc = ensure_smem(kernel, Ring<D>::kBytes + (kNear ? kNearBytes : 0), "cudaFuncSetAttribute(select)")) return rc;
+    if (int rc = ensure_smem(kernel, Ring<D>::kBytes + (kNear ? kNearPages<D> * 8 : 0), "cudaFuncSetAttribute(select)")) return rc;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -869,10 +911,12 @@ int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t 
         // Two CTAs to an SM: as many to a pair as there is room for and blocks for all their warps.
         p.ranks = 1;
         while (p.ranks < kMaxRanks && pairs * p.ranks * 2 <= 2 * 148 && p.ranks * kWarps < plan.blocks) p.ranks *= 2;
+        p.by_ranks = Divisor(p.ranks);
         int rc;
         if (!plan.near) rc = launch_select<D, 0, false>(p, pairs, stream);
         else if (width <= 8 * 32 * kWarps) rc = launch_select<D, 8, true>(p, pairs, stream);
-        else rc = launch_select<D, 0, true>(p, pairs, stream);
+        else if (width <= 32 * 32 * kWarps) rc = launch_select<D, 32, true>(p, pairs, stream);
+        else rc = launch_select<D, 64, true>(p, pairs, stream);
         if (rc) return rc;
     }
     return 0;
@@ -931,12 +975,15 @@ extern "C" int ktt_b200_paged_select(const ktt_b200_select_args* a, void* stream
     if (s.tokens == 0) return 0;
     if (s.tokens >= (1ll << 31)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_select: fewer than 2^31 tokens");
     if (!a->q || !a->bounds || !a->block_table || !a->lengths || !a->chosen || !a->keys) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_select: null pointer");
-    if (!a->workspace || a->workspace_bytes < s.bytes) {
+    if (s.bytes && (!a->workspace || a->workspace_bytes < s.bytes)) {
         return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_select: workspace holds %lld bytes, %lld needed", static_cast<long long>(a->workspace_bytes), static_cast<long long>(s.bytes));
     }
     if (reinterpret_cast<uintptr_t>(a->workspace) & 15) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_select: the workspace must be 16-byte aligned");
     SelectParams p = {};
     if (const char* why = bounds_of(p.bounds, const_cast<void*>(a->bounds), a->bounds_strides)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_select: %s", why);
+    p.by_page = Divisor(a->page_size);
+    p.by_sq = Divisor(a->sq < 1 ? 1 : a->sq);
+    p.by_heads = Divisor(a->kv_heads);
     p.q = static_cast<const __nv_bfloat16*>(a->q);
     for (int i = 0; i < 3; ++i) p.qs[i] = a->q_strides[i];
     p.cu = a->cu_seqlens_q;
@@ -958,8 +1005,10 @@ extern "C" int ktt_b200_paged_select(const ktt_b200_select_args* a, void* stream
     p.blocks = s.blocks;
     p.width = a->table_width;
     unsigned char* base = static_cast<unsigned char*>(a->workspace);
-    p.scores = s.near ? nullptr : reinterpret_cast<float*>(base);
-    p.exact = reinterpret_cast<double*>(base + s.exact_at);
+    if (!s.near) {
+        p.scores = reinterpret_cast<float*>(base);
+        p.exact = reinterpret_cast<double*>(base + s.exact_at);
+    }
     p.chosen = a->chosen;
     p.keys = a->keys;
     cudaStream_t st = static_cast<cudaStream_t>(stream);

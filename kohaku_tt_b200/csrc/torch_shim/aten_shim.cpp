@@ -1486,11 +1486,11 @@ bool tables_of(ktt_b200_tables& a, PyObject* const* args, PyObject* count_out) {
     return true;
 }
 
-// A vector in the memory of `whole`, from a byte on.
-Tensor part_of(const Tensor& whole, int64_t byte, int64_t size, at::ScalarType type) {
+// A tensor in the memory of `whole`, from a byte on.
+Tensor part_of(const Tensor& whole, int64_t byte, at::IntArrayRef sizes, at::ScalarType type) {
     Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), c10::scalarTypeToTypeMeta(type));
     t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(type)));
-    t.unsafeGetTensorImpl()->set_sizes_contiguous({size});
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
     return t;
 }
 
@@ -1509,10 +1509,10 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
         // In one allocation, slots first.
         const int64_t slots = (8 * static_cast<int64_t>(tokens) + 15) / 16 * 16, positions = (4 * static_cast<int64_t>(tokens) + 15) / 16 * 16, cu = (4 * (static_cast<int64_t>(a.batch) + 1) + 15) / 16 * 16;
         const Tensor all = empty_cuda({slots + positions + cu + 4 * static_cast<int64_t>(a.batch)}, at::kByte, table);
-        out[0] = part_of(all, slots + positions, a.batch + 1, at::kInt);
-        out[1] = part_of(all, slots, tokens, at::kInt);
-        out[2] = part_of(all, 0, tokens, at::kLong);
-        out[3] = part_of(all, slots + positions + cu, a.batch, at::kInt);
+        out[0] = part_of(all, slots + positions, {a.batch + 1}, at::kInt);
+        out[1] = part_of(all, slots, {tokens}, at::kInt);
+        out[2] = part_of(all, 0, {tokens}, at::kLong);
+        out[3] = part_of(all, slots + positions + cu, {a.batch}, at::kInt);
         raise_status(ktt_b200_paged_reserve(&a, tensor_of(args[2])->data_ptr<int32_t>(), tokens, out[0].data_ptr<int32_t>(), out[1].data_ptr<int32_t>(),
                                             out[2].data_ptr<int64_t>(), out[3].data_ptr<int32_t>(), at::cuda::getCurrentCUDAStream()),
                      "paged_reserve");
@@ -1612,12 +1612,16 @@ PyObject* py_paged_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
         set3(a.bounds_strides, *bounds);
         const int64_t need = ktt_b200_paged_select_workspace(&a);
         if (need < 0) raise_status(KTT_B200_ERR_UNSUPPORTED, "paged_select");
-        chosen = empty_cuda({tokens, a.kv_heads, a.top}, at::kInt, *q);
-        keys = empty_cuda({tokens, a.kv_heads}, at::kInt, *q);
-        const Tensor work = empty_cuda({std::max<int64_t>(need, 16)}, at::kByte, *q);
+        // In one allocation; a workspace is for long tables only.
+        const int64_t names = (tokens * a.kv_heads * a.top + 3) / 4 * 4;
+        const Tensor all = empty_cuda({4 * (names + tokens * a.kv_heads)}, at::kByte, *q);
+        chosen = part_of(all, 0, {tokens, a.kv_heads, a.top}, at::kInt);
+        keys = part_of(all, 4 * names, {tokens, a.kv_heads}, at::kInt);
+        Tensor work;
+        if (need > 0) work = empty_cuda({need}, at::kByte, *q);
         a.chosen = chosen.data_ptr<int32_t>();
         a.keys = keys.data_ptr<int32_t>();
-        a.workspace = work.data_ptr();
+        a.workspace = need > 0 ? work.data_ptr() : nullptr;
         a.workspace_bytes = need;
         raise_status(ktt_b200_paged_select(&a, at::cuda::getCurrentCUDAStream()), "paged_select");
     });

@@ -143,10 +143,12 @@ def test_selections_that_no_entry_takes(built_lib, kw, text):
 
 
 def test_select_refusals(built_lib):
-    need = built_lib.ktt_b200_paged_select_workspace(ctypes.byref(_select()))
+    assert built_lib.ktt_b200_paged_select_workspace(ctypes.byref(_select())) == 0
+    wide = dict(table_width=9000, table_stride=9000)      # scores that do not fit shared memory
+    need = built_lib.ktt_b200_paged_select_workspace(ctypes.byref(_select(**wide)))
     assert need > 0
-    for kw in (dict(batch=0), dict(sq=-1), dict(q=None, workspace_bytes=need), dict(bounds=None, workspace_bytes=need), dict(workspace=None, workspace_bytes=need),
-               dict(workspace_bytes=need - 1), dict(workspace=4104, workspace_bytes=need)):
+    for kw in (dict(batch=0), dict(sq=-1), dict(q=None), dict(bounds=None), dict(chosen=None), dict(keys=None), dict(workspace=None, workspace_bytes=need, **wide),
+               dict(workspace_bytes=need - 1, **wide), dict(workspace=4104, workspace_bytes=need, **wide)):
         assert built_lib.ktt_b200_paged_select(ctypes.byref(_select(**kw)), None) == _lib.ERR_BAD_ARGUMENT, kw
     a = _select(workspace_bytes=need)
     a.bounds_strides[0] = 4
