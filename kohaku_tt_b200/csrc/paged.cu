@@ -41,6 +41,7 @@ struct AppendParams {
     int batch, rows, heads, kv_heads;
     int groups;            // blocks of `loops` times kHeads queries' heads; those of the keys and of the values follow in the grid's y
     int loops;
+    unsigned pair_blocks, pair_rows;   // blocks of the first part (append_queries), and of one group of heads there; the others follow in the grid's x, if any
     int64_t tokens;        // rows of all sequences
     const __nv_bfloat16* q;
     __nv_bfloat16* q_out;
@@ -103,12 +104,103 @@ __device__ __forceinline__ uint2 put_four_bits(const Eight<__nv_bfloat16>& x, un
     return held;
 }
 
+// Where row n of the new ones goes: its sequence and how many keys that has; kEach threads of a warp share a row.
+struct Row {
+    int b, cached;
+    int64_t in;      // its place among the sequence's new ones
+    bool there;
+};
+template <int kEach>
+__device__ __forceinline__ Row row_at(const AppendParams& p, int64_t n, int b, int64_t r, bool in_range) {
+    Row x = {b, 0, r, in_range};
+    if (p.cu && p.batch < 32) {
+        // A lane looks at one sequence each, its length with it: one trip where a search takes log2(batch) + 2 that wait for one
+        // another (8 sequences, 10,240 tokens, 32 heads over 8, D 128, 4 bits: 61.5 us with a search).
+        const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31, start = p.cu[min(lane, p.batch)], keys = cached_keys(p.c, min(lane, p.batch - 1));
+#pragma unroll
+        for (int i = 0; i < 32 / kEach; ++i) {   // (the last sequence that starts at or before the token)
+            const int64_t token = __shfl_sync(0xffffffffu, n, i * kEach);
+            const uint32_t before = __ballot_sync(0xffffffffu, lane <= p.batch && start <= token);
+            if (token == n) x.b = __popc(before) - 1;
+        }
+        x.there = in_range && x.b >= 0 && x.b < p.batch;
+        if (!x.there) x.b = 0;
+        x.in = n - __shfl_sync(0xffffffffu, start, x.b);
+        x.there = x.there && x.in >= 0;   // (offsets that decrease)
+        x.cached = __shfl_sync(0xffffffffu, keys, x.b);
+    } else if (in_range) {
+        if (p.cu) {
+            x.b = sequence_of(p.cu, p.batch, n);
+            x.there = x.b >= 0;
+            x.b = x.there ? x.b : 0;
+            x.in = n - p.cu[x.b];
+        }
+        x.cached = cached_keys(p.c, x.b);
+    }
+    return x;
+}
+
+// What a row turns by: its place, or positions of its own. (Packed rows have one batch entry's positions; without any, the place is the only
+// axis, and all pairs are of axis 0.)
+template <bool kFast, typename Params>
+__device__ __forceinline__ void turn_of(Turned<kFast>& turned, const Params& p, const Row& x, int64_t r, int col) {
+    const int64_t pos = x.cached + x.in;
+    if constexpr (std::is_same_v<Params, AppendAtParams>) {
+        Positions<true> at = {};
+        if (p.positions.at) at = p.positions.all(p.axes.axes, p.cu ? 0 : x.b, r);
+        else at.at[0] = pos;
+        turned.load(p.turn, p.axes, at, col);
+    } else {
+        turned.load(p.turn, pos, col);
+    }
+}
+
+// Many queries in the half layout: a thread has eight pairs, both columns of each, of four heads of a token at a time, as in the rotation
+// (rotary_pairs_kernel), or 16 columns that do not turn.
+template <int D, typename Params>
+__device__ __forceinline__ void append_queries(const Params& p) {
+    constexpr int kEach = D / 16, kHeads = 4;
+    const uint32_t group = blockIdx.x / p.pair_rows, rows = blockIdx.x - group * p.pair_rows;
+    const int tid = threadIdx.y * blockDim.x + threadIdx.x, half = p.turn.half, pair = tid % kEach * 8;
+    const int64_t n = static_cast<int64_t>(rows) * (256 / kEach) + tid / kEach;
+    const bool in_range = n < p.tokens, turns = pair < half;
+    const int b = in_range && !p.cu ? static_cast<int>(static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows)) : 0;
+    const int64_t r = !in_range ? 0 : p.cu ? n : n - static_cast<int64_t>(b) * p.rows;
+    const int col = turns ? pair : 2 * pair, other = turns ? pair + half : 2 * pair + 8;
+    const __nv_bfloat16* from = p.q + (p.cu ? 0 : b * p.qs[0]) + r * p.qs[2];
+    Eight<__nv_bfloat16> lo[kHeads], hi[kHeads];
+    auto rows_of = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            const __nv_bfloat16* row = from + static_cast<int64_t>(min(h0 + i, p.heads - 1)) * p.qs[1];
+            lo[i].load(row + col);
+            hi[i].load(row + other);
+        }
+    };
+    int h0 = static_cast<int>(group) * (kHeads * p.loops);
+    const Row x = row_at<kEach>(p, n, b, r, in_range);
+    if (!x.there) return;
+    Turned<true> turned;
+    if (turns) turn_of(turned, p, x, r, col);
+    __nv_bfloat16* out = p.q_out + (p.cu ? 0 : x.b * p.qos[0]) + r * p.qos[2];
+    for (int loop = 0; loop < p.loops && h0 < p.heads; ++loop, h0 += kHeads) {
+        rows_of(h0);
+#pragma unroll
+        for (int i = 0; i < kHeads; ++i) {
+            if (h0 + i >= p.heads) break;
+            if (turns) turned.both(lo[i], hi[i]);
+            __nv_bfloat16* to = out + (h0 + i) * p.qos[1];
+            lo[i].store(to + col);
+            hi[i].store(to + other);
+        }
+    }
+}
+
 // A thread has eight columns of kHeads heads of one token, and of the next kHeads, `loops` times: of queries, keys or values. Its first rows are
 // requested before it knows where they go (a packed row's sequence takes a search). No thread leaves before the groups' shuffles.
 template <int D, int kBits, bool kFast, int kHeads, typename Params>
 __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const __grid_constant__ Params p) {
     constexpr bool kAt = std::is_same_v<Params, AppendAtParams>;
-    const int64_t n = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
     const int chunk = threadIdx.x, col = chunk * 8;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -118,19 +210,30 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
             p.lengths_out[b] = static_cast<int32_t>(all < p.c.cap ? all : p.c.cap);
         }
     }
+    if constexpr (kFast && kHeads > 1) {
+        if (blockIdx.x < p.pair_blocks) return append_queries<D>(p);
+    }
     // What the block has: queries, keys or values.
     const int loops = kHeads == 1 ? 1 : p.loops, per = kHeads * loops;
-    const int y = blockIdx.y, kv = (p.kv_heads + per - 1) / per;
-    const int what = y < p.groups ? 0 : y < p.groups + kv ? 1 : 2;
-    int h0 = (y - (what == 0 ? 0 : what == 1 ? p.groups : p.groups + kv)) * per;
+    const int kv = (p.kv_heads + per - 1) / per;
+    uint32_t bx = blockIdx.x, y = blockIdx.y;
+    if (kFast && kHeads > 1 && p.pair_blocks) {   // (keys and values, one group of heads after another)
+        const uint32_t blocks = (gridDim.x - p.pair_blocks) / (2 * kv);
+        y = (bx - p.pair_blocks) / blocks;
+        bx -= p.pair_blocks + y * blocks;
+        y += p.groups;
+    }
+    const int64_t n = static_cast<int64_t>(bx) * blockDim.y + threadIdx.y;
+    const int what = static_cast<int>(y) < p.groups ? 0 : static_cast<int>(y) < p.groups + kv ? 1 : 2;
+    int h0 = (static_cast<int>(y) - (what == 0 ? 0 : what == 1 ? p.groups : p.groups + kv)) * per;
     const int heads = what == 0 ? p.heads : p.kv_heads;
     const __nv_bfloat16* from = what == 0 ? p.q : what == 1 ? p.k : p.v;
     const int64_t sb = what == 0 ? p.qs[0] : what == 1 ? p.ks[0] : p.vs[0], sh = what == 0 ? p.qs[1] : what == 1 ? p.ks[1] : p.vs[1];
     const int64_t sr = what == 0 ? p.qs[2] : what == 1 ? p.ks[2] : p.vs[2];
     const bool in_range = n < p.tokens;
-    int b = in_range && !p.cu ? static_cast<int>(static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows)) : 0;   // (2^31 tokens at most)
-    int64_t r = !in_range ? 0 : p.cu ? n : n - static_cast<int64_t>(b) * p.rows;
-    from += (p.cu ? 0 : b * sb) + r * sr;
+    const int b0 = in_range && !p.cu ? static_cast<int>(static_cast<uint32_t>(n) / static_cast<uint32_t>(p.rows)) : 0;   // (2^31 tokens at most)
+    const int64_t r = !in_range ? 0 : p.cu ? n : n - static_cast<int64_t>(b0) * p.rows;
+    from += (p.cu ? 0 : b0 * sb) + r * sr;
     Eight<__nv_bfloat16> x[kHeads], other[kHeads];
     const int partner = what == 2 || !p.turn.cos || p.turn.interleaved || col >= 2 * p.turn.half ? -1 : col < p.turn.half ? col + p.turn.half : col - p.turn.half;
     auto rows_of = [&](int h0) {
@@ -147,48 +250,13 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
         }
     };
     rows_of(h0);
-    int64_t in = r;          // the row's place among the sequence's new ones
-    bool row_there = in_range;
-    int cached = 0;
-    if (p.cu && p.batch < 32) {
-        // A lane looks at one sequence each, its length with it: one trip where a search takes log2(batch) + 2 that wait for one
-        // another (8 sequences, 10,240 tokens, 32 heads over 8, D 128, 4 bits: 61.5 us with a search).
-        const int lane = (threadIdx.y * blockDim.x + threadIdx.x) & 31, start = p.cu[min(lane, p.batch)], keys = cached_keys(p.c, min(lane, p.batch - 1));
-        constexpr int kTokens = 32 / (D / 8);
-#pragma unroll
-        for (int i = 0; i < kTokens; ++i) {   // (the last sequence that starts at or before the token)
-            const int64_t token = __shfl_sync(0xffffffffu, n, i * (D / 8));
-            const uint32_t before = __ballot_sync(0xffffffffu, lane <= p.batch && start <= token);
-            if (token == n) b = __popc(before) - 1;
-        }
-        row_there = in_range && b >= 0 && b < p.batch;
-        if (!row_there) b = 0;
-        in = n - __shfl_sync(0xffffffffu, start, b);
-        row_there = row_there && in >= 0;   // (offsets that decrease)
-        cached = __shfl_sync(0xffffffffu, keys, b);
-    } else if (in_range) {
-        if (p.cu) {
-            b = sequence_of(p.cu, p.batch, n);
-            row_there = b >= 0;
-            b = row_there ? b : 0;
-            in = n - p.cu[b];
-        }
-        cached = cached_keys(p.c, b);
-    }
-    const int64_t pos = row_there ? cached + in : 0;
+    const Row x_row = row_at<D / 8>(p, n, b0, r, in_range);
+    const int b = x_row.b;
+    const bool row_there = x_row.there;
+    const int64_t pos = row_there ? x_row.cached + x_row.in : 0;
     Turned<kFast> turned;
     turned.count = 0;
-    if constexpr (kAt) {
-        if (what != 2 && row_there) {
-            // (Packed rows have one batch entry's positions; without any, the place is the only axis, and all pairs are of axis 0.)
-            Positions<true> at = {};
-            if (p.positions.at) at = p.positions.all(p.axes.axes, p.cu ? 0 : b, r);
-            else at.at[0] = pos;
-            turned.load(p.turn, p.axes, at, col);
-        }
-    } else {
-        if (what != 2 && row_there) turned.load(p.turn, pos, col);
-    }
+    if (what != 2 && row_there) turn_of(turned, p, x_row, r, col);
     if (what == 0) {
         if (!row_there) return;
         __nv_bfloat16* to = p.q_out + (p.cu ? 0 : b * p.qos[0]) + r * p.qos[2] + col;
@@ -444,26 +512,36 @@ int launch_append(const Params& given, cudaStream_t stream) {
     Params p = given;
     const dim3 block(D / 8, 256 / (D / 8));
     const int64_t blocks = (p.tokens + block.y - 1) / block.y;   // one at least: it writes the new lengths
-    auto go = [&](auto kernel, int per) {
+    auto go = [&](auto kernel, int per, bool pairs) {   // pairs: queries by append_queries
         per *= p.loops;
         p.groups = (p.heads + per - 1) / per;
-        const dim3 grid(static_cast<unsigned>(blocks > 0 ? blocks : 1), static_cast<unsigned>(p.groups + 2 * ((p.kv_heads + per - 1) / per)));
-        return launch_dependent(kernel, p, grid, block, stream, "paged_append launch");
+        const unsigned kv = 2 * ((p.kv_heads + per - 1) / per), rows = static_cast<unsigned>(blocks > 0 ? blocks : 1);
+        p.pair_blocks = 0;
+        if (pairs && p.heads) {
+            p.pair_rows = static_cast<unsigned>((p.tokens + 4096 / D - 1) / (4096 / D));
+            const int64_t all = static_cast<int64_t>(p.pair_rows) * p.groups + static_cast<int64_t>(rows) * kv;
+            if (all < (1ll << 31)) {
+                p.pair_blocks = p.pair_rows * p.groups;
+                return launch_dependent(kernel, p, dim3(static_cast<unsigned>(all)), block, stream, "paged_append launch");
+            }
+        }
+        return launch_dependent(kernel, p, dim3(rows, p.groups + kv), block, stream, "paged_append launch");
     };
     const bool fast = p.vec && turn_is_fast(p.turn);
     // Four heads to a thread once that makes threads enough, and four more after them: a token's place, page and table rows are looked up once for
-    // all of them. 32 heads over 8, D 128, us for 1 and 4 heads: 256 tokens, 4 bits 4.6 and 5.4; 512, bf16 6.0 and 3.9; 1,024, 4 bits 11.5 and 8.2. For
-    // 4, 8, 16 and 32 heads: 2,048 tokens, bf16 12.2, 10.8, 10.1, 16.0; 10,240 packed ones, bf16 52.3, 46.2, 44.5, 43.7 (5.4 TB/s), 4 bits 61.2, 54.1, 52.6,
-    // 51.0, and by positions of three axes 88, 70, 65, 61.
+    // all of them. 32 heads over 8, D 128, us for 1 and 4 heads: 256 tokens, 4 bits 4.6 and 5.4; 512, bf16 6.0 and 3.9; 1,024, 4 bits 11.5 and 7.7. For
+    // 4, 8, 16 and 32 heads: 1,024 tokens, 4 bits 7.7, 10.1, 10.6, 14.3; 2,048, bf16 10.9, 9.8, 12.4, 18.2; 4,096, 4 bits 23.1, 22.4, 19.7, 20.6; 10,240
+    // packed ones, 4 bits 54.4, 49.4, 48.1, 46.6 (bf16 42.0, 5.6 TB/s), by positions of three axes 67.4, 57.9, 56.7, 54.7. With queries in the
+    // half layout as keys are, eight columns to a thread, 51.0 and 61.4.
     p.loops = 1;
     const int64_t threads = p.tokens * (D / 8) * (p.heads + 2 * p.kv_heads);
     if (threads >= 3 << 17) {
-        p.loops = threads < 1 << 20 ? 1 : (threads < 1 << 22 ? 4 : 8);
-        if (fast) return go(append_kernel<D, kBits, true, 4, Params>, 4);
-        return go(append_kernel<D, kBits, false, 4, Params>, 4);
+        p.loops = threads < 7 << 17 ? 1 : (threads < 1 << 21 ? 2 : (threads < 1 << 22 ? 4 : 8));
+        if (fast) return go(append_kernel<D, kBits, true, 4, Params>, 4, p.turn.cos && !p.turn.interleaved);
+        return go(append_kernel<D, kBits, false, 4, Params>, 4, false);
     }
-    if (fast) return go(append_kernel<D, kBits, true, 1, Params>, 1);
-    return go(append_kernel<D, kBits, false, 1, Params>, 1);
+    if (fast) return go(append_kernel<D, kBits, true, 1, Params>, 1, false);
+    return go(append_kernel<D, kBits, false, 1, Params>, 1, false);
 }
 
 template <int D, int kBits>

@@ -268,15 +268,7 @@ __global__ void __launch_bounds__(256) rotary_pairs_kernel(const __grid_constant
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
             if (h0 + j >= heads) break;
-            if (turns) {
-                const Eight<T> first = lo[j];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float u = to_f32(first.get(e)), v = to_f32(hi[j].get(e)), c = turned.c[e], s = turned.s[e];
-                    lo[j].set(e, from_f32<T>(__fadd_rn(__fmul_rn(u, c), __fmul_rn(v, s))));
-                    hi[j].set(e, from_f32<T>(__fadd_rn(__fmul_rn(v, c), __fmul_rn(u, -s))));
-                }
-            }
+            if (turns) turned.both(lo[j], hi[j]);
             T* to = y + (h0 + j) * p.ys[which][1];
             lo[j].store(to + col);
             hi[j].store(to + other);

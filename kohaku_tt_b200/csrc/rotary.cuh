@@ -226,6 +226,17 @@ struct Turned {
         }
     }
 
+    // Half layout, loaded for eight first columns: they and their partners.
+    template <typename T>
+    __device__ __forceinline__ void both(Eight<T>& lo, Eight<T>& hi) const {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float u = to_f32(lo.get(e)), v = to_f32(hi.get(e));
+            lo.set(e, from_f32<T>(__fadd_rn(__fmul_rn(u, c[e]), __fmul_rn(v, s[e]))));
+            hi.set(e, from_f32<T>(__fadd_rn(__fmul_rn(v, c[e]), __fmul_rn(u, -s[e]))));
+        }
+    }
+
     // x: columns [col, col + 8) of a row of d columns that starts at `row`.
     template <typename T>
     __device__ __forceinline__ void apply(const Turn& t, Eight<T>& x, const Eight<T>& other, const T* row, int col) const {

@@ -251,17 +251,30 @@ def _chosen(q, k_pages, v_pages, chosen, keys, scale, max_k):
 
 # ---- operators for compiled graphs (which pass tensors, not lists) ---------------------------
 
-@torch.library.custom_op("ktt_b200::_paged_append", mutates_args=("k_pages", "v_pages", "lengths_out", "bounds"), device_types="cuda")
+@torch.library.custom_op("ktt_b200::_paged_append", mutates_args=("k_pages", "v_pages", "lengths_out"), device_types="cuda")
 def _append_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
                cos: torch.Tensor | None, sin: torch.Tensor | None, q: torch.Tensor | None, interleaved: bool, cu_seq: torch.Tensor | None,
-               lengths_out: torch.Tensor | None, positions: torch.Tensor | None = None, axes: Sequence[int] | None = None,
-               bounds: torch.Tensor | None = None) -> torch.Tensor:
+               lengths_out: torch.Tensor | None) -> torch.Tensor:
+    out = _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+    return k.new_empty((0,)) if out is None else out
+
+
+@torch.library.custom_op("ktt_b200::_paged_append_at", mutates_args=("k_pages", "v_pages", "lengths_out", "bounds"), device_types="cuda")
+def _append_at_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
+                  cos: torch.Tensor | None, sin: torch.Tensor | None, q: torch.Tensor | None, interleaved: bool, cu_seq: torch.Tensor | None,
+                  lengths_out: torch.Tensor | None, positions: torch.Tensor | None, axes: Sequence[int] | None, bounds: torch.Tensor | None) -> torch.Tensor:
+    """With positions or bounds. (As arguments of the operator above that are None by default they would be lost on their way.)"""
     out = _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
     return k.new_empty((0,)) if out is None else out
 
 
 @_append_op.register_fake
-def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions=None, axes=None, bounds=None):
+def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out):
+    return k.new_empty((0,)) if q is None else ops._empty_like_rows(q)
+
+
+@_append_at_op.register_fake
+def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds):
     return k.new_empty((0,)) if q is None else ops._empty_like_rows(q)
 
 
@@ -323,8 +336,11 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
     interleaved = bool(interleaved)
     if torch.compiler.is_compiling():
-        out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out,
-                                               positions, axes, bounds)
+        if positions is None and axes is None and bounds is None:
+            out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
+        else:
+            out = torch.ops.ktt_b200._paged_append_at(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out,
+                                                      positions, axes, bounds)
         return out if q is not None else None
     # Eager calls on plain CUDA tensors are served by C++ in one step.
     eager = _lib.native()
