@@ -161,6 +161,42 @@ def test_append(cuda, path, bits, d, pairs, interleaved, packed):
         assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(plain, got))
 
 
+@pytest.mark.parametrize("bits,d,h,hk,r,batch,tokens", [(16, 128, 13, 4, 128, 3, 1500), (4, 128, 12, 4, 64, 40, 4100), (16, 64, 14, 2, 64, 5, 12000), (4, 128, 33, 3, 128, 2, 7000),
+                                                        (4, 64, 9, 9, 32, 33, 21000), (16, 128, 16, 2, 20, 2, 6000)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_of_many_rows(cuda, bits, d, h, hk, r, batch, tokens, interleaved):
+    """Threads with several groups of heads, and queries by pairs: rows are those that `rotary` makes, at their places; packed rows of no sequence
+    are left, those of few sequences and of many are found."""
+    g = torch.Generator(device=cuda).manual_seed(1)
+    k, v, q = (torch.randn((tokens, x, d), generator=g, device=cuda).to(torch.bfloat16) for x in (hk, hk, h))
+    cut = torch.randint(0, tokens - 7, (batch - 1,), generator=torch.Generator().manual_seed(2)).sort().values.tolist()
+    cu = torch.tensor([0, *cut, tokens - 7], dtype=torch.int32, device=cuda)
+    counts = (cu[1:] - cu[:-1]).tolist()
+    lengths, page = torch.randint(0, 40, (batch,), generator=torch.Generator().manual_seed(3)).to(device=cuda, dtype=torch.int32), 16
+    wide = max(-(-(n + 40) // page) for n in counts)
+    used = [-(-(n + int(m)) // page) for n, m in zip(counts, lengths)]
+    table, names = torch.full((batch, wide), -1, dtype=torch.int32), torch.randperm(sum(used), generator=torch.Generator().manual_seed(4)).to(torch.int32)
+    for i, n in enumerate(used):
+        table[i, :n] = names[sum(used[:i]):sum(used[:i]) + n]
+    table = table.to(cuda)
+    cos, sin = ktt.rotary_table(wide * page, r, device=cuda)
+    at = torch.cat([torch.arange(n) + int(m) for n, m in zip(counts, lengths)] + [torch.zeros(7, dtype=torch.int64)]).to(cuda)
+    three = torch.randint(0, wide * page, (3, tokens), generator=g, device=cuda)
+    for pos, axes in ((None, None), (three, _axes("turns", r // 2, 3))):
+        want_q, want_k = ktt.rotary(q, k, cos, sin, positions=at if pos is None else pos, interleaved=interleaved, axes=axes)
+        plain, got = (ktt.paged_cache(sum(used), hk, page, d, bits=bits, device=cuda) for _ in range(2))
+        bounds = ktt.paged_bounds(got[0], table, lengths)
+        for b in range(batch):      # a sequence at a time, in lots of few rows
+            for i in range(0, counts[b], 300):
+                rows = slice(int(cu[b]) + i, int(cu[b]) + min(i + 300, counts[b]))
+                ktt.paged_append(want_k[rows].transpose(0, 1)[None], v[rows].transpose(0, 1)[None], *plain, table[b:b + 1], lengths[b:b + 1] + i)
+        out = ktt.paged_append(k, v, *got, table, lengths, cos, sin, q=q, interleaved=interleaved, cu_seq=cu, positions=pos, axes=axes, bounds=bounds)
+        assert torch.equal(out[:-7], want_q[:-7])
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(plain, got))
+        after = lengths + (cu[1:] - cu[:-1])
+        assert torch.equal(bounds, ktt.paged_bounds(plain[0], table, after))
+
+
 def test_compiled(cuda):
     """One graph, queries and keys, both gradients and one alone."""
     cos, sin = ktt.rotary_table(16, 64, device=cuda)
@@ -178,6 +214,14 @@ def test_compiled(cuda):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     (a,), (b,) = torch.autograd.grad(want[1], kl, k), torch.autograd.grad(torch.compile(lambda x: turned(q, x)[1], fullgraph=True)(kl), kl, k)
     assert torch.equal(a, b)
+    # An append by such positions, without bounds.
+    table, lens = torch.arange(4, dtype=torch.int32, device=cuda).view(2, 2), torch.zeros(2, dtype=torch.int32, device=cuda)
+    pages, same = ktt.paged_cache(4, 2, 16, 64, device=cuda), ktt.paged_cache(4, 2, 16, 64, device=cuda)
+
+    def append(kp, vp):
+        return ktt.paged_append(k, k, kp, vp, table, lens, cos, sin, q=q, positions=at, axes=axes)
+
+    assert torch.equal(torch.compile(append, fullgraph=True)(*pages), append(*same)) and torch.equal(pages[0], same[0])
     out = torch.ops.ktt_b200._rotary_axes(ql, kl, cos, sin, at, False, False, list(axes))
     assert torch.equal(torch.autograd.grad(out[1], kl, k)[0], a)
 
