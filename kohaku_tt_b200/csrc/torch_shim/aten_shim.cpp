@@ -1160,7 +1160,8 @@ struct Cache {
     ktt_b200_pages c;
     int64_t dim = 0, batch = 0, cap = 0;
 };
-bool cache_of(Cache& x, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, PyObject* max_k) {
+// own: a table for each token and head, [tokens, Hk, pages], as sequences of a token and head each.
+bool cache_of(Cache& x, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, PyObject* max_k, bool own = false) {
     if (!plain(k) || !plain(v) || !plain(table) || !plain(lengths)) return false;
     if (k.dim() != 4 || k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || k.device() != v.device() || k.numel() == 0) return false;
     const bool four = k.scalar_type() == at::kByte;
@@ -1169,10 +1170,18 @@ bool cache_of(Cache& x, const Tensor& k, const Tensor& v, const Tensor& table, c
     for (const Tensor* p : {&k, &v}) {
         if (p->stride(3) != 1 || (four && p->size(2) > 1 && p->stride(2) != p->size(3))) return false;
     }
-    if (table.scalar_type() != at::kInt || table.dim() != 2 || table.size(1) < 1 || table.stride(1) != 1 || table.device() != k.device()) return false;
-    if (!int32_vector(lengths, k, table.size(0))) return false;
-    x.batch = table.size(0);
-    x.cap = table.size(1) * k.size(2);
+    if (table.scalar_type() != at::kInt || table.device() != k.device()) return false;
+    if (own) {
+        if (table.dim() != 3 || !table.is_contiguous() || table.numel() == 0 || table.size(1) != k.size(1) || table.size(0) > INT32_MAX / table.size(1)) return false;
+        if (lengths.scalar_type() != at::kInt || lengths.device() != k.device() || lengths.dim() != 2 || !lengths.is_contiguous() || lengths.size(0) != table.size(0) ||
+            lengths.size(1) != table.size(1)) return false;
+        x.batch = table.size(0) * table.size(1);
+    } else {
+        if (table.dim() != 2 || table.size(1) < 1 || table.stride(1) != 1 || !int32_vector(lengths, k, table.size(0))) return false;
+        x.batch = table.size(0);
+    }
+    const int64_t width = table.size(table.dim() - 1);
+    x.cap = width * k.size(2);
     if (max_k != Py_None) {
         const int64_t most = PyLong_AsLongLong(max_k);
         if (PyErr_Occurred()) PyErr_Clear();
@@ -1187,12 +1196,12 @@ bool cache_of(Cache& x, const Tensor& k, const Tensor& v, const Tensor& table, c
     c.bits = four ? 4 : 16;
     c.page_size = static_cast<int32_t>(k.size(2));
     c.kv_heads = static_cast<int32_t>(k.size(1));
-    c.table_width = static_cast<int32_t>(table.size(1));
+    c.table_width = static_cast<int32_t>(width);
     c.pages = k.size(0);
     set3(c.k_strides, k);
     set3(c.v_strides, v);
     c.block_table = table.data_ptr<int32_t>();
-    c.table_stride = table.stride(0);
+    c.table_stride = own ? width : table.stride(0);
     c.lengths = lengths.data_ptr<int32_t>();
     c.max_keys = static_cast<int32_t>(x.cap);
     return true;
@@ -1398,18 +1407,8 @@ PyObject* py_sdpa_paged_chosen(PyObject*, PyObject* const* args, Py_ssize_t n) {
     c10::optional<double> scale;
     if (n != 7 || !callable_now() || !(q = tensor_of(args[0])) || !(k = tensor_of(args[1])) || !(v = tensor_of(args[2])) || !(table = tensor_of(args[3])) ||
         !(keys = tensor_of(args[4])) || !scale_of(args[5], scale)) Py_RETURN_NONE;
-    if (!plain(*table) || table->scalar_type() != at::kInt || table->dim() != 3 || !table->is_contiguous() || table->numel() == 0 || !plain(*keys) ||
-        keys->scalar_type() != at::kInt || keys->dim() != 2 || !keys->is_contiguous() || keys->size(0) != table->size(0) || keys->size(1) != table->size(1)) Py_RETURN_NONE;
-    if (k->dim() != 4 || k->size(1) != table->size(1) || table->size(0) > INT32_MAX / table->size(1)) Py_RETURN_NONE;
-    // As a cache of one sequence for each token and head, whose checks are the same.
-    Tensor rows_table, rows_keys;
-    {
-        at::AutoDispatchBelowADInplaceOrView guard;
-        rows_table = table->view({-1, table->size(2)});
-        rows_keys = keys->view({-1});
-    }
     Cache x;
-    if (!cache_of(x, *k, *v, rows_table, rows_keys, args[6])) Py_RETURN_NONE;
+    if (!cache_of(x, *k, *v, *table, *keys, args[6], true)) Py_RETURN_NONE;
     const bool packed = q->dim() == 3;
     if ((!packed && q->dim() != 4) || q->numel() == 0) Py_RETURN_NONE;
     const int64_t rows = packed ? q->size(0) : q->size(2), batch = packed ? 1 : q->size(0);
