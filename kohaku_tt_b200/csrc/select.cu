@@ -5,11 +5,12 @@
 // so the scores of all pages are two matrix products with the queries of a K / V head's group as columns. Bound: the reading of the
 // bounds, 4 D bytes a page and head (1 / P of the cache in bf16, for pages of P keys).
 //
-// What is selected is decided by the exact scores, so that it does not depend on an order of summation. The products of bf16 values are exact in
-// fp32; a score is the sum of four sums of up to 4 matrix instructions each, of which every one is off by 2^-22 of the magnitudes that it adds
-// up at most (two bits more than a sum of fp32 rounds by), all in all by e = 2^-19 max_h sum_d |q_hd| max |bound|. So the value of the
-// last page selected lies within e of the last by fp32: pages more than 2 e above or below are in or out, and those between, one or a few, get their
-// scores in 64 bits where they are not all in. (2 to 5 in 100 selections among 1,024 pages.)
+// What is selected is decided by the exact scores, so that it does not depend on an order of summation. The products of bf16 values are exact
+// in fp32; a score is the sum of four sums of up to 4 matrix instructions each, of which every one is off by 2^-22 of the magnitudes that it
+// adds up at most (two bits more than a sum of fp32 rounds by), all in all by e = 2^-19 max_h sum_d |q_hd| max |bound| (measured, over equal,
+// alternating and wide-ranging values: 2^-22 of it). So the value of the last page selected lies within e of the last by fp32: pages more than
+// 2 e above or below are in or out, and those between, one or a few, get their scores in 64 bits where they are not all in. Bounds whose
+// least value is above the largest select some pages or others, of those there are.
 #include <type_traits>
 
 #include "four_bits.cuh"
@@ -41,8 +42,9 @@ struct BoundsParams {
 
 constexpr int kLotOfTokens = 16;   // packed rows that a warp looks for pages in
 
-// A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, 16 or 8 rows requested before the first is used.
-// Packed rows: a warp looks at 16 of them and has the pages that begin among them, or in which a sequence's rows begin.
+// A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, 16 or 8 rows requested before the first is used
+// (8: 37 us where it is 31). Packed rows: a warp looks at 16 of them and has the pages that begin among them, or in which a sequence's rows
+// begin. Bound: the reading of the keys: 16 x up to 8,192 of 8 heads, D 128, pages of 32, 212 MB: 31.6 us, 6.7 TB/s.
 template <int D, int kBits, bool kPacked>
 __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ BoundsParams p) {
     constexpr int kChunks = D / 8, kStep = 32 / kChunks;
@@ -401,7 +403,8 @@ __device__ __forceinline__ double exact_score(const SelectParams& p, const Token
 //
 // Selection: the value of the k-th largest score, by counts in bins of equal width, of which the one that has it is cut again while it holds many,
 // and by rank among those of the last. A thread has kItems neighbouring pages in registers (0: reads them each time), and a sum over the
-// CTA places those that are in. (32 thresholds, one to a lane whose warp goes through its share of the scores, were 1,700 clocks a round of 1,024
+// CTA places those that are in: 64 x up to 16,384 keys, 16 heads over 2, D 128, pages of 16, 14.1 us, of which the reading of some 50 MB
+// is 8; 1 x 65,536, 32 over 8, pages of 64, 6.1, most of it waits one after another. (32 thresholds, one to a lane whose warp goes through its share of the scores, were 1,700 clocks a round of 1,024
 // scores, four at a time, each by a sum over the CTA, 950 and five rounds.) kNear: scores, names and exact scores lie in shared memory,
 // else scores and exact ones in the workspace.
 template <int D, int kItems, bool kNear>
@@ -418,6 +421,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t4 = lane & 3;
     if (tid == 0) sm.found = sm.count = 0;
     for (int i = tid; i < kBins; i += threads) sm.bins[i] = 0;
+    if (p.ranks > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");   // (met before the first store to another CTA)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t pair = p.by_ranks(blockIdx.x), local = p.by_heads(pair);
@@ -513,6 +517,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
         __nv_bfloat162 largest[2], least[2];
         largest[0] = largest[1] = least[0] = least[1] = __float2bfloat162_rn(0.f);
         float lo = INFINITY, hi = -INFINITY;
+        if (p.ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
         for (int block = 0; block < blocks; ++block) {
             // Two ahead. Names of a pair of blocks are those of the next two once their own are on their way.
             if (block & 1) {
@@ -626,7 +631,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_con
     float lo = from_ordered(__reduce_min_sync(0xffffffffu, slot ? sm.of_warp[1][lane] : 0x7fffffff)), hi = from_ordered(__reduce_max_sync(0xffffffffu, slot ? sm.of_warp[2][lane] : static_cast<int>(0x80000000)));
     // What the fp32 scores may be off by. (What the products could lose below fp32's least normal number is in the last terms.)
     const float off = fmaf(mass, 0x1p-19f, fmaf(norm + most, 0x1p-110f, 0x1p-110f));
-    const bool sure = mass < 0x1p120f;   // else, and where it is no number: all in 64 bits
+    // Else, and where it is no number, all in 64 bits. (Scores past it are of bounds whose least value is above the largest.)
+    const bool sure = mass < 0x1p120f && lo > -0x1p121f && hi < 0x1p121f;
     // This thread's pages and their scores, and (kItems) pages that are not asked about, whose scores are below all: f(page, score, bin).
     auto each = [&](auto f) {
         if constexpr (kItems > 0) {
@@ -908,15 +914,17 @@ int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t 
     for (int64_t t0 = 0; t0 < plan.tokens; t0 += plan.slice) {
         const int64_t n = plan.tokens - t0 < plan.slice ? plan.tokens - t0 : plan.slice, pairs = n * p.kv_heads;
         p.token0 = t0;
-        // Two CTAs to an SM: as many to a pair as there is room for and blocks for all their warps.
+        // Two CTAs to an SM: as many to a pair as there is room for and blocks for all their warps. Measured with half, twice and four times the
+        // CTAs, us: 64 x 16,384 keys, 16 heads over 2, D 128, pages of 16: 21.7, 16.1 as it is, 18.8, 25.7; 8 x 5 tokens over 8,192, 14 over 2, D 64,
+        // pages of 16: 10.0, 9.7, 9.5, 9.5.
         p.ranks = 1;
         while (p.ranks < kMaxRanks && pairs * p.ranks * 2 <= 2 * 148 && p.ranks * kWarps < plan.blocks) p.ranks *= 2;
         p.by_ranks = Divisor(p.ranks);
         int rc;
         if (!plan.near) rc = launch_select<D, 0, false>(p, pairs, stream);
         else if (width <= 8 * 32 * kWarps) rc = launch_select<D, 8, true>(p, pairs, stream);
-        else if (width <= 32 * 32 * kWarps) rc = launch_select<D, 32, true>(p, pairs, stream);
-        else rc = launch_select<D, 64, true>(p, pairs, stream);
+        else if (D == 64 || width <= 32 * 32 * kWarps) rc = launch_select<D, 32, true>(p, pairs, stream);
+        else rc = launch_select<D, D == 64 ? 32 : 64, true>(p, pairs, stream);
         if (rc) return rc;
     }
     return 0;

@@ -121,7 +121,8 @@ def paged_select(q, bounds, block_table, lengths, page_size, top, first=1, last=
     largest logit that a key between its bounds (paged_bounds) could have with any query of the head's group,
         max over h of the sum over d of max(q[h, d] least[d], q[h, d] largest[d]),
     and the exact value decides; ties go to the page that comes first. A score that is no number counts as infinite; an entry of
-    block_table that names no page has score 0.
+    block_table that names no page has score 0. (Where a least value is above the largest, as in a tensor that nothing was written to,
+    it is not said which pages.)
     chosen int32 [tokens, Hk, top]: names of pages in the order of their places, -1 behind them. keys int32 [tokens, Hk]: the keys of
     those that the token sees (0: it sees none). Packed rows of no sequence see none. H is a multiple of Hk, D 64 or 128. No gradients."""
     if torch.compiler.is_compiling():

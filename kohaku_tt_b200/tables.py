@@ -80,8 +80,9 @@ def paged_reserve(block_table, lengths, added, free, count, page_size, tokens, c
     and without a trip to the host: (cu_seq, positions, slots, granted).
 
     block_table int32 [B, W] is written in place: entries ceil(lengths / page_size) .. of each row that the new tokens reach. free
-    int32 [pool], with a place for each of the pool's pages 0 .. pool - 1, count int32 [1]: free[:count] are those that no sequence has. They are taken from the end, sequence by
-    sequence; neither is changed, count_out (int32 [1], another buffer) receives how many are left. lengths are not changed either.
+    int32 [pool], with a place for each of the pool's pages 0 .. pool - 1, count int32 [1]: free[:count] are those that no sequence
+    has. They are taken from the end, sequence by sequence; neither is changed, count_out (int32 [1], another buffer) receives how
+    many are left. lengths are not changed either.
     granted int32 [B]: added[b], or 0 for the first sequence that the list, or its row of the table, has no room for and for all
     behind it; their new entries become -1 (an append there goes nowhere), and they can be asked for again later.
     The new tokens are packed, row i of sequence b at cu_seq[b] + i, as paged_append and sdpa_paged take them: cu_seq int32 [B + 1];

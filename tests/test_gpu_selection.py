@@ -236,7 +236,7 @@ def test_scores_that_do_not_fit_shared_memory(cuda):
 
 def test_many_tokens_in_several_launches(cuda):
     """More scores than are kept at a time: tokens of a later launch are as those of the first."""
-    d, h, hk, page, wide, top, t = 64, 32, 32, 16, 4096, 5, 30
+    d, h, hk, page, wide, top, t = 64, 32, 32, 16, 9000, 5, 80
     x = _x(wide, hk, 2, d, seed=1).float().sort(dim=2).values.to(torch.bfloat16).to(cuda)
     table = torch.arange(wide, dtype=torch.int32, device=cuda).expand(t, wide).contiguous()
     q = _x(1, h, 1, d, seed=2).to(cuda).expand(t, h, 1, d).contiguous()
@@ -244,6 +244,54 @@ def test_many_tokens_in_several_launches(cuda):
     got, keys = ktt.paged_select(q, x, table, lens, page, top)
     one, _ = ktt.paged_select(q[:1], x, table[:1], lens[:1], page, top)
     assert torch.equal(got, one.expand_as(got)) and bool((keys == top * page).all())
+
+
+@pytest.mark.parametrize("d,wide", [(64, 1024), (64, 1025), (64, 4096), (64, 4097), (128, 1025), (128, 4096), (128, 4100), (128, 8192), (128, 8193)])
+def test_widths(cuda, d, wide):
+    """Tables about as wide as each way of holding the scores has room for: far apart, two thirds alike, all alike."""
+    page, top, h, hk = 16, 70, 4, 1
+    table = _table([wide], wide, wide, seed=2)
+    q = _x(2, h, d, seed=3)
+    x = _x(wide, hk, 2, d, seed=1).float().sort(dim=2).values.to(torch.bfloat16)
+    alike = x[:1].expand(wide, hk, 2, d).clone()
+    most = torch.where(torch.arange(wide).remainder(3)[:, None, None, None] == 0, x, alike)
+    for bounds in (x, most, alike):
+        for lengths in ([wide * page], [wide * page - 17 * page - 3]):
+            _selected(cuda, q, bounds, table, lengths, [2], page, top, 2, 3, False)
+
+
+def test_tensors_that_are_no_bounds(cuda):
+    """Values of any kind, in no order: pages of the table, each once, in its order, the first and the last among them."""
+    page, top, h, hk = 16, 40, 8, 2
+    for d, wide in ((64, 300), (128, 2000), (64, 5000)):
+        g = torch.Generator().manual_seed(wide)
+        table = _table([wide], wide, wide, seed=2)
+        place = torch.empty(wide, dtype=torch.long)
+        place[table[0].long()] = torch.arange(wide)
+        for kind in range(4):
+            x = torch.randint(-2 ** 15, 2 ** 15, (wide, hk, 2, d), generator=g, dtype=torch.int16).view(torch.bfloat16)
+            if kind == 1:       # large ones the wrong way round
+                x = torch.stack([torch.full((wide, hk, d), 3e38), torch.full((wide, hk, d), -3e38)], dim=2).to(torch.bfloat16)
+            if kind == 2:
+                x = _x(wide, hk, 2, d, seed=4).float().sort(dim=2, descending=True).values.to(torch.bfloat16)
+            if kind == 3:       # some of them the wrong way round
+                x[::7] = torch.tensor([3e38, -3e38], dtype=torch.bfloat16)[None, None, :, None]
+                x[1::7], x[2::7] = 1.0, float("-inf")
+            chosen, keys = ktt.paged_select(_x(1, h, 1, d, seed=3).to(cuda), x.to(cuda), table.to(cuda), _i32([wide * page], cuda), page, top)
+            assert bool((keys == top * page).all())
+            for row in chosen.cpu()[0]:
+                at = place[row.long()]
+                assert bool((at[1:] > at[:-1]).all()) and at[0] == 0 and at[-1] == wide - 1
+
+
+def test_no_tokens(cuda, path):
+    d, h, hk, page = 64, 4, 2, 16
+    kp = _x(4, hk, page, d, seed=1).to(cuda)
+    bounds, table, lens = torch.zeros((4, hk, 2, d), dtype=torch.bfloat16, device=cuda), _table([2, 2], 2, 4).to(cuda), _i32([20, 0], cuda)
+    for q, kw in ((_x(0, h, d).to(cuda), dict(cu_seq_q=_i32([0, 0, 0], cuda))), (_x(2, h, 0, d).to(cuda), {})):
+        chosen, keys = ktt.paged_select(q, bounds, table, lens, page, 3, **kw)
+        assert chosen.shape == (0, hk, 3) and keys.shape == (0, hk)
+        assert ktt.sdpa_paged(q, kp, kp, chosen, keys).shape == q.shape
 
 
 def test_layouts(cuda, path):
