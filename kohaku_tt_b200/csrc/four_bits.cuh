@@ -45,5 +45,7 @@ struct Edges {
 int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, cudaStream_t stream);
 // Bounds from an argument block's fields after their checks; null, or why not.
 const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3]);
+// Those that are written, of a cache of head dim d.
+const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3], const Pages& c, int kv_heads, int d);
 
 }  // namespace ktt

@@ -654,7 +654,7 @@ extern "C" int ktt_b200_paged_append_at(const ktt_b200_append_at_args* x, void* 
     }
     Bounds bounds = {};
     if (x->bounds) {
-        if (const char* why = bounds_of(bounds, x->bounds, x->bounds_strides)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: %s", why);
+        if (const char* why = bounds_of(bounds, x->bounds, x->bounds_strides, p.c, p.kv_heads, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: %s", why);
         if (a->batch > 65535) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: at most 65535 sequences with bounds");
     }
     // One new key of each sequence goes into its page's bounds as it passes; of several, those of a page meet in a launch behind this one, which
@@ -665,7 +665,6 @@ extern "C" int ktt_b200_paged_append_at(const ktt_b200_append_at_args* x, void* 
     if (int rc = launch(p, a->cache.bits, a->d, st)) return rc;
     return bounds.at && !passing ? keep_bounds(p.c, a->cache.bits, a->d, p.kv_heads, bounds, a->batch, a->rows, a->cu_seqlens, st) : 0;
 }
-
 
 extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_read: null arguments");

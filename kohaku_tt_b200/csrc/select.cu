@@ -26,6 +26,11 @@ const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3]) {
     }
     return reinterpret_cast<uintptr_t>(at) & 15 ? "bounds must be 16-byte aligned" : nullptr;
 }
+const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3], const Pages& c, int kv_heads, int d) {
+    auto apart = [d](int64_t stride) { return stride >= d || stride <= -d; };
+    if ((c.pages > 1 && !apart(strides[0])) || (kv_heads > 1 && !apart(strides[1])) || !apart(strides[2])) return "bounds that are written must not lie on one another";
+    return bounds_of(b, at, strides);
+}
 
 namespace {
 
@@ -955,7 +960,7 @@ extern "C" int ktt_b200_paged_bounds(const ktt_b200_bounds_args* a, void* stream
     if (a->batch < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_bounds: sizes must be positive");
     if (a->batch > 65535) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: at most 65535 sequences");
     if (!a->cache.k || !a->cache.block_table || !a->cache.lengths || !a->bounds) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_bounds: null pointer");
-    if (const char* why = bounds_of(p.bounds, a->bounds, a->bounds_strides)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: %s", why);
+    if (const char* why = bounds_of(p.bounds, a->bounds, a->bounds_strides, p.c, a->cache.kv_heads, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: %s", why);
     p.batch = a->batch;
     p.kv_heads = a->cache.kv_heads;
     p.since = a->since;

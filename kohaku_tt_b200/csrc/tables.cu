@@ -239,7 +239,7 @@ __global__ void __cluster_dims__(kReleaseCtas, 1, 1) __launch_bounds__(kReleaseT
     __syncthreads();
     const int all = entries_s[batch], each = (all + kReleaseCtas * kReleaseThreads - 1) / (kReleaseCtas * kReleaseThreads);
     const int64_t from = (static_cast<int64_t>(blockIdx.x) * kReleaseThreads + threadIdx.x) * each;
-    const int n0 = static_cast<int>(from < all ? from : all), n1 = min(n0 + each, all);
+    const int n0 = static_cast<int>(from < all ? from : all), n1 = all - n0 < each ? all : n0 + each;
     auto visit = [&](auto use) {   // this thread's entries
         if (n0 >= n1) return;
         int b = holder_of(entries_s, 0, batch - 1, n0), end, entry = first_free(b, end) + n0 - entries_s[b];
@@ -280,6 +280,7 @@ const char* tables_refusal(const ktt_b200_tables& a) {
     if (a.page_size < 16 || a.page_size % 16) return "the page size must be a multiple of 16";
     if (a.batch > kMaxSequences) return "at most 4096 sequences";
     if (static_cast<int64_t>(a.table_width) * a.page_size > (1 << 30)) return "at most 2^30 keys per sequence";
+    if (a.batch > 1 && a.table_stride < a.table_width && -a.table_stride < a.table_width) return "rows of the table must not lie on one another";
     if (static_cast<int64_t>(a.batch) * a.table_width >= (1ll << 31) || a.pool >= (1ll << 31)) return "fewer than 2^31 table entries and pages";
     return nullptr;
 }

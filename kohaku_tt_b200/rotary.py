@@ -286,7 +286,8 @@ def rotary(q, k, cos, sin, positions=None, interleaved=False, axes=None):
         out = eager.rotary(q, k, cos, sin, positions, interleaved, axes)
         if out is not None:
             return out
-    axes = pair_axes(axes, cos.shape[-1], "rotary")
+    if axes is not None:
+        axes = pair_axes(axes, cos.shape[-1], "rotary")
     _check(q, k, cos, sin, positions, axes)
     if torch.compiler.is_compiling():
         if axes is None:

@@ -400,6 +400,12 @@ def test_refusals(cuda, path):
     for bad in (dict(bounds=bounds.float()), dict(bounds=bounds[:3]), dict(bounds=bounds, since=n.long()), dict(bounds=bounds, since=_i32([1, 2], cuda))):
         with pytest.raises(ValueError):
             ktt.paged_bounds(kp, table, n, **bad)
+    row = torch.zeros((1, 2, 1, d), dtype=torch.bfloat16, device=cuda)
+    for bad in (bounds[:1].expand(4, 2, 2, d), bounds[:, :1].expand(4, 2, 2, d), bounds[:, :, :1].expand(4, 2, 2, d)):      # that lie on one another
+        with pytest.raises(_lib.UnsupportedAttention):
+            ktt.paged_bounds(kp, table, n, bounds=bad)
+        with pytest.raises(_lib.UnsupportedAttention):
+            ktt.paged_append(row, row, kp, kp, table, n, bounds=bad)
     chosen, keys = torch.zeros((1, 2, 3), dtype=torch.int32, device=cuda), torch.zeros((1, 2), dtype=torch.int32, device=cuda)
     for bad in ((q, kp, kp, chosen.long(), keys), (q, kp, kp, chosen, keys.long()), (q, kp, kp, chosen, keys[0]), (q, kp, kp, chosen[:, :1], keys[:, :1]),
                 (torch.cat([q, q]), kp, kp, chosen, keys), (q[0, 0], kp, kp, chosen, keys)):

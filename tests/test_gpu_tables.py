@@ -132,7 +132,8 @@ def test_refusals(cuda, path):
     for bad, error in (((t.long(), n, n, f, c, 16, 1, o), ValueError), ((t, n.long(), n, f, c, 16, 1, o), ValueError), ((t, n, _i32([0, 0], cuda), f, c, 16, 1, o), ValueError),
                        ((t, n, n, f.long(), c, 16, 1, o), ValueError), ((t, n, n, f, f, 16, 1, o), ValueError), ((t, n, n, f, c, 16, 1, c), ValueError),
                        ((t, n, n, f, c, 16, -1, o), ValueError), ((t, n, n, f, c, 20, 1, o), _lib.UnsupportedAttention), ((t, n, n, f[::2], c, 16, 1, o), None),
-                       ((t.t(), n, n, f, c, 16, 1, o), ValueError), ((t, n, n, f.cpu(), c, 16, 1, o), (RuntimeError, ValueError))):
+                       ((t.t(), n, n, f, c, 16, 1, o), ValueError), ((t.expand(2, 2), *[_i32([0, 0], cuda)] * 2, f, c, 16, 1, o), _lib.UnsupportedAttention),
+                       ((t, n, n, f.cpu(), c, 16, 1, o), (RuntimeError, ValueError))):
         if error is None:      # (one element: contiguous whatever its stride)
             ktt.paged_reserve(*bad)
             continue

@@ -38,7 +38,8 @@ def _tables(**kw):
 @pytest.mark.parametrize("kw,status,text", [
     (dict(batch=0), _lib.ERR_UNSUPPORTED, "positive"), (dict(table_width=0), _lib.ERR_UNSUPPORTED, "positive"), (dict(page_size=24), _lib.ERR_UNSUPPORTED, "multiple of 16"),
     (dict(page_size=0), _lib.ERR_UNSUPPORTED, "multiple of 16"), (dict(batch=4097), _lib.ERR_UNSUPPORTED, "4096"), (dict(table_width=1 << 27), _lib.ERR_UNSUPPORTED, "2^30"),
-    (dict(pool=1 << 31), _lib.ERR_UNSUPPORTED, "2^31"), (dict(pool=-1), _lib.ERR_UNSUPPORTED, "positive"), (dict(count=None), _lib.ERR_BAD_ARGUMENT, "null"),
+    (dict(table_stride=3), _lib.ERR_UNSUPPORTED, "on one another"), (dict(table_stride=0), _lib.ERR_UNSUPPORTED, "on one another"),
+    (dict(table_stride=-3), _lib.ERR_UNSUPPORTED, "on one another"), (dict(pool=1 << 31), _lib.ERR_UNSUPPORTED, "2^31"), (dict(pool=-1), _lib.ERR_UNSUPPORTED, "positive"), (dict(count=None), _lib.ERR_BAD_ARGUMENT, "null"),
     (dict(count_out=4096), _lib.ERR_BAD_ARGUMENT, "another word"), (dict(free_pages=None), _lib.ERR_BAD_ARGUMENT, "null"), (dict(block_table=None), _lib.ERR_BAD_ARGUMENT, "null")])
 def test_tables_that_no_entry_takes(built_lib, kw, status, text):
     assert built_lib.ktt_b200_paged_reserve(ctypes.byref(_tables(**kw)), 4096, 3, None, None, None, None, None) == status
@@ -107,7 +108,8 @@ def test_bounds_refusals(built_lib):
             setattr(a, name, x)
         return a
 
-    for a, status in ((args(bounds=4104), _lib.ERR_UNSUPPORTED), (args(strides=(512, 256, 100)), _lib.ERR_UNSUPPORTED), (args(d=96), _lib.ERR_UNSUPPORTED),
+    for a, status in ((args(bounds=4104), _lib.ERR_UNSUPPORTED), (args(strides=(512, 256, 100)), _lib.ERR_UNSUPPORTED),
+                      (args(strides=(0, 256, 128)), _lib.ERR_UNSUPPORTED), (args(strides=(512, 64, 128)), _lib.ERR_UNSUPPORTED), (args(strides=(512, 256, 0)), _lib.ERR_UNSUPPORTED), (args(d=96), _lib.ERR_UNSUPPORTED),
                       (args(batch=65536), _lib.ERR_UNSUPPORTED), (args(batch=0), _lib.ERR_BAD_ARGUMENT), (args(bounds=None), _lib.ERR_BAD_ARGUMENT)):
         assert built_lib.ktt_b200_paged_bounds(ctypes.byref(a), None) == status
     assert built_lib.ktt_b200_paged_bounds(None, None) == _lib.ERR_BAD_ARGUMENT
