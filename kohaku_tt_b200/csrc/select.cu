@@ -47,9 +47,10 @@ struct BoundsParams {
 
 constexpr int kLotOfTokens = 16;   // packed rows that a warp looks for pages in
 
-// A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, 16 or 8 rows requested before the first is used
+// A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, 16 rows requested before the first is used
 // (8: 37 us where it is 31). Packed rows: a warp looks at 16 of them and has the pages that begin among them, or in which a sequence's rows
-// begin. Bound: the reading of the keys: 16 x up to 8,192 of 8 heads, D 128, pages of 32, 212 MB: 31.6 us, 6.7 TB/s.
+// begin. Bound: bf16, the reading of the keys: 16 x up to 8,192 of 8 heads, D 128, pages of 32, 212 MB: 31.6 us, 6.7 TB/s. 4 bits, the
+// instructions that make values of codes, 16 for eight, and those that find a row's words: 26 us (38 with an address for each row).
 template <int D, int kBits, bool kPacked>
 __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ BoundsParams p) {
     constexpr int kChunks = D / 8, kStep = 32 / kChunks;
@@ -77,36 +78,53 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
             old.lo.load(p.bounds.edge(page, head, 0) + chunk * 8);
             old.hi.load(p.bounds.edge(page, head, 1) + chunk * 8);
         }
-        auto rows = [&](auto ahead, int r0) {
-            constexpr int kAhead = decltype(ahead)::value;
-            if constexpr (kBits == 16) {
+        if constexpr (kBits == 16) {
+            auto rows = [&](auto ahead, int r0) {
+                constexpr int kAhead = decltype(ahead)::value;
                 Eight<__nv_bfloat16> x[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) {
-                    const int r = r0 + i * kStep < end ? r0 + i * kStep : r0;   // (a row twice changes nothing)
+                    const int r = min(r0 + lane / kChunks + i * kStep, end - 1);   // (a row twice changes nothing)
                     x[i].load(reinterpret_cast<const __nv_bfloat16*>(from + r * p.c.ks[2]) + chunk * 8);
                 }
 #pragma unroll
                 for (int i = 0; i < kAhead; ++i) e.with(x[i], x[i]);
-            } else {
-                uint2 x[kAhead];
+            };
+            int r0 = begin;
+            for (; r0 + 8 * kStep < end; r0 += 16 * kStep) rows(std::integral_constant<int, 16>(), r0);
+            if (r0 < end) rows(std::integral_constant<int, 8>(), r0);
+        } else {
+            // Blocks of 16 rows, whose words lie at fixed places; of blocks that are not all there, a row that is not is the nearest that is.
+            constexpr int kRows = 16 / kStep, kLot = D == 128 ? 2 : 4;
+            auto rows = [&](auto blocks, int r0) {
+                constexpr int kBlocks = decltype(blocks)::value;
+                uint2 x[kBlocks * kRows];
+                if (r0 >= begin && r0 + 16 * kBlocks <= end) {
+                    const uint32_t* block = reinterpret_cast<const uint32_t*>(from + static_cast<int64_t>(r0 >> 4) * (9 * D));
+                    const uint32_t *word = block + key_word<D>(lane / kChunks, chunk), *step = block + step_word<D>(lane / kChunks, chunk / 8);
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    const int r = r0 + i * kStep < end ? r0 + i * kStep : r0;
-                    const uint32_t* block = reinterpret_cast<const uint32_t*>(from + static_cast<int64_t>(r >> 4) * (9 * D));
-                    x[i] = make_uint2(block[key_word<D>(r & 15, chunk)], block[step_word<D>(r & 15, chunk / 8)]);
+                    for (int i = 0; i < kBlocks * kRows; ++i) {
+                        const int at = i / kRows * (9 * D / 4), row = i % kRows * kStep;
+                        x[i] = make_uint2(word[at + row * (D / 8)], step[at + row * (D / 64)]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kBlocks * kRows; ++i) {
+                        const int r = min(max(r0 + lane / kChunks + i * kStep, begin), end - 1);
+                        const uint32_t* block = reinterpret_cast<const uint32_t*>(from + static_cast<int64_t>(r >> 4) * (9 * D));
+                        x[i] = make_uint2(block[key_word<D>(r & 15, chunk)], block[step_word<D>(r & 15, chunk / 8)]);
+                    }
                 }
 #pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
+                for (int i = 0; i < kBlocks * kRows; ++i) {
                     const Eight<__nv_bfloat16> y = of_four_bits(x[i].x, x[i].y);
                     e.with(y, y);
                 }
-            }
-        };
-        // (Whole lots while there are any, then as many as are left.)
-        int r0 = begin + lane / kChunks;
-        for (; r0 + 15 * kStep < end; r0 += 16 * kStep) rows(std::integral_constant<int, 16>(), r0);
-        for (; r0 < end; r0 += 8 * kStep) rows(std::integral_constant<int, 8>(), r0);
+            };
+            int r0 = begin & ~15;
+            for (; r0 + 16 < end; r0 += 16 * kLot) rows(std::integral_constant<int, kLot>(), r0);
+            if (r0 < end) rows(std::integral_constant<int, 1>(), r0);
+        }
 #pragma unroll
         for (int off = kChunks; off < 32; off <<= 1) {
             Edges other;
@@ -133,12 +151,13 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
         int keys = 0;
         if (p.batch < 32) {   // a lane looks at a sequence, its length with it, in one trip
             const int offset = p.cu[min(lane, p.batch)], have = cached_keys(p.c, min(lane, p.batch - 1));
+            // (The last that starts at or before the token, -1: none; five looks at another lane's.)
 #pragma unroll
-            for (int i = 0; i < kLotOfTokens; ++i) {   // (the last that starts at or before the token)
-                const uint32_t before = __ballot_sync(0xffffffffu, lane <= p.batch && offset <= lot * kLotOfTokens + i);
-                if (i == lane) b = 31 - __clz(before);
+            for (int step = 16; step > 0; step >>= 1) {
+                const int start_of = __shfl_sync(0xffffffffu, offset, min(b + step, 31));
+                if (b + step <= p.batch && start_of <= n) b += step;
             }
-            if (!mine || b < 0 || b >= p.batch) b = -1;
+            if (!mine || b >= p.batch) b = -1;
             start = __shfl_sync(0xffffffffu, offset, max(b, 0));
             behind = __shfl_sync(0xffffffffu, offset, max(b, 0) + 1);
             keys = __shfl_sync(0xffffffffu, have, max(b, 0));
@@ -150,7 +169,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
                 keys = cached_keys(p.c, b);
             }
         }
-        if (b >= 0 && n >= start) {   // (offsets that decrease)
+        if (b >= 0 && n >= start && n < behind) {   // (offsets that decrease)
             const int64_t in = n - start, at = keys + in, all = at + (behind - n);
             end = static_cast<int>(all < p.c.cap ? all : p.c.cap);
             leads = at < end && (in == 0 || static_cast<uint32_t>(at) % static_cast<uint32_t>(page_size) == 0);   // (at < end: 2^30 at most)
