@@ -421,16 +421,18 @@ __device__ __forceinline__ double exact_score(const SelectParams& p, const Token
 
 // A cluster of `ranks` CTAs has a (token, K / V head): all of their warps score its pages, the first selects.
 //
-// Scores: a warp takes neighbouring blocks of 16 pages through a ring of its own, two or three on their way while one is multiplied: pages are the
-// rows of m16n8k16, q+ and q- of 8 heads its columns. (Bounds in registers as they come, two blocks to a warp, were no faster than one after the
-// other: 16 us for 38 MB.) The products of a block are four sums, for the latency of one.
+// Scores: the blocks of 16 pages are dealt to the warps in turn, each of which takes them through a ring of its own, two or three on their way while
+// one is multiplied: pages are the rows of m16n8k16, q+ and q- of 8 heads its columns. (Bounds in registers as they come, two blocks to a warp, were
+// no faster than one after the other: 16 us for 38 MB.) The products of a block are four sums, for the latency of one.
 //
 // Selection: the value of the k-th largest score, by counts in bins of equal width, of which the one that has it is cut again while it holds many,
-// and by rank among those of the last. A thread has kItems neighbouring pages in registers (0: reads them each time), and a sum over the
-// CTA places those that are in: 64 x up to 16,384 keys, 16 heads over 2, D 128, pages of 16, 14.1 us, of which the reading of some 50 MB
-// is 8; 1 x 65,536, 32 over 8, pages of 64, 6.1, most of it waits one after another. (32 thresholds, one to a lane whose warp goes through its share of the scores, were 1,700 clocks a round of 1,024
-// scores, four at a time, each by a sum over the CTA, 950 and five rounds.) kNear: scores, names and exact scores lie in shared memory,
-// else scores and exact ones in the workspace.
+// and by rank among those of the last. A thread has kItems neighbouring pages in registers (0: reads them each time), and a sum over the CTA
+// places those that are in. (32 thresholds, one to a lane whose warp goes through its share of the scores, were 1,700 clocks a round of 1,024
+// scores; four at a time, each by a sum over the CTA, 950 and five rounds.) kNear: scores, names and exact scores lie in shared memory, else
+// scores and exact ones in the workspace.
+//
+// Measured: 64 x up to 16,384 keys, 16 heads over 2, D 128, pages of 16, 14.1 us, of which the reading of 40 MB is 6; 1 x up to 65,536, 32 over 8,
+// pages of 64, 6.1, waits that follow one another.
 template <int D, int kItems, bool kNear>
 __global__ void __launch_bounds__(32 * kWarps, 2) select_kernel(const __grid_constant__ SelectParams p) {
     using R = Ring<D>;
@@ -939,14 +941,19 @@ int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t 
         const int64_t n = plan.tokens - t0 < plan.slice ? plan.tokens - t0 : plan.slice, pairs = n * p.kv_heads;
         p.token0 = t0;
         // Two CTAs to an SM: as many to a pair as there is room for and blocks for all their warps. Measured with half, twice and four times the
-        // CTAs, us: 64 x 16,384 keys, 16 heads over 2, D 128, pages of 16: 21.7, 16.1 as it is, 18.8, 25.7; 8 x 5 tokens over 8,192, 14 over 2, D 64,
+        // CTAs, us: 64 x up to 16,384 keys, 16 heads over 2, D 128, pages of 16: 21.7, 16.1 as it is, 18.8, 25.7; 24 tokens over up to 8,192, 14 over 2, D 64,
         // pages of 16: 10.0, 9.7, 9.5, 9.5.
         p.ranks = 1;
         while (p.ranks < kMaxRanks && pairs * p.ranks * 2 <= 2 * 148 && p.ranks * kWarps < plan.blocks) p.ranks *= 2;
         p.by_ranks = Divisor(p.ranks);
+        // As few scores to a thread as the table's width asks for. us for one kind and the next, 16 heads over 2 or the like: 512 pages 6.0 (4 scores) and
+        // 6.4 (8); 1,024 9.6 and 12.0 (8 and 32); 2,048 10.2 and 11.6 (16 and 32); 3,184 15.4 and 18.5 (32 and 64); 8,192 21.5, read each time
+        // 31.2, in the workspace 57.
         int rc;
         if (!plan.near) rc = launch_select<D, 0, false>(p, pairs, stream);
+        else if (width <= 4 * 32 * kWarps) rc = launch_select<D, 4, true>(p, pairs, stream);
         else if (width <= 8 * 32 * kWarps) rc = launch_select<D, 8, true>(p, pairs, stream);
+        else if (width <= 16 * 32 * kWarps) rc = launch_select<D, 16, true>(p, pairs, stream);
         else if (D == 64 || width <= 32 * 32 * kWarps) rc = launch_select<D, 32, true>(p, pairs, stream);
         else rc = launch_select<D, D == 64 ? 32 : 64, true>(p, pairs, stream);
         if (rc) return rc;

@@ -246,7 +246,7 @@ def test_many_tokens_in_several_launches(cuda):
     assert torch.equal(got, one.expand_as(got)) and bool((keys == top * page).all())
 
 
-@pytest.mark.parametrize("d,wide", [(64, 1024), (64, 1025), (64, 4096), (64, 4097), (128, 1025), (128, 4096), (128, 4100), (128, 8192), (128, 8193)])
+@pytest.mark.parametrize("d,wide", [(64, 512), (64, 513), (64, 1024), (64, 1025), (64, 2049), (64, 4096), (64, 4097), (128, 512), (128, 1025), (128, 2048), (128, 2049), (128, 4096), (128, 4100), (128, 8192), (128, 8193)])
 def test_widths(cuda, d, wide):
     """Tables about as wide as each way of holding the scores has room for: far apart, two thirds alike, all alike."""
     page, top, h, hk = 16, 70, 4, 1
