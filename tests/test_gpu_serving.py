@@ -113,6 +113,41 @@ def test_captured_steps_are_eager_steps(cuda, bits):
         assert torch.equal(a.bounds, b.bounds) and torch.equal(a.table, b.table) and a.count.item() == b.count.item()
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_pools_past_32_bits(cuda, bits):
+    """Pages and bounds that lie more than 2^32 bytes (bounds: 2^31 values) behind the first: as in a small pool."""
+    d, h, hk, page, wide, pool = 128, 16, 8, 64, 6, 20000
+    row = d if bits == 16 else d // 2 + d // 16
+    kind = torch.bfloat16 if bits == 16 else torch.uint8
+    small = [torch.zeros((2 * wide, hk, page, row), dtype=kind, device=cuda) for _ in range(2)]
+    stride = 2 ** 18 if bits == 16 else 2 ** 18 + 16      # of a page, in bytes
+    big = torch.empty(pool * stride + 2 ** 18, dtype=torch.uint8, device=cuda).view(kind)
+    per = stride // big.element_size()
+    large = [big.as_strided((pool, hk, page, row), (per, page * row, row, 1), i * hk * page * row) for i in range(2)]
+    names = torch.tensor([[19999, 0, 16390, 8200, 19000, 3], [17000, 18000, 19990, 1, 16400, 12000]], dtype=torch.int32, device=cuda)
+    table = torch.arange(2 * wide, dtype=torch.int32, device=cuda).view(2, wide)
+    wider = torch.empty(pool * 2 ** 17, dtype=torch.bfloat16, device=cuda)
+    far = wider.as_strided((pool, hk, 2, d), (2 ** 17, 2 * d, d, 1))
+    near = torch.zeros((2 * wide, hk, 2, d), dtype=torch.bfloat16, device=cuda)
+    cos, sin = ktt.rotary_table(wide * page, d, device=cuda)
+    have, after = _i32([0, 0], cuda), _i32([0, 0], cuda)
+    for i, added in enumerate(([300, 77], [1, 1], [5, 200])):
+        t = sum(added)
+        q, k, v = (x.to(cuda) for x in (_x(t, h, d, seed=i), _x(t, hk, d, seed=i + 9), _x(t, hk, d, seed=i + 18)))
+        cu = _i32([0, added[0], t], cuda)
+        results = []
+        for (kp, vp), names_of, bounds in ((small, table, near), (large, names, far)):
+            turned = ktt.paged_append(k, v, kp, vp, names_of, have, cos, sin, q=q, cu_seq=cu, lengths_out=after, bounds=bounds)
+            chosen, keys = ktt.paged_select(turned, bounds, names_of, after, page, 3, cu_seq_q=cu)
+            results.append((turned, chosen, keys, ktt.sdpa_paged(turned, kp, vp, chosen, keys)))
+        (turned, chosen, keys, out), (other, chosen_far, keys_far, out_far) = results
+        assert torch.equal(turned, other) and torch.equal(keys, keys_far) and torch.equal(out, out_far)
+        assert torch.equal(torch.where(chosen >= 0, names.flatten()[chosen.clamp(min=0).long()], -1), chosen_far)
+        have.copy_(after)
+    assert torch.equal(near[table.long()][:, :5], far[names.long()][:, :5])
+    assert torch.equal(ktt.paged_bounds(large[0], names, have, bounds=torch.empty_like(wider).as_strided(far.shape, far.stride()))[names.long()][:, :5], near[table.long()][:, :5])
+
+
 def test_two_streams_and_two_graphs_at_once(cuda):
     """Calls share nothing: what runs beside another is as it is alone."""
     d, h, hk, page, wide, top = 128, 16, 2, 16, 400, 40
