@@ -418,7 +418,8 @@ typedef struct ktt_b200_tables {
 
 /* Pages for added[b] new keys of each sequence (int32 [batch] on the device), from the end of the list on: the i-th that the call
  * takes, sequence by sequence and entry by entry, is free_pages[*count - 1 - i]. The first sequence that the list (or its row of
- * the table) has no room for gets none, and none of those behind it do: their new entries are -1. The list is only read. Outputs,
+ * the table) has no room for gets none, and none of those behind it do: their new entries are -1, and their rows are kept out of the cache by
+ * ktt_b200_paged_append_granted (an append that is not told of `granted` writes those that fit into the last page they have). The list is only read. Outputs,
  * each of which may be NULL: granted int32 [batch] (added[b], or 0); cu_seqlens int32 [batch + 1], the sums of added; and of each
  * of `tokens` packed rows, row i of sequence b being cu_seqlens[b] + i: positions int32, lengths[b] + i, and slots int64, page *
  * page_size + row in the page; both -1 behind the last sequence's rows, slots also of sequences that got nothing. */
@@ -466,6 +467,10 @@ typedef struct ktt_b200_append_at_args {
     int64_t bounds_strides[3];
 } ktt_b200_append_at_args;
 KTT_B200_API int ktt_b200_paged_append_at(const ktt_b200_append_at_args* args, void* stream);
+
+/* That of the first granted[b] new rows of each sequence (int32 [batch] on the device, ktt_b200_paged_reserve's; NULL: all). Those behind them are
+ * in no page, in no bounds and not in lengths_out; queries turn all the same. */
+KTT_B200_API int ktt_b200_paged_append_granted(const ktt_b200_append_at_args* args, const int32_t* granted, void* stream);
 
 /* Bounds of the pages that keys since[b] .. lengths[b] - 1 of each sequence lie in (since int32 [batch] on the device, or NULL: all
  * pages); where since[b] lies inside a page, those that the page has already are kept and widened. cache.v is not used. */

@@ -71,6 +71,7 @@ EXPORTS = (
     "ktt_b200_paged_reserve",
     "ktt_b200_paged_release",
     "ktt_b200_paged_append_at",
+    "ktt_b200_paged_append_granted",
     "ktt_b200_paged_bounds",
     "ktt_b200_paged_select",
     "ktt_b200_paged_select_workspace",
@@ -534,6 +535,7 @@ def lib():
     handle.ktt_b200_paged_reserve.argtypes = [ctypes.POINTER(Tables), _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _ptr]
     handle.ktt_b200_paged_release.argtypes = [ctypes.POINTER(Tables), _ptr, _ptr]
     handle.ktt_b200_paged_append_at.argtypes = [ctypes.POINTER(AppendAtArgs), _ptr]
+    handle.ktt_b200_paged_append_granted.argtypes = [ctypes.POINTER(AppendAtArgs), _ptr, _ptr]
     handle.ktt_b200_paged_bounds.argtypes = [ctypes.POINTER(BoundsArgs), _ptr]
     handle.ktt_b200_paged_select_workspace.argtypes = [ctypes.POINTER(SelectArgs)]
     handle.ktt_b200_paged_select_workspace.restype = _i64

@@ -41,8 +41,12 @@ struct Edges {
     }
 };
 
-// The bounds of the pages that keys of an append lie in (select.cu): those of sequence b from lengths[b] on, `rows` of each, or packed.
-int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, cudaStream_t stream);
+// How many of its new rows a sequence takes.
+__device__ __forceinline__ int64_t granted_to(const int32_t* granted, int b) { return granted ? max(granted[b], 0) : INT64_MAX; }
+
+// The bounds of the pages that keys of an append lie in (select.cu): those of sequence b from lengths[b] on, `rows` of each, or packed, as many as are
+// granted.
+int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, const int32_t* granted, cudaStream_t stream);
 // Bounds from an argument block's fields after their checks; null, or why not.
 const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3]);
 // Those that are written, of a cache of head dim d.

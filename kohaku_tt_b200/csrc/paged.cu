@@ -52,11 +52,13 @@ struct AppendParams {
     int32_t* lengths_out;
     int vec;
 };
-// With positions of their own, and with bounds that a key of a sequence goes into on the way (one row for each sequence).
+// With positions of their own, with bounds that a key of a sequence goes into on the way (one row for each sequence), and with how many of
+// its new rows each sequence takes (null: all).
 struct AppendAtParams : AppendParams {
     Placed positions;
     PairAxes axes;
     Bounds bounds;
+    const int32_t* granted;
 };
 
 // Eight columns of one token in the cache's 4 bits. The 8 threads of a group of 64 columns are neighbours in a warp and
@@ -206,7 +208,9 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (p.lengths_out && blockIdx.x == 0 && blockIdx.y == 0) {
         for (int b = threadIdx.y * blockDim.x + threadIdx.x; b < p.batch; b += blockDim.x * blockDim.y) {
-            const int64_t more = p.cu ? max(p.cu[b + 1] - p.cu[b], 0) : p.rows, all = cached_keys(p.c, b) + more;
+            int64_t more = p.cu ? max(p.cu[b + 1] - p.cu[b], 0) : p.rows;
+            if constexpr (kAt) more = min(more, granted_to(p.granted, b));
+            const int64_t all = cached_keys(p.c, b) + more;
             p.lengths_out[b] = static_cast<int32_t>(all < p.c.cap ? all : p.c.cap);
         }
     }
@@ -273,6 +277,7 @@ __global__ void __launch_bounds__(256, kHeads == 4 ? 3 : 4) append_kernel(const 
     }
     int64_t page = -1;
     if (row_there && pos < p.c.cap) page = page_of(p.c, b, static_cast<int>(pos));
+    if constexpr (kAt) page = x_row.in < granted_to(p.granted, b) ? page : -1;   // (looked up beside it, not before it)
     const bool there = page >= 0;
     const int at = there ? static_cast<int>(pos) % p.c.page_size : 0;
     unsigned char* base = !there ? nullptr : what == 2 ? p.c.v + page * p.c.vs[0] : p.c.k + page * p.c.ks[0];
@@ -640,13 +645,19 @@ extern "C" int ktt_b200_paged_append(const ktt_b200_append_args* a, void* stream
     return go ? launch(p, a->cache.bits, a->d, static_cast<cudaStream_t>(stream)) : 0;
 }
 
-extern "C" int ktt_b200_paged_append_at(const ktt_b200_append_at_args* x, void* stream) {
+extern "C" int ktt_b200_paged_append_at(const ktt_b200_append_at_args* x, void* stream) { return ktt_b200_paged_append_granted(x, nullptr, stream); }
+
+extern "C" int ktt_b200_paged_append_granted(const ktt_b200_append_at_args* x, const int32_t* granted, void* stream) {
     if (!x) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: null arguments");
     const ktt_b200_append_args* a = &x->base;
     AppendAtParams p = {};
     bool go;
     if (int rc = fill(p, a, go)) return rc;
+    if (granted && p.lengths_out && granted < p.lengths_out + a->batch && p.lengths_out < granted + a->batch) {
+        return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: lengths_out must not overlap granted");
+    }
     if (!go) return 0;
+    p.granted = granted;
     p.axes.axes = 1;
     if (x->positions.positions && a->cos) {
         if (const char* why = axes_of(p.axes, x->positions, a->pairs)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_append: %s", why);
@@ -663,7 +674,7 @@ extern "C" int ktt_b200_paged_append_at(const ktt_b200_append_at_args* x, void* 
     if (passing) p.bounds = bounds;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (int rc = launch(p, a->cache.bits, a->d, st)) return rc;
-    return bounds.at && !passing ? keep_bounds(p.c, a->cache.bits, a->d, p.kv_heads, bounds, a->batch, a->rows, a->cu_seqlens, st) : 0;
+    return bounds.at && !passing ? keep_bounds(p.c, a->cache.bits, a->d, p.kv_heads, bounds, a->batch, a->rows, a->cu_seqlens, granted, st) : 0;
 }
 
 extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {

@@ -43,6 +43,7 @@ struct BoundsParams {
     const int32_t* since;   // without `rows`: the keys that pages have bounds of (null: none)
     int64_t rows;           // > 0: keys appended behind the lengths: of each sequence, or packed
     const int32_t* cu;
+    const int32_t* granted; // how many of these each sequence takes (null: all)
 };
 
 constexpr int kLotOfTokens = 16;   // packed rows that a warp looks for pages in
@@ -147,10 +148,11 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
         int b = -1, place = 0, end = 0;
         bool leads = false;
         const bool mine = lane < kLotOfTokens && n < p.rows;
-        int64_t start = 0, behind = 0;
+        int64_t start = 0, behind = 0, many = 0;
         int keys = 0;
         if (p.batch < 32) {   // a lane looks at a sequence, its length with it, in one trip
             const int offset = p.cu[min(lane, p.batch)], have = cached_keys(p.c, min(lane, p.batch - 1));
+            const int64_t takes = granted_to(p.granted, min(lane, p.batch - 1));
             // (The last that starts at or before the token, -1: none; five looks at another lane's.)
 #pragma unroll
             for (int step = 16; step > 0; step >>= 1) {
@@ -161,14 +163,17 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
             start = __shfl_sync(0xffffffffu, offset, max(b, 0));
             behind = __shfl_sync(0xffffffffu, offset, max(b, 0) + 1);
             keys = __shfl_sync(0xffffffffu, have, max(b, 0));
+            many = __shfl_sync(0xffffffffu, takes, max(b, 0));
         } else if (mine) {
             b = sequence_of(p.cu, p.batch, n);
             if (b >= 0) {
                 start = p.cu[b];
                 behind = p.cu[b + 1];
                 keys = cached_keys(p.c, b);
+                many = granted_to(p.granted, b);
             }
         }
+        behind = min(behind, start + min(many, static_cast<int64_t>(INT32_MAX)));
         if (b >= 0 && n >= start && n < behind) {   // (offsets that decrease)
             const int64_t in = n - start, at = keys + in, all = at + (behind - n);
             end = static_cast<int>(all < p.c.cap ? all : p.c.cap);
@@ -188,7 +193,8 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
         int begin = 0, end = len;
         if (p.rows > 0) {
             begin = len;
-            end = static_cast<int>(len + p.rows < p.c.cap ? len + p.rows : p.c.cap);
+            const int64_t all = len + min(p.rows, granted_to(p.granted, b));
+            end = static_cast<int>(all < p.c.cap ? all : p.c.cap);
         } else if (p.since) {
             begin = min(max(p.since[b], 0), len);
         }
@@ -963,7 +969,7 @@ int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t 
 
 }  // namespace
 
-int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, cudaStream_t stream) {
+int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, const int32_t* granted, cudaStream_t stream) {
     if (rows == 0) return 0;
     BoundsParams p = {};
     p.c = c;
@@ -972,6 +978,7 @@ int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bou
     p.kv_heads = kv_heads;
     p.rows = rows;
     p.cu = cu;
+    p.granted = granted;
     return launch_bounds(p, bits, d, stream);
 }
 

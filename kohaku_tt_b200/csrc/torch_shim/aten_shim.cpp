@@ -1230,13 +1230,13 @@ const Tensor* bounds_of(PyObject* o, const Tensor& like, int64_t pages, int64_t 
     return t;
 }
 
-// paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq (on the device), lengths_out, positions, axes, bounds):
+// paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq (on the device), lengths_out, positions, axes, bounds, granted):
 // the rotated queries or None; NotImplemented when the call is not one for the fast path.
 PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    const Tensor *k, *v, *q = nullptr, *cu = nullptr, *len_out = nullptr, *pos = nullptr, *bounds = nullptr;
+    const Tensor *k, *v, *q = nullptr, *cu = nullptr, *len_out = nullptr, *pos = nullptr, *bounds = nullptr, *granted = nullptr;
     Cache x;
-    if (n != 15 || !callable_now() || !(k = tensor_of(args[0])) || !(v = tensor_of(args[1])) || !cache_of(x, args + 2, Py_None)) Py_RETURN_NOTIMPLEMENTED;
+    if (n != 16 || !callable_now() || !(k = tensor_of(args[0])) || !(v = tensor_of(args[1])) || !cache_of(x, args + 2, Py_None)) Py_RETURN_NOTIMPLEMENTED;
     const Tensor& pages = *tensor_of(args[2]);
     const bool packed = args[10] != Py_None, turns = args[6] != Py_None;
     if (packed && (!(cu = tensor_of(args[10])) || !int32_vector(*cu, pages, x.batch + 1))) Py_RETURN_NOTIMPLEMENTED;
@@ -1260,6 +1260,7 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
         turn.positions = *pos;
     }
     if (args[14] != Py_None && !(bounds = bounds_of(args[14], pages, x.c.pages, x.c.kv_heads, x.dim))) Py_RETURN_NOTIMPLEMENTED;
+    if (args[15] != Py_None && (!(granted = tensor_of(args[15])) || !int32_vector(*granted, pages, x.batch))) Py_RETURN_NOTIMPLEMENTED;
     Tensor out;
     const bool done = attempted([&] {
         pybind11::gil_scoped_release release;
@@ -1299,7 +1300,9 @@ PyObject* py_paged_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
             placed.bounds = bounds->data_ptr();
             set3(placed.bounds_strides, *bounds);
         }
-        raise_status(pos || bounds ? ktt_b200_paged_append_at(&placed, at::cuda::getCurrentCUDAStream()) : ktt_b200_paged_append(&a, at::cuda::getCurrentCUDAStream()), "paged_append");
+        const cudaStream_t stream = at::cuda::getCurrentCUDAStream();
+        raise_status(pos || bounds || granted ? ktt_b200_paged_append_granted(&placed, granted ? granted->data_ptr<int32_t>() : nullptr, stream) : ktt_b200_paged_append(&a, stream),
+                     "paged_append");
     });
     if (!done) Py_RETURN_NOTIMPLEMENTED;
     if (!q) Py_RETURN_NONE;

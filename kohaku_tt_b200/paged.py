@@ -94,9 +94,9 @@ def check_bounds(bounds, like, pages, hk, dim, what):
         raise _lib.UnsupportedAttention(f"kohaku_tt_b200.{what}: the rows of bounds must be dense")
 
 
-def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions=None, axes=None, bounds=None):
+def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions=None, axes=None, bounds=None, granted=None):
     what = "paged_append"
-    ops._require_cuda(k, v, q, cos, sin, lengths_out, positions, bounds)
+    ops._require_cuda(k, v, q, cos, sin, lengths_out, positions, bounds, granted)
     at = _lib.AppendAtArgs()
     a = at.base
     dim, batch, cap = _pages(a.cache, k_pages, v_pages, block_table, lengths, None, what)
@@ -145,12 +145,15 @@ def _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleav
             if lengths_out.dtype != torch.int32 or lengths_out.shape != lengths.shape or not lengths_out.is_contiguous() or lengths_out.device != lengths.device:
                 raise ValueError("kohaku_tt_b200.paged_append: lengths_out must be a contiguous int32 [B]")
             a.lengths_out = lengths_out.data_ptr()
+        if granted is not None and (granted.dtype != torch.int32 or granted.shape != lengths.shape or not granted.is_contiguous() or granted.device != lengths.device):
+            raise ValueError("kohaku_tt_b200.paged_append: granted must be a contiguous int32 [B]")
         a.batch, a.rows, a.d, a.interleaved = batch, rows, dim, int(interleaved)
         a.k, a.v = k.data_ptr(), v.data_ptr()
         ops._set3(a.k_strides, strides(k))
         ops._set3(a.v_strides, strides(v))
-        if positions is not None or bounds is not None:
-            _lib.check(_lib.lib().ktt_b200_paged_append_at(ctypes.byref(at), ops._stream(k_pages.device)), what)
+        if positions is not None or bounds is not None or granted is not None:
+            given = None if granted is None else granted.data_ptr()
+            _lib.check(_lib.lib().ktt_b200_paged_append_granted(ctypes.byref(at), given, ops._stream(k_pages.device)), what)
         else:
             _lib.check(_lib.lib().ktt_b200_paged_append(ctypes.byref(a), ops._stream(k_pages.device)), what)
     return q_out
@@ -262,9 +265,10 @@ def _append_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages:
 @torch.library.custom_op("ktt_b200::_paged_append_at", mutates_args=("k_pages", "v_pages", "lengths_out", "bounds"), device_types="cuda")
 def _append_at_op(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor, lengths: torch.Tensor,
                   cos: torch.Tensor | None, sin: torch.Tensor | None, q: torch.Tensor | None, interleaved: bool, cu_seq: torch.Tensor | None,
-                  lengths_out: torch.Tensor | None, positions: torch.Tensor | None, axes: Sequence[int] | None, bounds: torch.Tensor | None) -> torch.Tensor:
-    """With positions or bounds. (As arguments of the operator above that are None by default they would be lost on their way.)"""
-    out = _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
+                  lengths_out: torch.Tensor | None, positions: torch.Tensor | None, axes: Sequence[int] | None, bounds: torch.Tensor | None,
+                  granted: torch.Tensor | None) -> torch.Tensor:
+    """With positions, bounds or granted. (As arguments of the operator above that are None by default they would be lost on their way.)"""
+    out = _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted)
     return k.new_empty((0,)) if out is None else out
 
 
@@ -274,7 +278,7 @@ def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu
 
 
 @_append_at_op.register_fake
-def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds):
+def _(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted):
     return k.new_empty((0,)) if q is None else ops._empty_like_rows(q)
 
 
@@ -316,7 +320,7 @@ def _(q, k_pages, v_pages, chosen, keys, scale, max_k):
 # ---- the entry points ------------------------------------------------------------------------
 
 def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=None, q=None, interleaved=False,
-                 cu_seq=None, lengths_out=None, positions=None, axes=None, bounds=None):
+                 cu_seq=None, lengths_out=None, positions=None, axes=None, bounds=None, granted=None):
     """Writes new keys and values behind what sequences have in a paged cache, the keys rotated on the way
     (and the step's queries alongside), in one launch.
 
@@ -332,24 +336,27 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     prompt; packed rows: [T], or [axes, T]); the tables then need not cover the places.
     bounds: a cache's bounds (paged_bounds), which are kept up to date for the pages that the new keys go to;
     what those held before must be in the bounds already.
+    granted: paged_reserve's, int32 [B] on the device: only the first granted[b] new rows of each sequence go into pages and bounds and
+    count in lengths_out (queries are rotated all the same). Without it all rows do, also those that the reservation had no room for: what of
+    them fits goes into the last page that the sequence has, and lengths_out counts the others too.
     Pages of 4 bits (paged_cache(bits=4)) hold each 64 channels of a row as codes 0 to 15 of
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
     interleaved = bool(interleaved)
     if torch.compiler.is_compiling():
-        if positions is None and axes is None and bounds is None:
+        if positions is None and axes is None and bounds is None and granted is None:
             out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
         else:
             out = torch.ops.ktt_b200._paged_append_at(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out,
-                                                      positions, axes, bounds)
+                                                      positions, axes, bounds, granted)
         return out if q is not None else None
     # Eager calls on plain CUDA tensors are served by C++ in one step.
     eager = _lib.native()
     if eager and _on_device(cu_seq):
-        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
+        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted)
         if out is not NotImplemented:
             return out
     with torch.no_grad():
-        return _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds)
+        return _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted)
 
 
 def paged_read(k_pages, v_pages, block_table, lengths, max_k=None):

@@ -84,7 +84,8 @@ def paged_reserve(block_table, lengths, added, free, count, page_size, tokens, c
     has. They are taken from the end, sequence by sequence; neither is changed, count_out (int32 [1], another buffer) receives how
     many are left. lengths are not changed either.
     granted int32 [B]: added[b], or 0 for the first sequence that the list, or its row of the table, has no room for and for all
-    behind it; their new entries become -1 (an append there goes nowhere), and they can be asked for again later.
+    behind it; their new entries become -1, and they can be asked for again later. Given to paged_append, it keeps their rows out of the
+    cache and out of lengths_out; where no call can run short it may be left out.
     The new tokens are packed, row i of sequence b at cu_seq[b] + i, as paged_append and sdpa_paged take them: cu_seq int32 [B + 1];
     for `tokens` rows (the sum of added; 0: not wanted), positions int32, lengths[b] + i, and slots int64, page * page_size + row in the
     page, which is where the token's row lies in a buffer [pages * page_size, ...]; -1 in rows behind the last sequence's, and

@@ -30,6 +30,19 @@ def reserve(table, lengths, added, free, count, page, tokens):
     return table, cu, positions + [-1] * (tokens - len(positions)), slots + [-1] * (tokens - len(slots)), granted, left
 
 
+def append(contents, table, lengths, rows, granted):
+    """New rows [n, Hk, D] of each sequence into bf16 `contents` [pages, Hk, page, D], in place, the first granted[b] of them; the new lengths."""
+    pages, page, cap, after = contents.shape[0], contents.shape[2], table.shape[1] * contents.shape[2], []
+    for b, (n, new, some) in enumerate(zip(lengths, rows, granted)):
+        n = min(max(n, 0), cap)
+        some = min(max(some, 0), len(new))
+        for at, row in zip(range(n, min(n + some, cap)), new):
+            if 0 <= table[b, at // page] < pages:
+                contents[table[b, at // page], :, at % page] = row
+        after.append(min(n + some, cap))
+    return after
+
+
 def release(table, lengths, kept, free, count, page):
     """(table, free, count) after it."""
     table, free, pool, width = [list(r) for r in table], list(free), len(free), len(table[0])

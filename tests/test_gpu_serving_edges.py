@@ -1,0 +1,188 @@
+"""A server's steps where they are not plain: reservations that run short, sequences cut back inside a page, modes that watch operators,
+scores that are equal, bounds that lie on one another."""
+
+import random
+
+import pytest
+import torch
+
+import kohaku_tt_b200 as ktt
+from kohaku_tt_b200 import _lib
+from oracle import paged_oracle as po
+from oracle import serving_oracle as so
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["native", "python"])
+def path(request, monkeypatch):
+    """Through the C++ edge, and through Python's."""
+    if request.param == "python":
+        monkeypatch.setattr(_lib, "_NATIVE", False)
+
+
+def _x(*shape, seed=0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+
+
+def _i32(x, cuda):
+    return torch.tensor(x, dtype=torch.int32, device=cuda)
+
+
+def _held(contents, bits, value=False):
+    """What pages of these bf16 values hold."""
+    return contents if bits == 16 else po.pack(contents, value)
+
+
+def _turned(k, at, cos, sin):
+    """Rows [n, Hk, D] by their positions."""
+    at = torch.tensor(at, dtype=torch.long)
+    return po.turn_fp32(k, cos[at][:, None], sin[at][:, None], False)
+
+
+def _near(got, want, mag, size):
+    """As in the tests of attention over tables of a token's own."""
+    e = 2.0 ** -8
+    room = e * want.abs() + (e + 2.0 ** -16 + torch.expm1(2 * 2.0 ** -18 * size[..., None])) * (1 + e) * mag + 1e-30
+    off = (got.double().cpu() - want).abs()
+    assert bool((off <= room).all()), (off - room).max().item()
+
+
+# ---- rows that a reservation had no room for ----------------------------------------------------
+
+GRANTED = [  # lengths, new rows of each sequence, granted
+    ([0, 20, 16, 47], [3, 30, 1, 40], [3, 0, 1, 0]),
+    ([5, 15, 31, 0], [1, 1, 1, 1], [1, 0, 0, 1]),
+    ([5, 15, 31, 0], [1, 1, 1, 1], [0, 0, 0, 0]),
+    ([100, 90, 3, 0], [70, 0, 33, 16], [12, 5, 99, -4]),     # some of a sequence's, more than there are, fewer than none
+    ([127, 128, 126, -3], [4, 4, 4, 4], [4, 4, 1, 4]),       # past the table's end
+]
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lengths,new,granted", GRANTED)
+@pytest.mark.parametrize("many", [False, True])
+def test_append_of_granted_rows(cuda, path, bits, d, lengths, new, granted, many):
+    """The first granted[b] rows of each sequence are in the cache, in the bounds and in the new lengths; queries turn all. Packed, and where
+    all have as many rows dense; of 4 and of 40 sequences (whose rows are looked up in another way)."""
+    hk, h, page, wide = 2, 4, 16, 8
+    if many:
+        lengths, new, granted = lengths * 10, new * 10, granted * 10
+    batch, total = len(lengths), sum(new)
+    table = torch.randperm(batch * wide, generator=torch.Generator().manual_seed(1)).view(batch, wide).to(torch.int32)
+    table[1, -1] = -1
+    k, v, q = _x(total, hk, d, seed=2), _x(total, hk, d, seed=3), _x(total, h, d, seed=4)
+    cos, sin = ktt.rotary_table(wide * page + 99, d, device=cuda)
+    starts = [min(max(n, 0), wide * page) for n in lengths]
+    places = [n + i for n, m in zip(starts, new) for i in range(m)]
+    for positions in (None, torch.tensor(places, dtype=torch.int32, device=cuda) // 2):
+        turned = _turned(k, places if positions is None else [x // 2 for x in places], cos.cpu(), sin.cpu())
+        kc, vc = _x(batch * wide, hk, page, d, seed=5), _x(batch * wide, hk, page, d, seed=6)
+        kp, vp = (_held(x, bits, value).to(cuda) for x, value in ((kc, False), (vc, True)))
+        td, lens = table.to(cuda), _i32(lengths, cuda)
+        plain = torch.full((batch * wide, hk, 2, d), 7.0, dtype=torch.bfloat16)
+        bounds = so.bounds(_held(kc, bits), table, lengths, plain)
+        after = so.append(kc, table, lengths, turned.split(new), granted)
+        assert after == so.append(vc, table, lengths, v.split(new), granted)
+        want_bounds = so.bounds(_held(kc, bits), table, after, plain)
+        want_q = _turned(q, places if positions is None else [x // 2 for x in places], cos.cpu(), sin.cpu())
+        forms = [(k, v, q, positions, dict(cu_seq=_i32([sum(new[:i]) for i in range(batch + 1)], cuda)))]
+        if len(set(new)) == 1:
+            dense = [x.view(batch, new[0], -1, d).transpose(1, 2) for x in (k, v, q)]
+            forms.append((*dense, None if positions is None else positions.view(batch, -1), {}))
+        for kn, vn, qn, pos, kw in forms:
+            for edges in (None, bounds.to(cuda)):
+                into, out = (kp.clone(), vp.clone()), _i32([-1] * batch, cuda)
+                got = ktt.paged_append(kn.to(cuda), vn.to(cuda), *into, td, lens, cos, sin, q=qn.to(cuda), lengths_out=out, positions=pos, bounds=edges,
+                                       granted=_i32(granted, cuda), **kw)
+                assert out.tolist() == after
+                assert torch.equal(into[0].cpu(), _held(kc, bits)) and torch.equal(into[1].cpu(), _held(vc, bits, True))
+                assert edges is None or torch.equal(edges.cpu(), want_bounds)
+                assert torch.equal((got if kw else got.transpose(1, 2).reshape(total, h, d)).cpu(), want_q)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_steps_that_run_short(cuda, path, bits):
+    """Steps of a server whose list of free pages runs short: what was refused is asked for again, pages come back as sequences end. Tables,
+    lengths, pages, bounds and outputs are the definitions'."""
+    d, h, hk, page, wide, pool, top, batch = 64, 4, 2, 16, 10, 17, 3, 4
+    rng = random.Random(3)
+    kp, vp = ktt.paged_cache(pool, hk, page, d, bits=bits, device=cuda)
+    kc, vc = torch.zeros((pool, hk, page, d), dtype=torch.bfloat16), torch.zeros((pool, hk, page, d), dtype=torch.bfloat16)
+    table, free, count = [[-1] * wide for _ in range(batch)], list(range(pool)), pool
+    td, fd, left, now = _i32(table, cuda), _i32(free, cuda), _i32([0], cuda), _i32([pool], cuda)
+    lens, after, have = _i32([0] * batch, cuda), _i32([0] * batch, cuda), [0] * batch
+    bounds = ktt.paged_bounds(kp, td, lens)
+    cos, sin = ktt.rotary_table(wide * page, d, device=cuda)
+    refused, waiting, later = 0, [False] * batch, 0
+    ask = [rng.randint(20, 60) for _ in range(batch)]
+    for step in range(24):
+        total = sum(ask)
+        q, k, v = _x(total, h, d, seed=step), _x(total, hk, d, seed=step + 100), _x(total, hk, d, seed=step + 200)
+        cu, at, slots, granted = ktt.paged_reserve(td, lens, _i32(ask, cuda), fd, now, page, total, left)
+        turned = ktt.paged_append(k.to(cuda), v.to(cuda), kp, vp, td, lens, cos, sin, q=q.to(cuda), cu_seq=cu, lengths_out=after, bounds=bounds, granted=granted)
+        chosen, keys = ktt.paged_select(turned, bounds, td, after, page, top, cu_seq_q=cu)
+        out = ktt.sdpa_paged(turned, kp, vp, chosen, keys)
+        table, _, places, want_slots, some, count = so.reserve(table, have, ask, free, count, page, total)
+        assert td.tolist() == table and granted.tolist() == some and left.item() == count and slots.tolist() == want_slots and at.tolist() == places
+        names = torch.tensor(table, dtype=torch.int32)
+        so.append(vc, names, have, v.split(ask), some)
+        have = so.append(kc, names, have, _turned(k, places, cos.cpu(), sin.cpu()).split(ask), some)
+        assert after.tolist() == have
+        assert torch.equal(kp.cpu(), _held(kc, bits)) and torch.equal(vp.cpu(), _held(vc, bits, True))
+        want = so.bounds(_held(kc, bits), names, have, bounds.cpu())
+        assert torch.equal(bounds.cpu(), want)
+        rows = [r for r, b in enumerate(b for b in range(batch) for _ in range(ask[b])) if some[b] == ask[b]]
+        owners = so.tokens(ask, have, wide * page)
+        want, want_keys = so.select(turned.cpu()[rows], bounds.cpu(), names, [owners[r] for r in rows], page, top, 1, 1)
+        assert torch.equal(chosen.cpu()[rows], want) and torch.equal(keys.cpu()[rows], want_keys)
+        _near(out[rows], *so.attend(turned.cpu()[rows], kp.cpu(), vp.cpu(), want, want_keys, d ** -0.5))
+        refused += sum(x != y for x, y in zip(ask, some))
+        later += sum(was and x == y for was, x, y in zip(waiting, ask, some))
+        waiting = [x != y for x, y in zip(ask, some)]
+        # Some sequences end; what was refused is asked for again.
+        kept = [0 if n > wide * page - 70 or rng.random() < 0.1 else n for n in have]
+        ktt.paged_release(td, after, _i32(kept, cuda), fd, left, page, now)
+        table, free, count = so.release(table, have, kept, free, count, page)
+        assert td.tolist() == table and now.item() == count and fd.tolist()[:count] == free[:count]
+        ask = [x if x != y else (rng.randint(1, 60) if n == 0 else rng.choice([1, 1, 20])) for x, y, n in zip(ask, some, kept)]
+        have = kept
+        lens.copy_(_i32(have, cuda))
+    assert refused > 5 and later > 2
+
+
+def test_granted_refusals(cuda, path):
+    row, kp = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16, device=cuda), torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16, device=cuda)
+    table, n, out = _i32([[0, 1]], cuda), _i32([3], cuda), _i32([0], cuda)
+    for bad in (n.long(), _i32([1, 1], cuda), _i32([[1]], cuda), out):      # (out: what the launch writes)
+        with pytest.raises(ValueError):
+            ktt.paged_append(row, row, kp, kp, table, n, lengths_out=out, granted=bad)
+    with pytest.raises((RuntimeError, ValueError)):
+        ktt.paged_append(row, row, kp, kp, table, n, granted=torch.ones(1, dtype=torch.int32))
+
+
+def test_granted_compiled_and_captured(cuda):
+    """The append of granted rows in a compiled graph and in a captured one, as the eager call."""
+    d, hk, page, wide, batch = 64, 2, 16, 4, 3
+    table, lens, granted = _i32([[0, 1, 2, 3], [4, 5, -1, -1], [6, -1, -1, -1]], cuda), _i32([20, 30, 0], cuda), _i32([1, 0, 1], cuda)
+    rows = [_x(batch, n, 1, d, seed=n).to(cuda) for n in (hk, hk, 4)]
+    cos, sin = ktt.rotary_table(wide * page, d, device=cuda)
+
+    def fresh():
+        return (*(_x(8, hk, page, d, seed=s).to(cuda) for s in (7, 8)), torch.zeros((8, hk, 2, d), dtype=torch.bfloat16, device=cuda), _i32([-1] * batch, cuda))
+
+    def step(k, v, q, kp, vp, bounds, out):
+        return ktt.paged_append(k, v, kp, vp, table, lens, cos, sin, q=q, lengths_out=out, bounds=bounds, granted=granted)
+
+    first, second, third = fresh(), fresh(), fresh()
+    want = step(*rows, *first)
+    assert first[3].tolist() == [21, 30, 1]
+    got = torch.compile(step, fullgraph=True)(*rows, *second)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(*rows, *third)
+    graph.replay()
+    assert torch.equal(got, want) and torch.equal(captured, want)
+    for a, b, c in zip(first, second, third):
+        assert torch.equal(a, b) and torch.equal(a, c)
