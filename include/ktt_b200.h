@@ -427,7 +427,7 @@ KTT_B200_API int ktt_b200_paged_reserve(const ktt_b200_tables* args, const int32
 
 /* Cuts sequences back to kept[b] keys (int32 [batch] on the device, clamped to [0, lengths[b]]; 0: all of its pages): the pages behind those
  * go to free_pages[*count ..], sequence by sequence and entry by entry, and their entries become -1. Entries outside [0, pool) give
- * nothing; pages past the list's end are dropped. */
+ * nothing; pages past the list's end are dropped. Bounds of a page that is cut inside: ktt_b200_paged_release_bounds. */
 KTT_B200_API int ktt_b200_paged_release(const ktt_b200_tables* args, const int32_t* kept, void* stream);
 
 /* Appends rows lengths[b] .. of sequence b: k rotated (as above, at the position it is cached at; cos NULL: as it is) and
@@ -482,6 +482,11 @@ typedef struct ktt_b200_bounds_args {
     int64_t bounds_strides[3];
 } ktt_b200_bounds_args;
 KTT_B200_API int ktt_b200_paged_bounds(const ktt_b200_bounds_args* args, void* stream);
+
+/* ktt_b200_paged_release with bounds of the same table and lengths (NULL: none; since is not used): those of a page that a sequence is cut
+ * in are made again, of the keys that are left there alone. An append behind kept[b] would else widen bounds that the dropped keys have a
+ * part in. */
+KTT_B200_API int ktt_b200_paged_release_bounds(const ktt_b200_tables* args, const int32_t* kept, const ktt_b200_bounds_args* bounds, void* stream);
 
 /* The `top` pages of its sequence that each query token goes to, for each K / V head: the first `first`, the last `last` (first + last
  * <= top, last >= 1), and of the others those of the largest score, ties to the lower place. A page's score is the largest logit that a key

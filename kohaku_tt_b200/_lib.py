@@ -73,6 +73,7 @@ EXPORTS = (
     "ktt_b200_paged_append_at",
     "ktt_b200_paged_append_granted",
     "ktt_b200_paged_bounds",
+    "ktt_b200_paged_release_bounds",
     "ktt_b200_paged_select",
     "ktt_b200_paged_select_workspace",
     "ktt_b200_paged_sdpa_chosen",
@@ -537,6 +538,7 @@ def lib():
     handle.ktt_b200_paged_append_at.argtypes = [ctypes.POINTER(AppendAtArgs), _ptr]
     handle.ktt_b200_paged_append_granted.argtypes = [ctypes.POINTER(AppendAtArgs), _ptr, _ptr]
     handle.ktt_b200_paged_bounds.argtypes = [ctypes.POINTER(BoundsArgs), _ptr]
+    handle.ktt_b200_paged_release_bounds.argtypes = [ctypes.POINTER(Tables), _ptr, ctypes.POINTER(BoundsArgs), _ptr]
     handle.ktt_b200_paged_select_workspace.argtypes = [ctypes.POINTER(SelectArgs)]
     handle.ktt_b200_paged_select_workspace.restype = _i64
     handle.ktt_b200_paged_select.argtypes = [ctypes.POINTER(SelectArgs), _ptr]

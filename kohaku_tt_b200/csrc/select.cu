@@ -41,6 +41,7 @@ struct BoundsParams {
     Bounds bounds;
     int batch, kv_heads;
     const int32_t* since;   // without `rows`: the keys that pages have bounds of (null: none)
+    const int32_t* kept;    // only the page that a sequence is cut in: made again of the keys before kept[b] (null: not asked for)
     int64_t rows;           // > 0: keys appended behind the lengths: of each sequence, or packed
     const int32_t* cu;
     const int32_t* granted; // how many of these each sequence takes (null: all)
@@ -195,6 +196,9 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
             begin = len;
             const int64_t all = len + min(p.rows, granted_to(p.granted, b));
             end = static_cast<int>(all < p.c.cap ? all : p.c.cap);
+        } else if (p.kept) {
+            end = min(max(p.kept[b], 0), len);
+            begin = end < len ? end - end % page_size : end;
         } else if (p.since) {
             begin = min(max(p.since[b], 0), len);
         }
@@ -207,6 +211,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
 template <int D, int kBits>
 int launch_bounds(const BoundsParams& p, cudaStream_t stream) {
     const int64_t lots = p.cu ? (p.rows + kLotOfTokens - 1) / kLotOfTokens
+                              : p.kept ? 1
                               : (p.rows > 0 ? (p.rows + p.c.page_size - 2) / p.c.page_size + 1 : (static_cast<int64_t>(p.c.cap) + p.c.page_size - 1) / p.c.page_size);
     const dim3 grid(static_cast<unsigned>((lots * p.kv_heads + 7) / 8), static_cast<unsigned>(p.cu ? 1 : p.batch));
     if (p.cu) return launch_dependent(bounds_kernel<D, kBits, true>, p, grid, dim3(256), stream, "paged_bounds launch");
@@ -986,9 +991,11 @@ int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bou
 
 using namespace ktt;
 
-extern "C" int ktt_b200_paged_bounds(const ktt_b200_bounds_args* a, void* stream) {
+namespace {
+
+// The checks of a call for bounds, and its parameters.
+int fill(BoundsParams& p, const ktt_b200_bounds_args* a) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_bounds: null arguments");
-    BoundsParams p = {};
     if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: %s", why);
     if (a->batch < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_bounds: sizes must be positive");
     if (a->batch > 65535) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: at most 65535 sequences");
@@ -997,6 +1004,25 @@ extern "C" int ktt_b200_paged_bounds(const ktt_b200_bounds_args* a, void* stream
     p.batch = a->batch;
     p.kv_heads = a->cache.kv_heads;
     p.since = a->since;
+    return 0;
+}
+
+}  // namespace
+
+namespace ktt {
+
+int cut_bounds(const ktt_b200_bounds_args* a, const int32_t* kept, bool launch, cudaStream_t stream) {
+    BoundsParams p = {};
+    if (int rc = fill(p, a)) return rc;
+    p.kept = kept;
+    return launch ? launch_bounds(p, a->cache.bits, a->d, stream) : 0;
+}
+
+}  // namespace ktt
+
+extern "C" int ktt_b200_paged_bounds(const ktt_b200_bounds_args* a, void* stream) {
+    BoundsParams p = {};
+    if (int rc = fill(p, a)) return rc;
     return launch_bounds(p, a->cache.bits, a->d, static_cast<cudaStream_t>(stream));
 }
 

@@ -5,7 +5,7 @@
 // free[count - 1 - before_b - i], a token's page is found without reading an entry that the same launch writes, and nothing waits for
 // anything: every CTA sums up the lengths for itself. Bound: 12 bytes written for a token and 8 moved for a page, which is nothing; one trip for
 // the lengths, a sum over the CTA and a search among the sequences are all that a call takes.
-#include "paged.cuh"
+#include "four_bits.cuh"
 
 namespace ktt {
 namespace {
@@ -320,11 +320,22 @@ extern "C" int ktt_b200_paged_reserve(const ktt_b200_tables* a, const int32_t* a
     return launch_dependent(reserve_kernel, p, grid, dim3(kThreads), static_cast<cudaStream_t>(stream), "paged_reserve launch");
 }
 
-extern "C" int ktt_b200_paged_release(const ktt_b200_tables* a, const int32_t* kept, void* stream) {
+extern "C" int ktt_b200_paged_release(const ktt_b200_tables* a, const int32_t* kept, void* stream) { return ktt_b200_paged_release_bounds(a, kept, nullptr, stream); }
+
+extern "C" int ktt_b200_paged_release_bounds(const ktt_b200_tables* a, const int32_t* kept, const ktt_b200_bounds_args* bounds, void* stream) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: null arguments");
     if (const char* why = tables_refusal(*a)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_release: %s", why);
     if (!a->block_table || !a->lengths || !kept || !a->count || !a->count_out || (a->pool && !a->free_pages)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: null pointer");
     if (a->count == a->count_out) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: count_out must be another word than count");
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (bounds) {   // (refused before anything is launched)
+        if (int rc = cut_bounds(bounds, kept, false, st)) return rc;
+        const ktt_b200_pages& c = bounds->cache;
+        if (bounds->batch != a->batch || c.page_size != a->page_size || c.table_width != a->table_width || c.block_table != a->block_table || c.table_stride != a->table_stride ||
+            c.lengths != a->lengths || (c.max_keys > 0 && c.max_keys < static_cast<int64_t>(a->table_width) * a->page_size)) {
+            return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: the bounds must be of the same table and lengths");
+        }
+    }
     ReleaseParams p = {};
     p.batch = a->batch;
     p.page_size = a->page_size;
@@ -337,5 +348,6 @@ extern "C" int ktt_b200_paged_release(const ktt_b200_tables* a, const int32_t* k
     p.pool = a->pool;
     p.count = a->count;
     p.count_out = a->count_out;
-    return launch_dependent(release_kernel, p, dim3(kReleaseCtas), dim3(kReleaseThreads), static_cast<cudaStream_t>(stream), "paged_release launch");
+    if (int rc = launch_dependent(release_kernel, p, dim3(kReleaseCtas), dim3(kReleaseThreads), st, "paged_release launch")) return rc;
+    return bounds ? cut_bounds(bounds, kept, true, st) : 0;   // (a page that is cut stays in its row)
 }

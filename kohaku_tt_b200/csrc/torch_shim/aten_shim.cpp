@@ -1527,16 +1527,35 @@ PyObject* py_paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// paged_release(block_table, lengths, kept, free, count, page_size, count_out): True, or None.
+// The block of a cache's bounds; cache: its k_pages (twice), block_table and lengths.
+ktt_b200_bounds_args bounds_block(const Cache& x, const Tensor& bounds) {
+    ktt_b200_bounds_args a;
+    std::memset(&a, 0, sizeof(a));
+    a.cache = x.c;
+    a.batch = static_cast<int32_t>(x.batch);
+    a.d = static_cast<int32_t>(x.dim);
+    a.bounds = bounds.data_ptr();
+    set3(a.bounds_strides, bounds);
+    return a;
+}
+
+// paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds): True, or None.
 PyObject* py_paged_release(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     ktt_b200_tables a;
-    if (n != 7 || !callable_now() || !tables_of(a, args, args[6])) Py_RETURN_NONE;
-    const Tensor& table = *tensor_of(args[0]);
+    if (n != 9 || !callable_now() || !tables_of(a, args, args[6])) Py_RETURN_NONE;
+    const Tensor &table = *tensor_of(args[0]), *k = nullptr, *bounds = nullptr;
+    Cache x;
+    if (args[7] != Py_None || args[8] != Py_None) {
+        if (!(k = tensor_of(args[7])) || !cache_of(x, *k, *k, table, *tensor_of(args[1]), Py_None) || !(bounds = bounds_of(args[8], *k, x.c.pages, x.c.kv_heads, x.dim)) ||
+            x.c.page_size != a.page_size) Py_RETURN_NONE;
+    }
     const bool done = attempted([&] {
         pybind11::gil_scoped_release release;
         c10::cuda::CUDAGuard device(table.device());
-        raise_status(ktt_b200_paged_release(&a, tensor_of(args[2])->data_ptr<int32_t>(), at::cuda::getCurrentCUDAStream()), "paged_release");
+        ktt_b200_bounds_args edges;
+        if (bounds) edges = bounds_block(x, *bounds);
+        raise_status(ktt_b200_paged_release_bounds(&a, tensor_of(args[2])->data_ptr<int32_t>(), bounds ? &edges : nullptr, at::cuda::getCurrentCUDAStream()), "paged_release");
     });
     if (!done) Py_RETURN_NONE;
     Py_RETURN_TRUE;
@@ -1554,14 +1573,8 @@ PyObject* py_paged_bounds(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const bool done = attempted([&] {
         pybind11::gil_scoped_release release;
         c10::cuda::CUDAGuard device(k->device());
-        ktt_b200_bounds_args a;
-        std::memset(&a, 0, sizeof(a));
-        a.cache = x.c;
-        a.batch = static_cast<int32_t>(x.batch);
-        a.d = static_cast<int32_t>(x.dim);
+        ktt_b200_bounds_args a = bounds_block(x, *bounds);
         a.since = since ? since->data_ptr<int32_t>() : nullptr;
-        a.bounds = bounds->data_ptr();
-        set3(a.bounds_strides, *bounds);
         raise_status(ktt_b200_paged_bounds(&a, at::cuda::getCurrentCUDAStream()), "paged_bounds");
     });
     if (!done) Py_RETURN_NONE;

@@ -335,7 +335,7 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     positions, axes: as in `rotary`, where rows turn by positions other than their places (pictures in a
     prompt; packed rows: [T], or [axes, T]); the tables then need not cover the places.
     bounds: a cache's bounds (paged_bounds), which are kept up to date for the pages that the new keys go to;
-    what those held before must be in the bounds already.
+    what those held before, and nothing else, must be in the bounds already (a sequence that was cut back inside a page: paged_release).
     granted: paged_reserve's, int32 [B] on the device: only the first granted[b] new rows of each sequence go into pages and bounds and
     count in lengths_out (queries are rotated all the same). Without it all rows do, also those that the reservation had no room for: what of
     them fits goes into the last page that the sequence has, and lengths_out counts the others too.

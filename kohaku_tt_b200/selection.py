@@ -9,18 +9,25 @@ from . import _lib, ops
 from .paged import _offsets, _on_device, _pages, check_bounds
 
 
-def _bounds(k_pages, block_table, lengths, bounds, since):
-    what = "paged_bounds"
+def bounds_block(k_pages, block_table, lengths, bounds, what):
+    """A ktt_b200_bounds_args block."""
     a = _lib.BoundsArgs()
     dim, batch, _ = _pages(a.cache, k_pages, k_pages, block_table, lengths, None, what)
-    ops._require_cuda(bounds, since)
+    ops._require_cuda(bounds)
     check_bounds(bounds, k_pages, k_pages.shape[0], k_pages.shape[1], dim, what)
+    a.batch, a.d, a.bounds = batch, dim, bounds.data_ptr()
+    ops._set3(a.bounds_strides, bounds.stride()[:3])
+    return a
+
+
+def _bounds(k_pages, block_table, lengths, bounds, since):
+    what = "paged_bounds"
+    a = bounds_block(k_pages, block_table, lengths, bounds, what)
+    ops._require_cuda(since)
     if since is not None:
         if since.dtype != torch.int32 or since.shape != lengths.shape or not since.is_contiguous() or since.device != lengths.device:
             raise ValueError("kohaku_tt_b200.paged_bounds: since must be a contiguous int32 [B]")
         a.since = since.data_ptr()
-    a.batch, a.d, a.bounds = batch, dim, bounds.data_ptr()
-    ops._set3(a.bounds_strides, bounds.stride()[:3])
     with torch.cuda.device(k_pages.device):
         _lib.check(_lib.lib().ktt_b200_paged_bounds(ctypes.byref(a), ops._stream(k_pages.device)), what)
 
@@ -97,7 +104,9 @@ def paged_bounds(k_pages, block_table, lengths, bounds=None, since=None):
     them, for the pages that hold the first lengths[b] keys of each sequence; a NaN among them stays one. Without bounds a new
     tensor, zero in all other pages; else it is written in place and returned. since (int32 [B] on the device): only the pages
     that keys since[b] .. lengths[b] - 1 lie in, of which the first keeps what its earlier keys left there. paged_append(bounds=)
-    does that on the way. Pages in bf16 or 4 bits."""
+    does that on the way. Bounds only ever widen, so those of a page that lost some of its keys (drafts that were not taken, a prompt cut
+    back) have to be made again from the page's first key: by paged_release(bounds=), or here with since at that key. Pages in
+    bf16 or 4 bits."""
     if bounds is None:
         dim = k_pages.shape[-1] if k_pages.dtype == torch.bfloat16 else k_pages.shape[-1] // 9 * 16
         bounds = k_pages.new_zeros((*k_pages.shape[:2], 2, dim), dtype=torch.bfloat16)

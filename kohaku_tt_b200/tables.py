@@ -6,6 +6,7 @@ import ctypes
 import torch
 
 from . import _lib, ops
+from .selection import bounds_block
 
 
 def _tables(block_table, lengths, free, count, page_size, count_out, what):
@@ -44,12 +45,20 @@ def _reserve(block_table, lengths, added, free, count, page_size, tokens, count_
     return cu, positions, slots, granted
 
 
-def _release(block_table, lengths, kept, free, count, page_size, count_out):
+def _release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds):
     what = "paged_release"
     a = _tables(block_table, lengths, free, count, page_size, count_out, what)
     _vector(kept, "kept", lengths, what)
+    if (k_pages is None) != (bounds is None):
+        raise ValueError("kohaku_tt_b200.paged_release: k_pages and bounds go together")
+    edges = None
+    if bounds is not None:
+        edges = bounds_block(k_pages, block_table, lengths, bounds, what)
+        if k_pages.shape[2] != page_size:
+            raise ValueError(f"kohaku_tt_b200.paged_release: pages of {k_pages.shape[2]} keys, and page_size {page_size}")
     with torch.cuda.device(block_table.device):
-        _lib.check(_lib.lib().ktt_b200_paged_release(ctypes.byref(a), kept.data_ptr(), ops._stream(block_table.device)), what)
+        _lib.check(_lib.lib().ktt_b200_paged_release_bounds(ctypes.byref(a), kept.data_ptr(), None if edges is None else ctypes.byref(edges),
+                                                            ops._stream(block_table.device)), what)
 
 
 @torch.library.custom_op("ktt_b200::_paged_reserve", mutates_args=("block_table", "count_out"), device_types="cuda")
@@ -64,14 +73,14 @@ def _(block_table, lengths, added, free, count, page_size, tokens, count_out):
     return lengths.new_empty((batch + 1,)), lengths.new_empty((tokens,)), lengths.new_empty((tokens,), dtype=torch.int64), lengths.new_empty((batch,))
 
 
-@torch.library.custom_op("ktt_b200::_paged_release", mutates_args=("block_table", "free", "count_out"), device_types="cuda")
+@torch.library.custom_op("ktt_b200::_paged_release", mutates_args=("block_table", "free", "count_out", "bounds"), device_types="cuda")
 def _release_op(block_table: torch.Tensor, lengths: torch.Tensor, kept: torch.Tensor, free: torch.Tensor, count: torch.Tensor, page_size: int,
-                count_out: torch.Tensor) -> None:
-    _release(block_table, lengths, kept, free, count, page_size, count_out)
+                count_out: torch.Tensor, k_pages: torch.Tensor | None, bounds: torch.Tensor | None) -> None:
+    _release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds)
 
 
 @_release_op.register_fake
-def _(block_table, lengths, kept, free, count, page_size, count_out):
+def _(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds):
     return None
 
 
@@ -100,15 +109,17 @@ def paged_reserve(block_table, lengths, added, free, count, page_size, tokens, c
     return _reserve(block_table, lengths, added, free, count, int(page_size), int(tokens), count_out)
 
 
-def paged_release(block_table, lengths, kept, free, count, page_size, count_out):
+def paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages=None, bounds=None):
     """Cuts sequences back to their first kept[b] keys (int32 [B] on the device; 0: the sequence has ended; lengths[b]: it goes on):
     the pages that hold none of those go to free[count:], sequence by sequence, and their entries of block_table become -1;
     count_out (int32 [1], another buffer than count) receives the new number. lengths are not changed: they are kept's from then on.
-    Entries that name no page give nothing back. A page that two sequences share must not be given back by both."""
+    Entries that name no page give nothing back. A page that two sequences share must not be given back by both.
+    k_pages, bounds: those of a cache with bounds (paged_bounds), which are made again, in a launch beside it, for the pages that
+    sequences are cut in: of the keys that are left there, so that later appends and selections know nothing of the others."""
     if torch.compiler.is_compiling():
-        torch.ops.ktt_b200._paged_release(block_table, lengths, kept, free, count, page_size, count_out)
+        torch.ops.ktt_b200._paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds)
         return
     eager = _lib.native()
-    if eager and eager.paged_release(block_table, lengths, kept, free, count, page_size, count_out):
+    if eager and eager.paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds):
         return
-    _release(block_table, lengths, kept, free, count, int(page_size), count_out)
+    _release(block_table, lengths, kept, free, count, int(page_size), count_out, k_pages, bounds)

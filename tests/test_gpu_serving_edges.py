@@ -186,3 +186,105 @@ def test_granted_compiled_and_captured(cuda):
     assert torch.equal(got, want) and torch.equal(captured, want)
     for a, b, c in zip(first, second, third):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# ---- sequences cut back inside a page -----------------------------------------------------------
+
+def _equal(got, want):
+    assert torch.equal(got.cpu().float().nan_to_num(7777.0), want.float().nan_to_num(7777.0))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 48)])
+@pytest.mark.parametrize("how", ["release", "since"])
+@pytest.mark.parametrize("odd", [False, True])
+def test_bounds_of_a_cut_back_cache(cuda, path, bits, d, page, how, odd):
+    """Drafts that were not taken leave nothing in the bounds, not even NaN: they are those made of the whole cache, after the cut and after
+    the appends behind it, of one row and of several, and so are the selections."""
+    hk, h, wide, batch, top = 2, 4, 7, 6, 3
+    lengths = [3 * page + 5, 2 * page, page + 1, 7, 5 * page - 1, 0]
+    drafts = 6
+    table = torch.randperm(batch * wide, generator=torch.Generator().manual_seed(1)).view(batch, wide).to(torch.int32)
+    kc = _x(batch * wide, hk, page, d, seed=2)
+    full = torch.full((batch * wide, hk, 2, d), 7.0, dtype=torch.bfloat16)
+    td, kp = table.to(cuda), _held(kc, bits).to(cuda)
+    vp, bounds = kp.clone(), so.bounds(_held(kc, bits), table, lengths, full).to(cuda)
+    free, left, count = _i32([0] * (batch * wide), cuda), _i32([0], cuda), _i32([0], cuda)
+
+    def append(k, have, n):
+        """k: [batch * n, hk, d]."""
+        after = _i32([0] * batch, cuda)
+        rows = k.view(batch, n, hk, d).transpose(1, 2).to(cuda)
+        ktt.paged_append(rows, rows, kp, vp, td, _i32(have, cuda), lengths_out=after, bounds=bounds)
+        got = so.append(kc, table, have, k.split(n), [n] * batch)
+        assert after.tolist() == got and (odd or torch.equal(kp.cpu(), _held(kc, bits)))
+        _equal(bounds, so.bounds(kp.cpu(), table, got, bounds.cpu()))
+        return got
+
+    bad = 0
+    have = lengths
+    for step, taken in enumerate(([0, 1, 2, 6, 5, 0], [9, -1, 6, 0, 3, 6], [6] * 6, [3, 0, 0, 1, 1, 5])):
+        k = _x(batch * drafts, hk, d, seed=10 + step) * 4
+        if odd:
+            k.view(batch, drafts, hk, d)[:, -1, :, 5::7] = float("nan")
+            k.view(batch, drafts, hk, d)[:, -2, 0, 3] = float("inf")
+        after = append(k, have, drafts)
+        kept = [n if t < 0 else min(n + t, a) for n, t, a in zip(have, taken, after)]
+        kept = [n - 3 if i == 1 and step == 2 and n > 3 else n for i, n in enumerate(kept)]      # a prompt cut back too
+        asked = [k + 5 if k == a else k for k, a in zip(kept, after)]                            # (past the length: it goes on)
+        before, held = bounds.cpu(), table.clone()
+        if how == "release":
+            ktt.paged_release(td, _i32(after, cuda), _i32(asked, cuda), free, count, page, left, k_pages=kp, bounds=bounds)
+            td.copy_(table)      # (the pages again, for the steps to come)
+        else:
+            ktt.paged_bounds(kp, td, _i32(kept, cuda), bounds=bounds, since=_i32(kept, cuda) // page * page)
+        assert torch.equal(table, held)
+        _equal(bounds, so.bounds(kp.cpu(), table, kept, before))
+        bad += int(before.isnan().sum()) > int(bounds.isnan().sum())
+        # (and of pages that are not cut nothing moved)
+        cut = {int(table[b, n // page]) for b, (n, a) in enumerate(zip(kept, after)) if n % page and n < a}
+        others = [i for i in range(batch * wide) if i not in cut]
+        _equal(bounds[others], before[others])
+        have = append(_x(batch, hk, d, seed=50 + step), kept, 1)
+        q = _x(batch, h, d, seed=70 + step)
+        chosen, keys = ktt.paged_select(q[:, :, None].to(cuda), bounds, td, _i32(have, cuda), page, top)
+        want, want_keys = so.select(q, bounds.cpu(), table, so.tokens([1] * batch, have, wide * page), page, top, 1, 1)
+        assert torch.equal(chosen.cpu(), want) and torch.equal(keys.cpu(), want_keys)
+    assert bool(bad) == odd
+
+
+def test_release_with_bounds_refusals(cuda, path):
+    kp = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16, device=cuda)
+    bounds = torch.zeros((4, 2, 2, 64), dtype=torch.bfloat16, device=cuda)
+    t, n, f, c, o = _i32([[0, 1]], cuda), _i32([20], cuda), _i32([0] * 4, cuda), _i32([0], cuda), _i32([0], cuda)
+    for kw, error in ((dict(k_pages=kp), ValueError), (dict(bounds=bounds), ValueError), (dict(k_pages=kp, bounds=bounds[:3]), ValueError), (dict(k_pages=kp, bounds=bounds.float()), ValueError),
+                      (dict(k_pages=torch.zeros((4, 2, 32, 64), dtype=torch.bfloat16, device=cuda), bounds=bounds), ValueError),
+                      (dict(k_pages=kp, bounds=bounds[:1].expand(4, 2, 2, 64)), _lib.UnsupportedAttention)):
+        with pytest.raises(error):
+            ktt.paged_release(t, n, _i32([3], cuda), f, c, 16, o, **kw)
+    torch.cuda.synchronize()
+    assert t.tolist() == [[0, 1]] and o.item() == 0      # (nothing was launched)
+
+
+def test_release_with_bounds_compiled_and_captured(cuda):
+    kp, table, n, kept = _x(8, 2, 16, 64, seed=1).to(cuda), _i32([[0, 1, 2], [3, 4, -1]], cuda), _i32([40, 20], cuda), _i32([21, 20], cuda)
+    base = ktt.paged_bounds(kp, table, n)
+
+    def fresh():
+        return table.clone(), base.clone(), _i32([9] * 8, cuda), _i32([-1], cuda)
+
+    def step(table, bounds, free, left):
+        ktt.paged_release(table, n, kept, free, _c, 16, left, k_pages=kp, bounds=bounds)
+        return left + 0
+
+    _c = _i32([0], cuda)
+    first, second, third = fresh(), fresh(), fresh()
+    step(*first)
+    assert first[3].item() == 1 and first[0].tolist() == [[0, 1, -1], [3, 4, -1]] and not torch.equal(first[1], base)
+    torch.compile(step, fullgraph=True)(*second)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*third)
+    graph.replay()
+    for a, b, c in zip(first, second, third):
+        assert torch.equal(a, b) and torch.equal(a, c)

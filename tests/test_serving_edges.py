@@ -37,3 +37,36 @@ def test_append_by_hand():
     rows = [torch.tensor([1.0, 2.0, 3.0]).view(3, 1, 1), torch.tensor([4.0]).view(1, 1, 1)]
     assert so.append(pages, torch.tensor([[2, 0], [1, -1]]), [15, 3], rows, [2, 0]) == [17, 3]
     assert pages[2, 0, 15] == 1 and pages[0, 0, 0] == 2 and pages.abs().sum() == 3
+
+
+def _tables(**kw):
+    a = _lib.Tables()
+    a.batch, a.table_width, a.page_size, a.table_stride, a.pool = 2, 4, 16, 4, 8
+    a.block_table = a.lengths = a.free_pages = a.count = 4096
+    a.count_out = 8192
+    for name, x in kw.items():
+        setattr(a, name, x)
+    return a
+
+
+def _bounds(strides=(256, 128, 64), **kw):
+    b = _lib.BoundsArgs(cache=_append().base.cache)
+    b.batch, b.d, b.bounds = 2, 64, 4096
+    for i, x in enumerate(strides):
+        b.bounds_strides[i] = x
+    for name, x in kw.items():
+        setattr(b if name in ("batch", "d", "bounds") else b.cache, name, x)
+    return b
+
+
+def test_release_with_bounds_refusals(built_lib):
+    """What is not of the same table is refused, and so is what either half refuses."""
+    for kw in (dict(batch=1), dict(page_size=32), dict(table_width=3), dict(block_table=8192), dict(lengths=8192), dict(table_stride=5), dict(max_keys=32)):
+        assert built_lib.ktt_b200_paged_release_bounds(ctypes.byref(_tables()), 4096, ctypes.byref(_bounds(**kw)), None) == _lib.ERR_BAD_ARGUMENT, kw
+        assert "same table" in _lib.last_error()
+    for kw, status in ((dict(bounds=None), _lib.ERR_BAD_ARGUMENT), (dict(bounds=4104), _lib.ERR_UNSUPPORTED), (dict(d=96), _lib.ERR_UNSUPPORTED), (dict(strides=(0, 128, 64)), _lib.ERR_UNSUPPORTED)):
+        assert built_lib.ktt_b200_paged_release_bounds(ctypes.byref(_tables()), 4096, ctypes.byref(_bounds(**kw)), None) == status
+    for kw, status in ((dict(batch=4097), _lib.ERR_UNSUPPORTED), (dict(count_out=4096), _lib.ERR_BAD_ARGUMENT)):
+        assert built_lib.ktt_b200_paged_release_bounds(ctypes.byref(_tables(**kw)), 4096, ctypes.byref(_bounds()), None) == status
+    assert built_lib.ktt_b200_paged_release_bounds(ctypes.byref(_tables()), None, ctypes.byref(_bounds()), None) == _lib.ERR_BAD_ARGUMENT
+    assert built_lib.ktt_b200_paged_release_bounds(None, 4096, ctypes.byref(_bounds()), None) == _lib.ERR_BAD_ARGUMENT
