@@ -57,6 +57,15 @@ def _require_cuda(*tensors):
             )
 
 
+def watched(*tensors):
+    """Whether something wants to see the call as an operator: a graph that is compiled, a dispatch mode (fake tensors, tracing), or tensors that
+    handle operators themselves."""
+    if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0:
+        return True
+    plain = torch.Tensor.__torch_dispatch__
+    return any(isinstance(t, torch.Tensor) and type(t).__torch_dispatch__ is not plain for t in tensors)
+
+
 def _rows_contiguous(t):
     """`t` with a unit innermost stride (head views pass through untouched)."""
     return t if t.stride(-1) == 1 else t.contiguous()

@@ -86,6 +86,11 @@ def _on_device(cu):
     return cu is None or (isinstance(cu, torch.Tensor) and cu.is_cuda)
 
 
+def operator_offsets(cu, batch, rows, like, what):
+    """Offsets as an operator takes them, on the device; as they are in a compiled graph."""
+    return cu if torch.compiler.is_compiling() or _on_device(cu) else _offsets(cu, batch, rows, like.device, what)[0]
+
+
 def check_bounds(bounds, like, pages, hk, dim, what):
     """The rules of a cache's bounds."""
     if tuple(bounds.shape) != (pages, hk, 2, dim) or bounds.dtype != torch.bfloat16 or bounds.device != like.device:
@@ -342,7 +347,8 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     Pages of 4 bits (paged_cache(bits=4)) hold each 64 channels of a row as codes 0 to 15 of
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
     interleaved = bool(interleaved)
-    if torch.compiler.is_compiling():
+    if ops.watched(k, v, k_pages, v_pages, block_table, lengths, q):
+        cu_seq = operator_offsets(cu_seq, block_table.shape[0], k.shape[0], k_pages, "paged_append")
         if positions is None and axes is None and bounds is None and granted is None:
             out = torch.ops.ktt_b200._paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out)
         else:
@@ -363,7 +369,7 @@ def paged_read(k_pages, v_pages, block_table, lengths, max_k=None):
     """(k, v), bf16 [B, Hk, capacity, D]: the first lengths[b] keys and values of each sequence out of its
     pages, as their values where the pages hold 4 bits; zeros behind them and where there is no page.
     capacity: block_table's, or max_k where that is less."""
-    if torch.compiler.is_compiling():
+    if ops.watched(k_pages, v_pages, block_table, lengths):
         return torch.ops.ktt_b200._paged_read(k_pages, v_pages, block_table, lengths, max_k)
     eager = _lib.native()
     if eager:
@@ -395,7 +401,7 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
     if block_table.dim() == 3:
         if cu_seq_q is not None or max_q is not None:
             raise ValueError("kohaku_tt_b200.sdpa_paged: with a table for each token there are no offsets")
-        if torch.compiler.is_compiling():
+        if ops.watched(q, k_pages, v_pages, block_table, lengths):
             return torch.ops.ktt_b200._sdpa_paged_chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
         eager = _lib.native()
         if eager:
@@ -404,7 +410,12 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
                 return out
         with torch.no_grad():
             return _chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
-    if torch.compiler.is_compiling():
+    if ops.watched(q, k_pages, v_pages, block_table, lengths):
+        if not torch.compiler.is_compiling() and not _on_device(cu_seq_q):
+            cu_seq_q, longest = _offsets(cu_seq_q, block_table.shape[0], q.shape[0], q.device, "sdpa_paged")
+            if max_q is not None and max_q < longest:
+                raise ValueError("kohaku_tt_b200.sdpa_paged: max_q is less than the longest sequence")
+            max_q = longest if max_q is None else max_q
         return torch.ops.ktt_b200._sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
     eager = _lib.native()
     if eager and _on_device(cu_seq_q):

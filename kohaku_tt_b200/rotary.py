@@ -289,7 +289,7 @@ def rotary(q, k, cos, sin, positions=None, interleaved=False, axes=None):
     if axes is not None:
         axes = pair_axes(axes, cos.shape[-1], "rotary")
     _check(q, k, cos, sin, positions, axes)
-    if torch.compiler.is_compiling():
+    if ops.watched(q, k, cos, sin, positions):
         if axes is None:
             out = torch.ops.ktt_b200._rotary(q, k, cos, sin, positions, interleaved, False)
         else:

@@ -99,7 +99,7 @@ def paged_reserve(block_table, lengths, added, free, count, page_size, tokens, c
     for `tokens` rows (the sum of added; 0: not wanted), positions int32, lengths[b] + i, and slots int64, page * page_size + row in the
     page, which is where the token's row lies in a buffer [pages * page_size, ...]; -1 in rows behind the last sequence's, and
     in the slots of sequences that were granted nothing. At most 4096 sequences."""
-    if torch.compiler.is_compiling():
+    if ops.watched(block_table, lengths, added, free, count):
         return torch.ops.ktt_b200._paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out)
     eager = _lib.native()
     if eager:
@@ -116,7 +116,7 @@ def paged_release(block_table, lengths, kept, free, count, page_size, count_out,
     Entries that name no page give nothing back. A page that two sequences share must not be given back by both.
     k_pages, bounds: those of a cache with bounds (paged_bounds), which are made again, in a launch beside it, for the pages that
     sequences are cut in: of the keys that are left there, so that later appends and selections know nothing of the others."""
-    if torch.compiler.is_compiling():
+    if ops.watched(block_table, lengths, kept, free, count):
         torch.ops.ktt_b200._paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds)
         return
     eager = _lib.native()

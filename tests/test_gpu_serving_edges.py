@@ -288,3 +288,55 @@ def test_release_with_bounds_compiled_and_captured(cuda):
     graph.replay()
     for a, b, c in zip(first, second, third):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+# ---- modes that watch operators -----------------------------------------------------------------
+
+def test_a_mode_sees_the_operators(cuda):
+    """Under a dispatch mode each entry is its operator, with the eager call's results; a rotation has its gradients there, and theirs."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        def __init__(self):
+            super().__init__()
+            self.names = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.names.append(str(func))
+            return func(*args, **(kwargs or {}))
+
+    b, h, hk, d, page, wide, t = 3, 8, 2, 64, 16, 4, 9
+    q, k, v = _x(t, h, d, seed=1).to(cuda), _x(t, hk, d, seed=2).to(cuda), _x(t, hk, d, seed=3).to(cuda)
+    cos, sin = ktt.rotary_table(wide * page, d, device=cuda)
+    axes, offsets = tuple(i % 3 for i in range(d // 2)), [0, 4, 4, 9]
+
+    def step():
+        kp, vp = ktt.paged_cache(12, hk, page, d, device=cuda)
+        table, lens, after = torch.full((b, wide), -1, dtype=torch.int32, device=cuda), _i32([0] * b, cuda), _i32([0] * b, cuda)
+        free, count, left = torch.arange(12, dtype=torch.int32, device=cuda), _i32([12], cuda), _i32([0], cuda)
+        bounds = torch.zeros((12, hk, 2, d), dtype=torch.bfloat16, device=cuda)
+        cu, at, slots, granted = ktt.paged_reserve(table, lens, _i32([4, 0, 5], cuda), free, count, page, t, left)
+        turned = ktt.paged_append(k, v, kp, vp, table, lens, cos, sin, q=q, cu_seq=offsets, lengths_out=after, positions=at.expand(3, t), axes=axes, bounds=bounds, granted=granted)
+        ktt.paged_append(k, v, kp, vp, table, after, cu_seq=cu)
+        again = ktt.paged_bounds(kp, table, after)
+        chosen, keys = ktt.paged_select(turned, bounds, table, after, page, 2, cu_seq_q=offsets)
+        outs = ktt.sdpa_paged(turned, kp, vp, chosen, keys), ktt.sdpa_paged(turned, kp, vp, table, after, cu_seq_q=offsets), *ktt.paged_read(kp, vp, table, after)
+        ktt.paged_release(table, after, _i32([0, 0, 2], cuda), free, left, page, count, k_pages=kp, bounds=bounds)
+        return cu, at, slots, granted, turned, again, chosen, keys, *outs, table, free, count, left, after, bounds, kp, vp
+
+    def gradients():
+        x, y, w = (z.clone().requires_grad_() for z in (q, k, q))
+        a, c = ktt.rotary(x, y, cos, sin, positions=torch.arange(t, device=cuda).expand(3, t), axes=axes)
+        (g,) = torch.autograd.grad((a * w).sum() + c.sum(), x, create_graph=True)
+        return a, c, g, torch.autograd.grad(g.sum(), w)[0], ktt.rotary(x, None, cos, sin, interleaved=True)[0]
+
+    want = step() + gradients()
+    with Seen() as seen:
+        got = step() + gradients()
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    for name in ("_paged_reserve", "_paged_append_at", "_paged_append", "_paged_select", "_sdpa_paged_chosen", "_sdpa_paged", "_paged_bounds", "_paged_read", "_paged_release", "_rotary",
+                 "_rotary_axes"):
+        assert f"ktt_b200.{name}.default" in seen.names, name
+    with Seen(), pytest.raises(ValueError, match="longest"):
+        ktt.sdpa_paged(q, *ktt.paged_cache(2, hk, page, d, device=cuda), _i32([[0], [1], [1]], cuda), _i32([1, 1, 1], cuda), cu_seq_q=offsets, max_q=2)

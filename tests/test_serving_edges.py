@@ -70,3 +70,54 @@ def test_release_with_bounds_refusals(built_lib):
         assert built_lib.ktt_b200_paged_release_bounds(ctypes.byref(_tables(**kw)), 4096, ctypes.byref(_bounds()), None) == status
     assert built_lib.ktt_b200_paged_release_bounds(ctypes.byref(_tables()), None, ctypes.byref(_bounds()), None) == _lib.ERR_BAD_ARGUMENT
     assert built_lib.ktt_b200_paged_release_bounds(None, 4096, ctypes.byref(_bounds()), None) == _lib.ERR_BAD_ARGUMENT
+
+
+def test_fake_tensors_reach_the_fake_operators():
+    """Under FakeTensorMode nothing reads a pointer: each entry gives what its operator says of shapes and types, traced or not."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    import kohaku_tt_b200 as ktt
+
+    b, h, hk, d, page, wide, pool, t, top = 3, 8, 2, 64, 16, 20, 50, 9, 4
+
+    def step(q, k, v, kp, vp, bounds, table, lengths, added, free, count, left, after, cos, sin):
+        cu, at, slots, granted = ktt.paged_reserve(table, lengths, added, free, count, page, t, left)
+        turned = ktt.paged_append(k, v, kp, vp, table, lengths, cos, sin, q=q, cu_seq=cu, lengths_out=after, positions=at.expand(3, t), axes=tuple(i % 3 for i in range(d // 2)),
+                                  bounds=bounds, granted=granted)
+        plain = ktt.paged_append(k, v, kp, vp, table, lengths, q=q, cu_seq=[0, 4, 4, 9])
+        assert ktt.paged_append(k, v, kp, vp, table, lengths, cu_seq=[0, 4, 4, 9]) is None
+        chosen, keys = ktt.paged_select(turned, bounds, table, after, page, top, cu_seq_q=cu)
+        other, _ = ktt.paged_select(turned, bounds, table, after, page, top, cu_seq_q=[0, 4, 4, 9])
+        out = ktt.sdpa_paged(turned, kp, vp, chosen, keys)
+        every = ktt.sdpa_paged(turned, kp, vp, table, after, cu_seq_q=[0, 4, 4, 9])
+        again = ktt.paged_bounds(kp, table, after)
+        dense = ktt.paged_read(kp, vp, table, after, max_k=100)
+        ktt.paged_release(table, after, lengths, free, left, page, count, k_pages=kp, bounds=bounds)
+        r = ktt.rotary(q, k, cos, sin, positions=at)
+        s = ktt.rotary(q, None, cos, sin, positions=at.expand(3, t), axes=tuple(i % 3 for i in range(d // 2)))
+        return cu, at, slots, granted, turned, plain, chosen, keys, other, out, every, again, *dense, *r, s[0]
+
+    def bf16(*shape):
+        return torch.empty(shape, dtype=torch.bfloat16, device="cuda")
+
+    def i32(*shape):
+        return torch.empty(shape, dtype=torch.int32, device="cuda")
+
+    with FakeTensorMode() as mode:
+        args = (bf16(t, h, d), bf16(t, hk, d), bf16(t, hk, d), bf16(pool, hk, page, d), bf16(pool, hk, page, d), bf16(pool, hk, 2, d), i32(b, wide), i32(b), i32(b), i32(pool), i32(1), i32(1),
+                i32(b), torch.empty((wide * page, d // 2), device="cuda"), torch.empty((wide * page, d // 2), device="cuda"))
+        got = step(*args)
+    want = [((b + 1,), torch.int32), ((t,), torch.int32), ((t,), torch.int64), ((b,), torch.int32), ((t, h, d), torch.bfloat16), ((t, h, d), torch.bfloat16), ((t, hk, top), torch.int32),
+            ((t, hk), torch.int32), ((t, hk, top), torch.int32), ((t, h, d), torch.bfloat16), ((t, h, d), torch.bfloat16), ((pool, hk, 2, d), torch.bfloat16), ((b, hk, 100, d), torch.bfloat16),
+            ((b, hk, 100, d), torch.bfloat16), ((t, h, d), torch.bfloat16), ((t, hk, d), torch.bfloat16), ((t, h, d), torch.bfloat16)]
+    assert [(tuple(x.shape), x.dtype) for x in got] == want and all(x.device.type == "cuda" for x in got)
+    # Outside of the mode too, as the tensors themselves are fake; and a traced graph has every operator.
+    chosen, keys = ktt.paged_select(got[4], args[5], args[6], args[12], page, top, cu_seq_q=got[0])
+    assert chosen.fake_mode is mode and tuple(chosen.shape) == (t, hk, top)
+    with mode:
+        graph = make_fx(step)(*args)
+    names = {str(n.target) for n in graph.graph.nodes if n.op == "call_function"}
+    for name in ("_paged_reserve", "_paged_append_at", "_paged_append", "_paged_select", "_sdpa_paged_chosen", "_sdpa_paged", "_paged_bounds", "_paged_read", "_paged_release", "_rotary",
+                 "_rotary_axes"):
+        assert f"ktt_b200.{name}.default" in names, (name, names)
