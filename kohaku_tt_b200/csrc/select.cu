@@ -11,6 +11,8 @@
 // alternating and wide-ranging values: 2^-22 of it). So the value of the last page selected lies within e of the last by fp32: pages more than
 // 2 e above or below are in or out, and those between, one or a few, get their scores in 64 bits where they are not all in. Bounds whose
 // least value is above the largest select some pages or others, of those there are.
+#include <algorithm>
+#include <cstdlib>
 #include <type_traits>
 
 #include "four_bits.cuh"
@@ -27,8 +29,18 @@ const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3]) {
     return reinterpret_cast<uintptr_t>(at) & 15 ? "bounds must be 16-byte aligned" : nullptr;
 }
 const char* bounds_of(Bounds& b, void* at, const int64_t (&strides)[3], const Pages& c, int kv_heads, int d) {
-    auto apart = [d](int64_t stride) { return stride >= d || stride <= -d; };
-    if ((c.pages > 1 && !apart(strides[0])) || (kv_heads > 1 && !apart(strides[1])) || !apart(strides[2])) return "bounds that are written must not lie on one another";
+    // Rows of d values are apart where each stride, from the least on, is as far as all that lies below it. (Layouts whose parts lie between one
+    // another's without touching are refused too.)
+    struct Dim {
+        int64_t stride, count;
+    } dims[3] = {{std::abs(strides[0]), c.pages}, {std::abs(strides[1]), kv_heads}, {std::abs(strides[2]), 2}};
+    std::sort(dims, dims + 3, [](const Dim& x, const Dim& y) { return x.stride < y.stride; });
+    __int128 below = d;   // values from the first to behind the last of all smaller strides
+    for (const Dim& x : dims) {
+        if (x.count == 1) continue;
+        if (x.stride < below) return "bounds that are written must not lie on one another";
+        below += static_cast<__int128>(x.stride) * (x.count - 1);
+    }
     return bounds_of(b, at, strides);
 }
 

@@ -340,3 +340,21 @@ def test_a_mode_sees_the_operators(cuda):
         assert f"ktt_b200.{name}.default" in seen.names, name
     with Seen(), pytest.raises(ValueError, match="longest"):
         ktt.sdpa_paged(q, *ktt.paged_cache(2, hk, page, d, device=cuda), _i32([[0], [1], [1]], cuda), _i32([1, 1, 1], cuda), cu_seq_q=offsets, max_q=2)
+
+
+# ---- bounds that lie on one another -------------------------------------------------------------
+
+def test_written_bounds_on_one_another(cuda, path):
+    """Refused where they are written, by strides against each other; read they may be."""
+    kp, table, n = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16, device=cuda), _i32([[0, 1, 2, 3]], cuda), _i32([50], cuda)
+    row, q = torch.zeros((1, 2, 1, 64), dtype=torch.bfloat16, device=cuda), torch.ones((1, 4, 1, 64), dtype=torch.bfloat16, device=cuda)
+    memory = torch.zeros(4096, dtype=torch.bfloat16, device=cuda)
+    for strides in ((64, 64, 64), (128, 64, 64), (64, 128, 64), (256, 64, 64), (64, 256, 128)):
+        bad = memory.as_strided((4, 2, 2, 64), (*strides, 1))
+        for call in (lambda: ktt.paged_bounds(kp, table, n, bounds=bad), lambda: ktt.paged_append(row, row, kp, kp, table, n, bounds=bad),
+                     lambda: ktt.paged_release(table, n, n, _i32([0] * 4, cuda), _i32([0], cuda), 16, _i32([0], cuda), k_pages=kp, bounds=bad)):
+            with pytest.raises(_lib.UnsupportedAttention, match="on one another"):
+                call()
+        ktt.paged_select(q, bad, table, n, 16, 2)
+    good = memory.as_strided((4, 2, 2, 64), (128, 512, 64, 1))
+    assert torch.equal(ktt.paged_bounds(kp + 1, table, n, bounds=good), torch.ones_like(good))

@@ -121,3 +121,25 @@ def test_fake_tensors_reach_the_fake_operators():
     for name in ("_paged_reserve", "_paged_append_at", "_paged_append", "_paged_select", "_sdpa_paged_chosen", "_sdpa_paged", "_paged_bounds", "_paged_read", "_paged_release", "_rotary",
                  "_rotary_axes"):
         assert f"ktt_b200.{name}.default" in names, (name, names)
+
+
+def test_written_bounds_that_lie_on_one_another(built_lib):
+    """Strides against each other, not each alone; layouts whose rows are apart pass (they are refused for a batch of none, behind this check)."""
+    def status(strides, pages=4, kv_heads=2, d=64):
+        b = _bounds(strides=strides, pages=pages, kv_heads=kv_heads, d=d)
+        b.batch = 70000
+        first = built_lib.ktt_b200_paged_bounds(ctypes.byref(b), None)
+        assert first == _lib.ERR_UNSUPPORTED and "65535" in _lib.last_error()
+        x = _append(batch=70000, d=d)      # (the number of sequences is checked after the bounds there)
+        x.bounds, x.base.cache.pages, x.base.cache.kv_heads = 4096, pages, kv_heads
+        for i, s in enumerate(strides):
+            x.bounds_strides[i] = s
+        assert built_lib.ktt_b200_paged_append_at(ctypes.byref(x), None) == _lib.ERR_UNSUPPORTED
+        return "on one another" in _lib.last_error()
+
+    for strides in ((64, 64, 64), (128, 64, 64), (64, 128, 64), (192, 128, 64), (256, 64, 64), (256, 128, 120), (64, 256, 128), (0, 128, 64), (256, 128, 0), (-128, 128, 64),
+                    (128, 256, -128), (2 ** 62, 2 ** 62, 64)):
+        assert status(strides), strides
+    for strides in ((256, 128, 64), (64, 512, 256), (128, 512, 64), (256, 64, 128), (-256, 128, -64), (4096, 64, 1024), (2 ** 62, 128, 64), (2 ** 62, 2 ** 61, 64)):
+        assert not status(strides), strides
+    assert not status((0, 128, 64), pages=1) and not status((128, 0, 64), kv_heads=1) and status((128, 0, 64), kv_heads=2) and status((100, 128, 64), pages=2)
