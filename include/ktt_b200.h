@@ -490,8 +490,8 @@ KTT_B200_API int ktt_b200_paged_release_bounds(const ktt_b200_tables* args, cons
 
 /* The `top` pages of its sequence that each query token goes to, for each K / V head: the first `first`, the last `last` (first + last
  * <= top, last >= 1), and of the others those of the largest score, ties to the lower place. A page's score is the largest logit that a key
- * between its bounds could have, over the queries q_h of the head's group: max_h sum_d max(q_hd least_d, q_hd largest_d), of which the exact
- * value decides; one that is no number counts as infinite, that of an entry that names no page as 0. q dense [B, H, sq, D] or packed
+ * between its bounds could have, over the queries q_h of the head's group: max_h sum_d max(q_hd least_d, q_hd largest_d), in 64 bits
+ * (exact where the products that are not 0 lie within a factor of 2^30 of one another); one that is no number counts as infinite, that of an entry that names no page as 0. q dense [B, H, sq, D] or packed
  * [total_q, H, D] (cu_seqlens_q); lengths count the keys with those of the call's own tokens, and query i of n sees keys
  * 0 .. length - n + i, and the pages these lie in. chosen int32 [tokens][kv_heads][top]: the pages' names in the order of their places, -1 behind
  * them; keys int32 [tokens][kv_heads]: how many keys they hold that the token sees (0: none). Tokens: batch * sq, or total_q. */

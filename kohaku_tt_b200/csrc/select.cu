@@ -5,7 +5,9 @@
 // so the scores of all pages are two matrix products with the queries of a K / V head's group as columns. Bound: the reading of the
 // bounds, 4 D bytes a page and head (1 / P of the cache in bf16, for pages of P keys).
 //
-// What is selected is decided by the exact scores, so that it does not depend on an order of summation. The products of bf16 values are exact
+// What is selected is decided by scores in 64 bits: exact, and so of no order of summation, where the products of a head and page that are not 0
+// lie within a factor of 2^30 of one another (multiples of 2^-15 of the least one's power of two, 128 of which are under 2^53 of these), else summed in one
+// fixed order with a rounding of 2^-53 at each addition. The products of bf16 values are exact
 // in fp32; a score is the sum of four sums of up to 4 matrix instructions each, of which every one is off by 2^-22 of the magnitudes that it
 // adds up at most (two bits more than a sum of fp32 rounds by), all in all by e = 2^-19 max_h sum_d |q_hd| max |bound| (measured, over equal,
 // alternating and wide-ranging values: 2^-22 of it). So the value of the last page selected lies within e of the last by fp32: pages more than
@@ -386,7 +388,7 @@ __device__ __forceinline__ int sum_before(int x, int* warps, int& all) {
 __device__ __forceinline__ void to_first(uint32_t at, float x) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(x) : "memory"); }
 __device__ __forceinline__ void to_first(uint32_t at, int x) { asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); }
 
-// The exact score of a page: 64-bit sums of products that are exact themselves. By one warp, a lane D / 32 neighbouring channels; eight heads at a
+// The score of a page in 64 bits: sums of products that are exact themselves. By one warp, a lane D / 32 neighbouring channels; eight heads at a
 // time, whose sums over the lanes halve the heads of a lane before its lanes.
 template <int D>
 __device__ __forceinline__ double exact_score(const SelectParams& p, const Token& tok, int hk, int64_t page) {

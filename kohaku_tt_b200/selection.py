@@ -129,7 +129,8 @@ def paged_select(q, bounds, block_table, lengths, page_size, top, first=1, last=
     least: its own key is there), and those with the largest scores, `top` in all (or all, where there are no more). The score of a page is the
     largest logit that a key between its bounds (paged_bounds) could have with any query of the head's group,
         max over h of the sum over d of max(q[h, d] least[d], q[h, d] largest[d]),
-    and the exact value decides; ties go to the page that comes first. A score that is no number counts as infinite; an entry of
+    in 64 bits, which is exact where the products that are not 0 lie within a factor of 2^30 of one another (else each of the sum's additions
+    rounds by 2^-53); ties go to the page that comes first. A score that is no number counts as infinite; an entry of
     block_table that names no page has score 0. (Where a least value is above the largest, as in a tensor that nothing was written to,
     it is not said which pages.)
     chosen int32 [tokens, Hk, top]: names of pages in the order of their places, -1 behind them. keys int32 [tokens, Hk]: the keys of

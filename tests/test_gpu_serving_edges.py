@@ -358,3 +358,43 @@ def test_written_bounds_on_one_another(cuda, path):
         ktt.paged_select(q, bad, table, n, 16, 2)
     good = memory.as_strided((4, 2, 2, 64), (128, 512, 64, 1))
     assert torch.equal(ktt.paged_bounds(kp + 1, table, n, bounds=good), torch.ones_like(good))
+
+
+# ---- scores that are equal ----------------------------------------------------------------------
+
+def _first_by_score(q, edge, table, top):
+    """Places of the pages between the first and the last, of the largest scores in whole numbers; bounds that are one edge [pages, d], and all values
+    multiples of 2^-40."""
+    scores = []
+    for name in table:
+        page = [int(x) for x in (edge[name].double() * 2 ** 40).tolist()]
+        scores.append(max(sum(int(a) * b for a, b in zip(row, page)) for row in (q.double() * 2 ** 20).tolist()))
+    rest = sorted(range(1, len(table) - 1), key=lambda e: (-scores[e], e))[:top - 2]
+    return [int(table[e]) for e in sorted(rest + [0, len(table) - 1])]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("wide", [60, 200, 700, 9000])
+def test_equal_scores_in_any_order_of_channels(cuda, d, wide):
+    """Pages whose products are the same numbers in other channels, over a factor of almost 2^30, have equal scores and go by place; one that is
+    larger by the least product goes first. Against sums in whole numbers."""
+    page, top, h = 16, 30, 3
+    g = torch.Generator().manual_seed(wide + d)
+    q = torch.tensor([1.0, -0.5, 0.25])[:, None].expand(h, d).mul(1.0 + 27 / 128).to(torch.bfloat16)      # a head's channels alike: 8 bits each
+    size = 2.0 ** -torch.arange(d).remainder(28) * (1 + torch.randint(0, 128, (d,), generator=g) / 128)
+    base = (size * torch.randint(0, 2, (d,), generator=g).mul(2).sub(1)).to(torch.bfloat16)
+    edge = torch.stack([base[torch.randperm(d, generator=g)] for _ in range(wide)])
+    table = torch.randperm(wide, generator=g).to(torch.int32)
+    for some in ([], range(5, wide - 1, 7), [wide // 2], range(1, wide - 1, 2)):
+        values = edge.clone()
+        least = base.float().abs().min()
+        for e in some:      # the least magnitude's sign turned where it is negative, else twice as large: a score that is a little larger
+            row = values[table[e].item()]
+            i = int((row.float().abs() == least).nonzero()[0])
+            row[i] = row[i].abs() if row[i] < 0 else row[i] * 2
+        want = _first_by_score(q, values, table.tolist(), top)
+        bounds = values[:, None, None].expand(wide, 1, 2, d).contiguous().to(cuda)
+        chosen, keys = ktt.paged_select(q.view(1, h, 1, d).to(cuda), bounds, table[None].to(cuda), _i32([wide * page], cuda), page, top)
+        assert chosen[0, 0].tolist() == want and keys.item() == top * page
+        if not some:
+            assert want == table[:top - 1].tolist() + table[-1:].tolist()
