@@ -57,6 +57,14 @@ def _require_cuda(*tensors):
             )
 
 
+def int32(x, name, what):
+    """A whole number as an argument block holds it (which would drop the bits past 32)."""
+    x = int(x)
+    if not -(2 ** 31) <= x < 2 ** 31:
+        raise _lib.UnsupportedAttention(f"kohaku_tt_b200.{what}: {name} must fit 32 bits, got {x}")
+    return x
+
+
 def watched(*tensors):
     """Whether something wants to see the call as an operator: a graph that is compiled, a dispatch mode (fake tensors, tracing), or tensors that
     handle operators themselves."""

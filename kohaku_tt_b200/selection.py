@@ -50,7 +50,7 @@ def _select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq
     if q.dtype != torch.bfloat16 or q.shape[-1] != dim or (not packed and q.shape[0] != batch):
         raise ValueError(f"kohaku_tt_b200.paged_select: q must be bf16, of {dim} columns and the table's sequences, got {q.dtype} {list(q.shape)}")
     rows = q.shape[0] if packed else q.shape[2]
-    if rows >= 2 ** 31 or q.shape[1] > 65535:
+    if rows >= 2 ** 31 or q.shape[1] > 65535 or hk > 4096:
         raise _lib.UnsupportedAttention("kohaku_tt_b200.paged_select: more rows or heads than the kernels count")
     if q.stride(-1) != 1 or q.data_ptr() % 16 or any(x % 8 for x in q.stride()[:-1]):
         q = q.clone(memory_format=torch.contiguous_format)
@@ -61,8 +61,8 @@ def _select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq
             cu, _ = _offsets(cu_seq_q, batch, rows, q.device, what)
             a.cu_seqlens_q, a.total_q = cu.data_ptr(), rows
         a.batch, a.heads, a.kv_heads, a.sq, a.d = batch, q.shape[1], hk, 0 if packed else rows, dim
-        a.page_size, a.table_width, a.pages, a.block_table, a.table_stride = page_size, block_table.shape[1], pages, block_table.data_ptr(), block_table.stride(0)
-        a.lengths, a.top, a.first, a.last = lengths.data_ptr(), top, first, last
+        a.page_size, a.table_width, a.pages, a.block_table, a.table_stride = ops.int32(page_size, "page_size", what), block_table.shape[1], pages, block_table.data_ptr(), block_table.stride(0)
+        a.lengths, a.top, a.first, a.last = lengths.data_ptr(), *(ops.int32(x, name, what) for x, name in ((top, "top"), (first, "first"), (last, "last")))
         a.q, a.bounds = q.data_ptr(), bounds.data_ptr()
         ops._set3(a.q_strides, (ops._ths_strides if packed else ops._bhs_strides)(q))
         ops._set3(a.bounds_strides, bounds.stride()[:3])
@@ -70,7 +70,7 @@ def _select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq
         if need < 0:
             _lib.check(_lib.ERR_UNSUPPORTED, what)
         tokens = rows if packed else batch * rows
-        chosen, keys = lengths.new_empty((tokens, hk, top)), lengths.new_empty((tokens, hk))
+        chosen, keys = lengths.new_empty((tokens, hk, a.top)), lengths.new_empty((tokens, hk))
         work = torch.empty((max(need, 16),), dtype=torch.uint8, device=q.device)
         a.chosen, a.keys, a.workspace, a.workspace_bytes = chosen.data_ptr(), keys.data_ptr(), work.data_ptr(), work.numel()
         _lib.check(_lib.lib().ktt_b200_paged_select(ctypes.byref(a), ops._stream(q.device)), what)

@@ -19,7 +19,7 @@ def _tables(block_table, lengths, free, count, page_size, count_out, what):
         if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != block_table.device:
             raise ValueError(f"kohaku_tt_b200.{what}: {name} must be a contiguous int32 {list(shape)} on the table's device")
     a = _lib.Tables()
-    a.batch, a.table_width, a.page_size = batch, block_table.shape[1], int(page_size)
+    a.batch, a.table_width, a.page_size = batch, block_table.shape[1], ops.int32(page_size, "page_size", what)
     a.block_table, a.table_stride, a.lengths = block_table.data_ptr(), block_table.stride(0), lengths.data_ptr()
     a.free_pages, a.pool, a.count, a.count_out = free.data_ptr(), free.numel(), count.data_ptr(), count_out.data_ptr()
     return a

@@ -398,3 +398,23 @@ def test_equal_scores_in_any_order_of_channels(cuda, d, wide):
         assert chosen[0, 0].tolist() == want and keys.item() == top * page
         if not some:
             assert want == table[:top - 1].tolist() + table[-1:].tolist()
+
+
+# ---- whole numbers past 32 bits -----------------------------------------------------------------
+
+def test_numbers_past_32_bits_are_refused(cuda, path):
+    """An argument block would hold what is left of them: pages of 2^32 + 16 keys were pages of 16."""
+    far = 2 ** 32
+    t, n, f, c, o = _i32([[0, 1]], cuda), _i32([20], cuda), _i32([0] * 4, cuda), _i32([0], cuda), _i32([0], cuda)
+    q, bounds = torch.ones((1, 4, 1, 64), dtype=torch.bfloat16, device=cuda), torch.zeros((4, 2, 2, 64), dtype=torch.bfloat16, device=cuda)
+    for page in (far + 16, 16 - far):
+        for call in (lambda: ktt.paged_reserve(t, n, n, f, c, page, 1, o), lambda: ktt.paged_release(t, n, n, f, c, page, o), lambda: ktt.paged_select(q, bounds, t, n, page, 2)):
+            with pytest.raises(_lib.UnsupportedAttention, match="32 bits"):
+                call()
+    for kw in (dict(top=far + 2), dict(top=2, first=far), dict(top=2, last=far + 1)):
+        with pytest.raises(_lib.UnsupportedAttention, match="32 bits"):
+            ktt.paged_select(q, bounds, t, n, 16, **kw)
+    # Whole numbers of another kind go on being taken.
+    import numpy as np
+    for page, top in ((np.int64(16), np.int32(2)), (torch.tensor(16), torch.tensor(2))):
+        assert ktt.paged_select(q, bounds, t, n, page, top)[0].tolist() == [[[0, 1], [0, 1]]]

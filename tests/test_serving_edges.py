@@ -2,6 +2,7 @@
 
 import ctypes
 
+import pytest
 import torch
 
 from kohaku_tt_b200 import _lib
@@ -143,3 +144,12 @@ def test_written_bounds_that_lie_on_one_another(built_lib):
     for strides in ((256, 128, 64), (64, 512, 256), (128, 512, 64), (256, 64, 128), (-256, 128, -64), (4096, 64, 1024), (2 ** 62, 128, 64), (2 ** 62, 2 ** 61, 64)):
         assert not status(strides), strides
     assert not status((0, 128, 64), pages=1) and not status((128, 0, 64), kv_heads=1) and status((128, 0, 64), kv_heads=2) and status((100, 128, 64), pages=2)
+
+
+def test_whole_numbers_of_an_argument_block():
+    from kohaku_tt_b200 import ops
+
+    assert [ops.int32(x, "x", "test") for x in (0, -(2 ** 31), 2 ** 31 - 1, 16.0)] == [0, -(2 ** 31), 2 ** 31 - 1, 16]
+    for x in (2 ** 31, -(2 ** 31) - 1, 2 ** 32 + 16):
+        with pytest.raises(_lib.UnsupportedAttention, match="must fit 32 bits"):
+            ops.int32(x, "x", "test")
