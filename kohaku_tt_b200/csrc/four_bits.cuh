@@ -45,8 +45,9 @@ struct Edges {
 __device__ __forceinline__ int64_t granted_to(const int32_t* granted, int b) { return granted ? max(granted[b], 0) : INT64_MAX; }
 
 // The bounds of the pages that keys of an append lie in (select.cu): those of sequence b from lengths[b] on, `rows` of each, or packed, as many as are
-// granted.
-int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, const int32_t* granted, cudaStream_t stream);
+// granted; without `launch` the checks alone.
+int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, const int32_t* granted, bool launch,
+                cudaStream_t stream);
 // Those of the pages that sequences are cut in, of their first kept[b] keys; without `launch` the checks alone.
 int cut_bounds(const ktt_b200_bounds_args* a, const int32_t* kept, bool launch, cudaStream_t stream);
 // Bounds from an argument block's fields after their checks; null, or why not.

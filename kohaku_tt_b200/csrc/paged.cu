@@ -673,8 +673,12 @@ extern "C" int ktt_b200_paged_append_granted(const ktt_b200_append_at_args* x, c
     const bool passing = !a->cu_seqlens && a->rows == 1;
     if (passing) p.bounds = bounds;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    auto behind = [&](bool go) {
+        return bounds.at && !passing ? keep_bounds(p.c, a->cache.bits, a->d, p.kv_heads, bounds, a->batch, a->rows, a->cu_seqlens, granted, go, st) : 0;
+    };
+    if (int rc = behind(false)) return rc;   // (refused before anything is launched)
     if (int rc = launch(p, a->cache.bits, a->d, st)) return rc;
-    return bounds.at && !passing ? keep_bounds(p.c, a->cache.bits, a->d, p.kv_heads, bounds, a->batch, a->rows, a->cu_seqlens, granted, st) : 0;
+    return behind(true);
 }
 
 extern "C" int ktt_b200_paged_read(const ktt_b200_read_args* a, void* stream) {

@@ -222,12 +222,18 @@ __global__ void __launch_bounds__(256) bounds_kernel(const __grid_constant__ Bou
     }
 }
 
+// Blocks of a launch in x: 8 pages (packed rows: lots of them) and heads each.
+int64_t blocks_of(const BoundsParams& p) {
+    const int64_t page = p.c.page_size, all = (p.c.cap + page - 1) / page;   // pages of a sequence
+    const int64_t lots = p.cu ? (p.rows + kLotOfTokens - 1) / kLotOfTokens : p.kept ? 1 : (p.rows > 0 ? std::min((p.rows + page - 2) / page + 1, all) : all);
+    return (lots * p.kv_heads + 7) / 8;
+}
+// Of lengths that the device alone knows, more pages and heads than a launch has blocks for.
+const char* too_many(const BoundsParams& p) { return blocks_of(p) >= (1ll << 31) ? "bounds of fewer than 2^34 pages and heads of a sequence" : nullptr; }
+
 template <int D, int kBits>
 int launch_bounds(const BoundsParams& p, cudaStream_t stream) {
-    const int64_t lots = p.cu ? (p.rows + kLotOfTokens - 1) / kLotOfTokens
-                              : p.kept ? 1
-                              : (p.rows > 0 ? (p.rows + p.c.page_size - 2) / p.c.page_size + 1 : (static_cast<int64_t>(p.c.cap) + p.c.page_size - 1) / p.c.page_size);
-    const dim3 grid(static_cast<unsigned>((lots * p.kv_heads + 7) / 8), static_cast<unsigned>(p.cu ? 1 : p.batch));
+    const dim3 grid(static_cast<unsigned>(blocks_of(p)), static_cast<unsigned>(p.cu ? 1 : p.batch));
     if (p.cu) return launch_dependent(bounds_kernel<D, kBits, true>, p, grid, dim3(256), stream, "paged_bounds launch");
     return launch_dependent(bounds_kernel<D, kBits, false>, p, grid, dim3(256), stream, "paged_bounds launch");
 }
@@ -988,7 +994,7 @@ int run_select(SelectParams& p, const SelectPlan& plan, int width, cudaStream_t 
 
 }  // namespace
 
-int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, const int32_t* granted, cudaStream_t stream) {
+int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bounds, int batch, int64_t rows, const int32_t* cu, const int32_t* granted, bool launch, cudaStream_t stream) {
     if (rows == 0) return 0;
     BoundsParams p = {};
     p.c = c;
@@ -998,7 +1004,8 @@ int keep_bounds(const Pages& c, int bits, int d, int kv_heads, const Bounds& bou
     p.rows = rows;
     p.cu = cu;
     p.granted = granted;
-    return launch_bounds(p, bits, d, stream);
+    if (const char* why = too_many(p)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_append: %s", why);
+    return launch ? launch_bounds(p, bits, d, stream) : 0;
 }
 
 }  // namespace ktt
@@ -1008,7 +1015,7 @@ using namespace ktt;
 namespace {
 
 // The checks of a call for bounds, and its parameters.
-int fill(BoundsParams& p, const ktt_b200_bounds_args* a) {
+int fill(BoundsParams& p, const ktt_b200_bounds_args* a, const int32_t* kept) {
     if (!a) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_bounds: null arguments");
     if (const char* why = pages_of(p.c, a->cache, a->d)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: %s", why);
     if (a->batch < 1) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_bounds: sizes must be positive");
@@ -1018,6 +1025,8 @@ int fill(BoundsParams& p, const ktt_b200_bounds_args* a) {
     p.batch = a->batch;
     p.kv_heads = a->cache.kv_heads;
     p.since = a->since;
+    p.kept = kept;
+    if (const char* why = too_many(p)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_bounds: %s", why);
     return 0;
 }
 
@@ -1027,8 +1036,7 @@ namespace ktt {
 
 int cut_bounds(const ktt_b200_bounds_args* a, const int32_t* kept, bool launch, cudaStream_t stream) {
     BoundsParams p = {};
-    if (int rc = fill(p, a)) return rc;
-    p.kept = kept;
+    if (int rc = fill(p, a, kept)) return rc;
     return launch ? launch_bounds(p, a->cache.bits, a->d, stream) : 0;
 }
 
@@ -1036,7 +1044,7 @@ int cut_bounds(const ktt_b200_bounds_args* a, const int32_t* kept, bool launch, 
 
 extern "C" int ktt_b200_paged_bounds(const ktt_b200_bounds_args* a, void* stream) {
     BoundsParams p = {};
-    if (int rc = fill(p, a)) return rc;
+    if (int rc = fill(p, a, nullptr)) return rc;
     return launch_bounds(p, a->cache.bits, a->d, static_cast<cudaStream_t>(stream));
 }
 

@@ -153,3 +153,15 @@ def test_whole_numbers_of_an_argument_block():
     for x in (2 ** 31, -(2 ** 31) - 1, 2 ** 32 + 16):
         with pytest.raises(_lib.UnsupportedAttention, match="must fit 32 bits"):
             ops.int32(x, "x", "test")
+
+
+def test_more_pages_and_heads_than_blocks(built_lib):
+    """Grids past 2^31 blocks are refused before anything is launched (past 2^32 their lower bits were)."""
+    b = _bounds(page_size=16, table_width=1 << 26, kv_heads=256, table_stride=1 << 26, pages=1)
+    b.bounds_strides[1] = 128
+    assert built_lib.ktt_b200_paged_bounds(ctypes.byref(b), None) == _lib.ERR_UNSUPPORTED and "2^34" in _lib.last_error()
+    x = _append(rows=1 << 30, cu_seqlens=4096)
+    x.bounds, x.base.cache.kv_heads = 4096, 4096
+    for i, s in enumerate((4096 * 128, 128, 64)):
+        x.bounds_strides[i] = s
+    assert built_lib.ktt_b200_paged_append_granted(ctypes.byref(x), None, None) == _lib.ERR_UNSUPPORTED and "2^34" in _lib.last_error()
