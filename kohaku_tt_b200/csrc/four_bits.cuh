@@ -42,7 +42,7 @@ struct Edges {
 };
 
 // How many of its new rows a sequence takes.
-__device__ __forceinline__ int64_t granted_to(const int32_t* granted, int b) { return granted ? max(granted[b], 0) : INT64_MAX; }
+__device__ __forceinline__ int64_t granted_to(const int32_t* granted, int b) { return max(granted[b], 0); }
 
 // The bounds of the pages that keys of an append lie in (select.cu): those of sequence b from lengths[b] on, `rows` of each, or packed, as many as are
 // granted; without `launch` the checks alone.
