@@ -347,6 +347,12 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
     Pages of 4 bits (paged_cache(bits=4)) hold each 64 channels of a row as codes 0 to 15 of
     least + step * code, step = bf16((most - least) / 15): codes are the nearest. No gradients."""
     interleaved = bool(interleaved)
+    # Eager calls on plain CUDA tensors are served by C++ in one step.
+    eager = not torch.compiler.is_compiling() and _lib.native()
+    if eager and _on_device(cu_seq):
+        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted)
+        if out is not NotImplemented:
+            return out
     if ops.watched(k, v, k_pages, v_pages, block_table, lengths, q):
         cu_seq = operator_offsets(cu_seq, block_table.shape[0], k.shape[0], k_pages, "paged_append")
         if positions is None and axes is None and bounds is None and granted is None:
@@ -355,12 +361,6 @@ def paged_append(k, v, k_pages, v_pages, block_table, lengths, cos=None, sin=Non
             out = torch.ops.ktt_b200._paged_append_at(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out,
                                                       positions, axes, bounds, granted)
         return out if q is not None else None
-    # Eager calls on plain CUDA tensors are served by C++ in one step.
-    eager = _lib.native()
-    if eager and _on_device(cu_seq):
-        out = eager.paged_append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted)
-        if out is not NotImplemented:
-            return out
     with torch.no_grad():
         return _append(k, v, k_pages, v_pages, block_table, lengths, cos, sin, q, interleaved, cu_seq, lengths_out, positions, axes, bounds, granted)
 
@@ -369,13 +369,13 @@ def paged_read(k_pages, v_pages, block_table, lengths, max_k=None):
     """(k, v), bf16 [B, Hk, capacity, D]: the first lengths[b] keys and values of each sequence out of its
     pages, as their values where the pages hold 4 bits; zeros behind them and where there is no page.
     capacity: block_table's, or max_k where that is less."""
-    if ops.watched(k_pages, v_pages, block_table, lengths):
-        return torch.ops.ktt_b200._paged_read(k_pages, v_pages, block_table, lengths, max_k)
-    eager = _lib.native()
+    eager = not torch.compiler.is_compiling() and _lib.native()
     if eager:
         out = eager.paged_read(k_pages, v_pages, block_table, lengths, max_k)
         if out is not None:
             return out
+    if ops.watched(k_pages, v_pages, block_table, lengths):
+        return torch.ops.ktt_b200._paged_read(k_pages, v_pages, block_table, lengths, max_k)
     with torch.no_grad():
         return _read(k_pages, v_pages, block_table, lengths, max_k)
 
@@ -398,18 +398,22 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
     for each K / V head, and sees the first lengths[t, h] keys of them; q [B, H, Sq, D] (token b * Sq + s) or
     [T, H, D], without offsets."""
     causal = bool(is_causal)
+    eager = not torch.compiler.is_compiling() and _lib.native()
     if block_table.dim() == 3:
         if cu_seq_q is not None or max_q is not None:
             raise ValueError("kohaku_tt_b200.sdpa_paged: with a table for each token there are no offsets")
-        if ops.watched(q, k_pages, v_pages, block_table, lengths):
-            return torch.ops.ktt_b200._sdpa_paged_chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
-        eager = _lib.native()
         if eager:
             out = eager.sdpa_paged_chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
             if out is not None:
                 return out
+        if ops.watched(q, k_pages, v_pages, block_table, lengths):
+            return torch.ops.ktt_b200._sdpa_paged_chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
         with torch.no_grad():
             return _chosen(q, k_pages, v_pages, block_table, lengths, scale, max_k)
+    if eager and _on_device(cu_seq_q):
+        out = eager.sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
+        if out is not None:
+            return out
     if ops.watched(q, k_pages, v_pages, block_table, lengths):
         if not torch.compiler.is_compiling() and not _on_device(cu_seq_q):
             cu_seq_q, longest = _offsets(cu_seq_q, block_table.shape[0], q.shape[0], q.device, "sdpa_paged")
@@ -417,10 +421,5 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
                 raise ValueError("kohaku_tt_b200.sdpa_paged: max_q is less than the longest sequence")
             max_q = longest if max_q is None else max_q
         return torch.ops.ktt_b200._sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
-    eager = _lib.native()
-    if eager and _on_device(cu_seq_q):
-        out = eager.sdpa_paged(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)
-        if out is not None:
-            return out
     with torch.no_grad():
         return _sdpa(q, k_pages, v_pages, block_table, lengths, causal, scale, cu_seq_q, max_q, max_k)

@@ -110,11 +110,11 @@ def paged_bounds(k_pages, block_table, lengths, bounds=None, since=None):
     if bounds is None:
         dim = k_pages.shape[-1] if k_pages.dtype == torch.bfloat16 else k_pages.shape[-1] // 9 * 16
         bounds = k_pages.new_zeros((*k_pages.shape[:2], 2, dim), dtype=torch.bfloat16)
+    eager = not torch.compiler.is_compiling() and _lib.native()
+    if eager and eager.paged_bounds(k_pages, block_table, lengths, bounds, since):
+        return bounds
     if ops.watched(k_pages, block_table, lengths, bounds):
         torch.ops.ktt_b200._paged_bounds(k_pages, block_table, lengths, bounds, since)
-        return bounds
-    eager = _lib.native()
-    if eager and eager.paged_bounds(k_pages, block_table, lengths, bounds, since):
         return bounds
     _bounds(k_pages, block_table, lengths, bounds, since)
     return bounds
@@ -135,13 +135,13 @@ def paged_select(q, bounds, block_table, lengths, page_size, top, first=1, last=
     it is not said which pages.)
     chosen int32 [tokens, Hk, top]: names of pages in the order of their places, -1 behind them. keys int32 [tokens, Hk]: the keys of
     those that the token sees (0: it sees none). Packed rows of no sequence see none. H is a multiple of Hk, D 64 or 128. No gradients."""
-    if ops.watched(q, bounds, block_table, lengths):
-        cu_seq_q = operator_offsets(cu_seq_q, block_table.shape[0], q.shape[0], q, "paged_select")
-        return torch.ops.ktt_b200._paged_select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq_q)
-    eager = _lib.native()
+    eager = not torch.compiler.is_compiling() and _lib.native()
     if eager and _on_device(cu_seq_q):
         out = eager.paged_select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq_q)
         if out is not None:
             return out
+    if ops.watched(q, bounds, block_table, lengths):
+        cu_seq_q = operator_offsets(cu_seq_q, block_table.shape[0], q.shape[0], q, "paged_select")
+        return torch.ops.ktt_b200._paged_select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq_q)
     with torch.no_grad():
         return _select(q, bounds, block_table, lengths, int(page_size), int(top), int(first), int(last), cu_seq_q)

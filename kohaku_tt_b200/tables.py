@@ -99,13 +99,13 @@ def paged_reserve(block_table, lengths, added, free, count, page_size, tokens, c
     for `tokens` rows (the sum of added; 0: not wanted), positions int32, lengths[b] + i, and slots int64, page * page_size + row in the
     page, which is where the token's row lies in a buffer [pages * page_size, ...]; -1 in rows behind the last sequence's, and
     in the slots of sequences that were granted nothing. At most 4096 sequences."""
-    if ops.watched(block_table, lengths, added, free, count):
-        return torch.ops.ktt_b200._paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out)
-    eager = _lib.native()
+    eager = not torch.compiler.is_compiling() and _lib.native()
     if eager:
         out = eager.paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out)
         if out is not None:
             return out
+    if ops.watched(block_table, lengths, added, free, count):
+        return torch.ops.ktt_b200._paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out)
     return _reserve(block_table, lengths, added, free, count, int(page_size), int(tokens), count_out)
 
 
@@ -116,10 +116,10 @@ def paged_release(block_table, lengths, kept, free, count, page_size, count_out,
     Entries that name no page give nothing back. A page that two sequences share must not be given back by both.
     k_pages, bounds: those of a cache with bounds (paged_bounds), which are made again, in a launch beside it, for the pages that
     sequences are cut in: of the keys that are left there, so that later appends and selections know nothing of the others."""
+    eager = not torch.compiler.is_compiling() and _lib.native()
+    if eager and eager.paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds):
+        return
     if ops.watched(block_table, lengths, kept, free, count):
         torch.ops.ktt_b200._paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds)
-        return
-    eager = _lib.native()
-    if eager and eager.paged_release(block_table, lengths, kept, free, count, page_size, count_out, k_pages, bounds):
         return
     _release(block_table, lengths, kept, free, count, int(page_size), count_out, k_pages, bounds)
