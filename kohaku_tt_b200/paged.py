@@ -70,7 +70,7 @@ def _offsets(cu, batch, tokens, device, what):
     host = attention.offsets(cu)
     if len(host) != batch + 1 or host[0] != 0 or host[-1] > tokens or any(x > y for x, y in zip(host, host[1:])):
         raise ValueError(f"kohaku_tt_b200.{what}: offsets must be [0, ..., at most {tokens}], {batch + 1} of them, and not decrease")
-    return torch.tensor(host, dtype=torch.int32, device=device), max((y - x for x, y in zip(host, host[1:])), default=0)
+    return torch.tensor(host, dtype=torch.int32, device=device), max([0, *[y - x for x, y in zip(host, host[1:])]])
 
 
 def _operand(t, name, heads, like, batch, rows, dim, packed, what):
@@ -87,8 +87,8 @@ def _on_device(cu):
 
 
 def operator_offsets(cu, batch, rows, like, what):
-    """Offsets as an operator takes them, on the device; as they are in a compiled graph."""
-    return cu if torch.compiler.is_compiling() or _on_device(cu) else _offsets(cu, batch, rows, like.device, what)[0]
+    """Offsets as an operator takes them, on the device."""
+    return cu if _on_device(cu) else _offsets(cu, batch, rows, like.device, what)[0]
 
 
 def check_bounds(bounds, like, pages, hk, dim, what):
@@ -415,7 +415,7 @@ def sdpa_paged(q, k_pages, v_pages, block_table, lengths, is_causal=True, scale=
         if out is not None:
             return out
     if ops.watched(q, k_pages, v_pages, block_table, lengths):
-        if not torch.compiler.is_compiling() and not _on_device(cu_seq_q):
+        if not _on_device(cu_seq_q):
             cu_seq_q, longest = _offsets(cu_seq_q, block_table.shape[0], q.shape[0], q.device, "sdpa_paged")
             if max_q is not None and max_q < longest:
                 raise ValueError("kohaku_tt_b200.sdpa_paged: max_q is less than the longest sequence")

@@ -418,3 +418,31 @@ def test_numbers_past_32_bits_are_refused(cuda, path):
     import numpy as np
     for page, top in ((np.int64(16), np.int32(2)), (torch.tensor(16), torch.tensor(2))):
         assert ktt.paged_select(q, bounds, t, n, page, top)[0].tolist() == [[[0, 1], [0, 1]]]
+
+
+# ---- offsets from a list in a compiled graph ----------------------------------------------------
+
+def test_offsets_from_a_list_compiled(cuda):
+    """A list of offsets is taken in a compiled graph as it is outside of one, and so are its refusals."""
+    h, hk, d, page, t = 4, 2, 64, 16, 9
+    q, k, v = (_x(t, n, d, seed=n).to(cuda) for n in (h, hk, hk))
+    table, lens, after = _i32([[0, 1], [2, 3], [4, 5]], cuda), _i32([20, 0, 3], cuda), _i32([24, 0, 8], cuda)
+    bounds = torch.zeros((6, hk, 2, d), dtype=torch.bfloat16, device=cuda)
+
+    def step(q, k, v, kp, vp, bounds, offsets):
+        turned = ktt.paged_append(k, v, kp, vp, table, lens, q=q, cu_seq=offsets, bounds=bounds)
+        chosen, keys = ktt.paged_select(turned, bounds, table, after, page, 2, cu_seq_q=offsets)
+        return turned, chosen, keys, ktt.sdpa_paged(turned, kp, vp, chosen, keys), ktt.sdpa_paged(turned, kp, vp, table, after, cu_seq_q=offsets)
+
+    def fresh():
+        return *(_x(6, hk, page, d, seed=s).to(cuda) for s in (7, 8)), bounds.clone()
+
+    # (By the graph as it was traced: a compiler would write the list's copy in C++, for which a machine that runs these tests need have nothing.)
+    compiled = torch.compile(step, fullgraph=True, backend="aot_eager")
+    for offsets in ([0, 4, 4, 9], [0, 0, 5, 9]):
+        first, second = fresh(), fresh()
+        for x, y in zip((*compiled(q, k, v, *first, offsets), *first), (*step(q, k, v, *second, offsets), *second)):
+            assert torch.equal(x, y)
+    for bad in ([0, 4, 4], [0, 5, 4, 9], [0, 4, 4, 10]):
+        with pytest.raises(Exception, match="offsets must be"):
+            torch.compile(step, fullgraph=True, backend="aot_eager")(q, k, v, *fresh(), bad)
