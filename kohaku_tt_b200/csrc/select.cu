@@ -65,8 +65,9 @@ constexpr int kLotOfTokens = 16;   // packed rows that a warp looks for pages in
 
 // A warp has a page and head: a lane eight channels of every second (D 128) or fourth row, 16 rows requested before the first is used
 // (8: 37 us where it is 31). Packed rows: a warp looks at 16 of them and has the pages that begin among them, or in which a sequence's rows
-// begin. Bound: bf16, the reading of the keys: 16 x up to 8,192 of 8 heads, D 128, pages of 32, 212 MB: 31.6 us, 6.7 TB/s. 4 bits, the
-// instructions that make values of codes, 16 for eight, and those that find a row's words: 26 us (38 with an address for each row).
+// begin. Bound: bf16, the reading of the keys: 16 x up to 8,192 of 8 heads, D 128, pages of 32, 212 MB: 31.6 us, 6.7 TB/s. 4 bits: 26 us
+// (38 with an address for each row), of which the reading of 59 MB is 9 and instructions, 16 to make eight values of a word and those that find the
+// words, are 16 at one a cycle; 0.57 are issued, as warps wait for memory and for the pipe of packed pairs by turns.
 //
 // kSome: keys of an append of which some are granted, or the page that a sequence is cut in. (Told apart by null pointers alone, 1,024 keys of 4 bits
 // took 2.25 us where it is 2.07.)

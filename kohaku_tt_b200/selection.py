@@ -134,7 +134,8 @@ def paged_select(q, bounds, block_table, lengths, page_size, top, first=1, last=
     block_table that names no page has score 0. (Where a least value is above the largest, as in a tensor that nothing was written to,
     it is not said which pages.)
     chosen int32 [tokens, Hk, top]: names of pages in the order of their places, -1 behind them. keys int32 [tokens, Hk]: the keys of
-    those that the token sees (0: it sees none). Packed rows of no sequence see none. H is a multiple of Hk, D 64 or 128. No gradients."""
+    those that the token sees (0: it sees none). Packed rows of no sequence see none. The two may share one allocation,
+    which then lasts as long as either. H is a multiple of Hk, D 64 or 128. No gradients."""
     eager = not torch.compiler.is_compiling() and _lib.native()
     if eager and _on_device(cu_seq_q):
         out = eager.paged_select(q, bounds, block_table, lengths, page_size, top, first, last, cu_seq_q)

@@ -94,11 +94,13 @@ def paged_reserve(block_table, lengths, added, free, count, page_size, tokens, c
     many are left. lengths are not changed either.
     granted int32 [B]: added[b], or 0 for the first sequence that the list, or its row of the table, has no room for and for all
     behind it; their new entries become -1, and they can be asked for again later. Given to paged_append, it keeps their rows out of the
-    cache and out of lengths_out; where no call can run short it may be left out.
+    cache and out of lengths_out; where no call can run short it may be left out. What selections and attention give for their queries
+    is of no use.
     The new tokens are packed, row i of sequence b at cu_seq[b] + i, as paged_append and sdpa_paged take them: cu_seq int32 [B + 1];
     for `tokens` rows (the sum of added; 0: not wanted), positions int32, lengths[b] + i, and slots int64, page * page_size + row in the
     page, which is where the token's row lies in a buffer [pages * page_size, ...]; -1 in rows behind the last sequence's, and
-    in the slots of sequences that were granted nothing. At most 4096 sequences."""
+    in the slots of sequences that were granted nothing. The four may share one allocation, which then lasts as long as any of them (clone what is
+    kept for long, or saved). At most 4096 sequences."""
     eager = not torch.compiler.is_compiling() and _lib.native()
     if eager:
         out = eager.paged_reserve(block_table, lengths, added, free, count, page_size, tokens, count_out)
@@ -113,7 +115,8 @@ def paged_release(block_table, lengths, kept, free, count, page_size, count_out,
     """Cuts sequences back to their first kept[b] keys (int32 [B] on the device; 0: the sequence has ended; lengths[b]: it goes on):
     the pages that hold none of those go to free[count:], sequence by sequence, and their entries of block_table become -1;
     count_out (int32 [1], another buffer than count) receives the new number. lengths are not changed: they are kept's from then on.
-    Entries that name no page give nothing back. A page that two sequences share must not be given back by both.
+    Entries that name no page give nothing back. A page that two sequences share must not be given back by both,
+    nor cut, with bounds, by the one that has fewer keys in it.
     k_pages, bounds: those of a cache with bounds (paged_bounds), which are made again, in a launch beside it, for the pages that
     sequences are cut in: of the keys that are left there, so that later appends and selections know nothing of the others."""
     eager = not torch.compiler.is_compiling() and _lib.native()
