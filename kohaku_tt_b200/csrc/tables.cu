@@ -275,6 +275,25 @@ __global__ void __cluster_dims__(kReleaseCtas, 1, 1) __launch_bounds__(kReleaseT
     ctas_meet();   // nobody's shared memory goes away while another reads it
 }
 
+// Bytes of an argument. (CTAs read what is given after others may have written what is returned.)
+struct Bytes {
+    const void* at;   // null: none
+    int64_t count;
+};
+bool meet(const Bytes& x, const Bytes& y) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x.at), b = reinterpret_cast<uintptr_t>(y.at);
+    return a && b && x.count > 0 && y.count > 0 && a < b + static_cast<uintptr_t>(y.count) && b < a + static_cast<uintptr_t>(x.count);
+}
+template <int N, int M>
+bool any_meet(const Bytes (&xs)[N], const Bytes (&ys)[M]) {
+    for (const Bytes& x : xs) {
+        for (const Bytes& y : ys) {
+            if (meet(x, y)) return true;
+        }
+    }
+    return false;
+}
+
 const char* tables_refusal(const ktt_b200_tables& a) {
     if (a.batch < 1 || a.table_width < 1 || a.pool < 0) return "sizes must be positive";
     if (a.page_size < 16 || a.page_size % 16) return "the page size must be a multiple of 16";
@@ -296,6 +315,10 @@ extern "C" int ktt_b200_paged_reserve(const ktt_b200_tables* a, const int32_t* a
     if (tokens < 0 || tokens >= (1ll << 31)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_reserve: 0 to 2^31 - 1 tokens");
     if (!a->block_table || !a->lengths || !added || !a->count || !a->count_out || (a->pool && !a->free_pages)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_reserve: null pointer");
     if (a->count == a->count_out) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_reserve: count_out must be another word than count");
+    const int64_t vector = 4 * static_cast<int64_t>(a->batch);
+    const Bytes given[] = {{a->lengths, vector}, {added, vector}, {a->free_pages, 4 * a->pool}, {a->count, 4}};
+    const Bytes returned[] = {{a->count_out, 4}, {cu, vector + 4}, {positions, 4 * tokens}, {slots, 8 * tokens}, {granted, vector}};
+    if (any_meet(given, returned)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_reserve: outputs must not overlap inputs");
     ReserveParams p = {};
     p.batch = a->batch;
     p.page_size = a->page_size;
@@ -327,6 +350,9 @@ extern "C" int ktt_b200_paged_release_bounds(const ktt_b200_tables* a, const int
     if (const char* why = tables_refusal(*a)) return fail(KTT_B200_ERR_UNSUPPORTED, "paged_release: %s", why);
     if (!a->block_table || !a->lengths || !kept || !a->count || !a->count_out || (a->pool && !a->free_pages)) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: null pointer");
     if (a->count == a->count_out) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: count_out must be another word than count");
+    const int64_t vector = 4 * static_cast<int64_t>(a->batch);
+    const Bytes given[] = {{a->lengths, vector}, {kept, vector}, {a->count, 4}}, returned[] = {{a->count_out, 4}, {a->free_pages, 4 * a->pool}};
+    if (any_meet(given, returned) || meet(returned[0], returned[1])) return fail(KTT_B200_ERR_BAD_ARGUMENT, "paged_release: outputs must not overlap inputs");
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (bounds) {   // (refused before anything is launched)
         if (int rc = cut_bounds(bounds, kept, false, st)) return rc;

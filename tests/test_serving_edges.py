@@ -43,8 +43,8 @@ def test_append_by_hand():
 def _tables(**kw):
     a = _lib.Tables()
     a.batch, a.table_width, a.page_size, a.table_stride, a.pool = 2, 4, 16, 4, 8
-    a.block_table = a.lengths = a.free_pages = a.count = 4096
-    a.count_out = 8192
+    a.block_table = a.lengths = a.count = 4096
+    a.free_pages, a.count_out = 1 << 20, 8192
     for name, x in kw.items():
         setattr(a, name, x)
     return a
@@ -165,3 +165,26 @@ def test_more_pages_and_heads_than_blocks(built_lib):
     for i, s in enumerate((4096 * 128, 128, 64)):
         x.bounds_strides[i] = s
     assert built_lib.ktt_b200_paged_append_granted(ctypes.byref(x), None, None) == _lib.ERR_UNSUPPORTED and "2^34" in _lib.last_error()
+
+
+def test_outputs_of_tables_over_their_inputs(built_lib):
+    """What some blocks of a launch read while others write is refused, in whole or in part; beside one another is fine (refused for their stride, behind it)."""
+    base = dict(block_table=1 << 20, lengths=4096, free_pages=8192, count=12288, count_out=16384)      # 2 sequences, a list of 8
+
+    def reserve(cu=None, positions=None, slots=None, granted=None, **kw):
+        status = built_lib.ktt_b200_paged_reserve(ctypes.byref(_tables(**{**base, **kw})), 20480, 3, cu, positions, slots, granted, None)
+        return status == _lib.ERR_BAD_ARGUMENT and "overlap" in _lib.last_error()
+
+    for given in (4096, 4100, 20480, 20484, 8192, 8192 + 28, 12288):      # lengths, added, the list, the count
+        assert reserve(granted=given) and reserve(cu=given) and reserve(positions=given) and reserve(slots=given & ~7), given
+        if given != 12288:
+            assert reserve(count_out=given)
+    assert reserve(cu=4096 - 8) and reserve(slots=4096 - 16) and reserve(positions=20480 - 8)
+
+    def release(kept=20480, **kw):
+        status = built_lib.ktt_b200_paged_release(ctypes.byref(_tables(**{**base, **kw})), kept, None)
+        return status == _lib.ERR_BAD_ARGUMENT and "overlap" in _lib.last_error()
+
+    for given in (4096, 4100, 20480, 20484, 8192, 8192 + 28):
+        assert release(count_out=given), given
+    assert release(kept=8192) and release(kept=8192 + 28) and release(lengths=8188) and release(count=8200)
