@@ -404,7 +404,7 @@ typedef struct ktt_b200_pages {
 } ktt_b200_pages;
 
 /* Block tables kept on the device. free_pages[0 .. *count) are the pages that no sequence has; a call reads *count and leaves the new
- * number in *count_out (another word). Sequence b has pages in the first ceil(lengths[b] / page_size) entries of its row. */
+ * number in *count_out (another word; what a call returns must not lie on what it reads). Sequence b has pages in the first ceil(lengths[b] / page_size) entries of its row. */
 typedef struct ktt_b200_tables {
     int32_t batch, table_width, page_size;   /* batch: 4096 at most */
     int32_t* block_table;          /* int32 [batch][table_width] */
@@ -418,9 +418,9 @@ typedef struct ktt_b200_tables {
 
 /* Pages for added[b] new keys of each sequence (int32 [batch] on the device), from the end of the list on: the i-th that the call
  * takes, sequence by sequence and entry by entry, is free_pages[*count - 1 - i]. The first sequence that the list (or its row of
- * the table) has no room for gets none, and none of those behind it do: their new entries are -1, and their rows are kept out of the cache by
- * ktt_b200_paged_append_granted (an append that is not told of `granted` writes those that fit into the last page they have). The list is only read. Outputs,
- * each of which may be NULL: granted int32 [batch] (added[b], or 0); cu_seqlens int32 [batch + 1], the sums of added; and of each
+ * the table) has no room for gets none, and none of those behind it do: their new entries are -1, and their rows are kept out of the cache
+ * by ktt_b200_paged_append_granted (an append that is not told of `granted` writes those that fit into the last page they have). The list
+ * is only read. Outputs, each of which may be NULL: granted int32 [batch] (added[b], or 0); cu_seqlens int32 [batch + 1], the sums of added; and of each
  * of `tokens` packed rows, row i of sequence b being cu_seqlens[b] + i: positions int32, lengths[b] + i, and slots int64, page *
  * page_size + row in the page; both -1 behind the last sequence's rows, slots also of sequences that got nothing. */
 KTT_B200_API int ktt_b200_paged_reserve(const ktt_b200_tables* args, const int32_t* added, int64_t tokens, int32_t* cu_seqlens, int32_t* positions, int64_t* slots, int32_t* granted, void* stream);
@@ -491,8 +491,8 @@ KTT_B200_API int ktt_b200_paged_release_bounds(const ktt_b200_tables* args, cons
 /* The `top` pages of its sequence that each query token goes to, for each K / V head: the first `first`, the last `last` (first + last
  * <= top, last >= 1), and of the others those of the largest score, ties to the lower place. A page's score is the largest logit that a key
  * between its bounds could have, over the queries q_h of the head's group: max_h sum_d max(q_hd least_d, q_hd largest_d), in 64 bits
- * (exact where the products that are not 0 lie within a factor of 2^30 of one another); one that is no number counts as infinite, that of an entry that names no page as 0. q dense [B, H, sq, D] or packed
- * [total_q, H, D] (cu_seqlens_q); lengths count the keys with those of the call's own tokens, and query i of n sees keys
+ * (exact where the products that are not 0 lie within a factor of 2^30 of one another); one that is no number counts as infinite, that of
+ * an entry that names no page as 0. q dense [B, H, sq, D] or packed [total_q, H, D] (cu_seqlens_q); lengths count the keys with those of the call's own tokens, and query i of n sees keys
  * 0 .. length - n + i, and the pages these lie in. chosen int32 [tokens][kv_heads][top]: the pages' names in the order of their places, -1 behind
  * them; keys int32 [tokens][kv_heads]: how many keys they hold that the token sees (0: none). Tokens: batch * sq, or total_q. */
 typedef struct ktt_b200_select_args {
